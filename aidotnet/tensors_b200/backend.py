@@ -59,6 +59,36 @@ class GpuBuffer:
         return self.tensor.dtype
 
 
+class KvCacheFp8:
+    """A paged key / value pool held in 8 bits: E4M3 codes [numBlocks, blockSize, kvHeads, headDim] (one byte each) and a
+    power-of-two fp32 scale per (block, KV head), for keys and for values.  An element stands for code * scale."""
+
+    def __init__(self, keys: GpuBuffer, values: GpuBuffer, keyScales: GpuBuffer, valueScales: GpuBuffer, blockSize: int,
+                 kvHeads: int, headDim: int):
+        if blockSize <= 0 or kvHeads <= 0 or headDim <= 0:
+            raise ValueError("blockSize, kvHeads and headDim must be positive")
+        if headDim % 8 != 0 or headDim > CudaBackend.MaxHeadDim:
+            raise ValueError(f"headDim must be a multiple of 8 up to {CudaBackend.MaxHeadDim} (got {headDim})")
+        for name, buf in (("keys", keys), ("values", values)):
+            if buf.tensor.element_size() != 1:
+                raise ValueError(f"{name} must be a buffer of one-byte elements")
+        per = blockSize * kvHeads * headDim
+        if keys.Size != values.Size or keys.Size < per or keys.Size % per != 0:
+            raise ValueError("keys and values must be equal-sized and a whole number of blocks")
+        self.numBlocks = keys.Size // per
+        for name, buf in (("keyScales", keyScales), ("valueScales", valueScales)):
+            if buf.dtype != torch.float32 or buf.Size < self.numBlocks * kvHeads:
+                raise ValueError(f"{name} must hold numBlocks * kvHeads fp32 values")
+        self.keys, self.values, self.keyScales, self.valueScales = keys, values, keyScales, valueScales
+        self.blockSize, self.kvHeads, self.headDim = blockSize, kvHeads, headDim
+
+    def _pack(self, blockTables: GpuBuffer, blocksPerSeq: int) -> bytes:
+        return N.kv8_cache(key_pool=self.keys.tensor.data_ptr(), value_pool=self.values.tensor.data_ptr(),
+                           key_scale=self.keyScales.tensor.data_ptr(), value_scale=self.valueScales.tensor.data_ptr(),
+                           block_table=blockTables.tensor.data_ptr(), block_table_stride=blocksPerSeq, num_blocks=self.numBlocks,
+                           block_size=self.blockSize, kv_heads=self.kvHeads, head_dim=self.headDim)
+
+
 class CudaBackend:
     """The attention slice of ``CudaBackend``: one device, one stream (``CudaBackend.cs:371-375``)."""
 
@@ -405,6 +435,107 @@ class CudaBackend:
             raise ValueError("PagedAttentionDecodeBatched: blockTables / seqLens are too small or not int32")
         return self._paged("PagedAttentionDecodeBatched", q, kcache, vcache, blockTables, heads, kvHeads, headDim,
                            blockSize, 1, maxSeqLen, 0, scale, batch=batch, seqLens=seqLens, tableStride=blocksPerSeq)
+
+    # -- paged K/V held in 8 bits (extension with no reference counterpart) ------------------------------------------
+    def AllocateKvCacheFp8(self, numBlocks: int, blockSize: int, kvHeads: int, headDim: int) -> KvCacheFp8:
+        """An empty pool: zero codes."""
+        if numBlocks <= 0:
+            raise ValueError("numBlocks must be positive")
+        codes = [torch.zeros(numBlocks * blockSize * kvHeads * headDim, dtype=torch.uint8, device=self._torch_device) for _ in range(2)]
+        scales = [torch.ones(numBlocks * kvHeads, device=self._torch_device) for _ in range(2)]
+        return KvCacheFp8(*(GpuBuffer(t) for t in codes + scales), blockSize, kvHeads, headDim)
+
+    @staticmethod
+    def _check_kv8(op, table, batch, columns, lens, starts, tokens):
+        if batch <= 0 or columns <= 0:
+            raise ValueError(f"{op}: batch and blocksPerSeq must be > 0")
+        t, n = table.tensor, lens.tensor
+        if t.numel() < batch * columns or n.numel() < batch or t.dtype != torch.int32 or n.dtype != torch.int32:
+            raise ValueError(f"{op}: block tables or lengths are too small or not int32")
+        if starts is not None and (starts.tensor.numel() < batch + 1 or starts.tensor.dtype != torch.int32):
+            raise ValueError(f"{op}: the first tokens must be int32 [batch + 1]")
+        if starts is None and tokens % batch != 0:
+            raise ValueError(f"{op}: {tokens} tokens are not the same number for each of {batch} sequences")
+
+    def PagedKvAppendFp8(self, qkv: GpuBuffer, queries: Optional[GpuBuffer], cache: KvCacheFp8, blockTables: GpuBuffer,
+                         startLens: GpuBuffer, batch: int, tokens: int, heads: int, blocksPerSeq: int,
+                         cos: Optional[GpuBuffer] = None, sin: Optional[GpuBuffer] = None, interleaved: bool = True,
+                         tokenStarts: Optional[GpuBuffer] = None, positions: Optional[GpuBuffer] = None) -> None:
+        """Puts a step's ``tokens`` new tokens into the cache.  ``qkv`` is [tokens, heads + 2 * kvHeads, headDim] as a packed
+        projection writes it (heads = 0: keys and values only); token i of sequence b (its tokens are
+        tokenStarts[b] .. tokenStarts[b + 1] - 1, without ``tokenStarts`` tokens / batch each) becomes position startLens[b] + i.
+        With ``cos`` / ``sin`` [maxPosition, headDim / 2] queries and keys are rotated by their positions (or ``positions``
+        [tokens]), in pairs (2i, 2i+1) or, not ``interleaved``, (i, i + headDim/2); the queries go to ``queries``."""
+        kvHeads, headDim = cache.kvHeads, cache.headDim
+        if tokens < 0 or heads < 0:
+            raise ValueError("PagedKvAppendFp8: tokens and heads must be >= 0")
+        self._check_kv8("PagedKvAppendFp8", blockTables, batch, blocksPerSeq, startLens, tokenStarts, tokens)
+        x, width = qkv.tensor, (heads + 2 * kvHeads) * headDim
+        if x.numel() < tokens * width:
+            raise ValueError("PagedKvAppendFp8: qkv is smaller than [tokens, heads + 2 * kvHeads, headDim]")
+        if heads > 0 and (queries is None or queries.tensor.numel() < tokens * heads * headDim or queries.tensor.dtype != x.dtype):
+            raise ValueError("PagedKvAppendFp8: queries must hold [tokens, heads, headDim] of qkv's dtype")
+        if (cos is None) != (sin is None):
+            raise ValueError("PagedKvAppendFp8: cos and sin come together")
+        reach = 0
+        if cos is not None:
+            c, s = cos.tensor, sin.tensor
+            reach = min(c.numel(), s.numel()) // (headDim // 2)
+            if c.dtype != torch.float32 or s.dtype != torch.float32:
+                raise ValueError("PagedKvAppendFp8: cos and sin are fp32 buffers")
+        if positions is not None and (positions.tensor.numel() < tokens or positions.tensor.dtype != torch.int32):
+            raise ValueError("PagedKvAppendFp8: positions must be int32 [tokens]")
+        size, at, row = x.element_size() * headDim, x.data_ptr(), (width, headDim)
+        N.kv8_append(cache._pack(blockTables, blocksPerSeq), query=at if heads else None, key=at + heads * size,
+                     value=at + (heads + kvHeads) * size, query_out=queries.tensor.data_ptr() if heads else None, heads=heads,
+                     start=startLens.tensor.data_ptr(), tokens=tokens, batch=batch, dtype=_DTYPE[x.dtype],
+                     cosine=cos.tensor.data_ptr() if cos is not None else None, sine=sin.tensor.data_ptr() if cos is not None else None,
+                     rope=N.ROPE_NONE if cos is None else (N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES),
+                     max_position=reach, token_starts=tokenStarts.tensor.data_ptr() if tokenStarts is not None else None,
+                     positions=positions.tensor.data_ptr() if positions is not None else None, query_stride=row, key_stride=row,
+                     value_stride=row, stream=self._raw_stream)
+        self.launch_count += 1
+
+    def PagedAttentionFp8(self, q: GpuBuffer, cache: KvCacheFp8, blockTables: GpuBuffer, seqLens: GpuBuffer, output: GpuBuffer,
+                          batch: int, heads: int, maxQueries: int, maxSeqLen: int, blocksPerSeq: int, scale: float,
+                          queryStarts: Optional[GpuBuffer] = None, softcap: float = 0.0, softmaxStats: Optional[GpuBuffer] = None,
+                          causal: bool = True) -> None:
+        """Attention of a step's queries over the cache: ``q`` and ``output`` are [queries, heads, headDim], sequence b's rows
+        queryStarts[b] .. queryStarts[b + 1] - 1 (at most ``maxQueries``; without ``queryStarts`` maxQueries each), its keys the
+        first seqLens[b] (at most ``maxSeqLen``) positions, the new tokens' own included.  Causal: query i of n sees positions up
+        to seqLens[b] - n + i.  ``softmaxStats`` [queries, heads] fp32 receives max + ln(sum)."""
+        kvHeads, headDim = cache.kvHeads, cache.headDim
+        if heads <= 0 or heads % kvHeads != 0:
+            raise ValueError(f"PagedAttentionFp8: heads must be a positive multiple of kvHeads (heads={heads}, kvHeads={kvHeads})")
+        if maxQueries <= 0 or maxSeqLen <= 0:
+            raise ValueError("PagedAttentionFp8: maxQueries and maxSeqLen must be > 0")
+        x, out = q.tensor, output.tensor
+        width = heads * headDim
+        queries = batch * maxQueries if queryStarts is None else x.numel() // width
+        self._check_kv8("PagedAttentionFp8", blockTables, batch, blocksPerSeq, seqLens, queryStarts, queries)
+        if x.numel() < queries * width or out.numel() < queries * width:
+            raise ValueError("PagedAttentionFp8: q or output is smaller than [queries, heads, headDim]")
+        if softmaxStats is not None and (softmaxStats.tensor.numel() < queries * heads or softmaxStats.tensor.dtype != torch.float32):
+            raise ValueError("PagedAttentionFp8: softmaxStats must hold [queries, heads] fp32 values")
+        h = self._handle(qkv_dtype=_DTYPE[x.dtype], out_dtype=_DTYPE[out.dtype], head_dim=headDim, num_q_heads=heads,
+                         num_kv_heads=kvHeads, causal=bool(causal), causal_bottom_right=True, softcap=float(softcap),
+                         emit_lse=softmaxStats is not None)
+        need = h.kv8_workspace_bytes(batch, maxQueries, maxSeqLen)
+        stream = self._raw_stream
+        ws, ws_bytes = None, 0
+        if need > 0:
+            held = self._scratch.get(0) if stream == 0 else None   # (stream 0 is never captured)
+            if held is not None and held.numel() >= need:
+                ws, ws_bytes = held.data_ptr(), held.numel()
+            else:
+                ws, ws_bytes = self._workspace(need, self.stream, optional=True)   # without one the keys are not cut
+        row = (maxQueries * width, headDim, width) if queryStarts is None else None
+        h.launch_kv8(q=x.data_ptr(), out=out.data_ptr(), cache=cache._pack(blockTables, blocksPerSeq), batch=batch, seq_q=maxQueries,
+                     seq_kv=maxSeqLen, stream=stream, query_starts=queryStarts.tensor.data_ptr() if queryStarts is not None else None,
+                     queries=queries, lse=softmaxStats.tensor.data_ptr() if softmaxStats is not None else None,
+                     kv_len=seqLens.tensor.data_ptr(), q_stride=row, o_stride=row, scale=float(scale), workspace=ws,
+                     workspace_bytes=ws_bytes)
+        self.launch_count += h.last_launch_count
 
     def FlashAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer,
                                output: GpuBuffer, softmaxStats: GpuBuffer, gradQuery: GpuBuffer, gradKey: GpuBuffer,

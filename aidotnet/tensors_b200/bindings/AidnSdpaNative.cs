@@ -55,6 +55,31 @@ namespace AiDotNet.Tensors.Engines.DirectGpu.CUDA
         public int num_blocks;
     }
 
+    /// <summary>A paged K/V pool held in 8 bits: E4M3 codes and a power-of-two scale per (block, KV head), and the block
+    /// table that it is read through.</summary>
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnKv8Cache
+    {
+        public IntPtr key_pool, value_pool, key_scale, value_scale, block_table;
+        public long block_table_stride;
+        public fixed long pool_stride[3];
+        public int num_blocks, block_size, kv_heads, head_dim;
+    }
+
+    /// <summary>Arguments of aidn_kv8_append: a step's queries, keys and values, their rotation, and where they go.</summary>
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnKv8AppendArgs
+    {
+        public IntPtr query, key, value, query_out;
+        public fixed long query_stride[2];
+        public fixed long key_stride[2];
+        public fixed long value_stride[2];
+        public fixed long query_out_stride[2];
+        public IntPtr cosine, sine, start, token_starts, positions;
+        public long tokens, max_position;
+        public int batch, heads, dtype, rope;
+    }
+
     /// <summary>Arguments of aidn_sdpa_backward: the forward block (out = O, lse = statistics) plus dO and the gradients.</summary>
     [StructLayout(LayoutKind.Sequential)]
     internal unsafe struct AidnSdpaBwdArgs
@@ -118,6 +143,9 @@ namespace AiDotNet.Tensors.Engines.DirectGpu.CUDA
         [DllImport(Lib)] public static extern int aidn_peer_open(byte[] handle64, out IntPtr basePtr);
         [DllImport(Lib)] public static extern int aidn_peer_close(IntPtr basePtr);
         [DllImport(Lib)] public static extern int aidn_paged_kv_append(IntPtr newKeys, IntPtr newValues, IntPtr keyPool, IntPtr valuePool, IntPtr blockTable, long startPosition, long tokens, int blockSize, int numBlocks, long rowBytes, IntPtr cuStream);
+        [DllImport(Lib)] public static extern int aidn_kv8_append(ref AidnKv8Cache cache, ref AidnKv8AppendArgs args, IntPtr cuStream);
+        [DllImport(Lib)] public static extern long aidn_sdpa_kv8_workspace_bytes(IntPtr handle, long batch, long seqQ, long seqKv);
+        [DllImport(Lib)] public static extern int aidn_sdpa_launch_kv8(IntPtr handle, ref AidnSdpaArgs args, ref AidnKv8Cache cache, IntPtr queryStarts, long queries, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_sdpa_backward_workspace_bytes(IntPtr handle, long batch, long seqQ);
         [DllImport(Lib)] public static extern int aidn_sdpa_backward(IntPtr handle, ref AidnSdpaBwdArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_mha_workspace_bytes(IntPtr handle, long batch, long seq, int inputDtype, int weightDtype);

@@ -12,6 +12,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "kv8.cuh"
 #include "../../../include/aidn_sdpa_debug.h"
 
 namespace {
@@ -104,7 +105,8 @@ struct aidn_sdpa {
   aidn_sdpa_desc d;
   int group;
   int head_count;
-  int32_t* status_dev;   // [0] status word, [1..2] scheduler counters of the persistent prefill kernel
+  int32_t* status_dev;   // [0] status word, [1..2] scheduler counters of the persistent prefill kernel, from [4] on kKv8Counters
+                         // counters of the attention over an 8-bit pool, which leaves them zero
   int num_sms;
   void* scratch;
   int64_t scratch_bytes;
@@ -116,6 +118,8 @@ struct aidn_sdpa {
 };
 
 namespace {
+
+constexpr int kHandleWords = 4 + aidn::kv8::kCounters;
 
 // Keys per split of the decode kernel.  Enough CTAs to fill 148 SMs several times over, but never more than
 // 512 keys per CTA so that ragged kv_len values balance, and never fewer than 64.
@@ -261,8 +265,8 @@ int aidn_sdpa_create(const aidn_sdpa_desc* desc, aidn_sdpa_t* out) {
   h->num_sms = 0;
   std::memset(&h->prefill_maps, 0, sizeof(h->prefill_maps));
   e = cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, d.device);
-  if (e == cudaSuccess) e = cudaMalloc(&h->status_dev, 4 * sizeof(int32_t));
-  if (e == cudaSuccess) e = cudaMemset(h->status_dev, 0, 4 * sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&h->status_dev, kHandleWords * sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaMemset(h->status_dev, 0, kHandleWords * sizeof(int32_t));
   if (e != cudaSuccess) {
     if (h->status_dev) cudaFree(h->status_dev);
     delete h;
@@ -797,6 +801,174 @@ int aidn_paged_kv_append(const void* new_keys, const void* new_values, void* key
                                             block_size, num_blocks, row_bytes, (cudaStream_t)cu_stream);
   if (e != cudaSuccess) return fail_cuda(e, "paged_kv_append");
   return AIDN_OK;
+}
+
+// ---- paged K / V held in 8 bits --------------------------------------------------------------------------------------
+namespace {
+// The pool's parameter block; `op` names the call in messages.
+int build_pool(const char* op, const aidn_kv8_cache* c, aidn::kv8::Pool& pool) {
+  if (!c) return fail(AIDN_EINVAL, "%s: null aidn_kv8_cache", op);
+  if (!c->key_pool || !c->value_pool || !c->key_scale || !c->value_scale || !c->block_table)
+    return fail(AIDN_EINVAL, "%s: null pool, scales or block table", op);
+  if (c->block_size <= 0 || c->block_size > 65536) return fail(AIDN_EINVAL, "%s: block_size %d outside [1,65536]", op, c->block_size);
+  if (c->num_blocks < 0 || c->block_table_stride <= 0) return fail(AIDN_EINVAL, "%s: num_blocks must be >= 0 and block_table_stride > 0", op);
+  if (c->kv_heads <= 0 || c->kv_heads > 65535) return fail(AIDN_EINVAL, "%s: kv_heads outside [1,65535]", op);
+  if (c->head_dim <= 0 || c->head_dim > 256) return fail(AIDN_EINVAL, "%s: head_dim %d outside [1,256]", op, c->head_dim);
+  if (c->head_dim % 8 != 0) return fail(AIDN_EUNSUPPORTED, "%s: head_dim %d is not a multiple of 8", op, c->head_dim);
+  pool.k = c->key_pool;
+  pool.v = c->value_pool;
+  pool.k_scale = c->key_scale;
+  pool.v_scale = c->value_scale;
+  pool.table = c->block_table;
+  pool.table_stride = c->block_table_stride;
+  const int64_t D = c->head_dim, dense[3] = {c->block_size * c->kv_heads * D, c->kv_heads * D, D};
+  std::memcpy(pool.stride, all_zero(c->pool_stride) ? dense : c->pool_stride, sizeof(pool.stride));
+  for (int i = 0; i < 3; ++i)
+    if (pool.stride[i] < 0 || pool.stride[i] % 4 != 0) return fail(AIDN_EINVAL, "%s: pool strides must be multiples of 4 and not negative", op);
+  if ((uintptr_t)c->key_pool % 4 != 0 || (uintptr_t)c->value_pool % 4 != 0 || (uintptr_t)c->key_scale % 4 != 0 || (uintptr_t)c->value_scale % 4 != 0)
+    return fail(AIDN_EINVAL, "%s: pools and scales must be 4-byte aligned", op);
+  pool.num_blocks = c->num_blocks;
+  pool.block_size = c->block_size;
+  pool.kv_heads = c->kv_heads;
+  pool.head_dim = c->head_dim;
+  pool.block_shift = -1;
+  for (int sft = 0; sft < 31; ++sft)
+    if ((1 << sft) == c->block_size) pool.block_shift = sft;
+  return AIDN_OK;
+}
+}  // namespace
+
+int aidn_kv8_append(const aidn_kv8_cache* cache, const aidn_kv8_append_args* a, void* cu_stream) {
+  g_err[0] = 0;
+  aidn::kv8::Append p;
+  std::memset(&p, 0, sizeof(p));
+  const int rc = build_pool("kv8_append", cache, p.c);
+  if (rc != AIDN_OK) return rc;
+  if (!a) return fail(AIDN_EINVAL, "kv8_append: null argument");
+  if (a->tokens < 0 || a->batch <= 0) return fail(AIDN_EINVAL, "kv8_append: tokens must be >= 0 and batch > 0");
+  if (a->tokens > 0x7fffffffll) return fail(AIDN_EINVAL, "kv8_append: more than 2^31-1 tokens");
+  if (a->dtype < AIDN_F32 || a->dtype > AIDN_BF16) return fail(AIDN_EINVAL, "kv8_append: unknown dtype %d", a->dtype);
+  if (a->rope < AIDN_ROPE_NONE || a->rope > AIDN_ROPE_HALVES) return fail(AIDN_EINVAL, "kv8_append: unknown rotation %d", a->rope);
+  if (!a->token_starts && a->tokens % a->batch != 0)
+    return fail(AIDN_EINVAL, "kv8_append: %lld tokens are not the same number for each of %d sequences, and token_starts is null",
+                (long long)a->tokens, a->batch);
+  if (a->tokens == 0) return AIDN_OK;
+  if (!a->key || !a->value || !a->start) return fail(AIDN_EINVAL, "kv8_append: null buffer");
+  if (a->query && (!a->query_out || a->heads <= 0)) return fail(AIDN_EINVAL, "kv8_append: queries need query_out and heads > 0");
+  if (a->rope != AIDN_ROPE_NONE && (!a->cosine || !a->sine || a->max_position < 0))
+    return fail(AIDN_EINVAL, "kv8_append: a rotation needs cosine, sine and max_position >= 0");
+  const int64_t D = cache->head_dim;
+  const size_t esz = elem_size(a->dtype);
+  const void* ptrs[] = {a->query, a->key, a->value, a->query_out, a->cosine, a->sine, a->start, a->token_starts, a->positions};
+  const size_t align[] = {esz, esz, esz, esz, 4, 4, 4, 4, 4};
+  for (int i = 0; i < 9; ++i)
+    if ((uintptr_t)ptrs[i] % align[i] != 0) return fail(AIDN_EINVAL, "kv8_append: a buffer is not aligned to its elements");
+  auto strides = [&](const int64_t* given, int64_t heads, int64_t* to) {
+    to[0] = given[0] == 0 && given[1] == 0 ? heads * D : given[0];
+    to[1] = given[0] == 0 && given[1] == 0 ? D : given[1];
+    return to[0] >= 0 && to[1] >= 0;
+  };
+  if (!strides(a->query_stride, a->heads, p.qs) || !strides(a->key_stride, cache->kv_heads, p.ks) ||
+      !strides(a->value_stride, cache->kv_heads, p.vs) || !strides(a->query_out_stride, a->heads, p.os))
+    return fail(AIDN_EINVAL, "kv8_append: negative stride");
+  p.q = a->query;
+  p.k = a->key;
+  p.v = a->value;
+  p.q_out = a->query_out;
+  p.cosine = a->cosine;
+  p.sine = a->sine;
+  p.start = a->start;
+  p.token_starts = a->token_starts;
+  p.positions = a->positions;
+  p.tokens = a->tokens;
+  p.max_position = a->max_position;
+  p.each = a->tokens / a->batch;
+  p.batch = a->batch;
+  p.heads = a->query ? a->heads : 0;
+  p.dtype = a->dtype;
+  p.rope = a->rope;
+  int launches = 0;
+  const cudaError_t e = aidn::kv8::launch_append(p, (cudaStream_t)cu_stream, &launches);
+  if (e != cudaSuccess) return fail_cuda(e, "kv8_append");
+  return post_launch_check((cudaStream_t)cu_stream, "aidn_kv8_append", nullptr);
+}
+
+int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_q, int64_t seq_kv) {
+  g_err[0] = 0;
+  if (!h || batch <= 0 || seq_q <= 0 || seq_kv <= 0) {
+    fail(AIDN_EINVAL, "kv8_workspace_bytes: bad argument");
+    return -1;
+  }
+  return 0;
+}
+
+int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_cache* cache, const int32_t* query_starts,
+                         int64_t queries, void* cu_stream) {
+  g_err[0] = 0;
+  if (!h || !a) return fail(AIDN_EINVAL, "launch_kv8: null argument");
+  const aidn_sdpa_desc& d = h->d;
+  aidn::kv8::Attend p;
+  std::memset(&p, 0, sizeof(p));
+  const int rc = build_pool("launch_kv8", cache, p.c);
+  if (rc != AIDN_OK) return rc;
+  if (cache->head_dim != d.head_dim || cache->kv_heads != d.num_kv_heads)
+    return fail(AIDN_EINVAL, "launch_kv8: the pool has %d heads of %d, the handle %d of %d", cache->kv_heads, cache->head_dim, d.num_kv_heads, d.head_dim);
+  if (!a->q || !a->out) return fail(AIDN_EINVAL, "launch_kv8: null tensor pointer");
+  if (a->batch <= 0 || a->batch > 65535 || a->seq_q <= 0 || a->seq_kv <= 0 || a->seq_q > 0x7fffffffll || a->seq_kv > 0x7fffffffll)
+    return fail(AIDN_EINVAL, "launch_kv8: batch, seq_q and seq_kv must be positive, batch at most 65535, lengths at most 2^31-1");
+  if (query_starts && (queries <= 0 || queries > 0x7fffffffll)) return fail(AIDN_EINVAL, "launch_kv8: query_starts needs the number of queries");
+  if (d.emit_lse && !a->lse) return fail(AIDN_EINVAL, "launch_kv8: emit_lse set but lse pointer is null");
+  if (d.mask_kind != AIDN_MASK_NONE && !a->mask) return fail(AIDN_EINVAL, "launch_kv8: mask_kind set but mask pointer is null");
+  if (d.mask_kind != AIDN_MASK_NONE && query_starts) return fail(AIDN_EUNSUPPORTED, "launch_kv8: masks with query_starts are not defined");
+  if (a->scale < 0.f || std::isnan(a->scale)) return fail(AIDN_EINVAL, "launch_kv8: scale must be >= 0");
+  if (a->weights || a->peer_count != 0 || a->gather_output)
+    return fail(AIDN_EUNSUPPORTED, "launch_kv8: attention weights, peer_out and gather_output are not served over an 8-bit pool");
+  if (d.path == AIDN_PATH_DECODE || d.path == AIDN_PATH_PREFILL_SM100)
+    return fail(AIDN_EUNSUPPORTED, "launch_kv8: desc.path must be AUTO or GENERIC");
+  const size_t esz = elem_size(d.qkv_dtype);
+  if ((uintptr_t)a->q % esz != 0 || (uintptr_t)a->out % elem_size(d.out_dtype) != 0) return fail(AIDN_EINVAL, "launch_kv8: q or out is not aligned to its elements");
+  const int64_t D = d.head_dim;
+  auto strides = [&](const int64_t* given, int64_t* to) {
+    if (!all_zero(given)) std::memcpy(to, given, 3 * sizeof(int64_t));
+    else if (query_starts) to[0] = 0, to[1] = D, to[2] = d.num_q_heads * D;
+    else dense_strides(to, d.num_q_heads, a->seq_q, D);
+    return to[0] >= 0 && to[1] >= 0 && to[2] >= 0;
+  };
+  if (!strides(a->q_stride, p.qs) || !strides(a->o_stride, p.os)) return fail(AIDN_EINVAL, "launch_kv8: negative stride");
+  p.q = a->q;
+  p.out = a->out;
+  p.lse = d.emit_lse ? a->lse : nullptr;
+  p.kv_len = a->kv_len;
+  p.query_starts = query_starts;
+  p.queries = query_starts ? queries : a->batch * a->seq_q;
+  p.mask = d.mask_kind != AIDN_MASK_NONE ? a->mask : nullptr;
+  p.mask_kind = d.mask_kind;
+  for (int i = 0; i < 4; ++i) p.mask_stride[i] = a->mask_stride[i];
+  p.seq_q = a->seq_q;
+  // kv_len lives on the device: no key beyond what a table row can address is looked up, whatever it says
+  const int64_t most = cache->block_table_stride < (0x7fffffffll / cache->block_size) ? cache->block_table_stride * cache->block_size : 0x7fffffffll;
+  p.seq_kv = a->seq_kv < most ? a->seq_kv : most;
+  p.causal = d.causal ? 1 : 0;
+  p.bottom_right = d.causal_bottom_right ? 1 : 0;
+  p.causal_offset = d.causal_offset;
+  p.batch = (int32_t)a->batch;
+  p.num_q_heads = d.num_q_heads;
+  p.group = h->group;
+  p.kv_begin = d.head_begin / h->group;
+  p.kv_count = h->head_count / h->group;
+  p.dtype = d.qkv_dtype;
+  p.out_f32 = d.out_dtype == AIDN_F32 ? 1 : 0;
+  p.scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt((float)d.head_dim);
+  p.softcap = d.softcap;
+  p.status = h->status_dev;
+  p.counters = reinterpret_cast<uint32_t*>(h->status_dev + 4);
+  cudaStream_t stream = (cudaStream_t)cu_stream;
+  int launches = 1;
+  const cudaError_t e = aidn::kv8::launch_attend_generic(p, stream);
+  if (e != cudaSuccess) return fail_cuda(e, "launch_kv8");
+  h->last_path = AIDN_PATH_GENERIC;
+  h->last_launches = launches;
+  return post_launch_check(stream, "aidn_sdpa_launch_kv8", h->status_dev);
 }
 
 // ---- fused multi-head attention forward ---------------------------------------------------------------------------

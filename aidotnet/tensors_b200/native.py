@@ -21,6 +21,8 @@ OK, EINVAL, EUNSUPPORTED, ECUDA, EWORKSPACE, ETIMEOUT, ENCCL = range(7)
 F32, F16, BF16 = 0, 1, 2
 # aidn_mask_kind
 MASK_NONE, MASK_KEEP_U8, MASK_KEEP_F32, MASK_ADD_F32 = 0, 1, 2, 3
+# aidn_rope
+ROPE_NONE, ROPE_INTERLEAVED, ROPE_HALVES = 0, 1, 2
 # aidn_path
 PATH_AUTO, PATH_GENERIC, PATH_DECODE, PATH_PREFILL_SM100 = 0, 1, 2, 3
 
@@ -31,6 +33,7 @@ EXPORTS = (
     "aidn_sdpa_decode_noalloc", "aidn_sdpa_launch_paged", "aidn_qkv_rope_cache", "aidn_qkv_rope_poll", "aidn_rope_interleaved",
     "aidn_sdpa_backward", "aidn_sdpa_backward_workspace_bytes", "aidn_paged_kv_append", "aidn_mha_forward",
     "aidn_mha_workspace_bytes", "aidn_peer_export", "aidn_peer_open", "aidn_peer_close",
+    "aidn_kv8_append", "aidn_sdpa_kv8_workspace_bytes", "aidn_sdpa_launch_kv8",
     "aidn_sdpa_debug_set",   # include/aidn_sdpa_debug.h
 )
 
@@ -96,13 +99,35 @@ class MhaArgs(ctypes.Structure):
     ]
 
 
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("key_pool", ctypes.c_void_p), ("value_pool", ctypes.c_void_p), ("key_scale", ctypes.c_void_p),
+        ("value_scale", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
+        ("pool_stride", ctypes.c_int64 * 3), ("num_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+    ]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p), ("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("query_out", ctypes.c_void_p),
+        ("query_stride", ctypes.c_int64 * 2), ("key_stride", ctypes.c_int64 * 2), ("value_stride", ctypes.c_int64 * 2),
+        ("query_out_stride", ctypes.c_int64 * 2), ("cosine", ctypes.c_void_p), ("sine", ctypes.c_void_p),
+        ("start", ctypes.c_void_p), ("token_starts", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("max_position", ctypes.c_int64), ("batch", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("rope", ctypes.c_int32),
+    ]
+
+
 # The argument blocks of the calls that a decode step makes, packed in one go: filling a ctypes structure field by field took
 # longer than the kernels of a small step.
 _SDPA_ARGS = struct.Struct("@6P4qP3q12qfPqiPi8P")
 _PAGED_KV = struct.Struct("@Pqii")
 _QKV_ROPE_ARGS = struct.Struct("@10P8i2q")
-assert (_SDPA_ARGS.size, _PAGED_KV.size, _QKV_ROPE_ARGS.size) == tuple(
-    ctypes.sizeof(t) for t in (SdpaArgs, PagedKv, QkvRopeArgs))
+_KV8_CACHE = struct.Struct("@5P4q4i")
+_KV8_APPEND_ARGS = struct.Struct("@4P8q5P2q4i")
+assert (_SDPA_ARGS.size, _PAGED_KV.size, _QKV_ROPE_ARGS.size, _KV8_CACHE.size, _KV8_APPEND_ARGS.size) == tuple(
+    ctypes.sizeof(t) for t in (SdpaArgs, PagedKv, QkvRopeArgs, Kv8Cache, Kv8AppendArgs))
 _NO_STRIDE, _NO_PEERS = (0, 0, 0), (0,) * 8
 
 
@@ -115,12 +140,12 @@ class AidnError(RuntimeError):
 
 _lib: Optional[ctypes.CDLL] = None
 # the entry points that take packed argument blocks (bytes)
-_launch_packed = _launch_paged_packed = _qkv_rope_packed = None
+_launch_packed = _launch_paged_packed = _qkv_rope_packed = _kv8_append_packed = _launch_kv8_packed = None
 
 
 def load() -> ctypes.CDLL:
     """Loads the CUDA library.  Raises if it has not been built: there is no CPU path behind this API."""
-    global _lib, _launch_packed, _launch_paged_packed, _qkv_rope_packed
+    global _lib, _launch_packed, _launch_paged_packed, _qkv_rope_packed, _kv8_append_packed, _launch_kv8_packed
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -179,12 +204,22 @@ def load() -> ctypes.CDLL:
     lib.aidn_rope_interleaved.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                           ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
     lib.aidn_rope_interleaved.restype = ctypes.c_int
+    lib.aidn_kv8_append.argtypes = [ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8AppendArgs), ctypes.c_void_p]
+    lib.aidn_kv8_append.restype = ctypes.c_int
+    lib.aidn_sdpa_kv8_workspace_bytes.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
+    lib.aidn_sdpa_kv8_workspace_bytes.restype = ctypes.c_int64
+    lib.aidn_sdpa_launch_kv8.argtypes = [ctypes.c_void_p, ctypes.POINTER(SdpaArgs), ctypes.POINTER(Kv8Cache), ctypes.c_void_p,
+                                         ctypes.c_int64, ctypes.c_void_p]
+    lib.aidn_sdpa_launch_kv8.restype = ctypes.c_int
     lib.aidn_sdpa_debug_set.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]
     lib.aidn_sdpa_debug_set.restype = ctypes.c_int
     pointer, block = ctypes.c_void_p, ctypes.c_char_p
     _launch_packed = ctypes.CFUNCTYPE(ctypes.c_int, pointer, block, pointer)(("aidn_sdpa_launch", lib))
     _launch_paged_packed = ctypes.CFUNCTYPE(ctypes.c_int, pointer, block, block, pointer)(("aidn_sdpa_launch_paged", lib))
     _qkv_rope_packed = ctypes.CFUNCTYPE(ctypes.c_int, block, pointer)(("aidn_qkv_rope_cache", lib))
+    _kv8_append_packed = ctypes.CFUNCTYPE(ctypes.c_int, block, block, pointer)(("aidn_kv8_append", lib))
+    _launch_kv8_packed = ctypes.CFUNCTYPE(ctypes.c_int, pointer, block, block, pointer, ctypes.c_int64, pointer)(
+        ("aidn_sdpa_launch_kv8", lib))
     _lib = lib
     return lib
 
@@ -295,6 +330,26 @@ class Handle:
             status = _launch_paged_packed(self._h, block, paged, stream)
         else:
             status = _launch_packed(self._h, block, stream)
+        if status != OK:
+            raise AidnError(status, last_error())
+
+    def kv8_workspace_bytes(self, batch: int, seq_q: int, seq_kv: int) -> int:
+        n = self._lib.aidn_sdpa_kv8_workspace_bytes(self._h, batch, seq_q, seq_kv)
+        if n < 0:
+            raise AidnError(EINVAL, last_error())
+        return int(n)
+
+    def launch_kv8(self, *, q: int, out: int, cache: bytes, batch: int, seq_q: int, seq_kv: int, stream: int,
+                   query_starts: Optional[int] = None, queries: int = 0, lse: Optional[int] = None,
+                   mask: Optional[int] = None, mask_stride: Sequence[int] = (0, 0, 0, 0), kv_len: Optional[int] = None,
+                   q_stride=None, o_stride=None, scale: float = 0.0, workspace: Optional[int] = None,
+                   workspace_bytes: int = 0) -> None:
+        """Enqueues attention over a pool held in 8 bits; ``cache`` is what ``kv8_cache`` packed."""
+        block = _SDPA_ARGS.pack(
+            q or 0, 0, 0, out or 0, lse or 0, mask or 0, *mask_stride, kv_len or 0, batch, seq_q, seq_kv,
+            *_strides(q_stride), *_NO_STRIDE, *_NO_STRIDE, *_strides(o_stride), scale, workspace or 0, workspace_bytes,
+            False, 0, 0, *_NO_PEERS)
+        status = _launch_kv8_packed(self._h, block, cache, query_starts, queries, stream)
         if status != OK:
             raise AidnError(status, last_error())
 
@@ -416,3 +471,26 @@ def paged_kv_append(new_keys: int, new_values: int, key_pool: int, value_pool: i
     check(load().aidn_paged_kv_append(ctypes.c_void_p(new_keys), ctypes.c_void_p(new_values), ctypes.c_void_p(key_pool),
                                       ctypes.c_void_p(value_pool), ctypes.c_void_p(block_table), start_position, tokens,
                                       block_size, num_blocks, row_bytes, ctypes.c_void_p(stream)))
+
+
+def kv8_cache(*, key_pool: int, value_pool: int, key_scale: int, value_scale: int, block_table: int, block_table_stride: int,
+              num_blocks: int, block_size: int, kv_heads: int, head_dim: int, pool_stride: Optional[Sequence[int]] = None) -> bytes:
+    """The ``aidn_kv8_cache`` block of a pool held in 8 bits and the table that it is read through."""
+    return _KV8_CACHE.pack(key_pool or 0, value_pool or 0, key_scale or 0, value_scale or 0, block_table or 0, block_table_stride,
+                           *_strides(pool_stride), num_blocks, block_size, kv_heads, head_dim)
+
+
+def kv8_append(cache: bytes, *, key: int, value: int, start: int, tokens: int, batch: int, dtype: int, stream: int,
+               query: Optional[int] = None, query_out: Optional[int] = None, heads: int = 0, cosine: Optional[int] = None,
+               sine: Optional[int] = None, rope: int = ROPE_NONE, max_position: int = 0, token_starts: Optional[int] = None,
+               positions: Optional[int] = None, query_stride=(0, 0), key_stride=(0, 0), value_stride=(0, 0),
+               query_out_stride=(0, 0)) -> None:
+    """Rotates a step's queries and keys and puts keys and values into their sequences' blocks of an 8-bit pool."""
+    if _lib is None:
+        load()
+    status = _kv8_append_packed(cache, _KV8_APPEND_ARGS.pack(
+        query or 0, key or 0, value or 0, query_out or 0, *query_stride, *key_stride, *value_stride, *query_out_stride,
+        cosine or 0, sine or 0, start or 0, token_starts or 0, positions or 0, tokens, max_position, batch, heads, dtype, rope),
+        stream)
+    if status != OK:
+        raise AidnError(status, last_error())

@@ -290,6 +290,71 @@ AIDN_API int aidn_rope_interleaved(const float* input, const float* cosine, cons
                                    int64_t rows, int32_t head_dim, int32_t seq_len, int32_t start_position,
                                    void* cu_stream);
 
+/* ---- paged K / V held in 8 bits ---------------------------------------------------------------------------------
+ * The pool of aidn_paged_kv with one byte an element: an E4M3 code, and for every (block, KV head) one fp32 scale for the keys
+ * and one for the values; an element stands for code * scale.  Half the bytes of a 16-bit pool, which is what a decode step is
+ * bound by.  No counterpart in the reference (its DevicePagedKVCache holds fp32).
+ *
+ * A scale is a power of two: the smallest from 2^-100 on with which no element of the block is above 448, the largest code.
+ * Dividing by it is exact, so that what an element loses is the rounding of its code alone (three mantissa bits), and when a
+ * block that already holds tokens needs a larger scale for a new one, the codes it has move by an exponent. */
+typedef struct {
+  uint8_t* key_pool;          /* code (block, token, head, d) at block*pool_stride[0] + token*pool_stride[1] + head*pool_stride[2] + d */
+  uint8_t* value_pool;
+  float* key_scale;           /* [num_blocks, kv_heads]                                                            */
+  float* value_scale;
+  const int32_t* block_table; /* [batch, block_table_stride] device, as in aidn_paged_kv                            */
+  int64_t block_table_stride; /* entries between consecutive sequences, and the most that one sequence may use      */
+  int64_t pool_stride[3];     /* bytes; all zero = dense [num_blocks, block_size, kv_heads, head_dim]               */
+  int32_t num_blocks;         /* > 0: entries outside [0, num_blocks) are skipped                                   */
+  int32_t block_size;         /* tokens per block, 1 .. 65536                                                       */
+  int32_t kv_heads;
+  int32_t head_dim;           /* a multiple of 8 up to 256                                                          */
+} aidn_kv8_cache;
+
+typedef enum { AIDN_ROPE_NONE = 0, AIDN_ROPE_INTERLEAVED = 1 /* pairs (2i, 2i+1) */, AIDN_ROPE_HALVES = 2 /* (i, i + D/2) */ } aidn_rope;
+
+/* A step's new tokens: queries and keys rotated by their positions (fp32, every product and sum rounded on its own), queries
+ * written out, keys and values put into their sequences' blocks.  Token i of sequence b is its cache position start[b] + i.
+ * One launch; the blocks that it writes must belong to one sequence each (copy-on-write is the caller's, as for
+ * aidn_paged_kv_append).  Only finite elements count for a scale: a NaN becomes the NaN code, an infinity
+ * +-448 * scale. */
+typedef struct {
+  const void* query;          /* [tokens, heads, head_dim] or NULL: no queries                                      */
+  const void* key;            /* [tokens, kv_heads, head_dim]                                                       */
+  const void* value;
+  void* query_out;            /* may be `query` itself, with the same strides                                       */
+  int64_t query_stride[2];    /* elements for (token, head); both zero = dense                                      */
+  int64_t key_stride[2];
+  int64_t value_stride[2];
+  int64_t query_out_stride[2];
+  const float* cosine;        /* [max_position, head_dim / 2], indexed by position; unused with AIDN_ROPE_NONE      */
+  const float* sine;
+  const int32_t* start;       /* [batch] tokens in the cache before these; a negative one skips the sequence's K / V */
+  const int32_t* token_starts;/* [batch + 1] first token of each sequence, ascending from 0; NULL: tokens / batch each */
+  const int32_t* positions;   /* [tokens] rotation position, or NULL: the cache position                            */
+  int64_t tokens;
+  int64_t max_position;       /* a position outside [0, max_position) is left unrotated                             */
+  int32_t batch;
+  int32_t heads;
+  int32_t dtype;              /* aidn_dtype of query, key, value and query_out                                      */
+  int32_t rope;               /* aidn_rope                                                                          */
+} aidn_kv8_append_args;
+AIDN_API int aidn_kv8_append(const aidn_kv8_cache* cache, const aidn_kv8_append_args* args, void* cu_stream);
+
+/* Attention over such a pool.  args.k, args.v and their strides are not looked at; args.seq_q is the largest number of queries
+ * of a sequence, args.seq_kv the largest number of keys, kv_len[b] (NULL: seq_kv) the keys of sequence b, its new tokens included.
+ * With query_starts (device, [batch + 1], ascending from 0 to `queries`) sequence b has the queries query_starts[b] ..
+ * query_starts[b + 1] - 1 of a [queries, Hq, D] tensor (strides: [1] head, [2] query; zero = dense), without it seq_q each in the
+ * layout of aidn_sdpa_launch.  desc.causal with causal_bottom_right aligns each sequence by its own lengths: query i of n sees
+ * key j iff j <= kv_len[b] - n + i.  A query that sees no key gives zeros and a log-sum-exp of -inf.  lse is dense
+ * [queries in order, Hq].  desc.mask_kind: masks over (b, h, i, j) run on the any-shape kernel, without query_starts only.
+ * A visible NaN code makes its rows NaN; codes past kv_len[b] may be anything.
+ * Workspace: aidn_sdpa_kv8_workspace_bytes() for the partial results of keys that are cut over CTAs; calls without one run uncut. */
+AIDN_API int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_q, int64_t seq_kv);
+AIDN_API int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* args, const aidn_kv8_cache* cache,
+                                  const int32_t* query_starts, int64_t queries, void* cu_stream);
+
 /* ---- fused multi-head attention forward ---------------------------------------------------------------------
  * IEngine.MultiHeadAttentionForward (src/AiDotNet.Tensors/Engines/IEngine.cs:4201-4208; CPU
  * CpuEngine.MultiHeadAttention.cs:68-338, GPU composition DirectGpuTensorEngine.MissingKernels.cs:5793-5870):
