@@ -114,6 +114,7 @@ struct aidn_sdpa {
   int last_launches;
   float* debug;
   int debug_mode;
+  uint64_t kv8_raised;                  // which kernels over 8-bit pools had their shared-memory limit raised in this context
   aidn::PrefillMapCache prefill_maps;   // tensor maps of the last tcgen05 prefill launch (see common.cuh)
 };
 
@@ -263,6 +264,7 @@ int aidn_sdpa_create(const aidn_sdpa_desc* desc, aidn_sdpa_t* out) {
   h->debug = nullptr;
   h->debug_mode = 0;
   h->num_sms = 0;
+  h->kv8_raised = 0;
   std::memset(&h->prefill_maps, 0, sizeof(h->prefill_maps));
   e = cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, d.device);
   if (e == cudaSuccess) e = cudaMalloc(&h->status_dev, kHandleWords * sizeof(int32_t));
@@ -899,7 +901,8 @@ int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_
     fail(AIDN_EINVAL, "kv8_workspace_bytes: bad argument");
     return -1;
   }
-  return 0;
+  if (h->d.path == AIDN_PATH_GENERIC || h->d.mask_kind != AIDN_MASK_NONE || h->d.head_dim % 16 != 0) return 0;
+  return align_up(aidn::kv8::split_workspace_bytes(h->d.head_dim, h->d.out_dtype == AIDN_F32, seq_q * h->group, h->num_sms), 256);
 }
 
 int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_cache* cache, const int32_t* query_starts,
@@ -964,9 +967,15 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   p.counters = reinterpret_cast<uint32_t*>(h->status_dev + 4);
   cudaStream_t stream = (cudaStream_t)cu_stream;
   int launches = 1;
-  const cudaError_t e = aidn::kv8::launch_attend_generic(p, stream);
+  cudaError_t e;
+  if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
+    e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);
+    h->last_path = AIDN_PATH_DECODE;
+  } else {
+    e = aidn::kv8::launch_attend_generic(p, stream);
+    h->last_path = AIDN_PATH_GENERIC;
+  }
   if (e != cudaSuccess) return fail_cuda(e, "launch_kv8");
-  h->last_path = AIDN_PATH_GENERIC;
   h->last_launches = launches;
   return post_launch_check(stream, "aidn_sdpa_launch_kv8", h->status_dev);
 }

@@ -147,6 +147,11 @@ __device__ __forceinline__ float inverse_pow2(float s) { return __uint_as_float(
 
 cudaError_t launch_append(const Append& p, cudaStream_t stream, int* launches);
 cudaError_t launch_attend_generic(const Attend& p, cudaStream_t stream);
+// Few queries (csrc/kv8_split.cu): head sizes that are a multiple of 16, 16-byte aligned pools, no mask.  Without its workspace keys are not
+// cut.  raised: a word of the handle, which kernels had their shared-memory limit raised.
+bool split_supported(const Attend& p);
+int64_t split_workspace_bytes(int head_dim, bool exact, int64_t rows, int num_sms);
+cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream);
 
 }  // namespace kv8
 }  // namespace aidn
