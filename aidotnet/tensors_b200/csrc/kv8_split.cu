@@ -31,7 +31,8 @@ constexpr float kLift = 9.f;
 struct Split {
   float* partial;    // [2 grid][8 NR][DP], or null: lines are not cut
   float2* stats;     // [2 grid][8 NR]: maximum and sum
-  int least;         // tiles of a share
+  int least;         // tiles of a warp's share
+  bool query_vec, out_vec;   // 16 bytes of the queries, four elements of the results are aligned
 };
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -44,6 +45,61 @@ __device__ __forceinline__ uint2 ld_stream8(const void* ptr) {
   asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(ptr));
   return r;
 }
+// Sixteen elements of a query as they lie: eight words of 16-bit elements, sixteen of 32-bit ones.  (Volatile: issued where they stand.)
+__device__ __forceinline__ void ld_words4(const void* ptr, uint32_t* w) {
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(ptr));
+}
+template <int T>
+__device__ __forceinline__ void load16(const Attend& p, int64_t at, bool vec, uint32_t* w) {
+  if (T == 2 && p.dtype == AIDN_F32) {
+    const float* q = static_cast<const float*>(p.q) + at;
+#pragma unroll
+    for (int e = 0; e < 8 * T; e += 4) {
+      if (vec) {
+        ld_words4(q + e, w + e);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[e + u] = __float_as_uint(q[e + u]);
+      }
+    }
+    return;
+  }
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+#pragma unroll
+  for (int e = 0; e < 8; e += 4) {
+    if (vec) {
+      ld_words4(q + 2 * e, w + e);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[e + u] = q[2 * (e + u)] | (uint32_t)q[2 * (e + u) + 1] << 16;
+    }
+  }
+}
+template <int T>
+__device__ __forceinline__ float widen(const Attend& p, const uint32_t* w, int e) {
+  if (T == 2 && p.dtype == AIDN_F32) return __uint_as_float(w[T == 2 ? e : 0]);
+  const uint32_t v = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+  return p.dtype == AIDN_F16 ? __half2float(__ushort_as_half((unsigned short)v)) : __uint_as_float(v << 16);
+}
+__device__ __forceinline__ void store4(const Attend& p, int64_t at, bool vec, float4 o) {
+  if (p.out_f32) {
+    float* to = static_cast<float*>(p.out) + at;
+    if (vec) {
+      *reinterpret_cast<float4*>(to) = o;
+    } else {
+      to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w;
+    }
+    return;
+  }
+  uint16_t* to = static_cast<uint16_t*>(p.out) + at;
+  const uint32_t a = p.dtype == AIDN_F16 ? pack_pair<__half>(o.x, o.y) : pack_pair<__nv_bfloat16>(o.x, o.y);
+  const uint32_t c = p.dtype == AIDN_F16 ? pack_pair<__half>(o.z, o.w) : pack_pair<__nv_bfloat16>(o.z, o.w);
+  if (vec) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(a, c);
+  } else {
+    to[0] = (uint16_t)a; to[1] = (uint16_t)(a >> 16); to[2] = (uint16_t)c; to[3] = (uint16_t)(c >> 16);
+  }
+}
 // tanh to 3e-7 of 1: the logits are off by that times the cap.
 __device__ __forceinline__ float tanh_ex2(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(x * (2.f * kLog2e), 80.f))); }
 // Whether any of four codes is a NaN.
@@ -53,16 +109,15 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   return x & ~(hit * 0xffu);
 }
 
-// What lies past the D bytes of a key is never read: the fragments' elements from D on are zeros.
 template <int DP, int NR, int T, bool UB>
 struct Config {
-  static constexpr int kWarps = NR == 1 ? 8 : 4;
-  static constexpr int kMinCtas = DP == 256 ? (NR == 1 ? 1 : 1) : (NR == 1 ? 2 : (NR == 2 && DP == 64 ? 4 : (NR == 4 && DP == 128 ? 2 : 3)));
+  static constexpr int kWarps = NR == 1 && DP < 256 ? 8 : 4;
+  static constexpr int kMinCtas = DP == 256 ? 2 : (NR == 1 ? 2 : 3);
   static constexpr int kSteps = DP / 16;                 // of 16 elements: fragments of a key
   static constexpr int kRows = 8 * NR;
-  static constexpr int kPitch = DP + 4;                  // floats between the rows of a warp's results
-  static constexpr int kQueryWords = T * NR * kSteps * 32 * 2;
-  static constexpr size_t kSmem = (size_t)kQueryWords * 4 + (size_t)kWarps * kRows * kPitch * 4;
+  static constexpr int kPitch = DP + 4;                  // floats between the rows of a partial result
+  static constexpr int kQueryWords = T * NR * kSteps * 32 * 2;   // of a warp
+  static constexpr size_t kSmem = (size_t)kWarps * (kQueryWords * 4 + 2 * kRows * kPitch * 4);
 };
 
 template <int DP, int NR, int T, bool UB>
@@ -74,18 +129,17 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
   constexpr int VB = DP == 64 ? 8 : 16;           // bytes of a value row a lane reads at a time
   constexpr int VC = DP == 256 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint2* const qfrag = reinterpret_cast<uint2*>(smem);                          // [T][NR][KS][32]
-  float* const wacc = reinterpret_cast<float*>(smem + C::kQueryWords * 4);      // [NW][ROWS][kPitch]
-  __shared__ float row_c[ROWS];
-  __shared__ int row_lim[ROWS];
-  __shared__ float2 wstat[NW][ROWS];
-  __shared__ float wref[NW];
-  __shared__ int64_t scan[NW + 1];
-  __shared__ int found_b;
-  __shared__ int64_t found_base;
-  __shared__ int last_flag;
+  float* const wacc = reinterpret_cast<float*>(smem + NW * C::kQueryWords * 4);   // [NW][2][ROWS][kPitch]: parts of cut lines
+  __shared__ float row_c[NW][ROWS];
+  __shared__ int row_lim[NW][ROWS];
+  __shared__ float2 wstat[NW][2][ROWS];
+  __shared__ int64_t wline[NW][2];      // the line's first tile, or -1
+  __shared__ int winfo[NW][2][3];       // its sequence, number and tiles
+  __shared__ int64_t scan[NW], prefix[NW * 32];
+  __shared__ int last_flag[2];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint2* const qfrag = reinterpret_cast<uint2*>(smem) + warp * (C::kQueryWords / 2);   // [T][NR][KS][32]
   const int D = p.c.head_dim, G = p.group;
   const bool cut = sp.partial != nullptr;
   pdl_wait();
@@ -93,15 +147,13 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 
   auto tiles_of = [&](int keys) { return keys > kTile ? (keys + kTile - 1) / kTile : 1; };
   auto lines_of = [&](int n) { return ((n * G + ROWS - 1) / ROWS) * p.kv_count; };
+  auto weight_of = [&](int b) { return (int64_t)lines_of(rows_of(p, b).count) * (cut ? tiles_of(keys_of(p, b)) : 1); };
 
-  // ---- the share of this CTA: all threads sum their sequences' tiles, the one whose sequences hold its first tile says so
+  // ---- the share of this CTA and of its warps: the threads sum up their sequences' tiles
   const int per = (p.batch + NW * 32 - 1) / (NW * 32);
   const int b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
   int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) {
-    const int64_t lines = lines_of(rows_of(p, b).count);
-    mine += cut ? lines * tiles_of(keys_of(p, b)) : lines;
-  }
+  for (int b = b_lo; b < b_hi; ++b) mine += weight_of(b);
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -109,6 +161,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     if (lane >= o) upto += v;
   }
   if (lane == 31) scan[warp] = upto;
+  if (lane < 2) wline[warp][lane] = -1;
   __syncthreads();
   int64_t total = 0, before = 0;
 #pragma unroll
@@ -116,30 +169,23 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     if (w == warp) before = total;
     total += scan[w];
   }
-  before += upto - mine;
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  if (cut) {
-    if (share < sp.least) share = sp.least;
-    share = (share + NW - 1) / NW * NW;
-  }
-  int64_t pos = (int64_t)blockIdx.x * share;
-  const int64_t end = min(pos + share, total);
-  if (pos >= end) return;
-  if (pos >= before && pos < before + mine) {
-    int64_t base = before;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const int64_t lines = lines_of(rows_of(p, b).count), w = cut ? lines * tiles_of(keys_of(p, b)) : lines;
-      if (pos < base + w) {
-        found_b = b;
-        found_base = base;
-        break;
-      }
-      base += w;
-    }
-  }
+  prefix[tid] = before + upto - mine;
+  int64_t share = (total + (int64_t)gridDim.x * NW - 1) / ((int64_t)gridDim.x * NW);   // of a warp
+  if (cut && share < sp.least) share = sp.least;
+  const int64_t cta_pos = (int64_t)blockIdx.x * share * NW, cta_end = min(cta_pos + share * NW, total);
+  if (cta_pos >= cta_end) return;
   __syncthreads();
-  int b = found_b;
-  int64_t base = found_base;
+  int64_t pos = min(cta_pos + warp * share, cta_end);
+  const int64_t end = min(pos + share, cta_end);
+  int b = 0;
+  int64_t base = 0;
+  if (pos < end) {   // the last thread whose sequences begin at or before pos, then the sequence among its own
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) at += __popc(__ballot_sync(0xffffffffu, prefix[w * 32 + lane] <= pos));
+    b = (at - 1) * per;
+    base = prefix[at - 1];
+  }
   bool bad = false;
 
   while (pos < end) {
@@ -151,7 +197,8 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       ++b;
       continue;
     }
-    const int off = (int)((pos - base) / tiles), t0 = cut ? (int)((pos - base) % tiles) : 0;
+    const int64_t into = pos - base;   // (a division of 64 bits takes over a hundred instructions)
+    const int off = into < 0x7fffffff ? (int)into / tiles : (int)(into / tiles), t0 = cut ? (int)(into - (int64_t)off * tiles) : 0;
     const int kvh = p.kv_begin + off % p.kv_count, r0 = off / p.kv_count * ROWS;
     const int rows = min(ROWS, rw.count * G - r0);
     const int t1 = cut ? (int)min((int64_t)tiles, t0 + (end - pos)) : tiles_of(keys);
@@ -159,58 +206,178 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     const int64_t line_pos = pos - t0;
     pos += cut ? t1 - t0 : 1;
 
-    // ---- queries: scaled by a power of two so that the largest element is in [2^12, 2^13), as fragments
-    for (int r = warp; r < ROWS; r += NW) {
-      float x[DP / 128 > 0 ? DP / 128 : 1][4];
-      float largest = 0.f;
-      const bool valid = r < rows;
-      const int i = (r0 + r) / G, h = kvh * G + (r0 + r) % G;
-      const int64_t at = valid ? query_at(p, p.qs, rw, b, h, i) : 0;
+    // the queries are on their way while the first keys are looked up: lane (g, t) takes of row g (of eight) what it is to multiply with
+    uint32_t qr[NR][KC][8 * T];
 #pragma unroll
-      for (int j = 0; j < (DP + 127) / 128; ++j) {
-        const int d = 128 * j + 4 * lane;
+    for (int n = 0; n < NR; ++n) {
+      const int r = 8 * n + g;
+      if (r >= rows) continue;
+      const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+      const int64_t at = query_at(p, p.qs, rw, b, h, i) + 16 * t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = 0.f;
-          if (valid && d < D) {
-            if (p.dtype == AIDN_F32) v = static_cast<const float*>(p.q)[at + d + e];
-            else if (p.dtype == AIDN_F16) v = __half2float(static_cast<const __half*>(p.q)[at + d + e]);
-            else v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[at + d + e]);
-          }
-          x[j][e] = v;
-          largest = fmaxf(largest, fabsf(v));
+      for (int j = 0; j < KC; ++j)
+        if (64 * j + 16 * t < D) load16<T>(p, at + 64 * j, sp.query_vec, qr[n][j]);
+    }
+
+    const int lim_least = visible(p, keys, rw.count, rw.count == 1 ? 0 : r0 / G);
+    const int lim_most = rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + rows - 1) / G);
+    const int t_end = min(t1, (lim_most + kTile - 1) / kTile);
+    // ---- tiles t0 .. t_end - 1.  The blocks of the next 32 are looked up together, a lane each.
+    const int32_t* table = p.c.table + b * p.c.table_stride;
+    const int64_t pitch = p.c.stride[1];
+    const uint8_t* const klane = p.c.k + kvh * p.c.stride[2] + 16 * t + (UB ? g * pitch : 0);
+    const uint8_t* const vlane = p.c.v + kvh * p.c.stride[2] + VB * g + (UB ? 2 * t * pitch : 0);
+    int entry = -1;
+    float ks_l = 0.f, vs_l = 0.f;
+    auto look_up = [&](int tile) {   // this lane's tile (UB: a tile lies in one block)
+      entry = -1;
+      ks_l = vs_l = 0.f;
+      if (tile < t_end) {
+        entry = checked_block(p.c, table[block_of(p.c, tile * kTile)], bad);
+        if (entry >= 0) {
+          ks_l = p.c.k_scale[(int64_t)entry * p.c.kv_heads + kvh];
+          vs_l = p.c.v_scale[(int64_t)entry * p.c.kv_heads + kvh];
         }
       }
+    };
+    // K fragments: keys g, g + 8 of the tile; V fragments: keys 2t, 2t + 1, 2t + 8, 2t + 9.
+    uint4 kr[2][KC];
+    uint4 vr[4][VC];
+    float ks[2], vs[2], ks_n[2], vs_n[2];   // of keys g and g + 8: this tile's, and (not UB) the next one's
+    bool full_n = false;                    // all keys of the tile are there, and a row has DP bytes
+    bool ok_n[2];
+    int64_t row_n = -1;                     // UB: offset of the tile's first row, -1 without one
+    int64_t vrow[UB ? 1 : 4];               // else of the values' rows
+    auto find = [&](int tile, int slot) {   // and loads the keys
+      const int key0 = tile * kTile;
+      if constexpr (UB) {
+        const int ent = __shfl_sync(0xffffffffu, entry, slot);
+        const int first = key0 - block_of(p.c, key0) * p.c.block_size;
+        row_n = ent >= 0 ? ent * p.c.stride[0] + first * pitch : -1;
+        full_n = ent >= 0 && key0 + kTile <= keys && D == DP;
+        if (full_n) {
+          const uint8_t* at = klane + row_n;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+          for (int q = 0; q < KC; ++q) kr[0][q] = ld_stream16(at + 64 * q);
+          at += 8 * pitch;
+#pragma unroll
+          for (int q = 0; q < KC; ++q) kr[1][q] = ld_stream16(at + 64 * q);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            ok_n[j] = ent >= 0 && key0 + g + 8 * j < keys;
+#pragma unroll
+            for (int q = 0; q < KC; ++q)
+              kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(klane + row_n + 8 * j * pitch + 64 * q) : make_uint4(0, 0, 0, 0);
+          }
+        }
+      } else {
+        auto lookup = [&](int key, float* ksv, float* vsv) -> int64_t {
+          if (key >= keys) return -1;
+          const int at = block_of(p.c, key);
+          const int ent = checked_block(p.c, table[at], bad);
+          if (ent < 0) return -1;
+          if (ksv) {
+            *ksv = p.c.k_scale[(int64_t)ent * p.c.kv_heads + kvh];
+            *vsv = p.c.v_scale[(int64_t)ent * p.c.kv_heads + kvh];
+          }
+          return ent * p.c.stride[0] + (key - at * p.c.block_size) * pitch;
+        };
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ks_n[j] = vs_n[j] = 0.f;
+          const int64_t row = lookup(key0 + g + 8 * j, &ks_n[j], &vs_n[j]);
+          ok_n[j] = row >= 0;
+#pragma unroll
+          for (int q = 0; q < KC; ++q)
+            kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(klane + row + 64 * q) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vrow[UB ? 0 : j] = lookup(key0 + 2 * t + (j & 1) + 8 * (j >> 1), nullptr, nullptr);
+      }
+    };
+    auto load_v = [&](int key0) {
+      if (UB && full_n) {
+        const uint8_t* at = vlane + row_n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int q = 0; q < VC; ++q) {
+            if (VB == 8) {
+              const uint2 x = ld_stream8(at + 128 * q);
+              vr[j][q].x = x.x; vr[j][q].y = x.y;
+            } else {
+              vr[j][q] = ld_stream16(at + 128 * q);
+            }
+          }
+          at += j == 1 ? 7 * pitch : pitch;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = (j & 1) + 8 * (j >> 1);
+          const int64_t row = UB ? (row_n >= 0 && key0 + 2 * t + k < keys ? row_n + k * pitch : -1) : vrow[UB ? 0 : j];
+#pragma unroll
+          for (int q = 0; q < VC; ++q) {
+            const bool there = row >= 0 && 128 * q + VB * g < D;
+            if (VB == 8) {
+              const uint2 x = there ? ld_stream8(vlane + row) : make_uint2(0, 0);
+              vr[j][q].x = x.x; vr[j][q].y = x.y;
+            } else {
+              vr[j][q] = there ? ld_stream16(vlane + row + 128 * q) : make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+      }
+    };
+    int tile = t0, slot = 0;
+    if (tile < t_end) {   // (the first keys are on their way while the queries are laid out)
+      if (UB) look_up(tile + lane);
+      find(tile, 0);
+      load_v(tile * kTile);
+    }
+
+    // ---- queries: scaled by a power of two so that the largest element is in [2^12, 2^13), as fragments
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const int r = 8 * n + g;
+      const bool valid = r < rows;
+      float largest = 0.f;
+#pragma unroll
+      for (int j = 0; j < KC; ++j)
+        if (valid && 64 * j + 16 * t < D) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) largest = fmaxf(largest, fabsf(widen<T>(p, qr[n][j], e)));
+        }
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
       int up = 12 - ((int)(__float_as_uint(largest) >> 23) - 127);   // (zeros and what is below the normal floats: 2^126)
       up = max(-110, min(up, 126));
       const float f = __uint_as_float((uint32_t)(up + 127) << 23);
 #pragma unroll
-      for (int j = 0; j < (DP + 127) / 128; ++j) {
-        const int d = 128 * j + 4 * lane;
-        if (d >= DP) continue;
-        const int step = d / 64 * 4 + d % 16 / 4, to = (r % 8) * 4 + d % 64 / 16;
-        __half2 hi[2], lo[2];
+      for (int j = 0; j < KC; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float a = x[j][2 * e] * f, c = x[j][2 * e + 1] * f;
-          hi[e] = __floats2half2_rn(a, c);
-          if (T == 2) lo[e] = __floats2half2_rn(a - __low2float(hi[e]), c - __high2float(hi[e]));
+        for (int i = 0; i < 4; ++i) {
+          __half2 hi[2] = {}, lo[2] = {};
+          if (valid && 64 * j + 16 * t < D) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float a = widen<T>(p, qr[n][j], 4 * i + 2 * e) * f, c = widen<T>(p, qr[n][j], 4 * i + 2 * e + 1) * f;
+              hi[e] = __floats2half2_rn(a, c);
+              if (T == 2) lo[e] = __floats2half2_rn(a - __low2float(hi[e]), c - __high2float(hi[e]));
+            }
+          }
+          uint2* const dst = qfrag + (n * KS + 4 * j + i) * 32 + lane;
+          dst[0] = make_uint2(*reinterpret_cast<uint32_t*>(&hi[0]), *reinterpret_cast<uint32_t*>(&hi[1]));
+          if (T == 2) dst[NR * KS * 32] = make_uint2(*reinterpret_cast<uint32_t*>(&lo[0]), *reinterpret_cast<uint32_t*>(&lo[1]));
         }
-        qfrag[((r / 8) * KS + step) * 32 + to] = make_uint2(*reinterpret_cast<uint32_t*>(&hi[0]), *reinterpret_cast<uint32_t*>(&hi[1]));
-        if (T == 2)
-          qfrag[((NR + r / 8) * KS + step) * 32 + to] = make_uint2(*reinterpret_cast<uint32_t*>(&lo[0]), *reinterpret_cast<uint32_t*>(&lo[1]));
-      }
-      if (lane == 0) {
-        row_c[r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (p.softcap > 0.f ? 1.f : kLog2e);
-        row_lim[r] = valid ? visible(p, keys, rw.count, i) : keys;
+      if (t == 0) {
+        row_c[warp][r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (p.softcap > 0.f ? 1.f : kLog2e);
+        row_lim[warp][r] = !valid ? keys : (rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + r) / G));
       }
     }
-    __syncthreads();
+    __syncwarp();
 
-    const int lim_least = visible(p, keys, rw.count, r0 / G), lim_most = visible(p, keys, rw.count, (r0 + rows - 1) / G);
-    const int t_end = min(t1, (lim_most + kTile - 1) / kTile);
     float acc[NR][MT][4];
     float m[NR][2], l[NR][2], c[NR][2];
     int lim[NR][2];
@@ -225,108 +392,24 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       for (int e = 0; e < 2; ++e) {
         m[n][e] = kUnset;
         l[n][e] = 0.f;
-        c[n][e] = row_c[8 * n + 2 * t + e];
-        lim[n][e] = row_lim[8 * n + 2 * t + e];
+        c[n][e] = row_c[warp][8 * n + 2 * t + e];
+        lim[n][e] = row_lim[warp][8 * n + 2 * t + e];
       }
     }
-    uint2 qreg[NR == 1 && T == 1 ? KS : 1];
-    if constexpr (NR == 1 && T == 1) {
+    for (; tile < t_end; ++tile) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qreg[s] = qfrag[s * 32 + lane];
-    }
-
-    // ---- tiles of this warp: t0 + warp, + NW, ...  The blocks of the next 32 are looked up together, a lane each.
-    const int32_t* table = p.c.table + b * p.c.table_stride;
-    const uint8_t* const kbase = p.c.k + kvh * p.c.stride[2];
-    const uint8_t* const vbase = p.c.v + kvh * p.c.stride[2];
-    int entry = -1;
-    float ks_l = 0.f, vs_l = 0.f;
-    auto look_up = [&](int tile) {   // this lane's tile (UB: a tile lies in one block)
-      entry = -1;
-      ks_l = vs_l = 0.f;
-      if (tile < t_end) {
-        entry = checked_block(p.c, table[block_of(p.c, tile * kTile)], bad);
-        if (entry >= 0) {
-          ks_l = p.c.k_scale[(int64_t)entry * p.c.kv_heads + kvh];
-          vs_l = p.c.v_scale[(int64_t)entry * p.c.kv_heads + kvh];
-        }
+      for (int j = 0; j < 2; ++j) {
+        ks[j] = UB ? __shfl_sync(0xffffffffu, ks_l, slot) : ks_n[j];
+        vs[j] = UB ? __shfl_sync(0xffffffffu, vs_l, slot) : vs_n[j];
       }
-    };
-    uint4 kr[2][KC];
-    uint4 vr[4][VC];
-    float ks[2], vs[2], ks_n[2], vs_n[2];   // of keys g and g + 8: this tile's, and the next one's
-    bool ok[2], ok_n[2];
-    int64_t vrow[4];
-    // Rows and scales of a tile's keys.  K fragments: keys g, g + 8; V fragments: keys 2t, 2t + 1, 2t + 8, 2t + 9.
-    auto find = [&](int tile, int slot) {
+      // rows of which not all keys of the tile are seen, or keys that are not there
       const int key0 = tile * kTile;
-      if constexpr (UB) {
-        const int ent = __shfl_sync(0xffffffffu, entry, slot);
-        ks_n[0] = ks_n[1] = __shfl_sync(0xffffffffu, ks_l, slot);
-        vs_n[0] = vs_n[1] = __shfl_sync(0xffffffffu, vs_l, slot);
-        const int first = key0 - block_of(p.c, key0) * p.c.block_size;
-        const int64_t row = ent * p.c.stride[0] + first * p.c.stride[1];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          ok_n[j] = ent >= 0 && key0 + g + 8 * j < keys;
-          const uint8_t* at = kbase + row + (g + 8 * j) * p.c.stride[1];
-#pragma unroll
-          for (int q = 0; q < KC; ++q)
-            kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(at + 64 * q + 16 * t) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = 2 * t + (j & 1) + 8 * (j >> 1);
-          vrow[j] = ent >= 0 && key0 + k < keys ? row + k * p.c.stride[1] : -1;
-        }
-      } else {
-        auto lookup = [&](int key, float* ksv, float* vsv) -> int64_t {
-          if (key >= keys) return -1;
-          const int at = block_of(p.c, key);
-          const int ent = checked_block(p.c, table[at], bad);
-          if (ent < 0) return -1;
-          if (ksv) {
-            *ksv = p.c.k_scale[(int64_t)ent * p.c.kv_heads + kvh];
-            *vsv = p.c.v_scale[(int64_t)ent * p.c.kv_heads + kvh];
-          }
-          return ent * p.c.stride[0] + (key - at * p.c.block_size) * p.c.stride[1];
-        };
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          ks_n[j] = vs_n[j] = 0.f;
-          const int64_t row = lookup(key0 + g + 8 * j, &ks_n[j], &vs_n[j]);
-          ok_n[j] = row >= 0;
-#pragma unroll
-          for (int q = 0; q < KC; ++q)
-            kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(kbase + row + 64 * q + 16 * t) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vrow[j] = lookup(key0 + 2 * t + (j & 1) + 8 * (j >> 1), nullptr, nullptr);
+      const bool full = full_n, edge = !full || key0 + kTile > lim_least;
+      bool ok[2] = {true, true};
+      if (!full) {
+        ok[0] = ok_n[0];
+        ok[1] = ok_n[1];
       }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int q = 0; q < VC; ++q) {
-          const int d = 128 * q + VB * g;
-          if (VB == 8) {
-            const uint2 x = vrow[j] >= 0 && d < D ? ld_stream8(vbase + vrow[j] + d) : make_uint2(0, 0);
-            vr[j][q] = make_uint4(x.x, x.y, 0, 0);
-          } else {
-            vr[j][q] = vrow[j] >= 0 && d < D ? ld_stream16(vbase + vrow[j] + d) : make_uint4(0, 0, 0, 0);
-          }
-        }
-    };
-    int tile = t0 + warp, slot = 0;
-    if (tile < t_end) {
-      if (UB) look_up(tile + NW * lane);
-      find(tile, 0);
-      load_v();
-    }
-    for (; tile < t_end; tile += NW) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) { ks[j] = ks_n[j]; vs[j] = vs_n[j]; ok[j] = ok_n[j]; }
       float s[NR][4];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -342,26 +425,21 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
           for (int n = 0; n < NR; ++n)
 #pragma unroll
             for (int term = 0; term < T; ++term) {
-              uint2 bq;
-              if constexpr (NR == 1 && T == 1) bq = qreg[4 * q + i];
-              else bq = qfrag[((term * NR + n) * KS + 4 * q + i) * 32 + lane];
+              const uint2 bq = qfrag[((term * NR + n) * KS + 4 * q + i) * 32 + lane];
               mma16816<__half>(s[n], a0, a1, a2, a3, bq.x, bq.y);
             }
         }
       }
       // the next tile's keys, while this one's weights are formed
-      const int next = tile + NW;
+      const int next = tile + 1;
       if (next < t_end) {
         if (++slot == 32) {
           slot = 0;
-          if (UB) look_up(next + NW * lane);
+          if (UB) look_up(next + lane);
         }
         find(next, slot);
       }
 
-      const int key0 = tile * kTile;
-      // rows of which not all keys of the tile are seen, or keys that are not there
-      const bool edge = key0 + kTile > lim_least || __any_sync(0xffffffffu, !ok[0] || !ok[1]);
       uint32_t nan_keys = 0;   // keys of which a value is NaN: where rows do not see the key it must not reach them, so that it goes through the logit
       if (edge) {
 #pragma unroll
@@ -369,9 +447,12 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
           bool hit = false;
 #pragma unroll
           for (int q = 0; q < VC; ++q) {
-            hit = hit || any_nan(vr[j][q].x) || any_nan(vr[j][q].y) || any_nan(vr[j][q].z) || any_nan(vr[j][q].w);
+            hit = hit || any_nan(vr[j][q].x) || any_nan(vr[j][q].y);
             vr[j][q].x = without_nan(vr[j][q].x); vr[j][q].y = without_nan(vr[j][q].y);
-            vr[j][q].z = without_nan(vr[j][q].z); vr[j][q].w = without_nan(vr[j][q].w);
+            if (VB == 16) {
+              hit = hit || any_nan(vr[j][q].z) || any_nan(vr[j][q].w);
+              vr[j][q].z = without_nan(vr[j][q].z); vr[j][q].w = without_nan(vr[j][q].w);
+            }
           }
           const uint32_t who = __ballot_sync(0xffffffffu, hit);   // lanes (g, t): key 2t + (j & 1) + 8 (j >> 1)
 #pragma unroll
@@ -465,98 +546,171 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             }
           }
       }
-      if (next < t_end) load_v();
+      if (next < t_end) load_v(next * kTile);
     }
 
-    // ---- the warps' results meet in shared memory
+    // ---- a whole line is written, a part of one kept: of the line that began before this warp's share, and of the one that goes on
+    float sum[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l[n][e];
+        sum[n][e] = l[n][e];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (g == 0) wstat[warp][8 * n + 2 * t + e] = make_float2(m[n][e] - kLift, sum);
-        float* to = wacc + (warp * ROWS + 8 * n + 2 * t + e) * C::kPitch;
+        for (int o = 4; o < 32; o <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
+      }
+    const int part = t0 == 0 ? 1 : 0;
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + 2 * t + e;
+        if (r >= rows) continue;
+        const float f = whole ? (sum[n][e] == 0.f ? 0.f : vref / sum[n][e]) : vref;
+        const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+        const int64_t at = whole ? query_at(p, p.os, rw, b, h, i) : 0;
+        float* const to = wacc + ((warp * 2 + part) * ROWS + r) * C::kPitch;
+#pragma unroll
+        for (int j = 0; j < MT; j += 2) {
           const int d = DP == 256 ? 128 * (j / 8) + 16 * g + 2 * (j % 8) : VB * g + 2 * j;
-          *reinterpret_cast<float2*>(to + d) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+          const float4 o = make_float4(acc[n][j][e] * f, acc[n][j][e + 2] * f, acc[n][j + 1][e] * f, acc[n][j + 1][e + 2] * f);
+          if (!whole) *reinterpret_cast<float4*>(to + d) = o;
+          else if (d < D) store4(p, at + d, sp.out_vec, o);
+        }
+        if (g == 0) {
+          if (!whole) wstat[warp][part][r] = make_float2(m[n][e] - kLift, sum[n][e]);
+          else if (p.lse) *lse_at(p, rw, h, i) = sum[n][e] == 0.f ? -INFINITY : (m[n][e] - kLift + log2f(sum[n][e])) * kLn2;
         }
       }
-    if (lane == 0) wref[warp] = vref;
-    __syncthreads();
-
-    auto write = [&](int r, int d, float4 o, float top, float sum) {
-      const int i = (r0 + r) / G, h = kvh * G + (r0 + r) % G;
-      const float f = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = query_at(p, p.os, rw, b, h, i) + d;
-      const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (p.out_f32) static_cast<float*>(p.out)[at + e] = v[e];
-        else if (p.dtype == AIDN_F16) static_cast<__half*>(p.out)[at + e] = __float2half_rn(v[e]);
-        else static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(v[e]);
-      }
-      if (p.lse && d == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-    };
-    const int slot_out = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
-    for (int at = tid; at < rows * (DP / 4); at += NW * 32) {
-      const int r = at / (DP / 4), d = at % (DP / 4) * 4;
-      if (d >= D) continue;
-      float top = kUnset;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) top = fmaxf(top, wstat[w][r].x);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float2 st = wstat[w][r];
-        const float f = ex2_approx(st.x - top), fv = f * wref[w];
-        const float4 x = *reinterpret_cast<const float4*>(wacc + (w * ROWS + r) * C::kPitch + d);
-        sum += f * st.y;
-        o.x += fv * x.x; o.y += fv * x.y; o.z += fv * x.z; o.w += fv * x.w;
-      }
-      if (whole) {
-        write(r, d, o, top, sum);
-      } else {
-        __stcg(reinterpret_cast<float4*>(sp.partial + ((int64_t)slot_out * ROWS + r) * DP + d), o);
-        if (d == 0) __stcg(sp.stats + (int64_t)slot_out * ROWS + r, make_float2(top, sum));
-      }
+    if (!whole && lane == 0) {
+      wline[warp][part] = line_pos;
+      winfo[warp][part][0] = b;
+      winfo[warp][part][1] = off;
+      winfo[warp][part][2] = tiles;
     }
-    if (!whole) {
-      // CTAs first .. first + parts - 1 have a part of the line; where it begins it is the CTA's last, elsewhere its first
-      const int first = (int)(line_pos / share), parts = (int)((line_pos + tiles - 1) / share) - first + 1;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) last_flag = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
-      __syncthreads();
-      if (last_flag) {
-        __threadfence();
-        for (int at = tid; at < rows * (DP / 4); at += NW * 32) {
-          const int r = at / (DP / 4), d = at % (DP / 4) * 4;
-          if (d >= D) continue;
-          float top = kUnset;
-#pragma unroll 8
-          for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(sp.stats + (int64_t)(2 * (first + q) + (q == 0)) * ROWS + r).x);
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float sum = 0.f;
-#pragma unroll 8
-          for (int q = 0; q < parts; ++q) {
-            const int64_t from = (int64_t)(2 * (first + q) + (q == 0)) * ROWS + r;
-            const float2 st = __ldcg(sp.stats + from);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(sp.partial + from * DP + d));
-            const float f = ex2_approx(st.x - top);
-            sum += f * st.y;
-            o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
-          }
-          write(r, d, o, top, sum);
-        }
-      }
-    }
-    __syncthreads();   // (shared memory is filled again)
+    __syncwarp();
   }
   if (bad && p.status) atomicOr(p.status, kStatusBadBlock);
+  __syncthreads();
+
+  // ---- the parts of a line in this CTA are consecutive: merged by all threads, and written, or left in the workspace
+  auto finish = [&](const Rows& rw, int b, int off, int r, int d, float4 o, float top, float sum) {
+    const int kvh = p.kv_begin + off % p.kv_count, r0 = off / p.kv_count * ROWS;
+    const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    store4(p, query_at(p, p.os, rw, b, h, i) + d, sp.out_vec, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    if (p.lse && d == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  };
+  int64_t handed0 = -1, handed1 = -1;   // lines of which other CTAs have parts too: the one that began before, the one that goes on
+  int at0 = 0, at1 = 0;
+  unsigned used = 0;   // slots that hold a part
+#pragma unroll
+  for (int q = 0; q < 2 * NW; ++q) used |= (unsigned)(wline[q >> 1][q & 1] >= 0) << q;
+  while (used) {
+    const int at = __ffs(used) - 1;
+    const int64_t line = wline[at >> 1][at & 1];
+    unsigned group = 0;
+    for (unsigned left = used; left; left &= left - 1) {
+      const int q = __ffs(left) - 1;
+      if (wline[q >> 1][q & 1] != line) break;
+      group |= 1u << q;
+    }
+    used &= ~group;
+    const int b = winfo[at >> 1][at & 1][0], off = winfo[at >> 1][at & 1][1], tiles = winfo[at >> 1][at & 1][2];
+    const Rows rw = rows_of(p, b);
+    const int rows = min(ROWS, rw.count * G - off / p.kv_count * ROWS);
+    const bool early = line < cta_pos, late = line + tiles > cta_end, whole = !early && !late;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (early ? 0 : 1);
+    for (int x = tid; x < rows * (DP / 4); x += NW * 32) {
+      const int r = x / (DP / 4), d = x % (DP / 4) * 4;
+      if (d >= D) continue;
+      float top = kUnset;
+      for (unsigned left = group; left; left &= left - 1) top = fmaxf(top, (&wstat[0][0][0])[(__ffs(left) - 1) * ROWS + r].x);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+      for (unsigned left = group; left; left &= left - 1) {
+        const int q = __ffs(left) - 1;
+        const float2 st = (&wstat[0][0][0])[q * ROWS + r];
+        const float f = ex2_approx(st.x - top);
+        const float4 v = *reinterpret_cast<const float4*>(wacc + (q * ROWS + r) * C::kPitch + d);
+        sum += f * st.y;
+        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+      }
+      if (whole) {
+        finish(rw, b, off, r, d, o, top, sum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(sp.partial + (slot * ROWS + r) * DP + d), o);
+        if (d == 0) __stcg(sp.stats + slot * ROWS + r, make_float2(top, sum));
+      }
+    }
+    if (early) {
+      handed0 = line;
+      at0 = at;
+    } else if (late) {
+      handed1 = line;
+      at1 = at;
+    }
+  }
+  if (handed0 < 0 && handed1 < 0) return;
+  // CTAs first .. first + parts - 1 have a part of such a line; in the CTA where it begins it is the last one, elsewhere the first
+  const int64_t cta_share = share * NW;
+  __syncthreads();
+  if (tid < 2) {
+    const int64_t line = tid ? handed1 : handed0;
+    bool last = false;
+    if (line >= 0) {
+      const int at = tid ? at1 : at0, first = tid ? (int)blockIdx.x : (int)(line / cta_share);
+      const int parts = (int)((line + winfo[at >> 1][at & 1][2] - 1) / cta_share) - first + 1;
+      __threadfence();   // (what the other threads wrote, too: the barrier lies between)
+      last = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
+      __threadfence();
+    }
+    last_flag[tid] = last;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if (!last_flag[k]) continue;
+    const int64_t line = k ? handed1 : handed0;
+    const int at = k ? at1 : at0;
+    const int* info = winfo[at >> 1][at & 1];
+    const int b = info[0], off = info[1], tiles = info[2];
+    const int first = k ? (int)blockIdx.x : (int)(line / cta_share), parts = (int)((line + tiles - 1) / cta_share) - first + 1;
+    const Rows rw = rows_of(p, b);
+    const int rows = min(ROWS, rw.count * G - off / p.kv_count * ROWS);
+    for (int x = tid; x < rows * (DP / 4); x += NW * 32) {
+      const int r = x / (DP / 4), d = x % (DP / 4) * 4;
+      if (d >= D) continue;
+      float top = kUnset, sum = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < parts; q += 8) {
+        float2 st[8];
+        float4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int part = min(q + u, parts - 1);
+          const int64_t from = (int64_t)(2 * (first + part) + (part == 0)) * ROWS + r;
+          st[u] = __ldcg(sp.stats + from);
+          v[u] = __ldcg(reinterpret_cast<const float4*>(sp.partial + from * DP + d));
+        }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) now = fmaxf(now, st[u].x);
+        const float keep = ex2_approx(top - now);
+        top = now;
+        sum *= keep;
+        o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (q + u >= parts) continue;
+          const float f = ex2_approx(st[u].x - top);
+          sum += f * st[u].y;
+          o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
+        }
+      }
+      finish(rw, b, off, r, d, o, top, sum);
+    }
+  }
 }
 
 template <int DP, int NR, int T, bool UB>
@@ -586,7 +740,7 @@ cudaError_t one(const Attend* p, int num_sms, void* workspace, int64_t* bytes, u
     return cudaSuccess;
   }
   auto k = kv8_split_kernel<DP, NR, T, UB>;
-  const int id = ((DP == 64 ? 0 : DP == 128 ? 1 : 2) * 3 + (NR == 1 ? 0 : NR == 2 ? 1 : 2)) * 4 + (T - 1) * 2 + (UB ? 1 : 0);
+  const int id = ((DP == 64 ? 0 : DP == 128 ? 1 : 2) * 2 + NR - 1) * 4 + (T - 1) * 2 + (UB ? 1 : 0);
   if (!(*raised >> id & 1)) {   // once a handle: the limit belongs to the context
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
     if (e != cudaSuccess) return e;
@@ -595,7 +749,12 @@ cudaError_t one(const Attend* p, int num_sms, void* workspace, int64_t* bytes, u
   Split sp;
   sp.partial = static_cast<float*>(workspace);
   sp.stats = workspace ? reinterpret_cast<float2*>(static_cast<char*>(workspace) + acc) : nullptr;
-  sp.least = 2 * C::kWarps;
+  sp.least = 2;
+  auto vec = [](const void* ptr, const int64_t* st, int esz, int bytes) {
+    return ((uintptr_t)ptr | (uint64_t)(st[0] * esz) | (uint64_t)(st[1] * esz) | (uint64_t)(st[2] * esz)) % bytes == 0;
+  };
+  sp.query_vec = vec(p->q, p->qs, p->dtype == AIDN_F32 ? 4 : 2, 16);
+  sp.out_vec = vec(p->out, p->os, p->out_f32 ? 4 : 2, p->out_f32 ? 16 : 8);
   return launch_dependent(k, dim3((unsigned)grid), C::kWarps * 32, C::kSmem, stream, *p, sp);
 }
 
@@ -606,9 +765,7 @@ cudaError_t pick_block(bool ub, const Attend* p, int num_sms, void* workspace, i
 template <int DP, int T>
 cudaError_t pick_rows(int64_t rows, bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
   if (rows <= 8) return pick_block<DP, 1, T>(ub, p, num_sms, workspace, bytes, raised, stream);
-  if (rows <= 16 || DP == 256) return pick_block<DP, 2, T>(ub, p, num_sms, workspace, bytes, raised, stream);
-  if constexpr (DP < 256) return pick_block<DP, 4, T>(ub, p, num_sms, workspace, bytes, raised, stream);
-  return cudaErrorInvalidValue;
+  return pick_block<DP, 2, T>(ub, p, num_sms, workspace, bytes, raised, stream);
 }
 template <int DP>
 cudaError_t pick(bool exact, int64_t rows, bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
