@@ -338,7 +338,7 @@ int aidn_sdpa_poll(aidn_sdpa_t h, void* cu_stream) {
   e = cudaMemcpy(&st, h->status_dev, sizeof(st), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return fail_cuda(e, "poll: status read");
   if (st != 0) {
-    cudaMemset(h->status_dev, 0, 4 * sizeof(int32_t));
+    cudaMemset(h->status_dev, 0, kHandleWords * sizeof(int32_t));   // (a launch that gave up leaves counters)
     if (st & aidn::kStatusTimeout)
       return fail(AIDN_ETIMEOUT, "poll: a kernel gave up a bounded wait (status word 0x%x)", st);
     return fail(AIDN_EINVAL, "poll: a block-table entry outside [0, num_blocks) was skipped (status word 0x%x)", st);
@@ -902,7 +902,10 @@ int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_
     return -1;
   }
   if (h->d.path == AIDN_PATH_GENERIC || h->d.mask_kind != AIDN_MASK_NONE || h->d.head_dim % 16 != 0) return 0;
-  return align_up(aidn::kv8::split_workspace_bytes(h->d.head_dim, h->d.out_dtype == AIDN_F32, seq_q * h->group, h->num_sms), 256);
+  const int64_t few = aidn::kv8::split_workspace_bytes(h->d.head_dim, h->d.out_dtype == AIDN_F32, seq_q * h->group, h->num_sms);
+  const int64_t many = seq_q * h->group > aidn::kv8::kFewRows && h->d.out_dtype != AIDN_F32 && (h->d.head_dim == 64 || h->d.head_dim == 128)
+                           ? aidn::kv8::sm100_workspace_bytes(h->d.head_dim, h->num_sms) : 0;
+  return align_up(few > many ? few : many, 256);
 }
 
 int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_cache* cache, const int32_t* query_starts,
@@ -968,7 +971,10 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   cudaStream_t stream = (cudaStream_t)cu_stream;
   int launches = 1;
   cudaError_t e;
-  if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
+  if (d.path != AIDN_PATH_GENERIC && p.seq_q * p.group > aidn::kv8::kFewRows && aidn::kv8::sm100_supported(p)) {
+    e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);
+    h->last_path = AIDN_PATH_PREFILL_SM100;
+  } else if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
     e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);
     h->last_path = AIDN_PATH_DECODE;
   } else {

@@ -1,0 +1,784 @@
+// Attention of many queries over a paged pool held in 8 bits (kv8.cuh) on tcgen05: prompt chunks, ragged batches, drafted tokens.
+//
+//   x = (Q K^T) c_r k_scale(block)      (base 2; c_r = scale log2(e) / the query's own factor)
+//   P = 2^(x - m + e - e_ref + lift),   e = log2(v_scale(block)),   O += P V,   l += 2^(x - m)
+//   o = O 2^(e_ref - lift) / l
+//
+// A line is (sequence, KV head, pair of 128-row tiles); a row is a (query, query head of the group), so that a few queries of a
+// group fill a tile as well as many of one head.  4 D operations a (row, key): bound by the tensor cores for two full tiles, and by the
+// pool's bytes where a line has few rows.  Codes become fp16 on the way into shared memory, exactly; the scales of the blocks touch
+// sixteen scores at a time, as a factor of the logits and an offset of the exponents, so that they cost nothing per score, and
+// queries are scaled by a power of two into fp16 (bf16 and fp16 queries lose nothing that their largest element leaves visible).
+// Weights are fp16, 11 bits, lifted so that they stay normal down to 2^-18 of the largest.
+//
+//   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
+//                     (16 bits), the running maximum (the accumulator is scaled again only when a logit is 2^8 above it), results
+//   warps 8-11        keys: 16-byte loads through the block table, codes to fp16, into a ring of two 128-key tiles
+//   warps 12-15       values, the same
+//   warp 16           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V; while the softmax works on one tile's scores the other's are formed
+//
+// Tensor memory: S_0 | S_1 (128 columns each, P in the first 64), O_0 | O_1.  The tiles of all lines are one row that is cut into
+// equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice); parts of cut lines meet in the
+// workspace as in kv8_split.cu, merged by the CTA that arrives last.
+#include "kv8.cuh"
+#include "sm100_ptx.cuh"
+
+namespace aidn {
+namespace kv8 {
+namespace {
+
+using namespace ptx;
+
+constexpr int kKeys = 128;            // keys of a tile
+constexpr int kTileRows = 128;
+constexpr int kPairRows = 2 * kTileRows;
+constexpr int kThreads = 640;
+constexpr int kKeyWarp = 8, kValueWarp = 12, kMmaWarp = 16;
+constexpr int kSoftmaxRegs = 144, kConvertRegs = 64, kMmaRegs = 56;
+// setmaxnreg.inc waits without a bound for registers that are not there: the shares must not exceed what the CTA is launched with
+static_assert(256 * kSoftmaxRegs + 256 * kConvertRegs + 128 * kMmaRegs <= kThreads * 96, "registers of the launch");
+constexpr int kRing = 4;              // tiles whose scales are kept
+constexpr float kUnset = -1e30f;
+constexpr float kLazy = 8.f, kRefSlack = 3.f, kLift = 4.f;   // 2^(8 + 3 + 4) is in fp16's range
+
+template <int HD>
+struct Cfg {
+  static constexpr int kSlab = kKeys * 128;              // 64 elements of 128 rows, 128-byte swizzle
+  static constexpr int kTile = kSlab * (HD / 64);        // a query, key or value tile in fp16
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
+  static constexpr int kMisc = 6 * kTile;
+  static constexpr int kSmem = kMisc + 2048 + 1024 /* alignment */;
+  static constexpr uint32_t kO = 256;                    // accumulators' first column
+};
+// barriers: q_full[2] k_full[2] k_empty[2] v_full[2] v_empty[2] s_full[2] p_full[2] o_full[2] scales[kRing]
+enum { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kOFull = 14, kScales = 16, kBars = 16 + kRing };
+
+struct Misc {
+  uint64_t bars[kBars];
+  uint32_t tmem;
+  int abort;
+  float k_scale[kRing][8], v_exp[kRing][8];   // of a tile's groups of sixteen keys; v_exp -inf: no such keys
+  uint32_t nan_keys[kRing][4];                // keys with a NaN among their values, in tiles of which rows do not see all
+  int64_t scan[kThreads / 32];
+  int64_t start_base;
+  int start_b, start_u;
+  int last[2];
+};
+static_assert(sizeof(Misc) <= 2048, "");
+
+struct Cut {
+  float* partial;   // [2 grid][256][HD], or null: lines are not cut
+  float2* stats;    // [2 grid][256]: maximum and sum
+  bool query_vec, out_vec;
+};
+
+// The lines of this CTA's share, in order; every role walks them by itself.
+struct Walk {
+  const Attend* p;
+  int64_t pos, end, share, base;   // base: position of the line's first tile
+  bool cut;
+  int b, u, kvh;
+  Rows rw;
+  int keys, pairs;
+  // the line
+  int rows, cost, tiles, t0, t1;
+  bool whole;
+
+  __device__ __forceinline__ void sequence() {
+    rw = rows_of(*p, b);
+    keys = keys_of(*p, b);
+    pairs = (rw.count * p->group + kPairRows - 1) / kPairRows;
+  }
+  __device__ __forceinline__ void line() {
+    const int left = rw.count * p->group - u * kPairRows;
+    rows = left < kPairRows ? left : kPairRows;
+    cost = rows > kTileRows ? 2 : 1;
+    tiles = tiles_of(*p, rw.count, keys, u);
+  }
+  static __device__ __forceinline__ int tiles_of(const Attend& p, int n, int keys, int u) {
+    const int last = min(n * p.group, (u + 1) * kPairRows) - 1;
+    const int end = visible(p, keys, n, last / p.group);
+    return end > kKeys ? (end + kKeys - 1) / kKeys : 1;
+  }
+  // On to the next line that this CTA has tiles of; false at the end.
+  __device__ __forceinline__ bool next(bool first) {
+    for (;;) {
+      if (!first) {
+        base += (int64_t)tiles * cost;
+        if (++kvh == p->kv_count) {
+          kvh = 0;
+          if (++u == pairs) {
+            u = 0;
+            do {
+              if (++b >= p->batch || base >= end) return false;
+              sequence();
+            } while (pairs == 0);
+          }
+          line();
+        }
+      }
+      first = false;
+      if (base >= end) return false;
+      if (cut) {
+        t0 = pos > base ? (int)((pos - base + cost - 1) / cost) : 0;
+        const int64_t most = (end - base + cost - 1) / cost;
+        t1 = most < tiles ? (int)most : tiles;
+        if (t0 >= t1) continue;
+        whole = t0 == 0 && t1 == tiles;
+      } else {
+        if (base < pos) continue;   // a line belongs to the share that it begins in
+        t0 = 0;
+        t1 = tiles;
+        whole = true;
+      }
+      return true;
+    }
+  }
+};
+
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float cap(float x, float softcap, float inverse) {   // tanh to 3e-7 of 1
+  const float y = fminf(x * (2.f * kLog2e) * inverse, 80.f);
+  return softcap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2_approx(y)));
+}
+__device__ __forceinline__ bool any_nan(uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+__device__ __forceinline__ uint32_t without_nan(uint32_t x) {
+  const uint32_t hit = (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return x & ~(hit * 0xffu);
+}
+// Eight 16-bit elements at `at`, as floats.
+__device__ __forceinline__ void query8(const Attend& p, int64_t at, bool vec, float* x) {
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+  uint32_t w[4];
+  if (vec) {
+    const uint4 v = *reinterpret_cast<const uint4*>(q);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t v = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+    x[e] = p.dtype == AIDN_F16 ? __half2float(__ushort_as_half((unsigned short)v)) : __uint_as_float(v << 16);
+  }
+}
+__device__ __forceinline__ void store8(const Attend& p, int64_t at, bool vec, const float* x) {
+  uint16_t* to = static_cast<uint16_t*>(p.out) + at;
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = p.dtype == AIDN_F16 ? pack2<false>(x[2 * e], x[2 * e + 1]) : pack2<true>(x[2 * e], x[2 * e + 1]);
+  if (vec) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      to[2 * e] = (uint16_t)w[e];
+      to[2 * e + 1] = (uint16_t)(w[e] >> 16);
+    }
+  }
+}
+
+template <int HD, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_constant__ Attend p, const Cut cut) {
+  using C = Cfg<HD>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  Misc& ms = *reinterpret_cast<Misc*>(smem + C::kMisc);
+  volatile int* const abort_flag = &ms.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
+  const uint32_t base = smem_u32(smem);
+  auto bar = [&](int i) { return smem_u32(&ms.bars[i]); };
+  if (tid == 0) {
+    ms.abort = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kQFull + i), 4);
+      mbar_init(bar(kKFull + i), 4);
+      mbar_init(bar(kKEmpty + i), 1);
+      mbar_init(bar(kVFull + i), 4);
+      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kSFull + i), 1);
+      mbar_init(bar(kPFull + i), 4);
+      mbar_init(bar(kOFull + i), 1);
+    }
+    for (int i = 0; i < kRing; ++i) mbar_init(bar(kScales + i), 8);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&ms.tmem), 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- shares: a thread sums up the lines of some sequences, or of some row pairs of one; their prefix gives where a share begins
+  const bool is_cut = cut.partial != nullptr;
+  const int spread = p.batch < kThreads ? kThreads / p.batch : 1, per = (p.batch + kThreads - 1) / kThreads;   // threads a sequence, sequences a thread
+  const int b_lo = spread > 1 ? min(tid / spread, p.batch) : min(tid * per, p.batch);
+  const int b_hi = spread > 1 ? min(b_lo + 1, p.batch) : min(b_lo + per, p.batch);
+  auto pairs_of = [&](int n, int* lo, int* hi) {   // this thread's row pairs of a sequence of n queries
+    const int pairs = (n * G + kPairRows - 1) / kPairRows, each = (pairs + spread - 1) / spread;
+    *lo = spread > 1 ? min((tid % spread) * each, pairs) : 0;
+    *hi = spread > 1 ? min(*lo + each, pairs) : pairs;
+  };
+  auto weight = [&](int n, int keys, int u) {
+    return (int64_t)Walk::tiles_of(p, n, keys, u) * p.kv_count * (n * G - u * kPairRows > kTileRows ? 2 : 1);
+  };
+  int64_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int n = rows_of(p, b).count, keys = keys_of(p, b);
+    int lo, hi;
+    pairs_of(n, &lo, &hi);
+    for (int u = lo; u < hi; ++u) mine += weight(n, keys, u);
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) ms.scan[warp] = upto;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w == warp) before = total;
+    total += ms.scan[w];
+  }
+  before += upto - mine;
+  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  if (share < 4) share = 4;
+  const int64_t pos = blockIdx.x * share, end = min(pos + share, total);
+  const uint32_t tmem = ms.tmem;
+  if (pos < end && pos >= before && pos < before + mine) {
+    int64_t at = before;
+    bool found = false;
+    for (int b = b_lo; b < b_hi && !found; ++b) {
+      const int n = rows_of(p, b).count, keys = keys_of(p, b);
+      int lo, hi;
+      pairs_of(n, &lo, &hi);
+      for (int u = lo; u < hi; ++u) {
+        const int64_t w = weight(n, keys, u);
+        if (pos < at + w) {
+          ms.start_b = b;
+          ms.start_u = u;
+          ms.start_base = at;
+          found = true;
+          break;
+        }
+        at += w;
+      }
+    }
+  }
+  __syncthreads();
+
+  auto walk = [&]() {   // at the first line; the head within the pair is the quotient
+    Walk w;
+    w.p = &p;
+    w.pos = pos;
+    w.end = end;
+    w.share = share;
+    w.cut = is_cut;
+    w.b = ms.start_b;
+    w.u = ms.start_u;
+    w.sequence();
+    w.line();
+    const int64_t a_line = (int64_t)w.tiles * w.cost;
+    w.kvh = (int)((pos - ms.start_base) / a_line);
+    w.base = ms.start_base + w.kvh * a_line;
+    return w;
+  };
+  bool alive = pos < end;
+  bool bad = false;
+
+  if (warp < kKeyWarp) {
+    // ================================================= softmax =================================================
+    setmaxnreg_inc<kSoftmaxRegs>();
+    const int a = warp >> 2, row_in = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + (uint32_t)(a * 128), to = tmem + lanes + C::kO + (uint32_t)(a * HD);
+    uint32_t q_uses = 0, s_uses = 0;
+    uint32_t tile_count = 0;   // of this CTA, for the scales' ring
+    if (alive) {
+      Walk w = walk();
+      for (bool first = true; alive && w.next(first); first = false) {
+        const int n_tiles = w.t1 - w.t0;
+        if (a == 1 && w.rows <= kTileRows) {   // (tile 1 has no rows: not taken part in)
+          tile_count += n_tiles;
+          continue;
+        }
+        const int r = w.u * kPairRows + a * kTileRows + row_in;
+        const bool valid = a * kTileRows + row_in < w.rows;
+        const int i = valid ? r / G : 0, h = (p.kv_begin + w.kvh) * G + (valid ? r - i * G : 0);
+        // ---- this row's query: scaled by a power of two so that the largest element is in [2^8, 2^9)
+        float c;
+        {
+          const int64_t at = query_at(p, p.qs, w.rw, w.b, h, i);
+          float largest = 0.f;
+          if (valid) {
+#pragma unroll 4
+            for (int j = 0; j < HD / 8; ++j) {
+              float x[8];
+              query8(p, at + 8 * j, cut.query_vec, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[e]));
+            }
+          }
+          int up = 8 - ((int)(__float_as_uint(largest) >> 23) - 127);
+          up = max(-110, min(up, 126));
+          const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+          c = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (CAP ? 1.f : kLog2e);
+          const uint32_t dst = base + C::kQ + a * C::kTile + row_in * 128;
+#pragma unroll 4
+          for (int j = 0; j < HD / 8; ++j) {
+            float x[8] = {};
+            if (valid) query8(p, at + 8 * j, cut.query_vec, x);
+            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), pack2<false>(x[0] * f, x[1] * f), pack2<false>(x[2] * f, x[3] * f),
+                         pack2<false>(x[4] * f, x[5] * f), pack2<false>(x[6] * f, x[7] * f));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQFull + a));
+        ++q_uses;
+        const int lim = valid ? visible(p, w.keys, w.rw.count, i) : 0x7fffffff;
+        const int lim_least = visible(p, w.keys, w.rw.count, (w.u * kPairRows + a * kTileRows) / G);
+        const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
+        float m = kUnset, l = 0.f, eref = -INFINITY;
+
+        for (int t = w.t0; t < w.t1 && alive; ++t, ++tile_count) {
+          const uint32_t ring = tile_count % kRing;
+          // (in this order: once a tile's scores are there, its scales are the next that the ring's slot waits for)
+          if (!mbar_wait(bar(kSFull + a), s_uses & 1, abort_flag) || !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
+            alive = false;
+            break;
+          }
+          ++s_uses;
+          tc_fence_after();
+          const int key0 = t * kKeys;
+          const bool edge = key0 + kKeys > lim_least || key0 + kKeys > w.keys;   // (uniform)
+          const float* ksc = ms.k_scale[ring];
+          const float* vex = ms.v_exp[ring];
+          uint32_t s[2][32];
+          // the score of column k: what a row does not see is -inf, a key with a NaN among its values NaN
+          auto mask = [&](uint32_t* x, int col0) {
+            const uint32_t nan = ms.nan_keys[ring][col0 >> 5];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (nan >> e & 1) x[e] = 0x7fffffffu;
+              if (key0 + col0 + e >= lim) x[e] = 0xff800000u;
+            }
+          };
+          // ---- the maximum
+          float top = kUnset;
+          tmem_ld32(ts, s[0]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tc_wait_ld();
+            if (q < 3) tmem_ld32(ts + 32 * (q + 1), s[(q + 1) & 1]);
+            uint32_t* x = s[q & 1];
+            if (edge) mask(x, 32 * q);
+#pragma unroll
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              float mx = __uint_as_float(x[16 * hlf]);
+#pragma unroll
+              for (int e = 1; e < 15; e += 2) mx = fmax3(mx, __uint_as_float(x[16 * hlf + e]), __uint_as_float(x[16 * hlf + e + 1]));
+              mx = fmaxf(mx, __uint_as_float(x[16 * hlf + 15]));
+              const int g = 2 * q + hlf;
+              if (vex[g] != -INFINITY && mx != -INFINITY) {
+                mx *= c * ksc[g];
+                top = fmaxf(top, CAP ? cap(mx, p.softcap, cap_inverse) : mx);
+              }
+            }
+          }
+          float emax = vex[0];
+#pragma unroll
+          for (int g = 1; g < 8; ++g) emax = fmaxf(emax, vex[g]);
+          float keep = 1.f;
+          if (top > m + kLazy) {
+            const float f = ex2_approx(m - top);
+            keep = f;
+            l *= f;
+            m = top;
+          }
+          if (emax > eref + kRefSlack) {
+            keep *= eref == -INFINITY ? 0.f : ex2_approx(eref - emax);
+            eref = emax;
+          }
+          if (t > w.t0 && __any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll
+            for (int q = 0; q < HD / 32; ++q) {
+              tmem_ld32(to + 32 * q, s[0]);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * keep);
+              tmem_st32(to + 32 * q, s[0]);
+            }
+            tc_wait_st();
+          }
+          // ---- weights
+          tmem_ld32(ts, s[0]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tc_wait_ld();
+            if (q < 3) tmem_ld32(ts + 32 * (q + 1), s[(q + 1) & 1]);
+            uint32_t* x = s[q & 1];
+            if (edge) mask(x, 32 * q);
+            uint32_t packed[16];
+#pragma unroll
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              const int g = 2 * q + hlf;
+              const float cg = c * ksc[g], e = vex[g], off = e == -INFINITY ? -INFINITY : e - eref - m + kLift;
+              float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                float u = __uint_as_float(x[16 * hlf + k]), v = __uint_as_float(x[16 * hlf + k + 1]);
+                if (CAP) {
+                  // (a masked score stays -inf, whatever the cap makes of it)
+                  u = u == -INFINITY ? u : cap(u * cg, p.softcap, cap_inverse);
+                  v = v == -INFINITY ? v : cap(v * cg, p.softcap, cap_inverse);
+                  u = ex2_approx(u + off);
+                  v = ex2_approx(v + off);
+                } else if (edge) {
+                  u = u == -INFINITY ? 0.f : ex2_approx(fmaf(u, cg, off));   // (a scale of zero times -inf)
+                  v = v == -INFINITY ? 0.f : ex2_approx(fmaf(v, cg, off));
+                } else {
+                  u = ex2_approx(fmaf(u, cg, off));
+                  v = ex2_approx(fmaf(v, cg, off));
+                }
+                sum0 += u;
+                sum1 += v;
+                packed[8 * hlf + (k >> 1)] = pack2<false>(u, v);
+              }
+              if (e != -INFINITY) l = fmaf(sum0 + sum1, ex2_approx(eref - e - kLift), l);
+            }
+            tmem_st16(ts + 16 * q, packed);
+          }
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kPFull + a));
+        }
+        if (!alive) break;
+        // ---- results
+        if (!mbar_wait(bar(kOFull + a), (q_uses - 1) & 1, abort_flag)) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+        const float unit = eref == -INFINITY ? 0.f : ex2_approx(eref - kLift);
+        const float f = w.whole ? (l == 0.f ? 0.f : unit / l) : unit;
+        const int slot = 2 * (int)blockIdx.x + (w.t0 == 0 ? 1 : 0), prow = a * kTileRows + row_in;
+        const int64_t at = w.whole ? query_at(p, p.os, w.rw, w.b, h, i) : ((int64_t)slot * kPairRows + prow) * HD;
+#pragma unroll
+        for (int q = 0; q < HD / 32; ++q) {
+          uint32_t x[32];
+          tmem_ld32(to + 32 * q, x);
+          tc_wait_ld();
+          float y[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(x[e]) * f;
+          if (valid && w.whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) store8(p, at + 32 * q + e, cut.out_vec, y + e);
+          } else if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) __stcg(reinterpret_cast<float4*>(cut.partial + at + 32 * q + e), make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]));
+          }
+        }
+        if (valid && w.whole && p.lse) *lse_at(p, w.rw, h, i) = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (valid && !w.whole) __stcg(cut.stats + (int64_t)slot * kPairRows + prow, make_float2(m, l));
+        tc_fence_before();   // (the next line's products come behind this warp's next arrival)
+      }
+    }
+  } else if (warp < kMmaWarp) {
+    // ======================================= keys and values: codes to fp16 =======================================
+    setmaxnreg_dec<kConvertRegs>();
+    const bool is_key = warp < kValueWarp;
+    const int quarter = warp & 3, t4 = lane & 3, g8 = lane >> 2;   // this warp: keys 32 quarter .. + 31; a lane: row g8 (+ 8 i), 16 bytes t4
+    constexpr int H = HD / 64;
+    const int64_t pitch = p.c.stride[1];
+    const int full = is_key ? kKFull : kVFull, empty = is_key ? kKEmpty : kVEmpty;
+    const uint32_t dst0 = base + (is_key ? C::kK : C::kV) + (uint32_t)((32 * quarter + g8) * 128);
+    uint32_t count = 0;
+    if (alive) {
+      Walk w = walk();
+      for (bool first = true; alive && w.next(first); first = false) {
+        const int kvh = p.kv_begin + w.kvh;
+        const uint8_t* const src = (is_key ? p.c.k : p.c.v) + kvh * p.c.stride[2] + 16 * t4;
+        const float* const scales = is_key ? p.c.k_scale : p.c.v_scale;
+        const int32_t* const table = p.c.table + w.b * p.c.table_stride;
+        // lane e of this: the block of keys 32 quarter + 16 (e & 1) .. of a tile
+        auto entry_of = [&](int t) {
+          const int key = t * kKeys + 32 * quarter + 16 * (lane & 1);
+          return t < w.t1 && key < w.keys ? checked_block(p.c, table[block_of(p.c, key)], bad) : -1;
+        };
+        uint4 x[4][H];
+        float scale;
+        int entry = entry_of(w.t0), entry_n;
+        auto load = [&](int t) {
+          const int key0 = t * kKeys + 32 * quarter;
+          scale = entry >= 0 ? scales[(int64_t)entry * p.c.kv_heads + kvh] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ent = __shfl_sync(0xffffffffu, entry, i >> 1), key = key0 + 16 * (i >> 1);
+            const int in_block = key - block_of(p.c, key) * p.c.block_size + 8 * (i & 1) + g8;
+            const bool there = ent >= 0 && key0 + 8 * i + g8 < w.keys;
+            const uint8_t* at = src + ent * p.c.stride[0] + in_block * pitch;
+#pragma unroll
+            for (int q = 0; q < H; ++q) x[i][q] = there ? ld_stream16(at + 64 * q) : make_uint4(0, 0, 0, 0);
+          }
+        };
+        const int lim_least = visible(p, w.keys, w.rw.count, w.u * kPairRows / G);
+        load(w.t0);
+        entry_n = entry_of(w.t0 + 1);
+        for (int t = w.t0; t < w.t1; ++t, ++count) {
+          const uint32_t stage = count & 1, ring = count % kRing;
+          if (!mbar_wait(bar(empty + stage), (count >> 1 & 1) ^ 1, abort_flag)) {
+            alive = false;
+            break;
+          }
+          uint32_t nan = 0;
+          if (!is_key && t * kKeys + kKeys > lim_least) {   // NaN values of keys that some rows do not see
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              bool hit = false;
+#pragma unroll
+              for (int q = 0; q < H; ++q) {
+                hit = hit || any_nan(x[i][q].x) || any_nan(x[i][q].y) || any_nan(x[i][q].z) || any_nan(x[i][q].w);
+                x[i][q].x = without_nan(x[i][q].x); x[i][q].y = without_nan(x[i][q].y);
+                x[i][q].z = without_nan(x[i][q].z); x[i][q].w = without_nan(x[i][q].w);
+              }
+              const uint32_t who = __ballot_sync(0xffffffffu, hit);
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                if (who >> (4 * r) & 15) nan |= 1u << (8 * i + r);
+            }
+          }
+          if (lane < 2) {
+            const int g = 2 * quarter + lane;
+            float exponent = log2_approx(scale);
+            if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
+            if (entry < 0) exponent = -INFINITY;
+            if (is_key) ms.k_scale[ring][g] = scale;
+            else ms.v_exp[ring][g] = exponent;
+          }
+          if (!is_key && lane == 0) ms.nan_keys[ring][quarter] = nan;
+          const uint32_t dst = dst0 + stage * C::kTile;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int q = 0; q < H; ++q) {
+              const uint4 v = x[i][q];
+              const uint32_t at = dst + i * 1024 + q * C::kSlab;   // 16 elements: chunks 2 t4 and 2 t4 + 1 of the row's eight
+              st_shared_v4(at + (((2 * t4) ^ g8) << 4), codes_to_f16(v.x), codes_to_f16_hi(v.x), codes_to_f16(v.y), codes_to_f16_hi(v.y));
+              st_shared_v4(at + (((2 * t4 + 1) ^ g8) << 4), codes_to_f16(v.z), codes_to_f16_hi(v.z), codes_to_f16(v.w), codes_to_f16_hi(v.w));
+            }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar(full + stage));
+            mbar_arrive(bar(kScales + ring));
+          }
+          if (t + 1 < w.t1) {
+            entry = entry_n;
+            load(t + 1);
+            entry_n = entry_of(t + 2);
+          }
+        }
+      }
+    }
+  } else {
+    // ================================================ products ================================================
+    setmaxnreg_dec<kMmaRegs>();
+    if (warp == kMmaWarp && alive) {
+      const bool leader = elect_one();
+      constexpr uint32_t idesc_s = make_idesc(kTileRows, kKeys, false, false), idesc_o = make_idesc(kTileRows, HD, false, true);
+      const uint64_t qd = make_smem_desc(base + C::kQ, 16, 1024), kd = make_smem_desc(base + C::kK, 16, 1024);
+      const uint64_t vd = make_smem_desc(base + C::kV, C::kSlab, 1024);
+      uint32_t count = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+      auto scores = [&](int a, uint32_t stage) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint64_t off = (uint64_t)((k >> 2) * (C::kSlab >> 4) + (k & 3) * 2);
+          if (leader) mma_ss(tmem + a * 128, qd + (uint64_t)(a * (C::kTile >> 4)) + off, kd + (uint64_t)(stage * (C::kTile >> 4)) + off, idesc_s, k > 0);
+        }
+        if (leader) tc_commit(bar(kSFull + a));
+      };
+      Walk w = walk();
+      for (bool first = true; alive && w.next(first); first = false) {
+        const int two = w.rows > kTileRows ? 2 : 1;
+        for (int a = 0; a < two; ++a)
+          alive = alive && mbar_wait(bar(kQFull + a), q_uses[a]++ & 1, abort_flag);
+        alive = alive && mbar_wait(bar(kKFull + (count & 1)), count >> 1 & 1, abort_flag);
+        if (!alive) break;
+        tc_fence_after();
+        for (int a = 0; a < two; ++a) scores(a, count & 1);
+        if (leader) tc_commit(bar(kKEmpty + (count & 1)));
+        for (int t = w.t0; t < w.t1; ++t, ++count) {
+          const uint32_t stage = count & 1, next = count + 1;
+          const bool more = t + 1 < w.t1;
+          alive = alive && mbar_wait(bar(kVFull + stage), count >> 1 & 1, abort_flag);
+          if (more) alive = alive && mbar_wait(bar(kKFull + (next & 1)), next >> 1 & 1, abort_flag);
+          if (!alive) break;
+          for (int a = 0; a < two; ++a) {
+            if (!mbar_wait(bar(kPFull + a), p_uses[a]++ & 1, abort_flag)) {
+              alive = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              if (leader)
+                mma_ts(tmem + C::kO + a * HD, tmem + a * 128 + k * 8, vd + (uint64_t)(stage * (C::kTile >> 4)) + (uint64_t)(k * (2048 >> 4)), idesc_o,
+                       t > w.t0 || k > 0);
+            if (more) scores(a, next & 1);
+            else if (leader) tc_commit(bar(kOFull + a));
+          }
+          if (!alive) break;
+          if (leader) {
+            tc_commit(bar(kVEmpty + stage));
+            if (more) tc_commit(bar(kKEmpty + (next & 1)));
+          }
+        }
+      }
+    }
+  }
+
+  // ---- teardown
+  if (bad && p.status) atomicOr(p.status, kStatusBadBlock);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  const bool gave_up = *abort_flag != 0;
+  if (gave_up) {
+    if (tid == 0) {
+      abort_grace();
+      if (p.status) atomicOr(p.status, kStatusTimeout);
+    }
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (!is_cut || gave_up || pos >= end) return;
+
+  // ---- lines of which other CTAs have parts too: the one that began before this share and the one that goes on behind it
+  int64_t line_base[2] = {-1, -1};
+  int line_b[2], line_u[2], line_kvh[2], line_tiles[2], line_cost[2], line_rows[2];
+  {
+    Walk w = walk();
+    for (bool first = true; w.next(first); first = false)
+      if (!w.whole) {
+        const int k = w.t0 == 0 ? 1 : 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (j == k) {
+            line_base[j] = w.base;
+            line_b[j] = w.b; line_u[j] = w.u; line_kvh[j] = w.kvh; line_tiles[j] = w.tiles; line_cost[j] = w.cost; line_rows[j] = w.rows;
+          }
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (line_base[k] < 0) continue;   // (uniform)
+    const int first = (int)(line_base[k] / share), parts = (int)((line_base[k] + (int64_t)(line_tiles[k] - 1) * line_cost[k]) / share) - first + 1;
+    if (tid == 0) {
+      __threadfence();
+      ms.last[k] = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
+      __threadfence();
+    }
+    __syncthreads();
+    if (!ms.last[k]) continue;
+    const Rows rw = rows_of(p, line_b[k]);
+    for (int r = warp; r < line_rows[k]; r += kThreads / 32) {
+      const int rr = line_u[k] * kPairRows + r, i = rr / G, h = (p.kv_begin + line_kvh[k]) * G + rr - i * G;
+      float top = kUnset, sum = 0.f;
+      constexpr int N = HD / 32;
+      float o[N] = {};
+      for (int q = 0; q < parts; q += 4) {
+        float2 st[4];
+        float v[4][N];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int part = min(q + x, parts - 1);
+          const int64_t from = (int64_t)(2 * (first + part) + (part == 0)) * kPairRows + r;
+          st[x] = __ldcg(cut.stats + from);
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[x][e] = __ldcg(cut.partial + from * HD + 32 * e + lane);
+        }
+        float now = top;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x].x);
+        const float keep = ex2_approx(top - now);
+        top = now;
+        sum *= keep;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] *= keep;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (q + x >= parts) continue;
+          const float f = ex2_approx(st[x].x - top);
+          sum += f * st[x].y;
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] += f * v[x][e];
+        }
+      }
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t at = query_at(p, p.os, rw, line_b[k], h, i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int64_t to = at + 32 * e + lane;
+        if (p.dtype == AIDN_F16) static_cast<__half*>(p.out)[to] = __float2half_rn(o[e] * f);
+        else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(o[e] * f);
+      }
+      if (p.lse && lane == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+  }
+}
+
+template <int HD, bool CAP>
+cudaError_t launch(const Attend& p, int grid, const Cut& cut, uint64_t* raised, cudaStream_t stream) {
+  auto k = kv8_sm100_kernel<HD, CAP>;
+  const int id = 60 + (HD == 128 ? 2 : 0) + (CAP ? 1 : 0);
+  if (!(*raised >> id & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::kSmem);
+    if (e != cudaSuccess) return e;
+    *raised |= 1ull << id;
+  }
+  return launch_dependent(k, dim3((unsigned)grid), kThreads, Cfg<HD>::kSmem, stream, p, cut);
+}
+
+}  // namespace
+
+bool sm100_supported(const Attend& p) {
+  if (p.dtype == AIDN_F32 || p.out_f32 || (p.c.head_dim != 64 && p.c.head_dim != 128) || p.mask_kind != AIDN_MASK_NONE) return false;
+  if (p.c.block_size % 16 != 0 || (uintptr_t)p.c.k % 16 != 0 || (uintptr_t)p.c.v % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (p.c.stride[i] % 16 != 0) return false;
+  return p.seq_q * p.group < 0x7fffffff - kPairRows;
+}
+int64_t sm100_workspace_bytes(int head_dim, int num_sms) { return (int64_t)2 * num_sms * kPairRows * (head_dim * 4 + 8); }
+
+cudaError_t launch_attend_sm100(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream) {
+  const int grid = num_sms < kCounters ? num_sms : kCounters;
+  if (workspace_bytes < sm100_workspace_bytes(p.c.head_dim, grid) || (uintptr_t)workspace % 16 != 0) workspace = nullptr;
+  Cut cut;
+  cut.partial = static_cast<float*>(workspace);
+  cut.stats = workspace ? reinterpret_cast<float2*>(cut.partial + (int64_t)2 * grid * kPairRows * p.c.head_dim) : nullptr;
+  auto vec = [](const void* ptr, const int64_t* st) { return ((uintptr_t)ptr | (uint64_t)(st[0] * 2) | (uint64_t)(st[1] * 2) | (uint64_t)(st[2] * 2)) % 16 == 0; };
+  cut.query_vec = vec(p.q, p.qs);
+  cut.out_vec = vec(p.out, p.os);
+  if (p.c.head_dim == 64) return p.softcap > 0.f ? launch<64, true>(p, grid, cut, raised, stream) : launch<64, false>(p, grid, cut, raised, stream);
+  return p.softcap > 0.f ? launch<128, true>(p, grid, cut, raised, stream) : launch<128, false>(p, grid, cut, raised, stream);
+}
+
+}  // namespace kv8
+}  // namespace aidn
