@@ -13,13 +13,15 @@
 //
 //   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
 //                     (16 bits), the running maximum (the accumulator is scaled again only when a logit is 2^8 above it), results
-//   warps 8-11        keys: 16-byte loads through the block table, codes to fp16, into a ring of two 128-key tiles
-//   warps 12-15       values, the same
-//   warp 16           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V; while the softmax works on one tile's scores the other's are formed
+//   warps 8-11        keys and values: 16-byte loads through the block table, codes to fp16, into rings of two 128-key tiles
+//   warp 12           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V; while the softmax works on one tile's scores the other's are formed
 //
 // Tensor memory: S_0 | S_1 (128 columns each, P in the first 64), O_0 | O_1.  The tiles of all lines are one row that is cut into
 // equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice); parts of cut lines meet in the
 // workspace as in kv8_split.cu, merged by the CTA that arrives last.
+#include <type_traits>
+
+#include "ffma2.cuh"
 #include "kv8.cuh"
 #include "sm100_ptx.cuh"
 
@@ -32,11 +34,11 @@ using namespace ptx;
 constexpr int kKeys = 128;            // keys of a tile
 constexpr int kTileRows = 128;
 constexpr int kPairRows = 2 * kTileRows;
-constexpr int kThreads = 640;
-constexpr int kKeyWarp = 8, kValueWarp = 12, kMmaWarp = 16;
-constexpr int kSoftmaxRegs = 144, kConvertRegs = 64, kMmaRegs = 56;
+constexpr int kThreads = 512;
+constexpr int kConvertWarp = 8, kMmaWarp = 12;
+constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kMmaRegs = 48;
 // setmaxnreg.inc waits without a bound for registers that are not there: the shares must not exceed what the CTA is launched with
-static_assert(256 * kSoftmaxRegs + 256 * kConvertRegs + 128 * kMmaRegs <= kThreads * 96, "registers of the launch");
+static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kMmaRegs <= kThreads * 128, "registers of the launch");
 constexpr int kRing = 4;              // tiles whose scales are kept
 constexpr float kUnset = -1e30f;
 constexpr float kLazy = 8.f, kRefSlack = 3.f, kLift = 4.f;   // 2^(8 + 3 + 4) is in fp16's range
@@ -57,7 +59,7 @@ struct Misc {
   uint64_t bars[kBars];
   uint32_t tmem;
   int abort;
-  float k_scale[kRing][8], v_exp[kRing][8];   // of a tile's groups of sixteen keys; v_exp -inf: no such keys
+  alignas(16) float k_scale[kRing][8], v_exp[kRing][8];   // of a tile's groups of sixteen keys; v_exp -inf: no such keys
   uint32_t nan_keys[kRing][4];                // keys with a NaN among their values, in tiles of which rows do not see all
   int64_t scan[kThreads / 32];
   int64_t start_base;
@@ -171,7 +173,7 @@ __device__ __forceinline__ void store8(const Attend& p, int64_t at, bool vec, co
   uint16_t* to = static_cast<uint16_t*>(p.out) + at;
   uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = p.dtype == AIDN_F16 ? pack2<false>(x[2 * e], x[2 * e + 1]) : pack2<true>(x[2 * e], x[2 * e + 1]);
+  for (int e = 0; e < 4; ++e) w[e] = p.dtype == AIDN_F16 ? ptx::pack2<false>(x[2 * e], x[2 * e + 1]) : ptx::pack2<true>(x[2 * e], x[2 * e + 1]);
   if (vec) {
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
       mbar_init(bar(kPFull + i), 4);
       mbar_init(bar(kOFull + i), 1);
     }
-    for (int i = 0; i < kRing; ++i) mbar_init(bar(kScales + i), 8);
+    for (int i = 0; i < kRing; ++i) mbar_init(bar(kScales + i), 4);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   bool alive = pos < end;
   bool bad = false;
 
-  if (warp < kKeyWarp) {
+  if (warp < kConvertWarp) {
     // ================================================= softmax =================================================
     setmaxnreg_inc<kSoftmaxRegs>();
     const int a = warp >> 2, row_in = tid & 127;
@@ -339,8 +341,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           for (int j = 0; j < HD / 8; ++j) {
             float x[8] = {};
             if (valid) query8(p, at + 8 * j, cut.query_vec, x);
-            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), pack2<false>(x[0] * f, x[1] * f), pack2<false>(x[2] * f, x[3] * f),
-                         pack2<false>(x[4] * f, x[5] * f), pack2<false>(x[6] * f, x[7] * f));
+            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), ptx::pack2<false>(x[0] * f, x[1] * f), ptx::pack2<false>(x[2] * f, x[3] * f),
+                         ptx::pack2<false>(x[4] * f, x[5] * f), ptx::pack2<false>(x[6] * f, x[7] * f));
           }
         }
         fence_proxy_async_smem();
@@ -362,104 +364,103 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           ++s_uses;
           tc_fence_after();
           const int key0 = t * kKeys;
-          const bool edge = key0 + kKeys > lim_least || key0 + kKeys > w.keys;   // (uniform)
-          const float* ksc = ms.k_scale[ring];
-          const float* vex = ms.v_exp[ring];
-          uint32_t s[2][32];
-          // the score of column k: what a row does not see is -inf, a key with a NaN among its values NaN
-          auto mask = [&](uint32_t* x, int col0) {
-            const uint32_t nan = ms.nan_keys[ring][col0 >> 5];
+          auto step = [&](auto edge_t) {
+            constexpr bool EDGE = decltype(edge_t)::value;
+            uint32_t s[128];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (nan >> e & 1) x[e] = 0x7fffffffu;
-              if (key0 + col0 + e >= lim) x[e] = 0xff800000u;
+            for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, s + 32 * q);
+            float ck[8], e[8];   // of the tile's groups of sixteen keys: factor of the scores, exponent of the weights
+#pragma unroll
+            for (int g = 0; g < 8; g += 4) {
+              const float4 u = *reinterpret_cast<const float4*>(&ms.k_scale[ring][g]), v = *reinterpret_cast<const float4*>(&ms.v_exp[ring][g]);
+              ck[g] = c * u.x; ck[g + 1] = c * u.y; ck[g + 2] = c * u.z; ck[g + 3] = c * u.w;
+              e[g] = v.x; e[g + 1] = v.y; e[g + 2] = v.z; e[g + 3] = v.w;
+            }
+            tc_wait_ld();
+            if constexpr (EDGE) {   // what a row does not see is -inf, a key with a NaN among its values NaN
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t nan = ms.nan_keys[ring][q];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  if (nan >> k & 1) s[32 * q + k] = 0x7fffffffu;
+                  if (key0 + 32 * q + k >= lim) s[32 * q + k] = 0xff800000u;
+                }
+              }
+            }
+            float top = kUnset, emax = e[0];
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              const uint32_t* x = s + 16 * g;
+              float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[8]);
+#pragma unroll
+              for (int k = 1; k < 7; k += 2) {
+                m0 = fmax3(m0, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                m1 = fmax3(m1, __uint_as_float(x[8 + k]), __uint_as_float(x[9 + k]));
+              }
+              m0 = fmax3(fmaxf(m0, m1), __uint_as_float(x[7]), __uint_as_float(x[15]));
+              float y = m0 * ck[g];
+              if (CAP) y = cap(y, p.softcap, cap_inverse);
+              if (EDGE) y = m0 == -INFINITY ? kUnset : y;   // (a scale of zero times -inf, and the cap of -inf)
+              top = fmaxf(top, e[g] == -INFINITY ? kUnset : y);
+              emax = fmaxf(emax, e[g]);
+            }
+            float keep = 1.f;
+            if (top > m + kLazy) {
+              keep = ex2_approx(m - top);
+              l *= keep;
+              m = top;
+            }
+            if (emax > eref + kRefSlack) {
+              keep *= eref == -INFINITY ? 0.f : ex2_approx(eref - emax);
+              eref = emax;
+            }
+            if (t > w.t0 && __any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll 1
+              for (int q = 0; q < HD / 16; ++q) {
+                uint32_t o[16];
+                tmem_ld16(to + 16 * q, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                tmem_st16(to + 16 * q, o);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t packed[16];
+#pragma unroll
+              for (int hlf = 0; hlf < 2; ++hlf) {
+                const int g = 2 * q + hlf;
+                const float off = e[g] == -INFINITY ? -INFINITY : e[g] - eref - m + kLift;
+                const uint64_t ck2 = aidn::pack2(ck[g], ck[g]), off2 = aidn::pack2(off, off);
+                uint64_t sum = 0;
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                  const float u = __uint_as_float(s[16 * g + k]), v = __uint_as_float(s[16 * g + k + 1]);
+                  float2 y;
+                  if constexpr (CAP) {
+                    y.x = cap(u * ck[g], p.softcap, cap_inverse) + off;
+                    y.y = cap(v * ck[g], p.softcap, cap_inverse) + off;
+                  } else {
+                    y = unpack2(fma2(aidn::pack2(u, v), ck2, off2));
+                  }
+                  y.x = ex2_approx(y.x);
+                  y.y = ex2_approx(y.y);
+                  if constexpr (EDGE) {
+                    y.x = u == -INFINITY ? 0.f : y.x;
+                    y.y = v == -INFINITY ? 0.f : y.y;
+                  }
+                  sum = add2(sum, aidn::pack2(y.x, y.y));
+                  packed[8 * hlf + (k >> 1)] = ptx::pack2<false>(y.x, y.y);
+                }
+                l = fmaf(sum2(sum), e[g] == -INFINITY ? 0.f : ex2_approx(eref - e[g] - kLift), l);
+              }
+              tmem_st16(ts + 16 * q, packed);
             }
           };
-          // ---- the maximum
-          float top = kUnset;
-          tmem_ld32(ts, s[0]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            tc_wait_ld();
-            if (q < 3) tmem_ld32(ts + 32 * (q + 1), s[(q + 1) & 1]);
-            uint32_t* x = s[q & 1];
-            if (edge) mask(x, 32 * q);
-#pragma unroll
-            for (int hlf = 0; hlf < 2; ++hlf) {
-              float mx = __uint_as_float(x[16 * hlf]);
-#pragma unroll
-              for (int e = 1; e < 15; e += 2) mx = fmax3(mx, __uint_as_float(x[16 * hlf + e]), __uint_as_float(x[16 * hlf + e + 1]));
-              mx = fmaxf(mx, __uint_as_float(x[16 * hlf + 15]));
-              const int g = 2 * q + hlf;
-              if (vex[g] != -INFINITY && mx != -INFINITY) {
-                mx *= c * ksc[g];
-                top = fmaxf(top, CAP ? cap(mx, p.softcap, cap_inverse) : mx);
-              }
-            }
-          }
-          float emax = vex[0];
-#pragma unroll
-          for (int g = 1; g < 8; ++g) emax = fmaxf(emax, vex[g]);
-          float keep = 1.f;
-          if (top > m + kLazy) {
-            const float f = ex2_approx(m - top);
-            keep = f;
-            l *= f;
-            m = top;
-          }
-          if (emax > eref + kRefSlack) {
-            keep *= eref == -INFINITY ? 0.f : ex2_approx(eref - emax);
-            eref = emax;
-          }
-          if (t > w.t0 && __any_sync(0xffffffffu, keep != 1.f)) {
-#pragma unroll
-            for (int q = 0; q < HD / 32; ++q) {
-              tmem_ld32(to + 32 * q, s[0]);
-              tc_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * keep);
-              tmem_st32(to + 32 * q, s[0]);
-            }
-            tc_wait_st();
-          }
-          // ---- weights
-          tmem_ld32(ts, s[0]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            tc_wait_ld();
-            if (q < 3) tmem_ld32(ts + 32 * (q + 1), s[(q + 1) & 1]);
-            uint32_t* x = s[q & 1];
-            if (edge) mask(x, 32 * q);
-            uint32_t packed[16];
-#pragma unroll
-            for (int hlf = 0; hlf < 2; ++hlf) {
-              const int g = 2 * q + hlf;
-              const float cg = c * ksc[g], e = vex[g], off = e == -INFINITY ? -INFINITY : e - eref - m + kLift;
-              float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                float u = __uint_as_float(x[16 * hlf + k]), v = __uint_as_float(x[16 * hlf + k + 1]);
-                if (CAP) {
-                  // (a masked score stays -inf, whatever the cap makes of it)
-                  u = u == -INFINITY ? u : cap(u * cg, p.softcap, cap_inverse);
-                  v = v == -INFINITY ? v : cap(v * cg, p.softcap, cap_inverse);
-                  u = ex2_approx(u + off);
-                  v = ex2_approx(v + off);
-                } else if (edge) {
-                  u = u == -INFINITY ? 0.f : ex2_approx(fmaf(u, cg, off));   // (a scale of zero times -inf)
-                  v = v == -INFINITY ? 0.f : ex2_approx(fmaf(v, cg, off));
-                } else {
-                  u = ex2_approx(fmaf(u, cg, off));
-                  v = ex2_approx(fmaf(v, cg, off));
-                }
-                sum0 += u;
-                sum1 += v;
-                packed[8 * hlf + (k >> 1)] = pack2<false>(u, v);
-              }
-              if (e != -INFINITY) l = fmaf(sum0 + sum1, ex2_approx(eref - e - kLift), l);
-            }
-            tmem_st16(ts + 16 * q, packed);
-          }
+          if (key0 + kKeys > lim_least || key0 + kKeys > w.keys) step(std::true_type{});   // (uniform)
+          else step(std::false_type{});
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -500,77 +501,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   } else if (warp < kMmaWarp) {
     // ======================================= keys and values: codes to fp16 =======================================
     setmaxnreg_dec<kConvertRegs>();
-    const bool is_key = warp < kValueWarp;
     const int quarter = warp & 3, t4 = lane & 3, g8 = lane >> 2;   // this warp: keys 32 quarter .. + 31; a lane: row g8 (+ 8 i), 16 bytes t4
     constexpr int H = HD / 64;
     const int64_t pitch = p.c.stride[1];
-    const int full = is_key ? kKFull : kVFull, empty = is_key ? kKEmpty : kVEmpty;
-    const uint32_t dst0 = base + (is_key ? C::kK : C::kV) + (uint32_t)((32 * quarter + g8) * 128);
+    const uint32_t dst0 = base + (uint32_t)((32 * quarter + g8) * 128);
     uint32_t count = 0;
     if (alive) {
       Walk w = walk();
       for (bool first = true; alive && w.next(first); first = false) {
         const int kvh = p.kv_begin + w.kvh;
-        const uint8_t* const src = (is_key ? p.c.k : p.c.v) + kvh * p.c.stride[2] + 16 * t4;
-        const float* const scales = is_key ? p.c.k_scale : p.c.v_scale;
+        const int64_t lane_at = kvh * p.c.stride[2] + 16 * t4 + g8 * pitch;
         const int32_t* const table = p.c.table + w.b * p.c.table_stride;
         // lane e of this: the block of keys 32 quarter + 16 (e & 1) .. of a tile
         auto entry_of = [&](int t) {
           const int key = t * kKeys + 32 * quarter + 16 * (lane & 1);
           return t < w.t1 && key < w.keys ? checked_block(p.c, table[block_of(p.c, key)], bad) : -1;
         };
-        uint4 x[4][H];
-        float scale;
-        int entry = entry_of(w.t0), entry_n;
-        auto load = [&](int t) {
+        uint4 xk[4][H], xv[4][H];
+        int entry = entry_of(w.t0), entry_n;   // of the tile that is loaded, and of the next
+        auto load = [&](const uint8_t* pool, int t, uint4 (&x)[4][H]) {
           const int key0 = t * kKeys + 32 * quarter;
-          scale = entry >= 0 ? scales[(int64_t)entry * p.c.kv_heads + kvh] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int ent = __shfl_sync(0xffffffffu, entry, i >> 1), key = key0 + 16 * (i >> 1);
-            const int in_block = key - block_of(p.c, key) * p.c.block_size + 8 * (i & 1) + g8;
-            const bool there = ent >= 0 && key0 + 8 * i + g8 < w.keys;
-            const uint8_t* at = src + ent * p.c.stride[0] + in_block * pitch;
+          for (int j = 0; j < 2; ++j) {
+            const int ent = __shfl_sync(0xffffffffu, entry, j), key = key0 + 16 * j;
+            const uint8_t* at = pool + lane_at + ent * p.c.stride[0] + (key - block_of(p.c, key) * p.c.block_size) * pitch;
+            if (ent >= 0 && key + 16 <= w.keys) {
 #pragma unroll
-            for (int q = 0; q < H; ++q) x[i][q] = there ? ld_stream16(at + 64 * q) : make_uint4(0, 0, 0, 0);
-          }
-        };
-        const int lim_least = visible(p, w.keys, w.rw.count, w.u * kPairRows / G);
-        load(w.t0);
-        entry_n = entry_of(w.t0 + 1);
-        for (int t = w.t0; t < w.t1; ++t, ++count) {
-          const uint32_t stage = count & 1, ring = count % kRing;
-          if (!mbar_wait(bar(empty + stage), (count >> 1 & 1) ^ 1, abort_flag)) {
-            alive = false;
-            break;
-          }
-          uint32_t nan = 0;
-          if (!is_key && t * kKeys + kKeys > lim_least) {   // NaN values of keys that some rows do not see
+              for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              bool hit = false;
+                for (int q = 0; q < H; ++q) x[2 * j + i][q] = ld_stream16(at + i * 8 * pitch + 64 * q);
+            } else {
 #pragma unroll
-              for (int q = 0; q < H; ++q) {
-                hit = hit || any_nan(x[i][q].x) || any_nan(x[i][q].y) || any_nan(x[i][q].z) || any_nan(x[i][q].w);
-                x[i][q].x = without_nan(x[i][q].x); x[i][q].y = without_nan(x[i][q].y);
-                x[i][q].z = without_nan(x[i][q].z); x[i][q].w = without_nan(x[i][q].w);
-              }
-              const uint32_t who = __ballot_sync(0xffffffffu, hit);
+              for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int r = 0; r < 8; ++r)
-                if (who >> (4 * r) & 15) nan |= 1u << (8 * i + r);
+                for (int q = 0; q < H; ++q)
+                  x[2 * j + i][q] = ent >= 0 && key + 8 * i + g8 < w.keys ? ld_stream16(at + i * 8 * pitch + 64 * q) : make_uint4(0, 0, 0, 0);
             }
           }
-          if (lane < 2) {
-            const int g = 2 * quarter + lane;
-            float exponent = log2_approx(scale);
-            if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
-            if (entry < 0) exponent = -INFINITY;
-            if (is_key) ms.k_scale[ring][g] = scale;
-            else ms.v_exp[ring][g] = exponent;
-          }
-          if (!is_key && lane == 0) ms.nan_keys[ring][quarter] = nan;
-          const uint32_t dst = dst0 + stage * C::kTile;
+        };
+        auto convert = [&](uint32_t dst, const uint4 (&x)[4][H]) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -582,14 +551,62 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
             }
           fence_proxy_async_smem();
           __syncwarp();
+        };
+        auto scale_of = [&](const float* scales) { return entry >= 0 ? scales[(int64_t)entry * p.c.kv_heads + kvh] : 0.f; };
+        const int lim_least = visible(p, w.keys, w.rw.count, w.u * kPairRows / G);
+        load(p.c.k, w.t0, xk);
+        load(p.c.v, w.t0, xv);
+        float ks = scale_of(p.c.k_scale), vs = scale_of(p.c.v_scale);
+        entry_n = entry_of(w.t0 + 1);
+        for (int t = w.t0; t < w.t1; ++t, ++count) {
+          const uint32_t stage = count & 1, ring = count % kRing;
+          const int before = entry;
+          entry = entry_n;
+          entry_n = entry_of(t + 2);
+          if (!mbar_wait(bar(kKEmpty + stage), (count >> 1 & 1) ^ 1, abort_flag)) {
+            alive = false;
+            break;
+          }
+          convert(dst0 + C::kK + stage * C::kTile, xk);
+          if (lane == 0) mbar_arrive(bar(kKFull + stage));
+          if (t + 1 < w.t1) load(p.c.k, t + 1, xk);
+          if (!mbar_wait(bar(kVEmpty + stage), (count >> 1 & 1) ^ 1, abort_flag)) {
+            alive = false;
+            break;
+          }
+          uint32_t nan = 0;
+          if (t * kKeys + kKeys > lim_least) {   // NaN values of keys that some rows do not see
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              bool hit = false;
+#pragma unroll
+              for (int q = 0; q < H; ++q) {
+                hit = hit || any_nan(xv[i][q].x) || any_nan(xv[i][q].y) || any_nan(xv[i][q].z) || any_nan(xv[i][q].w);
+                xv[i][q].x = without_nan(xv[i][q].x); xv[i][q].y = without_nan(xv[i][q].y);
+                xv[i][q].z = without_nan(xv[i][q].z); xv[i][q].w = without_nan(xv[i][q].w);
+              }
+              const uint32_t who = __ballot_sync(0xffffffffu, hit);
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                if (who >> (4 * r) & 15) nan |= 1u << (8 * i + r);
+            }
+          }
+          if (lane < 2) {
+            float exponent = log2_approx(vs);
+            if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
+            ms.k_scale[ring][2 * quarter + lane] = ks;
+            ms.v_exp[ring][2 * quarter + lane] = before < 0 ? -INFINITY : exponent;
+          }
+          if (lane == 0) ms.nan_keys[ring][quarter] = nan;
+          convert(dst0 + C::kV + stage * C::kTile, xv);
           if (lane == 0) {
-            mbar_arrive(bar(full + stage));
+            mbar_arrive(bar(kVFull + stage));
             mbar_arrive(bar(kScales + ring));
           }
           if (t + 1 < w.t1) {
-            entry = entry_n;
-            load(t + 1);
-            entry_n = entry_of(t + 2);
+            load(p.c.v, t + 1, xv);
+            ks = scale_of(p.c.k_scale);
+            vs = scale_of(p.c.v_scale);
           }
         }
       }
