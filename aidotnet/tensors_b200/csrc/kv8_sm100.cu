@@ -14,9 +14,11 @@
 //   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
 //                     (16 bits), the running maximum (the accumulator is scaled again only when a logit is 2^8 above it), results
 //   warps 8-11        keys and values: 16-byte loads through the block table, codes to fp16, into rings of two 128-key tiles
-//   warp 12           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V; while the softmax works on one tile's scores the other's are formed
+//   warp 12           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V, for 64 keys at a time
 //
-// Tensor memory: S_0 | S_1 (128 columns each, P in the first 64), O_0 | O_1.  The tiles of all lines are one row that is cut into
+// Tensor memory: two score buffers of 64 columns for each row tile (P in the first half of each), O_0 | O_1.  The scores of 64 keys
+// are formed while the softmax works on the 64 before: with one buffer of 128 keys a tile the chain softmax -> P V -> next scores
+// was the period, 4500 to 5300 cycles for 128 keys where the products take 2050 and the softmax 2900.  The tiles of all lines are one row that is cut into
 // equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice); parts of cut lines meet in the
 // workspace as in kv8_split.cu, merged by the CTA that arrives last.
 #include <type_traits>
@@ -52,8 +54,8 @@ struct Cfg {
   static constexpr int kSmem = kMisc + 2048 + 1024 /* alignment */;
   static constexpr uint32_t kO = 256;                    // accumulators' first column
 };
-// barriers: q_full[2] k_full[2] k_empty[2] v_full[2] v_empty[2] s_full[2] p_full[2] o_full[2] scales[kRing]
-enum { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kOFull = 14, kScales = 16, kBars = 16 + kRing };
+// barriers: q_full[2] k_full[2] k_empty[2] v_full[2] v_empty[2] s_full[2][2] p_full[2][2] o_done[2] scales[kRing]
+enum { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 14, kODone = 18, kScales = 20, kBars = 20 + kRing };
 
 struct Misc {
   uint64_t bars[kBars];
@@ -65,8 +67,15 @@ struct Misc {
   int64_t start_base;
   int start_b, start_u;
   int last[2];
+  // the lines of which other CTAs have parts too (base -1: none): the one that began before this share, the one that goes on
+  struct { int64_t base, first_row; int b, u, kvh, tiles, cost, rows, count; } open[2];
 };
 static_assert(sizeof(Misc) <= 2048, "");
+
+// (a division of 64 bits takes over a hundred instructions)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 
 struct Cut {
   float* partial;   // [2 grid][256][HD], or null: lines are not cut
@@ -122,8 +131,8 @@ struct Walk {
       first = false;
       if (base >= end) return false;
       if (cut) {
-        t0 = pos > base ? (int)((pos - base + cost - 1) / cost) : 0;
-        const int64_t most = (end - base + cost - 1) / cost;
+        t0 = pos > base ? (int)((pos - base + cost - 1) >> (cost - 1)) : 0;   // (cost 1 or 2)
+        const int64_t most = (end - base + cost - 1) >> (cost - 1);
         t1 = most < tiles ? (int)most : tiles;
         if (t0 >= t1) continue;
         whole = t0 == 0 && t1 == tiles;
@@ -152,10 +161,9 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   const uint32_t hit = (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
   return x & ~(hit * 0xffu);
 }
-// Eight 16-bit elements at `at`, as floats.
-__device__ __forceinline__ void query8(const Attend& p, int64_t at, bool vec, float* x) {
+// Eight 16-bit elements of the queries as they lie, and two of them as floats.
+__device__ __forceinline__ void query8(const Attend& p, int64_t at, bool vec, uint32_t* w) {
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
-  uint32_t w[4];
   if (vec) {
     const uint4 v = *reinterpret_cast<const uint4*>(q);
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -163,11 +171,10 @@ __device__ __forceinline__ void query8(const Attend& p, int64_t at, bool vec, fl
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t v = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-    x[e] = p.dtype == AIDN_F16 ? __half2float(__ushort_as_half((unsigned short)v)) : __uint_as_float(v << 16);
-  }
+}
+__device__ __forceinline__ float2 widen2(const Attend& p, uint32_t w) {
+  if (p.dtype == AIDN_F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 __device__ __forceinline__ void store8(const Attend& p, int64_t at, bool vec, const float* x) {
   uint16_t* to = static_cast<uint16_t*>(p.out) + at;
@@ -203,10 +210,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
       mbar_init(bar(kKEmpty + i), 1);
       mbar_init(bar(kVFull + i), 4);
       mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kODone + i), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kSFull + i), 1);
       mbar_init(bar(kPFull + i), 4);
-      mbar_init(bar(kOFull + i), 1);
     }
+    ms.open[0].base = ms.open[1].base = -1;
     for (int i = 0; i < kRing; ++i) mbar_init(bar(kScales + i), 4);
     fence_mbar_init();
   }
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     total += ms.scan[w];
   }
   before += upto - mine;
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
   if (share < 4) share = 4;
   const int64_t pos = blockIdx.x * share, end = min(pos + share, total);
   const uint32_t tmem = ms.tmem;
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     w.sequence();
     w.line();
     const int64_t a_line = (int64_t)w.tiles * w.cost;
-    w.kvh = (int)((pos - ms.start_base) / a_line);
+    w.kvh = (int)quotient(pos - ms.start_base, a_line);
     w.base = ms.start_base + w.kvh * a_line;
     return w;
   };
@@ -304,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     setmaxnreg_inc<kSoftmaxRegs>();
     const int a = warp >> 2, row_in = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + (uint32_t)(a * 128), to = tmem + lanes + C::kO + (uint32_t)(a * HD);
-    uint32_t q_uses = 0, s_uses = 0;
+    const uint32_t ts0 = tmem + lanes + (uint32_t)(a * 128), to = tmem + lanes + C::kO + (uint32_t)(a * HD);
+    uint32_t steps = 0;        // of 64 keys, that this row tile took part in
     uint32_t tile_count = 0;   // of this CTA, for the scales' ring
     if (alive) {
       Walk w = walk();
@@ -322,65 +332,69 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         float c;
         {
           const int64_t at = query_at(p, p.qs, w.rw, w.b, h, i);
-          float largest = 0.f;
+          uint32_t x[HD / 2];
           if (valid) {
-#pragma unroll 4
-            for (int j = 0; j < HD / 8; ++j) {
-              float x[8];
-              query8(p, at + 8 * j, cut.query_vec, x);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[e]));
-            }
+            for (int j = 0; j < HD / 8; ++j) query8(p, at + 8 * j, cut.query_vec, x + 4 * j);
+          }
+          float largest = 0.f;
+#pragma unroll
+          for (int j = 0; j < HD / 2; ++j) {
+            if (!valid) x[j] = 0;
+            const float2 y = widen2(p, x[j]);
+            largest = fmaxf(largest, fmaxf(fabsf(y.x), fabsf(y.y)));
           }
           int up = 8 - ((int)(__float_as_uint(largest) >> 23) - 127);
           up = max(-110, min(up, 126));
           const float f = __uint_as_float((uint32_t)(up + 127) << 23);
           c = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (CAP ? 1.f : kLog2e);
           const uint32_t dst = base + C::kQ + a * C::kTile + row_in * 128;
-#pragma unroll 4
+#pragma unroll
           for (int j = 0; j < HD / 8; ++j) {
-            float x[8] = {};
-            if (valid) query8(p, at + 8 * j, cut.query_vec, x);
-            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), ptx::pack2<false>(x[0] * f, x[1] * f), ptx::pack2<false>(x[2] * f, x[3] * f),
-                         ptx::pack2<false>(x[4] * f, x[5] * f), ptx::pack2<false>(x[6] * f, x[7] * f));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 y = widen2(p, x[4 * j + e]);
+              x[4 * j + e] = ptx::pack2<false>(y.x * f, y.y * f);
+            }
+            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kQFull + a));
-        ++q_uses;
         const int lim = valid ? visible(p, w.keys, w.rw.count, i) : 0x7fffffff;
         const int lim_least = visible(p, w.keys, w.rw.count, (w.u * kPairRows + a * kTileRows) / G);
         const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
         float m = kUnset, l = 0.f, eref = -INFINITY;
 
-        for (int t = w.t0; t < w.t1 && alive; ++t, ++tile_count) {
-          const uint32_t ring = tile_count % kRing;
+        if (!w.whole && tid == 0) {
+          auto& o = ms.open[w.t0 == 0 ? 1 : 0];
+          o.base = w.base; o.first_row = w.rw.first; o.b = w.b; o.u = w.u; o.kvh = w.kvh;
+          o.tiles = w.tiles; o.cost = w.cost; o.rows = w.rows; o.count = w.rw.count;
+        }
+        for (int u = 0; u < 2 * n_tiles; ++u, ++steps) {
+          const uint32_t ring = tile_count % kRing, buf = u & 1;   // (a line's steps come in pairs: so does every buffer's phase)
           // (in this order: once a tile's scores are there, its scales are the next that the ring's slot waits for)
-          if (!mbar_wait(bar(kSFull + a), s_uses & 1, abort_flag) || !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
+          if (!mbar_wait(bar(kSFull + 2 * a + buf), steps >> 1 & 1, abort_flag) || !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
             alive = false;
             break;
           }
-          ++s_uses;
           tc_fence_after();
-          const int key0 = t * kKeys;
+          const int key0 = (w.t0 + (u >> 1)) * kKeys + 64 * buf;
+          const uint32_t ts = ts0 + 64 * buf;
           auto step = [&](auto edge_t) {
             constexpr bool EDGE = decltype(edge_t)::value;
-            uint32_t s[128];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, s + 32 * q);
-            float ck[8], e[8];   // of the tile's groups of sixteen keys: factor of the scores, exponent of the weights
-#pragma unroll
-            for (int g = 0; g < 8; g += 4) {
-              const float4 u = *reinterpret_cast<const float4*>(&ms.k_scale[ring][g]), v = *reinterpret_cast<const float4*>(&ms.v_exp[ring][g]);
-              ck[g] = c * u.x; ck[g + 1] = c * u.y; ck[g + 2] = c * u.z; ck[g + 3] = c * u.w;
-              e[g] = v.x; e[g + 1] = v.y; e[g + 2] = v.z; e[g + 3] = v.w;
-            }
+            uint32_t s[64];
+            tmem_ld32(ts, s);
+            tmem_ld32(ts + 32, s + 32);
+            // of the groups of sixteen keys: factor of the scores, exponent of the weights
+            const float4 k4 = *reinterpret_cast<const float4*>(&ms.k_scale[ring][4 * buf]), v4 = *reinterpret_cast<const float4*>(&ms.v_exp[ring][4 * buf]);
+            const float ck[4] = {c * k4.x, c * k4.y, c * k4.z, c * k4.w}, e[4] = {v4.x, v4.y, v4.z, v4.w};
             tc_wait_ld();
             if constexpr (EDGE) {   // what a row does not see is -inf, a key with a NaN among its values NaN
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint32_t nan = ms.nan_keys[ring][q];
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t nan = ms.nan_keys[ring][2 * buf + q];
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                   if (nan >> k & 1) s[32 * q + k] = 0x7fffffffu;
@@ -390,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
             }
             float top = kUnset, emax = e[0];
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
+            for (int g = 0; g < 4; ++g) {
               const uint32_t* x = s + 16 * g;
               float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[8]);
 #pragma unroll
@@ -415,7 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               keep *= eref == -INFINITY ? 0.f : ex2_approx(eref - emax);
               eref = emax;
             }
-            if (t > w.t0 && __any_sync(0xffffffffu, keep != 1.f)) {
+            if (u > 0 && __any_sync(0xffffffffu, keep != 1.f)) {   // (one product at most is on its way, that of the step before: the next needs these weights)
+              if (!mbar_wait(bar(kODone + a), (steps - 1) & 1, abort_flag)) alive = false;
+              tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < HD / 16; ++q) {
                 uint32_t o[16];
@@ -427,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               }
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
               uint32_t packed[16];
 #pragma unroll
               for (int hlf = 0; hlf < 2; ++hlf) {
@@ -437,19 +453,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
                 uint64_t sum = 0;
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
-                  const float u = __uint_as_float(s[16 * g + k]), v = __uint_as_float(s[16 * g + k + 1]);
+                  const float x = __uint_as_float(s[16 * g + k]), z = __uint_as_float(s[16 * g + k + 1]);
                   float2 y;
                   if constexpr (CAP) {
-                    y.x = cap(u * ck[g], p.softcap, cap_inverse) + off;
-                    y.y = cap(v * ck[g], p.softcap, cap_inverse) + off;
+                    y.x = cap(x * ck[g], p.softcap, cap_inverse) + off;
+                    y.y = cap(z * ck[g], p.softcap, cap_inverse) + off;
                   } else {
-                    y = unpack2(fma2(aidn::pack2(u, v), ck2, off2));
+                    y = unpack2(fma2(aidn::pack2(x, z), ck2, off2));
                   }
                   y.x = ex2_approx(y.x);
                   y.y = ex2_approx(y.y);
                   if constexpr (EDGE) {
-                    y.x = u == -INFINITY ? 0.f : y.x;
-                    y.y = v == -INFINITY ? 0.f : y.y;
+                    y.x = x == -INFINITY ? 0.f : y.x;
+                    y.y = z == -INFINITY ? 0.f : y.y;
                   }
                   sum = add2(sum, aidn::pack2(y.x, y.y));
                   packed[8 * hlf + (k >> 1)] = ptx::pack2<false>(y.x, y.y);
@@ -459,16 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               tmem_st16(ts + 16 * q, packed);
             }
           };
-          if (key0 + kKeys > lim_least || key0 + kKeys > w.keys) step(std::true_type{});   // (uniform)
+          if (key0 + 64 > lim_least || key0 + 64 > w.keys) step(std::true_type{});   // (uniform)
           else step(std::false_type{});
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kPFull + a));
+          if (lane == 0) mbar_arrive(bar(kPFull + 2 * a + buf));
+          if (!alive) break;
+          tile_count += buf;
         }
         if (!alive) break;
-        // ---- results
-        if (!mbar_wait(bar(kOFull + a), (q_uses - 1) & 1, abort_flag)) {
+        // ---- results.  The last step's scores say that the product of two steps before is done: the one before it may still be on
+        // its way, and a wait tells two phases apart, not three.
+        if (!mbar_wait(bar(kODone + a), (steps - 2) & 1, abort_flag) || !mbar_wait(bar(kODone + a), (steps - 1) & 1, abort_flag)) {
           alive = false;
           break;
         }
@@ -616,54 +635,60 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     setmaxnreg_dec<kMmaRegs>();
     if (warp == kMmaWarp && alive) {
       const bool leader = elect_one();
-      constexpr uint32_t idesc_s = make_idesc(kTileRows, kKeys, false, false), idesc_o = make_idesc(kTileRows, HD, false, true);
+      constexpr uint32_t idesc_s = make_idesc(kTileRows, 64, false, false), idesc_o = make_idesc(kTileRows, HD, false, true);
       const uint64_t qd = make_smem_desc(base + C::kQ, 16, 1024), kd = make_smem_desc(base + C::kK, 16, 1024);
       const uint64_t vd = make_smem_desc(base + C::kV, C::kSlab, 1024);
-      uint32_t count = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-      auto scores = [&](int a, uint32_t stage) {
+      uint32_t count = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};   // tiles of all lines; lines and steps of a row tile
+      auto scores = [&](int a, uint32_t tile, int buf) {   // the 64 keys `buf` of a tile
+        const uint64_t k0 = kd + (uint64_t)((tile & 1) * (C::kTile >> 4) + buf * (64 * 128 >> 4));
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint64_t off = (uint64_t)((k >> 2) * (C::kSlab >> 4) + (k & 3) * 2);
-          if (leader) mma_ss(tmem + a * 128, qd + (uint64_t)(a * (C::kTile >> 4)) + off, kd + (uint64_t)(stage * (C::kTile >> 4)) + off, idesc_s, k > 0);
+          if (leader) mma_ss(tmem + a * 128 + 64 * buf, qd + (uint64_t)(a * (C::kTile >> 4)) + off, k0 + off, idesc_s, k > 0);
         }
-        if (leader) tc_commit(bar(kSFull + a));
+        if (leader) tc_commit(bar(kSFull + 2 * a + buf));
       };
       Walk w = walk();
       for (bool first = true; alive && w.next(first); first = false) {
-        const int two = w.rows > kTileRows ? 2 : 1;
+        const int two = w.rows > kTileRows ? 2 : 1, steps = 2 * (w.t1 - w.t0);
         for (int a = 0; a < two; ++a)
           alive = alive && mbar_wait(bar(kQFull + a), q_uses[a]++ & 1, abort_flag);
         alive = alive && mbar_wait(bar(kKFull + (count & 1)), count >> 1 & 1, abort_flag);
         if (!alive) break;
         tc_fence_after();
-        for (int a = 0; a < two; ++a) scores(a, count & 1);
+        for (int buf = 0; buf < 2; ++buf)
+          for (int a = 0; a < two; ++a) scores(a, count, buf);
         if (leader) tc_commit(bar(kKEmpty + (count & 1)));
-        for (int t = w.t0; t < w.t1; ++t, ++count) {
-          const uint32_t stage = count & 1, next = count + 1;
-          const bool more = t + 1 < w.t1;
-          alive = alive && mbar_wait(bar(kVFull + stage), count >> 1 & 1, abort_flag);
-          if (more) alive = alive && mbar_wait(bar(kKFull + (next & 1)), next >> 1 & 1, abort_flag);
+        for (int u = 0; u < steps; ++u) {
+          const int buf = u & 1;
+          const uint32_t tile = count + (u >> 1);
+          const bool more = u + 2 < steps;
+          if (buf == 0) {
+            alive = alive && mbar_wait(bar(kVFull + (tile & 1)), tile >> 1 & 1, abort_flag);
+            if (more) alive = alive && mbar_wait(bar(kKFull + ((tile + 1) & 1)), (tile + 1) >> 1 & 1, abort_flag);
+          }
           if (!alive) break;
           for (int a = 0; a < two; ++a) {
-            if (!mbar_wait(bar(kPFull + a), p_uses[a]++ & 1, abort_flag)) {
+            if (!mbar_wait(bar(kPFull + 2 * a + buf), p_uses[a]++ >> 1 & 1, abort_flag)) {
               alive = false;
               break;
             }
             tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
+            for (int k = 0; k < 4; ++k)
               if (leader)
-                mma_ts(tmem + C::kO + a * HD, tmem + a * 128 + k * 8, vd + (uint64_t)(stage * (C::kTile >> 4)) + (uint64_t)(k * (2048 >> 4)), idesc_o,
-                       t > w.t0 || k > 0);
-            if (more) scores(a, next & 1);
-            else if (leader) tc_commit(bar(kOFull + a));
+                mma_ts(tmem + C::kO + a * HD, tmem + a * 128 + 64 * buf + k * 8,
+                       vd + (uint64_t)((tile & 1) * (C::kTile >> 4)) + (uint64_t)((4 * buf + k) * (2048 >> 4)), idesc_o, u > 0 || k > 0);
+            if (leader) tc_commit(bar(kODone + a));
+            if (more) scores(a, tile + 1, buf);
           }
           if (!alive) break;
-          if (leader) {
-            tc_commit(bar(kVEmpty + stage));
-            if (more) tc_commit(bar(kKEmpty + (next & 1)));
+          if (buf == 1 && leader) {
+            tc_commit(bar(kVEmpty + (tile & 1)));
+            if (more) tc_commit(bar(kKEmpty + ((tile + 1) & 1)));
           }
         }
+        count += steps >> 1;
       }
     }
   }
@@ -687,36 +712,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   }
   if (!is_cut || gave_up || pos >= end) return;
 
-  // ---- lines of which other CTAs have parts too: the one that began before this share and the one that goes on behind it
-  int64_t line_base[2] = {-1, -1};
-  int line_b[2], line_u[2], line_kvh[2], line_tiles[2], line_cost[2], line_rows[2];
-  {
-    Walk w = walk();
-    for (bool first = true; w.next(first); first = false)
-      if (!w.whole) {
-        const int k = w.t0 == 0 ? 1 : 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (j == k) {
-            line_base[j] = w.base;
-            line_b[j] = w.b; line_u[j] = w.u; line_kvh[j] = w.kvh; line_tiles[j] = w.tiles; line_cost[j] = w.cost; line_rows[j] = w.rows;
-          }
-      }
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (line_base[k] < 0) continue;   // (uniform)
-    const int first = (int)(line_base[k] / share), parts = (int)((line_base[k] + (int64_t)(line_tiles[k] - 1) * line_cost[k]) / share) - first + 1;
-    if (tid == 0) {
-      __threadfence();
-      ms.last[k] = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
+  // ---- lines of which other CTAs have parts too
+  if (ms.open[0].base < 0 && ms.open[1].base < 0) return;
+  if (tid < 2) {
+    const auto& o = ms.open[tid];
+    bool last = false;
+    if (o.base >= 0) {
+      const int first = (int)quotient(o.base, share), parts = (int)quotient(o.base + (int64_t)(o.tiles - 1) * o.cost, share) - first + 1;
+      __threadfence();   // (what the other threads wrote, too: the barrier lies between)
+      last = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
       __threadfence();
     }
-    __syncthreads();
+    ms.last[tid] = last;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
     if (!ms.last[k]) continue;
-    const Rows rw = rows_of(p, line_b[k]);
-    for (int r = warp; r < line_rows[k]; r += kThreads / 32) {
-      const int rr = line_u[k] * kPairRows + r, i = rr / G, h = (p.kv_begin + line_kvh[k]) * G + rr - i * G;
+    const auto& line = ms.open[k];
+    const int first = (int)quotient(line.base, share), parts = (int)quotient(line.base + (int64_t)(line.tiles - 1) * line.cost, share) - first + 1;
+    const Rows rw = {line.first_row, line.count};
+    const int b = line.b, kvh = line.kvh;
+    for (int r = warp; r < line.rows; r += kThreads / 32) {
+      const int rr = line.u * kPairRows + r, i = rr / G, h = (p.kv_begin + kvh) * G + rr - i * G;
       float top = kUnset, sum = 0.f;
       constexpr int N = HD / 32;
       float o[N] = {};
@@ -749,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         }
       }
       const float f = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = query_at(p, p.os, rw, line_b[k], h, i);
+      const int64_t at = query_at(p, p.os, rw, b, h, i);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const int64_t to = at + 32 * e + lane;
