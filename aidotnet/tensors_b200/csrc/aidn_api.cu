@@ -947,11 +947,7 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   p.kv_len = a->kv_len;
   p.query_starts = query_starts;
   p.queries = query_starts ? queries : a->batch * a->seq_q;
-#ifdef KV8_TRACE
-  p.mask = a->mask;
-#else
   p.mask = d.mask_kind != AIDN_MASK_NONE ? a->mask : nullptr;
-#endif
   p.mask_kind = d.mask_kind;
   for (int i = 0; i < 4; ++i) p.mask_stride[i] = a->mask_stride[i];
   p.seq_q = a->seq_q;

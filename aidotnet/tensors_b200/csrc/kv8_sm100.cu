@@ -54,8 +54,8 @@ struct Cfg {
   static constexpr int kSmem = kMisc + 2048 + 1024 /* alignment */;
   static constexpr uint32_t kO = 256;                    // accumulators' first column
 };
-// barriers: q_full[2] k_full[2] k_empty[2] v_full[2] v_empty[2] s_full[2][2] p_full[2][2] o_done[2] scales[kRing]
-enum { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 14, kODone = 18, kScales = 20, kBars = 20 + kRing };
+// barriers: q_full[2] k_full[2] k_empty[2] v_full[2] v_empty[2] s_full[2][2] p_full[2][2] o_done[2][2] scales[kRing]
+enum { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 14, kODone = 18, kScales = 22, kBars = 22 + kRing };
 
 struct Misc {
   uint64_t bars[kBars];
@@ -210,10 +210,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
       mbar_init(bar(kKEmpty + i), 1);
       mbar_init(bar(kVFull + i), 4);
       mbar_init(bar(kVEmpty + i), 1);
-      mbar_init(bar(kODone + i), 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kSFull + i), 1);
+      mbar_init(bar(kODone + i), 1);
       mbar_init(bar(kPFull + i), 4);
     }
     ms.open[0].base = ms.open[1].base = -1;
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               eref = emax;
             }
             if (u > 0 && __any_sync(0xffffffffu, keep != 1.f)) {   // (one product at most is on its way, that of the step before: the next needs these weights)
-              if (!mbar_wait(bar(kODone + a), (steps - 1) & 1, abort_flag)) alive = false;
+              if (!mbar_wait(bar(kODone + 2 * a + (buf ^ 1)), (steps - 1) >> 1 & 1, abort_flag)) alive = false;
               tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < HD / 16; ++q) {
@@ -485,9 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           tile_count += buf;
         }
         if (!alive) break;
-        // ---- results.  The last step's scores say that the product of two steps before is done: the one before it may still be on
-        // its way, and a wait tells two phases apart, not three.
-        if (!mbar_wait(bar(kODone + a), (steps - 2) & 1, abort_flag) || !mbar_wait(bar(kODone + a), (steps - 1) & 1, abort_flag)) {
+        // ---- results (a line's last step is one of the second buffer)
+        if (!mbar_wait(bar(kODone + 2 * a + 1), (steps - 1) >> 1 & 1, abort_flag)) {
           alive = false;
           break;
         }
@@ -679,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               if (leader)
                 mma_ts(tmem + C::kO + a * HD, tmem + a * 128 + 64 * buf + k * 8,
                        vd + (uint64_t)((tile & 1) * (C::kTile >> 4)) + (uint64_t)((4 * buf + k) * (2048 >> 4)), idesc_o, u > 0 || k > 0);
-            if (leader) tc_commit(bar(kODone + a));
+            if (leader) tc_commit(bar(kODone + 2 * a + buf));
             if (more) scores(a, tile + 1, buf);
           }
           if (!alive) break;
