@@ -12,7 +12,8 @@
 // Weights are fp16, 11 bits, lifted so that they stay normal down to 2^-18 of the largest.
 //
 //   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
-//                     (16 bits), the running maximum (the accumulator is scaled again only when a logit is 2^8 above it), results
+//                     (16 bits), results.  A row keeps the maximum that it has until sixteen weights sum up to 2^15 (a logit about
+//                     2^8 above it): then it takes the new one, and scales its accumulator
 //   warps 8-11        keys and values: 16-byte loads through the block table, codes to fp16, into rings of two 128-key tiles
 //   warp 12           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V, for 64 keys at a time
 //
@@ -43,7 +44,8 @@ constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kMmaRegs = 48;
 static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kMmaRegs <= kThreads * 128, "registers of the launch");
 constexpr int kRing = 4;              // tiles whose scales are kept
 constexpr float kUnset = -1e30f;
-constexpr float kLazy = 8.f, kRefSlack = 3.f, kLift = 4.f;   // 2^(8 + 3 + 4) is in fp16's range
+constexpr float kLift = 4.f;
+constexpr float kMostWeights = 32768.f;   // of sixteen weights together: each is then in fp16's range
 
 template <int HD>
 struct Cfg {
@@ -61,7 +63,8 @@ struct Misc {
   uint64_t bars[kBars];
   uint32_t tmem;
   int abort;
-  alignas(16) float k_scale[kRing][8], v_exp[kRing][8];   // of a tile's groups of sixteen keys; v_exp -inf: no such keys
+  // of a tile's groups of sixteen keys: scale of the keys, log2 of the values' (-inf: no such keys) and its inverse (then 0)
+  alignas(16) float k_scale[kRing][8], v_exp[kRing][8], v_inverse[kRing][8];
   uint32_t nan_keys[kRing][4];                // keys with a NaN among their values, in tiles of which rows do not see all
   int64_t scan[kThreads / 32];
   int64_t start_base;
@@ -365,31 +368,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         const int lim = valid ? visible(p, w.keys, w.rw.count, i) : 0x7fffffff;
         const int lim_least = visible(p, w.keys, w.rw.count, (w.u * kPairRows + a * kTileRows) / G);
         const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
-        float m = kUnset, l = 0.f, eref = -INFINITY;
+        float m = kUnset, l = 0.f, eref = kUnset, l_unit = 0.f;   // l_unit = 2^(eref - lift): sums of weights over it and the scale are l's
 
         if (!w.whole && tid == 0) {
           auto& o = ms.open[w.t0 == 0 ? 1 : 0];
           o.base = w.base; o.first_row = w.rw.first; o.b = w.b; o.u = w.u; o.kvh = w.kvh;
           o.tiles = w.tiles; o.cost = w.cost; o.rows = w.rows; o.count = w.rw.count;
         }
-        for (int u = 0; u < 2 * n_tiles; ++u, ++steps) {
-          const uint32_t ring = tile_count % kRing, buf = u & 1;   // (a line's steps come in pairs: so does every buffer's phase)
-          // (in this order: once a tile's scores are there, its scales are the next that the ring's slot waits for)
-          if (!mbar_wait(bar(kSFull + 2 * a + buf), steps >> 1 & 1, abort_flag) || !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
+        // The scores of a step are read behind the weights of the one before.
+        uint32_t s[64];
+        auto fetch = [&](uint32_t step) {
+          const uint32_t buf = step & 1;   // (a line's steps come in pairs: so does every buffer's phase)
+          if (!mbar_wait(bar(kSFull + 2 * a + buf), step >> 1 & 1, abort_flag)) return false;
+          tc_fence_after();
+          tmem_ld32(ts0 + 64 * buf, s);
+          tmem_ld32(ts0 + 64 * buf + 32, s + 32);
+          return true;
+        };
+        alive = fetch(steps);
+        for (int u = 0; u < 2 * n_tiles && alive; ++u, ++steps) {
+          const uint32_t ring = tile_count % kRing, buf = u & 1;
+          // (behind the scores: once a tile's scores are there, its scales are the next that the ring's slot waits for)
+          if (buf == 0 && !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
             alive = false;
             break;
           }
-          tc_fence_after();
           const int key0 = (w.t0 + (u >> 1)) * kKeys + 64 * buf;
-          const uint32_t ts = ts0 + 64 * buf;
           auto step = [&](auto edge_t) {
             constexpr bool EDGE = decltype(edge_t)::value;
-            uint32_t s[64];
-            tmem_ld32(ts, s);
-            tmem_ld32(ts + 32, s + 32);
             // of the groups of sixteen keys: factor of the scores, exponent of the weights
             const float4 k4 = *reinterpret_cast<const float4*>(&ms.k_scale[ring][4 * buf]), v4 = *reinterpret_cast<const float4*>(&ms.v_exp[ring][4 * buf]);
             const float ck[4] = {c * k4.x, c * k4.y, c * k4.z, c * k4.w}, e[4] = {v4.x, v4.y, v4.z, v4.w};
+            const float4 i4 = *reinterpret_cast<const float4*>(&ms.v_inverse[ring][4 * buf]);
+            const float inverse[4] = {i4.x, i4.y, i4.z, i4.w};
             tc_wait_ld();
             if constexpr (EDGE) {   // what a row does not see is -inf, a key with a NaN among its values NaN
 #pragma unroll
@@ -402,78 +413,83 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
                 }
               }
             }
-            float top = kUnset, emax = e[0];
+            // The weights are formed with the maximum so far: again if their sum says that they may not fit.
+            float sum;
+            for (;;) {
+              float most = 0.f;
+              sum = 0.f;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint32_t* x = s + 16 * g;
-              float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[8]);
+              for (int q = 0; q < 2; ++q) {
+                uint32_t packed[16];
 #pragma unroll
-              for (int k = 1; k < 7; k += 2) {
-                m0 = fmax3(m0, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                m1 = fmax3(m1, __uint_as_float(x[8 + k]), __uint_as_float(x[9 + k]));
-              }
-              m0 = fmax3(fmaxf(m0, m1), __uint_as_float(x[7]), __uint_as_float(x[15]));
-              float y = m0 * ck[g];
-              if (CAP) y = cap(y, p.softcap, cap_inverse);
-              if (EDGE) y = m0 == -INFINITY ? kUnset : y;   // (a scale of zero times -inf, and the cap of -inf)
-              top = fmaxf(top, e[g] == -INFINITY ? kUnset : y);
-              emax = fmaxf(emax, e[g]);
-            }
-            float keep = 1.f;
-            if (top > m + kLazy) {
-              keep = ex2_approx(m - top);
-              l *= keep;
-              m = top;
-            }
-            if (emax > eref + kRefSlack) {
-              keep *= eref == -INFINITY ? 0.f : ex2_approx(eref - emax);
-              eref = emax;
-            }
-            if (u > 0 && __any_sync(0xffffffffu, keep != 1.f)) {   // (one product at most is on its way, that of the step before: the next needs these weights)
-              if (!mbar_wait(bar(kODone + 2 * a + (buf ^ 1)), (steps - 1) >> 1 & 1, abort_flag)) alive = false;
-              tc_fence_after();
-#pragma unroll 1
-              for (int q = 0; q < HD / 16; ++q) {
-                uint32_t o[16];
-                tmem_ld16(to + 16 * q, o);
-                tc_wait_ld();
+                for (int h2 = 0; h2 < 2; ++h2) {
+                  const int g = 2 * q + h2;
+                  const float off = e[g] - (eref + m - kLift);
+                  const uint64_t ck2 = aidn::pack2(ck[g], ck[g]), off2 = aidn::pack2(off, off);
+                  uint64_t sum_g = 0;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                tmem_st16(to + 16 * q, o);
-              }
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t packed[16];
-#pragma unroll
-              for (int hlf = 0; hlf < 2; ++hlf) {
-                const int g = 2 * q + hlf;
-                const float off = e[g] == -INFINITY ? -INFINITY : e[g] - eref - m + kLift;
-                const uint64_t ck2 = aidn::pack2(ck[g], ck[g]), off2 = aidn::pack2(off, off);
-                uint64_t sum = 0;
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                  const float x = __uint_as_float(s[16 * g + k]), z = __uint_as_float(s[16 * g + k + 1]);
-                  float2 y;
-                  if constexpr (CAP) {
-                    y.x = cap(x * ck[g], p.softcap, cap_inverse) + off;
-                    y.y = cap(z * ck[g], p.softcap, cap_inverse) + off;
-                  } else {
-                    y = unpack2(fma2(aidn::pack2(x, z), ck2, off2));
+                  for (int k = 0; k < 16; k += 2) {
+                    const float u0 = __uint_as_float(s[16 * g + k]), u1 = __uint_as_float(s[16 * g + k + 1]);
+                    float2 y;
+                    if constexpr (CAP) {
+                      y.x = cap(u0 * ck[g], p.softcap, cap_inverse) + off;
+                      y.y = cap(u1 * ck[g], p.softcap, cap_inverse) + off;
+                    } else {
+                      y = unpack2(fma2(aidn::pack2(u0, u1), ck2, off2));
+                    }
+                    y.x = ex2_approx(y.x);
+                    y.y = ex2_approx(y.y);
+                    if constexpr (EDGE) {   // (a scale of zero times -inf, and the cap of -inf)
+                      y.x = u0 == -INFINITY ? 0.f : y.x;
+                      y.y = u1 == -INFINITY ? 0.f : y.y;
+                    }
+                    sum_g = add2(sum_g, aidn::pack2(y.x, y.y));
+                    packed[8 * h2 + (k >> 1)] = ptx::pack2<false>(y.x, y.y);
                   }
-                  y.x = ex2_approx(y.x);
-                  y.y = ex2_approx(y.y);
-                  if constexpr (EDGE) {
-                    y.x = x == -INFINITY ? 0.f : y.x;
-                    y.y = z == -INFINITY ? 0.f : y.y;
-                  }
-                  sum = add2(sum, aidn::pack2(y.x, y.y));
-                  packed[8 * hlf + (k >> 1)] = ptx::pack2<false>(y.x, y.y);
+                  const float part = sum2(sum_g);
+                  most = fmaxf(most, part);
+                  sum = fmaf(part, inverse[g], sum);
                 }
-                l = fmaf(sum2(sum), e[g] == -INFINITY ? 0.f : ex2_approx(eref - e[g] - kLift), l);
+                tmem_st16(ts0 + 64 * buf + 16 * q, packed);
               }
-              tmem_st16(ts + 16 * q, packed);
+              const bool far = most > kMostWeights;
+              if (!__any_sync(0xffffffffu, far)) break;
+              float keep = 1.f;
+              if (far) {
+                float top = m, emax = eref;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  float m0 = __uint_as_float(s[16 * g]);
+#pragma unroll
+                  for (int k = 1; k < 15; k += 2) m0 = fmax3(m0, __uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1]));
+                  m0 = fmaxf(m0, __uint_as_float(s[16 * g + 15]));
+                  float y = m0 * ck[g];
+                  if (CAP) y = cap(y, p.softcap, cap_inverse);
+                  if (e[g] != -INFINITY && m0 != -INFINITY) top = fmaxf(top, y);
+                  emax = fmaxf(emax, e[g]);
+                }
+                const float f = ex2_approx(m - top);
+                keep = f * ex2_approx(eref - emax);
+                l *= f;
+                m = top;
+                eref = emax;
+                l_unit = ex2_approx(eref - kLift);
+              }
+              if (u > 0) {   // (one product at most is on its way, that of the step before: the next needs these weights)
+                if (!mbar_wait(bar(kODone + 2 * a + (buf ^ 1)), (steps - 1) >> 1 & 1, abort_flag)) alive = false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int q = 0; q < HD / 16; ++q) {
+                  uint32_t o[16];
+                  tmem_ld16(to + 16 * q, o);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                  tmem_st16(to + 16 * q, o);
+                }
+              }
             }
+            l = fmaf(sum, l_unit, l);
           };
           if (key0 + 64 > lim_least || key0 + 64 > w.keys) step(std::true_type{});   // (uniform)
           else step(std::false_type{});
@@ -481,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(kPFull + 2 * a + buf));
-          if (!alive) break;
+          if (u + 1 < 2 * n_tiles) alive = alive && fetch(steps + 1);
           tile_count += buf;
         }
         if (!alive) break;
@@ -491,8 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           break;
         }
         tc_fence_after();
-        const float unit = eref == -INFINITY ? 0.f : ex2_approx(eref - kLift);
-        const float f = w.whole ? (l == 0.f ? 0.f : unit / l) : unit;
+        const float f = w.whole ? (l == 0.f ? 0.f : l_unit / l) : l_unit;
         const int slot = 2 * (int)blockIdx.x + (w.t0 == 0 ? 1 : 0), prow = a * kTileRows + row_in;
         const int64_t at = w.whole ? query_at(p, p.os, w.rw, w.b, h, i) : ((int64_t)slot * kPairRows + prow) * HD;
 #pragma unroll
@@ -614,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
             if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
             ms.k_scale[ring][2 * quarter + lane] = ks;
             ms.v_exp[ring][2 * quarter + lane] = before < 0 ? -INFINITY : exponent;
+            ms.v_inverse[ring][2 * quarter + lane] = before < 0 ? 0.f : ex2_approx(-exponent);
           }
           if (lane == 0) ms.nan_keys[ring][quarter] = nan;
           convert(dst0 + C::kV + stage * C::kTile, xv);
