@@ -972,7 +972,7 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   int launches = 1;
   cudaError_t e;
   if (d.path != AIDN_PATH_GENERIC && p.seq_q * p.group > aidn::kv8::kFewRows && aidn::kv8::sm100_supported(p)) {
-    e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);
+    e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);
     h->last_path = AIDN_PATH_PREFILL_SM100;
   } else if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
     e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);

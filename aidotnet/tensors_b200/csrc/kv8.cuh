@@ -11,7 +11,7 @@ constexpr float kLargestCode = 448.f;
 constexpr int kCounters = 2048;
 
 // Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 3;
 
 constexpr int kLeastExponent = -100, kMostExponent = 119;   // of a scale: 448 * 2^119 is below the largest float
 
@@ -158,7 +158,8 @@ cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, i
 // Many queries of 16 bits (csrc/kv8_sm100.cu): head sizes 64 and 128, blocks of a multiple of 16 tokens, 16-byte aligned pools, no mask.
 bool sm100_supported(const Attend& p);
 int64_t sm100_workspace_bytes(int head_dim, int num_sms);
-cudaError_t launch_attend_sm100(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream);
+cudaError_t launch_attend_sm100(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, int* launches,
+                                cudaStream_t stream);
 
 }  // namespace kv8
 }  // namespace aidn

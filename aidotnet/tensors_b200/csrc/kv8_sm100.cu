@@ -20,8 +20,9 @@
 // Tensor memory: two score buffers of 64 columns for each row tile (P in the first half of each), O_0 | O_1.  The scores of 64 keys
 // are formed while the softmax works on the 64 before: with one buffer of 128 keys a tile the chain softmax -> P V -> next scores
 // was the period, 4500 to 5300 cycles for 128 keys where the products take 2050 and the softmax 2900.  The tiles of all lines are one row that is cut into
-// equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice); parts of cut lines meet in the
-// workspace as in kv8_split.cu, merged by the CTA that arrives last.
+// equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice).  A line that is cut leaves one
+// partial result a CTA in the workspace, and the CTA in which it begins a note about it, from which a second launch merges them:
+// 256 rows of up to 148 parts take one CTA 25 to 80 us (measured, merged by the last CTA to arrive), spread over all SMs 4 to 8.
 #include <type_traits>
 
 #include "ffma2.cuh"
@@ -69,9 +70,6 @@ struct Misc {
   int64_t scan[kThreads / 32];
   int64_t start_base;
   int start_b, start_u;
-  int last[2];
-  // the lines of which other CTAs have parts too (base -1: none): the one that began before this share, the one that goes on
-  struct { int64_t base, first_row; int b, u, kvh, tiles, cost, rows, count; } open[2];
 };
 static_assert(sizeof(Misc) <= 2048, "");
 
@@ -80,9 +78,15 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
+// A line that begins in a CTA's share and goes on behind it: in how many CTAs it has parts (0: there is none).
+struct Note {
+  int64_t first_row;
+  int b, kvh, row, rows, parts;
+};
 struct Cut {
   float* partial;   // [2 grid][256][HD], or null: lines are not cut
   float2* stats;    // [2 grid][256]: maximum and sum
+  Note* notes;      // [grid]
   bool query_vec, out_vec;
 };
 
@@ -219,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
       mbar_init(bar(kODone + i), 1);
       mbar_init(bar(kPFull + i), 4);
     }
-    ms.open[0].base = ms.open[1].base = -1;
     for (int i = 0; i < kRing; ++i) mbar_init(bar(kScales + i), 4);
     fence_mbar_init();
   }
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   };
   bool alive = pos < end;
   bool bad = false;
+  if (is_cut && tid == 0) cut.notes[blockIdx.x].parts = 0;
 
   if (warp < kConvertWarp) {
     // ================================================= softmax =================================================
@@ -370,10 +374,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
         float m = kUnset, l = 0.f, eref = kUnset, l_unit = 0.f;   // l_unit = 2^(eref - lift): sums of weights over it and the scale are l's
 
-        if (!w.whole && tid == 0) {
-          auto& o = ms.open[w.t0 == 0 ? 1 : 0];
-          o.base = w.base; o.first_row = w.rw.first; o.b = w.b; o.u = w.u; o.kvh = w.kvh;
-          o.tiles = w.tiles; o.cost = w.cost; o.rows = w.rows; o.count = w.rw.count;
+        if (!w.whole && w.t0 == 0 && tid == 0) {
+          const int parts = (int)quotient(w.base + (int64_t)(w.tiles - 1) * w.cost, share) - (int)blockIdx.x + 1;
+          cut.notes[blockIdx.x] = {w.rw.first, w.b, w.kvh, w.u * kPairRows, w.rows, parts};
         }
         // The scores of a step are read behind the weights of the one before.
         uint32_t s[64];
@@ -725,77 +728,78 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (!is_cut || gave_up || pos >= end) return;
+}
 
-  // ---- lines of which other CTAs have parts too
-  if (ms.open[0].base < 0 && ms.open[1].base < 0) return;
-  if (tid < 2) {
-    const auto& o = ms.open[tid];
-    bool last = false;
-    if (o.base >= 0) {
-      const int first = (int)quotient(o.base, share), parts = (int)quotient(o.base + (int64_t)(o.tiles - 1) * o.cost, share) - first + 1;
-      __threadfence();   // (what the other threads wrote, too: the barrier lies between)
-      last = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
-      __threadfence();
+// CTA (c, i): 32 rows of the line that begins in the share of CTA c and goes on behind it, a warp four of them.
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_sm100_merge_kernel(const __grid_constant__ Attend p, const Cut cut) {
+  pdl_wait();
+  pdl_trigger();
+  const Note note = cut.notes[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = 32 * blockIdx.y + 4 * warp;
+  if (note.parts == 0 || r0 >= note.rows) return;
+  constexpr int N = HD / 32;
+  float top[4], sum[4] = {}, o[4][N] = {};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) top[r] = kUnset;
+  for (int q = 0; q < note.parts; q += 4) {
+    float2 st[4][4];
+    float v[4][4][N];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int part = min(q + x, note.parts - 1);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t from = (int64_t)(2 * (blockIdx.x + part) + (part == 0)) * kPairRows + min(r0 + r, note.rows - 1);
+        st[x][r] = cut.stats[from];
+        const float* at = cut.partial + from * HD + N * lane;
+        if constexpr (N == 4) {
+          const float4 u = *reinterpret_cast<const float4*>(at);
+          v[x][r][0] = u.x; v[x][r][1] = u.y; v[x][r][2] = u.z; v[x][r][3] = u.w;
+        } else {
+          const float2 u = *reinterpret_cast<const float2*>(at);
+          v[x][r][0] = u.x; v[x][r][1] = u.y;
+        }
+      }
     }
-    ms.last[tid] = last;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float now = top[r];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x][r].x);
+      const float keep = ex2_approx(top[r] - now);
+      top[r] = now;
+      sum[r] *= keep;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[r][e] *= keep;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (q + x >= note.parts) continue;
+        const float f = ex2_approx(st[x][r].x - now);
+        sum[r] += f * st[x][r].y;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[r][e] += f * v[x][r][e];
+      }
+    }
   }
-  __syncthreads();
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    if (!ms.last[k]) continue;
-    const auto& line = ms.open[k];
-    const int first = (int)quotient(line.base, share), parts = (int)quotient(line.base + (int64_t)(line.tiles - 1) * line.cost, share) - first + 1;
-    const Rows rw = {line.first_row, line.count};
-    const int b = line.b, kvh = line.kvh;
-    for (int r = warp; r < line.rows; r += kThreads / 32) {
-      const int rr = line.u * kPairRows + r, i = rr / G, h = (p.kv_begin + kvh) * G + rr - i * G;
-      float top = kUnset, sum = 0.f;
-      constexpr int N = HD / 32;
-      float o[N] = {};
-      for (int q = 0; q < parts; q += 4) {
-        float2 st[4];
-        float v[4][N];
+  const Rows rw = {note.first_row, 0};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int part = min(q + x, parts - 1);
-          const int64_t from = (int64_t)(2 * (first + part) + (part == 0)) * kPairRows + r;
-          st[x] = __ldcg(cut.stats + from);
+  for (int r = 0; r < 4; ++r) {
+    if (r0 + r >= note.rows) continue;
+    const int row = note.row + r0 + r, i = row / p.group, h = (p.kv_begin + note.kvh) * p.group + row - i * p.group;
+    const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+    const int64_t at = query_at(p, p.os, rw, note.b, h, i) + N * lane;
 #pragma unroll
-          for (int e = 0; e < N; ++e) v[x][e] = __ldcg(cut.partial + from * HD + 32 * e + lane);
-        }
-        float now = top;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x].x);
-        const float keep = ex2_approx(top - now);
-        top = now;
-        sum *= keep;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] *= keep;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (q + x >= parts) continue;
-          const float f = ex2_approx(st[x].x - top);
-          sum += f * st[x].y;
-#pragma unroll
-          for (int e = 0; e < N; ++e) o[e] += f * v[x][e];
-        }
-      }
-      const float f = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = query_at(p, p.os, rw, b, h, i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int64_t to = at + 32 * e + lane;
-        if (p.dtype == AIDN_F16) static_cast<__half*>(p.out)[to] = __float2half_rn(o[e] * f);
-        else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(o[e] * f);
-      }
-      if (p.lse && lane == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    for (int e = 0; e < N; ++e) {
+      if (p.dtype == AIDN_F16) static_cast<__half*>(p.out)[at + e] = __float2half_rn(o[r][e] * f);
+      else static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(o[r][e] * f);
     }
+    if (p.lse && lane == 0) *lse_at(p, rw, h, i) = sum[r] == 0.f ? -INFINITY : (top[r] + log2f(sum[r])) * kLn2;
   }
 }
 
 template <int HD, bool CAP>
-cudaError_t launch(const Attend& p, int grid, const Cut& cut, uint64_t* raised, cudaStream_t stream) {
+cudaError_t launch(const Attend& p, int grid, const Cut& cut, uint64_t* raised, int* launches, cudaStream_t stream) {
   auto k = kv8_sm100_kernel<HD, CAP>;
   const int id = 60 + (HD == 128 ? 2 : 0) + (CAP ? 1 : 0);
   if (!(*raised >> id & 1)) {
@@ -803,7 +807,12 @@ cudaError_t launch(const Attend& p, int grid, const Cut& cut, uint64_t* raised, 
     if (e != cudaSuccess) return e;
     *raised |= 1ull << id;
   }
-  return launch_dependent(k, dim3((unsigned)grid), kThreads, Cfg<HD>::kSmem, stream, p, cut);
+  const cudaError_t e = launch_dependent(k, dim3((unsigned)grid), kThreads, Cfg<HD>::kSmem, stream, p, cut);
+  if (e != cudaSuccess || !cut.partial) return e;
+  const int64_t rows = p.seq_q * p.group;
+  const unsigned slices = (unsigned)((rows < kPairRows ? rows : kPairRows) + 31) / 32;
+  ++*launches;
+  return launch_dependent(kv8_sm100_merge_kernel<HD>, dim3((unsigned)grid, slices), 256, 0, stream, p, cut);
 }
 
 }  // namespace
@@ -815,19 +824,20 @@ bool sm100_supported(const Attend& p) {
     if (p.c.stride[i] % 16 != 0) return false;
   return p.seq_q * p.group < 0x7fffffff - kPairRows;
 }
-int64_t sm100_workspace_bytes(int head_dim, int num_sms) { return (int64_t)2 * num_sms * kPairRows * (head_dim * 4 + 8); }
+int64_t sm100_workspace_bytes(int head_dim, int num_sms) { return (int64_t)2 * num_sms * kPairRows * (head_dim * 4 + 8) + num_sms * (int64_t)sizeof(Note); }
 
-cudaError_t launch_attend_sm100(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream) {
-  const int grid = num_sms < kCounters ? num_sms : kCounters;
+cudaError_t launch_attend_sm100(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  const int grid = num_sms;
   if (workspace_bytes < sm100_workspace_bytes(p.c.head_dim, grid) || (uintptr_t)workspace % 16 != 0) workspace = nullptr;
   Cut cut;
   cut.partial = static_cast<float*>(workspace);
   cut.stats = workspace ? reinterpret_cast<float2*>(cut.partial + (int64_t)2 * grid * kPairRows * p.c.head_dim) : nullptr;
+  cut.notes = workspace ? reinterpret_cast<Note*>(cut.stats + (int64_t)2 * grid * kPairRows) : nullptr;
   auto vec = [](const void* ptr, const int64_t* st) { return ((uintptr_t)ptr | (uint64_t)(st[0] * 2) | (uint64_t)(st[1] * 2) | (uint64_t)(st[2] * 2)) % 16 == 0; };
   cut.query_vec = vec(p.q, p.qs);
   cut.out_vec = vec(p.out, p.os);
-  if (p.c.head_dim == 64) return p.softcap > 0.f ? launch<64, true>(p, grid, cut, raised, stream) : launch<64, false>(p, grid, cut, raised, stream);
-  return p.softcap > 0.f ? launch<128, true>(p, grid, cut, raised, stream) : launch<128, false>(p, grid, cut, raised, stream);
+  if (p.c.head_dim == 64) return p.softcap > 0.f ? launch<64, true>(p, grid, cut, raised, launches, stream) : launch<64, false>(p, grid, cut, raised, launches, stream);
+  return p.softcap > 0.f ? launch<128, true>(p, grid, cut, raised, launches, stream) : launch<128, false>(p, grid, cut, raised, launches, stream);
 }
 
 }  // namespace kv8
