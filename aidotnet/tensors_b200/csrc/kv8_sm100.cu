@@ -23,6 +23,7 @@
 // equal shares for the CTAs, one an SM (a 128-key tile of a line with two row tiles counts twice).  A line that is cut leaves one
 // partial result a CTA in the workspace, and the CTA in which it begins a note about it, from which a second launch merges them:
 // 256 rows of up to 148 parts take one CTA 25 to 80 us (measured, merged by the last CTA to arrive), spread over all SMs 4 to 8.
+#include <cstddef>
 #include <type_traits>
 
 #include "ffma2.cuh"
@@ -65,8 +66,11 @@ struct Misc {
   uint32_t tmem;
   int abort;
   // of a tile's groups of sixteen keys: scale of the keys, log2 of the values' (-inf: no such keys) and its inverse (then 0)
-  alignas(16) float k_scale[kRing][8], v_exp[kRing][8], v_inverse[kRing][8];
-  uint32_t nan_keys[kRing][4];                // keys with a NaN among their values, in tiles of which rows do not see all
+  struct Scales {
+    alignas(16) float k[8];
+    float v_exp[8], v_inverse[8];
+    uint32_t nan[4];   // keys with a NaN among their values, in tiles of which rows do not see all
+  } scales[kRing];
   int64_t scan[kThreads / 32];
   int64_t start_base;
   int start_b, start_u;
@@ -154,6 +158,16 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float log2_approx(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -208,7 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   volatile int* const abort_flag = &ms.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
   const uint32_t base = smem_u32(smem);
-  auto bar = [&](int i) { return smem_u32(&ms.bars[i]); };
+  const uint32_t bars = base + C::kMisc + (uint32_t)offsetof(Misc, bars), scales_at = base + C::kMisc + (uint32_t)offsetof(Misc, scales);
+  auto bar = [&](uint32_t i) { return bars + 8 * i; };
   if (tid == 0) {
     ms.abort = 0;
     for (int i = 0; i < 2; ++i) {
@@ -378,37 +393,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           const int parts = (int)quotient(w.base + (int64_t)(w.tiles - 1) * w.cost, share) - (int)blockIdx.x + 1;
           cut.notes[blockIdx.x] = {w.rw.first, w.b, w.kvh, w.u * kPairRows, w.rows, parts};
         }
-        // The scores of a step are read behind the weights of the one before.
+        // The scores of a step are read as soon as the weights of the one before are formed; if they are there, beside the storing of those.
         uint32_t s[64];
-        auto fetch = [&](uint32_t step) {
-          const uint32_t buf = step & 1;   // (a line's steps come in pairs: so does every buffer's phase)
-          if (!mbar_wait(bar(kSFull + 2 * a + buf), step >> 1 & 1, abort_flag)) return false;
+        auto fetch = [&](uint32_t buf) {
           tc_fence_after();
           tmem_ld32(ts0 + 64 * buf, s);
           tmem_ld32(ts0 + 64 * buf + 32, s + 32);
-          return true;
         };
-        alive = fetch(steps);
+        // (a line's steps come in pairs: so does every buffer's phase)
+        alive = mbar_wait(bar(kSFull + 2 * a), steps >> 1 & 1, abort_flag);
+        fetch(0);
+        // Its scales, of four groups of sixteen keys: factors of the scores, exponents of the weights and their inverses.  (Waited for behind
+        // the first scores: once a tile's are there, its scales are the next that the ring's slot waits for.)
+        float4 k4, v4, i4;
+        auto scales = [&](uint32_t tile, uint32_t buf) {
+          const uint32_t at = scales_at + tile % kRing * (uint32_t)sizeof(Misc::Scales) + 16 * buf;
+          k4 = ld_shared_f4(at);
+          v4 = ld_shared_f4(at + 32);
+          i4 = ld_shared_f4(at + 64);
+        };
+        alive = alive && mbar_wait(bar(kScales + tile_count % kRing), tile_count / kRing & 1, abort_flag);
+        scales(tile_count, 0);
         for (int u = 0; u < 2 * n_tiles && alive; ++u, ++steps) {
-          const uint32_t ring = tile_count % kRing, buf = u & 1;
-          // (behind the scores: once a tile's scores are there, its scales are the next that the ring's slot waits for)
-          if (buf == 0 && !mbar_wait(bar(kScales + ring), tile_count / kRing & 1, abort_flag)) {
-            alive = false;
-            break;
-          }
+          const uint32_t buf = u & 1, next = buf ^ 1;
+          const bool more = u + 1 < 2 * n_tiles;
+          const uint32_t next_bar = bar(kSFull + 2 * a + next), next_phase = (steps + 1) >> 1 & 1;
+          const uint32_t next_tile = tile_count + buf, scales_bar = bar(kScales + next_tile % kRing), scales_phase = next_tile / kRing & 1;
+          bool scored = false, scaled = false;   // whether the next step's scores and scales are there
           const int key0 = (w.t0 + (u >> 1)) * kKeys + 64 * buf;
           auto step = [&](auto edge_t) {
             constexpr bool EDGE = decltype(edge_t)::value;
-            // of the groups of sixteen keys: factor of the scores, exponent of the weights
-            const float4 k4 = *reinterpret_cast<const float4*>(&ms.k_scale[ring][4 * buf]), v4 = *reinterpret_cast<const float4*>(&ms.v_exp[ring][4 * buf]);
             const float ck[4] = {c * k4.x, c * k4.y, c * k4.z, c * k4.w}, e[4] = {v4.x, v4.y, v4.z, v4.w};
-            const float4 i4 = *reinterpret_cast<const float4*>(&ms.v_inverse[ring][4 * buf]);
             const float inverse[4] = {i4.x, i4.y, i4.z, i4.w};
             tc_wait_ld();
             if constexpr (EDGE) {   // what a row does not see is -inf, a key with a NaN among its values NaN
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const uint32_t nan = ms.nan_keys[ring][2 * buf + q];
+                const uint32_t nan = ld_shared_u32(scales_at + tile_count % kRing * (uint32_t)sizeof(Misc::Scales) + 96 + 8 * buf + 4 * q);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                   if (nan >> k & 1) s[32 * q + k] = 0x7fffffffu;
@@ -423,6 +444,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               sum = 0.f;
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
+                if (q == 1) {   // (looked at beside the arithmetic: shared memory is busy with the products' operands, and answers in 200 cycles)
+                  scored = mbar_test(next_bar, next_phase);
+                  scaled = mbar_test(scales_bar, scales_phase);
+                }
                 uint32_t packed[16];
 #pragma unroll
                 for (int h2 = 0; h2 < 2; ++h2) {
@@ -496,11 +521,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           };
           if (key0 + 64 > lim_least || key0 + 64 > w.keys) step(std::true_type{});   // (uniform)
           else step(std::false_type{});
+          scored = __all_sync(0xffffffffu, scored) && more;
+          scaled = __all_sync(0xffffffffu, scaled) && more;
+          if (scaled) scales(next_tile, next);
+          if (scored) fetch(next);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(kPFull + 2 * a + buf));
-          if (u + 1 < 2 * n_tiles) alive = alive && fetch(steps + 1);
+          if (more && !scored) {
+            alive = alive && mbar_wait(next_bar, next_phase, abort_flag);
+            fetch(next);
+          }
+          if (more && !scaled) {
+            alive = alive && mbar_wait(scales_bar, scales_phase, abort_flag);
+            scales(next_tile, next);
+          }
           tile_count += buf;
         }
         if (!alive) break;
@@ -630,11 +666,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           if (lane < 2) {
             float exponent = log2_approx(vs);
             if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
-            ms.k_scale[ring][2 * quarter + lane] = ks;
-            ms.v_exp[ring][2 * quarter + lane] = before < 0 ? -INFINITY : exponent;
-            ms.v_inverse[ring][2 * quarter + lane] = before < 0 ? 0.f : ex2_approx(-exponent);
+            Misc::Scales& sc = ms.scales[ring];
+            sc.k[2 * quarter + lane] = ks;
+            sc.v_exp[2 * quarter + lane] = before < 0 ? -INFINITY : exponent;
+            sc.v_inverse[2 * quarter + lane] = before < 0 ? 0.f : ex2_approx(-exponent);
           }
-          if (lane == 0) ms.nan_keys[ring][quarter] = nan;
+          if (lane == 0) ms.scales[ring].nan[quarter] = nan;
           convert(dst0 + C::kV + stage * C::kTile, xv);
           if (lane == 0) {
             mbar_arrive(bar(kVFull + stage));
