@@ -11,7 +11,7 @@ constexpr float kLargestCode = 448.f;
 constexpr int kCounters = 2048;
 
 // Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one.
-constexpr int kFewRows = 3;
+constexpr int kFewRows = 32;
 
 constexpr int kLeastExponent = -100, kMostExponent = 119;   // of a scale: 448 * 2^119 is below the largest float
 

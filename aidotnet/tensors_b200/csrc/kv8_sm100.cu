@@ -163,6 +163,11 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -182,37 +187,11 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   const uint32_t hit = (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
   return x & ~(hit * 0xffu);
 }
-// Eight 16-bit elements of the queries as they lie, and two of them as floats.
-__device__ __forceinline__ void query8(const Attend& p, int64_t at, bool vec, uint32_t* w) {
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
-  if (vec) {
-    const uint4 v = *reinterpret_cast<const uint4*>(q);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
-  }
-}
+// Two 16-bit elements of the queries as floats.
 __device__ __forceinline__ float2 widen2(const Attend& p, uint32_t w) {
   if (p.dtype == AIDN_F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-__device__ __forceinline__ void store8(const Attend& p, int64_t at, bool vec, const float* x) {
-  uint16_t* to = static_cast<uint16_t*>(p.out) + at;
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = p.dtype == AIDN_F16 ? ptx::pack2<false>(x[2 * e], x[2 * e + 1]) : ptx::pack2<true>(x[2 * e], x[2 * e + 1]);
-  if (vec) {
-    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      to[2 * e] = (uint16_t)w[e];
-      to[2 * e + 1] = (uint16_t)(w[e] >> 16);
-    }
-  }
-}
-
 template <int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_constant__ Attend p, const Cut cut) {
   using C = Cfg<HD>;
@@ -350,35 +329,52 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         const int r = w.u * kPairRows + a * kTileRows + row_in;
         const bool valid = a * kTileRows + row_in < w.rows;
         const int i = valid ? r / G : 0, h = (p.kv_begin + w.kvh) * G + (valid ? r - i * G : 0);
-        // ---- this row's query: scaled by a power of two so that the largest element is in [2^8, 2^9)
+        // ---- this warp's 32 queries: HD / 8 lanes a row, scaled by a power of two so that the largest element is in [2^8, 2^9)
+        constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;   // lanes of a row, rows of a load
+        const int sub = lane / kLanes, chunk = lane % kLanes;
+        const int warp_row = (warp & 3) * 32, warp_rows = min(32, w.rows - a * kTileRows - warp_row);   // (may be negative)
         float c;
         {
-          const int64_t at = query_at(p, p.qs, w.rw, w.b, h, i);
-          uint32_t x[HD / 2];
-          if (valid) {
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j) query8(p, at + 8 * j, cut.query_vec, x + 4 * j);
+          // (loops, not unrolled: code that runs once a line costs its fetch from memory, 40 us over a step of 24 sequences)
+          const uint32_t tile = base + C::kQ + a * C::kTile + warp_row * 128;
+          const int first = w.u * kPairRows + a * kTileRows + warp_row;
+#pragma unroll 2
+          for (int j = 0; j < HD / 8; ++j) {
+            const int row = j * kAtOnce + sub, qi = (first + row) / G, gh = (first + row) - qi * G;
+            const uint32_t dst = tile + (chunk >> 3) * C::kSlab + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+            uint32_t x[4] = {0, 0, 0, 0};
+            if (row < warp_rows) {
+              const uint16_t* q = static_cast<const uint16_t*>(p.q) + query_at(p, p.qs, w.rw, w.b, (p.kv_begin + w.kvh) * G + gh, qi) + 8 * chunk;
+              if (cut.query_vec) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(q) : "memory");
+                continue;
+              }
+              for (int e = 0; e < 4; ++e) x[e] = q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
+            }
+            st_shared_v4(dst, x[0], x[1], x[2], x[3]);
           }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+          // a thread its own row
+          auto piece = [&](int j) { return tile + (j >> 3) * C::kSlab + lane * 128 + (((j & 7) ^ (lane & 7)) << 4); };
           float largest = 0.f;
-#pragma unroll
-          for (int j = 0; j < HD / 2; ++j) {
-            if (!valid) x[j] = 0;
-            const float2 y = widen2(p, x[j]);
-            largest = fmaxf(largest, fmaxf(fabsf(y.x), fabsf(y.y)));
+#pragma unroll 2
+          for (int j = 0; j < HD / 8; ++j) {
+            const uint4 x = ld_shared_v4(piece(j));
+            const float2 y0 = widen2(p, x.x), y1 = widen2(p, x.y), y2 = widen2(p, x.z), y3 = widen2(p, x.w);
+            largest = fmaxf(largest, fmaxf(fmaxf(fmaxf(fabsf(y0.x), fabsf(y0.y)), fmaxf(fabsf(y1.x), fabsf(y1.y))),
+                                           fmaxf(fmaxf(fabsf(y2.x), fabsf(y2.y)), fmaxf(fabsf(y3.x), fabsf(y3.y)))));
           }
           int up = 8 - ((int)(__float_as_uint(largest) >> 23) - 127);
           up = max(-110, min(up, 126));
           const float f = __uint_as_float((uint32_t)(up + 127) << 23);
           c = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (CAP ? 1.f : kLog2e);
-          const uint32_t dst = base + C::kQ + a * C::kTile + row_in * 128;
-#pragma unroll
+#pragma unroll 2
           for (int j = 0; j < HD / 8; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 y = widen2(p, x[4 * j + e]);
-              x[4 * j + e] = ptx::pack2<false>(y.x * f, y.y * f);
-            }
-            st_shared_v4(dst + (j >> 3) * C::kSlab + (((j & 7) ^ (row_in & 7)) << 4), x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+            const uint4 x = ld_shared_v4(piece(j));
+            const float2 y0 = widen2(p, x.x), y1 = widen2(p, x.y), y2 = widen2(p, x.z), y3 = widen2(p, x.w);
+            st_shared_v4(piece(j), ptx::pack2<false>(y0.x * f, y0.y * f), ptx::pack2<false>(y1.x * f, y1.y * f), ptx::pack2<false>(y2.x * f, y2.y * f),
+                         ptx::pack2<false>(y3.x * f, y3.y * f));
           }
         }
         fence_proxy_async_smem();
@@ -547,22 +543,72 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         }
         tc_fence_after();
         const float f = w.whole ? (l == 0.f ? 0.f : l_unit / l) : l_unit;
+        // Rows go out through this warp's part of the queries' tile, which nothing reads any more: 256 bytes a row at a time, lanes along rows.
         const int slot = 2 * (int)blockIdx.x + (w.t0 == 0 ? 1 : 0), prow = a * kTileRows + row_in;
-        const int64_t at = w.whole ? query_at(p, p.os, w.rw, w.b, h, i) : ((int64_t)slot * kPairRows + prow) * HD;
+        const uint32_t stage = base + C::kQ + a * C::kTile + warp_row * 128;
+        constexpr int kSlabs = HD / 64;
+        auto put = [&](int at16, uint32_t x, uint32_t y, uint32_t z, uint32_t v) {   // sixteen bytes of this thread's row
+          st_shared_v4(stage + (at16 >> 3) * C::kSlab + lane * 128 + (((at16 & 7) ^ (lane & 7)) << 4), x, y, z, v);
+        };
+        auto rows_out = [&](auto&& store) {   // store(row, sixteen bytes' number, them)
+          __syncwarp();
+          constexpr int kOut = 8 * kSlabs, kRowsAtOnce = 32 / kOut;
+          const int at16 = lane % kOut, s2 = lane / kOut;
+#pragma unroll 2
+          for (int j = 0; j < 32 / kRowsAtOnce; ++j) {
+            const int row = j * kRowsAtOnce + s2;
+            const uint4 v = ld_shared_v4(stage + (at16 >> 3) * C::kSlab + row * 128 + (((at16 & 7) ^ (row & 7)) << 4));
+            if (row < warp_rows) store(row, at16, v);
+          }
+          __syncwarp();
+        };
+        if (w.whole) {
+#pragma unroll 1
+          for (int q = 0; q < HD / 32; ++q) {
+            uint32_t x[32];
+            tmem_ld32(to + 32 * q, x);
+            tc_wait_ld();
 #pragma unroll
-        for (int q = 0; q < HD / 32; ++q) {
-          uint32_t x[32];
-          tmem_ld32(to + 32 * q, x);
-          tc_wait_ld();
-          float y[32];
+            for (int e = 0; e < 32; e += 2) {
+              const float y = __uint_as_float(x[e]) * f, z = __uint_as_float(x[e + 1]) * f;
+              x[e / 2] = p.dtype == AIDN_F16 ? ptx::pack2<false>(y, z) : ptx::pack2<true>(y, z);
+            }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(x[e]) * f;
-          if (valid && w.whole) {
+            for (int e = 0; e < 4; ++e) put(4 * q + e, x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+          }
+          const int first = w.u * kPairRows + a * kTileRows + warp_row;
+          rows_out([&](int row, int at16, uint4 v) {
+            const int qi = (first + row) / G, gh = (first + row) - qi * G;
+            const int64_t at = query_at(p, p.os, w.rw, w.b, (p.kv_begin + w.kvh) * G + gh, qi) + 8 * at16;
+            uint16_t* const dst = static_cast<uint16_t*>(p.out) + at;
+            if (cut.out_vec) {
+              *reinterpret_cast<uint4*>(dst) = v;
+            } else {
+              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) store8(p, at + 32 * q + e, cut.out_vec, y + e);
-          } else if (valid) {
+              for (int e = 0; e < 4; ++e) {
+                dst[2 * e] = (uint16_t)words[e];
+                dst[2 * e + 1] = (uint16_t)(words[e] >> 16);
+              }
+            }
+          });
+        } else {
+          float* const part = cut.partial + ((int64_t)slot * kPairRows + a * kTileRows + warp_row) * HD;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {   // HD / 2 floats: as many bytes as a row of queries
+#pragma unroll 1
+            for (int q = 0; q < HD / 64; ++q) {
+              uint32_t x[32];
+              tmem_ld32(to + half * (HD / 2) + 32 * q, x);
+              tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) __stcg(reinterpret_cast<float4*>(cut.partial + at + 32 * q + e), make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]));
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) put(8 * q + e, x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            }
+            rows_out([&](int row, int at16, uint4 v) {
+              __stcg(reinterpret_cast<uint4*>(part + (int64_t)row * HD + half * (HD / 2) + 4 * at16), v);
+            });
           }
         }
         if (valid && w.whole && p.lse) *lse_at(p, w.rw, h, i) = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
