@@ -82,11 +82,11 @@ class KvCacheFp8:
         self.keys, self.values, self.keyScales, self.valueScales = keys, values, keyScales, valueScales
         self.blockSize, self.kvHeads, self.headDim = blockSize, kvHeads, headDim
 
-    def _pack(self, blockTables: GpuBuffer, blocksPerSeq: int) -> bytes:
-        return N.kv8_cache(key_pool=self.keys.tensor.data_ptr(), value_pool=self.values.tensor.data_ptr(),
-                           key_scale=self.keyScales.tensor.data_ptr(), value_scale=self.valueScales.tensor.data_ptr(),
-                           block_table=blockTables.tensor.data_ptr(), block_table_stride=blocksPerSeq, num_blocks=self.numBlocks,
-                           block_size=self.blockSize, kv_heads=self.kvHeads, head_dim=self.headDim)
+    def _pack(self, table: int, blocksPerSeq: int) -> bytes:
+        """The ``aidn_kv8_cache`` block, packed in one go (a decode step waits for this code, not for the GPU)."""
+        return N._KV8_CACHE.pack(self.keys.tensor.data_ptr(), self.values.tensor.data_ptr(), self.keyScales.tensor.data_ptr(),
+                                 self.valueScales.tensor.data_ptr(), table, blocksPerSeq, 0, 0, 0, self.numBlocks, self.blockSize,
+                                 self.kvHeads, self.headDim)
 
 
 class CudaBackend:
@@ -449,13 +449,13 @@ class CudaBackend:
     def _check_kv8(op, table, batch, columns, lens, starts, tokens):
         if batch <= 0 or columns <= 0:
             raise ValueError(f"{op}: batch and blocksPerSeq must be > 0")
-        t, n = table.tensor, lens.tensor
-        if t.numel() < batch * columns or n.numel() < batch or t.dtype != torch.int32 or n.dtype != torch.int32:
+        if table.numel() < batch * columns or lens.numel() < batch or table.dtype != torch.int32 or lens.dtype != torch.int32:
             raise ValueError(f"{op}: block tables or lengths are too small or not int32")
-        if starts is not None and (starts.tensor.numel() < batch + 1 or starts.tensor.dtype != torch.int32):
+        if starts is None:
+            if tokens % batch != 0:
+                raise ValueError(f"{op}: {tokens} tokens are not the same number for each of {batch} sequences")
+        elif starts.tensor.numel() < batch + 1 or starts.tensor.dtype != torch.int32:
             raise ValueError(f"{op}: the first tokens must be int32 [batch + 1]")
-        if starts is None and tokens % batch != 0:
-            raise ValueError(f"{op}: {tokens} tokens are not the same number for each of {batch} sequences")
 
     def PagedKvAppendFp8(self, qkv: GpuBuffer, queries: Optional[GpuBuffer], cache: KvCacheFp8, blockTables: GpuBuffer,
                          startLens: GpuBuffer, batch: int, tokens: int, heads: int, blocksPerSeq: int,
@@ -469,31 +469,36 @@ class CudaBackend:
         kvHeads, headDim = cache.kvHeads, cache.headDim
         if tokens < 0 or heads < 0:
             raise ValueError("PagedKvAppendFp8: tokens and heads must be >= 0")
-        self._check_kv8("PagedKvAppendFp8", blockTables, batch, blocksPerSeq, startLens, tokenStarts, tokens)
+        table, lens = blockTables.tensor, startLens.tensor
+        self._check_kv8("PagedKvAppendFp8", table, batch, blocksPerSeq, lens, tokenStarts, tokens)
         x, width = qkv.tensor, (heads + 2 * kvHeads) * headDim
         if x.numel() < tokens * width:
             raise ValueError("PagedKvAppendFp8: qkv is smaller than [tokens, heads + 2 * kvHeads, headDim]")
-        if heads > 0 and (queries is None or queries.tensor.numel() < tokens * heads * headDim or queries.tensor.dtype != x.dtype):
-            raise ValueError("PagedKvAppendFp8: queries must hold [tokens, heads, headDim] of qkv's dtype")
-        if (cos is None) != (sin is None):
-            raise ValueError("PagedKvAppendFp8: cos and sin come together")
-        reach = 0
-        if cos is not None:
-            c, s = cos.tensor, sin.tensor
-            reach = min(c.numel(), s.numel()) // (headDim // 2)
-            if c.dtype != torch.float32 or s.dtype != torch.float32:
+        dtype = x.dtype
+        at, q, out = x.data_ptr(), 0, 0
+        if heads > 0:
+            if queries is None or queries.tensor.numel() < tokens * heads * headDim or queries.tensor.dtype != dtype:
+                raise ValueError("PagedKvAppendFp8: queries must hold [tokens, heads, headDim] of qkv's dtype")
+            q, out = at, queries.tensor.data_ptr()
+        c, s, reach, rope = 0, 0, 0, N.ROPE_NONE
+        if cos is not None and sin is not None:
+            if cos.tensor.dtype != torch.float32 or sin.tensor.dtype != torch.float32:
                 raise ValueError("PagedKvAppendFp8: cos and sin are fp32 buffers")
+            c, s = cos.tensor.data_ptr(), sin.tensor.data_ptr()
+            reach = min(cos.tensor.numel(), sin.tensor.numel()) // (headDim // 2)
+            rope = N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES
+        elif cos is not None or sin is not None:
+            raise ValueError("PagedKvAppendFp8: cos and sin come together")
         if positions is not None and (positions.tensor.numel() < tokens or positions.tensor.dtype != torch.int32):
             raise ValueError("PagedKvAppendFp8: positions must be int32 [tokens]")
-        size, at, row = x.element_size() * headDim, x.data_ptr(), (width, headDim)
-        N.kv8_append(cache._pack(blockTables, blocksPerSeq), query=at if heads else None, key=at + heads * size,
-                     value=at + (heads + kvHeads) * size, query_out=queries.tensor.data_ptr() if heads else None, heads=heads,
-                     start=startLens.tensor.data_ptr(), tokens=tokens, batch=batch, dtype=_DTYPE[x.dtype],
-                     cosine=cos.tensor.data_ptr() if cos is not None else None, sine=sin.tensor.data_ptr() if cos is not None else None,
-                     rope=N.ROPE_NONE if cos is None else (N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES),
-                     max_position=reach, token_starts=tokenStarts.tensor.data_ptr() if tokenStarts is not None else None,
-                     positions=positions.tensor.data_ptr() if positions is not None else None, query_stride=row, key_stride=row,
-                     value_stride=row, stream=self._raw_stream)
+        size = headDim * (4 if dtype == torch.float32 else 2)
+        # (the block of native.kv8_append; its row strides are those of the packed tensor, the written queries are dense)
+        status = N._kv8_append_packed(cache._pack(table.data_ptr(), blocksPerSeq), N._KV8_APPEND_ARGS.pack(
+            q, at + heads * size, at + (heads + kvHeads) * size, out, width, headDim, width, headDim, width, headDim, 0, 0, c, s, lens.data_ptr(),
+            0 if tokenStarts is None else tokenStarts.tensor.data_ptr(), 0 if positions is None else positions.tensor.data_ptr(), tokens, reach,
+            batch, heads, _DTYPE[dtype], rope), self._raw_stream)
+        if status != N.OK:
+            raise N.AidnError(status, N.last_error())
         self.launch_count += 1
 
     def PagedAttentionFp8(self, q: GpuBuffer, cache: KvCacheFp8, blockTables: GpuBuffer, seqLens: GpuBuffer, output: GpuBuffer,
@@ -512,7 +517,8 @@ class CudaBackend:
         x, out = q.tensor, output.tensor
         width = heads * headDim
         queries = batch * maxQueries if queryStarts is None else x.numel() // width
-        self._check_kv8("PagedAttentionFp8", blockTables, batch, blocksPerSeq, seqLens, queryStarts, queries)
+        table, lens = blockTables.tensor, seqLens.tensor
+        self._check_kv8("PagedAttentionFp8", table, batch, blocksPerSeq, lens, queryStarts, queries)
         if x.numel() < queries * width or out.numel() < queries * width:
             raise ValueError("PagedAttentionFp8: q or output is smaller than [queries, heads, headDim]")
         if softmaxStats is not None and (softmaxStats.tensor.numel() < queries * heads or softmaxStats.tensor.dtype != torch.float32):
@@ -522,19 +528,23 @@ class CudaBackend:
                          emit_lse=softmaxStats is not None)
         need = h.kv8_workspace_bytes(batch, maxQueries, maxSeqLen)
         stream = self._raw_stream
-        ws, ws_bytes = None, 0
+        ws, ws_bytes = 0, 0
         if need > 0:
             held = self._scratch.get(0) if stream == 0 else None   # (stream 0 is never captured)
             if held is not None and held.numel() >= need:
                 ws, ws_bytes = held.data_ptr(), held.numel()
             else:
                 ws, ws_bytes = self._workspace(need, self.stream, optional=True)   # without one the keys are not cut
-        row = (maxQueries * width, headDim, width) if queryStarts is None else None
-        h.launch_kv8(q=x.data_ptr(), out=out.data_ptr(), cache=cache._pack(blockTables, blocksPerSeq), batch=batch, seq_q=maxQueries,
-                     seq_kv=maxSeqLen, stream=stream, query_starts=queryStarts.tensor.data_ptr() if queryStarts is not None else None,
-                     queries=queries, lse=softmaxStats.tensor.data_ptr() if softmaxStats is not None else None,
-                     kv_len=seqLens.tensor.data_ptr(), q_stride=row, o_stride=row, scale=float(scale), workspace=ws,
-                     workspace_bytes=ws_bytes)
+        row = (maxQueries * width, headDim, width) if queryStarts is None else N._NO_STRIDE
+        # (the block of Handle.launch_kv8)
+        block = N._SDPA_ARGS.pack(
+            x.data_ptr(), 0, 0, out.data_ptr(), 0 if softmaxStats is None else softmaxStats.tensor.data_ptr(), 0, 0, 0, 0, 0,
+            lens.data_ptr(), batch, maxQueries, maxSeqLen, *row, 0, 0, 0, 0, 0, 0, *row, float(scale), ws or 0, ws_bytes, False, 0, 0,
+            *N._NO_PEERS)
+        status = N._launch_kv8_packed(h._h, block, cache._pack(table.data_ptr(), blocksPerSeq),
+                                      None if queryStarts is None else queryStarts.tensor.data_ptr(), queries, stream)
+        if status != N.OK:
+            raise N.AidnError(status, N.last_error())
         self.launch_count += h.last_launch_count
 
     def FlashAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer,
