@@ -105,8 +105,7 @@ struct aidn_sdpa {
   aidn_sdpa_desc d;
   int group;
   int head_count;
-  int32_t* status_dev;   // [0] status word, [1..2] scheduler counters of the persistent prefill kernel, from [4] on kKv8Counters
-                         // counters of the attention over an 8-bit pool, which leaves them zero
+  int32_t* status_dev;   // [0] status word, [1..2] scheduler counters of the persistent prefill kernel
   int num_sms;
   void* scratch;
   int64_t scratch_bytes;
@@ -120,7 +119,6 @@ struct aidn_sdpa {
 
 namespace {
 
-constexpr int kHandleWords = 4 + aidn::kv8::kCounters;
 
 // Keys per split of the decode kernel.  Enough CTAs to fill 148 SMs several times over, but never more than
 // 512 keys per CTA so that ragged kv_len values balance, and never fewer than 64.
@@ -267,8 +265,8 @@ int aidn_sdpa_create(const aidn_sdpa_desc* desc, aidn_sdpa_t* out) {
   h->kv8_raised = 0;
   std::memset(&h->prefill_maps, 0, sizeof(h->prefill_maps));
   e = cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, d.device);
-  if (e == cudaSuccess) e = cudaMalloc(&h->status_dev, kHandleWords * sizeof(int32_t));
-  if (e == cudaSuccess) e = cudaMemset(h->status_dev, 0, kHandleWords * sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&h->status_dev, 4 * sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaMemset(h->status_dev, 0, 4 * sizeof(int32_t));
   if (e != cudaSuccess) {
     if (h->status_dev) cudaFree(h->status_dev);
     delete h;
@@ -338,7 +336,7 @@ int aidn_sdpa_poll(aidn_sdpa_t h, void* cu_stream) {
   e = cudaMemcpy(&st, h->status_dev, sizeof(st), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return fail_cuda(e, "poll: status read");
   if (st != 0) {
-    cudaMemset(h->status_dev, 0, kHandleWords * sizeof(int32_t));   // (a launch that gave up leaves counters)
+    cudaMemset(h->status_dev, 0, 4 * sizeof(int32_t));
     if (st & aidn::kStatusTimeout)
       return fail(AIDN_ETIMEOUT, "poll: a kernel gave up a bounded wait (status word 0x%x)", st);
     return fail(AIDN_EINVAL, "poll: a block-table entry outside [0, num_blocks) was skipped (status word 0x%x)", st);
@@ -902,7 +900,8 @@ int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_
     return -1;
   }
   if (h->d.path == AIDN_PATH_GENERIC || h->d.mask_kind != AIDN_MASK_NONE || h->d.head_dim % 16 != 0) return 0;
-  const int64_t few = aidn::kv8::split_workspace_bytes(h->d.head_dim, h->d.out_dtype == AIDN_F32, seq_q * h->group, h->num_sms);
+  const int64_t few = aidn::kv8::split_workspace_bytes(h->d.head_dim, h->d.out_dtype == AIDN_F32, batch, seq_q * h->group, seq_kv,
+                                                        h->head_count / h->group, h->num_sms);
   const int64_t many = seq_q * h->group > aidn::kv8::kFewRows && h->d.out_dtype != AIDN_F32 && (h->d.head_dim == 64 || h->d.head_dim == 128)
                            ? aidn::kv8::sm100_workspace_bytes(h->d.head_dim, h->num_sms) : 0;
   return align_up(few > many ? few : many, 256);
@@ -967,7 +966,6 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   p.scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt((float)d.head_dim);
   p.softcap = d.softcap;
   p.status = h->status_dev;
-  p.counters = reinterpret_cast<uint32_t*>(h->status_dev + 4);
   cudaStream_t stream = (cudaStream_t)cu_stream;
   int launches = 1;
   cudaError_t e;
@@ -975,7 +973,7 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
     e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);
     h->last_path = AIDN_PATH_PREFILL_SM100;
   } else if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
-    e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, stream);
+    e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);
     h->last_path = AIDN_PATH_DECODE;
   } else {
     e = aidn::kv8::launch_attend_generic(p, stream);

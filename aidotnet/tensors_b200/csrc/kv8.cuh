@@ -7,9 +7,6 @@ namespace aidn {
 namespace kv8 {
 
 constexpr float kLargestCode = 448.f;
-// Counters that a handle keeps for the launches that cut keys over CTAs (one a CTA).
-constexpr int kCounters = 2048;
-
 // Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one.
 constexpr int kFewRows = 32;
 
@@ -61,7 +58,6 @@ struct Attend {
   int32_t dtype, out_f32, mask_kind, causal, bottom_right;
   float scale, softcap;
   int32_t* status;
-  uint32_t* counters;   // of the handle: zero between launches
 };
 
 // ---- addressing -----------------------------------------------------------------------------------------------------
@@ -153,8 +149,9 @@ cudaError_t launch_attend_generic(const Attend& p, cudaStream_t stream);
 // Few queries (csrc/kv8_split.cu): head sizes that are a multiple of 16, 16-byte aligned pools, no mask.  Without its workspace keys are not
 // cut.  raised: a word of the handle, which kernels had their shared-memory limit raised.
 bool split_supported(const Attend& p);
-int64_t split_workspace_bytes(int head_dim, bool exact, int64_t rows, int num_sms);
-cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream);
+int64_t split_workspace_bytes(int head_dim, bool exact, int64_t batch, int64_t rows, int64_t seq_kv, int kv_count, int num_sms);
+cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, int* launches,
+                                cudaStream_t stream);
 // Many queries of 16 bits (csrc/kv8_sm100.cu): head sizes 64 and 128, blocks of a multiple of 16 tokens, 16-byte aligned pools, no mask.
 bool sm100_supported(const Attend& p);
 int64_t sm100_workspace_bytes(int head_dim, int num_sms);

@@ -4,18 +4,19 @@
 //   P = 2^(x - m) with a running maximum m,   O^T += V^T (P v_scale(block) / v_ref)^T,   o = O v_ref / sum P
 //
 // Bound by the pool's bytes: 2 D bytes a key and KV head, a few operations a byte.  So every key is read once for all the queries of its
-// sequence and KV head (a "line": up to 8 NR query rows = query heads of the group x queries), straight from global memory into the
-// registers that feed mma.sync: a product does not care about the order of its terms, so the head dimension is permuted such
-// that a lane's 16 bytes of a key are its own elements of four A fragments, and a lane's 16 bytes of a value row its own rows of eight
-// (queries are laid out in the matching order once a line).  No shared memory and no transposition lie on the way of the keys; a
-// code becomes fp16 exactly (cvt, two at a time), a query is scaled by a power of two into fp16 (two terms for fp32 results),
-// and the scales of the blocks are applied to the products in fp32.  Weights are rounded to fp16 (11 bits, of 2^9 times their
-// value so that they stay normal down to 2^-23 of the largest); for fp32 results they are two terms too.
+// sequence and KV head (a "line": up to 8 NR query rows = query heads of the group x queries).  A warp has a line's next tiles of 16 keys
+// in shared memory or on their way to it (asynchronous copies of 16 bytes), and reads them as fragments of mma.sync without transposing: a
+// product does not care about the order of its terms, so the head dimension is permuted such that a lane's 16 bytes of a key are its
+// own elements of four A fragments, and a lane's 16 bytes of a value row its own rows of eight (queries are laid out in the
+// matching order once a line).  A code becomes fp16 exactly (cvt, two at a time), a query is scaled by a power of two into
+// fp16 (two terms for fp32 results), and the scales of the blocks are applied to the products in fp32.  Weights are rounded to fp16
+// (11 bits, of 2^9 times their value so that they stay normal down to 2^-23 of the largest); for fp32 results they are two terms too.
 //
-// The lines' 16-key tiles are one row, cut into equal shares for the CTAs that are resident whatever the lengths are; the warps of a
-// CTA take the tiles of its share in turn and merge through shared memory.  A line that is cut leaves one partial result a CTA in
-// the workspace, and the CTA that arrives last (a counter that wraps to zero by itself) merges them in their order: the
-// result does not depend on who was last, and there is no second launch.
+// The warps of a "unit" do the same tiles of neighbouring KV heads, whose rows are neighbours in the pool: memory is read in runs
+// of up to 1 KB (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 240 us, and 279 us where each warp went through lines of its own).  The
+// lines' tiles are one row, cut into equal shares for the units that are resident whatever the lengths are.  No warp waits for
+// another one: a line that is cut leaves a partial result a unit in the workspace, and a second launch merges them in their order, so that
+// the result does not depend on which was first.
 #include "kv8.cuh"
 #include "mma_sync.cuh"
 
@@ -27,11 +28,19 @@ constexpr int kTile = 16;           // keys
 constexpr float kUnset = -1e30f;    // running maximum before any key
 constexpr float kLazy = 6.f;        // the maximum follows when a logit is 2^6 above it: weights stay below 2^(9 + 6), in fp16's range
 constexpr float kLift = 9.f;
+constexpr int kMergeThreads = 256;
+constexpr int kMostUnits = 4096;
 
+// A line that is cut: begun by unit `at` of the list, parts of it in the `parts - 1` units behind.
+struct Note {
+  int parts, b, off, rows;
+};
 struct Split {
-  float* partial;    // [2 grid][8 NR][DP], or null: lines are not cut
-  float2* stats;     // [2 grid][8 NR]: maximum and sum
-  int least;         // tiles of a warp's share
+  float* partial;    // [2 units][heads of a unit][row_most][DP], or null: lines are not cut
+  float2* stats;     // [2 units][heads of a unit][row_most]: maximum and sum
+  Note* notes;       // [units]
+  int units, heads_log2, row_most;
+  int least;         // tiles of a unit's share
   bool query_vec, out_vec;   // 16 bytes of the queries, four elements of the results are aligned
 };
 
@@ -40,9 +49,25 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint2 ld_stream8(const void* ptr) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t at) {
   uint2 r;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(ptr));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ float lds_f(uint32_t at) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
   return r;
 }
 // Sixteen elements of a query as they lie: eight words of 16-bit elements, sixteen of 32-bit ones.  (Volatile: issued where they stand.)
@@ -109,47 +134,62 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   return x & ~(hit * 0xffu);
 }
 
+// First element of group x of four: groups of a row lie in the workspace in the order in which lanes hold them.
+template <int DP>
+__device__ __forceinline__ int group_column(int x) {
+  return DP == 64 ? 8 * (x & 7) + 4 * (x >> 3) : 128 * (x >> 5) + 16 * (x & 7) + 4 * (x >> 3 & 3);
+}
+
+// What the host knows of a call.
+struct Sizes {
+  int64_t batch, rows, seq_kv;   // rows: of a sequence and KV head, at most
+  int kv_count, num_sms;
+  int64_t workspace_bytes;
+};
+
 template <int DP, int NR, int T, bool UB>
 struct Config {
   static constexpr int kWarps = NR == 1 && DP < 256 ? 8 : 4;
   static constexpr int kMinCtas = DP == 256 ? 2 : (NR == 1 ? 2 : 3);
   static constexpr int kSteps = DP / 16;                 // of 16 elements: fragments of a key
   static constexpr int kRows = 8 * NR;
-  static constexpr int kPitch = DP + 4;                  // floats between the rows of a partial result
-  static constexpr int kQueryWords = T * NR * kSteps * 32 * 2;   // of a warp
-  static constexpr size_t kSmem = (size_t)kWarps * (kQueryWords * 4 + 2 * kRows * kPitch * 4);
+  static constexpr int kQueryBytes = T * NR * kSteps * 32 * 8;   // of a warp
+  static constexpr int kScales = UB ? 16 : 128;                  // bytes of a stage: the block's two, or those of 16 keys
+  static constexpr int kStage = 2 * kTile * DP + kScales;
+  // three tiles of a warp are in shared memory or on their way to it, two where three would cost a CTA
+  static constexpr int kStages = kWarps * (kQueryBytes + 3 * kStage) + 1024 <= 233472 / kMinCtas ? 3 : 2;
+  static constexpr size_t kSmem = (size_t)kWarps * (kQueryBytes + kStages * kStage);
 };
 
 template <int DP, int NR, int T, bool UB>
 __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP, NR, T, UB>::kMinCtas)
-    kv8_split_kernel(const __grid_constant__ Attend p, const Split sp) {
+    kv8_split_kernel(const __grid_constant__ Attend p, const __grid_constant__ Split sp) {
   using C = Config<DP, NR, T, UB>;
-  constexpr int NW = C::kWarps, KS = C::kSteps, MT = DP / 16, ROWS = C::kRows;
-  constexpr int KC = DP / 64;                     // 64-byte pieces of a key: 16 bytes a lane
+  constexpr int NW = C::kWarps, KS = C::kSteps, MT = DP / 16, ROWS = C::kRows, STAGES = C::kStages;
+  constexpr int KC = DP / 64;                     // 16-byte pieces of a key a lane multiplies
   constexpr int VB = DP == 64 ? 8 : 16;           // bytes of a value row a lane reads at a time
   constexpr int VC = DP == 256 ? 2 : 1;
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* const wacc = reinterpret_cast<float*>(smem + NW * C::kQueryWords * 4);   // [NW][2][ROWS][kPitch]: parts of cut lines
-  __shared__ float row_c[NW][ROWS];
-  __shared__ int row_lim[NW][ROWS];
-  __shared__ float2 wstat[NW][2][ROWS];
-  __shared__ int64_t wline[NW][2];      // the line's first tile, or -1
-  __shared__ int winfo[NW][2][3];       // its sequence, number and tiles
-  __shared__ int64_t scan[NW], prefix[NW * 32];
-  __shared__ int last_flag[2];
+  constexpr int CPR = DP / 16, RPI = 32 / CPR, NI = kTile / RPI;   // 16-byte chunks of a row; rows and copies of a warp's instruction
+  extern __shared__ __align__(128) uint8_t smem[];
+  // (the sums of the scan lie where the tiles will)
+  int64_t* const scan = reinterpret_cast<int64_t*>(smem);
+  int64_t* const prefix = scan + NW;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint2* const qfrag = reinterpret_cast<uint2*>(smem) + warp * (C::kQueryWords / 2);   // [T][NR][KS][32]
-  const int D = p.c.head_dim, G = p.group;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * C::kStage;
+  uint2* const qfrag = reinterpret_cast<uint2*>(smem + NW * STAGES * C::kStage + warp * C::kQueryBytes);   // [T][NR][KS][32]
+  const int D = p.c.head_dim, G = p.group, groups = p.kv_count >> sp.heads_log2;
+  const int unit = ((int)blockIdx.x * NW + warp) >> sp.heads_log2, sub = warp & ((1 << sp.heads_log2) - 1);
   const bool cut = sp.partial != nullptr;
+  auto column = [](int j, int t) { return DP == 64 ? 16 * t : 128 * (j >> 1) + 32 * t + 16 * (j & 1); };   // first element of a lane's piece j
   pdl_wait();
   pdl_trigger();
 
   auto tiles_of = [&](int keys) { return keys > kTile ? (keys + kTile - 1) / kTile : 1; };
-  auto lines_of = [&](int n) { return ((n * G + ROWS - 1) / ROWS) * p.kv_count; };
+  auto lines_of = [&](int n) { return ((n * G + ROWS - 1) / ROWS) * groups; };
   auto weight_of = [&](int b) { return (int64_t)lines_of(rows_of(p, b).count) * (cut ? tiles_of(keys_of(p, b)) : 1); };
 
-  // ---- the share of this CTA and of its warps: the threads sum up their sequences' tiles
+  // ---- the share of this unit: the threads sum up their sequences' tiles
   const int per = (p.batch + NW * 32 - 1) / (NW * 32);
   const int b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
   int64_t mine = 0;
@@ -161,7 +201,6 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     if (lane >= o) upto += v;
   }
   if (lane == 31) scan[warp] = upto;
-  if (lane < 2) wline[warp][lane] = -1;
   __syncthreads();
   int64_t total = 0, before = 0;
 #pragma unroll
@@ -170,13 +209,11 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     total += scan[w];
   }
   prefix[tid] = before + upto - mine;
-  int64_t share = (total + (int64_t)gridDim.x * NW - 1) / ((int64_t)gridDim.x * NW);   // of a warp
-  if (cut && share < sp.least) share = sp.least;
-  const int64_t cta_pos = (int64_t)blockIdx.x * share * NW, cta_end = min(cta_pos + share * NW, total);
-  if (cta_pos >= cta_end) return;
   __syncthreads();
-  int64_t pos = min(cta_pos + warp * share, cta_end);
-  const int64_t end = min(pos + share, cta_end);
+  int64_t share = total < 0x7fffffff - sp.units ? ((int)total + sp.units - 1) / sp.units : (total + sp.units - 1) / sp.units;
+  if (cut && share < sp.least) share = sp.least;
+  int64_t pos = unit < sp.units ? min(unit * share, total) : total;
+  const int64_t end = min(pos + share, total);
   int b = 0;
   int64_t base = 0;
   if (pos < end) {   // the last thread whose sequences begin at or before pos, then the sequence among its own
@@ -186,7 +223,9 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     b = (at - 1) * per;
     base = prefix[at - 1];
   }
+  __syncthreads();
   bool bad = false;
+  Note note = {0, 0, 0, 0};
 
   while (pos < end) {
     const Rows rw = rows_of(p, b);
@@ -199,12 +238,25 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     }
     const int64_t into = pos - base;   // (a division of 64 bits takes over a hundred instructions)
     const int off = into < 0x7fffffff ? (int)into / tiles : (int)(into / tiles), t0 = cut ? (int)(into - (int64_t)off * tiles) : 0;
-    const int kvh = p.kv_begin + off % p.kv_count, r0 = off / p.kv_count * ROWS;
+    const int chunk = off / groups, kvh = p.kv_begin + ((off - chunk * groups) << sp.heads_log2) + sub, r0 = chunk * ROWS;
     const int rows = min(ROWS, rw.count * G - r0);
     const int t1 = cut ? (int)min((int64_t)tiles, t0 + (end - pos)) : tiles_of(keys);
     const bool whole = !cut || (t0 == 0 && t1 == tiles);
-    const int64_t line_pos = pos - t0;
+    if (!whole && t0 == 0) note = {(int)((pos + tiles - 1) / share) - unit + 1, b, off, rows};
     pos += cut ? t1 - t0 : 1;
+
+    const int lim_least = visible(p, keys, rw.count, rw.count == 1 ? 0 : r0 / G);
+    const int lim_most = rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + rows - 1) / G);
+    const int t_end = min(t1, (lim_most + kTile - 1) / kTile);
+    // ---- tiles t0 .. t_end - 1.  A lane holds the table's entry of one of 32 blocks, and of one of the next 32.
+    const int32_t* table = p.c.table + b * p.c.table_stride;
+    int window = 0, entry = 0, entry_n = 0, last_block = 0;
+    if (t0 < t_end) {
+      window = block_of(p.c, t0 * kTile);
+      last_block = block_of(p.c, min(t_end * kTile, keys) - 1);
+      if (window + lane <= last_block) entry = table[window + lane];
+      if (window + 32 + lane <= last_block) entry_n = table[window + 32 + lane];
+    }
 
     // the queries are on their way while the first keys are looked up: lane (g, t) takes of row g (of eight) what it is to multiply with
     uint32_t qr[NR][KC][8 * T];
@@ -213,131 +265,82 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       const int r = 8 * n + g;
       if (r >= rows) continue;
       const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-      const int64_t at = query_at(p, p.qs, rw, b, h, i) + 16 * t;
+      const int64_t at = query_at(p, p.qs, rw, b, h, i);
 #pragma unroll
       for (int j = 0; j < KC; ++j)
-        if (64 * j + 16 * t < D) load16<T>(p, at + 64 * j, sp.query_vec, qr[n][j]);
+        if (column(j, t) < D) load16<T>(p, at + column(j, t), sp.query_vec, qr[n][j]);
     }
 
-    const int lim_least = visible(p, keys, rw.count, rw.count == 1 ? 0 : r0 / G);
-    const int lim_most = rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + rows - 1) / G);
-    const int t_end = min(t1, (lim_most + kTile - 1) / kTile);
-    // ---- tiles t0 .. t_end - 1.  The blocks of the next 32 are looked up together, a lane each.
-    const int32_t* table = p.c.table + b * p.c.table_stride;
+    // A tile's keys and values go to shared memory, 16 bytes a lane and copy.  All of them exist: where a row is shorter than DP bytes its
+    // first chunk comes again (the queries are zero there, and those values are not written), and keys behind the last one, or of a
+    // block outside the pool, are other rows of the pool, masked below.
     const int64_t pitch = p.c.stride[1];
-    const uint8_t* const klane = p.c.k + kvh * p.c.stride[2] + 16 * t + (UB ? g * pitch : 0);
-    const uint8_t* const vlane = p.c.v + kvh * p.c.stride[2] + VB * g + (UB ? 2 * t * pitch : 0);
-    int entry = -1;
-    float ks_l = 0.f, vs_l = 0.f;
-    auto look_up = [&](int tile) {   // this lane's tile (UB: a tile lies in one block)
-      entry = -1;
-      ks_l = vs_l = 0.f;
-      if (tile < t_end) {
-        entry = checked_block(p.c, table[block_of(p.c, tile * kTile)], bad);
-        if (entry >= 0) {
-          ks_l = p.c.k_scale[(int64_t)entry * p.c.kv_heads + kvh];
-          vs_l = p.c.v_scale[(int64_t)entry * p.c.kv_heads + kvh];
-        }
-      }
+    const int my_row = lane / CPR, my_chunk = lane % CPR;
+    const int64_t from = kvh * p.c.stride[2] + (my_chunk * 16 < D ? my_chunk * 16 : 0) + (UB ? my_row * pitch : 0);
+    auto key_chunk = [](int row, int chunk) { return row * DP + (DP == 64 ? chunk : chunk ^ (row & 7)) * 16; };
+    // (64 bytes a row: rows 0 and 2 share a line of the banks, 1 and 3 the next)
+    auto value_chunk = [](int row, int chunk) {
+      return DP == 64 ? ((row >> 2) * 2 + (row & 1)) * 128 + (row & 2) * 32 + (chunk ^ (row >> 1 & 2)) * 16 : row * DP + (chunk ^ (row & 7)) * 16;
     };
-    // K fragments: keys g, g + 8 of the tile; V fragments: keys 2t, 2t + 1, 2t + 8, 2t + 9.
-    uint4 kr[2][KC];
-    uint4 vr[4][VC];
-    float ks[2], vs[2], ks_n[2], vs_n[2];   // of keys g and g + 8: this tile's, and (not UB) the next one's
-    bool full_n = false;                    // all keys of the tile are there, and a row has DP bytes
-    bool ok_n[2];
-    int64_t row_n = -1;                     // UB: offset of the tile's first row, -1 without one
-    int64_t vrow[UB ? 1 : 4];               // else of the values' rows
-    auto find = [&](int tile, int slot) {   // and loads the keys
-      const int key0 = tile * kTile;
+    auto issue = [&](int tile, int stage) {
+      const uint32_t at = ring + stage * C::kStage;
+      const int key0 = tile * kTile, first = block_of(p.c, key0);
+      if (first - window >= 32) {
+        window += 32;
+        entry = entry_n;
+        if (window + 32 + lane <= last_block) entry_n = table[window + 32 + lane];
+      }
       if constexpr (UB) {
-        const int ent = __shfl_sync(0xffffffffu, entry, slot);
-        const int first = key0 - block_of(p.c, key0) * p.c.block_size;
-        row_n = ent >= 0 ? ent * p.c.stride[0] + first * pitch : -1;
-        full_n = ent >= 0 && key0 + kTile <= keys && D == DP;
-        if (full_n) {
-          const uint8_t* at = klane + row_n;
+        const int ent = checked_block(p.c, __shfl_sync(0xffffffffu, entry, first - window), bad);
+        const int64_t row = (int64_t)max(ent, 0) * p.c.stride[0] + (key0 - first * p.c.block_size) * pitch + from;
+        const uint8_t* k = p.c.k + row;
+        const uint8_t* v = p.c.v + row;
 #pragma unroll
-          for (int q = 0; q < KC; ++q) kr[0][q] = ld_stream16(at + 64 * q);
-          at += 8 * pitch;
-#pragma unroll
-          for (int q = 0; q < KC; ++q) kr[1][q] = ld_stream16(at + 64 * q);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            ok_n[j] = ent >= 0 && key0 + g + 8 * j < keys;
-#pragma unroll
-            for (int q = 0; q < KC; ++q)
-              kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(klane + row_n + 8 * j * pitch + 64 * q) : make_uint4(0, 0, 0, 0);
-          }
+        for (int i = 0; i < NI; ++i) {
+          copy16(at + key_chunk(my_row + i * RPI, my_chunk), k);
+          copy16(at + kTile * DP + value_chunk(my_row + i * RPI, my_chunk), v);
+          k += RPI * pitch;
+          v += RPI * pitch;
+        }
+        if (lane < 2) {
+          const uint32_t to = at + 2 * kTile * DP + lane * 4;
+          if (ent >= 0) copy4(to, (lane ? p.c.v_scale : p.c.k_scale) + (int64_t)ent * p.c.kv_heads + kvh);
+          else asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(-1.f) : "memory");
         }
       } else {
-        auto lookup = [&](int key, float* ksv, float* vsv) -> int64_t {
-          if (key >= keys) return -1;
-          const int at = block_of(p.c, key);
-          const int ent = checked_block(p.c, table[at], bad);
-          if (ent < 0) return -1;
-          if (ksv) {
-            *ksv = p.c.k_scale[(int64_t)ent * p.c.kv_heads + kvh];
-            *vsv = p.c.v_scale[(int64_t)ent * p.c.kv_heads + kvh];
-          }
-          return ent * p.c.stride[0] + (key - at * p.c.block_size) * pitch;
+        auto entry_of = [&](int key, int& within) {
+          key = min(key, keys - 1);
+          const int block = block_of(p.c, key), rel = block - window;
+          const int a = __shfl_sync(0xffffffffu, entry, rel & 31), c = __shfl_sync(0xffffffffu, entry_n, rel & 31);
+          within = key - block * p.c.block_size;
+          return checked_block(p.c, rel < 32 ? a : c, bad);
         };
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          ks_n[j] = vs_n[j] = 0.f;
-          const int64_t row = lookup(key0 + g + 8 * j, &ks_n[j], &vs_n[j]);
-          ok_n[j] = row >= 0;
-#pragma unroll
-          for (int q = 0; q < KC; ++q)
-            kr[j][q] = ok_n[j] && 64 * q + 16 * t < D ? ld_stream16(klane + row + 64 * q) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < NI; ++i) {
+          int within;
+          const int ent = entry_of(key0 + my_row + i * RPI, within);
+          const int64_t row = (int64_t)max(ent, 0) * p.c.stride[0] + within * pitch + from;
+          copy16(at + key_chunk(my_row + i * RPI, my_chunk), p.c.k + row);
+          copy16(at + kTile * DP + value_chunk(my_row + i * RPI, my_chunk), p.c.v + row);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vrow[UB ? 0 : j] = lookup(key0 + 2 * t + (j & 1) + 8 * (j >> 1), nullptr, nullptr);
+        int within;
+        const int ent = entry_of(key0 + (lane & 15), within);
+        const uint32_t to = at + 2 * kTile * DP + lane * 4;
+        if (ent >= 0) copy4(to, (lane < 16 ? p.c.k_scale : p.c.v_scale) + (int64_t)ent * p.c.kv_heads + kvh);
+        else asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(-1.f) : "memory");
       }
     };
-    auto load_v = [&](int key0) {
-      if (UB && full_n) {
-        const uint8_t* at = vlane + row_n;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int q = 0; q < VC; ++q) {
-            if (VB == 8) {
-              const uint2 x = ld_stream8(at + 128 * q);
-              vr[j][q].x = x.x; vr[j][q].y = x.y;
-            } else {
-              vr[j][q] = ld_stream16(at + 128 * q);
-            }
-          }
-          at += j == 1 ? 7 * pitch : pitch;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = (j & 1) + 8 * (j >> 1);
-          const int64_t row = UB ? (row_n >= 0 && key0 + 2 * t + k < keys ? row_n + k * pitch : -1) : vrow[UB ? 0 : j];
-#pragma unroll
-          for (int q = 0; q < VC; ++q) {
-            const bool there = row >= 0 && 128 * q + VB * g < D;
-            if (VB == 8) {
-              const uint2 x = there ? ld_stream8(vlane + row) : make_uint2(0, 0);
-              vr[j][q].x = x.x; vr[j][q].y = x.y;
-            } else {
-              vr[j][q] = there ? ld_stream16(vlane + row + 128 * q) : make_uint4(0, 0, 0, 0);
-            }
-          }
-        }
-      }
-    };
-    int tile = t0, slot = 0;
-    if (tile < t_end) {   // (the first keys are on their way while the queries are laid out)
-      if (UB) look_up(tile + lane);
-      find(tile, 0);
-      load_v(tile * kTile);
+    int stage = 0;
+    __syncwarp();   // (the last line's tiles and queries have been read)
+#pragma unroll 1
+    for (int a = 0; a < STAGES - 1; ++a) {
+      if (t0 + a < t_end) issue(t0 + a, a);
+      cp_async_commit();
     }
 
     // ---- queries: scaled by a power of two so that the largest element is in [2^12, 2^13), as fragments
+    float c_row[NR];
+    int lim_row[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = 8 * n + g;
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       float largest = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j)
-        if (valid && 64 * j + 16 * t < D) {
+        if (valid && column(j, t) < D) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) largest = fmaxf(largest, fabsf(widen<T>(p, qr[n][j], e)));
         }
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __half2 hi[2] = {}, lo[2] = {};
-          if (valid && 64 * j + 16 * t < D) {
+          if (valid && column(j, t) < D) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float a = widen<T>(p, qr[n][j], 4 * i + 2 * e) * f, c = widen<T>(p, qr[n][j], 4 * i + 2 * e + 1) * f;
@@ -371,10 +374,8 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
           dst[0] = make_uint2(*reinterpret_cast<uint32_t*>(&hi[0]), *reinterpret_cast<uint32_t*>(&hi[1]));
           if (T == 2) dst[NR * KS * 32] = make_uint2(*reinterpret_cast<uint32_t*>(&lo[0]), *reinterpret_cast<uint32_t*>(&lo[1]));
         }
-      if (t == 0) {
-        row_c[warp][r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (p.softcap > 0.f ? 1.f : kLog2e);
-        row_lim[warp][r] = !valid ? keys : (rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + r) / G));
-      }
+      c_row[n] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (p.softcap > 0.f ? 1.f : kLog2e);
+      lim_row[n] = !valid ? keys : (rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + r) / G));
     }
     __syncwarp();
 
@@ -392,24 +393,36 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       for (int e = 0; e < 2; ++e) {
         m[n][e] = kUnset;
         l[n][e] = 0.f;
-        c[n][e] = row_c[warp][8 * n + 2 * t + e];
-        lim[n][e] = row_lim[warp][8 * n + 2 * t + e];
+        c[n][e] = __shfl_sync(0xffffffffu, c_row[n], 4 * (2 * t + e));
+        lim[n][e] = __shfl_sync(0xffffffffu, lim_row[n], 4 * (2 * t + e));
       }
     }
-    for (; tile < t_end; ++tile) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        ks[j] = UB ? __shfl_sync(0xffffffffu, ks_l, slot) : ks_n[j];
-        vs[j] = UB ? __shfl_sync(0xffffffffu, vs_l, slot) : vs_n[j];
-      }
-      // rows of which not all keys of the tile are seen, or keys that are not there
+#pragma unroll 1
+    for (int tile = t0; tile < t_end; ++tile) {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();   // all lanes' copies have landed, and all have read the stage that is filled again now
+      const uint32_t at = ring + stage * C::kStage;
+      if (tile + STAGES - 1 < t_end) issue(tile + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+      cp_async_commit();
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+
       const int key0 = tile * kTile;
-      const bool full = full_n, edge = !full || key0 + kTile > lim_least;
-      bool ok[2] = {true, true};
-      if (!full) {
-        ok[0] = ok_n[0];
-        ok[1] = ok_n[1];
+      float ks[2], vs[2];
+      if constexpr (UB) {
+        const uint2 x = lds8(at + 2 * kTile * DP);
+        ks[0] = ks[1] = __uint_as_float(x.x);
+        vs[0] = vs[1] = __uint_as_float(x.y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ks[j] = lds_f(at + 2 * kTile * DP + (g + 8 * j) * 4);
+          vs[j] = lds_f(at + 2 * kTile * DP + (16 + g + 8 * j) * 4);
+        }
       }
+      const bool ok[2] = {__float_as_int(ks[0]) >= 0, __float_as_int(ks[1]) >= 0};   // (a block outside the pool: -1)
+      // rows of which not all keys of the tile are seen, or keys that are not there
+      bool edge = key0 + kTile > lim_least || !ok[0];
+      if constexpr (!UB) edge = edge || __any_sync(0xffffffffu, !ok[0] || !ok[1]);
       float s[NR][4];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -417,7 +430,9 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
         for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
       for (int q = 0; q < KC; ++q) {
-        const uint32_t w0[4] = {kr[0][q].x, kr[0][q].y, kr[0][q].z, kr[0][q].w}, w1[4] = {kr[1][q].x, kr[1][q].y, kr[1][q].z, kr[1][q].w};
+        const int chunk = DP == 64 ? t : 8 * (q >> 1) + 2 * t + (q & 1);
+        const uint4 x0 = lds16(at + key_chunk(g, chunk)), x1 = lds16(at + key_chunk(g, chunk) + 8 * DP);
+        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t a0 = codes_to_f16(w0[i]), a1 = codes_to_f16(w1[i]), a2 = codes_to_f16_hi(w0[i]), a3 = codes_to_f16_hi(w1[i]);
@@ -430,16 +445,19 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             }
         }
       }
-      // the next tile's keys, while this one's weights are formed
-      const int next = tile + 1;
-      if (next < t_end) {
-        if (++slot == 32) {
-          slot = 0;
-          if (UB) look_up(next + lane);
+      uint4 vr[4][VC];   // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < VC; ++q) {
+          const uint32_t from_v = at + kTile * DP + value_chunk(2 * t + (j & 1) + 8 * (j >> 1), VB == 8 ? g >> 1 : g + 8 * q);
+          if (VB == 8) {
+            const uint2 x = lds8(from_v + (g & 1) * 8);
+            vr[j][q].x = x.x; vr[j][q].y = x.y;
+          } else {
+            vr[j][q] = lds16(from_v);
+          }
         }
-        find(next, slot);
-      }
-
       uint32_t nan_keys = 0;   // keys of which a value is NaN: where rows do not see the key it must not reach them, so that it goes through the logit
       if (edge) {
 #pragma unroll
@@ -546,10 +564,9 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             }
           }
       }
-      if (next < t_end) load_v(next * kTile);
     }
 
-    // ---- a whole line is written, a part of one kept: of the line that began before this warp's share, and of the one that goes on
+    // ---- a whole line is written, a part of one left in the workspace: of the line that began before this unit's share, or of the one that goes on
     float sum[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -559,157 +576,131 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
       }
-    const int part = t0 == 0 ? 1 : 0;
+    const int64_t part = ((int64_t)(2 * unit + (t0 == 0 ? 1 : 0)) << sp.heads_log2) + sub;
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * n + 2 * t + e;
         if (r >= rows) continue;
-        const float f = whole ? (sum[n][e] == 0.f ? 0.f : vref / sum[n][e]) : vref;
+        if (!whole) {   // (a lane's groups of four elements lie 8 groups apart: a line of 128 bytes is written at a time)
+          const int64_t to = part * sp.row_most + r;
+          float4* const dst = reinterpret_cast<float4*>(sp.partial + to * DP) + g;
+#pragma unroll
+          for (int j = 0; j < MT; j += 2)
+            __stcg(dst + 4 * j, make_float4(acc[n][j][e] * vref, acc[n][j][e + 2] * vref, acc[n][j + 1][e] * vref, acc[n][j + 1][e + 2] * vref));
+          if (g == 0) __stcg(sp.stats + to, make_float2(m[n][e] - kLift, sum[n][e]));
+          continue;
+        }
+        const float f = sum[n][e] == 0.f ? 0.f : vref / sum[n][e];
         const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-        const int64_t at = whole ? query_at(p, p.os, rw, b, h, i) : 0;
-        float* const to = wacc + ((warp * 2 + part) * ROWS + r) * C::kPitch;
+        const int64_t to = query_at(p, p.os, rw, b, h, i);
 #pragma unroll
         for (int j = 0; j < MT; j += 2) {
-          const int d = DP == 256 ? 128 * (j / 8) + 16 * g + 2 * (j % 8) : VB * g + 2 * j;
-          const float4 o = make_float4(acc[n][j][e] * f, acc[n][j][e + 2] * f, acc[n][j + 1][e] * f, acc[n][j + 1][e + 2] * f);
-          if (!whole) *reinterpret_cast<float4*>(to + d) = o;
-          else if (d < D) store4(p, at + d, sp.out_vec, o);
+          const int d = group_column<DP>(4 * j + g);
+          if (d < D) store4(p, to + d, sp.out_vec, make_float4(acc[n][j][e] * f, acc[n][j][e + 2] * f, acc[n][j + 1][e] * f, acc[n][j + 1][e + 2] * f));
         }
-        if (g == 0) {
-          if (!whole) wstat[warp][part][r] = make_float2(m[n][e] - kLift, sum[n][e]);
-          else if (p.lse) *lse_at(p, rw, h, i) = sum[n][e] == 0.f ? -INFINITY : (m[n][e] - kLift + log2f(sum[n][e])) * kLn2;
-        }
+        if (p.lse && g == 0) *lse_at(p, rw, h, i) = sum[n][e] == 0.f ? -INFINITY : (m[n][e] - kLift + log2f(sum[n][e])) * kLn2;
       }
-    if (!whole && lane == 0) {
-      wline[warp][part] = line_pos;
-      winfo[warp][part][0] = b;
-      winfo[warp][part][1] = off;
-      winfo[warp][part][2] = tiles;
-    }
-    __syncwarp();
   }
+  cp_async_wait<0>();
+  if (cut && sub == 0 && lane == 0 && unit < sp.units) *reinterpret_cast<int4*>(sp.notes + unit) = make_int4(note.parts, note.b, note.off, note.rows);
   if (bad && p.status) atomicOr(p.status, kStatusBadBlock);
+}
+
+// The cut lines' parts: a CTA takes rows (of a line, a head) in turn, its threads four elements of some of the parts each.
+template <int DP>
+__global__ void __launch_bounds__(kMergeThreads) kv8_split_merge_kernel(const __grid_constant__ Attend p, const __grid_constant__ Split sp, int line_rows) {
+  constexpr int C4 = DP / 4, PL = kMergeThreads / C4, WARPS = kMergeThreads / 32;
+  __shared__ int counts[WARPS];
+  __shared__ uint16_t list[kMostUnits];
+  __shared__ float4 held[PL][C4];
+  __shared__ float2 held_stats[PL];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, x = tid % C4, pl = tid / C4;
+  pdl_wait();
+  pdl_trigger();
+  // the units that began a line which is cut
+  const int per = (sp.units + kMergeThreads - 1) / kMergeThreads, u_lo = min(tid * per, sp.units), u_hi = min(u_lo + per, sp.units);
+  int mine = 0;
+  for (int u = u_lo; u < u_hi; ++u) mine += sp.notes[u].parts > 0;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) counts[warp] = upto;
+  __syncthreads();
+  int total = 0, to = upto - mine;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) to += counts[w];
+    total += counts[w];
+  }
+  if (mine > 0)
+    for (int u = u_lo; u < u_hi; ++u)
+      if (sp.notes[u].parts > 0) list[to++] = (uint16_t)u;
   __syncthreads();
 
-  // ---- the parts of a line in this CTA are consecutive: merged by all threads, and written, or left in the workspace
-  auto finish = [&](const Rows& rw, int b, int off, int r, int d, float4 o, float top, float sum) {
-    const int kvh = p.kv_begin + off % p.kv_count, r0 = off / p.kv_count * ROWS;
-    const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    store4(p, query_at(p, p.os, rw, b, h, i) + d, sp.out_vec, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-    if (p.lse && d == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-  };
-  int64_t handed0 = -1, handed1 = -1;   // lines of which other CTAs have parts too: the one that began before, the one that goes on
-  int at0 = 0, at1 = 0;
-  unsigned used = 0;   // slots that hold a part
+  const int D = p.c.head_dim, G = p.group, H = 1 << sp.heads_log2, groups = p.kv_count >> sp.heads_log2;
+  const int each = sp.row_most << sp.heads_log2;
+  for (int item = blockIdx.x; item < total * each; item += gridDim.x) {
+    const int unit = list[item / each], rest = item % each, sub = rest & (H - 1), r = rest >> sp.heads_log2;
+    const int4 raw = *reinterpret_cast<const int4*>(sp.notes + unit);
+    const Note note = {raw.x, raw.y, raw.z, raw.w};
+    if (r >= note.rows) continue;
+    float top = kUnset, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = pl; q < note.parts; q += 4 * PL) {
+      float2 st[4];
+      float4 v[4];
 #pragma unroll
-  for (int q = 0; q < 2 * NW; ++q) used |= (unsigned)(wline[q >> 1][q & 1] >= 0) << q;
-  while (used) {
-    const int at = __ffs(used) - 1;
-    const int64_t line = wline[at >> 1][at & 1];
-    unsigned group = 0;
-    for (unsigned left = used; left; left &= left - 1) {
-      const int q = __ffs(left) - 1;
-      if (wline[q >> 1][q & 1] != line) break;
-      group |= 1u << q;
+      for (int u = 0; u < 4; ++u) {
+        const int part = min(q + u * PL, note.parts - 1);
+        const int64_t from = (((int64_t)(2 * (unit + part) + (part == 0)) << sp.heads_log2) + sub) * sp.row_most + r;
+        st[u] = __ldcg(sp.stats + from);
+        v[u] = __ldcg(reinterpret_cast<const float4*>(sp.partial + from * DP) + x);
+      }
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) now = fmaxf(now, st[u].x);
+      const float keep = ex2_approx(top - now);
+      top = now;
+      sum *= keep;
+      o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (q + u * PL >= note.parts) continue;
+        const float f = ex2_approx(st[u].x - top);
+        sum += f * st[u].y;
+        o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
+      }
     }
-    used &= ~group;
-    const int b = winfo[at >> 1][at & 1][0], off = winfo[at >> 1][at & 1][1], tiles = winfo[at >> 1][at & 1][2];
-    const Rows rw = rows_of(p, b);
-    const int rows = min(ROWS, rw.count * G - off / p.kv_count * ROWS);
-    const bool early = line < cta_pos, late = line + tiles > cta_end, whole = !early && !late;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (early ? 0 : 1);
-    for (int x = tid; x < rows * (DP / 4); x += NW * 32) {
-      const int r = x / (DP / 4), d = x % (DP / 4) * 4;
-      if (d >= D) continue;
-      float top = kUnset;
-      for (unsigned left = group; left; left &= left - 1) top = fmaxf(top, (&wstat[0][0][0])[(__ffs(left) - 1) * ROWS + r].x);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-      for (unsigned left = group; left; left &= left - 1) {
-        const int q = __ffs(left) - 1;
-        const float2 st = (&wstat[0][0][0])[q * ROWS + r];
+    held[pl][x] = o;
+    if (x == 0) held_stats[pl] = make_float2(top, sum);
+    __syncthreads();
+    const int d = group_column<DP>(x);
+    if (pl == 0 && d < D) {
+#pragma unroll
+      for (int u = 1; u < PL; ++u) top = fmaxf(top, held_stats[u].x);
+      sum = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < PL; ++u) {
+        const float2 st = held_stats[u];
+        const float4 v = held[u][x];
         const float f = ex2_approx(st.x - top);
-        const float4 v = *reinterpret_cast<const float4*>(wacc + (q * ROWS + r) * C::kPitch + d);
         sum += f * st.y;
         o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
       }
-      if (whole) {
-        finish(rw, b, off, r, d, o, top, sum);
-      } else {
-        __stcg(reinterpret_cast<float4*>(sp.partial + (slot * ROWS + r) * DP + d), o);
-        if (d == 0) __stcg(sp.stats + slot * ROWS + r, make_float2(top, sum));
-      }
+      const Rows rw = rows_of(p, note.b);
+      const int chunk = note.off / groups, kvh = p.kv_begin + ((note.off - chunk * groups) << sp.heads_log2) + sub, at = chunk * line_rows + r;
+      const int i = at / G, h = kvh * G + at - i * G;
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      store4(p, query_at(p, p.os, rw, note.b, h, i) + d, sp.out_vec, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (p.lse && x == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
-    if (early) {
-      handed0 = line;
-      at0 = at;
-    } else if (late) {
-      handed1 = line;
-      at1 = at;
-    }
-  }
-  if (handed0 < 0 && handed1 < 0) return;
-  // CTAs first .. first + parts - 1 have a part of such a line; in the CTA where it begins it is the last one, elsewhere the first
-  const int64_t cta_share = share * NW;
-  __syncthreads();
-  if (tid < 2) {
-    const int64_t line = tid ? handed1 : handed0;
-    bool last = false;
-    if (line >= 0) {
-      const int at = tid ? at1 : at0, first = tid ? (int)blockIdx.x : (int)(line / cta_share);
-      const int parts = (int)((line + winfo[at >> 1][at & 1][2] - 1) / cta_share) - first + 1;
-      __threadfence();   // (what the other threads wrote, too: the barrier lies between)
-      last = atomicInc(p.counters + first, parts - 1) == (unsigned)(parts - 1);
-      __threadfence();
-    }
-    last_flag[tid] = last;
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    if (!last_flag[k]) continue;
-    const int64_t line = k ? handed1 : handed0;
-    const int at = k ? at1 : at0;
-    const int* info = winfo[at >> 1][at & 1];
-    const int b = info[0], off = info[1], tiles = info[2];
-    const int first = k ? (int)blockIdx.x : (int)(line / cta_share), parts = (int)((line + tiles - 1) / cta_share) - first + 1;
-    const Rows rw = rows_of(p, b);
-    const int rows = min(ROWS, rw.count * G - off / p.kv_count * ROWS);
-    for (int x = tid; x < rows * (DP / 4); x += NW * 32) {
-      const int r = x / (DP / 4), d = x % (DP / 4) * 4;
-      if (d >= D) continue;
-      float top = kUnset, sum = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < parts; q += 8) {
-        float2 st[8];
-        float4 v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int part = min(q + u, parts - 1);
-          const int64_t from = (int64_t)(2 * (first + part) + (part == 0)) * ROWS + r;
-          st[u] = __ldcg(sp.stats + from);
-          v[u] = __ldcg(reinterpret_cast<const float4*>(sp.partial + from * DP + d));
-        }
-        float now = top;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) now = fmaxf(now, st[u].x);
-        const float keep = ex2_approx(top - now);
-        top = now;
-        sum *= keep;
-        o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (q + u >= parts) continue;
-          const float f = ex2_approx(st[u].x - top);
-          sum += f * st[u].y;
-          o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
-        }
-      }
-      finish(rw, b, off, r, d, o, top, sum);
-    }
+    __syncthreads();
   }
 }
 
@@ -725,18 +716,31 @@ int resident(int num_sms) {
     }
     return n;
   }();
-  const int n = ctas * num_sms;
-  return n < 1 ? 1 : (n < kCounters ? n : kCounters);
+  const int n = ctas * num_sms, most = kMostUnits / Config<DP, NR, T, UB>::kWarps;
+  return n < 1 ? 1 : (n < most ? n : most);
 }
 
-// One instantiation: its workspace, or its launch (workspace null: the lines are not cut).
+// One instantiation: its workspace, or its launches (workspace null: the lines are not cut).
 template <int DP, int NR, int T, bool UB>
-cudaError_t one(const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
+cudaError_t one(const Attend* p, const Sizes& z, void* workspace, int64_t* bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
   using C = Config<DP, NR, T, UB>;
-  const int grid = resident<DP, NR, T, UB>(num_sms);
-  const int64_t acc = (int64_t)2 * grid * C::kRows * DP * 4;
+  const int most = resident<DP, NR, T, UB>(z.num_sms);
+  Split sp;
+  sp.row_most = (int)(z.rows < C::kRows ? z.rows : C::kRows);
+  sp.least = 2;
+  sp.heads_log2 = 0;
+  while ((2 << sp.heads_log2) <= C::kWarps && z.kv_count % (2 << sp.heads_log2) == 0) ++sp.heads_log2;
+  const int units_cta = C::kWarps >> sp.heads_log2;
+  // no more units than there can be shares (or, uncut, lines)
+  const int64_t lines = z.batch * ((z.rows + C::kRows - 1) / C::kRows) * (z.kv_count >> sp.heads_log2);
+  const int64_t shares = (lines * (z.seq_kv > 0 ? (z.seq_kv + kTile - 1) / kTile : 1) + sp.least - 1) / sp.least;
+  auto grid_for = [&](int64_t n) { return (int)((n + units_cta - 1) / units_cta < most ? (n + units_cta - 1) / units_cta : most); };
+  int grid = grid_for(shares);   // (at least one: a call has sequences, queries and room for keys)
+  sp.units = grid * units_cta;
+  const int64_t rows = (int64_t)2 * grid * C::kWarps * sp.row_most, acc = rows * DP * 4;
+  const int64_t need = acc + (rows * 8 + 15) / 16 * 16 + sp.units * (int64_t)sizeof(Note);
   if (bytes) {
-    *bytes = acc + (int64_t)2 * grid * C::kRows * 8;
+    if (*bytes < need) *bytes = need;
     return cudaSuccess;
   }
   auto k = kv8_split_kernel<DP, NR, T, UB>;
@@ -746,35 +750,45 @@ cudaError_t one(const Attend* p, int num_sms, void* workspace, int64_t* bytes, u
     if (e != cudaSuccess) return e;
     *raised |= 1ull << id;
   }
-  Split sp;
+  if (z.workspace_bytes < need || (uintptr_t)workspace % 16 != 0) workspace = nullptr;
   sp.partial = static_cast<float*>(workspace);
   sp.stats = workspace ? reinterpret_cast<float2*>(static_cast<char*>(workspace) + acc) : nullptr;
-  sp.least = 2;
+  sp.notes = workspace ? reinterpret_cast<Note*>(static_cast<char*>(workspace) + need) - sp.units : nullptr;
+  if (!workspace) {
+    grid = grid_for(lines);
+    sp.units = grid * units_cta;
+  }
   auto vec = [](const void* ptr, const int64_t* st, int esz, int bytes) {
     return ((uintptr_t)ptr | (uint64_t)(st[0] * esz) | (uint64_t)(st[1] * esz) | (uint64_t)(st[2] * esz)) % bytes == 0;
   };
   sp.query_vec = vec(p->q, p->qs, p->dtype == AIDN_F32 ? 4 : 2, 16);
   sp.out_vec = vec(p->out, p->os, p->out_f32 ? 4 : 2, p->out_f32 ? 16 : 8);
-  return launch_dependent(k, dim3((unsigned)grid), C::kWarps * 32, C::kSmem, stream, *p, sp);
+  const cudaError_t e = launch_dependent(k, dim3((unsigned)grid), C::kWarps * 32, C::kSmem, stream, *p, sp);
+  *launches = 1;
+  if (e != cudaSuccess || !workspace) return e;
+  *launches = 2;
+  const int64_t items = (lines < sp.units ? lines : sp.units) * ((int64_t)sp.row_most << sp.heads_log2);
+  const int64_t merge = items < 8 * z.num_sms ? items : 8 * z.num_sms;
+  return launch_dependent(kv8_split_merge_kernel<DP>, dim3((unsigned)merge), kMergeThreads, 0, stream, *p, sp, C::kRows);
 }
 
 template <int DP, int NR, int T>
-cudaError_t pick_block(bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
-  return ub ? one<DP, NR, T, true>(p, num_sms, workspace, bytes, raised, stream) : one<DP, NR, T, false>(p, num_sms, workspace, bytes, raised, stream);
+cudaError_t pick_block(bool ub, const Attend* p, const Sizes& z, void* workspace, int64_t* bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  return ub ? one<DP, NR, T, true>(p, z, workspace, bytes, raised, launches, stream) : one<DP, NR, T, false>(p, z, workspace, bytes, raised, launches, stream);
 }
 template <int DP, int T>
-cudaError_t pick_rows(int64_t rows, bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
-  if (rows <= 8) return pick_block<DP, 1, T>(ub, p, num_sms, workspace, bytes, raised, stream);
-  return pick_block<DP, 2, T>(ub, p, num_sms, workspace, bytes, raised, stream);
+cudaError_t pick_rows(bool ub, const Attend* p, const Sizes& z, void* workspace, int64_t* bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  if (z.rows <= 8) return pick_block<DP, 1, T>(ub, p, z, workspace, bytes, raised, launches, stream);
+  return pick_block<DP, 2, T>(ub, p, z, workspace, bytes, raised, launches, stream);
 }
 template <int DP>
-cudaError_t pick(bool exact, int64_t rows, bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
-  return exact ? pick_rows<DP, 2>(rows, ub, p, num_sms, workspace, bytes, raised, stream) : pick_rows<DP, 1>(rows, ub, p, num_sms, workspace, bytes, raised, stream);
+cudaError_t pick(bool exact, bool ub, const Attend* p, const Sizes& z, void* workspace, int64_t* bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  return exact ? pick_rows<DP, 2>(ub, p, z, workspace, bytes, raised, launches, stream) : pick_rows<DP, 1>(ub, p, z, workspace, bytes, raised, launches, stream);
 }
-cudaError_t pick_dim(int dim, bool exact, int64_t rows, bool ub, const Attend* p, int num_sms, void* workspace, int64_t* bytes, uint64_t* raised, cudaStream_t stream) {
-  if (dim <= 64) return pick<64>(exact, rows, ub, p, num_sms, workspace, bytes, raised, stream);
-  if (dim <= 128) return pick<128>(exact, rows, ub, p, num_sms, workspace, bytes, raised, stream);
-  return pick<256>(exact, rows, ub, p, num_sms, workspace, bytes, raised, stream);
+cudaError_t pick_dim(int dim, bool exact, bool ub, const Attend* p, const Sizes& z, void* workspace, int64_t* bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  if (dim <= 64) return pick<64>(exact, ub, p, z, workspace, bytes, raised, launches, stream);
+  if (dim <= 128) return pick<128>(exact, ub, p, z, workspace, bytes, raised, launches, stream);
+  return pick<256>(exact, ub, p, z, workspace, bytes, raised, launches, stream);
 }
 
 }  // namespace
@@ -787,23 +801,15 @@ bool split_supported(const Attend& p) {
   return true;
 }
 // (whatever the block size: the larger of the two kernels' needs)
-int64_t split_workspace_bytes(int head_dim, bool exact, int64_t rows, int num_sms) {
+int64_t split_workspace_bytes(int head_dim, bool exact, int64_t batch, int64_t rows, int64_t seq_kv, int kv_count, int num_sms) {
   int64_t most = 0;
-  for (int ub = 0; ub < 2; ++ub) {
-    int64_t n = 0;
-    pick_dim(head_dim, exact, rows, ub, nullptr, num_sms, nullptr, &n, nullptr, nullptr);
-    if (n > most) most = n;
-  }
+  const Sizes z = {batch, rows, seq_kv, kv_count, num_sms, 0};
+  for (int ub = 0; ub < 2; ++ub) pick_dim(head_dim, exact, ub, nullptr, z, nullptr, &most, nullptr, nullptr, nullptr);
   return most;
 }
-cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, cudaStream_t stream) {
-  const bool exact = p.out_f32 != 0;
-  const int64_t rows = p.seq_q * p.group;
-  const bool ub = p.c.block_size % kTile == 0;
-  int64_t need = 0;
-  pick_dim(p.c.head_dim, exact, rows, ub, nullptr, num_sms, nullptr, &need, nullptr, nullptr);
-  if (workspace_bytes < need || (uintptr_t)workspace % 16 != 0) workspace = nullptr;
-  return pick_dim(p.c.head_dim, exact, rows, ub, &p, num_sms, workspace, nullptr, raised, stream);
+cudaError_t launch_attend_split(const Attend& p, int num_sms, void* workspace, int64_t workspace_bytes, uint64_t* raised, int* launches, cudaStream_t stream) {
+  const Sizes z = {p.batch, p.seq_q * p.group, p.seq_kv, p.kv_count, num_sms, workspace_bytes};
+  return pick_dim(p.c.head_dim, p.out_f32 != 0, p.c.block_size % kTile == 0, &p, z, workspace, nullptr, raised, launches, stream);
 }
 
 }  // namespace kv8
