@@ -13,7 +13,8 @@
 // (11 bits, of 2^9 times their value so that they stay normal down to 2^-23 of the largest); for fp32 results they are two terms too.
 //
 // The warps of a "unit" do the same tiles of neighbouring KV heads, whose rows are neighbours in the pool: memory is read in runs
-// of up to 1 KB (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 240 us, and 279 us where each warp went through lines of its own).  The
+// of up to 1 KB (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 228 us, and 265 us
+// where each warp goes through lines of its own).  The
 // lines' tiles are one row, cut into equal shares for the units that are resident whatever the lengths are.  No warp waits for
 // another one: a line that is cut leaves a partial result a unit in the workspace, and a second launch merges them in their order, so that
 // the result does not depend on which was first.
@@ -29,7 +30,7 @@ constexpr float kUnset = -1e30f;    // running maximum before any key
 constexpr float kLazy = 6.f;        // the maximum follows when a logit is 2^6 above it: weights stay below 2^(9 + 6), in fp16's range
 constexpr float kLift = 9.f;
 constexpr int kMergeThreads = 256;
-constexpr int kMostUnits = 4096;
+constexpr int kMostUnits = 4096;   // (twelve bits in the merging kernel)
 
 // A line that is cut: begun by unit `at` of the list, parts of it in the `parts - 1` units behind.
 struct Note {
@@ -70,41 +71,8 @@ __device__ __forceinline__ float lds_f(uint32_t at) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
   return r;
 }
-// Sixteen elements of a query as they lie: eight words of 16-bit elements, sixteen of 32-bit ones.  (Volatile: issued where they stand.)
-__device__ __forceinline__ void ld_words4(const void* ptr, uint32_t* w) {
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(ptr));
-}
-template <int T>
-__device__ __forceinline__ void load16(const Attend& p, int64_t at, bool vec, uint32_t* w) {
-  if (T == 2 && p.dtype == AIDN_F32) {
-    const float* q = static_cast<const float*>(p.q) + at;
-#pragma unroll
-    for (int e = 0; e < 8 * T; e += 4) {
-      if (vec) {
-        ld_words4(q + e, w + e);
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) w[e + u] = __float_as_uint(q[e + u]);
-      }
-    }
-    return;
-  }
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
-#pragma unroll
-  for (int e = 0; e < 8; e += 4) {
-    if (vec) {
-      ld_words4(q + 2 * e, w + e);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w[e + u] = q[2 * (e + u)] | (uint32_t)q[2 * (e + u) + 1] << 16;
-    }
-  }
-}
-template <int T>
-__device__ __forceinline__ float widen(const Attend& p, const uint32_t* w, int e) {
-  if (T == 2 && p.dtype == AIDN_F32) return __uint_as_float(w[T == 2 ? e : 0]);
-  const uint32_t v = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-  return p.dtype == AIDN_F16 ? __half2float(__ushort_as_half((unsigned short)v)) : __uint_as_float(v << 16);
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void store4(const Attend& p, int64_t at, bool vec, float4 o) {
   if (p.out_f32) {
@@ -134,12 +102,6 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   return x & ~(hit * 0xffu);
 }
 
-// First element of group x of four: groups of a row lie in the workspace in the order in which lanes hold them.
-template <int DP>
-__device__ __forceinline__ int group_column(int x) {
-  return DP == 64 ? 8 * (x & 7) + 4 * (x >> 3) : 128 * (x >> 5) + 16 * (x & 7) + 4 * (x >> 3 & 3);
-}
-
 // What the host knows of a call.
 struct Sizes {
   int64_t batch, rows, seq_kv;   // rows: of a sequence and KV head, at most
@@ -156,8 +118,7 @@ struct Config {
   static constexpr int kQueryBytes = T * NR * kSteps * 32 * 8;   // of a warp
   static constexpr int kScales = UB ? 16 : 128;                  // bytes of a stage: the block's two, or those of 16 keys
   static constexpr int kStage = 2 * kTile * DP + kScales;
-  // three tiles of a warp are in shared memory or on their way to it, two where three would cost a CTA
-  static constexpr int kStages = kWarps * (kQueryBytes + 3 * kStage) + 1024 <= 233472 / kMinCtas ? 3 : 2;
+  static constexpr int kStages = 2;   // tiles of a warp in shared memory or on their way to it (with three: 228 us, and 208, of the case above)
   static constexpr size_t kSmem = (size_t)kWarps * (kQueryBytes + kStages * kStage);
 };
 
@@ -177,7 +138,9 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * C::kStage;
-  uint2* const qfrag = reinterpret_cast<uint2*>(smem + NW * STAGES * C::kStage + warp * C::kQueryBytes);   // [T][NR][KS][32]
+  // Fragments of the queries, [NR][SLOTS][32 lanes] of 16 bytes: two steps, or the two terms of one
+  constexpr int SLOTS = T == 1 ? KS / 2 : KS, SLOT = T == 1 ? 8 : 4;   // elements
+  uint4* const qfrag = reinterpret_cast<uint4*>(smem + NW * STAGES * C::kStage + warp * C::kQueryBytes);
   const int D = p.c.head_dim, G = p.group, groups = p.kv_count >> sp.heads_log2;
   const int unit = ((int)blockIdx.x * NW + warp) >> sp.heads_log2, sub = warp & ((1 << sp.heads_log2) - 1);
   const bool cut = sp.partial != nullptr;
@@ -258,18 +221,36 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       if (window + 32 + lane <= last_block) entry_n = table[window + 32 + lane];
     }
 
-    // the queries are on their way while the first keys are looked up: lane (g, t) takes of row g (of eight) what it is to multiply with
-    uint32_t qr[NR][KC][8 * T];
-#pragma unroll
+    // The queries are on their way while the first keys are looked up.  Lane (g, t) copies of row g (of eight) what it will multiply with to where
+    // the fragments of it will be.
+    __syncwarp();   // (the last line's tiles and queries have been read)
+#pragma unroll 1
     for (int n = 0; n < NR; ++n) {
-      const int r = 8 * n + g;
-      if (r >= rows) continue;
-      const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-      const int64_t at = query_at(p, p.qs, rw, b, h, i);
-#pragma unroll
-      for (int j = 0; j < KC; ++j)
-        if (column(j, t) < D) load16<T>(p, at + column(j, t), sp.query_vec, qr[n][j]);
+      const int r = 8 * n + g, i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+      const int64_t at = r < rows ? query_at(p, p.qs, rw, b, h, i) : 0;
+      const bool wide = T == 2 && p.dtype == AIDN_F32;
+      const int64_t esz = wide ? 4 : 2;
+#pragma unroll 2
+      for (int x = 0; x < SLOTS; ++x) {
+        const int d = T == 1 ? column(x >> 1, t) + 8 * (x & 1) : column(x >> 2, t) + 4 * (x & 3);
+        uint4* const dst = qfrag + (n * SLOTS + x) * 32 + lane;
+        const uint8_t* const src = static_cast<const uint8_t*>(p.q) + (at + d) * esz;
+        if (r >= rows || d >= D) {
+          *dst = make_uint4(0, 0, 0, 0);
+        } else if (sp.query_vec) {
+          const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+          if (T == 1 || wide) copy16(to, src);
+          else copy8(to, src);
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < SLOT; ++e) {
+            if (wide) reinterpret_cast<uint32_t*>(dst)[e] = reinterpret_cast<const uint32_t*>(src)[e];
+            else reinterpret_cast<uint16_t*>(dst)[e] = reinterpret_cast<const uint16_t*>(src)[e];
+          }
+        }
+      }
     }
+    cp_async_commit();
 
     // A tile's keys and values go to shared memory, 16 bytes a lane and copy.  All of them exist: where a row is shorter than DP bytes its
     // first chunk comes again (the queries are zero there, and those values are not written), and keys behind the last one, or of a
@@ -331,7 +312,6 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       }
     };
     int stage = 0;
-    __syncwarp();   // (the last line's tiles and queries have been read)
 #pragma unroll 1
     for (int a = 0; a < STAGES - 1; ++a) {
       if (t0 + a < t_end) issue(t0 + a, a);
@@ -339,45 +319,77 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     }
 
     // ---- queries: scaled by a power of two so that the largest element is in [2^12, 2^13), as fragments
+    cp_async_wait<STAGES - 1>();   // (the tiles are behind them)
+    auto values = [&](uint4 w, float* x) {
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      if (T == 2 && p.dtype == AIDN_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(u[e]);
+      } else if (p.dtype == AIDN_F16) {
+#pragma unroll
+        for (int e = 0; e < SLOT / 2; ++e) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+          x[2 * e] = f.x;
+          x[2 * e + 1] = f.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < SLOT / 2; ++e) {
+          x[2 * e] = __uint_as_float(u[e] << 16);
+          x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+        }
+      }
+    };
+    constexpr int UNROLL = SLOTS <= 4 ? SLOTS : 2;   // (code that runs once a line is fetched once a line)
     float c_row[NR];
     int lim_row[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = 8 * n + g;
-      const bool valid = r < rows;
-      float largest = 0.f;
+      uint4* const mine = qfrag + n * SLOTS * 32 + lane;
+      uint32_t most = 0;   // the largest magnitudes by their bits (a NaN makes the row's logits NaN whatever the factor)
+#pragma unroll UNROLL
+      for (int x = 0; x < SLOTS; ++x) {
+        const uint4 w = mine[x * 32];
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        if (T == 2 && p.dtype == AIDN_F32) {
 #pragma unroll
-      for (int j = 0; j < KC; ++j)
-        if (valid && column(j, t) < D) {
+          for (int e = 0; e < 4; ++e) most = max(most, u[e] & 0x7fffffffu);
+        } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) largest = fmaxf(largest, fabsf(widen<T>(p, qr[n][j], e)));
+          for (int e = 0; e < SLOT / 2; ++e) most = __vmaxu2(most, u[e] & 0x7fff7fffu);
         }
+      }
+      float largest = __uint_as_float(most);
+      if (T == 1 || p.dtype != AIDN_F32) {
+        most = max(most >> 16, most & 0xffffu);
+        largest = p.dtype == AIDN_F16 ? __half2float(__ushort_as_half((unsigned short)most)) : __uint_as_float(most << 16);
+      }
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
       int up = 12 - ((int)(__float_as_uint(largest) >> 23) - 127);   // (zeros and what is below the normal floats: 2^126)
       up = max(-110, min(up, 126));
       const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+#pragma unroll UNROLL
+      for (int x = 0; x < SLOTS; ++x) {
+        float v[SLOT];
+        values(mine[x * 32], v);
+        uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < KC; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          __half2 hi[2] = {}, lo[2] = {};
-          if (valid && column(j, t) < D) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float a = widen<T>(p, qr[n][j], 4 * i + 2 * e) * f, c = widen<T>(p, qr[n][j], 4 * i + 2 * e + 1) * f;
-              hi[e] = __floats2half2_rn(a, c);
-              if (T == 2) lo[e] = __floats2half2_rn(a - __low2float(hi[e]), c - __high2float(hi[e]));
-            }
+        for (int e = 0; e < SLOT / 2; ++e) {
+          const float a = v[2 * e] * f, c = v[2 * e + 1] * f;
+          const __half2 hi = __floats2half2_rn(a, c);
+          w[e] = *reinterpret_cast<const uint32_t*>(&hi);
+          if (T == 2) {
+            const __half2 lo = __floats2half2_rn(a - __low2float(hi), c - __high2float(hi));
+            w[T == 2 ? 2 + e : e] = *reinterpret_cast<const uint32_t*>(&lo);
           }
-          uint2* const dst = qfrag + (n * KS + 4 * j + i) * 32 + lane;
-          dst[0] = make_uint2(*reinterpret_cast<uint32_t*>(&hi[0]), *reinterpret_cast<uint32_t*>(&hi[1]));
-          if (T == 2) dst[NR * KS * 32] = make_uint2(*reinterpret_cast<uint32_t*>(&lo[0]), *reinterpret_cast<uint32_t*>(&lo[1]));
         }
+        mine[x * 32] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
       c_row[n] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * (p.softcap > 0.f ? 1.f : kLog2e);
-      lim_row[n] = !valid ? keys : (rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + r) / G));
+      lim_row[n] = r >= rows ? keys : (rw.count == 1 ? lim_least : visible(p, keys, rw.count, (r0 + r) / G));
     }
-    __syncwarp();
 
     float acc[NR][MT][4];
     float m[NR][2], l[NR][2], c[NR][2];
@@ -433,16 +445,22 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
         const int chunk = DP == 64 ? t : 8 * (q >> 1) + 2 * t + (q & 1);
         const uint4 x0 = lds16(at + key_chunk(g, chunk)), x1 = lds16(at + key_chunk(g, chunk) + 8 * DP);
         const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+        uint4 bq[NR];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t a0 = codes_to_f16(w0[i]), a1 = codes_to_f16(w1[i]), a2 = codes_to_f16_hi(w0[i]), a3 = codes_to_f16_hi(w1[i]);
 #pragma unroll
-          for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int term = 0; term < T; ++term) {
-              const uint2 bq = qfrag[((term * NR + n) * KS + 4 * q + i) * 32 + lane];
-              mma16816<__half>(s[n], a0, a1, a2, a3, bq.x, bq.y);
+          for (int n = 0; n < NR; ++n) {
+            if constexpr (T == 1) {
+              if (i % 2 == 0) bq[n] = qfrag[(n * SLOTS + 2 * q + i / 2) * 32 + lane];
+              if (i % 2 == 0) mma16816<__half>(s[n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+              else mma16816<__half>(s[n], a0, a1, a2, a3, bq[n].z, bq[n].w);
+            } else {
+              bq[n] = qfrag[(n * SLOTS + 4 * q + i) * 32 + lane];
+              mma16816<__half>(s[n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+              mma16816<__half>(s[n], a0, a1, a2, a3, bq[n].z, bq[n].w);
             }
+          }
         }
       }
       uint4 vr[4][VC];   // keys 2t, 2t + 1, 2t + 8, 2t + 9
@@ -576,53 +594,72 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
       }
-    const int64_t part = ((int64_t)(2 * unit + (t0 == 0 ? 1 : 0)) << sp.heads_log2) + sub;
+    // (row r's to lane r; its elements through the tiles' place, in which no copy is under way, groups of four in an order without conflicts)
+    float my_top = 0.f, my_sum = 0.f;
+    cp_async_wait<0>();
+    __syncwarp();
+    float* const rows_at = reinterpret_cast<float*>(smem + warp * STAGES * C::kStage);
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = 8 * n + 2 * t + e;
-        if (r >= rows) continue;
-        if (!whole) {   // (a lane's groups of four elements lie 8 groups apart: a line of 128 bytes is written at a time)
-          const int64_t to = part * sp.row_most + r;
-          float4* const dst = reinterpret_cast<float4*>(sp.partial + to * DP) + g;
-#pragma unroll
-          for (int j = 0; j < MT; j += 2)
-            __stcg(dst + 4 * j, make_float4(acc[n][j][e] * vref, acc[n][j][e + 2] * vref, acc[n][j + 1][e] * vref, acc[n][j + 1][e + 2] * vref));
-          if (g == 0) __stcg(sp.stats + to, make_float2(m[n][e] - kLift, sum[n][e]));
-          continue;
+        const float top_e = __shfl_sync(0xffffffffu, m[n][e] - kLift, lane >> 1 & 3), sum_e = __shfl_sync(0xffffffffu, sum[n][e], lane >> 1 & 3);
+        if (lane >> 3 == n && (lane & 1) == e) {
+          my_top = top_e;
+          my_sum = sum_e;
         }
-        const float f = sum[n][e] == 0.f ? 0.f : vref / sum[n][e];
-        const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-        const int64_t to = query_at(p, p.os, rw, b, h, i);
+        float* const to = rows_at + (8 * n + 2 * t + e) * DP;
 #pragma unroll
         for (int j = 0; j < MT; j += 2) {
-          const int d = group_column<DP>(4 * j + g);
-          if (d < D) store4(p, to + d, sp.out_vec, make_float4(acc[n][j][e] * f, acc[n][j][e + 2] * f, acc[n][j + 1][e] * f, acc[n][j + 1][e + 2] * f));
+          const int d = DP == 256 ? 128 * (j / 8) + 16 * g + 2 * (j % 8) : VB * g + 2 * j;
+          *reinterpret_cast<float4*>(to + (d ^ 4 * t)) = make_float4(acc[n][j][e], acc[n][j][e + 2], acc[n][j + 1][e], acc[n][j + 1][e + 2]);
         }
-        if (p.lse && g == 0) *lse_at(p, rw, h, i) = sum[n][e] == 0.f ? -INFINITY : (m[n][e] - kLift + log2f(sum[n][e])) * kLn2;
       }
+    __syncwarp();
+    const int64_t part = ((int64_t)(2 * unit + (t0 == 0 ? 1 : 0)) << sp.heads_log2) + sub;
+    const float mine_f = !whole ? vref : (my_sum == 0.f ? 0.f : vref / my_sum);
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      const float f = __shfl_sync(0xffffffffu, mine_f, r);
+      const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+      const int64_t to = whole ? query_at(p, p.os, rw, b, h, i) : (part * sp.row_most + r) * DP;
+#pragma unroll 1
+      for (int d = lane * 4; d < D; d += 128) {
+        float4 o = *reinterpret_cast<const float4*>(rows_at + r * DP + (d ^ 4 * (r >> 1 & 3)));
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+        if (whole) store4(p, to + d, sp.out_vec, o);
+        else __stcg(reinterpret_cast<float4*>(sp.partial + to + d), o);
+      }
+      if (lane != r) continue;
+      if (!whole) __stcg(sp.stats + part * sp.row_most + r, make_float2(my_top, my_sum));
+      else if (p.lse) *lse_at(p, rw, h, i) = my_sum == 0.f ? -INFINITY : (my_top + log2f(my_sum)) * kLn2;
+    }
   }
-  cp_async_wait<0>();
   if (cut && sub == 0 && lane == 0 && unit < sp.units) *reinterpret_cast<int4*>(sp.notes + unit) = make_int4(note.parts, note.b, note.off, note.rows);
   if (bad && p.status) atomicOr(p.status, kStatusBadBlock);
 }
 
-// The cut lines' parts: a CTA takes rows (of a line, a head) in turn, its threads four elements of some of the parts each.
+// The cut lines' parts: warps take rows in turn, or, where a line has many parts (and so there are few lines), CTAs; four elements a lane.
 template <int DP>
-__global__ void __launch_bounds__(kMergeThreads) kv8_split_merge_kernel(const __grid_constant__ Attend p, const __grid_constant__ Split sp, int line_rows) {
-  constexpr int C4 = DP / 4, PL = kMergeThreads / C4, WARPS = kMergeThreads / 32;
+__global__ void __launch_bounds__(kMergeThreads, 4) kv8_split_merge_kernel(const __grid_constant__ Attend p, const __grid_constant__ Split sp, int line_rows) {
+  constexpr int C4 = DP / 4, PL = kMergeThreads / C4, WARPS = kMergeThreads / 32, AHEAD = 4;
+  constexpr int SMALL = 16;
   __shared__ int counts[WARPS];
-  __shared__ uint16_t list[kMostUnits];
+  __shared__ uint32_t list[kMostUnits];   // units, their lines' parts and rows
   __shared__ float4 held[PL][C4];
   __shared__ float2 held_stats[PL];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, x = tid % C4, pl = tid / C4;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   pdl_trigger();
   // the units that began a line which is cut
   const int per = (sp.units + kMergeThreads - 1) / kMergeThreads, u_lo = min(tid * per, sp.units), u_hi = min(u_lo + per, sp.units);
   int mine = 0;
-  for (int u = u_lo; u < u_hi; ++u) mine += sp.notes[u].parts > 0;
+  bool many = false;
+  for (int u = u_lo; u < u_hi; ++u) {
+    const int parts = sp.notes[u].parts;
+    mine += parts > 0;
+    many = many || parts > SMALL;
+  }
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -630,7 +667,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv8_split_merge_kernel(const __
     if (lane >= o) upto += v;
   }
   if (lane == 31) counts[warp] = upto;
-  __syncthreads();
+  many = __syncthreads_or(many);
   int total = 0, to = upto - mine;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
@@ -639,68 +676,86 @@ __global__ void __launch_bounds__(kMergeThreads) kv8_split_merge_kernel(const __
   }
   if (mine > 0)
     for (int u = u_lo; u < u_hi; ++u)
-      if (sp.notes[u].parts > 0) list[to++] = (uint16_t)u;
+      if (sp.notes[u].parts > 0) list[to++] = (uint32_t)u | (uint32_t)sp.notes[u].parts << 12 | (uint32_t)sp.notes[u].rows << 25;
   __syncthreads();
 
   const int D = p.c.head_dim, G = p.group, H = 1 << sp.heads_log2, groups = p.kv_count >> sp.heads_log2;
-  const int each = sp.row_most << sp.heads_log2;
-  for (int item = blockIdx.x; item < total * each; item += gridDim.x) {
-    const int unit = list[item / each], rest = item % each, sub = rest & (H - 1), r = rest >> sp.heads_log2;
-    const int4 raw = *reinterpret_cast<const int4*>(sp.notes + unit);
-    const Note note = {raw.x, raw.y, raw.z, raw.w};
-    if (r >= note.rows) continue;
-    float top = kUnset, sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = pl; q < note.parts; q += 4 * PL) {
-      float2 st[4];
-      float4 v[4];
+  const int items = total * sp.row_most << sp.heads_log2;
+  float top, sum;
+  float4 o;
+  // parts first, first + step, ... of row r: four elements from the 4 x-th on
+  auto join = [&](int parts, int unit, int sub, int r, int x, int first, int step) {
+    top = kUnset;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int q = first; q < parts; q += AHEAD * step) {
+      float2 st[AHEAD];
+      float4 v[AHEAD];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int part = min(q + u * PL, note.parts - 1);
+      for (int u = 0; u < AHEAD; ++u) {
+        const int part = min(q + u * step, parts - 1);
         const int64_t from = (((int64_t)(2 * (unit + part) + (part == 0)) << sp.heads_log2) + sub) * sp.row_most + r;
         st[u] = __ldcg(sp.stats + from);
         v[u] = __ldcg(reinterpret_cast<const float4*>(sp.partial + from * DP) + x);
       }
       float now = top;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) now = fmaxf(now, st[u].x);
+      for (int u = 0; u < AHEAD; ++u) now = fmaxf(now, st[u].x);
       const float keep = ex2_approx(top - now);
       top = now;
       sum *= keep;
       o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (q + u * PL >= note.parts) continue;
+      for (int u = 0; u < AHEAD; ++u) {
+        if (q + u * step >= parts) continue;
         const float f = ex2_approx(st[u].x - top);
         sum += f * st[u].y;
         o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
       }
     }
-    held[pl][x] = o;
-    if (x == 0) held_stats[pl] = make_float2(top, sum);
-    __syncthreads();
-    const int d = group_column<DP>(x);
-    if (pl == 0 && d < D) {
+  };
+  const int each = sp.row_most << sp.heads_log2, step = many ? gridDim.x : gridDim.x * WARPS;
+#pragma unroll 1
+  for (int item = many ? blockIdx.x : blockIdx.x * WARPS + warp; item < items; item += step) {
+    const int line = item / each, rest = item - line * each, sub = rest & (H - 1), r = rest >> sp.heads_log2;
+    const int unit = list[line] & 4095, parts = list[line] >> 12 & 8191;
+    if (r >= list[line] >> 25) continue;
+    const int b = sp.notes[unit].b, off = sp.notes[unit].off;
+#pragma unroll 1
+    for (int x = many ? tid % C4 : lane; x < C4; x += many ? C4 : 32) {
+      join(parts, unit, sub, r, x, many ? tid / C4 : 0, many ? PL : 1);
+      if (many) {
+        const int pl = tid / C4;
+        held[pl][x] = o;
+        if (x == 0) held_stats[pl] = make_float2(top, sum);
+        __syncthreads();
+        if (pl == 0) {
 #pragma unroll
-      for (int u = 1; u < PL; ++u) top = fmaxf(top, held_stats[u].x);
-      sum = 0.f;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int u = 1; u < PL; ++u) top = fmaxf(top, held_stats[u].x);
+          sum = 0.f;
+          o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < PL; ++u) {
-        const float2 st = held_stats[u];
-        const float4 v = held[u][x];
-        const float f = ex2_approx(st.x - top);
-        sum += f * st.y;
-        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+          for (int u = 0; u < PL; ++u) {
+            const float2 st = held_stats[u];
+            const float4 v = held[u][x];
+            const float f = ex2_approx(st.x - top);
+            sum += f * st.y;
+            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+          }
+        }
+        __syncthreads();
+        if (pl != 0) continue;
       }
-      const Rows rw = rows_of(p, note.b);
-      const int chunk = note.off / groups, kvh = p.kv_begin + ((note.off - chunk * groups) << sp.heads_log2) + sub, at = chunk * line_rows + r;
+      const int d = 4 * x;
+      if (d >= D) continue;
+      const Rows rw = rows_of(p, b);
+      const int chunk = off / groups, kvh = p.kv_begin + ((off - chunk * groups) << sp.heads_log2) + sub, at = chunk * line_rows + r;
       const int i = at / G, h = kvh * G + at - i * G;
       const float f = sum == 0.f ? 0.f : 1.f / sum;
-      store4(p, query_at(p, p.os, rw, note.b, h, i) + d, sp.out_vec, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      store4(p, query_at(p, p.os, rw, b, h, i) + d, sp.out_vec, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
       if (p.lse && x == 0) *lse_at(p, rw, h, i) = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
-    __syncthreads();
   }
 }
 
