@@ -132,11 +132,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
   constexpr int VC = DP == 256 ? 2 : 1;
   constexpr int CPR = DP / 16, RPI = 32 / CPR, NI = kTile / RPI;   // 16-byte chunks of a row; rows and copies of a warp's instruction
   extern __shared__ __align__(128) uint8_t smem[];
-  // (the sums of the scan lie where the tiles will)
-  int64_t* const scan = reinterpret_cast<int64_t*>(smem);
-  int64_t* const prefix = scan + NW;
-
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * C::kStage;
   // Fragments of the queries, [NR][SLOTS][32 lanes] of 16 bytes: two steps, or the two terms of one
   constexpr int SLOTS = T == 1 ? KS / 2 : KS, SLOT = T == 1 ? 8 : 4;   // elements
@@ -150,43 +146,32 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 
   auto tiles_of = [&](int keys) { return keys > kTile ? (keys + kTile - 1) / kTile : 1; };
   auto lines_of = [&](int n) { return ((n * G + ROWS - 1) / ROWS) * groups; };
-  auto weight_of = [&](int b) { return (int64_t)lines_of(rows_of(p, b).count) * (cut ? tiles_of(keys_of(p, b)) : 1); };
+  auto weight_of = [&](int b) { return lines_of(rows_of(p, b).count) * (cut ? tiles_of(keys_of(p, b)) : 1); };
 
-  // ---- the share of this unit: the threads sum up their sequences' tiles
-  const int per = (p.batch + NW * 32 - 1) / (NW * 32);
-  const int b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  int64_t mine = 0;
+  // ---- the share of this unit: the lanes sum up their sequences' tiles (of each warp: there is nothing to wait for.  The host cuts lines
+  // only where all tiles together are fewer than 2^31)
+  const int per = (p.batch + 31) >> 5;
+  const int b_lo = min(lane * per, p.batch), b_hi = min(b_lo + per, p.batch);
+  int mine = 0;
+#pragma unroll 4
   for (int b = b_lo; b < b_hi; ++b) mine += weight_of(b);
-  int64_t upto = mine;
+  int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
-  if (lane == 31) scan[warp] = upto;
-  __syncthreads();
-  int64_t total = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w == warp) before = total;
-    total += scan[w];
-  }
-  prefix[tid] = before + upto - mine;
-  __syncthreads();
-  int64_t share = total < 0x7fffffff - sp.units ? ((int)total + sp.units - 1) / sp.units : (total + sp.units - 1) / sp.units;
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
+  int share = (int)(((uint32_t)total + sp.units - 1) / (uint32_t)sp.units);
   if (cut && share < sp.least) share = sp.least;
-  int64_t pos = unit < sp.units ? min(unit * share, total) : total;
-  const int64_t end = min(pos + share, total);
-  int b = 0;
-  int64_t base = 0;
-  if (pos < end) {   // the last thread whose sequences begin at or before pos, then the sequence among its own
-    int at = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) at += __popc(__ballot_sync(0xffffffffu, prefix[w * 32 + lane] <= pos));
-    b = (at - 1) * per;
-    base = prefix[at - 1];
+  int pos = (int)min((int64_t)unit * share, (int64_t)total);
+  const int end = min((uint32_t)pos + (uint32_t)share, (uint32_t)total);
+  int b = 0, base = 0;
+  if (pos < end) {   // the last lane whose sequences begin at or before pos, then the sequence among its own
+    const int at = __popc(__ballot_sync(0xffffffffu, upto - mine <= pos)) - 1;
+    b = at * per;
+    base = __shfl_sync(0xffffffffu, upto - mine, at);
   }
-  __syncthreads();
   bool bad = false;
   Note note = {0, 0, 0, 0};
 
@@ -194,18 +179,18 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     const Rows rw = rows_of(p, b);
     const int keys = keys_of(p, b), lines = lines_of(rw.count);
     const int tiles = cut ? tiles_of(keys) : 1;
-    if (pos >= base + (int64_t)lines * tiles) {   // on to the next sequence
-      base += (int64_t)lines * tiles;
+    const int into = pos - base;
+    if (into >= lines * tiles) {   // on to the next sequence
+      base += lines * tiles;
       ++b;
       continue;
     }
-    const int64_t into = pos - base;   // (a division of 64 bits takes over a hundred instructions)
-    const int off = into < 0x7fffffff ? (int)into / tiles : (int)(into / tiles), t0 = cut ? (int)(into - (int64_t)off * tiles) : 0;
-    const int chunk = off / groups, kvh = p.kv_begin + ((off - chunk * groups) << sp.heads_log2) + sub, r0 = chunk * ROWS;
+    const int off = into / tiles, t0 = cut ? into - off * tiles : 0;
+    const int chunk = off < groups ? 0 : off / groups, kvh = p.kv_begin + ((off - chunk * groups) << sp.heads_log2) + sub, r0 = chunk * ROWS;
     const int rows = min(ROWS, rw.count * G - r0);
-    const int t1 = cut ? (int)min((int64_t)tiles, t0 + (end - pos)) : tiles_of(keys);
+    const int t1 = cut ? min(tiles, t0 + (end - pos)) : tiles_of(keys);
     const bool whole = !cut || (t0 == 0 && t1 == tiles);
-    if (!whole && t0 == 0) note = {(int)((pos + tiles - 1) / share) - unit + 1, b, off, rows};
+    if (!whole && t0 == 0) note = {(pos + tiles - 1) / share - unit + 1, b, off, rows};
     pos += cut ? t1 - t0 : 1;
 
     const int lim_least = visible(p, keys, rw.count, rw.count == 1 ? 0 : r0 / G);
@@ -230,7 +215,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       const int64_t at = r < rows ? query_at(p, p.qs, rw, b, h, i) : 0;
       const bool wide = T == 2 && p.dtype == AIDN_F32;
       const int64_t esz = wide ? 4 : 2;
-#pragma unroll 2
+#pragma unroll 4
       for (int x = 0; x < SLOTS; ++x) {
         const int d = T == 1 ? column(x >> 1, t) + 8 * (x & 1) : column(x >> 2, t) + 4 * (x & 3);
         uint4* const dst = qfrag + (n * SLOTS + x) * 32 + lane;
@@ -618,11 +603,13 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     __syncwarp();
     const int64_t part = ((int64_t)(2 * unit + (t0 == 0 ? 1 : 0)) << sp.heads_log2) + sub;
     const float mine_f = !whole ? vref : (my_sum == 0.f ? 0.f : vref / my_sum);
-#pragma unroll 1
+    // (lane r knows where row r goes)
+    const int my_i = rw.count == 1 ? 0 : (r0 + lane) / G, my_h = kvh * G + (r0 + lane) - my_i * G;
+    const int64_t my_to = whole ? query_at(p, p.os, rw, b, my_h, my_i) : (part * sp.row_most + lane) * DP;
+#pragma unroll 2
     for (int r = 0; r < rows; ++r) {
       const float f = __shfl_sync(0xffffffffu, mine_f, r);
-      const int i = rw.count == 1 ? 0 : (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-      const int64_t to = whole ? query_at(p, p.os, rw, b, h, i) : (part * sp.row_most + r) * DP;
+      const int64_t to = __shfl_sync(0xffffffffu, my_to, r);
 #pragma unroll 1
       for (int d = lane * 4; d < D; d += 128) {
         float4 o = *reinterpret_cast<const float4*>(rows_at + r * DP + (d ^ 4 * (r >> 1 & 3)));
@@ -630,9 +617,10 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
         if (whole) store4(p, to + d, sp.out_vec, o);
         else __stcg(reinterpret_cast<float4*>(sp.partial + to + d), o);
       }
-      if (lane != r) continue;
-      if (!whole) __stcg(sp.stats + part * sp.row_most + r, make_float2(my_top, my_sum));
-      else if (p.lse) *lse_at(p, rw, h, i) = my_sum == 0.f ? -INFINITY : (my_top + log2f(my_sum)) * kLn2;
+    }
+    if (lane < rows) {
+      if (!whole) __stcg(sp.stats + part * sp.row_most + lane, make_float2(my_top, my_sum));
+      else if (p.lse) *lse_at(p, rw, my_h, my_i) = my_sum == 0.f ? -INFINITY : (my_top + log2f(my_sum)) * kLn2;
     }
   }
   if (cut && sub == 0 && lane == 0 && unit < sp.units) *reinterpret_cast<int4*>(sp.notes + unit) = make_int4(note.parts, note.b, note.off, note.rows);
@@ -805,7 +793,7 @@ cudaError_t one(const Attend* p, const Sizes& z, void* workspace, int64_t* bytes
     if (e != cudaSuccess) return e;
     *raised |= 1ull << id;
   }
-  if (z.workspace_bytes < need || (uintptr_t)workspace % 16 != 0) workspace = nullptr;
+  if (z.workspace_bytes < need || (uintptr_t)workspace % 16 != 0 || shares * sp.least >= 0x7fffffff - C::kWarps * most) workspace = nullptr;
   sp.partial = static_cast<float*>(workspace);
   sp.stats = workspace ? reinterpret_cast<float2*>(static_cast<char*>(workspace) + acc) : nullptr;
   sp.notes = workspace ? reinterpret_cast<Note*>(static_cast<char*>(workspace) + need) - sp.units : nullptr;
@@ -853,7 +841,7 @@ bool split_supported(const Attend& p) {
   if ((uintptr_t)p.c.k % 16 != 0 || (uintptr_t)p.c.v % 16 != 0) return false;
   for (int i = 0; i < 3; ++i)
     if (p.c.stride[i] % 16 != 0) return false;
-  return true;
+  return p.batch * ((p.seq_q * p.group + 7) / 8) * p.kv_count < 0x7ff00000;   // lines are counted in 32 bits
 }
 // (whatever the block size: the larger of the two kernels' needs)
 int64_t split_workspace_bytes(int head_dim, bool exact, int64_t batch, int64_t rows, int64_t seq_kv, int kv_count, int num_sms) {
