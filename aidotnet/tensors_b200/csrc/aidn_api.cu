@@ -969,8 +969,21 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   cudaStream_t stream = (cudaStream_t)cu_stream;
   int launches = 1;
   cudaError_t e;
+  p.rows_above = 0;
+  p.rows_upto = INT64_MAX;
   if (d.path != AIDN_PATH_GENERIC && p.seq_q * p.group > aidn::kv8::kFewRows && aidn::kv8::sm100_supported(p)) {
-    e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);
+    // sequences of few rows among others: a launch of their own, at the speed of memory.  (The launches take turns on the workspace.)
+    int few = 0;
+    e = cudaSuccess;
+    if (query_starts && p.batch > 1 && p.group <= aidn::kv8::kFewRows && aidn::kv8::split_supported(p)) {
+      aidn::kv8::Attend f = p;
+      f.rows_upto = aidn::kv8::kFewRows;
+      f.seq_q = aidn::kv8::kFewRows / p.group;
+      e = aidn::kv8::launch_attend_split(f, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &few, stream);
+      p.rows_above = aidn::kv8::kFewRows;
+    }
+    if (e == cudaSuccess) e = aidn::kv8::launch_attend_sm100(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);
+    launches += few;
     h->last_path = AIDN_PATH_PREFILL_SM100;
   } else if (d.path != AIDN_PATH_GENERIC && aidn::kv8::split_supported(p)) {
     e = aidn::kv8::launch_attend_split(p, h->num_sms, a->workspace, a->workspace_bytes, &h->kv8_raised, &launches, stream);

@@ -54,6 +54,7 @@ struct Attend {
   int64_t seq_q, seq_kv;
   int64_t causal_offset;
   int32_t batch, num_q_heads, group;
+  int64_t rows_above, rows_upto;   // with query_starts: sequences of no more, or more rows (queries x query heads of a group) are left out
   int32_t kv_begin, kv_count;   // KV heads of the handle's shard
   int32_t dtype, out_f32, mask_kind, causal, bottom_right;
   float scale, softcap;
@@ -83,6 +84,7 @@ __device__ __forceinline__ Rows rows_of(const Attend& p, int b) {
   // (what the host cannot see: no row outside [0, queries) is touched whatever the starts are)
   int64_t n = (last < p.queries ? last : p.queries) - first;
   if (first < 0 || n < 0) n = 0;
+  if (n * p.group <= p.rows_above || n * p.group > p.rows_upto) n = 0;   // another launch's
   if (n > p.seq_q) n = p.seq_q;
   return {first, (int)n};
 }

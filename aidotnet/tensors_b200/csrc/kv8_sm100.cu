@@ -47,6 +47,7 @@ static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kMmaRegs <= kThrea
 constexpr int kRing = 4;              // tiles whose scales are kept
 constexpr float kUnset = -1e30f;
 constexpr float kLift = 4.f;
+constexpr int kTileCost = 3, kPairCost = 4;   // of 128 keys with one row tile, and with two, which overlap (64 keys: 1700 cycles, and 2300)
 constexpr float kMostWeights = 32768.f;   // of sixteen weights together: each is then in fp16's range
 
 template <int HD>
@@ -114,8 +115,11 @@ struct Walk {
   __device__ __forceinline__ void line() {
     const int left = rw.count * p->group - u * kPairRows;
     rows = left < kPairRows ? left : kPairRows;
-    cost = rows > kTileRows ? 2 : 1;
+    cost = rows > kTileRows ? kPairCost : kTileCost;
     tiles = tiles_of(*p, rw.count, keys, u);
+  }
+  __device__ __forceinline__ int tiles_before(int64_t cost_of_them) const {   // rounded up, all of the line's at most
+    return cost_of_them >= (int64_t)tiles * cost ? tiles : ((int)cost_of_them + cost - 1) / cost;
   }
   static __device__ __forceinline__ int tiles_of(const Attend& p, int n, int keys, int u) {
     const int last = min(n * p.group, (u + 1) * kPairRows) - 1;
@@ -142,9 +146,8 @@ struct Walk {
       first = false;
       if (base >= end) return false;
       if (cut) {
-        t0 = pos > base ? (int)((pos - base + cost - 1) >> (cost - 1)) : 0;   // (cost 1 or 2)
-        const int64_t most = (end - base + cost - 1) >> (cost - 1);
-        t1 = most < tiles ? (int)most : tiles;
+        t0 = pos > base ? tiles_before(pos - base) : 0;
+        t1 = tiles_before(end - base);
         if (t0 >= t1) continue;
         whole = t0 == 0 && t1 == tiles;
       } else {
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
     *hi = spread > 1 ? min(*lo + each, pairs) : pairs;
   };
   auto weight = [&](int n, int keys, int u) {
-    return (int64_t)Walk::tiles_of(p, n, keys, u) * p.kv_count * (n * G - u * kPairRows > kTileRows ? 2 : 1);
+    return (int64_t)Walk::tiles_of(p, n, keys, u) * p.kv_count * (n * G - u * kPairRows > kTileRows ? kPairCost : kTileCost);
   };
   int64_t mine = 0;
   for (int b = b_lo; b < b_hi; ++b) {
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   }
   before += upto - mine;
   int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
-  if (share < 4) share = 4;
+  if (share < 2 * kPairCost) share = 2 * kPairCost;   // (no line passes over a share)
   const int64_t pos = blockIdx.x * share, end = min(pos + share, total);
   const uint32_t tmem = ms.tmem;
   if (pos < end && pos >= before && pos < before + mine) {
