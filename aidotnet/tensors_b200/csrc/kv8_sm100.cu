@@ -847,26 +847,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
   }
 }
 
-// CTA (c, i): 32 rows of the line that begins in the share of CTA c and goes on behind it, a warp four of them.
+// CTA (c, i): 16 rows of the line that begins in the share of CTA c and goes on behind it, a warp two of them.  (Bound by the latency of the parts: with
+// four rows a warp and so many registers that an SM held one or two CTAs it took 19 us where it takes 12.)
+constexpr int kMergeRows = 2;
 template <int HD>
-__global__ void __launch_bounds__(256) kv8_sm100_merge_kernel(const __grid_constant__ Attend p, const Cut cut) {
+__global__ void __launch_bounds__(256, HD == 128 ? 3 : 4) kv8_sm100_merge_kernel(const __grid_constant__ Attend p, const Cut cut) {
   pdl_wait();
   pdl_trigger();
   const Note note = cut.notes[blockIdx.x];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = 32 * blockIdx.y + 4 * warp;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = 8 * kMergeRows * blockIdx.y + kMergeRows * warp;
   if (note.parts == 0 || r0 >= note.rows) return;
-  constexpr int N = HD / 32;
-  float top[4], sum[4] = {}, o[4][N] = {};
+  constexpr int N = HD / 32, R = kMergeRows;
+  float top[R], sum[R] = {}, o[R][N] = {};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) top[r] = kUnset;
+  for (int r = 0; r < R; ++r) top[r] = kUnset;
   for (int q = 0; q < note.parts; q += 4) {
-    float2 st[4][4];
-    float v[4][4][N];
+    float2 st[4][R];
+    float v[4][R][N];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int part = min(q + x, note.parts - 1);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < R; ++r) {
         const int64_t from = (int64_t)(2 * (blockIdx.x + part) + (part == 0)) * kPairRows + min(r0 + r, note.rows - 1);
         st[x][r] = cut.stats[from];
         const float* at = cut.partial + from * HD + N * lane;
@@ -880,7 +882,7 @@ __global__ void __launch_bounds__(256) kv8_sm100_merge_kernel(const __grid_const
       }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < R; ++r) {
       float now = top[r];
 #pragma unroll
       for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x][r].x);
@@ -901,15 +903,25 @@ __global__ void __launch_bounds__(256) kv8_sm100_merge_kernel(const __grid_const
   }
   const Rows rw = {note.first_row, 0};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < R; ++r) {
     if (r0 + r >= note.rows) continue;
     const int row = note.row + r0 + r, i = row / p.group, h = (p.kv_begin + note.kvh) * p.group + row - i * p.group;
     const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
     const int64_t at = query_at(p, p.os, rw, note.b, h, i) + N * lane;
+    uint16_t* const dst = static_cast<uint16_t*>(p.out) + at;
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (p.dtype == AIDN_F16) static_cast<__half*>(p.out)[at + e] = __float2half_rn(o[r][e] * f);
-      else static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(o[r][e] * f);
+    for (int e = 0; e < N / 2; ++e)
+      w[e] = p.dtype == AIDN_F16 ? ptx::pack2<false>(o[r][2 * e] * f, o[r][2 * e + 1] * f) : ptx::pack2<true>(o[r][2 * e] * f, o[r][2 * e + 1] * f);
+    if (cut.out_vec) {
+      if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(dst) = w[0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        dst[2 * e] = (uint16_t)w[e];
+        dst[2 * e + 1] = (uint16_t)(w[e] >> 16);
+      }
     }
     if (p.lse && lane == 0) *lse_at(p, rw, h, i) = sum[r] == 0.f ? -INFINITY : (top[r] + log2f(sum[r])) * kLn2;
   }
@@ -927,7 +939,7 @@ cudaError_t launch(const Attend& p, int grid, const Cut& cut, uint64_t* raised, 
   const cudaError_t e = launch_dependent(k, dim3((unsigned)grid), kThreads, Cfg<HD>::kSmem, stream, p, cut);
   if (e != cudaSuccess || !cut.partial) return e;
   const int64_t rows = p.seq_q * p.group;
-  const unsigned slices = (unsigned)((rows < kPairRows ? rows : kPairRows) + 31) / 32;
+  const unsigned slices = (unsigned)((rows < kPairRows ? rows : kPairRows) + 8 * kMergeRows - 1) / (8 * kMergeRows);
   ++*launches;
   return launch_dependent(kv8_sm100_merge_kernel<HD>, dim3((unsigned)grid, slices), 256, 0, stream, p, cut);
 }
