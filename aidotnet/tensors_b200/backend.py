@@ -499,7 +499,8 @@ class CudaBackend:
             batch, heads, _DTYPE[dtype], rope), self._raw_stream)
         if status != N.OK:
             raise N.AidnError(status, N.last_error())
-        self.launch_count += 1
+        if tokens > 0:
+            self.launch_count += 1
 
     def PagedAttentionFp8(self, q: GpuBuffer, cache: KvCacheFp8, blockTables: GpuBuffer, seqLens: GpuBuffer, output: GpuBuffer,
                           batch: int, heads: int, maxQueries: int, maxSeqLen: int, blocksPerSeq: int, scale: float,
