@@ -13,7 +13,7 @@
 // (11 bits, of 2^9 times their value so that they stay normal down to 2^-23 of the largest); for fp32 results they are two terms too.
 //
 // The warps of a "unit" do the same tiles of neighbouring KV heads, whose rows are neighbours in the pool: memory is read in runs
-// of up to 1 KB (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 228 us, and 265 us
+// of up to 512 bytes (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 228 us, and 265 us
 // where each warp goes through lines of its own).  The
 // lines' tiles are one row, cut into equal shares for the units that are resident whatever the lengths are.  No warp waits for
 // another one: a line that is cut leaves a partial result a unit in the workspace, and a second launch merges them in their order, so that
@@ -111,8 +111,8 @@ struct Sizes {
 
 template <int DP, int NR, int T, bool UB>
 struct Config {
-  static constexpr int kWarps = NR == 1 && DP < 256 ? 8 : 4;
-  static constexpr int kMinCtas = DP == 256 ? 2 : (NR == 1 ? 2 : 3);
+  static constexpr int kWarps = 4;   // (8 and 16: 2 % slower with 64 sequences, 6 to 10 % with one)
+  static constexpr int kMinCtas = DP == 256 ? 2 : (NR == 1 ? 4 : 3);
   static constexpr int kSteps = DP / 16;                 // of 16 elements: fragments of a key
   static constexpr int kRows = 8 * NR;
   static constexpr int kQueryBytes = T * NR * kSteps * 32 * 8;   // of a warp
@@ -770,7 +770,7 @@ cudaError_t one(const Attend* p, const Sizes& z, void* workspace, int64_t* bytes
   const int most = resident<DP, NR, T, UB>(z.num_sms);
   Split sp;
   sp.row_most = (int)(z.rows < C::kRows ? z.rows : C::kRows);
-  sp.least = 2;
+  sp.least = NR * T > 1 ? 1 : 2;   // (one query row of 16 bits, 1237 keys: 10.3 us, and 11.0 with one; nine rows of 32 bits: 24.1, and 19.1 with one)
   sp.heads_log2 = 0;
   while ((2 << sp.heads_log2) <= C::kWarps && z.kv_count % (2 << sp.heads_log2) == 0) ++sp.heads_log2;
   const int units_cta = C::kWarps >> sp.heads_log2;
