@@ -7,7 +7,8 @@ namespace aidn {
 namespace kv8 {
 
 constexpr float kLargestCode = 448.f;
-// Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one.
+// Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one: 24 sequences of 2000 to 4096 keys, 8 KV
+// heads of 128, take 54 us with 16 rows, 84 with 32, 112 with 40 and 143 with 64, and the tcgen05 kernel 92, 95, 95 and 96.
 constexpr int kFewRows = 32;
 
 constexpr int kLeastExponent = -100, kMostExponent = 119;   // of a scale: 448 * 2^119 is below the largest float

@@ -350,7 +350,8 @@ AIDN_API int aidn_kv8_append(const aidn_kv8_cache* cache, const aidn_kv8_append_
  * key j iff j <= kv_len[b] - n + i.  A query that sees no key gives zeros and a log-sum-exp of -inf.  lse is dense
  * [queries in order, Hq].  desc.mask_kind: masks over (b, h, i, j) run on the any-shape kernel, without query_starts only.
  * A visible NaN code makes its rows NaN; codes past kv_len[b] may be anything.
- * Workspace: aidn_sdpa_kv8_workspace_bytes() for the partial results of keys that are cut over CTAs; calls without one run uncut. */
+ * Workspace: aidn_sdpa_kv8_workspace_bytes() for the partial results of keys that are cut over CTAs; calls without one run uncut.
+ * Up to four launches: few queries or many, each with a merge of the parts; a ragged batch may have sequences of both kinds. */
 AIDN_API int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_q, int64_t seq_kv);
 AIDN_API int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* args, const aidn_kv8_cache* cache,
                                   const int32_t* query_starts, int64_t queries, void* cu_stream);
