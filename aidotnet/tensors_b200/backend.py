@@ -81,12 +81,11 @@ class KvCacheFp8:
                 raise ValueError(f"{name} must hold numBlocks * kvHeads fp32 values")
         self.keys, self.values, self.keyScales, self.valueScales = keys, values, keyScales, valueScales
         self.blockSize, self.kvHeads, self.headDim = blockSize, kvHeads, headDim
+        self._own = tuple(b.tensor.data_ptr() for b in (keys, values, keyScales, valueScales))   # (its buffers for as long as it lives)
 
     def _pack(self, table: int, blocksPerSeq: int) -> bytes:
         """The ``aidn_kv8_cache`` block, packed in one go (a decode step waits for this code, not for the GPU)."""
-        return N._KV8_CACHE.pack(self.keys.tensor.data_ptr(), self.values.tensor.data_ptr(), self.keyScales.tensor.data_ptr(),
-                                 self.valueScales.tensor.data_ptr(), table, blocksPerSeq, 0, 0, 0, self.numBlocks, self.blockSize,
-                                 self.kvHeads, self.headDim)
+        return N._KV8_CACHE.pack(*self._own, table, blocksPerSeq, 0, 0, 0, self.numBlocks, self.blockSize, self.kvHeads, self.headDim)
 
 
 class CudaBackend:
@@ -139,12 +138,12 @@ class CudaBackend:
 
     def _handle(self, **kw) -> N.Handle:
         key = frozenset(kw.items())   # (field, value) pairs, in whatever order the caller names them
-        h = self._handles.get(key)
-        if h is None:
-            if len(self._handles) >= 128:  # e.g. one handle per startPos of a long chunked prefill: drop the oldest
-                self._handles.pop(next(iter(self._handles))).close()
-            h = N.Handle(device=self.device, path=self._path, decode_chunk=self._decode_chunk, **kw)
-            self._handles[key] = h
+        return self._handles.get(key) or self._new_handle(key, **kw)
+
+    def _new_handle(self, key, **kw) -> N.Handle:
+        if len(self._handles) >= 128:  # e.g. one handle per startPos of a long chunked prefill: drop the oldest
+            self._handles.pop(next(iter(self._handles))).close()
+        h = self._handles[key] = N.Handle(device=self.device, path=self._path, decode_chunk=self._decode_chunk, **kw)
         return h
 
     def _workspace(self, nbytes: int, stream: torch.cuda.Stream, optional: bool = False) -> Tuple[Optional[int], int]:
@@ -524,9 +523,12 @@ class CudaBackend:
             raise ValueError("PagedAttentionFp8: q or output is smaller than [queries, heads, headDim]")
         if softmaxStats is not None and (softmaxStats.tensor.numel() < queries * heads or softmaxStats.tensor.dtype != torch.float32):
             raise ValueError("PagedAttentionFp8: softmaxStats must hold [queries, heads] fp32 values")
-        h = self._handle(qkv_dtype=_DTYPE[x.dtype], out_dtype=_DTYPE[out.dtype], head_dim=headDim, num_q_heads=heads,
-                         num_kv_heads=kvHeads, causal=bool(causal), causal_bottom_right=True, softcap=float(softcap),
-                         emit_lse=softmaxStats is not None)
+        hkey = (x.dtype, out.dtype, headDim, heads, kvHeads, causal, softcap, softmaxStats is None)   # (a tuple of its own: a step's host time)
+        h = self._handles.get(hkey)
+        if h is None:
+            h = self._new_handle(hkey, qkv_dtype=_DTYPE[x.dtype], out_dtype=_DTYPE[out.dtype], head_dim=headDim, num_q_heads=heads,
+                                 num_kv_heads=kvHeads, causal=bool(causal), causal_bottom_right=True, softcap=float(softcap),
+                                 emit_lse=softmaxStats is not None)
         need = h.kv8_workspace_bytes(batch, maxQueries, maxSeqLen)
         stream = self._raw_stream
         ws, ws_bytes = 0, 0

@@ -291,6 +291,7 @@ class Handle:
                  path: int = PATH_AUTO, head_begin: int = 0, head_count: int = 0, decode_chunk: int = 0,
                  max_batch: int = 0, max_seq_q: int = 0, max_seq_kv: int = 0, nccl_comm: Optional[int] = None):
         self._lib = load()
+        self._kv8_sizes = self._kv8_need = None
         d = SdpaDesc()
         d.device, d.qkv_dtype, d.out_dtype, d.head_dim = device, qkv_dtype, out_dtype, head_dim
         d.num_q_heads = num_q_heads
@@ -334,10 +335,13 @@ class Handle:
             raise AidnError(status, last_error())
 
     def kv8_workspace_bytes(self, batch: int, seq_q: int, seq_kv: int) -> int:
-        n = self._lib.aidn_sdpa_kv8_workspace_bytes(self._h, batch, seq_q, seq_kv)
-        if n < 0:
-            raise AidnError(EINVAL, last_error())
-        return int(n)
+        sizes = (batch, seq_q, seq_kv)
+        if sizes != self._kv8_sizes:   # (a function of them and of the handle; consecutive steps mostly ask for the same)
+            n = self._lib.aidn_sdpa_kv8_workspace_bytes(self._h, batch, seq_q, seq_kv)
+            if n < 0:
+                raise AidnError(EINVAL, last_error())
+            self._kv8_sizes, self._kv8_need = sizes, int(n)
+        return self._kv8_need
 
     def launch_kv8(self, *, q: int, out: int, cache: bytes, batch: int, seq_q: int, seq_kv: int, stream: int,
                    query_starts: Optional[int] = None, queries: int = 0, lse: Optional[int] = None,
