@@ -106,3 +106,12 @@ def test_results_do_not_depend_on_what_else_runs():
         again = attend(pool, q, lens, counts, 8, dtype="bf16")
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dim", [16, 32, 48, 80, 112, 144, 208, 240])
+@pytest.mark.parametrize("dtype,count", [("bf16", 1), ("f16", 6), ("f32", 1), ("f32", 4)])
+def test_head_sizes_between_the_tiles(dim, dtype, count):
+    """Head sizes that fill a part of a kernel's 64, 128 or 256 columns; blocks of 16 and of 40 tokens."""
+    for block, lens in ((16, [300, 77]), (40, [33, 410])):
+        pool = Pool(lens, block, 2, dim, seed=42).cuda()
+        check(pool, queries(2 * count, 6, dim, dtype, 43), lens, [count] * 2, 6, dtype=dtype)
