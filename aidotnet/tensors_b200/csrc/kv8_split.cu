@@ -114,6 +114,8 @@ struct Sizes {
 template <int DP, int NR, int T, bool UB>
 struct Config {
   static constexpr int kWarps = 4;   // (8 and 16: 2 % slower with 64 sequences, 6 to 10 % with one)
+  // registers: 16 warps an SM with one fragment of rows (12: 64 tokens 194 -> 211 us; 20: 216), 12 with two (16: drafts 57 -> 77; 8: 66).  Fragments of 32
+  // rows leave 8 warps (drafts 77), and passing over those without rows costs more than it saves (60).
   static constexpr int kMinCtas = DP == 256 ? 2 : (NR == 1 ? 4 : 3);
   static constexpr int kSteps = DP / 16;                 // of 16 elements: fragments of a key
   static constexpr int kRows = 8 * NR;
