@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import sys
 from typing import Optional, Sequence, Tuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -291,6 +292,8 @@ class Handle:
                  path: int = PATH_AUTO, head_begin: int = 0, head_count: int = 0, decode_chunk: int = 0,
                  max_batch: int = 0, max_seq_q: int = 0, max_seq_kv: int = 0, nccl_comm: Optional[int] = None):
         self._lib = load()
+        while _left and not _capturing():
+            self._lib.aidn_sdpa_destroy(_left.pop())
         self._kv8_sizes = self._kv8_need = None
         d = SdpaDesc()
         d.device, d.qkv_dtype, d.out_dtype, d.head_dim = device, qkv_dtype, out_dtype, head_dim
@@ -418,8 +421,12 @@ class Handle:
             self._h = None
 
     def __del__(self):
+        # The collector may run inside a graph's capture, which freeing device memory would end: such a handle is destroyed with the next one made.
         try:
-            self.close()
+            if _capturing():
+                _left.append(self._h)
+            else:
+                self.close()
         except Exception:
             pass
 
@@ -428,6 +435,14 @@ class Handle:
 
     def __exit__(self, *exc):
         self.close()
+
+
+_left: list = []   # handles that were collected during a capture
+
+
+def _capturing() -> bool:
+    torch = sys.modules.get("torch")
+    return torch is not None and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 def cast(kind: str, src: int, dst: int, n: int, stream: int) -> None:
