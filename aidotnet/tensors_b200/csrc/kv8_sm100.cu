@@ -52,6 +52,7 @@ constexpr float kUnset = -1e30f;
 constexpr float kLift = 4.f;
 constexpr int kTileCost = 3, kPairCost = 4;   // of 128 keys with one row tile, and with two, which overlap (64 keys: 1700 cycles, and 2300)
 constexpr float kMostWeights = 32768.f;   // of sixteen weights together: each is then in fp16's range
+constexpr float kLargeLogit = 1048576.f;  // (to base 2) a rounding of half a unit of its last place is 2^-4 here
 
 template <int HD>
 struct Cfg {
@@ -476,9 +477,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
                 }
               }
             }
-            // The weights are formed with the maximum so far: again if their sum says that they may not fit.
-            float sum;
+            // The weights are formed with the maximum so far: again, once, if their sum says that they may not fit, with the step's own.  From logits
+            // of 2^20 on the exponents are formed from differences, of products that are rounded as the maximum was: none is then above it, where a
+            // fused multiply-add has the product's rounding, 2^(p - 24) for a logit of 2^p, in the exponent.  Such rows take the maximum first.
+            auto large = [&] { return __any_sync(0xffffffffu, fabsf(m) > kLargeLogit && m != kUnset); };
+            bool again = large(), far = again;   // (again: of the warp)
+            float sum, base_m = m;               // base_m: what the scores, or differences, have to come down by
             for (;;) {
+              if (again) {
+                float keep = 1.f;
+                if (far) {
+                  float top = m, emax = eref;
+#pragma unroll
+                  for (int g = 0; g < 4; ++g) {
+                    float m0 = __uint_as_float(s[16 * g]);
+#pragma unroll
+                    for (int k = 1; k < 15; k += 2) m0 = fmax3(m0, __uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1]));
+                    m0 = fmaxf(m0, __uint_as_float(s[16 * g + 15]));
+                    const float y = m0 * ck[g];
+                    if (e[g] != -INFINITY && m0 != -INFINITY) top = fmaxf(top, y);
+                    emax = fmaxf(emax, e[g]);
+                  }
+                  const float f = ex2_approx(m - top);
+                  keep = f * ex2_approx(eref - emax);
+                  l *= f;
+                  m = top;
+                  eref = emax;
+                  l_unit = ex2_approx(eref - kLift);
+                }
+                if (u > 0 && __any_sync(0xffffffffu, keep != 1.f)) {   // (one product at most is on its way, that of the step before: the next needs these weights)
+                  if (!mbar_wait(bar(kODone + 2 * a + (buf ^ 1)), (steps - 1) >> 1 & 1, abort_flag)) alive = false;
+                  tc_fence_after();
+#pragma unroll 1
+                  for (int q = 0; q < HD / 16; ++q) {
+                    uint32_t o[16];
+                    tmem_ld16(to + 16 * q, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                    tmem_st16(to + 16 * q, o);
+                  }
+                }
+                base_m = m;
+                if (large()) {
+#pragma unroll
+                  for (int k = 0; k < 64; ++k) {
+                    const float x = __uint_as_float(s[k]);
+                    if (!EDGE || x != -INFINITY) s[k] = __float_as_uint(__fsub_rn(__fmul_rn(x, ck[k / 16]), m));
+                  }
+#pragma unroll
+                  for (int g = 0; g < 4; ++g) ck[g] = 1.f;
+                  base_m = 0.f;
+                }
+              }
               float most = 0.f;
               sum = 0.f;
 #pragma unroll
@@ -491,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
 #pragma unroll
                 for (int h2 = 0; h2 < 2; ++h2) {
                   const int g = 2 * q + h2;
-                  const float off = e[g] - (eref + m - kLift);
+                  const float off = e[g] - (eref + base_m - kLift);
                   const uint64_t ck2 = aidn::pack2(ck[g], ck[g]), off2 = aidn::pack2(off, off);
                   uint64_t sum_g = 0;
 #pragma unroll
@@ -514,41 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
                 }
                 tmem_st16(ts0 + 64 * buf + 16 * q, packed);
               }
-              const bool far = most > kMostWeights;
+              if (again) break;
+              far = most > kMostWeights;
               if (!__any_sync(0xffffffffu, far)) break;
-              float keep = 1.f;
-              if (far) {
-                float top = m, emax = eref;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  float m0 = __uint_as_float(s[16 * g]);
-#pragma unroll
-                  for (int k = 1; k < 15; k += 2) m0 = fmax3(m0, __uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1]));
-                  m0 = fmaxf(m0, __uint_as_float(s[16 * g + 15]));
-                  const float y = m0 * ck[g];
-                  if (e[g] != -INFINITY && m0 != -INFINITY) top = fmaxf(top, y);
-                  emax = fmaxf(emax, e[g]);
-                }
-                const float f = ex2_approx(m - top);
-                keep = f * ex2_approx(eref - emax);
-                l *= f;
-                m = top;
-                eref = emax;
-                l_unit = ex2_approx(eref - kLift);
-              }
-              if (u > 0) {   // (one product at most is on its way, that of the step before: the next needs these weights)
-                if (!mbar_wait(bar(kODone + 2 * a + (buf ^ 1)), (steps - 1) >> 1 & 1, abort_flag)) alive = false;
-                tc_fence_after();
-#pragma unroll 1
-                for (int q = 0; q < HD / 16; ++q) {
-                  uint32_t o[16];
-                  tmem_ld16(to + 16 * q, o);
-                  tc_wait_ld();
-#pragma unroll
-                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                  tmem_st16(to + 16 * q, o);
-                }
-              }
+              again = true;
             }
             l = fmaf(sum, l_unit, l);
           };

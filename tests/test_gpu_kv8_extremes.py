@@ -1,0 +1,70 @@
+"""Attention over an 8-bit pool far from ordinary values: large logits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests._harness import TORCH_DT
+from tests.test_gpu_kv8 import Pool, attend, attend64, bounds, queries
+
+pytestmark = pytest.mark.gpu
+
+CODES = {0: (0x38, 0x3c, 0x3e), 1: (0x30, 0x34, 0x36)}   # 1, 1.5, 1.75, and half of each
+
+
+def tied(lens, block, kv_heads, dim, seed):
+    """A pool whose keys begin with 2^-7 times 1, 1.5 or 1.75, in blocks of two scales: many keys share the largest logit of a query
+    that looks at the first element alone, exactly, and the next one is far below."""
+    pool = Pool(lens, block, kv_heads, dim, seed=seed)
+    g = np.random.default_rng(seed)
+    half = g.integers(0, 2, pool.scales[0].shape)
+    pick = g.integers(0, 3, pool.codes[0].shape[:3])
+    table = np.array([CODES[0], CODES[1]], np.uint8)
+    pool.codes[0][..., 0] = table[half[:, None, :], pick]
+    pool.scales[0] = np.exp2(half - 7.0).astype(np.float32)
+    return pool.cuda()
+
+
+def looking_at_the_first(n, heads, dim, dtype, sign):
+    q = torch.zeros((n, heads, dim))
+    q[..., 0] = sign
+    return q.to(TORCH_DT[dtype]).cuda()
+
+
+def check_tied(lens, counts, heads, kv_heads, dim, block, dtype, exponent, sign, out=None, **kw):
+    """A query's logits to base 2 are about 2^exponent.  Equal logits are equal in 32 bits too (the scales are powers of two), whatever a
+    rounding of 2^(exponent - 24) does to them, so that the weights of those that share the maximum are equal to 2^-11 and all others are zero."""
+    pool = tied(lens, block, kv_heads, dim, seed=50 + exponent)
+    q = looking_at_the_first(sum(counts), heads, dim, dtype, sign)
+    scale = 2.0 ** (exponent + 7) / math.log2(math.e)
+    o, lse, a, top = attend64(pool, q.double().cpu().numpy(), lens, counts, heads, scale=np.float64(np.float32(scale)))
+    bo, bl = bounds(o, lse, a, np.zeros_like(top), dtype, out or dtype, dim)
+    got, stats = attend(pool, q, lens, counts, heads, dtype=dtype, out=out, scale=scale, **kw)
+    got, stats = got.double().cpu().numpy(), stats.double().cpu().numpy()
+    assert np.isfinite(got).all() and np.isfinite(stats).all()
+    assert (np.abs(got - o) <= bo).all()
+    assert (np.abs(stats - lse) <= bl).all()
+
+
+LARGE = [16, 19, 20, 21, 24, 25, 26, 27, 28, 29, 30, 33, 40, 60]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("exponent", LARGE)
+@pytest.mark.parametrize("dtype,dim,workspace", [("bf16", 128, True), ("f16", 64, True), ("bf16", 64, False)])
+def test_large_logits_of_many_queries(exponent, sign, dtype, dim, workspace):
+    check_tied([300, 1290], [150, 70], 8, 2, dim, 16, dtype, exponent, sign, workspace=workspace)
+
+
+@pytest.mark.parametrize("size", [3e2, 2e4, 1e6, 1e12])
+@pytest.mark.parametrize("softcap", [0.0, 1e9])
+def test_queries_of_a_diverged_model(size, softcap):
+    """Normal queries and keys, of logits that differ by far more than a weight can show: results are within the values that they are made of."""
+    lens, counts = [700, 900], [400, 128]
+    pool = Pool(lens, 16, 2, 128, seed=51).cuda()
+    q = queries(sum(counts), 8, 128, "bf16", 52) * size
+    out, stats = attend(pool, q, lens, counts, 8, dtype="bf16", softcap=softcap)
+    most = max(np.abs(pool.rows(1, b, n)).max() for b, n in enumerate(lens))
+    assert bool(out.isfinite().all()) and bool(stats.isfinite().all())
+    assert float(out.abs().max()) <= most * (1 + 2.0 ** -7)
