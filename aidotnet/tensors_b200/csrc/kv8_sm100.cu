@@ -74,7 +74,7 @@ struct Misc {
   struct Scales {
     alignas(16) float k[8];
     float v_exp[8], v_inverse[8];
-    uint32_t nan[4];   // keys with a NaN among their values, in tiles of which rows do not see all
+    uint32_t nan[4];   // keys with a NaN among their values, in tiles of which rows of the pair do not see all: their codes are zeros there
   } scales[kRing];
   int64_t scan[kThreads / 32];
   int64_t start_base;
@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         if (lane == 0) mbar_arrive(bar(kQFull + a));
         const int lim = valid ? visible(p, w.keys, w.rw.count, i) : 0x7fffffff;
         const int lim_least = visible(p, w.keys, w.rw.count, (w.u * kPairRows + a * kTileRows) / G);
+        const int lim_pair = visible(p, w.keys, w.rw.count, w.u * kPairRows / G);   // what the converters clean a tile by
         const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
         float m = kUnset, l = 0.f, eref = kUnset, l_unit = 0.f;   // l_unit = 2^(eref - lift): sums of weights over it and the scale are l's
 
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
             if constexpr (EDGE) {   // what a row does not see is -inf, a key with a NaN among its values NaN
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const uint32_t nan = ld_shared_u32(scales_at + tile_count % kRing * (uint32_t)sizeof(Misc::Scales) + 96 + 8 * buf + 4 * q);
+                const uint32_t nan = ld_shared_u32(scales_at + tile_count % kRing * (uint32_t)sizeof(Misc::Scales) + (uint32_t)offsetof(Misc::Scales, nan) + 8 * buf + 4 * q);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                   if (nan >> k & 1) s[32 * q + k] = 0x7fffffffu;
@@ -572,7 +573,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
             }
             l = fmaf(sum, l_unit, l);
           };
-          if (key0 + 64 > lim_least || key0 + 64 > w.keys) step(std::true_type{});   // (uniform)
+          // (uniform.  All of these rows may see all of these keys, and yet their tile be one that was cleaned, for its other keys or the pair's first rows)
+          bool edge = key0 + 64 > lim_least || key0 + 64 > w.keys;
+          if (!edge && key0 - 64 * (int)buf + kKeys > lim_pair) {
+            const uint32_t nan = scales_at + tile_count % kRing * (uint32_t)sizeof(Misc::Scales) + (uint32_t)offsetof(Misc::Scales, nan) + 8 * buf;
+            edge = (ld_shared_u32(nan) | ld_shared_u32(nan + 4)) != 0;
+          }
+          if (edge) step(std::true_type{});
           else step(std::false_type{});
           scored = __all_sync(0xffffffffu, scored) && more;
           scaled = __all_sync(0xffffffffu, scaled) && more;

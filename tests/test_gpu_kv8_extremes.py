@@ -1,4 +1,4 @@
-"""Attention over an 8-bit pool far from ordinary values: large logits."""
+"""Attention over an 8-bit pool far from ordinary values: large logits, NaN."""
 import math
 
 import numpy as np
@@ -68,3 +68,26 @@ def test_queries_of_a_diverged_model(size, softcap):
     most = max(np.abs(pool.rows(1, b, n)).max() for b, n in enumerate(lens))
     assert bool(out.isfinite().all()) and bool(stats.isfinite().all())
     assert float(out.abs().max()) <= most * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("lens,counts,heads", [([300], [90], 2), ([300], [90], 8), ([463], [300], 1), ([100], [100], 4), ([333], [8], 4), ([129], [3], 6)])
+def test_nan_anywhere_in_the_last_tiles(lens, counts, heads, which, causal):
+    """One NaN among a key's elements or a key's values, at every eighth of the last keys in turn (and at both ends): the rows that see it
+    are NaN, the others what they are without it."""
+    n, c = lens[0], counts[0]
+    pool = Pool(lens, 16, 1, 64, seed=53).cuda()
+    q = queries(c, heads, 64, "bf16", 54)
+    clean, _ = attend(pool, q, lens, counts, heads, dtype="bf16", causal=causal)
+    codes, stash = pool.t[which], pool.t[which].clone()
+    for key in sorted({n - 1, *range(max(0, n - 330), n, 8)}):
+        at = (int(pool.table[0, key // 16]), key % 16, 0, key % 64)
+        codes[at] = 0xff if key % 16 else 0x7f
+        dirty, _ = attend(pool, q, lens, counts, heads, dtype="bf16", causal=causal)
+        codes[at] = stash[at]
+        first = max(0, key - (n - c)) if causal else 0
+        nan = dirty.isnan().any(-1).any(-1)
+        assert not bool(nan[:first].any()), key
+        assert bool(dirty[first:].isnan().any(-1).all()), key
+        assert torch.equal(dirty[:first], clean[:first]), key
