@@ -147,6 +147,13 @@ __device__ __forceinline__ float scale_for(float m) {
 // 1 / a power of two in [2^-126, 2^126].
 __device__ __forceinline__ float inverse_pow2(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
 
+// tanh(x) = 1 - 2 / (1 + e^2x), to 3e-7 of 1: the logits are off by that times the cap.  A NaN stays one.
+__device__ __forceinline__ float tanh_ex2(float x) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x * (2.f * kLog2e)), "f"(80.f));
+  return 1.f - __fdividef(2.f, 1.f + ex2_approx(y));
+}
+
 cudaError_t launch_append(const Append& p, cudaStream_t stream, int* launches);
 cudaError_t launch_attend_generic(const Attend& p, cudaStream_t stream);
 // Few queries (csrc/kv8_split.cu): head sizes that are a multiple of 16, 16-byte aligned pools, no mask.  Without its workspace keys are not

@@ -185,8 +185,6 @@ __device__ __forceinline__ float log2_approx(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh(x) = 1 - 2 / (1 + e^2x), to 3e-7 of 1.
-__device__ __forceinline__ float tanh_ex2(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(x * (2.f * kLog2e), 80.f))); }
 // tanh of two numbers up to 1, to 7e-7 of itself: x q(x^2), q the polynomial of degree 5 with the least relative error (a weighted least-squares
 // fit whose weights were adapted until the error was even).  Four multiply-adds an element in place of two of the special functions, of which a
 // multiprocessor does 16 a cycle: with those, logits that are capped took three a score where others take one.

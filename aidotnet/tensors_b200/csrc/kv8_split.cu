@@ -95,8 +95,6 @@ __device__ __forceinline__ void store4(const Attend& p, int64_t at, bool vec, fl
     to[0] = (uint16_t)a; to[1] = (uint16_t)(a >> 16); to[2] = (uint16_t)c; to[3] = (uint16_t)(c >> 16);
   }
 }
-// tanh to 3e-7 of 1: the logits are off by that times the cap.
-__device__ __forceinline__ float tanh_ex2(float x) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(x * (2.f * kLog2e), 80.f))); }
 // Whether any of four codes is a NaN.
 __device__ __forceinline__ bool any_nan(uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
 __device__ __forceinline__ uint32_t without_nan(uint32_t x) {

@@ -91,3 +91,26 @@ def test_nan_anywhere_in_the_last_tiles(lens, counts, heads, which, causal):
         assert not bool(nan[:first].any()), key
         assert bool(dirty[first:].isnan().any(-1).all()), key
         assert torch.equal(dirty[:first], clean[:first]), key
+
+
+@pytest.mark.parametrize("factor", [0.02, 20.0])
+@pytest.mark.parametrize("which", ["key", "query"])
+@pytest.mark.parametrize("dtype,out,counts", [("bf16", "bf16", [1, 1]), ("f16", "f16", [3, 3]), ("f32", "f32", [2, 2]), ("bf16", "f32", [5, 4]), ("bf16", "bf16", [150, 60])])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_nan_behind_a_softcap(dtype, out, counts, which, factor, dim):
+    """A NaN key or query element with capped logits, the other logits far below the cap or beyond it: the rows that have it are NaN, no other row is."""
+    lens, heads, cap = [400, 100], 8, 5.0
+    pool = Pool(lens, 16, 2, dim, seed=55).cuda()
+    q = queries(sum(counts), heads, dim, dtype, 56) * factor
+    clean, _ = attend(pool, q, lens, counts, heads, dtype=dtype, out=out, softcap=cap)
+    hit = torch.zeros(clean.shape[:2], dtype=torch.bool, device="cuda")
+    if which == "key":
+        key = lens[0] - counts[0] + counts[0] // 2
+        pool.t[0][int(pool.table[0, key // 16]), key % 16, 1, 9] = 0x7f
+        hit[counts[0] // 2:counts[0], 4:] = True
+    else:
+        q[counts[0] // 2, 3, 11] = float("nan")
+        hit[counts[0] // 2, 3] = True
+    dirty, stats = attend(pool, q, lens, counts, heads, dtype=dtype, out=out, softcap=cap)
+    assert torch.equal(dirty.isnan().any(-1), hit) and torch.equal(stats.isnan(), hit)
+    assert bool(clean.isfinite().all())
