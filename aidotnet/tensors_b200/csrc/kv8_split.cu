@@ -1,7 +1,7 @@
 // Attention of few queries over a paged pool held in 8 bits (kv8.cuh): decode steps, drafted tokens, short chunks.
 //
 //   S^T = K Q^T,  x = S c_r k_scale(block)   (base 2; c_r = scale log2(e) / the query's own factor)
-//   P = 2^(x - m) with a running maximum m,   O^T += V^T (P v_scale(block) / v_ref)^T,   o = O v_ref / sum P
+//   P = 2^(x - m), m the running maximum less 9,   O^T += V^T (P v_scale(block) / v_ref)^T,   o = O v_ref / sum P
 //
 // Bound by the pool's bytes: 2 D bytes a key and KV head, a few operations a byte.  So every key is read once for all the queries of its
 // sequence and KV head (a "line": up to 8 NR query rows = query heads of the group x queries).  A warp has a line's next tiles of 16 keys
@@ -29,8 +29,8 @@ namespace {
 
 constexpr int kTile = 16;           // keys
 constexpr float kUnset = -1e30f;    // running maximum before any key
-constexpr float kLazy = 6.f;        // the maximum follows when a logit is 2^6 above it: weights stay below 2^(9 + 6), in fp16's range
-constexpr float kLift = 9.f;
+constexpr float kLift = 9.f;        // m is the running maximum less this: the largest weight is 2^9
+constexpr float kMost = 15.f;       // m follows when a weight is above 2^15: all are in fp16's range
 constexpr int kMergeThreads = 256;
 constexpr int kMostUnits = 4096;   // (twelve bits in the merging kernel)
 
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             if (!ok[e >> 1] || key0 + k >= lim[n][e & 1]) x = -INFINITY;
           }
           s[n][e] = x;
-          grow = grow || x > m[n][e & 1] + kLazy;
+          grow = grow || x - m[n][e & 1] > kMost;   // (the weight's exponent as it is formed: large logits round m, but not the difference)
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -506,7 +506,9 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             float top = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float now = fmaxf(m[n][e], top), keep = ex2_approx(m[n][e] - now);
+            float lifted = top - kLift;
+            if (top - lifted > kLift) lifted = top;   // (it was rounded)
+            const float now = fmaxf(m[n][e], lifted), keep = ex2_approx(m[n][e] - now);
             m[n][e] = now;
             l[n][e] *= keep;
 #pragma unroll
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {   // key g + 8 j, rows 2t and 2t + 1
-          float a = ex2_approx(s[n][2 * j] - (m[n][0] - kLift)), w = ex2_approx(s[n][2 * j + 1] - (m[n][1] - kLift));
+          float a = ex2_approx(s[n][2 * j] - m[n][0]), w = ex2_approx(s[n][2 * j + 1] - m[n][1]);
           l[n][0] += a;
           l[n][1] += w;
           const float f = vs[j] * inv_vref;
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float top_e = __shfl_sync(0xffffffffu, m[n][e] - kLift, lane >> 1 & 3), sum_e = __shfl_sync(0xffffffffu, sum[n][e], lane >> 1 & 3);
+        const float top_e = __shfl_sync(0xffffffffu, m[n][e], lane >> 1 & 3), sum_e = __shfl_sync(0xffffffffu, sum[n][e], lane >> 1 & 3);
         if (lane >> 3 == n && (lane & 1) == e) {
           my_top = top_e;
           my_sum = sum_e;

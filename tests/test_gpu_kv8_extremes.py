@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from aidotnet.tensors_b200 import native as N
 from tests._harness import TORCH_DT
 from tests.test_gpu_kv8 import Pool, attend, attend64, bounds, queries
 
@@ -55,6 +56,33 @@ LARGE = [16, 19, 20, 21, 24, 25, 26, 27, 28, 29, 30, 33, 40, 60]
 @pytest.mark.parametrize("dtype,dim,workspace", [("bf16", 128, True), ("f16", 64, True), ("bf16", 64, False)])
 def test_large_logits_of_many_queries(exponent, sign, dtype, dim, workspace):
     check_tied([300, 1290], [150, 70], 8, 2, dim, 16, dtype, exponent, sign, workspace=workspace)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("exponent", LARGE)
+@pytest.mark.parametrize("dtype,out,dim,count,block", [("bf16", "bf16", 128, 1, 16), ("f16", "f16", 64, 4, 16), ("bf16", "f32", 128, 1, 16), ("f32", "f32", 256, 3, 24)])
+def test_large_logits_of_few_queries(exponent, sign, dtype, out, dim, count, block):
+    check_tied([300, 1290, 17], [count] * 3, 8, 2, dim, block, dtype, exponent, sign, out=out)
+
+
+@pytest.mark.parametrize("exponent", [26, 27, 28, 30])
+@pytest.mark.parametrize("path", [N.PATH_AUTO, N.PATH_GENERIC])
+def test_large_logits_one_after_the_other(exponent, path):
+    """Keys whose logits rise by one or two units in the last place of the largest: each new maximum is a little above the one before.  (Within a few
+    units the weights depend on how the products were rounded: results lie between the values.)"""
+    dim, lens = 64, [900, 333]
+    pool = Pool(lens, 16, 2, dim, seed=57)
+    pool.codes[0][..., 0], pool.codes[0][..., 1:] = 0x38, 0x38
+    pool.scales[0][:] = 1.0
+    for b in range(2):
+        for j in range(-(-lens[b] // 16)):
+            pool.scales[0][pool.table[b, j]] = 1 + j * 2.0 ** -23
+    pool.cuda()
+    q = looking_at_the_first(2, 4, dim, "bf16", 1)
+    out, stats = attend(pool, q, lens, [1, 1], 4, dtype="bf16", scale=2.0 ** exponent / math.log2(math.e), path=path)
+    most = max(np.abs(pool.rows(1, b, n)).max() for b, n in enumerate(lens))
+    assert bool(out.isfinite().all()) and bool(stats.isfinite().all())
+    assert float(out.abs().max()) <= most * (1 + 2.0 ** -7)
 
 
 @pytest.mark.parametrize("size", [3e2, 2e4, 1e6, 1e12])
