@@ -1,15 +1,15 @@
 // Attention of many queries over a paged pool held in 8 bits (kv8.cuh) on tcgen05: prompt chunks, ragged batches, drafted tokens.
 //
 //   x = (Q K^T) c_r k_scale(block)      (base 2; c_r = scale log2(e) / the query's own factor)
-//   P = 2^(x - m + e - e_ref + lift),   e = log2(v_scale(block)),   O += P V,   l += 2^(x - m)
-//   o = O 2^(e_ref - lift) / l
+//   P = 2^((x - m) + e - e_ref + lift),   e = log2(v_scale(block)),   O += P V,   l += 2^(x - m)
+//   o = O 2^(e_ref - lift) / l,           m, e_ref: the largest x and (x - m) + e that the row has seen, when they were last taken
 //
 // A line is (sequence, KV head, pair of 128-row tiles); a row is a (query, query head of the group), so that a few queries of a
 // group fill a tile as well as many of one head.  4 D operations a (row, key): bound by the tensor cores for two full tiles, and by the
 // pool's bytes where a line has few rows.  Codes become fp16 on the way into shared memory, exactly; the scales of the blocks touch
 // sixteen scores at a time, as a factor of the logits and an offset of the exponents, so that they cost nothing per score, and
 // queries are scaled by a power of two into fp16 (bf16 and fp16 queries lose nothing that their largest element leaves visible).
-// Weights are fp16, 11 bits, lifted so that they stay normal down to 2^-18 of the largest.
+// Weights are fp16, 11 bits, lifted so that they stay normal down to 2^-18 of the row's largest product of weight and scale.
 //
 //   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
 //                     (16 bits), results.  A row keeps the maximum that it has until sixteen weights sum up to 2^15 (a logit about
@@ -50,8 +50,10 @@ static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kMmaRegs <= kThrea
 constexpr int kRing = 4;              // tiles whose scales are kept
 constexpr float kUnset = -1e30f;
 constexpr float kLift = 4.f;
+constexpr float kLeastScale = -110.f;     // log2 of a scale at least: below that of any block that an append wrote (2^-100); sixteen weights over it are in fp32's range
 constexpr int kTileCost = 3, kPairCost = 4;   // of 128 keys with one row tile, and with two, which overlap (64 keys: 1700 cycles, and 2300)
 constexpr float kMostWeights = 32768.f;   // of sixteen weights together: each is then in fp16's range
+constexpr float kMostSum = 0x1p100f;      // of sixty-four weights without their scales: logits rise above m where blocks of small values follow large ones
 constexpr float kLargeLogit = 1048576.f;  // (to base 2) a rounding of half a unit of its last place is 2^-4 here
 
 template <int HD>
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
         const int lim_least = visible(p, w.keys, w.rw.count, (w.u * kPairRows + a * kTileRows) / G);
         const int lim_pair = visible(p, w.keys, w.rw.count, w.u * kPairRows / G);   // what the converters clean a tile by
         const float cap_inverse = CAP ? 1.f / p.softcap : 0.f;
-        float m = kUnset, l = 0.f, eref = kUnset, l_unit = 0.f;   // l_unit = 2^(eref - lift): sums of weights over it and the scale are l's
+        float m = kUnset, l = 0.f, eref = 0.f, l_unit = 0.f;   // l_unit = 2^(eref - lift): sums of weights over it and the scale are l's
 
         if (!w.whole && w.t0 == 0 && tid == 0) {
           const int parts = (int)quotient(w.base + (int64_t)(w.tiles - 1) * w.cost, share) - (int)blockIdx.x + 1;
@@ -486,22 +488,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
               if (again) {
                 float keep = 1.f;
                 if (far) {
-                  float top = m, emax = eref;
+                  float top = m, y[4];   // of the groups of which the row sees a key
 #pragma unroll
                   for (int g = 0; g < 4; ++g) {
                     float m0 = __uint_as_float(s[16 * g]);
 #pragma unroll
                     for (int k = 1; k < 15; k += 2) m0 = fmax3(m0, __uint_as_float(s[16 * g + k]), __uint_as_float(s[16 * g + k + 1]));
                     m0 = fmaxf(m0, __uint_as_float(s[16 * g + 15]));
-                    const float y = m0 * ck[g];
-                    if (e[g] != -INFINITY && m0 != -INFINITY) top = fmaxf(top, y);
-                    emax = fmaxf(emax, e[g]);
+                    y[g] = e[g] != -INFINITY && m0 != -INFINITY ? m0 * ck[g] : -INFINITY;
+                    top = fmaxf(top, y[g]);
                   }
-                  const float f = ex2_approx(m - top);
-                  keep = f * ex2_approx(eref - emax);
-                  l *= f;
+                  const float down = m - top;
+                  float now = eref + down;   // eref: the largest (x - m) + e
+#pragma unroll
+                  for (int g = 0; g < 4; ++g) now = fmaxf(now, (y[g] - top) + e[g]);
+                  keep = ex2_approx(down + (eref - now));
+                  l *= ex2_approx(down);
                   m = top;
-                  eref = emax;
+                  eref = now;
                   l_unit = ex2_approx(eref - kLift);
                 }
                 if (u > 0 && __any_sync(0xffffffffu, keep != 1.f)) {   // (one product at most is on its way, that of the step before: the next needs these weights)
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
                 tmem_st16(ts0 + 64 * buf + 16 * q, packed);
               }
               if (again) break;
-              far = most > kMostWeights;
+              far = most > kMostWeights || sum * l_unit > kMostSum;
               if (!__any_sync(0xffffffffu, far)) break;
               again = true;
             }
@@ -773,11 +777,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_sm100_kernel(const __grid_con
           }
           if (lane < 2) {
             float exponent = log2_approx(vs);
-            if (exponent < -120.f) exponent = -120.f;   // (a NaN stays one)
+            if (exponent < kLeastScale) exponent = kLeastScale;   // (a NaN stays one)
             Misc::Scales& sc = ms.scales[ring];
             sc.k[2 * quarter + lane] = ks;
             sc.v_exp[2 * quarter + lane] = before < 0 ? -INFINITY : exponent;
-            sc.v_inverse[2 * quarter + lane] = before < 0 ? 0.f : ex2_approx(-exponent);
+            // (of a NaN something finite: it is multiplied with zero for rows that do not see the keys)
+            sc.v_inverse[2 * quarter + lane] = before < 0 ? 0.f : exponent == exponent ? ex2_approx(-exponent) : 1.f;
           }
           if (lane == 0) ms.scales[ring].nan[quarter] = nan;
           convert(dst0 + C::kV + stage * C::kTile, xv);

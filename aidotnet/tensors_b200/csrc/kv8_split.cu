@@ -1,7 +1,8 @@
 // Attention of few queries over a paged pool held in 8 bits (kv8.cuh): decode steps, drafted tokens, short chunks.
 //
 //   S^T = K Q^T,  x = S c_r k_scale(block)   (base 2; c_r = scale log2(e) / the query's own factor)
-//   P = 2^(x - m), m the running maximum less 9,   O^T += V^T (P v_scale(block) / v_ref)^T,   o = O v_ref / sum P
+//   with running maxima m of x and b of (x - m) + log2(v_scale(block)) - 9 (rounded up):
+//   P = 2^(x - m) (v_scale(block) 2^-b),   O^T += V^T P^T,   l += 2^(x - m),   o = O 2^b / l
 //
 // Bound by the pool's bytes: 2 D bytes a key and KV head, a few operations a byte.  So every key is read once for all the queries of its
 // sequence and KV head (a "line": up to 8 NR query rows = query heads of the group x queries).  A warp has a line's next tiles of 16 keys
@@ -9,8 +10,9 @@
 // product does not care about the order of its terms, so the head dimension is permuted such that a lane's 16 bytes of a key are its
 // own elements of four A fragments, and a lane's 16 bytes of a value row its own rows of eight (queries are laid out in the
 // matching order once a line).  A code becomes fp16 exactly (cvt, two at a time), a query is scaled by a power of two into
-// fp16 (two terms for fp32 results), and the scales of the blocks are applied to the products in fp32.  Weights are rounded to fp16
-// (11 bits, of 2^9 times their value so that they stay normal down to 2^-23 of the largest); for fp32 results they are two terms too.
+// fp16 (two terms for fp32 results), the scales of the blocks are applied to the products in fp32 and those of the values to the weights, and
+// these rounded to fp16: 11 bits, of up to 2^9 so that they stay normal down to 2^-23 of the row's largest product of weight and scale; for fp32
+// results they are two terms too.  What a row does not see has no part in its maxima.
 //
 // The warps of a "unit" do the same tiles of neighbouring KV heads, whose rows are neighbours in the pool: memory is read in runs
 // of up to 512 bytes (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 228 us, and 265 us where each warp goes through lines of its own;
@@ -29,8 +31,10 @@ namespace {
 
 constexpr int kTile = 16;           // keys
 constexpr float kUnset = -1e30f;    // running maximum before any key
-constexpr float kLift = 9.f;        // m is the running maximum less this: the largest weight is 2^9
-constexpr float kMost = 15.f;       // m follows when a weight is above 2^15: all are in fp16's range
+constexpr float kLift = 9.f;        // the largest weight is 2^9
+constexpr float kMost = 32768.f;    // the maxima follow when a weight is above this: all are in fp16's range
+constexpr float kMostSum = 0x1p100f;   // or l: logits rise above m where blocks of small values follow large ones
+constexpr float kMostFactor = 0x1p126f;
 constexpr int kMergeThreads = 256;
 constexpr int kMostUnits = 4096;   // (twelve bits in the merging kernel)
 
@@ -73,6 +77,13 @@ __device__ __forceinline__ float lds_f(uint32_t at) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
   return r;
 }
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float pow2(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }   // of a whole number in [-126, 127]
+__device__ __forceinline__ float exponent_of(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
 __device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -379,9 +390,8 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
     }
 
     float acc[NR][MT][4];
-    float m[NR][2], l[NR][2], c[NR][2];
+    float m[NR][2], factor[NR][2], l[NR][2], c[NR][2];   // factor: 2^-b, exactly
     int lim[NR][2];
-    float vref = 0.f, inv_vref = 0.f;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
@@ -391,6 +401,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         m[n][e] = kUnset;
+        factor[n][e] = 1.f;
         l[n][e] = 0.f;
         c[n][e] = __shfl_sync(0xffffffffu, c_row[n], 4 * (2 * t + e));
         lim[n][e] = __shfl_sync(0xffffffffu, lim_row[n], 4 * (2 * t + e));
@@ -483,7 +494,13 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             if (who & (0x11111111u << tt)) nan_keys |= 1u << (2 * tt + (j & 1) + 8 * (j >> 1));
         }
       }
-      bool grow = false;
+      // (a scale of the values that is no number makes the logits none, of the rows that see them)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (!(vs[j] < INFINITY)) {
+          ks[j] = NAN;
+          vs[j] = 1.f;
+        }
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -496,9 +513,25 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             if (!ok[e >> 1] || key0 + k >= lim[n][e & 1]) x = -INFINITY;
           }
           s[n][e] = x;
-          grow = grow || x - m[n][e & 1] > kMost;   // (the weight's exponent as it is formed: large logits round m, but not the difference)
         }
-      if (__any_sync(0xffffffffu, grow)) {
+      // The weights with the maxima so far; again, once, with the tile's own where one does not fit, or the sum may not.
+      float a[NR][4], sum[NR][2];
+#pragma unroll 1
+      for (bool again = false;; again = true) {
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = ex2_approx(s[n][e] - m[n][e]), y = ex2_approx(s[n][e + 2] - m[n][e]);
+            sum[n][e] = l[n][e] + x + y;
+            // (factors that are finite, for keys that a row does not see)
+            a[n][e] = x * fminf(vs[0] * factor[n][e], kMostFactor);
+            a[n][e + 2] = y * fminf(vs[1] * factor[n][e], kMostFactor);
+            grow = grow || fmaxf(a[n][e], a[n][e + 2]) > kMost || sum[n][e] > kMostSum;
+          }
+        if (again || !__any_sync(0xffffffffu, grow)) break;
+        const float lv[2] = {lg2_approx(vs[0]), lg2_approx(vs[1])};
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -506,11 +539,16 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             float top = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float lifted = top - kLift;
-            if (top - lifted > kLift) lifted = top;   // (it was rounded)
-            const float now = fmaxf(m[n][e], lifted), keep = ex2_approx(m[n][e] - now);
-            m[n][e] = now;
-            l[n][e] *= keep;
+            top = fmaxf(m[n][e], top);
+            float most = fmaxf((s[n][e] - top) + lv[0], (s[n][e + 2] - top) + lv[1]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float down = m[n][e] - top, before = exponent_of(factor[n][e]);
+            const float now = fmaxf(-126.f, fminf(ceilf(fmaxf(down - before, most - kLift)), 126.f));   // b
+            const float keep = ex2_approx(down - before - now);
+            factor[n][e] = pow2(-now);
+            m[n][e] = top;
+            l[n][e] *= ex2_approx(down);
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               acc[n][j][e] *= keep;
@@ -518,38 +556,16 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
             }
           }
       }
-      // scales of the values relative to the largest so far
-      float vtop = fmaxf(vs[0], vs[1]);
-      if (!UB) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
-      }
-      if (vtop > vref) {
-        const float keep = vref / vtop;
-        vref = vtop;
-        inv_vref = 1.f / vtop;
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][j][e] *= keep;
-      }
       uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {   // key g + 8 j, rows 2t and 2t + 1
-          float a = ex2_approx(s[n][2 * j] - m[n][0]), w = ex2_approx(s[n][2 * j + 1] - m[n][1]);
-          l[n][0] += a;
-          l[n][1] += w;
-          const float f = vs[j] * inv_vref;
-          a *= f;
-          w *= f;
-          const __half2 hi = __floats2half2_rn(a, w);
+          l[n][j] = sum[n][j];
+          const __half2 hi = __floats2half2_rn(a[n][2 * j], a[n][2 * j + 1]);
           ph[n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
           if constexpr (T == 2) {
-            const __half2 lo = __floats2half2_rn(a - __low2float(hi), w - __high2float(hi));
+            const __half2 lo = __floats2half2_rn(a[n][2 * j] - __low2float(hi), a[n][2 * j + 1] - __high2float(hi));
             pl[n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
           }
         }
@@ -584,7 +600,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
         for (int o = 4; o < 32; o <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
       }
     // (row r's to lane r; its elements through the tiles' place, in which no copy is under way, groups of four in an order without conflicts)
-    float my_top = 0.f, my_sum = 0.f;
+    float my_top = 0.f, my_sum = 0.f, my_unit = 0.f;
     cp_async_wait<0>();
     __syncwarp();
     float* const rows_at = reinterpret_cast<float*>(smem + warp * STAGES * C::kStage);
@@ -593,9 +609,11 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float top_e = __shfl_sync(0xffffffffu, m[n][e], lane >> 1 & 3), sum_e = __shfl_sync(0xffffffffu, sum[n][e], lane >> 1 & 3);
+        const float unit_e = __shfl_sync(0xffffffffu, inverse_pow2(factor[n][e]), lane >> 1 & 3);
         if (lane >> 3 == n && (lane & 1) == e) {
           my_top = top_e;
           my_sum = sum_e;
+          my_unit = unit_e;
         }
         float* const to = rows_at + (8 * n + 2 * t + e) * DP;
 #pragma unroll
@@ -606,7 +624,7 @@ __global__ void __launch_bounds__(Config<DP, NR, T, UB>::kWarps * 32, Config<DP,
       }
     __syncwarp();
     const int64_t part = ((int64_t)(2 * unit + (t0 == 0 ? 1 : 0)) << sp.heads_log2) + sub;
-    const float mine_f = !whole ? vref : (my_sum == 0.f ? 0.f : vref / my_sum);
+    const float mine_f = !whole ? my_unit : (my_sum == 0.f ? 0.f : my_unit / my_sum);
     // (lane r knows where row r goes)
     const int my_i = rw.count == 1 ? 0 : (r0 + lane) / G, my_h = kvh * G + (r0 + lane) - my_i * G;
     const int64_t my_to = whole ? query_at(p, p.os, rw, b, my_h, my_i) : (part * sp.row_most + lane) * DP;

@@ -1,4 +1,4 @@
-"""Attention over an 8-bit pool far from ordinary values: large logits, NaN."""
+"""Attention over an 8-bit pool far from ordinary values: large logits, NaN, scales far apart."""
 import math
 
 import numpy as np
@@ -142,3 +142,69 @@ def test_nan_behind_a_softcap(dtype, out, counts, which, factor, dim):
     dirty, stats = attend(pool, q, lens, counts, heads, dtype=dtype, out=out, softcap=cap)
     assert torch.equal(dirty.isnan().any(-1), hit) and torch.equal(stats.isnan(), hit)
     assert bool(clean.isfinite().all())
+
+
+def loud_and_quiet(lens, block, dim, seed, loud, quiet, every):
+    """Blocks with number 2 mod `every` of a sequence: values of scale 2^loud, and keys whose logits for a query that begins with 60 are about 40 (natural) below those of
+    the others, whose values' scale is 2^quiet.  Other elements are ordinary."""
+    pool = Pool(lens, block, 2, dim, seed=seed)
+    pool.scales[0][:] = 2.0 ** -7
+    pool.codes[0][..., 0] = 0
+    pool.scales[1][:] = 2.0 ** quiet
+    for b in range(pool.batch):
+        for j in range(2, -(-lens[b] // block), every):
+            pool.codes[0][pool.table[b, j], ..., 0] = 0xfe   # -448
+            pool.scales[1][pool.table[b, j]] = 2.0 ** loud
+    return pool
+
+
+VALUE_CASES = [("bf16", "bf16", 128, [1, 1], 16), ("f16", "f16", 64, [4, 4], 16), ("f16", "f32", 64, [1, 1], 24), ("f32", "f32", 64, [5, 3], 16),
+               ("bf16", "bf16", 128, [150, 60], 16), ("f16", "f16", 64, [150, 60], 16)]
+
+
+@pytest.mark.parametrize("dtype,out,dim,counts,block", VALUE_CASES)
+@pytest.mark.parametrize("loud,quiet", [(18, -6), (28, -6), (20, -26), (5, -100), (-100, 5), (100, 60)])
+def test_large_values_that_have_no_weight(dtype, out, dim, counts, block, loud, quiet):
+    """The weights' precision goes by what they add to the result: blocks of large values but weights of 2^-58 cost the others nothing."""
+    lens = [700, 410]
+    pool = loud_and_quiet(lens, block, dim, 58, loud, quiet, 4)
+    if quiet == -100:
+        pool.codes[1][:] = np.where((pool.scales[1] == 2.0 ** quiet)[:, None, :, None], 0, pool.codes[1])   # as an append writes zeros
+    pool.cuda()
+    q = queries(sum(counts), 8, dim, dtype, 59)
+    q[..., 0] = 60 * math.sqrt(dim) / math.sqrt(32)
+    o, lse, a, top = attend64(pool, q.double().cpu().numpy(), lens, counts, 8, scale=1 / math.sqrt(dim))
+    bo, bl = bounds(o, lse, a, top, dtype, out, dim)
+    got, stats = attend(pool, q, lens, counts, 8, dtype=dtype, out=out)
+    got, stats = got.double().cpu().numpy(), stats.double().cpu().numpy()
+    if out == "f16":   # (what 16 bits hold)
+        assert np.abs(o).max() < 65504 or loud > 30
+        o, bo = np.clip(o, -65504, 65504), np.where(np.abs(o) + bo > 65504, np.inf, bo)
+    assert (np.abs(got - o) <= bo)[np.isfinite(bo)].all()
+    assert (np.abs(stats - lse) <= bl).all()
+
+
+@pytest.mark.parametrize("dtype,out,dim,counts,block", VALUE_CASES)
+@pytest.mark.parametrize("scale", [2.0 ** 30, float("nan"), float("inf")])
+def test_scales_of_values_that_a_query_does_not_see(dtype, out, dim, counts, block, scale):
+    """Causal: the last block's values have a scale far above the others', or one that is no number.  Queries before that block's first key have the results
+    that they have without it, up to how the sums are ordered; those that see it are not finite where it is not."""
+    lens = [64 * 5 + 3, 64 * 2 + 2]
+    counts = [max(counts[0], 5), max(counts[1], 4)]
+    pool = Pool(lens, block, 2, dim, seed=60).cuda()
+    q = queries(sum(counts), 8, dim, dtype, 61)
+    for b, n in enumerate(lens):
+        pool.s[1][int(pool.table[b, (n - 1) // block])] = scale
+        pool.scales[1][pool.table[b, (n - 1) // block]] = scale
+    with np.errstate(invalid="ignore", over="ignore"):
+        o, lse, a, top = attend64(pool, q.double().cpu().numpy(), lens, counts, 8, scale=1 / math.sqrt(dim))
+    bo, _ = bounds(o, lse, a, top, dtype, out, dim)
+    got, _ = attend(pool, q, lens, counts, 8, dtype=dtype, out=out)
+    got, r = got.double().cpu().numpy(), 0
+    for n, c in zip(lens, counts):
+        edge = (n - 1) // block * block   # the block's first key
+        blind = max(0, edge - (n - c))    # queries that do not see it
+        assert (np.abs(got - o) <= bo)[r:r + blind].all()
+        if not math.isfinite(scale):
+            assert not np.isfinite(got[r + blind:r + c]).all(-1).any()
+        r += c
