@@ -48,7 +48,7 @@ constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kMmaRegs = 48;
 // setmaxnreg.inc waits without a bound for registers that are not there: the shares must not exceed what the CTA is launched with
 static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kMmaRegs <= kThreads * 128, "registers of the launch");
 constexpr int kRing = 4;              // tiles whose scales are kept
-constexpr float kUnset = -1e30f;
+constexpr float kUnset = -3e38f;      // maximum before any key: below every finite logit but the last few
 constexpr float kLift = 4.f;
 constexpr float kLeastScale = -110.f;     // log2 of a scale at least: below that of any block that an append wrote (2^-100); sixteen weights over it are in fp32's range
 constexpr int kTileCost = 3, kPairCost = 4;   // of 128 keys with one row tile, and with two, which overlap (64 keys: 1700 cycles, and 2300)

@@ -30,7 +30,7 @@ namespace kv8 {
 namespace {
 
 constexpr int kTile = 16;           // keys
-constexpr float kUnset = -1e30f;    // running maximum before any key
+constexpr float kUnset = -3e38f;    // running maximum before any key: below every finite logit but the last few
 constexpr float kLift = 9.f;        // the largest weight is 2^9
 constexpr float kMost = 32768.f;    // the maxima follow when a weight is above this: all are in fp16's range
 constexpr float kMostSum = 0x1p100f;   // or l: logits rise above m where blocks of small values follow large ones

@@ -208,3 +208,11 @@ def test_scales_of_values_that_a_query_does_not_see(dtype, out, dim, counts, blo
         if not math.isfinite(scale):
             assert not np.isfinite(got[r + blind:r + c]).all(-1).any()
         r += c
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("exponent", [99, 100, 112, 120])
+@pytest.mark.parametrize("dtype,dim,count", [("bf16", 128, 1), ("f32", 64, 3), ("bf16", 128, 150), ("f16", 64, 90)])
+def test_logits_of_every_finite_size(exponent, sign, dtype, dim, count):
+    """Logits of up to 2^121, none of them above -2^98 where they are negative: the largest still has the weight."""
+    check_tied([300, 290], [count] * 2, 8, 2, dim, 16, dtype, exponent, sign)
