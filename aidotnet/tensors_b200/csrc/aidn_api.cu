@@ -821,7 +821,7 @@ int build_pool(const char* op, const aidn_kv8_cache* c, aidn::kv8::Pool& pool) {
   pool.v_scale = c->value_scale;
   pool.table = c->block_table;
   pool.table_stride = c->block_table_stride;
-  const int64_t D = c->head_dim, dense[3] = {c->block_size * c->kv_heads * D, c->kv_heads * D, D};
+  const int64_t D = c->head_dim, dense[3] = {c->block_size * (c->kv_heads * D), c->kv_heads * D, D};
   std::memcpy(pool.stride, all_zero(c->pool_stride) ? dense : c->pool_stride, sizeof(pool.stride));
   for (int i = 0; i < 3; ++i)
     if (pool.stride[i] < 0 || pool.stride[i] % 4 != 0) return fail(AIDN_EINVAL, "%s: pool strides must be multiples of 4 and not negative", op);

@@ -82,3 +82,8 @@ def test_append_refuses(lib, cache, args, word):
 
 def test_append_of_nothing_is_no_launch(lib):
     N.kv8_append(N.kv8_cache(**GOOD), stream=0, **{**ARGS, "tokens": 0, "key": 0, "value": 0, "start": 0})
+
+
+def test_blocks_of_more_than_2_to_the_31_rows(lib):
+    """The strides of a dense pool are 64-bit whatever its block size and heads are: such a pool is taken."""
+    N.kv8_append(N.kv8_cache(**{**GOOD, "block_size": 65536, "kv_heads": 32768}), stream=0, **{**ARGS, "tokens": 0})
