@@ -294,7 +294,7 @@ class Handle:
         self._lib = load()
         while _left and not _capturing():
             self._lib.aidn_sdpa_destroy(_left.pop())
-        self._kv8_sizes = self._kv8_need = None
+        self._kv8_asked = None
         d = SdpaDesc()
         d.device, d.qkv_dtype, d.out_dtype, d.head_dim = device, qkv_dtype, out_dtype, head_dim
         d.num_q_heads = num_q_heads
@@ -339,12 +339,13 @@ class Handle:
 
     def kv8_workspace_bytes(self, batch: int, seq_q: int, seq_kv: int) -> int:
         sizes = (batch, seq_q, seq_kv)
-        if sizes != self._kv8_sizes:   # (a function of them and of the handle; consecutive steps mostly ask for the same)
+        asked = self._kv8_asked   # (sizes and their need in one: another thread may ask the same handle for others)
+        if asked is None or asked[0] != sizes:   # (a function of them and of the handle; consecutive steps mostly ask for the same)
             n = self._lib.aidn_sdpa_kv8_workspace_bytes(self._h, batch, seq_q, seq_kv)
             if n < 0:
                 raise AidnError(EINVAL, last_error())
-            self._kv8_sizes, self._kv8_need = sizes, int(n)
-        return self._kv8_need
+            asked = self._kv8_asked = (sizes, int(n))
+        return asked[1]
 
     def launch_kv8(self, *, q: int, out: int, cache: bytes, batch: int, seq_q: int, seq_kv: int, stream: int,
                    query_starts: Optional[int] = None, queries: int = 0, lse: Optional[int] = None,

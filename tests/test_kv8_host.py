@@ -87,3 +87,28 @@ def test_append_of_nothing_is_no_launch(lib):
 def test_blocks_of_more_than_2_to_the_31_rows(lib):
     """The strides of a dense pool are 64-bit whatever its block size and heads are: such a pool is taken."""
     N.kv8_append(N.kv8_cache(**{**GOOD, "block_size": 65536, "kv_heads": 32768}), stream=0, **{**ARGS, "tokens": 0})
+
+
+def test_workspace_size_between_two_threads():
+    """A thread that asks at any moment at which another one's answer is being kept gets the need of its own sizes."""
+    class Sizes:
+        @staticmethod
+        def aidn_sdpa_kv8_workspace_bytes(handle, batch, seq_q, seq_kv):
+            return batch * 1000000 + seq_q * 1000 + seq_kv
+
+    class Watched(N.Handle):
+        def __init__(self):
+            self.__dict__.update(_lib=Sizes, _h=None, _kv8_asked=None, _kv8_sizes=None, _kv8_need=None, other=None)
+
+        def __setattr__(self, name, value):
+            object.__setattr__(self, name, value)
+            if name != "other" and self.other is None:   # what a thread that runs now would see
+                self.other = True
+                wrong.extend(s for s in ((1, 2, 3), (4, 5, 6)) if self.kv8_workspace_bytes(*s) != Sizes.aidn_sdpa_kv8_workspace_bytes(None, *s))
+                self.other = None
+
+    wrong = []
+    h = Watched()
+    for sizes in ((1, 2, 3), (4, 5, 6), (1, 2, 3)):
+        assert h.kv8_workspace_bytes(*sizes) == Sizes.aidn_sdpa_kv8_workspace_bytes(None, *sizes)
+    assert not wrong
