@@ -6,6 +6,7 @@ call fails, an exception is raised.
 """
 from __future__ import annotations
 
+import atexit
 import ctypes
 import os
 import struct
@@ -292,8 +293,8 @@ class Handle:
                  path: int = PATH_AUTO, head_begin: int = 0, head_count: int = 0, decode_chunk: int = 0,
                  max_batch: int = 0, max_seq_q: int = 0, max_seq_kv: int = 0, nccl_comm: Optional[int] = None):
         self._lib = load()
-        while _left and not _capturing():
-            self._lib.aidn_sdpa_destroy(_left.pop())
+        if _left:
+            _destroy_left()
         self._kv8_asked = None
         d = SdpaDesc()
         d.device, d.qkv_dtype, d.out_dtype, d.head_dim = device, qkv_dtype, out_dtype, head_dim
@@ -310,6 +311,8 @@ class Handle:
         self._h = h
 
     def workspace_bytes(self, batch: int, seq_q: int, seq_kv: int) -> int:
+        if _left:
+            _destroy_left()
         n = self._lib.aidn_sdpa_workspace_bytes(self._h, batch, seq_q, seq_kv)
         if n < 0:
             raise AidnError(EINVAL, last_error())
@@ -338,6 +341,8 @@ class Handle:
             raise AidnError(status, last_error())
 
     def kv8_workspace_bytes(self, batch: int, seq_q: int, seq_kv: int) -> int:
+        if _left:
+            _destroy_left()
         sizes = (batch, seq_q, seq_kv)
         asked = self._kv8_asked   # (sizes and their need in one: another thread may ask the same handle for others)
         if asked is None or asked[0] != sizes:   # (a function of them and of the handle; consecutive steps mostly ask for the same)
@@ -403,6 +408,8 @@ class Handle:
         check(self._lib.aidn_mha_forward(self._h, ctypes.byref(a), ctypes.c_void_p(stream)))
 
     def poll(self, stream: int) -> None:
+        if _left:
+            _destroy_left()
         check(self._lib.aidn_sdpa_poll(self._h, ctypes.c_void_p(stream)))
 
     @property
@@ -422,10 +429,18 @@ class Handle:
             self._h = None
 
     def __del__(self):
-        # The collector may run inside a graph's capture, which freeing device memory would end: such a handle is destroyed with the next one made.
+        # The collector may run inside a graph's capture, which freeing device memory would end: such a handle is destroyed by the next call on any
+        # handle that allocates, sizes or polls, and at the latest when the interpreter ends.
         try:
-            if _capturing():
-                _left.append(self._h)
+            if not getattr(self, "_h", None):
+                return
+            try:
+                busy = _capturing()
+            except Exception:   # the interpreter ends: nothing is captured
+                busy = False
+            if busy:
+                _left.append((self._lib, self._h))
+                self._h = None
             else:
                 self.close()
         except Exception:
@@ -438,12 +453,24 @@ class Handle:
         self.close()
 
 
-_left: list = []   # handles that were collected during a capture
+_left: list = []   # (library, handle) of those that were collected during a capture
 
 
 def _capturing() -> bool:
     torch = sys.modules.get("torch")
     return torch is not None and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _destroy_left() -> None:
+    while not _capturing():
+        try:
+            lib, h = _left.pop()
+        except IndexError:
+            return
+        lib.aidn_sdpa_destroy(h)
+
+
+atexit.register(_destroy_left)
 
 
 def cast(kind: str, src: int, dst: int, n: int, stream: int) -> None:
