@@ -827,6 +827,7 @@ int build_pool(const char* op, const aidn_kv8_cache* c, aidn::kv8::Pool& pool) {
     if (pool.stride[i] < 0 || pool.stride[i] % 4 != 0) return fail(AIDN_EINVAL, "%s: pool strides must be multiples of 4 and not negative", op);
   if ((uintptr_t)c->key_pool % 4 != 0 || (uintptr_t)c->value_pool % 4 != 0 || (uintptr_t)c->key_scale % 4 != 0 || (uintptr_t)c->value_scale % 4 != 0)
     return fail(AIDN_EINVAL, "%s: pools and scales must be 4-byte aligned", op);
+  if ((uintptr_t)c->block_table % 4 != 0) return fail(AIDN_EINVAL, "%s: the block table is not aligned to its entries", op);
   pool.num_blocks = c->num_blocks;
   pool.block_size = c->block_size;
   pool.kv_heads = c->kv_heads;
@@ -932,6 +933,9 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
     return fail(AIDN_EUNSUPPORTED, "launch_kv8: desc.path must be AUTO or GENERIC");
   const size_t esz = elem_size(d.qkv_dtype);
   if ((uintptr_t)a->q % esz != 0 || (uintptr_t)a->out % elem_size(d.out_dtype) != 0) return fail(AIDN_EINVAL, "launch_kv8: q or out is not aligned to its elements");
+  if ((uintptr_t)a->kv_len % 4 != 0 || (uintptr_t)query_starts % 4 != 0) return fail(AIDN_EINVAL, "launch_kv8: kv_len or query_starts is not aligned to its entries");
+  if ((d.emit_lse && (uintptr_t)a->lse % 4 != 0) || (d.mask_kind > AIDN_MASK_KEEP_U8 && (uintptr_t)a->mask % 4 != 0))
+    return fail(AIDN_EINVAL, "launch_kv8: lse or mask is not aligned to its elements");
   const int64_t D = d.head_dim;
   auto strides = [&](const int64_t* given, int64_t* to) {
     if (!all_zero(given)) std::memcpy(to, given, 3 * sizeof(int64_t));

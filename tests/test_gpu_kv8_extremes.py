@@ -216,3 +216,29 @@ def test_scales_of_values_that_a_query_does_not_see(dtype, out, dim, counts, blo
 def test_logits_of_every_finite_size(exponent, sign, dtype, dim, count):
     """Logits of up to 2^121, none of them above -2^98 where they are negative: the largest still has the weight."""
     check_tied([300, 290], [count] * 2, 8, 2, dim, 16, dtype, exponent, sign)
+
+
+@pytest.mark.parametrize("kind", [N.MASK_NONE, N.MASK_KEEP_U8, N.MASK_KEEP_F32, N.MASK_ADD_F32])
+def test_arrays_between_their_elements_are_refused(kind):
+    """Before anything is launched; a mask of bytes may lie anywhere."""
+    pool = Pool([40], 16, 2, 64, seed=62).cuda()
+    q, out = queries(1, 4, 64, "bf16", 63), torch.empty(4 * 64, dtype=torch.bfloat16, device="cuda")
+    lens, starts = torch.tensor([40, 0], dtype=torch.int32, device="cuda"), torch.tensor([0, 1, 0], dtype=torch.int32, device="cuda")
+    lse, mask = torch.empty(8, device="cuda"), torch.ones(256, device="cuda")
+    h = N.Handle(device=0, qkv_dtype=N.BF16, out_dtype=N.BF16, head_dim=64, num_q_heads=4, num_kv_heads=2, causal=True, emit_lse=True, mask_kind=kind)
+    good = dict(q=q.data_ptr(), out=out.data_ptr(), cache=pool.packed(), batch=1, seq_q=1, seq_kv=40, kv_len=lens.data_ptr(), lse=lse.data_ptr(),
+                mask=mask.data_ptr() if kind else None, stream=torch.cuda.current_stream().cuda_stream)
+    h.launch_kv8(**good)
+    bad = [dict(kv_len=lens.data_ptr() + 2), dict(lse=lse.data_ptr() + 1), dict(cache=pool.packed(block_table=pool.tab.data_ptr() + 2))]
+    if kind == N.MASK_NONE:
+        h.launch_kv8(**good, query_starts=starts.data_ptr(), queries=1)
+        bad.append(dict(query_starts=starts.data_ptr() + 2, queries=1))
+    elif kind == N.MASK_KEEP_U8:
+        h.launch_kv8(**{**good, "mask": mask.data_ptr() + 1})
+    else:
+        bad.append(dict(mask=mask.data_ptr() + 2))
+    for b in bad:
+        with pytest.raises(N.AidnError) as e:
+            h.launch_kv8(**{**good, **b})
+        assert e.value.status == N.EINVAL and "aligned" in str(e.value)
+    h.poll(torch.cuda.current_stream().cuda_stream)

@@ -112,3 +112,9 @@ def test_workspace_size_between_two_threads():
     for sizes in ((1, 2, 3), (4, 5, 6), (1, 2, 3)):
         assert h.kv8_workspace_bytes(*sizes) == Sizes.aidn_sdpa_kv8_workspace_bytes(None, *sizes)
     assert not wrong
+
+
+def test_append_refuses_a_block_table_between_entries(lib):
+    with pytest.raises(N.AidnError) as e:
+        N.kv8_append(N.kv8_cache(**{**GOOD, "block_table": 4098}), stream=0, **{**ARGS, "tokens": 0})
+    assert "aligned" in str(e.value)
