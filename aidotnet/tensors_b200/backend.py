@@ -61,7 +61,8 @@ class GpuBuffer:
 
 class KvCacheFp8:
     """A paged key / value pool held in 8 bits: E4M3 codes [numBlocks, blockSize, kvHeads, headDim] (one byte each) and a
-    power-of-two fp32 scale per (block, KV head), for keys and for values.  An element stands for code * scale."""
+    power-of-two fp32 scale per (block, KV head), for keys and for values.  An element stands for code * scale.  Its buffers and
+    sizes are what it was made with: a pool of others is another object."""
 
     def __init__(self, keys: GpuBuffer, values: GpuBuffer, keyScales: GpuBuffer, valueScales: GpuBuffer, blockSize: int,
                  kvHeads: int, headDim: int):
@@ -75,13 +76,18 @@ class KvCacheFp8:
         per = blockSize * kvHeads * headDim
         if keys.Size != values.Size or keys.Size < per or keys.Size % per != 0:
             raise ValueError("keys and values must be equal-sized and a whole number of blocks")
-        self.numBlocks = keys.Size // per
+        numBlocks = keys.Size // per
         for name, buf in (("keyScales", keyScales), ("valueScales", valueScales)):
-            if buf.dtype != torch.float32 or buf.Size < self.numBlocks * kvHeads:
+            if buf.dtype != torch.float32 or buf.Size < numBlocks * kvHeads:
                 raise ValueError(f"{name} must hold numBlocks * kvHeads fp32 values")
-        self.keys, self.values, self.keyScales, self.valueScales = keys, values, keyScales, valueScales
-        self.blockSize, self.kvHeads, self.headDim = blockSize, kvHeads, headDim
-        self._own = tuple(b.tensor.data_ptr() for b in (keys, values, keyScales, valueScales))   # (its buffers for as long as it lives)
+        buffers = (keys, values, keyScales, valueScales)
+        self.__dict__.update(
+            keys=keys, values=values, keyScales=keyScales, valueScales=valueScales, numBlocks=numBlocks, blockSize=blockSize, kvHeads=kvHeads,
+            headDim=headDim, _held=tuple(b.tensor for b in buffers),   # (the memory that the addresses are of, whatever becomes of the buffer objects)
+            _own=tuple(b.tensor.data_ptr() for b in buffers))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KvCacheFp8.{name} cannot be changed")
 
     def _pack(self, table: int, blocksPerSeq: int) -> bytes:
         """The ``aidn_kv8_cache`` block, packed in one go (a decode step waits for this code, not for the GPU)."""

@@ -1,10 +1,13 @@
 """The 8-bit paged cache without a GPU: structs against the header, arguments that are refused before anything is launched."""
 import os
 import subprocess
+import weakref
 
 import pytest
+import torch
 
 from aidotnet.tensors_b200 import native as N
+from aidotnet.tensors_b200.backend import KvCacheFp8
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -118,3 +121,26 @@ def test_append_refuses_a_block_table_between_entries(lib):
     with pytest.raises(N.AidnError) as e:
         N.kv8_append(N.kv8_cache(**{**GOOD, "block_table": 4098}), stream=0, **{**ARGS, "tokens": 0})
     assert "aligned" in str(e.value)
+
+
+class HostBuffer:
+    """What KvCacheFp8 looks at of a GpuBuffer, on the host."""
+
+    def __init__(self, tensor):
+        self.tensor, self.Size, self.dtype = tensor, tensor.numel(), tensor.dtype
+
+
+def test_a_cache_reads_the_buffers_that_it_was_made_with():
+    """Neither a buffer nor a size can be put in another's place, and the memory lives as long as the cache does."""
+    made = [HostBuffer(torch.zeros(2 * 16 * 2 * 64, dtype=torch.uint8)) for _ in range(2)] + [HostBuffer(torch.ones(4)) for _ in range(2)]
+    cache = KvCacheFp8(*made, 16, 2, 64)
+    block = cache._pack(4096, 3)
+    for name in ("keys", "values", "keyScales", "valueScales", "numBlocks", "blockSize", "kvHeads", "headDim"):
+        before = getattr(cache, name)
+        with pytest.raises(AttributeError):
+            setattr(cache, name, before)
+    was = [b.tensor.data_ptr() for b in made]
+    held = weakref.ref(made[0].tensor)
+    made[0].tensor = torch.zeros_like(made[0].tensor)
+    assert held() is not None and cache._pack(4096, 3) == block
+    assert list(N._KV8_CACHE.unpack(block)[:4]) == was
