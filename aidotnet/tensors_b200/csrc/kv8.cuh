@@ -7,8 +7,14 @@ namespace aidn {
 namespace kv8 {
 
 constexpr float kLargestCode = 448.f;
-// Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one: 24 sequences of 2000 to 4096 keys, 8 KV
-// heads of 128, take 54 us with 16 rows, 84 with 32, 112 with 40 and 143 with 64, and the tcgen05 kernel 92, 95, 95 and 96.
+// Rows (queries x query heads of a group) of a sequence up to which the kernel for few queries is the faster one in all of these.  Us of the one and the other, L2
+// flushed, 8 KV heads, with 32, 40, 64 and 96 rows (where the sides meet beyond 32 depends on how many sequences there are, and how long):
+//   heads of 128   24 sequences of 2048 to 4096 keys   99 / 115   128 / 115   160 / 117   222 / 117
+//                  2 sequences of 2048 to 4096 keys    35 / 50     40 / 50     44 / 50     52 / 52
+//                  64 sequences of 350 to 700 keys     66 / 130    87 / 130   105 / 134   140 / 134
+//   heads of 64    24                                  81 / 95    103 / 97    128 / 95    173 / 97
+//                  2                                   31 / 42     35 / 42     40 / 42     46 / 42
+//                  64                                  58 / 103    74 / 103    89 / 103   113 / 105
 constexpr int kFewRows = 32;
 
 constexpr int kLeastExponent = -100, kMostExponent = 119;   // of a scale: 448 * 2^119 is below the largest float

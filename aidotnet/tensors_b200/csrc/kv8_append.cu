@@ -5,7 +5,8 @@
 //   s = max(scale_for(largest new magnitude), the block's scale if it holds tokens already);   code = e4m3(x / s)
 //
 // 3 operations an element: bound by the bytes where there are many tokens and by the chain start -> table -> scale -> store where
-// there are few.  The scale is one for all tokens of a block, so that a block and head is the unit of work: a warp (several for
+// there are few.  (With many tokens by the latency of the loads, in fact: rows are held as the 32-bit floats that they became, and part of them on the
+// stack.)  The scale is one for all tokens of a block, so that a block and head is the unit of work: a warp (several for
 // blocks of more rows than its registers hold) loads the new rows of one block and head once, keeps them rotated in registers
 // across the maximum, and stores codes.  Scales being powers of two, a block's older codes change only when its scale does, and
 // then by an exponent: only then are they read.  8192 tokens of 32 + 2 x 8 heads of 128: 47 us, 4.0 TB/s (a warp a token, one element at a time:
@@ -142,8 +143,10 @@ __device__ __forceinline__ Sequence sequence_of(const Append& p, int b) {
   return {first, first < 0 || n < 0 ? 0 : n};
 }
 
-// CTAs an SM: their loads have to cover one another's latency.  8192 tokens of 32 and 8 heads of 128, pairs: 47 us with four, 50 with three
-// (and 99 with two of eight row groups a warp); 13 prompts of 16 heads of 64, halves, whose loads are twice as many: 38 and 33.
+// CTAs an SM: their loads have to cover one another's latency, and more of them are worth registers that are spilled.  8192 tokens of 32 and 8 heads of
+// 128, pairs: 47.5 us with four (64 registers, 216 bytes of spill stores a thread), 50.6 with three (80, 12 bytes), 59.5 with two (115, none), and 99
+// with two of eight row groups a warp; 13 prompts of 16 heads of 64, halves, whose loads are twice as many: 38 with four, 33.9 with three (80, 96
+// bytes), 36.2 with two (118, none).
 template <Form F>
 constexpr int kMinCtas = F == kHalves ? 3 : 4;
 

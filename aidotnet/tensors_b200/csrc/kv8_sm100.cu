@@ -12,8 +12,8 @@
 // Weights are fp16, 11 bits, lifted so that they stay normal down to 2^-18 of the row's largest product of weight and scale.
 //
 //   warps 0-3, 4-7    softmax of tile 0 and 1, a row a thread: queries into shared memory, S from tensor memory, P back over it
-//                     (16 bits), results.  A row keeps the maximum that it has until sixteen weights sum up to 2^15 (a logit about
-//                     2^8 above it): then it takes the new one, and scales its accumulator
+//                     (16 bits), results.  A row keeps the maxima that it has until sixteen weights sum up to 2^15 (a product of weight
+//                     and scale about 2^8 above them): then it takes the step's, scales its accumulator, and forms the weights again
 //   warps 8-11        keys and values: 16-byte loads through the block table, codes to fp16, into rings of two 128-key tiles
 //   warp 12           tcgen05.mma: S_a = Q_a K^T, O_a += P_a V, for 64 keys at a time
 //
@@ -24,8 +24,8 @@
 // partial result a CTA in the workspace, and the CTA in which it begins a note about it, from which a second launch merges them:
 // 256 rows of up to 148 parts take one CTA 25 to 80 us (measured, merged by the last CTA to arrive), spread over all SMs 4 to 8.
 //
-// 2048 queries at 14336, 32 heads of 128 on 8: 515 us, 1002 TFLOP/s (bound by the softmax warps, 2300 cycles for 64 keys of two tiles; the products
-// take 620); 12 sequences of up to 509 queries, 16 heads of 64 on 4, capped logits: 255 us (4 multiply-adds more a score and a look at its size).
+// 2048 queries at 14336, 32 heads of 128 on 8: 510 us, 1010 TFLOP/s (bound by the softmax warps, 2300 cycles for 64 keys of two tiles, 46 bytes of
+// spill stores and 288 of loads a thread among them; the products take 620); 12 sequences of up to 509 queries, 16 heads of 64 on 4, capped logits: 255 us (4 multiply-adds more a score and a look at its size).
 #include <cstddef>
 #include <type_traits>
 

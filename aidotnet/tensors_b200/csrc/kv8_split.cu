@@ -16,11 +16,11 @@
 //
 // The warps of a "unit" do the same tiles of neighbouring KV heads, whose rows are neighbours in the pool: memory is read in runs
 // of up to 512 bytes (64 sequences of 512 to 4096 keys, 32 KV heads of 128: 228 us, and 265 us where each warp goes through lines of its own;
-// 195 us, 5.9 TB/s, by now).  The lines' tiles are one row, cut into equal shares for the units that are resident whatever the lengths are.  No
+// 197 us, 5.9 TB/s, by now).  The lines' tiles are one row, cut into equal shares for the units that are resident whatever the lengths are.  No
 // warp waits for another one: a line that is cut leaves a partial result a unit in the workspace, and a second launch merges them in their
 // order, so that the result does not depend on which was first.
 //
-// Small calls are one latency after the other (16 sequences of up to 2048 keys, 8 KV heads: 19.5 us for 37 MB, of which the loop over
+// Small calls are one latency after the other (16 sequences of up to 2048 keys, 8 KV heads: 19.4 us for 37 MB, of which the loop over
 // tiles takes 6), and code that runs once is fetched once: what is not the loop stays small, in loops that are not unrolled.
 #include "kv8.cuh"
 #include "mma_sync.cuh"

@@ -349,7 +349,9 @@ AIDN_API int aidn_kv8_append(const aidn_kv8_cache* cache, const aidn_kv8_append_
  * layout of aidn_sdpa_launch.  desc.causal with causal_bottom_right aligns each sequence by its own lengths: query i of n sees
  * key j iff j <= kv_len[b] - n + i.  A query that sees no key gives zeros and a log-sum-exp of -inf.  lse is dense
  * [queries in order, Hq].  desc.mask_kind: masks over (b, h, i, j) run on the any-shape kernel, without query_starts only.
- * A visible NaN code makes its rows NaN; codes past kv_len[b] may be anything.
+ * A visible NaN code, or a scale of NaN, makes its rows NaN; codes past kv_len[b] may be anything.  Logits may have any finite size; with
+ * desc.softcap those of 16-bit results are formed to 2^-20 of the cap.  Weights times value scales are rounded to 16-bit floats (two of them for
+ * fp32 results), relative to the row's largest such product: to 11 bits down to 2^-18 of it, to a part of it below.
  * Workspace: aidn_sdpa_kv8_workspace_bytes() for the partial results of keys that are cut over CTAs; calls without one run uncut.
  * Up to four launches: few queries or many, each with a merge of the parts; a ragged batch may have sequences of both kinds. */
 AIDN_API int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int64_t seq_q, int64_t seq_kv);
