@@ -23,13 +23,42 @@ Differences from the reference methods, all deliberate:
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import native as N
 
 _DTYPE = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+
+
+def _address(buf: Optional["GpuBuffer"]) -> int:
+    return 0 if buf is None else buf.tensor.data_ptr()
+
+
+def rotary_frequencies(rotaryDim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, originalLength: int = 0,
+                       fastTurns: float = 32.0, slowTurns: float = 1.0) -> torch.Tensor:
+    """``CudaBackend.RotaryFrequencies`` on the host: [rotaryDim / 2] radians a position, 64 bits."""
+    if rotaryDim < 2 or rotaryDim % 2 != 0:
+        raise ValueError("rotaryDim must be even and positive")
+    if not base > 0 or not factor > 0:
+        raise ValueError("base and factor must be positive")
+    i = torch.arange(rotaryDim // 2, dtype=torch.float64)
+    if scaling == "base":
+        if rotaryDim == 2:
+            raise ValueError("a raised base changes nothing for a single pair")
+        base = base * factor ** (rotaryDim / (rotaryDim - 2))
+    f = torch.tensor(base, dtype=torch.float64) ** (-2 * i / rotaryDim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        if originalLength <= 0 or not fastTurns > slowTurns:
+            raise ValueError("scaling by parts needs originalLength > 0 and fastTurns > slowTurns")
+        keep = ((originalLength * f / (2 * math.pi) - slowTurns) / (fastTurns - slowTurns)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    elif scaling not in ("none", "base"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return f
 
 
 class GpuBuffer:
@@ -555,6 +584,219 @@ class CudaBackend:
         if status != N.OK:
             raise N.AidnError(status, N.last_error())
         self.launch_count += h.last_launch_count
+
+    # -- rotary positions, linear attention (extensions with no reference counterpart) --------------------------------------
+    def RotaryFrequencies(self, rotaryDim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                          originalLength: int = 0, fastTurns: float = 32.0, slowTurns: float = 1.0) -> GpuBuffer:
+        """The frequencies that ``RotaryEmbedding`` takes: base^(-2i / rotaryDim) radians a position for pair i, in 64 bits.  For contexts
+        ``factor`` times as long as those trained on: "linear" divides them all by ``factor``; "base" raises the base until the slowest
+        pair is ``factor`` times slower; "parts" divides those of pairs that make fewer than ``slowTurns`` turns within
+        ``originalLength`` positions, leaves those that make more than ``fastTurns``, and goes over linearly in between."""
+        return GpuBuffer(rotary_frequencies(rotaryDim, base, scaling, factor, originalLength, fastTurns, slowTurns).to(self._torch_device))
+
+    def RotaryEmbedding(self, query: GpuBuffer, queryOut: GpuBuffer, key: Optional[GpuBuffer], keyOut: Optional[GpuBuffer],
+                        frequencies: GpuBuffer, tokens: int, heads: int, kvHeads: int, headDim: int, seqLen: int = 0, startPosition: int = 0,
+                        positions: Optional[GpuBuffer] = None, interleaved: bool = True, amplitude: float = 1.0,
+                        queryStride: Optional[Sequence[int]] = None, keyStride: Optional[Sequence[int]] = None) -> None:
+        """Turns the first 2 * frequencies.Size elements of every head of ``query`` [tokens, heads, headDim] and, if given, ``key``
+        [tokens, kvHeads, headDim] by their token's position: in pairs (2i, 2i+1) or, not ``interleaved``, (i, i + half).  Token t is
+        at ``positions``[t] (int32 or int64), without them at startPosition + t % seqLen (0: tokens).  The turned elements are multiplied by
+        ``amplitude``, the others copied.  The outputs are dense, or the inputs themselves.  ``queryStride`` / ``keyStride``: elements
+        from a token to the next and from a head to the next, for rows that hold more than these heads (a packed projection,
+        whose queries and keys are heads + kvHeads heads side by side)."""
+        self._rotary("RotaryEmbedding", False, query, queryOut, key, keyOut, frequencies, tokens, heads, kvHeads, headDim, seqLen, startPosition,
+                     positions, interleaved, amplitude, queryStride, keyStride)
+
+    def RotaryEmbeddingBackward(self, gradQueryOut: GpuBuffer, gradQuery: GpuBuffer, gradKeyOut: Optional[GpuBuffer],
+                                gradKey: Optional[GpuBuffer], frequencies: GpuBuffer, tokens: int, heads: int, kvHeads: int, headDim: int,
+                                seqLen: int = 0, startPosition: int = 0, positions: Optional[GpuBuffer] = None, interleaved: bool = True,
+                                amplitude: float = 1.0, queryStride: Optional[Sequence[int]] = None,
+                                keyStride: Optional[Sequence[int]] = None) -> None:
+        """The gradients of ``RotaryEmbedding``'s inputs from those of its outputs: the same turn backwards."""
+        self._rotary("RotaryEmbeddingBackward", True, gradQueryOut, gradQuery, gradKeyOut, gradKey, frequencies, tokens, heads, kvHeads, headDim,
+                     seqLen, startPosition, positions, interleaved, amplitude, queryStride, keyStride)
+
+    def _rotary(self, op, inverse, query, queryOut, key, keyOut, frequencies, tokens, heads, kvHeads, headDim, seqLen, startPosition, positions,
+                interleaved, amplitude, queryStride, keyStride) -> None:
+        if tokens < 0 or heads <= 0 or kvHeads < 0 or headDim <= 0:
+            raise ValueError(f"{op}: tokens must be >= 0, heads and headDim positive, kvHeads >= 0")
+        if (key is None) != (keyOut is None) or (key is None) != (kvHeads == 0):
+            raise ValueError(f"{op}: key, keyOut and kvHeads > 0 come together")
+        f = frequencies.tensor
+        if f.dtype != torch.float64:
+            raise ValueError(f"{op}: frequencies must be a buffer of 64-bit floats")
+        x, dtype, spans, pointers = query.tensor, query.tensor.dtype, [], []
+        for name, src, dst, h, stride in (("query", query, queryOut, heads, queryStride), ("key", key, keyOut, kvHeads, keyStride)):
+            if src is None:
+                spans.append((0, 0, 0, 0))
+                pointers += [0, 0]
+                continue
+            row, step = (h * headDim, headDim) if stride is None else stride
+            if row < 0 or step < 0:
+                raise ValueError(f"{op}: a stride of {name} is negative")
+            reach = (tokens - 1) * row + (h - 1) * step + headDim if tokens > 0 else 0
+            at, to = src.tensor, dst.tensor
+            same = at.data_ptr() == to.data_ptr()
+            if at.dtype != dtype or to.dtype != dtype:
+                raise ValueError(f"{op}: queries and keys, in and out, must share a dtype")
+            if at.numel() < reach or (not same and to.numel() < tokens * h * headDim):
+                raise ValueError(f"{op}: a buffer of {name} is smaller than [tokens, heads, headDim]")
+            spans.append((row, step) + ((row, step) if same else (h * headDim, headDim)))
+            pointers += [at.data_ptr(), to.data_ptr()]
+        at, width = 0, 4
+        if positions is not None:
+            if positions.tensor.dtype not in (torch.int32, torch.int64) or positions.tensor.numel() < tokens:
+                raise ValueError(f"{op}: positions must be int32 or int64 [tokens]")
+            at, width = positions.tensor.data_ptr(), positions.tensor.element_size()
+        (qr, qh, qor, qoh), (kr, kh, kor, koh) = spans
+        status = N._rotary_packed(N._ROTARY_ARGS.pack(
+            *pointers, qr, qh, qor, qoh, kr, kh, kor, koh, f.data_ptr(), at, tokens, seqLen, startPosition, heads, kvHeads, headDim,
+            2 * f.numel(), _DTYPE[dtype], N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES, width, inverse, amplitude, 0), self._raw_stream)
+        if status != N.OK:
+            raise N.AidnError(status, N.last_error())
+        if tokens > 0:
+            self.launch_count += 1
+
+    def _linear_checks(self, op, tensors, batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts, decay, states,
+                       stateSlots):
+        """``tensors``: (name, buffer, heads, size).  Returns the number of packed rows, of states, and the strides by (heads, size)."""
+        if batch <= 0 or heads <= 0 or kvHeads <= 0 or seqLen <= 0 or keyDim <= 0 or valueDim <= 0:
+            raise ValueError(f"{op}: dimensions must be positive")
+        if heads % kvHeads != 0:
+            raise ValueError(f"{op}: heads must be an integer multiple of kvHeads (heads={heads}, kvHeads={kvHeads})")
+        if lengths is not None and tokenStarts is not None:
+            raise ValueError(f"{op}: lengths and tokenStarts exclude one another")
+        for name, buf, least in (("lengths", lengths, batch), ("tokenStarts", tokenStarts, batch + 1), ("stateSlots", stateSlots, batch)):
+            if buf is not None and (buf.tensor.dtype != torch.int32 or buf.tensor.numel() < least):
+                raise ValueError(f"{op}: {name} must be int32 with {least} entries")
+        if decay is not None and (decay.tensor.dtype != torch.float32 or decay.tensor.numel() < heads):
+            raise ValueError(f"{op}: decay must hold an fp32 value for each head")
+        dtype = tensors[0][1].tensor.dtype
+        if dtype not in _DTYPE:
+            raise ValueError(f"{op}: {dtype} is not served")
+        tokens = 0 if tokenStarts is None else tensors[0][1].tensor.numel() // (tensors[0][2] * tensors[0][3])
+        rows = batch * seqLen if tokenStarts is None else tokens
+        for name, buf, h, size in tensors:
+            if buf.tensor.dtype != dtype:
+                raise ValueError(f"{op}: {name} must have the dtype of the other tensors")
+            if buf.tensor.numel() < rows * h * size:
+                raise ValueError(f"{op}: {name} is smaller than the requested dimensions")
+        per, slots = heads * keyDim * valueDim, batch
+        given = [s for _, s in states if s is not None]
+        if stateSlots is not None and given:
+            slots = min(s.tensor.numel() for s in given) // per
+        for name, buf in states:
+            if buf is not None and (buf.tensor.dtype != torch.float32 or buf.tensor.numel() < max(slots, 1) * per):
+                raise ValueError(f"{op}: {name} must hold fp32 states [.., heads, keyDim, valueDim]")
+
+        def stride(h, size):
+            if tokenStarts is not None or not tokenMajor:
+                return N._NO_STRIDE
+            return (seqLen * h * size, size, h * size)
+
+        return tokens, slots, _DTYPE[dtype], stride
+
+    def _linear_workspace(self, block, optional):
+        """(stream, address, bytes) of a call's workspace."""
+        need = N.linear_workspace_bytes(block)
+        stream = self._raw_stream
+        if need <= 0:
+            return stream, 0, 0
+        held = self._scratch.get(0) if stream == 0 else None   # (stream 0 is never captured)
+        if held is not None and held.numel() >= need:
+            return stream, held.data_ptr(), held.numel()
+        ws, ws_bytes = self._workspace(need, self.stream, optional=optional)
+        return stream, ws or 0, ws_bytes
+
+    def LinearAttention(self, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, output: GpuBuffer, decay: Optional[GpuBuffer], batch: int,
+                        heads: int, kvHeads: int, seqLen: int, keyDim: int, valueDim: int, scale: float = 0.0, tokenMajor: bool = False,
+                        lengths: Optional[GpuBuffer] = None, tokenStarts: Optional[GpuBuffer] = None,
+                        initialStates: Optional[GpuBuffer] = None, finalStates: Optional[GpuBuffer] = None,
+                        stateSlots: Optional[GpuBuffer] = None) -> None:
+        """Linear attention of whole sequences: S_t = exp(decay) S_(t-1) + k_t v_t^T, o_t = scale * q_t S_t (scale 0: 1/sqrt(keyDim)) with
+        the head's log ``decay`` [heads] fp32, at most 0 (None: no decay).  ``query`` [batch, heads, seqLen, keyDim], ``key`` and
+        ``value`` [batch, kvHeads, seqLen, ..], ``output`` [batch, heads, seqLen, valueDim]; ``tokenMajor``: [batch, seqLen, heads, ..].
+        ``lengths`` int32 [batch]: the rows behind them are padding, and zeros in ``output``.  ``tokenStarts`` int32 [batch + 1]: packed
+        rows [tokens, heads, ..] instead, sequence b's from tokenStarts[b] on, at most seqLen of them; rows of no sequence are left.
+        Sequence b begins with state stateSlots[b] (or b) of ``initialStates`` [.., heads, keyDim, valueDim] fp32 (None or a negative
+        slot: zeros) and leaves its last in ``finalStates``, which may be the same buffer.  A slot that is not there, or an earlier
+        sequence's, gives NaN and touches no state."""
+        op = "LinearAttention"
+        tokens, slots, dtype, stride = self._linear_checks(
+            op, (("query", query, heads, keyDim), ("key", key, kvHeads, keyDim), ("value", value, kvHeads, valueDim),
+                 ("output", output, heads, valueDim)), batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts, decay,
+            (("initialStates", initialStates), ("finalStates", finalStates)), stateSlots)
+        args = dict(q=query.tensor.data_ptr(), k=key.tensor.data_ptr(), v=value.tensor.data_ptr(), out=output.tensor.data_ptr(), batch=batch,
+                    heads=heads, kv_heads=kvHeads, seq_len=seqLen, key_dim=keyDim, value_dim=valueDim, dtype=dtype,
+                    decay=_address(decay), lengths=_address(lengths), token_starts=_address(tokenStarts), tokens=tokens,
+                    initial_state=_address(initialStates), final_state=_address(finalStates), state_slots=_address(stateSlots), num_slots=slots,
+                    q_stride=stride(heads, keyDim), k_stride=stride(kvHeads, keyDim), v_stride=stride(kvHeads, valueDim),
+                    o_stride=stride(heads, valueDim), scale=float(scale), path=self._path)
+        stream, ws, ws_bytes = self._linear_workspace(N.linear_block(**args), optional=True)
+        N.linear_attention(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), stream)
+        self.launch_count += 1
+
+    def LinearAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, gradQuery: GpuBuffer,
+                                gradKey: GpuBuffer, gradValue: GpuBuffer, decay: Optional[GpuBuffer], batch: int, heads: int, kvHeads: int,
+                                seqLen: int, keyDim: int, valueDim: int, scale: float = 0.0, tokenMajor: bool = False,
+                                lengths: Optional[GpuBuffer] = None, tokenStarts: Optional[GpuBuffer] = None,
+                                initialStates: Optional[GpuBuffer] = None, gradFinalStates: Optional[GpuBuffer] = None,
+                                gradInitialStates: Optional[GpuBuffer] = None) -> None:
+        """The gradients of ``LinearAttention``'s query, key, value and initial states (all by sequence, [batch, heads, keyDim, valueDim]) from
+        those of its output and of its final states.  Gradients have the inputs' dtype and layout; those of shared heads are summed in
+        fp32.  decay has none."""
+        op = "LinearAttentionBackward"
+        tokens, _, dtype, stride = self._linear_checks(
+            op, (("query", query, heads, keyDim), ("key", key, kvHeads, keyDim), ("value", value, kvHeads, valueDim),
+                 ("gradOutput", gradOutput, heads, valueDim), ("gradQuery", gradQuery, heads, keyDim), ("gradKey", gradKey, kvHeads, keyDim),
+                 ("gradValue", gradValue, kvHeads, valueDim)), batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts,
+            decay, (("initialStates", initialStates), ("gradFinalStates", gradFinalStates), ("gradInitialStates", gradInitialStates)), None)
+        qs, ks, os, vs = stride(heads, keyDim), stride(kvHeads, keyDim), stride(heads, valueDim), stride(kvHeads, valueDim)
+        args = dict(q=query.tensor.data_ptr(), k=key.tensor.data_ptr(), v=value.tensor.data_ptr(), batch=batch, heads=heads, kv_heads=kvHeads,
+                    seq_len=seqLen, key_dim=keyDim, value_dim=valueDim, dtype=dtype, decay=_address(decay), lengths=_address(lengths),
+                    token_starts=_address(tokenStarts), tokens=tokens, initial_state=_address(initialStates), q_stride=qs, k_stride=ks,
+                    v_stride=vs, scale=float(scale), path=self._path)
+        grads = dict(dout=gradOutput.tensor.data_ptr(), dq=gradQuery.tensor.data_ptr(), dk=gradKey.tensor.data_ptr(),
+                     dv=gradValue.tensor.data_ptr(), d_final_state=_address(gradFinalStates), d_initial_state=_address(gradInitialStates),
+                     do_stride=os, dq_stride=qs, dk_stride=ks, dv_stride=vs)
+        stream, ws, ws_bytes = self._linear_workspace(N.linear_bwd_block(N.linear_block(**args), **grads), optional=False)
+        N.linear_attention_backward(N.linear_bwd_block(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), **grads), stream)
+        self.launch_count += 1
+
+    def LinearAttentionStep(self, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, output: GpuBuffer, states: GpuBuffer,
+                            decay: Optional[GpuBuffer], batch: int, heads: int, kvHeads: int, keyDim: int, valueDim: int, scale: float = 0.0,
+                            stateSlots: Optional[GpuBuffer] = None) -> None:
+        """One token of each of ``batch`` sequences: ``query`` [batch, heads, keyDim], ``key`` and ``value`` [batch, kvHeads, ..], ``output``
+        [batch, heads, valueDim].  State stateSlots[b] (or b) of ``states`` [.., heads, keyDim, valueDim] fp32 is updated in place.  A
+        negative slot is a row of padding: zeros, and no state is touched.  A slot that is not there, or an earlier row's, gives NaN and
+        touches no state."""
+        op = "LinearAttentionStep"
+        if batch < 0 or heads <= 0 or kvHeads <= 0 or keyDim <= 0 or valueDim <= 0:
+            raise ValueError(f"{op}: batch must be >= 0, the other dimensions positive")
+        if heads % kvHeads != 0:
+            raise ValueError(f"{op}: heads must be an integer multiple of kvHeads (heads={heads}, kvHeads={kvHeads})")
+        q, k, v, o, s = query.tensor, key.tensor, value.tensor, output.tensor, states.tensor
+        dtype = q.dtype
+        if k.dtype != dtype or v.dtype != dtype or o.dtype != dtype:
+            raise ValueError(f"{op}: query, key, value and output must share a dtype")
+        if (q.numel() < batch * heads * keyDim or k.numel() < batch * kvHeads * keyDim or v.numel() < batch * kvHeads * valueDim or
+                o.numel() < batch * heads * valueDim):
+            raise ValueError(f"{op}: a buffer is smaller than the requested dimensions")
+        slots = s.numel() // (heads * keyDim * valueDim)
+        if s.dtype != torch.float32 or slots < (batch if stateSlots is None else 1):
+            raise ValueError(f"{op}: states must hold fp32 states [.., heads, keyDim, valueDim]")
+        if stateSlots is not None and (stateSlots.tensor.dtype != torch.int32 or stateSlots.tensor.numel() < batch):
+            raise ValueError(f"{op}: stateSlots must be int32 [batch]")
+        if decay is not None and (decay.tensor.dtype != torch.float32 or decay.tensor.numel() < heads):
+            raise ValueError(f"{op}: decay must hold an fp32 value for each head")
+        status = N._linear_step_packed(N._LINEAR_STEP_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), s.data_ptr(), 0 if decay is None else decay.tensor.data_ptr(),
+            0 if stateSlots is None else stateSlots.tensor.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, batch, heads, kvHeads, keyDim, valueDim,
+            _DTYPE[dtype], slots, float(scale)), self._raw_stream)
+        if status != N.OK:
+            raise N.AidnError(status, N.last_error())
+        if batch > 0:
+            self.launch_count += 1
 
     def FlashAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer,
                                output: GpuBuffer, softmaxStats: GpuBuffer, gradQuery: GpuBuffer, gradKey: GpuBuffer,

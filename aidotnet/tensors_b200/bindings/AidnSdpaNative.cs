@@ -115,6 +115,60 @@ namespace AiDotNet.Tensors.Engines.DirectGpu.CUDA
         public long cache_capacity, max_position;
     }
 
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnRotaryArgs
+    {
+        public IntPtr query, query_out, key, key_out;
+        public fixed long query_stride[2];
+        public fixed long query_out_stride[2];
+        public fixed long key_stride[2];
+        public fixed long key_out_stride[2];
+        public IntPtr frequencies, positions;
+        public long tokens, seq_len, start_position;
+        public int heads, kv_heads, head_dim, rotary_dim, dtype, layout, position_bytes, inverse;
+        public float amplitude;
+        public int reserved;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnLinearArgs
+    {
+        public IntPtr q, k, v, @out, decay, lengths, token_starts, initial_state, final_state, state_slots;
+        public fixed long q_stride[3];
+        public fixed long k_stride[3];
+        public fixed long v_stride[3];
+        public fixed long o_stride[3];
+        public long tokens, seq_len;
+        public int batch, heads, kv_heads, key_dim, value_dim, dtype, num_slots, path;
+        public float scale;
+        public int reserved;
+        public IntPtr workspace;
+        public long workspace_bytes;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnLinearBwdArgs
+    {
+        public AidnLinearArgs fwd;
+        public IntPtr dout, d_final_state, dq, dk, dv, d_initial_state;
+        public fixed long do_stride[3];
+        public fixed long dq_stride[3];
+        public fixed long dk_stride[3];
+        public fixed long dv_stride[3];
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal unsafe struct AidnLinearStepArgs
+    {
+        public IntPtr q, k, v, @out, states, decay, state_slots;
+        public fixed long q_stride[2];
+        public fixed long k_stride[2];
+        public fixed long v_stride[2];
+        public fixed long o_stride[2];
+        public int batch, heads, kv_heads, key_dim, value_dim, dtype, num_slots;
+        public float scale;
+    }
+
     internal static class AidnSdpaNative
     {
         private const string Lib = "aidotnet_sdpa_sm100";
@@ -146,6 +200,12 @@ namespace AiDotNet.Tensors.Engines.DirectGpu.CUDA
         [DllImport(Lib)] public static extern int aidn_kv8_append(ref AidnKv8Cache cache, ref AidnKv8AppendArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_sdpa_kv8_workspace_bytes(IntPtr handle, long batch, long seqQ, long seqKv);
         [DllImport(Lib)] public static extern int aidn_sdpa_launch_kv8(IntPtr handle, ref AidnSdpaArgs args, ref AidnKv8Cache cache, IntPtr queryStarts, long queries, IntPtr cuStream);
+        [DllImport(Lib)] public static extern int aidn_rotary(ref AidnRotaryArgs args, IntPtr cuStream);
+        [DllImport(Lib)] public static extern long aidn_linear_attention_workspace_bytes(ref AidnLinearArgs args);
+        [DllImport(Lib)] public static extern int aidn_linear_attention(ref AidnLinearArgs args, IntPtr cuStream);
+        [DllImport(Lib)] public static extern long aidn_linear_attention_backward_workspace_bytes(ref AidnLinearBwdArgs args);
+        [DllImport(Lib)] public static extern int aidn_linear_attention_backward(ref AidnLinearBwdArgs args, IntPtr cuStream);
+        [DllImport(Lib)] public static extern int aidn_linear_attention_step(ref AidnLinearStepArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_sdpa_backward_workspace_bytes(IntPtr handle, long batch, long seqQ);
         [DllImport(Lib)] public static extern int aidn_sdpa_backward(IntPtr handle, ref AidnSdpaBwdArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_mha_workspace_bytes(IntPtr handle, long batch, long seq, int inputDtype, int weightDtype);

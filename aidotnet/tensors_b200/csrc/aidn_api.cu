@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "kv8.cuh"
+#include "linear.cuh"
 #include "../../../include/aidn_sdpa_debug.h"
 
 namespace {
@@ -999,6 +1000,311 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
   if (e != cudaSuccess) return fail_cuda(e, "launch_kv8");
   h->last_launches = launches;
   return post_launch_check(stream, "aidn_sdpa_launch_kv8", h->status_dev);
+}
+
+// ---- rotary positions, linear attention ------------------------------------------------------------------------------
+namespace {
+// What a device is, looked up once (handle-less entry points have nowhere else to keep it; racing threads write the same values).
+int device_facts(const char* op, int* sms) {
+  static int g_sms[64] = {0}, g_ok[64] = {0};
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail_cuda(e, op);
+  }
+  if (dev < 0 || dev >= 64) return fail(AIDN_EUNSUPPORTED, "%s: device ordinal %d", op, dev);
+  if (g_sms[dev] == 0) {
+    int n = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return fail_cuda(e, op);
+    g_ok[dev] = aidn_sdpa_device_supported(dev);
+    g_sms[dev] = n;
+  }
+  if (!g_ok[dev]) return fail(AIDN_EUNSUPPORTED, "%s: device %d is not compute capability 10.x", op, dev);
+  *sms = g_sms[dev];
+  return AIDN_OK;
+}
+
+// Element strides of a tensor: given, or dense.
+bool take_strides(int n, const int64_t* given, const int64_t* dense, int64_t* to) {
+  bool zero = true;
+  for (int i = 0; i < n; ++i) zero = zero && given[i] == 0;
+  for (int i = 0; i < n; ++i) {
+    to[i] = zero ? dense[i] : given[i];
+    if (to[i] < 0) return false;
+  }
+  return true;
+}
+
+// The sizes and pointers that a forward and a backward call share.
+int linear_common(const char* op, const aidn_linear_args& a, aidn::lin::Params& p) {
+  if (a.batch <= 0 || a.heads <= 0 || a.kv_heads <= 0) return fail(AIDN_EINVAL, "%s: batch, heads and kv_heads must be positive", op);
+  if (a.batch > 65535 || a.heads > 65535) return fail(AIDN_EINVAL, "%s: batch and heads must be at most 65535", op);
+  if (a.heads % a.kv_heads != 0) return fail(AIDN_EINVAL, "%s: kv_heads (%d) must divide heads (%d)", op, a.kv_heads, a.heads);
+  if (a.key_dim <= 0 || a.key_dim > 256 || a.key_dim % 8 != 0 || a.value_dim <= 0 || a.value_dim > 256 || a.value_dim % 8 != 0)
+    return fail(AIDN_EINVAL, "%s: key_dim (%d) and value_dim (%d) must be multiples of 8 in [8, 256]", op, a.key_dim, a.value_dim);
+  if (a.dtype < AIDN_F32 || a.dtype > AIDN_BF16) return fail(AIDN_EINVAL, "%s: unknown dtype %d", op, a.dtype);
+  if (a.path != AIDN_PATH_AUTO && a.path != AIDN_PATH_GENERIC) return fail(AIDN_EINVAL, "%s: path must be AUTO or GENERIC", op);
+  if (a.seq_len <= 0 || a.seq_len > 0x7fffffffll) return fail(AIDN_EINVAL, "%s: seq_len must be in [1, 2^31-1]", op);
+  if (!(a.scale >= 0.f) || std::isinf(a.scale)) return fail(AIDN_EINVAL, "%s: scale must be finite and >= 0", op);
+  if (a.token_starts && a.lengths) return fail(AIDN_EINVAL, "%s: lengths and token_starts exclude one another", op);
+  if (a.token_starts && (a.tokens < 0 || a.tokens > 0x7fffffffll)) return fail(AIDN_EINVAL, "%s: token_starts needs the number of tokens, at most 2^31-1", op);
+  if ((uintptr_t)a.decay % 4 != 0 || (uintptr_t)a.lengths % 4 != 0 || (uintptr_t)a.token_starts % 4 != 0 || (uintptr_t)a.state_slots % 4 != 0)
+    return fail(AIDN_EINVAL, "%s: decay, lengths, token_starts or state_slots is not aligned to its elements", op);
+  if (a.state_slots && a.num_slots <= 0) return fail(AIDN_EINVAL, "%s: state_slots needs num_slots > 0", op);
+  std::memset(&p, 0, sizeof(p));
+  p.decay = a.decay;
+  p.lengths = a.lengths;
+  p.starts = a.token_starts;
+  p.slots = a.state_slots;
+  p.tokens = a.tokens;
+  p.seq_len = a.seq_len;
+  p.batch = a.batch;
+  p.heads = a.heads;
+  p.num_slots = a.state_slots ? a.num_slots : a.batch;
+  p.dtype = a.dtype;
+  p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt((float)a.key_dim);
+  return AIDN_OK;
+}
+
+// One tensor of such a call: its pointer's alignment and its strides.
+bool linear_tensor(const aidn_linear_args& a, const void* ptr, const int64_t* given, int64_t heads, int64_t size, int64_t* to) {
+  const int64_t packed[3] = {0, size, heads * size}, dense[3] = {heads * a.seq_len * size, a.seq_len * size, size};
+  return (uintptr_t)ptr % elem_size(a.dtype) == 0 && (a.token_starts ? take_strides(3, given, packed, to) : take_strides(3, given, dense, to));
+}
+
+bool no_rows(const aidn_linear_args& a) { return a.token_starts && a.tokens == 0; }
+}  // namespace
+
+int aidn_rotary(const aidn_rotary_args* a, void* cu_stream) {
+  g_err[0] = 0;
+  if (!a) return fail(AIDN_EINVAL, "rotary: null argument");
+  if (a->tokens < 0) return fail(AIDN_EINVAL, "rotary: tokens must be >= 0");
+  if (a->heads <= 0 || a->heads > 65535 || a->kv_heads < 0 || a->kv_heads > 65535) return fail(AIDN_EINVAL, "rotary: heads must be in [1, 65535], kv_heads in [0, 65535]");
+  if (a->head_dim <= 0 || a->head_dim > 256 || a->head_dim % 8 != 0) return fail(AIDN_EINVAL, "rotary: head_dim %d is not a multiple of 8 in [8, 256]", a->head_dim);
+  if (a->rotary_dim < 2 || a->rotary_dim > a->head_dim || a->rotary_dim % 2 != 0) return fail(AIDN_EINVAL, "rotary: rotary_dim %d is not even and in [2, head_dim]", a->rotary_dim);
+  if (a->dtype < AIDN_F32 || a->dtype > AIDN_BF16) return fail(AIDN_EINVAL, "rotary: unknown dtype %d", a->dtype);
+  if (a->layout != AIDN_ROPE_INTERLEAVED && a->layout != AIDN_ROPE_HALVES) return fail(AIDN_EINVAL, "rotary: unknown layout %d", a->layout);
+  if (a->positions && a->position_bytes != 4 && a->position_bytes != 8) return fail(AIDN_EINVAL, "rotary: position_bytes must be 4 or 8");
+  if (!a->positions && (a->seq_len < 0 || a->start_position < 0)) return fail(AIDN_EINVAL, "rotary: seq_len and start_position must be >= 0");
+  if (std::isnan(a->amplitude) || std::isinf(a->amplitude)) return fail(AIDN_EINVAL, "rotary: amplitude must be finite");
+  if (a->tokens == 0) return AIDN_OK;
+  if (!a->query || !a->query_out || !a->frequencies) return fail(AIDN_EINVAL, "rotary: null buffer");
+  if ((a->kv_heads > 0) != (a->key != nullptr) || (a->key != nullptr) != (a->key_out != nullptr))
+    return fail(AIDN_EINVAL, "rotary: key, key_out and kv_heads > 0 come together");
+  const size_t esz = elem_size(a->dtype);
+  if ((uintptr_t)a->query % esz || (uintptr_t)a->query_out % esz || (uintptr_t)a->key % esz || (uintptr_t)a->key_out % esz ||
+      (uintptr_t)a->frequencies % 8 || (a->positions && (uintptr_t)a->positions % a->position_bytes))
+    return fail(AIDN_EINVAL, "rotary: a buffer is not aligned to its elements");
+  aidn::lin::Rotary p;
+  std::memset(&p, 0, sizeof(p));
+  p.x[0] = a->query; p.y[0] = a->query_out; p.x[1] = a->key; p.y[1] = a->key_out;
+  p.heads[0] = a->heads; p.heads[1] = a->kv_heads;
+  const int64_t* in[2] = {a->query_stride, a->key_stride};
+  const int64_t* out[2] = {a->query_out_stride, a->key_out_stride};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t dense[2] = {(int64_t)p.heads[i] * a->head_dim, a->head_dim};
+    if (!take_strides(2, in[i], dense, p.xs[i]) || !take_strides(2, out[i], dense, p.ys[i])) return fail(AIDN_EINVAL, "rotary: negative stride");
+    if (p.heads[i] > 0 && p.x[i] == p.y[i] && (p.xs[i][0] != p.ys[i][0] || p.xs[i][1] != p.ys[i][1]))
+      return fail(AIDN_EINVAL, "rotary: in place needs the same strides in and out");
+  }
+  p.frequencies = a->frequencies;
+  p.positions = a->positions;
+  p.tokens = a->tokens;
+  p.seq_len = a->seq_len > 0 ? a->seq_len : a->tokens;
+  p.start = a->start_position;
+  p.head_dim = a->head_dim;
+  p.rotary_dim = a->rotary_dim;
+  p.dtype = a->dtype;
+  p.halves = a->layout == AIDN_ROPE_HALVES;
+  p.wide_positions = a->position_bytes == 8;
+  p.amplitude = a->amplitude != 0.f ? a->amplitude : 1.f;
+  p.sign = a->inverse ? -1.f : 1.f;
+  int sms = 0;
+  const int rc = device_facts("rotary", &sms);
+  if (rc != AIDN_OK) return rc;
+  const cudaError_t e = aidn::lin::launch_rotary(p, (cudaStream_t)cu_stream);
+  if (e != cudaSuccess) return fail_cuda(e, "rotary");
+  return post_launch_check((cudaStream_t)cu_stream, "aidn_rotary", nullptr);
+}
+
+int64_t aidn_linear_attention_workspace_bytes(const aidn_linear_args* a) {
+  g_err[0] = 0;
+  aidn::lin::Params p;
+  if (!a) return fail(AIDN_EINVAL, "linear_attention_workspace_bytes: null argument"), -1;
+  if (linear_common("linear_attention_workspace_bytes", *a, p) != AIDN_OK) return -1;
+  return 0;
+}
+
+int aidn_linear_attention(const aidn_linear_args* a, void* cu_stream) {
+  g_err[0] = 0;
+  if (!a) return fail(AIDN_EINVAL, "linear_attention: null argument");
+  aidn::lin::Params p;
+  int rc = linear_common("linear_attention", *a, p);
+  if (rc != AIDN_OK) return rc;
+  if (!no_rows(*a) && (!a->q || !a->k || !a->v || !a->out)) return fail(AIDN_EINVAL, "linear_attention: null tensor pointer");
+  if ((uintptr_t)a->initial_state % 16 != 0 || (uintptr_t)a->final_state % 16 != 0) return fail(AIDN_EINVAL, "linear_attention: states must be 16-byte aligned");
+  if ((uintptr_t)a->workspace % 256 != 0) return fail(AIDN_EINVAL, "linear_attention: workspace must be 256-byte aligned");
+  aidn::lin::Scan& s = p.scan[0];
+  if (!linear_tensor(*a, a->q, a->q_stride, a->heads, a->key_dim, s.as) || !linear_tensor(*a, a->k, a->k_stride, a->kv_heads, a->key_dim, s.bs) ||
+      !linear_tensor(*a, a->v, a->v_stride, a->kv_heads, a->value_dim, s.cs) || !linear_tensor(*a, a->out, a->o_stride, a->heads, a->value_dim, s.ys))
+    return fail(AIDN_EINVAL, "linear_attention: a tensor is not aligned to its elements, or a stride is negative");
+  p.scans = 1;
+  s.a = a->q; s.b = a->k; s.c = a->v; s.y = a->out;
+  s.a_group = 1;
+  s.b_group = s.c_group = a->heads / a->kv_heads;
+  s.d1 = a->key_dim; s.d2 = a->value_dim;
+  s.lag = 1;
+  s.row_scale = p.scale;
+  s.key_scale = 1.f;
+  s.x_first = a->initial_state;
+  s.x_last = a->final_state;
+  int sms = 0;
+  rc = device_facts("linear_attention", &sms);
+  if (rc != AIDN_OK) return rc;
+  int launches = 0;
+  const cudaError_t e = aidn::lin::launch_scan_generic(p, (cudaStream_t)cu_stream, &launches);
+  if (e != cudaSuccess) return fail_cuda(e, "linear_attention");
+  return post_launch_check((cudaStream_t)cu_stream, "aidn_linear_attention", nullptr);
+}
+
+// Bytes of the partial sums of dk and dv for shared heads.
+static int64_t linear_partial_bytes(const aidn_linear_args& a, int64_t size) {
+  const int64_t rows = a.token_starts ? a.tokens : a.batch * a.seq_len;
+  return a.heads == a.kv_heads ? 0 : align_up(rows * a.heads * size * 4, 256);
+}
+
+int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linear_bwd_args* a) {
+  g_err[0] = 0;
+  aidn::lin::Params p;
+  if (!a) return fail(AIDN_EINVAL, "linear_attention_backward_workspace_bytes: null argument"), -1;
+  if (linear_common("linear_attention_backward_workspace_bytes", a->fwd, p) != AIDN_OK) return -1;
+  return linear_partial_bytes(a->fwd, a->fwd.key_dim) + linear_partial_bytes(a->fwd, a->fwd.value_dim);
+}
+
+int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_stream) {
+  g_err[0] = 0;
+  if (!a) return fail(AIDN_EINVAL, "linear_attention_backward: null argument");
+  const aidn_linear_args& f = a->fwd;
+  aidn::lin::Params p;
+  int rc = linear_common("linear_attention_backward", f, p);
+  if (rc != AIDN_OK) return rc;
+  if (f.state_slots) return fail(AIDN_EUNSUPPORTED, "linear_attention_backward: states are by sequence, state_slots must be NULL");
+  if (!no_rows(f) && (!f.q || !f.k || !f.v || !a->dout || !a->dq || !a->dk || !a->dv)) return fail(AIDN_EINVAL, "linear_attention_backward: null tensor pointer");
+  if ((uintptr_t)f.initial_state % 16 != 0 || (uintptr_t)a->d_final_state % 16 != 0 || (uintptr_t)a->d_initial_state % 16 != 0)
+    return fail(AIDN_EINVAL, "linear_attention_backward: states must be 16-byte aligned");
+  if ((uintptr_t)f.workspace % 256 != 0) return fail(AIDN_EINVAL, "linear_attention_backward: workspace must be 256-byte aligned");
+  const int group = f.heads / f.kv_heads;
+  const int64_t dk = f.key_dim, dv = f.value_dim, part[2] = {linear_partial_bytes(f, dk), linear_partial_bytes(f, dv)};
+  int64_t qs[3], ks[3], vs[3], dos[3], dqs[3], dks[3], dvs[3];
+  if (!linear_tensor(f, f.q, f.q_stride, f.heads, dk, qs) || !linear_tensor(f, f.k, f.k_stride, f.kv_heads, dk, ks) ||
+      !linear_tensor(f, f.v, f.v_stride, f.kv_heads, dv, vs) || !linear_tensor(f, a->dout, a->do_stride, f.heads, dv, dos) ||
+      !linear_tensor(f, a->dq, a->dq_stride, f.heads, dk, dqs) || !linear_tensor(f, a->dk, a->dk_stride, f.kv_heads, dk, dks) ||
+      !linear_tensor(f, a->dv, a->dv_stride, f.kv_heads, dv, dvs))
+    return fail(AIDN_EINVAL, "linear_attention_backward: a tensor is not aligned to its elements, or a stride is negative");
+  if (group > 1 && part[0] + part[1] > 0 && (!f.workspace || f.workspace_bytes < part[0] + part[1]))
+    return fail(AIDN_EWORKSPACE, "linear_attention_backward: workspace of %lld bytes, need %lld", (long long)(f.workspace ? f.workspace_bytes : 0),
+                (long long)(part[0] + part[1]));
+  auto copy3 = [](int64_t* to, const int64_t* from) { std::memcpy(to, from, 3 * sizeof(int64_t)); };
+  const int64_t rows = f.token_starts ? f.tokens : f.seq_len;   // of a head of the partial sums
+  p.scans = 3;
+  aidn::lin::Scan& sq = p.scan[0];
+  sq.a = a->dout; sq.b = f.v; sq.c = f.k; sq.y = a->dq;
+  copy3(sq.as, dos); copy3(sq.bs, vs); copy3(sq.cs, ks); copy3(sq.ys, dqs);
+  sq.a_group = 1; sq.b_group = sq.c_group = group;
+  sq.d1 = (int)dv; sq.d2 = (int)dk;
+  sq.lag = 1;
+  sq.row_scale = p.scale; sq.key_scale = 1.f;
+  sq.x_first = f.initial_state;
+  sq.x_transposed = 1;
+  aidn::lin::Scan& sk = p.scan[1];
+  sk.a = f.v; sk.b = a->dout; sk.c = f.q; sk.y = group > 1 ? f.workspace : a->dk;
+  copy3(sk.as, vs); copy3(sk.bs, dos); copy3(sk.cs, qs); copy3(sk.ys, dks);
+  sk.a_group = group; sk.b_group = sk.c_group = 1;
+  sk.d1 = (int)dv; sk.d2 = (int)dk;
+  sk.x_first = a->d_final_state;
+  sk.x_transposed = 1;
+  aidn::lin::Scan& sv = p.scan[2];
+  sv.a = f.k; sv.b = f.q; sv.c = a->dout; sv.y = group > 1 ? static_cast<char*>(f.workspace) + part[0] : a->dv;
+  copy3(sv.as, ks); copy3(sv.bs, qs); copy3(sv.cs, dos); copy3(sv.ys, dvs);
+  sv.a_group = group; sv.b_group = sv.c_group = 1;
+  sv.d1 = (int)dk; sv.d2 = (int)dv;
+  sv.x_first = a->d_final_state;
+  sv.x_last = a->d_initial_state;
+  for (aidn::lin::Scan* s : {&sk, &sv}) {
+    s->reverse = 1;
+    s->row_scale = 1.f;
+    s->key_scale = p.scale;
+    if (group > 1) {
+      s->y_f32 = 1;
+      s->ys[0] = f.heads * rows * s->d2;
+      s->ys[1] = rows * s->d2;
+      s->ys[2] = s->d2;
+    }
+  }
+  int sms = 0;
+  rc = device_facts("linear_attention_backward", &sms);
+  if (rc != AIDN_OK) return rc;
+  cudaStream_t stream = (cudaStream_t)cu_stream;
+  int launches = 0;
+  cudaError_t e = aidn::lin::launch_scan_generic(p, stream, &launches);
+  if (e == cudaSuccess && group > 1) {
+    aidn::lin::GroupSum g;
+    std::memset(&g, 0, sizeof(g));
+    g.partial[0] = static_cast<const float*>(sk.y);
+    g.partial[1] = static_cast<const float*>(sv.y);
+    g.out[0] = a->dk; g.out[1] = a->dv;
+    copy3(g.os[0], dks); copy3(g.os[1], dvs);
+    g.d[0] = (int)dk; g.d[1] = (int)dv;
+    g.rows = rows;
+    g.lengths = f.lengths; g.starts = f.token_starts;
+    g.tokens = f.tokens; g.seq_len = f.seq_len;
+    g.batch = f.batch; g.kv_heads = f.kv_heads; g.group = group; g.dtype = f.dtype;
+    e = aidn::lin::launch_group_sum(g, stream);
+  }
+  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_backward");
+  return post_launch_check(stream, "aidn_linear_attention_backward", nullptr);
+}
+
+int aidn_linear_attention_step(const aidn_linear_step_args* a, void* cu_stream) {
+  g_err[0] = 0;
+  if (!a) return fail(AIDN_EINVAL, "linear_attention_step: null argument");
+  if (a->batch < 0 || a->heads <= 0 || a->kv_heads <= 0) return fail(AIDN_EINVAL, "linear_attention_step: batch must be >= 0, heads and kv_heads positive");
+  if (a->batch > 65535 || a->heads > 65535) return fail(AIDN_EINVAL, "linear_attention_step: batch and heads must be at most 65535");
+  if (a->heads % a->kv_heads != 0) return fail(AIDN_EINVAL, "linear_attention_step: kv_heads (%d) must divide heads (%d)", a->kv_heads, a->heads);
+  if (a->key_dim <= 0 || a->key_dim > 256 || a->key_dim % 8 != 0 || a->value_dim <= 0 || a->value_dim > 256 || a->value_dim % 8 != 0)
+    return fail(AIDN_EINVAL, "linear_attention_step: key_dim (%d) and value_dim (%d) must be multiples of 8 in [8, 256]", a->key_dim, a->value_dim);
+  if (a->dtype < AIDN_F32 || a->dtype > AIDN_BF16) return fail(AIDN_EINVAL, "linear_attention_step: unknown dtype %d", a->dtype);
+  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return fail(AIDN_EINVAL, "linear_attention_step: scale must be finite and >= 0");
+  if (a->state_slots && a->num_slots <= 0) return fail(AIDN_EINVAL, "linear_attention_step: state_slots needs num_slots > 0");
+  if (a->batch == 0) return AIDN_OK;
+  if (!a->q || !a->k || !a->v || !a->out || !a->states) return fail(AIDN_EINVAL, "linear_attention_step: null buffer");
+  const size_t esz = elem_size(a->dtype);
+  if ((uintptr_t)a->q % esz || (uintptr_t)a->k % esz || (uintptr_t)a->v % esz || (uintptr_t)a->out % esz || (uintptr_t)a->decay % 4 || (uintptr_t)a->state_slots % 4)
+    return fail(AIDN_EINVAL, "linear_attention_step: a buffer is not aligned to its elements");
+  if ((uintptr_t)a->states % 16 != 0) return fail(AIDN_EINVAL, "linear_attention_step: states must be 16-byte aligned");
+  aidn::lin::Step p;
+  std::memset(&p, 0, sizeof(p));
+  const int64_t kd = a->key_dim, vd = a->value_dim;
+  const int64_t dq[2] = {a->heads * kd, kd}, dk[2] = {a->kv_heads * kd, kd}, dv[2] = {a->kv_heads * vd, vd}, dout[2] = {a->heads * vd, vd};
+  if (!take_strides(2, a->q_stride, dq, p.qs) || !take_strides(2, a->k_stride, dk, p.ks) || !take_strides(2, a->v_stride, dv, p.vs) || !take_strides(2, a->o_stride, dout, p.os))
+    return fail(AIDN_EINVAL, "linear_attention_step: negative stride");
+  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
+  p.states = a->states;
+  p.decay = a->decay;
+  p.slots = a->state_slots;
+  p.batch = a->batch; p.heads = a->heads; p.group = a->heads / a->kv_heads;
+  p.key_dim = a->key_dim; p.value_dim = a->value_dim;
+  p.num_slots = a->state_slots ? a->num_slots : a->batch;
+  p.dtype = a->dtype;
+  p.scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt((float)a->key_dim);
+  int sms = 0;
+  const int rc = device_facts("linear_attention_step", &sms);
+  if (rc != AIDN_OK) return rc;
+  const cudaError_t e = aidn::lin::launch_step(p, sms, (cudaStream_t)cu_stream);
+  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_step");
+  return post_launch_check((cudaStream_t)cu_stream, "aidn_linear_attention_step", nullptr);
 }
 
 // ---- fused multi-head attention forward ---------------------------------------------------------------------------

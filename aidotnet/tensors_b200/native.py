@@ -36,6 +36,8 @@ EXPORTS = (
     "aidn_sdpa_backward", "aidn_sdpa_backward_workspace_bytes", "aidn_paged_kv_append", "aidn_mha_forward",
     "aidn_mha_workspace_bytes", "aidn_peer_export", "aidn_peer_open", "aidn_peer_close",
     "aidn_kv8_append", "aidn_sdpa_kv8_workspace_bytes", "aidn_sdpa_launch_kv8",
+    "aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_workspace_bytes", "aidn_linear_attention_backward",
+    "aidn_linear_attention_backward_workspace_bytes", "aidn_linear_attention_step",
     "aidn_sdpa_debug_set",   # include/aidn_sdpa_debug.h
 )
 
@@ -121,6 +123,49 @@ class Kv8AppendArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p), ("query_out", ctypes.c_void_p), ("key", ctypes.c_void_p), ("key_out", ctypes.c_void_p),
+        ("query_stride", ctypes.c_int64 * 2), ("query_out_stride", ctypes.c_int64 * 2), ("key_stride", ctypes.c_int64 * 2),
+        ("key_out_stride", ctypes.c_int64 * 2), ("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("seq_len", ctypes.c_int64), ("start_position", ctypes.c_int64), ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("layout", ctypes.c_int32), ("position_bytes", ctypes.c_int32), ("inverse", ctypes.c_int32), ("amplitude", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p), ("decay", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p), ("token_starts", ctypes.c_void_p), ("initial_state", ctypes.c_void_p),
+        ("final_state", ctypes.c_void_p), ("state_slots", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3), ("o_stride", ctypes.c_int64 * 3),
+        ("tokens", ctypes.c_int64), ("seq_len", ctypes.c_int64), ("batch", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("key_dim", ctypes.c_int32), ("value_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32), ("path", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", LinearArgs), ("dout", ctypes.c_void_p), ("d_final_state", ctypes.c_void_p), ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p), ("d_initial_state", ctypes.c_void_p), ("do_stride", ctypes.c_int64 * 3),
+        ("dq_stride", ctypes.c_int64 * 3), ("dk_stride", ctypes.c_int64 * 3), ("dv_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class LinearStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p), ("states", ctypes.c_void_p),
+        ("decay", ctypes.c_void_p), ("state_slots", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 2), ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2), ("batch", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("key_dim", ctypes.c_int32), ("value_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
 # The argument blocks of the calls that a decode step makes, packed in one go: filling a ctypes structure field by field took
 # longer than the kernels of a small step.
 _SDPA_ARGS = struct.Struct("@6P4qP3q12qfPqiPi8P")
@@ -128,8 +173,13 @@ _PAGED_KV = struct.Struct("@Pqii")
 _QKV_ROPE_ARGS = struct.Struct("@10P8i2q")
 _KV8_CACHE = struct.Struct("@5P4q4i")
 _KV8_APPEND_ARGS = struct.Struct("@4P8q5P2q4i")
-assert (_SDPA_ARGS.size, _PAGED_KV.size, _QKV_ROPE_ARGS.size, _KV8_CACHE.size, _KV8_APPEND_ARGS.size) == tuple(
-    ctypes.sizeof(t) for t in (SdpaArgs, PagedKv, QkvRopeArgs, Kv8Cache, Kv8AppendArgs))
+_ROTARY_ARGS = struct.Struct("@4P8q2P3q8ifi")
+_LINEAR_ARGS = struct.Struct("@10P14q8ifiPq")
+_LINEAR_BWD_TAIL = struct.Struct("@6P12q")   # behind the forward's block
+_LINEAR_STEP_ARGS = struct.Struct("@7P8q7if")
+assert (_SDPA_ARGS.size, _PAGED_KV.size, _QKV_ROPE_ARGS.size, _KV8_CACHE.size, _KV8_APPEND_ARGS.size, _ROTARY_ARGS.size, _LINEAR_ARGS.size,
+        _LINEAR_ARGS.size + _LINEAR_BWD_TAIL.size, _LINEAR_STEP_ARGS.size) == tuple(
+    ctypes.sizeof(t) for t in (SdpaArgs, PagedKv, QkvRopeArgs, Kv8Cache, Kv8AppendArgs, RotaryArgs, LinearArgs, LinearBwdArgs, LinearStepArgs))
 _NO_STRIDE, _NO_PEERS = (0, 0, 0), (0,) * 8
 
 
@@ -143,11 +193,13 @@ class AidnError(RuntimeError):
 _lib: Optional[ctypes.CDLL] = None
 # the entry points that take packed argument blocks (bytes)
 _launch_packed = _launch_paged_packed = _qkv_rope_packed = _kv8_append_packed = _launch_kv8_packed = None
+_rotary_packed = _linear_packed = _linear_bwd_packed = _linear_step_packed = None
 
 
 def load() -> ctypes.CDLL:
     """Loads the CUDA library.  Raises if it has not been built: there is no CPU path behind this API."""
     global _lib, _launch_packed, _launch_paged_packed, _qkv_rope_packed, _kv8_append_packed, _launch_kv8_packed
+    global _rotary_packed, _linear_packed, _linear_bwd_packed, _linear_step_packed
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -213,6 +265,14 @@ def load() -> ctypes.CDLL:
     lib.aidn_sdpa_launch_kv8.argtypes = [ctypes.c_void_p, ctypes.POINTER(SdpaArgs), ctypes.POINTER(Kv8Cache), ctypes.c_void_p,
                                          ctypes.c_int64, ctypes.c_void_p]
     lib.aidn_sdpa_launch_kv8.restype = ctypes.c_int
+    lib.aidn_rotary.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.aidn_linear_attention.argtypes = [ctypes.POINTER(LinearArgs), ctypes.c_void_p]
+    lib.aidn_linear_attention_backward.argtypes = [ctypes.POINTER(LinearBwdArgs), ctypes.c_void_p]
+    lib.aidn_linear_attention_step.argtypes = [ctypes.POINTER(LinearStepArgs), ctypes.c_void_p]
+    for name in ("aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_backward", "aidn_linear_attention_step"):
+        getattr(lib, name).restype = ctypes.c_int
+    for name in ("aidn_linear_attention_workspace_bytes", "aidn_linear_attention_backward_workspace_bytes"):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.c_char_p], ctypes.c_int64   # a packed block
     lib.aidn_sdpa_debug_set.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]
     lib.aidn_sdpa_debug_set.restype = ctypes.c_int
     pointer, block = ctypes.c_void_p, ctypes.c_char_p
@@ -222,6 +282,9 @@ def load() -> ctypes.CDLL:
     _kv8_append_packed = ctypes.CFUNCTYPE(ctypes.c_int, block, block, pointer)(("aidn_kv8_append", lib))
     _launch_kv8_packed = ctypes.CFUNCTYPE(ctypes.c_int, pointer, block, block, pointer, ctypes.c_int64, pointer)(
         ("aidn_sdpa_launch_kv8", lib))
+    _rotary_packed, _linear_packed, _linear_bwd_packed, _linear_step_packed = (
+        ctypes.CFUNCTYPE(ctypes.c_int, block, pointer)((name, lib)) for name in (
+            "aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_backward", "aidn_linear_attention_step"))
     _lib = lib
     return lib
 
@@ -539,5 +602,86 @@ def kv8_append(cache: bytes, *, key: int, value: int, start: int, tokens: int, b
         query or 0, key or 0, value or 0, query_out or 0, *query_stride, *key_stride, *value_stride, *query_out_stride,
         cosine or 0, sine or 0, start or 0, token_starts or 0, positions or 0, tokens, max_position, batch, heads, dtype, rope),
         stream)
+    if status != OK:
+        raise AidnError(status, last_error())
+
+
+_NO_ROW_STRIDE = (0, 0)
+
+
+def rotary(*, query: int, query_out: int, frequencies: int, tokens: int, heads: int, head_dim: int, rotary_dim: int, dtype: int, stream: int,
+           key: Optional[int] = None, key_out: Optional[int] = None, kv_heads: int = 0, positions: Optional[int] = None,
+           position_bytes: int = 4, seq_len: int = 0, start_position: int = 0, layout: int = ROPE_INTERLEAVED, inverse: bool = False,
+           amplitude: float = 1.0, query_stride=_NO_ROW_STRIDE, query_out_stride=_NO_ROW_STRIDE, key_stride=_NO_ROW_STRIDE,
+           key_out_stride=_NO_ROW_STRIDE) -> None:
+    """Turns the pairs of queries and keys by their positions; ``inverse`` turns them back (the gradient)."""
+    if _lib is None:
+        load()
+    status = _rotary_packed(_ROTARY_ARGS.pack(
+        query or 0, query_out or 0, key or 0, key_out or 0, *query_stride, *query_out_stride, *key_stride, *key_out_stride, frequencies or 0,
+        positions or 0, tokens, seq_len, start_position, heads, kv_heads, head_dim, rotary_dim, dtype, layout, position_bytes, bool(inverse),
+        amplitude, 0), stream)
+    if status != OK:
+        raise AidnError(status, last_error())
+
+
+def linear_block(*, q: int = 0, k: int = 0, v: int = 0, out: int = 0, batch: int, heads: int, kv_heads: int, seq_len: int, key_dim: int,
+                 value_dim: int, dtype: int, decay: Optional[int] = None, lengths: Optional[int] = None, token_starts: Optional[int] = None,
+                 tokens: int = 0, initial_state: Optional[int] = None, final_state: Optional[int] = None, state_slots: Optional[int] = None,
+                 num_slots: int = 0, q_stride=None, k_stride=None, v_stride=None, o_stride=None, scale: float = 0.0, path: int = PATH_AUTO,
+                 workspace: Optional[int] = None, workspace_bytes: int = 0) -> bytes:
+    """The ``aidn_linear_args`` block."""
+    return _LINEAR_ARGS.pack(
+        q or 0, k or 0, v or 0, out or 0, decay or 0, lengths or 0, token_starts or 0, initial_state or 0, final_state or 0, state_slots or 0,
+        *_strides(q_stride), *_strides(k_stride), *_strides(v_stride), *_strides(o_stride), tokens, seq_len, batch, heads, kv_heads, key_dim,
+        value_dim, dtype, num_slots, path, scale, 0, workspace or 0, workspace_bytes)
+
+
+def linear_bwd_block(fwd: bytes, *, dout: int = 0, dq: int = 0, dk: int = 0, dv: int = 0, d_final_state: Optional[int] = None,
+                     d_initial_state: Optional[int] = None, do_stride=None, dq_stride=None, dk_stride=None, dv_stride=None) -> bytes:
+    """The ``aidn_linear_bwd_args`` block around a forward's."""
+    return fwd + _LINEAR_BWD_TAIL.pack(
+        dout or 0, d_final_state or 0, dq or 0, dk or 0, dv or 0, d_initial_state or 0, *_strides(do_stride), *_strides(dq_stride),
+        *_strides(dk_stride), *_strides(dv_stride))
+
+
+def linear_workspace_bytes(block: bytes) -> int:
+    """Workspace of the forward or (a block of ``linear_bwd_block``) the backward call with these arguments."""
+    lib = _lib or load()
+    size = lib.aidn_linear_attention_workspace_bytes if len(block) == _LINEAR_ARGS.size else lib.aidn_linear_attention_backward_workspace_bytes
+    n = size(block)
+    if n < 0:
+        raise AidnError(EINVAL, last_error())
+    return int(n)
+
+
+def linear_attention(block: bytes, stream: int) -> None:
+    """Linear attention of whole sequences; ``block`` is what ``linear_block`` packed."""
+    if _lib is None:
+        load()
+    status = _linear_packed(block, stream)
+    if status != OK:
+        raise AidnError(status, last_error())
+
+
+def linear_attention_backward(block: bytes, stream: int) -> None:
+    """Its gradients; ``block`` is what ``linear_bwd_block`` packed."""
+    if _lib is None:
+        load()
+    status = _linear_bwd_packed(block, stream)
+    if status != OK:
+        raise AidnError(status, last_error())
+
+
+def linear_attention_step(*, q: int, k: int, v: int, out: int, states: int, batch: int, heads: int, kv_heads: int, key_dim: int, value_dim: int,
+                          dtype: int, stream: int, decay: Optional[int] = None, state_slots: Optional[int] = None, num_slots: int = 0,
+                          scale: float = 0.0, q_stride=_NO_ROW_STRIDE, k_stride=_NO_ROW_STRIDE, v_stride=_NO_ROW_STRIDE,
+                          o_stride=_NO_ROW_STRIDE) -> None:
+    """One token of each sequence against the states, which it updates in place."""
+    if _lib is None:
+        load()
+    status = _linear_step_packed(_LINEAR_STEP_ARGS.pack(
+        q or 0, k or 0, v or 0, out or 0, states or 0, decay or 0, state_slots or 0, *q_stride, *k_stride, *v_stride, *o_stride, batch, heads,
+        kv_heads, key_dim, value_dim, dtype, num_slots, scale), stream)
     if status != OK:
         raise AidnError(status, last_error())

@@ -358,6 +358,127 @@ AIDN_API int64_t aidn_sdpa_kv8_workspace_bytes(aidn_sdpa_t h, int64_t batch, int
 AIDN_API int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* args, const aidn_kv8_cache* cache,
                                   const int32_t* query_starts, int64_t queries, void* cu_stream);
 
+/* ---- rotary positions -------------------------------------------------------------------------------------------------
+ * The pairs of the first rotary_dim elements of every head, turned by position * frequency:
+ * (a, b) -> amplitude * (a cos - b sin, a sin + b cos); the elements behind them are copied.  Angles are formed in 64 bits from the
+ * frequencies, so that a position far into a long context is as exact as the first, and any scaling for long contexts is a choice of
+ * frequencies and amplitude.  Products and sums in fp32, one rounding.  With `inverse` the angles are negated: the gradient.
+ * Queries, and keys if there are any, in one launch.  An output may be its input itself, with the same strides; otherwise nothing overlaps. */
+typedef struct {
+  const void* query;          /* [tokens, heads, head_dim]                                                          */
+  void* query_out;
+  const void* key;            /* [tokens, kv_heads, head_dim] or NULL                                               */
+  void* key_out;
+  int64_t query_stride[2];    /* elements for (token, head); both zero = dense                                      */
+  int64_t query_out_stride[2];
+  int64_t key_stride[2];
+  int64_t key_out_stride[2];
+  const double* frequencies;  /* [rotary_dim / 2] radians a position                                                */
+  const void* positions;      /* [tokens] of position_bytes each, or NULL: start_position + token % seq_len         */
+  int64_t tokens;
+  int64_t seq_len;            /* 0 = tokens; unused with positions                                                  */
+  int64_t start_position;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;           /* a multiple of 8 up to 256                                                          */
+  int32_t rotary_dim;         /* even, 2 .. head_dim                                                                */
+  int32_t dtype;              /* aidn_dtype of queries and keys, in and out                                         */
+  int32_t layout;             /* AIDN_ROPE_INTERLEAVED: pairs (2i, 2i+1), AIDN_ROPE_HALVES: (i, i + rotary_dim / 2)  */
+  int32_t position_bytes;     /* 4 or 8                                                                             */
+  int32_t inverse;
+  float amplitude;            /* a factor of the turned elements; 0 = 1                                             */
+  int32_t reserved;
+} aidn_rotary_args;
+AIDN_API int aidn_rotary(const aidn_rotary_args* args, void* cu_stream);
+
+/* ---- linear attention with a decay for each head -----------------------------------------------------------------------
+ * The state S of a head is a [key_dim, value_dim] matrix:
+ *     S_t = exp(decay) S_(t-1) + k_t v_t^T,   o_t = scale * q_t S_t.
+ * decay is the head's log decay, at most 0 (-inf: nothing is kept; above 0 or NaN: the head's outputs are NaN).  Query head h reads key and
+ * value head h / (heads / kv_heads); every query head has a state of its own, in fp32.  Sums and states are fp32; 16-bit inputs run on the
+ * tensor cores where both sizes are 64 or 128 (the state, and the weighted products q . k, are rounded to the 16-bit type, relative to their own
+ * size, where they meet a 16-bit operand; what is added to a state is not), other sizes and fp32 on FFMA.  Results do not depend on launch order.
+ * Nothing that follows a row reaches it.  No counterpart in the reference.
+ *
+ * Sequences: [batch, heads, seq_len, size] by strides, of lengths[b] rows each if given; the rows behind them are written as zeros.  Or packed
+ * rows [tokens, heads, size] with token_starts (device, [batch + 1], ascending from 0): sequence b has the rows token_starts[b] ..
+ * token_starts[b + 1] - 1, at most seq_len; rows of no sequence are left as they are.
+ * States: sequence b begins with initial_state[s] (NULL, or s < 0: zeros) and leaves final_state[s], s = state_slots[b] or b.  final_state may be
+ * initial_state itself.  A slot at or above num_slots, or one that an earlier sequence of the call has, gives rows of NaN and touches no state.
+ * out overlaps nothing else. */
+typedef struct {
+  const void* q;                /* element (b,h,t,d) at b*stride[0] + h*stride[1] + t*stride[2] + d; packed rows: stride[0] unused */
+  const void* k;
+  const void* v;
+  void* out;
+  const float* decay;           /* [heads] or NULL: 0                                                               */
+  const int32_t* lengths;       /* [batch] or NULL                                                                  */
+  const int32_t* token_starts;  /* [batch + 1] or NULL                                                              */
+  const float* initial_state;   /* [num_slots, heads, key_dim, value_dim] dense, 16-byte aligned, or NULL            */
+  float* final_state;           /* or NULL                                                                          */
+  const int32_t* state_slots;   /* [batch] or NULL                                                                  */
+  int64_t q_stride[3];          /* all zero = dense [batch, heads, seq_len, size], or packed [tokens, heads, size]    */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t tokens;               /* rows of packed tensors                                                           */
+  int64_t seq_len;              /* the most rows of a sequence                                                      */
+  int32_t batch, heads, kv_heads;
+  int32_t key_dim, value_dim;   /* multiples of 8 up to 256                                                         */
+  int32_t dtype;                /* aidn_dtype of q, k, v and out                                                    */
+  int32_t num_slots;            /* states behind initial_state / final_state; unused without state_slots            */
+  int32_t path;                 /* AIDN_PATH_AUTO, or AIDN_PATH_GENERIC: FFMA                                       */
+  float scale;                  /* 0 = 1/sqrt(key_dim)                                                              */
+  int32_t reserved;
+  void* workspace;              /* device, 256-byte aligned, of aidn_linear_attention_workspace_bytes(), or NULL (slower) */
+  int64_t workspace_bytes;
+} aidn_linear_args;
+AIDN_API int64_t aidn_linear_attention_workspace_bytes(const aidn_linear_args* args);
+AIDN_API int aidn_linear_attention(const aidn_linear_args* args, void* cu_stream);
+
+/* Its gradients, from the same argument block (out, final_state and o_stride are not looked at; state_slots must be NULL): dq, dk, dv in the type of
+ * q, from those of out (dout, in that type) and of final_state (d_final_state, or NULL); d_initial_state (or NULL) receives those of
+ * initial_state.  States are [batch, heads, key_dim, value_dim].  Gradients of shared heads are summed in fp32 in the heads' order and
+ * rounded once; decay has none.  Rows behind a sequence's length are zeros, rows of no sequence are left.  Gradients overlap neither one another nor what the call
+ * reads.  The workspace is needed where aidn_linear_attention_backward_workspace_bytes() says so and kv_heads < heads. */
+typedef struct {
+  aidn_linear_args fwd;
+  const void* dout;
+  const float* d_final_state;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* d_initial_state;
+  int64_t do_stride[3];         /* all zero = dense, as in aidn_linear_args                                         */
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+} aidn_linear_bwd_args;
+AIDN_API int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linear_bwd_args* args);
+AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, void* cu_stream);
+
+/* One token of each of `batch` sequences against states that stay where they are: state state_slots[b] (NULL: b) is updated in place.  A
+ * negative slot is a row of padding: its output is zeros and no state is touched.  Other slots as above.  One launch. */
+typedef struct {
+  const void* q;                /* [batch, heads, key_dim]                                                          */
+  const void* k;                /* [batch, kv_heads, key_dim]                                                       */
+  const void* v;                /* [batch, kv_heads, value_dim]                                                     */
+  void* out;                    /* [batch, heads, value_dim]                                                        */
+  float* states;                /* [num_slots, heads, key_dim, value_dim] dense, 16-byte aligned                    */
+  const float* decay;           /* [heads] or NULL: 0                                                               */
+  const int32_t* state_slots;   /* [batch] or NULL                                                                  */
+  int64_t q_stride[2];          /* elements for (row, head); both zero = dense                                      */
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t o_stride[2];
+  int32_t batch, heads, kv_heads;
+  int32_t key_dim, value_dim;   /* multiples of 8 up to 256                                                         */
+  int32_t dtype;
+  int32_t num_slots;            /* unused without state_slots                                                       */
+  float scale;                  /* 0 = 1/sqrt(key_dim)                                                              */
+} aidn_linear_step_args;
+AIDN_API int aidn_linear_attention_step(const aidn_linear_step_args* args, void* cu_stream);
+
 /* ---- fused multi-head attention forward ---------------------------------------------------------------------
  * IEngine.MultiHeadAttentionForward (src/AiDotNet.Tensors/Engines/IEngine.cs:4201-4208; CPU
  * CpuEngine.MultiHeadAttention.cs:68-338, GPU composition DirectGpuTensorEngine.MissingKernels.cs:5793-5870):
