@@ -19,6 +19,7 @@
 namespace {
 
 thread_local char g_err[512] = "";
+thread_local bool g_expire_linear = false;   // the same for aidn_linear_attention and its backward
 thread_local bool g_expire_qkv = false;   // test hook: this thread's next aidn_qkv_rope_cache lets its bounded waits run out
 
 int fail(int code, const char* fmt, ...) {
@@ -321,7 +322,8 @@ int aidn_sdpa_last_launch_count(aidn_sdpa_t h) { return h ? h->last_launches : -
 int aidn_sdpa_debug_set(aidn_sdpa_t h, float* buf, int mode) {
   if (!h) {
     g_expire_qkv = mode == 3;
-    return mode == 0 || mode == 3 ? AIDN_OK : AIDN_EINVAL;
+    g_expire_linear = mode == 5;
+    return mode == 0 || mode == 3 || mode == 5 ? AIDN_OK : AIDN_EINVAL;
   }
   h->debug = buf;
   h->debug_mode = (buf || mode == 3) ? mode : 0;
@@ -1075,6 +1077,19 @@ bool linear_tensor(const aidn_linear_args& a, const void* ptr, const int64_t* gi
 }
 
 bool no_rows(const aidn_linear_args& a) { return a.token_starts && a.tokens == 0; }
+
+// The scans of a call, and the check behind them.
+cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int sms, char* work, int64_t work_bytes, cudaStream_t stream, bool* waits) {
+  const bool expire = g_expire_linear;
+  g_expire_linear = false;
+  int launches = 0;
+  *waits = a.path != AIDN_PATH_GENERIC && aidn::lin::scan_sm100_supported(p);
+  return *waits ? aidn::lin::launch_scan_sm100(p, sms, reinterpret_cast<float*>(work), work_bytes, expire, stream, &launches)
+                : aidn::lin::launch_scan_generic(p, stream, &launches);
+}
+int linear_check(const char* what, cudaStream_t stream, bool waits) {
+  return post_launch_check(stream, what, waits && launch_check_enabled() ? aidn::lin::sm100_status() : nullptr, true);
+}
 }  // namespace
 
 int aidn_rotary(const aidn_rotary_args* a, void* cu_stream) {
@@ -1163,10 +1178,10 @@ int aidn_linear_attention(const aidn_linear_args* a, void* cu_stream) {
   int sms = 0;
   rc = device_facts("linear_attention", &sms);
   if (rc != AIDN_OK) return rc;
-  int launches = 0;
-  const cudaError_t e = aidn::lin::launch_scan_generic(p, (cudaStream_t)cu_stream, &launches);
+  bool waits = false;
+  const cudaError_t e = run_scans(*a, p, sms, static_cast<char*>(a->workspace), a->workspace_bytes, (cudaStream_t)cu_stream, &waits);
   if (e != cudaSuccess) return fail_cuda(e, "linear_attention");
-  return post_launch_check((cudaStream_t)cu_stream, "aidn_linear_attention", nullptr);
+  return linear_check("aidn_linear_attention", (cudaStream_t)cu_stream, waits);
 }
 
 // Bytes of the partial sums of dk and dv for shared heads.
@@ -1247,8 +1262,9 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
   rc = device_facts("linear_attention_backward", &sms);
   if (rc != AIDN_OK) return rc;
   cudaStream_t stream = (cudaStream_t)cu_stream;
-  int launches = 0;
-  cudaError_t e = aidn::lin::launch_scan_generic(p, stream, &launches);
+  bool waits = false;
+  cudaError_t e = run_scans(f, p, sms, f.workspace ? static_cast<char*>(f.workspace) + part[0] + part[1] : nullptr,
+                            f.workspace_bytes - part[0] - part[1], stream, &waits);
   if (e == cudaSuccess && group > 1) {
     aidn::lin::GroupSum g;
     std::memset(&g, 0, sizeof(g));
@@ -1264,7 +1280,21 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
     e = aidn::lin::launch_group_sum(g, stream);
   }
   if (e != cudaSuccess) return fail_cuda(e, "linear_attention_backward");
-  return post_launch_check(stream, "aidn_linear_attention_backward", nullptr);
+  return linear_check("aidn_linear_attention_backward", stream, waits);
+}
+
+int aidn_linear_attention_poll(void* cu_stream) {
+  g_err[0] = 0;
+  cudaError_t e = cudaStreamSynchronize((cudaStream_t)cu_stream);
+  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_poll: stream");
+  int32_t* status = aidn::lin::sm100_status();
+  if (!status) return fail(AIDN_ECUDA, "linear_attention_poll: no status word in the current context");
+  int32_t st = 0;
+  e = cudaMemcpy(&st, status, sizeof(st), cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_poll: status read");
+  if (st == 0) return AIDN_OK;
+  cudaMemset(status, 0, sizeof(st));
+  return fail(AIDN_ETIMEOUT, "linear_attention_poll: a kernel gave up a bounded wait (status word 0x%x)", st);
 }
 
 int aidn_linear_attention_step(const aidn_linear_step_args* a, void* cu_stream) {

@@ -43,7 +43,6 @@ struct Params {
   int64_t seq_len;           // the most rows of a sequence
   int32_t batch, heads, num_slots, dtype;
   float scale;
-  int32_t* status;
 };
 
 // A sequence's rows and state.
@@ -92,6 +91,13 @@ __device__ __forceinline__ float log2_decay(const float* decay, int h) {
 
 // a scan on FFMA, any sizes and types
 cudaError_t launch_scan_generic(const Params& p, cudaStream_t stream, int* launches);
+
+// 16-bit types with sizes of 64 and 128 on tcgen05 (csrc/linear_sm100.cu).  Without its workspace long sequences are not cut.
+bool scan_sm100_supported(const Params& p);
+int64_t scan_sm100_bytes(const Params& p, int num_sms);
+// expire: test hook - the loads are withheld and bounded waits give up after 20 ms.
+cudaError_t launch_scan_sm100(const Params& p, int num_sms, float* work, int64_t work_bytes, bool expire, cudaStream_t stream, int* launches);
+int32_t* sm100_status();   // address of its status word in the current context, or null
 
 // dk / dv of shared heads: fp32 partial sums [.., heads, .., d] summed over each group in order
 struct GroupSum {

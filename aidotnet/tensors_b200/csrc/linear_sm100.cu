@@ -1,0 +1,766 @@
+// The scan of linear.cuh for 16-bit tensors with sizes of 64 and 128, on tcgen05.  A CTA walks the rows of one sequence and head (or of one segment of
+// them) in chunks of 64, with tensor memory lanes along c's columns, so that the state never leaves the registers of the threads that own it:
+//
+//     S   = A B^T                      scores, 64 x 64 (rows of A in lanes 0-63; the lanes above hold what is not looked at)
+//     P   = S weighted by lam^(i-j), zeros where j follows i, in 16 bits to shared memory
+//     T^T = C^T B~                     B~ = rows of B weighted by lam^(n-lag-j), as two 16-bit terms: what is added to a state is not rounded
+//     O^T = X^T A^T  and  C^T P^T      apart, since their columns have different factors; X^T in 16 bits in tensor memory
+//     X   = lam^n X + T                in fp32 registers, then X^T rounded for the next chunk
+//
+//   warps 0-1    P            warp 2   TMA producer            warp 3   MMA issuer, owner of tensor memory
+//   warps 4-11   B~ and the state, a lane (column of c) and half of b's columns to a thread
+//   warps 12-15  output: O^T from tensor memory, weighted, pairs of lanes exchanged, 4-byte stores along c's columns
+//
+// Rows are taken from a sequence's last to its first for the gradients of keys and values: a tile is loaded as it lies, and only masks and
+// exponents turn around.  The last chunk's missing rows are zeros in C and B~.
+//
+// fp16: a row of P and a lane's row of X^T are scaled by a power of two to their own largest value, as neither is bound by fp16's range; the
+// second term of B~ is held 2^11 times as large, where fp16's smallest numbers do not cut it, and its product divided on the way into the first's.
+//
+// What is not finite in C would reach earlier rows of its chunk as 0 * NaN in C^T P^T: a thread whose column came out not finite sums it again, row by
+// row, over what the row may see.
+//
+// Few sequences and heads: their rows are cut into segments.  A first launch forms what each segment adds to the state, a second one turns
+// those into the states before the segments, and the scan then runs on all segments at once, at the price of b and c read twice.
+//
+// Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
+#include <cuda.h>
+
+#include "linear.cuh"
+#include "sm100_ptx.cuh"
+#include "tensor_map.hpp"
+
+namespace aidn {
+namespace lin {
+namespace {
+
+using namespace ptx;
+
+__device__ int32_t g_linear_status;   // set when a bounded wait gave up (the entry points have no handle whose status word could say so)
+
+constexpr int kChunk = 64;
+constexpr int kBlock = kChunk * 128;   // 64 rows of 64 16-bit elements
+constexpr int kThreads = 512;
+constexpr int kWarpLoad = 2, kWarpMma = 3, kWarpState = 4, kWarpOut = 12;   // (warps 0 and 1: P)
+
+template <int D1, int D2>
+struct Cfg {
+  static constexpr int kN1 = D1 / 64, kN2 = D2 / 64;
+  static constexpr int kStageBytes = (2 * kN1 + kN2) * kBlock;
+  static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
+  static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
+  static constexpr int kOffP = kStages * kStageBytes;             // two buffers
+  static constexpr int kOffBt = kOffP + 2 * kBlock;               // the two terms of B~
+  static constexpr int kOffTab = kOffBt + 2 * kN1 * kBlock;
+  // tables: powers [66], row weights [64], row scales of P [2][64], lane scales of X [4][128], exchange of maxima [2][2][128]
+  static constexpr int kTabPower = 0, kTabRow = 68, kTabP = 132, kTabX = 260, kTabMax = 772, kTabFloats = 1284;
+  static constexpr int kOffBar = kOffTab + kTabFloats * 4;
+  static constexpr int kBars = 2 * kStages + 17;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmem = kOffMisc + 16 + 1024;
+  // tensor memory columns
+  static constexpr int kColX = 0, kColT = D1 / 2, kColS = kColT + D1, kColO = kColS + 64;   // O: [2][state part, row part]
+  static_assert(kColO + 256 <= 512, "tensor memory");
+};
+
+struct Maps {
+  CUtensorMap t[4];
+};
+
+struct Args {
+  Params p;
+  int32_t ia[3], ib[3], ic[3];   // maps of a, b, c of each scan
+  int32_t first, count;          // scans of this launch
+  int32_t segments, seg_len;     // seg_len: a multiple of kChunk
+  int32_t states_only;
+  float* work;                   // [scan][sequence, head][segment][D1][D2]
+  uint64_t wait_ns;
+  int32_t withhold;              // test hook: no loads, so that the waits run out
+};
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+template <bool BF16>
+__device__ __forceinline__ float lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
+  if constexpr (BF16) return __uint_as_float((uint32_t)v << 16);
+  else return __half2float(*reinterpret_cast<__half*>(&v));
+}
+// Powers of two that bring a largest value into [2^14, 2^15) and back.  (What is not finite, or so small that the power has no
+// reciprocal, is left near where it is.)
+__device__ __forceinline__ void scale_of(float largest, float& to, float& back) {
+  int e = (__float_as_int(largest) >> 23) & 255;
+  if (e == 255) {
+    to = back = 1.f;
+    return;
+  }
+  e = e < 15 ? 15 : e;
+  to = __int_as_float((268 - e) << 23);
+  back = __int_as_float((e - 14) << 23);
+}
+
+// D[tmem] = A[smem] * B[smem] + D * 2^-11
+__device__ __forceinline__ void mma_ss_down11(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc)
+      : "memory");
+}
+
+template <int D1, int D2, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args args) {
+  using C = Cfg<D1, D2>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  float* table = reinterpret_cast<float*>(gen + C::kOffTab);
+  const uint32_t bars = base + C::kOffBar;
+  const uint32_t b_full = bars, b_empty = bars + 8 * C::kStages;
+  const uint32_t b_s_full = bars + 16 * C::kStages, b_s_empty = b_s_full + 8;
+  const uint32_t b_p_full = b_s_full + 16;                    // [2]
+  const uint32_t b_o_full = b_s_full + 32, b_o_empty = b_s_full + 48;   // [2] each
+  const uint32_t b_bt_full = b_s_full + 64, b_t_full = b_s_full + 72, b_t_empty = b_s_full + 80;
+  const uint32_t b_x_full = b_s_full + 88, b_x_empty = b_s_full + 96;
+  const uint32_t b_max = b_s_full + 104;                      // [4]: of the two warps that share lanes
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(gen + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
+
+  const Params& p = args.p;
+  const int which = args.first + (int)(blockIdx.x % (unsigned)args.count);
+  const unsigned unit = blockIdx.x / (unsigned)args.count;
+  const int seg = (int)(unit % (unsigned)args.segments);
+  const int item = (int)(unit / (unsigned)args.segments);
+  const int b = item / p.heads, h = item - b * p.heads;
+  const Scan& s = p.scan[which];
+  const bool states_only = args.states_only != 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool reverse = s.reverse != 0;
+  const uint64_t wait_ns = args.wait_ns;
+
+  const Sequence q = sequence_of(p, b);
+  const int64_t t0 = (int64_t)seg * args.seg_len;
+  const int rows = q.bad || q.n <= t0 ? 0 : (int)(q.n - t0 < args.seg_len ? q.n - t0 : args.seg_len);
+  const int chunks = (rows + kChunk - 1) / kChunk;
+  const int64_t y0 = (p.starts ? 0 : b * s.ys[0]) + h * s.ys[1] + q.row0 * s.ys[2];
+  // rows from tile row r of chunk c: token_of(c) + r, of the sequence
+  auto token_of = [&](int c) { return reverse ? (int)(q.n - t0) - (c + 1) * kChunk : (int)t0 + c * kChunk; };
+
+  // the segments that were empty have nothing before them either, but a state may have to be handed on
+  const bool run = chunks > 0 || (!q.bad && args.segments == 1 && s.x_last && q.state >= 0);
+  if (run) {
+    if (threadIdx.x == 0) {
+      *abort_flag = 0;
+      for (int i = 0; i < C::kStages; ++i) {
+        mbar_init(b_full + 8 * i, 1);
+        mbar_init(b_empty + 8 * i, states_only ? 1 : 5);
+      }
+      mbar_init(b_s_full, 1);
+      mbar_init(b_s_empty, 2);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(b_p_full + 8 * i, 2);
+        mbar_init(b_o_full + 8 * i, 1);
+        mbar_init(b_o_empty + 8 * i, 4);
+      }
+      mbar_init(b_bt_full, 8);
+      mbar_init(b_t_full, 1);
+      mbar_init(b_t_empty, 8);
+      mbar_init(b_x_full, 8);
+      mbar_init(b_x_empty, 1);
+      for (int i = 0; i < 4; ++i) mbar_init(b_max + 8 * i, 2);
+      fence_mbar_init();
+    }
+    const float g = log2_decay(p.decay, h);
+    if (threadIdx.x < 65) table[C::kTabPower + threadIdx.x] = exp2f(g * threadIdx.x);
+    else if (threadIdx.x >= 96 && threadIdx.x < 160) {
+      const int r = threadIdx.x - 96;
+      table[C::kTabRow + r] = s.row_scale * exp2f(g * ((reverse ? kChunk - 1 - r : r) + s.lag));
+    }
+    if (warp == kWarpMma) {
+      tmem_alloc(smem_u32(tmem_ptr), 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+    const float* power = table + C::kTabPower;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, wait_ns)); };
+    auto arrive = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+
+    if (warp == kWarpLoad) {
+      // ---- tiles in ----
+      const bool leader = elect_one();
+      const CUtensorMap* ma = &maps.t[args.ia[which]];
+      const CUtensorMap* mb = &maps.t[args.ib[which]];
+      const CUtensorMap* mc = &maps.t[args.ic[which]];
+      const int ha = h / s.a_group, hb = h / s.b_group, hc = h / s.c_group, bb = p.starts ? 0 : b;
+      for (int c = 0; c < chunks; ++c) {
+        const int st = c % C::kStages;
+        if (!wait(b_empty + 8 * st, (uint32_t)((c / C::kStages) & 1) ^ 1u)) break;
+        if (leader && !args.withhold) {
+          const uint32_t bar = b_full + 8 * st, dst = base + (uint32_t)(st * C::kStageBytes);
+          const int row = (int)q.row0 + token_of(c);
+          mbar_expect_tx(bar, (uint32_t)(states_only ? C::kStageBytes - C::kOffB : C::kStageBytes));
+#pragma unroll
+          for (int i = 0; i < C::kN1; ++i) {
+            if (!states_only) tma_load_4d(dst + i * kBlock, ma, bar, i * 64, row, ha, bb);
+            tma_load_4d(dst + C::kOffB + i * kBlock, mb, bar, i * 64, row, hb, bb);
+          }
+#pragma unroll
+          for (int i = 0; i < C::kN2; ++i) tma_load_4d(dst + C::kOffC + i * kBlock, mc, bar, i * 64, row, hc, bb);
+        }
+        __syncwarp();
+      }
+    } else if (warp == kWarpMma) {
+      // ---- products ----
+      const bool leader = elect_one();
+      constexpr uint32_t kTransposeA = 1u << 15;
+      constexpr uint32_t idesc_s = make_idesc(128, 64, BF16, false);                  // A and B along their rows
+      constexpr uint32_t idesc_x = make_idesc(128, 64, BF16, false);                  // X^T from tensor memory, A along its rows
+      constexpr uint32_t idesc_p = make_idesc(128, 64, BF16, false) | kTransposeA;    // C^T, P along its rows
+      constexpr uint32_t idesc_t = make_idesc(128, D1, BF16, true) | kTransposeA;     // C^T, B~ across its rows
+      auto stage = [&](int c) { return base + (uint32_t)((c % C::kStages) * C::kStageBytes); };
+      auto scores = [&](int c) {
+        if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
+        if (!wait(b_s_empty, (uint32_t)(c & 1) ^ 1u)) return false;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D1 / 16; ++k) {
+            const uint32_t off = (uint32_t)((k / 4) * kBlock + (k % 4) * 32);
+            mma_ss(tmem + C::kColS, make_smem_desc(stage(c) + off, 16, 1024), make_smem_desc(stage(c) + C::kOffB + off, 16, 1024), idesc_s, k > 0);
+          }
+          tc_commit(b_s_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = states_only || chunks == 0 || scores(0);
+      for (int c = 0; c < chunks && ok; ++c) {
+        if (!states_only && c + 1 < chunks && !(ok = scores(c + 1))) break;
+        if (states_only && !(ok = wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1)))) break;
+        const uint32_t ct = stage(c) + C::kOffC;
+        if (!(ok = wait(b_bt_full, (uint32_t)(c & 1)))) break;
+        if (!(ok = wait(b_t_empty, (uint32_t)(c & 1) ^ 1u))) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int term = 1; term >= 0; --term)   // the second term first: fp16 holds it 2^11 times as large
+#pragma unroll
+            for (int k = 0; k < kChunk / 16; ++k) {
+              const uint64_t cd = make_smem_desc(ct + k * 2048, kBlock, 1024);
+              const uint64_t bd = make_smem_desc(base + C::kOffBt + term * C::kN1 * kBlock + k * 2048, kBlock, 1024);
+              if (!BF16 && term == 0 && k == 0) mma_ss_down11(tmem + C::kColT, cd, bd, idesc_t);
+              else mma_ss(tmem + C::kColT, cd, bd, idesc_t, term == 0 || k > 0);
+            }
+          tc_commit(b_t_full);
+          if (states_only) tc_commit(b_empty + 8 * (c % C::kStages));
+        }
+        __syncwarp();
+        if (states_only) continue;
+        const uint32_t o = tmem + C::kColO + (c & 1) * 128;
+        if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
+        if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D1 / 16; ++k)
+            mma_ts(o, tmem + C::kColX + k * 8, make_smem_desc(stage(c) + (uint32_t)((k / 4) * kBlock + (k % 4) * 32), 16, 1024), idesc_x, k > 0);
+          tc_commit(b_x_empty);
+        }
+        __syncwarp();
+        if (!(ok = wait(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k)
+            mma_ss(o + 64, make_smem_desc(ct + k * 2048, kBlock, 1024), make_smem_desc(base + C::kOffP + (c & 1) * kBlock + k * 32, 16, 1024), idesc_p, k > 0);
+          tc_commit(b_o_full + 8 * (c & 1));
+          tc_commit(b_empty + 8 * (c % C::kStages));
+        }
+        __syncwarp();
+      }
+    } else if (warp < kWarpLoad) {
+      // ---- P ----
+      if (!states_only && chunks > 0) {
+        const int i = warp * 32 + lane;
+        const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16) + C::kColS;
+        float w[kChunk];   // of the row's scores; exactly zero behind the row
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const int d = reverse ? j - i : i - j;
+          w[j] = d >= 0 ? p.scale * power[d < 0 ? 0 : d] : 0.f;
+        }
+        for (int c = 0; c < chunks; ++c) {
+          if (!wait(b_s_full, (uint32_t)(c & 1))) break;
+          if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
+          tc_fence_after();
+          float to = 1.f;
+          if constexpr (!BF16) {
+            float most = 0.f, back;
+#pragma unroll
+            for (int j0 = 0; j0 < kChunk; j0 += 32) {
+              uint32_t r[32];
+              tmem_ld32(t_s + j0, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) most = fmaxf(most, w[j0 + j] == 0.f ? 0.f : fabsf(__uint_as_float(r[j]) * w[j0 + j]));
+            }
+            scale_of(most, to, back);
+            table[C::kTabP + (c & 1) * 64 + i] = back;
+          }
+          const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
+#pragma unroll
+          for (int j0 = 0; j0 < kChunk; j0 += 32) {
+            uint32_t r[32], v[16];
+            tmem_ld32(t_s + j0, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float x = w[j0 + j] == 0.f ? 0.f : __uint_as_float(r[j]) * w[j0 + j];
+              float y = w[j0 + j + 1] == 0.f ? 0.f : __uint_as_float(r[j + 1]) * w[j0 + j + 1];
+              if constexpr (!BF16) x *= to, y *= to;
+              v[j / 2] = pack2<BF16>(x, y);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              st_shared_v4(row + (((uint32_t)(j0 / 8 + u) ^ (uint32_t)(i & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+          }
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(b_s_empty);
+            mbar_arrive(b_p_full + 8 * (c & 1));
+          }
+        }
+      }
+    } else if (warp < kWarpOut) {
+      // ---- B~ and the state ----
+      const int tid = threadIdx.x - kWarpState * 32, quarter = warp & 3, half = (warp - kWarpState) >> 2;
+      constexpr int kCols = D1 / 2;              // of a thread
+      const int d2 = quarter * 32 + lane, d1 = half * kCols;
+      const bool owner = d2 < D2;                // (with 64 columns, the lanes above hold nothing; whole warps)
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const int64_t matrix = (int64_t)D1 * D2;
+      float x[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) x[i] = 0.f;
+      float* work = args.segments > 1 ? args.work + (((int64_t)which * p.batch * p.heads + item) * args.segments + seg) * matrix : nullptr;
+      if (owner && !states_only) {
+        const float* from = work ? work : (s.x_first && q.state >= 0 ? s.x_first + (q.state * p.heads + h) * matrix : nullptr);
+        if (from) {
+          const bool turned = !work && s.x_transposed;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) x[i] = from[turned ? (int64_t)d2 * D1 + d1 + i : (int64_t)(d1 + i) * D2 + d2];
+        }
+      }
+      // X^T of chunk c to tensor memory
+      auto put_state = [&](int c) {
+        if (owner) {
+          float to = 1.f;
+          if constexpr (!BF16) {
+            float most = 0.f, back;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) most = fmaxf(most, fabsf(x[i]));
+            float* most_of = table + C::kTabMax + (c & 1) * 256;   // (two in turn: the other warp has read c's before it takes part in c + 1)
+            most_of[half * 128 + d2] = most;
+            arrive(b_max + 8 * quarter);
+            if (!wait(b_max + 8 * quarter, (uint32_t)(c & 1))) return false;
+            most = fmaxf(most, most_of[(half ^ 1) * 128 + d2]);
+            scale_of(most, to, back);
+            if (half == 0) table[C::kTabX + (c & 3) * 128 + d2] = back;
+          }
+#pragma unroll
+          for (int i0 = 0; i0 < kCols; i0 += 32) {
+            uint32_t v[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) v[i / 2] = BF16 ? pack2<BF16>(x[i0 + i], x[i0 + i + 1]) : pack2<BF16>(x[i0 + i] * to, x[i0 + i + 1] * to);
+            tmem_st16(tmem + lanes + C::kColX + (d1 + i0) / 2, v);
+          }
+          tc_wait_st();
+        }
+        tc_fence_before();
+        arrive(b_x_full);
+        return true;
+      };
+      bool ok = states_only || put_state(0);
+      for (int c = 0; c < chunks && ok; ++c) {
+        const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
+        const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes);
+        if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) break;
+#pragma unroll
+        for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
+          const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
+          uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+          if (j < n) {
+            const float w = power[n - s.lag - j];
+            const uint4 v = lds128(st + C::kOffB + u * 16);
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+            uint32_t a[4], e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float2 f = unpack2<BF16>(in[k]);
+              f.x *= w;
+              f.y *= w;
+              a[k] = pack2<BF16>(f.x, f.y);
+              const float2 t = unpack2<BF16>(a[k]);
+              e[k] = BF16 ? pack2<BF16>(f.x - t.x, f.y - t.y) : pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+            }
+            hi = make_uint4(a[0], a[1], a[2], a[3]);
+            lo = make_uint4(e[0], e[1], e[2], e[3]);
+          }
+          st_shared_v4(base + C::kOffBt + u * 16, hi.x, hi.y, hi.z, hi.w);
+          st_shared_v4(base + C::kOffBt + C::kN1 * kBlock + u * 16, lo.x, lo.y, lo.z, lo.w);
+        }
+        if (n < kChunk)
+          for (int u = tid; u < C::kN2 * kBlock / 16; u += 256) {
+            const int r = (u % (kBlock / 16)) / 8;
+            if ((reverse ? kChunk - 1 - r : r) >= n) st_shared_v4(st + C::kOffC + u * 16, 0, 0, 0, 0);
+          }
+        fence_proxy_async_smem();
+        arrive(b_bt_full);
+        if (!wait(b_t_full, (uint32_t)(c & 1))) break;
+        tc_fence_after();
+        if (owner) {
+          const float keep = power[n];
+#pragma unroll
+          for (int i0 = 0; i0 < kCols; i0 += 32) {
+            uint32_t r[32];
+            tmem_ld32(tmem + lanes + C::kColT + d1 + i0, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(keep, x[i0 + i], s.key_scale * __uint_as_float(r[i]));
+          }
+        }
+        tc_fence_before();
+        arrive(b_t_empty);
+        if (!states_only && c + 1 < chunks) {
+          if (!wait(b_x_empty, (uint32_t)(c & 1))) break;
+          tc_fence_after();
+          ok = put_state(c + 1);
+        }
+      }
+      if (owner && !*abort_flag) {
+        if (states_only) {
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) work[(int64_t)(d1 + i) * D2 + d2] = x[i];
+        } else if (args.segments == 1 && s.x_last && q.state >= 0) {
+          float* to = s.x_last + (q.state * p.heads + h) * matrix;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) to[s.x_transposed ? (int64_t)d2 * D1 + d1 + i : (int64_t)(d1 + i) * D2 + d2] = x[i];
+        }
+      }
+    } else if (!states_only) {
+      // ---- output ----
+      const int quarter = warp & 3, d2 = quarter * 32 + lane;
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const bool owner = quarter * 32 < D2;
+      uint16_t* y16 = static_cast<uint16_t*>(s.y) + y0;
+      float* y32 = static_cast<float*>(s.y) + y0;
+      for (int c = 0; c < chunks; ++c) {
+        const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
+        const int low = reverse ? kChunk - n : 0, high = reverse ? kChunk : n;   // the tile's rows
+        const int token = token_of(c);
+        if (!wait(b_o_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
+        tc_fence_after();
+        if (owner) {
+          const uint32_t t_o = tmem + lanes + C::kColO + (c & 1) * 128;
+          const float xs = BF16 ? 1.f : table[C::kTabX + (c & 3) * 128 + d2];
+          const float* row_w = table + C::kTabRow;
+          const float* row_p = table + C::kTabP + (c & 1) * 64;
+          float probe = 0.f;   // NaN as soon as a value of the row part is not finite
+          auto store = [&](int r, float a, float z) {   // rows r and r + 1
+            if (s.y_f32) {
+              if (r >= low && r < high) y32[(int64_t)(token + r) * s.ys[2] + d2] = a;
+              if (r + 1 >= low && r + 1 < high) y32[(int64_t)(token + r + 1) * s.ys[2] + d2] = z;
+            } else {
+              // even lanes take row r, odd ones row r + 1, of two columns each
+              const bool odd = lane & 1;
+              const float got = __shfl_xor_sync(0xffffffffu, odd ? a : z, 1);
+              const int mine = r + (odd ? 1 : 0);
+              if (mine >= low && mine < high)
+                *reinterpret_cast<uint32_t*>(y16 + (int64_t)(token + mine) * s.ys[2] + (d2 & ~1)) = odd ? pack2<BF16>(got, z) : pack2<BF16>(a, got);
+            }
+          };
+#pragma unroll
+          for (int r0 = 0; r0 < kChunk; r0 += 32) {
+            uint32_t u[32], v[32];
+            tmem_ld32(t_o + r0, u);
+            tmem_ld32(t_o + 64 + r0, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int r = 0; r < 32; r += 2) {
+              float e[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int at = r0 + r + k;
+                const float part = __uint_as_float(v[r + k]);
+                if (n == kChunk || (at >= low && at < high)) probe = fmaf(part, 0.f, probe);
+                float f = row_w[at] * __uint_as_float(u[r + k]);
+                if constexpr (!BF16) f *= xs;
+                e[k] = BF16 ? f + part : fmaf(row_p[at], part, f);
+              }
+              store(r0 + r, e[0], e[1]);
+            }
+          }
+          const bool again = probe != probe;
+          // (the tile is there since before the products; this thread has to see that for itself)
+          if (__any_sync(0xffffffffu, again) && wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) {
+            const uint32_t ct = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + C::kOffC + (d2 / 64) * kBlock, pt = base + C::kOffP + (c & 1) * kBlock;
+#pragma unroll 1
+            for (int r = 0; r < kChunk; r += 2) {
+              uint32_t u[2], v[2];
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(u[0]), "=r"(u[1]) : "r"(t_o + r) : "memory");
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(t_o + 64 + r) : "memory");
+              tc_wait_ld();
+              float e[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int at = r + k;
+                float part = __uint_as_float(v[k]);
+                if (again) {
+                  part = 0.f;
+                  for (int j = reverse ? at : low; j < (reverse ? high : at + 1); ++j)
+                    part = fmaf(lds16<BF16>(pt + at * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(at & 7)) << 4) + (j & 7) * 2),
+                                lds16<BF16>(ct + j * 128 + (((uint32_t)((d2 & 63) >> 3) ^ (uint32_t)(j & 7)) << 4) + (d2 & 7) * 2), part);
+                }
+                float f = row_w[at] * __uint_as_float(u[k]);
+                if constexpr (!BF16) f *= xs;
+                e[k] = BF16 ? f + part : fmaf(row_p[at], part, f);
+              }
+              store(r, e[0], e[1]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(b_o_empty + 8 * (c & 1));
+          mbar_arrive(b_empty + 8 * (c % C::kStages));
+        }
+      }
+    }
+
+    // ---- teardown ----
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+      if (threadIdx.x == 0) {
+        abort_grace();
+        atomicOr(&g_linear_status, kStatusTimeout);
+      }
+      __syncthreads();
+    }
+    if (warp == kWarpMma) {
+      tc_fence_after();
+      tmem_dealloc(tmem, 512);
+    }
+  }
+  // rows without a state, and rows of padding
+  if (states_only || (!q.bad && p.starts)) return;
+  const int64_t end = p.starts ? q.n : p.seq_len;
+  const int64_t from = q.bad || q.n < t0 ? t0 : q.n, upto = end < t0 + args.seg_len ? end : t0 + args.seg_len;
+  for (int64_t e = from * D2 + threadIdx.x; e < upto * D2; e += kThreads) {
+    const int64_t r = e / D2;
+    const float f = r < q.n ? __int_as_float(0x7fffffff) : 0.f;
+    const int64_t at = y0 + r * s.ys[2] + (e - r * D2);
+    if (s.y_f32) static_cast<float*>(s.y)[at] = f;
+    else if constexpr (BF16) static_cast<__nv_bfloat16*>(s.y)[at] = from_float<__nv_bfloat16>(f);
+    else static_cast<__half*>(s.y)[at] = from_float<__half>(f);
+  }
+}
+
+// The states before the segments, from what each adds, in place; and the state behind the last.  A thread has the same four elements of all
+// segments of a scan, sequence and head.
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args args, const int matrix) {
+  const Params& p = args.p;
+  const int parts = matrix / 1024;
+  const unsigned unit = blockIdx.x / (unsigned)parts;
+  const int which = args.first + (int)(unit % (unsigned)args.count), item = (int)(unit / (unsigned)args.count);
+  const int e = ((int)(blockIdx.x % (unsigned)parts) * 256 + threadIdx.x) * 4;
+  const Scan& s = p.scan[which];
+  const int b = item / p.heads, h = item - b * p.heads;
+  const Sequence q = sequence_of(p, b);
+  if (q.bad) return;
+  const float g = log2_decay(p.decay, h);
+  float* work = args.work + ((int64_t)which * p.batch * p.heads + item) * args.segments * matrix + e;
+  const int64_t state = (q.state * p.heads + h) * (int64_t)matrix;
+  const int d2 = s.d2, r = e / d2, c = e - r * d2;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s.x_first && q.state >= 0) {
+    if (s.x_transposed) {
+      const float* f = s.x_first + state + (int64_t)c * s.d1 + r;
+      x = make_float4(f[0], f[s.d1], f[2 * s.d1], f[3 * s.d1]);
+    } else {
+      x = *reinterpret_cast<const float4*>(s.x_first + state + e);
+    }
+  }
+  for (int i = 0; i < args.segments; ++i) {
+    const int64_t left = q.n - (int64_t)i * args.seg_len;
+    if (left <= 0) break;
+    const float keep = exp2f(g * (float)(left < args.seg_len ? left : args.seg_len));
+    float4* at = reinterpret_cast<float4*>(work + (int64_t)i * matrix);
+    const float4 t = *at;
+    *at = x;
+    x.x = fmaf(keep, x.x, t.x);
+    x.y = fmaf(keep, x.y, t.y);
+    x.z = fmaf(keep, x.z, t.z);
+    x.w = fmaf(keep, x.w, t.w);
+  }
+  if (s.x_last && q.state >= 0) {
+    if (s.x_transposed) {
+      float* f = s.x_last + state + (int64_t)c * s.d1 + r;
+      f[0] = x.x;
+      f[s.d1] = x.y;
+      f[2 * s.d1] = x.z;
+      f[3 * s.d1] = x.w;
+    } else {
+      *reinterpret_cast<float4*>(s.x_last + state + e) = x;
+    }
+  }
+}
+
+template <int D1, int D2, bool BF16>
+cudaError_t launch_t(const Maps& maps, Args& args, cudaStream_t stream, int* launches) {
+  using C = Cfg<D1, D2>;
+  auto kern = scan_sm100_kernel<D1, D2, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  const unsigned items = (unsigned)args.p.batch * args.p.heads, grid = items * (unsigned)args.count * (unsigned)args.segments;
+  if (args.segments > 1) {
+    args.states_only = 1;
+    kern<<<grid, kThreads, C::kSmem, stream>>>(maps, args);
+    args.states_only = 0;
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    join_kernel<<<items * (unsigned)args.count * (D1 * D2 / 1024), 256, 0, stream>>>(args, D1 * D2);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    *launches += 2;
+  }
+  kern<<<grid, kThreads, C::kSmem, stream>>>(maps, args);
+  ++*launches;
+  return cudaGetLastError();
+}
+
+template <bool BF16>
+cudaError_t launch_sizes(const Maps& maps, Args& args, cudaStream_t stream, int* launches) {
+  const Scan& s = args.p.scan[args.first];
+  if (s.d1 == 128) return s.d2 == 128 ? launch_t<128, 128, BF16>(maps, args, stream, launches) : launch_t<128, 64, BF16>(maps, args, stream, launches);
+  return s.d2 == 128 ? launch_t<64, 128, BF16>(maps, args, stream, launches) : launch_t<64, 64, BF16>(maps, args, stream, launches);
+}
+
+// Rows of a segment.
+int segments_of(const Params& p, int num_sms) {
+  (void)p;
+  (void)num_sms;
+  return 1;
+}
+
+}  // namespace
+
+int32_t* sm100_status() {
+  void* addr = nullptr;
+  if (cudaGetSymbolAddress(&addr, g_linear_status) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  return static_cast<int32_t*>(addr);
+}
+
+bool scan_sm100_supported(const Params& p) {
+  if (p.dtype == AIDN_F32 || (p.starts && p.tokens == 0)) return false;
+  if ((int64_t)p.batch * p.heads > (1 << 24)) return false;
+  const int64_t rows = p.starts ? p.tokens : p.seq_len;
+  for (int i = 0; i < p.scans; ++i) {
+    const Scan& s = p.scan[i];
+    if ((s.d1 != 64 && s.d1 != 128) || (s.d2 != 64 && s.d2 != 128)) return false;
+    const void* ptr[3] = {s.a, s.b, s.c};
+    const int64_t* stride[3] = {s.as, s.bs, s.cs};
+    const int group[3] = {s.a_group, s.b_group, s.c_group};
+    for (int t = 0; t < 3; ++t) {
+      if ((uintptr_t)ptr[t] % 16 != 0) return false;
+      const int64_t extent[3] = {p.starts ? 1 : p.batch, p.heads / group[t], rows};
+      for (int d = 0; d < 3; ++d)
+        if (extent[d] > 1 && (stride[t][d] <= 0 || stride[t][d] % 8 != 0 || stride[t][d] >= (1ll << 38))) return false;
+    }
+    if (!s.y_f32 && ((uintptr_t)s.y % 4 != 0 || s.ys[0] % 2 != 0 || s.ys[1] % 2 != 0 || s.ys[2] % 2 != 0)) return false;
+  }
+  return true;
+}
+
+int64_t scan_sm100_bytes(const Params& p, int num_sms) {
+  const int n = segments_of(p, num_sms);
+  return n == 1 ? 0 : (int64_t)p.scans * p.batch * p.heads * n * p.scan[0].d1 * p.scan[0].d2 * 4;
+}
+
+cudaError_t launch_scan_sm100(const Params& p, int num_sms, float* work, int64_t work_bytes, bool expire, cudaStream_t stream, int* launches) {
+  cudaError_t e = tmap::resolve_encode();
+  if (e != cudaSuccess) return e;
+  const bool bf16 = p.dtype == AIDN_BF16;
+  const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int64_t rows = p.starts ? p.tokens : p.seq_len, batch = p.starts ? 1 : p.batch;
+  Maps maps;
+  Args args;
+  args.p = p;
+  // one map for each tensor (of the three scans' nine operands, four are different)
+  int known = 0;
+  struct Key {
+    const void* ptr;
+    int64_t stride[3];
+    int size, group;
+  } made[4];
+  auto map_of = [&](const void* ptr, const int64_t* stride, int size, int group) {
+    for (int i = 0; i < known; ++i)
+      if (made[i].ptr == ptr && made[i].size == size && made[i].group == group && made[i].stride[0] == stride[0] && made[i].stride[1] == stride[1] &&
+          made[i].stride[2] == stride[2])
+        return i;
+    if (known == 4) return -1;
+    int64_t st[3] = {stride[0], stride[1], rows > 1 ? stride[2] : size};
+    if (!tmap::encode_bhsd(&maps.t[known], dt, 2, CU_TENSOR_MAP_SWIZZLE_128B, ptr, size, rows, p.heads / group, batch, st, 64, kChunk)) return -1;
+    made[known] = {ptr, {stride[0], stride[1], stride[2]}, size, group};
+    return known++;
+  };
+  for (int i = 0; i < p.scans; ++i) {
+    const Scan& s = p.scan[i];
+    args.ia[i] = map_of(s.a, s.as, s.d1, s.a_group);
+    args.ib[i] = map_of(s.b, s.bs, s.d1, s.b_group);
+    args.ic[i] = map_of(s.c, s.cs, s.d2, s.c_group);
+    if (args.ia[i] < 0 || args.ib[i] < 0 || args.ic[i] < 0) return cudaErrorInvalidValue;
+  }
+  args.segments = work && work_bytes >= scan_sm100_bytes(p, num_sms) ? segments_of(p, num_sms) : 1;
+  const int64_t per = (p.seq_len + args.segments - 1) / args.segments;
+  args.seg_len = (int)((per + kChunk - 1) / kChunk * kChunk < 0x7fffffc0ll ? (per + kChunk - 1) / kChunk * kChunk : 0x7fffffc0ll);
+  args.states_only = 0;
+  args.work = work;
+  args.wait_ns = expire ? 20000000ull : kWaitBudgetNs;
+  args.withhold = expire ? 1 : 0;
+  // scans of the same sizes share a launch
+  for (args.first = 0; args.first < p.scans && e == cudaSuccess; args.first += args.count) {
+    args.count = 1;
+    while (args.first + args.count < p.scans && p.scan[args.first + args.count].d1 == p.scan[args.first].d1 &&
+           p.scan[args.first + args.count].d2 == p.scan[args.first].d2)
+      ++args.count;
+    e = bf16 ? launch_sizes<true>(maps, args, stream, launches) : launch_sizes<false>(maps, args, stream, launches);
+  }
+  return e;
+}
+
+}  // namespace lin
+}  // namespace aidn

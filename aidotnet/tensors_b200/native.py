@@ -37,7 +37,7 @@ EXPORTS = (
     "aidn_mha_workspace_bytes", "aidn_peer_export", "aidn_peer_open", "aidn_peer_close",
     "aidn_kv8_append", "aidn_sdpa_kv8_workspace_bytes", "aidn_sdpa_launch_kv8",
     "aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_workspace_bytes", "aidn_linear_attention_backward",
-    "aidn_linear_attention_backward_workspace_bytes", "aidn_linear_attention_step",
+    "aidn_linear_attention_backward_workspace_bytes", "aidn_linear_attention_poll", "aidn_linear_attention_step",
     "aidn_sdpa_debug_set",   # include/aidn_sdpa_debug.h
 )
 
@@ -269,7 +269,9 @@ def load() -> ctypes.CDLL:
     lib.aidn_linear_attention.argtypes = [ctypes.POINTER(LinearArgs), ctypes.c_void_p]
     lib.aidn_linear_attention_backward.argtypes = [ctypes.POINTER(LinearBwdArgs), ctypes.c_void_p]
     lib.aidn_linear_attention_step.argtypes = [ctypes.POINTER(LinearStepArgs), ctypes.c_void_p]
-    for name in ("aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_backward", "aidn_linear_attention_step"):
+    lib.aidn_linear_attention_poll.argtypes = [ctypes.c_void_p]
+    for name in ("aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_backward", "aidn_linear_attention_step",
+                 "aidn_linear_attention_poll"):
         getattr(lib, name).restype = ctypes.c_int
     for name in ("aidn_linear_attention_workspace_bytes", "aidn_linear_attention_backward_workspace_bytes"):
         getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.c_char_p], ctypes.c_int64   # a packed block
@@ -685,3 +687,8 @@ def linear_attention_step(*, q: int, k: int, v: int, out: int, states: int, batc
         kv_heads, key_dim, value_dim, dtype, num_slots, scale), stream)
     if status != OK:
         raise AidnError(status, last_error())
+
+
+def linear_attention_poll(stream: int) -> None:
+    """Synchronises ``stream`` and raises if a linear attention call gave up a bounded wait since the last report."""
+    check(load().aidn_linear_attention_poll(ctypes.c_void_p(stream)))

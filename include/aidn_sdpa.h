@@ -457,6 +457,10 @@ typedef struct {
 AIDN_API int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linear_bwd_args* args);
 AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, void* cu_stream);
 
+/* Synchronises `cu_stream` and returns AIDN_ETIMEOUT if one of these calls gave up a bounded wait since the last report (its outputs are then
+ * not to be used), AIDN_ECUDA on a CUDA error, else AIDN_OK.  They have no handle: the word is one per CUDA context, and reporting it clears it. */
+AIDN_API int aidn_linear_attention_poll(void* cu_stream);
+
 /* One token of each of `batch` sequences against states that stay where they are: state state_slots[b] (NULL: b) is updated in place.  A
  * negative slot is a row of padding: its output is zeros and no state is touched.  Other slots as above.  One launch. */
 typedef struct {

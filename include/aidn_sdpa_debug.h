@@ -18,6 +18,7 @@ extern "C" {
  *         is ignored.
  *         With a null handle: the calling thread's next aidn_qkv_rope_cache does so, and aidn_qkv_rope_poll reports it
  *         (mode 0 takes that back).
+ * mode 5: with a null handle only: the same for the thread's next aidn_linear_attention or its backward and aidn_linear_attention_poll.
  * modes 1, 2 and 4 exist only in development builds of the library (compiled with -DAIDN_PREFILL_TRACE=1): value tap,
  *         per-work-item timeline and per-step clock stamps of the prefill kernel, written to `buf`.  The shipped build
  *         ignores them. */

@@ -223,9 +223,13 @@ def test_forward_magnitudes(backend, dtype, size, dim):
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("dim", [64, 128, 48])
 def test_what_follows_a_row_does_not_reach_it(backend, dtype, dim):
-    """NaN and infinities in the last rows of keys, values and queries: the rows before them are what they were, bit for bit."""
+    """NaN and infinities in the last rows of keys, values and queries: the rows before them are what they were.  (A kernel may sum a row that shares
+    a tile with such a value in another order.  Two fp32 sums of the same 64 products are each off by 64 * 2^-24 of their terms, and with the
+    factors behind them differ by 2^-16 A at most; each is rounded once, by u of it.)"""
     c = Case(dtype, [140], 2, 2, dim, dim, "head", seed=6)
     clean, _ = run_forward(backend, c)
+    top, _ = recurrence(*(x[0].double().abs() for x in (c.q, c.k, c.v)), c.log_decay(), dim ** -0.5)
+    most = 2 * torch.finfo(TORCH_DT[dtype]).eps / 2 * clean.double().abs() + 2.0 ** -16 * top
     for at in (139, 100, 64, 3):
         for bad in (float("nan"), float("inf")):
             q, k, v = c.q.clone(), c.k.clone(), c.v.clone()
@@ -236,7 +240,7 @@ def test_what_follows_a_row_does_not_reach_it(backend, dtype, dim):
             c.q, c.k, c.v = q, k, v
             out, _ = run_forward(backend, c)
             c.q, c.k, c.v = keep
-            assert torch.equal(out[:, :, :at], clean[:, :, :at]), (at, bad)
+            assert bool(((out.double() - clean.double()).abs() <= most)[:, :, :at].all()), (at, bad)
             assert bool(torch.isnan(out[:, :, at]).any())
 
 
@@ -251,7 +255,9 @@ def test_a_value_that_is_not_finite_stays_in_its_column(backend):
             hit = torch.zeros_like(out, dtype=torch.bool)
             hit[0, 0, 70:, 5] = True
             assert torch.equal(torch.isnan(out), hit)
-            assert torch.equal(out[~hit], clean[~hit])
+            top, _ = recurrence(*(x[0].double().abs().nan_to_num() for x in (c.q, c.k, c.v)), c.log_decay(), dim ** -0.5)
+            most = 2 * torch.finfo(TORCH_DT[dtype]).eps / 2 * clean.double().abs() + 2.0 ** -16 * top   # (as above)
+            assert bool(((out.double() - clean.double()).abs() <= most)[~hit].all())
 
 
 def test_decay_above_zero_or_nan_shows(backend):
@@ -513,6 +519,22 @@ def test_layer_with_rotated_heads(backend):
     grads = torch.autograd.grad((ref * c.do[0].double().transpose(0, 1)).sum(), (x, y, v))
     for a, b in zip((out, gq, gk, got["dv"]), (ref.detach(), *grads)):
         assert float((a[0].double().transpose(0, 1) - b).norm() / b.norm()) <= 1e-5
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_waits_that_run_out_are_reported(backend, dim):
+    """The kernel with bounded waits, its loads withheld: it ends, says so once, and the next call is right."""
+    c = Case("bf16", [300], 2, 2, dim, dim, "head", seed=17)
+    clean, _ = run_forward(backend, c)
+    stream = torch.cuda.current_stream().cuda_stream
+    N.linear_attention_poll(stream)
+    assert N.load().aidn_sdpa_debug_set(None, None, 5) == N.OK
+    run_forward(backend, c)
+    with pytest.raises(N.AidnError) as e:
+        N.linear_attention_poll(stream)
+    assert e.value.status == N.ETIMEOUT
+    N.linear_attention_poll(stream)
+    assert torch.equal(run_forward(backend, c)[0], clean)
 
 
 @pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("f32", 40)])
