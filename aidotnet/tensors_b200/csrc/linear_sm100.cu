@@ -26,6 +26,8 @@
 // Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "linear.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_map.hpp"
@@ -50,12 +52,13 @@ struct Cfg {
   static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
   static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
   static constexpr int kOffP = kStages * kStageBytes;             // two buffers
-  static constexpr int kOffBt = kOffP + 2 * kBlock;               // the two terms of B~
-  static constexpr int kOffTab = kOffBt + 2 * kN1 * kBlock;
-  // tables: powers [66], row weights [64], row scales of P [2][64], lane scales of X [4][128], exchange of maxima [2][2][128]
-  static constexpr int kTabPower = 0, kTabRow = 68, kTabP = 132, kTabX = 260, kTabMax = 772, kTabFloats = 1284;
+  static constexpr int kOffBt = kOffP + 2 * kBlock;               // up to three terms of B~
+  static constexpr int kOffTab = kOffBt + 3 * kN1 * kBlock;
+  // tables: powers [65], weights of the scores by distance [127], of the state's rows [64]; row scales of P [2][64], lane scales of
+  // X [4][128], exchange of maxima [2][2][128], terms of B~'s weights in pairs [65][4]
+  static constexpr int kTabPower = 0, kTabScore = 68, kTabRow = 196, kTabP = 260, kTabX = 388, kTabMax = 900, kTabW = 1412, kTabFloats = 1672;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
-  static constexpr int kBars = 2 * kStages + 17;
+  static constexpr int kBars = 2 * kStages + 16;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = kOffMisc + 16 + 1024;
   // tensor memory columns
@@ -73,6 +76,7 @@ struct Args {
   int32_t first, count;          // scans of this launch
   int32_t segments, seg_len;     // seg_len: a multiple of kChunk
   int32_t states_only;
+  int32_t terms;                 // of B~: 2, or 3 for bf16 where states go out
   float* work;                   // [scan][sequence, head][segment][D1][D2]
   uint64_t wait_ns;
   int32_t withhold;              // test hook: no loads, so that the waits run out
@@ -82,6 +86,21 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
+}
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf16x2_sub(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
@@ -131,8 +150,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   const uint32_t b_p_full = b_s_full + 16;                    // [2]
   const uint32_t b_o_full = b_s_full + 32, b_o_empty = b_s_full + 48;   // [2] each
   const uint32_t b_bt_full = b_s_full + 64, b_t_full = b_s_full + 72, b_t_empty = b_s_full + 80;
-  const uint32_t b_x_full = b_s_full + 88, b_x_empty = b_s_full + 96;
-  const uint32_t b_max = b_s_full + 104;                      // [4]: of the two warps that share lanes
+  const uint32_t b_x_full = b_s_full + 88;
+  const uint32_t b_max = b_s_full + 96;                      // [4]: of the two warps that share lanes
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(gen + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
 
@@ -176,15 +195,29 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       mbar_init(b_t_full, 1);
       mbar_init(b_t_empty, 8);
       mbar_init(b_x_full, 8);
-      mbar_init(b_x_empty, 1);
       for (int i = 0; i < 4; ++i) mbar_init(b_max + 8 * i, 2);
       fence_mbar_init();
     }
     const float g = log2_decay(p.decay, h);
-    if (threadIdx.x < 65) table[C::kTabPower + threadIdx.x] = exp2f(g * threadIdx.x);
+    if (threadIdx.x < 65) {
+      const float w = exp2f(g * threadIdx.x);
+      table[C::kTabPower + threadIdx.x] = w;
+      if constexpr (BF16) {
+        float left = w * s.key_scale;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t t = pack2<true>(left, left);
+          table[C::kTabW + threadIdx.x * 4 + i] = __uint_as_float(t);
+          left -= __uint_as_float(t & 0xffff0000u);
+        }
+      }
+    }
     else if (threadIdx.x >= 96 && threadIdx.x < 160) {
       const int r = threadIdx.x - 96;
       table[C::kTabRow + r] = s.row_scale * exp2f(g * ((reverse ? kChunk - 1 - r : r) + s.lag));
+    } else if (threadIdx.x >= 256 && threadIdx.x < 383) {   // at 63 + (i - j); zeros where j follows i
+      const int d = reverse ? 63 - (int)(threadIdx.x - 256) : (int)(threadIdx.x - 256) - 63;
+      table[C::kTabScore + threadIdx.x - 256] = d >= 0 ? p.scale * exp2f(g * d) : 0.f;
     }
     if (warp == kWarpMma) {
       tmem_alloc(smem_u32(tmem_ptr), 512);
@@ -233,17 +266,18 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       constexpr uint32_t idesc_x = make_idesc(128, 64, BF16, false);                  // X^T from tensor memory, A along its rows
       constexpr uint32_t idesc_p = make_idesc(128, 64, BF16, false) | kTransposeA;    // C^T, P along its rows
       constexpr uint32_t idesc_t = make_idesc(128, D1, BF16, true) | kTransposeA;     // C^T, B~ across its rows
-      auto stage = [&](int c) { return base + (uint32_t)((c % C::kStages) * C::kStageBytes); };
+      // (a descriptor's start address is counted in 16 bytes; what is added to it stays within its field)
+      const uint64_t rows_desc = make_smem_desc(base, 16, 1024), cols_desc = make_smem_desc(base, kBlock, 1024);
+      auto stage = [&](int c) { return (uint64_t)((c % C::kStages) * (C::kStageBytes >> 4)); };
+      auto row_step = [](int k) { return (uint64_t)(((k / 4) * kBlock + (k % 4) * 32) >> 4); };   // 16 elements along a row
       auto scores = [&](int c) {
         if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
         if (!wait(b_s_empty, (uint32_t)(c & 1) ^ 1u)) return false;
         tc_fence_after();
         if (leader) {
+          const uint64_t ad = rows_desc + stage(c), bd = ad + (C::kOffB >> 4);
 #pragma unroll
-          for (int k = 0; k < D1 / 16; ++k) {
-            const uint32_t off = (uint32_t)((k / 4) * kBlock + (k % 4) * 32);
-            mma_ss(tmem + C::kColS, make_smem_desc(stage(c) + off, 16, 1024), make_smem_desc(stage(c) + C::kOffB + off, 16, 1024), idesc_s, k > 0);
-          }
+          for (int k = 0; k < D1 / 16; ++k) mma_ss(tmem + C::kColS, ad + row_step(k), bd + row_step(k), idesc_s, k > 0);
           tc_commit(b_s_full);
         }
         __syncwarp();
@@ -251,60 +285,59 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       };
       bool ok = states_only || chunks == 0 || scores(0);
       for (int c = 0; c < chunks && ok; ++c) {
-        if (!states_only && c + 1 < chunks && !(ok = scores(c + 1))) break;
-        if (states_only && !(ok = wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1)))) break;
-        const uint32_t ct = stage(c) + C::kOffC;
+        const uint64_t ct = cols_desc + stage(c) + (C::kOffC >> 4);
+        const uint32_t o = tmem + C::kColO + (c & 1) * 128;
+        if (states_only) {
+          if (!(ok = wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1)))) break;
+        } else {
+          // in front of T, which the state waits for: the state's columns are free as soon as T is there
+          if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
+          if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < D1 / 16; ++k) mma_ts(o, tmem + C::kColX + k * 8, rows_desc + stage(c) + row_step(k), idesc_x, k > 0);
+          }
+          __syncwarp();
+        }
         if (!(ok = wait(b_bt_full, (uint32_t)(c & 1)))) break;
         if (!(ok = wait(b_t_empty, (uint32_t)(c & 1) ^ 1u))) break;
         tc_fence_after();
         if (leader) {
-#pragma unroll
-          for (int term = 1; term >= 0; --term)   // the second term first: fp16 holds it 2^11 times as large
+          for (int term = args.terms - 1; term >= 0; --term)   // the smallest first (fp16 holds its second 2^11 times as large)
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k) {
-              const uint64_t cd = make_smem_desc(ct + k * 2048, kBlock, 1024);
-              const uint64_t bd = make_smem_desc(base + C::kOffBt + term * C::kN1 * kBlock + k * 2048, kBlock, 1024);
+              const uint64_t cd = ct + k * (2048 >> 4), bd = cols_desc + (uint64_t)((C::kOffBt + term * C::kN1 * kBlock + k * 2048) >> 4);
               if (!BF16 && term == 0 && k == 0) mma_ss_down11(tmem + C::kColT, cd, bd, idesc_t);
-              else mma_ss(tmem + C::kColT, cd, bd, idesc_t, term == 0 || k > 0);
+              else mma_ss(tmem + C::kColT, cd, bd, idesc_t, term < args.terms - 1 || k > 0);
             }
           tc_commit(b_t_full);
           if (states_only) tc_commit(b_empty + 8 * (c % C::kStages));
         }
         __syncwarp();
         if (states_only) continue;
-        const uint32_t o = tmem + C::kColO + (c & 1) * 128;
-        if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
-        if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
-        tc_fence_after();
-        if (leader) {
-#pragma unroll
-          for (int k = 0; k < D1 / 16; ++k)
-            mma_ts(o, tmem + C::kColX + k * 8, make_smem_desc(stage(c) + (uint32_t)((k / 4) * kBlock + (k % 4) * 32), 16, 1024), idesc_x, k > 0);
-          tc_commit(b_x_empty);
-        }
-        __syncwarp();
         if (!(ok = wait(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
         tc_fence_after();
         if (leader) {
 #pragma unroll
           for (int k = 0; k < kChunk / 16; ++k)
-            mma_ss(o + 64, make_smem_desc(ct + k * 2048, kBlock, 1024), make_smem_desc(base + C::kOffP + (c & 1) * kBlock + k * 32, 16, 1024), idesc_p, k > 0);
+            mma_ss(o + 64, ct + k * (2048 >> 4), rows_desc + (uint64_t)((C::kOffP + (c & 1) * kBlock + k * 32) >> 4), idesc_p, k > 0);
           tc_commit(b_o_full + 8 * (c & 1));
           tc_commit(b_empty + 8 * (c % C::kStages));
         }
         __syncwarp();
+        if (c + 1 < chunks && !(ok = scores(c + 1))) break;
       }
     } else if (warp < kWarpLoad) {
       // ---- P ----
       if (!states_only && chunks > 0) {
         const int i = warp * 32 + lane;
         const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16) + C::kColS;
-        float w[kChunk];   // of the row's scores; exactly zero behind the row
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const int d = reverse ? j - i : i - j;
-          w[j] = d >= 0 ? p.scale * power[d < 0 ? 0 : d] : 0.f;
-        }
+        const float* weight = table + C::kTabScore + 63 + i;   // of column j at -j; exactly zero behind the row
+        auto weighted = [&](uint32_t v, int j) {
+          const float w = weight[-j];
+          return w == 0.f ? 0.f : __uint_as_float(v) * w;   // (whatever stands there)
+        };
         for (int c = 0; c < chunks; ++c) {
           if (!wait(b_s_full, (uint32_t)(c & 1))) break;
           if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
@@ -312,32 +345,31 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           float to = 1.f;
           if constexpr (!BF16) {
             float most = 0.f, back;
-#pragma unroll
-            for (int j0 = 0; j0 < kChunk; j0 += 32) {
-              uint32_t r[32];
-              tmem_ld32(t_s + j0, r);
+#pragma unroll 1
+            for (int j0 = 0; j0 < kChunk; j0 += 16) {
+              uint32_t r[16];
+              tmem_ld16(t_s + j0, r);
               tc_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) most = fmaxf(most, w[j0 + j] == 0.f ? 0.f : fabsf(__uint_as_float(r[j]) * w[j0 + j]));
+              for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(weighted(r[j], j0 + j)));
             }
             scale_of(most, to, back);
             table[C::kTabP + (c & 1) * 64 + i] = back;
           }
           const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
-#pragma unroll
-          for (int j0 = 0; j0 < kChunk; j0 += 32) {
-            uint32_t r[32], v[16];
-            tmem_ld32(t_s + j0, r);
+#pragma unroll 1   // (code that is small enough to stay in the instruction cache: unrolled over the row it took 7400 cycles a chunk)
+          for (int j0 = 0; j0 < kChunk; j0 += 16) {
+            uint32_t r[16], v[8];
+            tmem_ld16(t_s + j0, r);
             tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float x = w[j0 + j] == 0.f ? 0.f : __uint_as_float(r[j]) * w[j0 + j];
-              float y = w[j0 + j + 1] == 0.f ? 0.f : __uint_as_float(r[j + 1]) * w[j0 + j + 1];
+            for (int j = 0; j < 16; j += 2) {
+              float x = weighted(r[j], j0 + j), y = weighted(r[j + 1], j0 + j + 1);
               if constexpr (!BF16) x *= to, y *= to;
               v[j / 2] = pack2<BF16>(x, y);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 2; ++u)
               st_shared_v4(row + (((uint32_t)(j0 / 8 + u) ^ (uint32_t)(i & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
           }
           fence_proxy_async_smem();
@@ -357,6 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const bool owner = d2 < D2;                // (with 64 columns, the lanes above hold nothing; whole warps)
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const int64_t matrix = (int64_t)D1 * D2;
+      const int lag = s.lag;
+      const float key_scale = s.key_scale;   // in B~'s weights, or behind the product where they might leave fp16's range
       float x[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) x[i] = 0.f;
@@ -365,8 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         const float* from = work ? work : (s.x_first && q.state >= 0 ? s.x_first + (q.state * p.heads + h) * matrix : nullptr);
         if (from) {
           const bool turned = !work && s.x_transposed;
+          const int step = turned ? 1 : D2;
+          from += turned ? d2 * D1 + d1 : d1 * D2 + d2;
 #pragma unroll
-          for (int i = 0; i < kCols; ++i) x[i] = from[turned ? (int64_t)d2 * D1 + d1 + i : (int64_t)(d1 + i) * D2 + d2];
+          for (int i = 0; i < kCols; ++i) x[i] = from[i * step];
         }
       }
       // X^T of chunk c to tensor memory
@@ -403,29 +439,54 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
         const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes);
         if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) break;
-#pragma unroll
-        for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
-          const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
-          uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-          if (j < n) {
-            const float w = power[n - s.lag - j];
+        if constexpr (BF16) {
+          // b w as terms of 16 bits by packed multiply-adds, with w = w0 + w1 + w2 of 8 bits each: b w0 has 16 bits, so that what its rounding leaves is
+          // exact, and so on.  (In fp32, with conversions there and back, it took three times the instructions.)
+#pragma unroll 2
+          for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
+            const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
             const uint4 v = lds128(st + C::kOffB + u * 16);
+            const uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabW + (j < n ? n - lag - j : 0) * 4);
             const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-            uint32_t a[4], e[4];
+            uint32_t a[4], e[4], f[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              float2 f = unpack2<BF16>(in[k]);
-              f.x *= w;
-              f.y *= w;
-              a[k] = pack2<BF16>(f.x, f.y);
-              const float2 t = unpack2<BF16>(a[k]);
-              e[k] = BF16 ? pack2<BF16>(f.x - t.x, f.y - t.y) : pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+              const uint32_t b2 = j < n ? in[k] : 0u;   // (whatever stands in rows that are not there)
+              a[k] = bf16x2_mul(b2, w.x);
+              const uint32_t rest = bf16x2_fma(b2, w.x, a[k] ^ 0x80008000u);
+              e[k] = bf16x2_fma(b2, w.y, rest);
+              if (args.terms == 3) f[k] = bf16x2_fma(b2, w.z, bf16x2_fma(b2, w.y, bf16x2_sub(rest, e[k])));
             }
-            hi = make_uint4(a[0], a[1], a[2], a[3]);
-            lo = make_uint4(e[0], e[1], e[2], e[3]);
+            const uint32_t to = base + C::kOffBt + u * 16;
+            st_shared_v4(to, a[0], a[1], a[2], a[3]);
+            st_shared_v4(to + C::kN1 * kBlock, e[0], e[1], e[2], e[3]);
+            if (args.terms == 3) st_shared_v4(to + 2 * C::kN1 * kBlock, f[0], f[1], f[2], f[3]);
           }
-          st_shared_v4(base + C::kOffBt + u * 16, hi.x, hi.y, hi.z, hi.w);
-          st_shared_v4(base + C::kOffBt + C::kN1 * kBlock + u * 16, lo.x, lo.y, lo.z, lo.w);
+        } else {
+#pragma unroll 2
+          for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
+            const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (j < n) {
+              const float w = power[n - lag - j];
+              const uint4 v = lds128(st + C::kOffB + u * 16);
+              const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+              uint32_t a[4], e[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float2 f = unpack2<BF16>(in[k]);
+                f.x *= w;
+                f.y *= w;
+                a[k] = pack2<BF16>(f.x, f.y);
+                const float2 t = unpack2<BF16>(a[k]);
+                e[k] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+              }
+              hi = make_uint4(a[0], a[1], a[2], a[3]);
+              lo = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+            st_shared_v4(base + C::kOffBt + u * 16, hi.x, hi.y, hi.z, hi.w);
+            st_shared_v4(base + C::kOffBt + C::kN1 * kBlock + u * 16, lo.x, lo.y, lo.z, lo.w);
+          }
         }
         if (n < kChunk)
           for (int u = tid; u < C::kN2 * kBlock / 16; u += 256) {
@@ -444,25 +505,23 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             tmem_ld32(tmem + lanes + C::kColT + d1 + i0, r);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(keep, x[i0 + i], s.key_scale * __uint_as_float(r[i]));
+            for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(keep, x[i0 + i], BF16 ? __uint_as_float(r[i]) : key_scale * __uint_as_float(r[i]));
           }
         }
         tc_fence_before();
         arrive(b_t_empty);
         if (!states_only && c + 1 < chunks) {
-          if (!wait(b_x_empty, (uint32_t)(c & 1))) break;
-          tc_fence_after();
           ok = put_state(c + 1);
         }
       }
       if (owner && !*abort_flag) {
-        if (states_only) {
+        float* to = states_only ? work : args.segments == 1 && s.x_last && q.state >= 0 ? s.x_last + (q.state * p.heads + h) * matrix : nullptr;
+        if (to) {
+          const bool turned = !states_only && s.x_transposed;
+          const int step = turned ? 1 : D2;
+          to += turned ? d2 * D1 + d1 : d1 * D2 + d2;
 #pragma unroll
-          for (int i = 0; i < kCols; ++i) work[(int64_t)(d1 + i) * D2 + d2] = x[i];
-        } else if (args.segments == 1 && s.x_last && q.state >= 0) {
-          float* to = s.x_last + (q.state * p.heads + h) * matrix;
-#pragma unroll
-          for (int i = 0; i < kCols; ++i) to[s.x_transposed ? (int64_t)d2 * D1 + d1 + i : (int64_t)(d1 + i) * D2 + d2] = x[i];
+          for (int i = 0; i < kCols; ++i) to[i * step] = x[i];
         }
       }
     } else if (!states_only) {
@@ -472,6 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const bool owner = quarter * 32 < D2;
       uint16_t* y16 = static_cast<uint16_t*>(s.y) + y0;
       float* y32 = static_cast<float*>(s.y) + y0;
+      const int64_t pitch = s.ys[2];
+      const bool y_f32 = s.y_f32 != 0;
+      const int odd = lane & 1;
       for (int c = 0; c < chunks; ++c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
         const int low = reverse ? kChunk - n : 0, high = reverse ? kChunk : n;   // the tile's rows
@@ -484,39 +546,50 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           const float* row_w = table + C::kTabRow;
           const float* row_p = table + C::kTabP + (c & 1) * 64;
           float probe = 0.f;   // NaN as soon as a value of the row part is not finite
-          auto store = [&](int r, float a, float z) {   // rows r and r + 1
-            if (s.y_f32) {
-              if (r >= low && r < high) y32[(int64_t)(token + r) * s.ys[2] + d2] = a;
-              if (r + 1 >= low && r + 1 < high) y32[(int64_t)(token + r + 1) * s.ys[2] + d2] = z;
+          auto value = [&](float state, float part, float w, float ps) { return BF16 ? fmaf(w, state, part) : fmaf(ps, part, w * xs * state); };
+          // rows r .. r + N - 1: 16-bit values in pairs of columns, even lanes of the even rows and odd lanes of the odd ones.  (All exchanges, then
+          // all stores, none behind a branch: one row pair after the other took 100 cycles each.)
+          auto store = [&](int r, const float* e, auto count) {
+            constexpr int N = decltype(count)::value;
+            if (y_f32) {
+#pragma unroll
+              for (int i = 0; i < N; ++i)
+                if (r + i >= low && r + i < high) y32[(int64_t)(token + r + i) * pitch + d2] = e[i];
             } else {
-              // even lanes take row r, odd ones row r + 1, of two columns each
-              const bool odd = lane & 1;
-              const float got = __shfl_xor_sync(0xffffffffu, odd ? a : z, 1);
-              const int mine = r + (odd ? 1 : 0);
-              if (mine >= low && mine < high)
-                *reinterpret_cast<uint32_t*>(y16 + (int64_t)(token + mine) * s.ys[2] + (d2 & ~1)) = odd ? pack2<BF16>(got, z) : pack2<BF16>(a, got);
+              uint32_t v[N / 2];
+#pragma unroll
+              for (int i = 0; i < N; i += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, odd ? e[i] : e[i + 1], 1);
+                v[i / 2] = pack2<BF16>(odd ? got : e[i], odd ? e[i + 1] : got);
+              }
+              uint16_t* at = y16 + (int64_t)(token + r + odd) * pitch + (d2 & ~1);
+#pragma unroll
+              for (int i = 0; i < N; i += 2) {
+                if (r + i + odd >= low && r + i + odd < high) *reinterpret_cast<uint32_t*>(at) = v[i / 2];
+                at += 2 * pitch;
+              }
             }
           };
+#pragma unroll 1
+          for (int r0 = 0; r0 < kChunk; r0 += 16) {
+            uint32_t u[16], v[16];
+            tmem_ld16(t_o + r0, u);
+            tmem_ld16(t_o + 64 + r0, v);
+            float w[16], ps[16];
 #pragma unroll
-          for (int r0 = 0; r0 < kChunk; r0 += 32) {
-            uint32_t u[32], v[32];
-            tmem_ld32(t_o + r0, u);
-            tmem_ld32(t_o + 64 + r0, v);
-            tc_wait_ld();
-#pragma unroll
-            for (int r = 0; r < 32; r += 2) {
-              float e[2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int at = r0 + r + k;
-                const float part = __uint_as_float(v[r + k]);
-                if (n == kChunk || (at >= low && at < high)) probe = fmaf(part, 0.f, probe);
-                float f = row_w[at] * __uint_as_float(u[r + k]);
-                if constexpr (!BF16) f *= xs;
-                e[k] = BF16 ? f + part : fmaf(row_p[at], part, f);
-              }
-              store(r0 + r, e[0], e[1]);
+            for (int r = 0; r < 16; r += 4) {
+              *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(row_w + r0 + r);
+              if constexpr (!BF16) *reinterpret_cast<float4*>(ps + r) = *reinterpret_cast<const float4*>(row_p + r0 + r);
             }
+            tc_wait_ld();
+            float e[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float part = __uint_as_float(v[r]);
+              probe = fmaf(part, 0.f, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
+              e[r] = value(__uint_as_float(u[r]), part, w[r], BF16 ? 1.f : ps[r]);
+            }
+            store(r0, e, std::integral_constant<int, 16>());
           }
           const bool again = probe != probe;
           // (the tile is there since before the products; this thread has to see that for itself)
@@ -539,11 +612,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
                     part = fmaf(lds16<BF16>(pt + at * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(at & 7)) << 4) + (j & 7) * 2),
                                 lds16<BF16>(ct + j * 128 + (((uint32_t)((d2 & 63) >> 3) ^ (uint32_t)(j & 7)) << 4) + (d2 & 7) * 2), part);
                 }
-                float f = row_w[at] * __uint_as_float(u[k]);
-                if constexpr (!BF16) f *= xs;
-                e[k] = BF16 ? f + part : fmaf(row_p[at], part, f);
+                e[k] = value(__uint_as_float(u[k]), part, row_w[at], BF16 ? 1.f : row_p[at]);
               }
-              store(r, e[0], e[1]);
+              store(r, e, std::integral_constant<int, 2>());
             }
           }
         }
@@ -748,6 +819,11 @@ cudaError_t launch_scan_sm100(const Params& p, int num_sms, float* work, int64_t
   const int64_t per = (p.seq_len + args.segments - 1) / args.segments;
   args.seg_len = (int)((per + kChunk - 1) / kChunk * kChunk < 0x7fffffc0ll ? (per + kChunk - 1) / kChunk * kChunk : 0x7fffffc0ll);
   args.states_only = 0;
+  // two bf16 terms leave 2^-17 of a key: enough for outputs of 8 bits, not for states that go out in 32
+  args.terms = 2;
+  if (bf16)
+    for (int i = 0; i < p.scans; ++i)
+      if (p.scan[i].x_last) args.terms = 3;
   args.work = work;
   args.wait_ns = expire ? 20000000ull : kWaitBudgetNs;
   args.withhold = expire ? 1 : 0;
