@@ -52,13 +52,13 @@ struct Cfg {
   static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
   static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
   static constexpr int kOffP = kStages * kStageBytes;             // two buffers
-  static constexpr int kOffBt = kOffP + 2 * kBlock;               // up to three terms of B~
-  static constexpr int kOffTab = kOffBt + 3 * kN1 * kBlock;
+  static constexpr int kOffBt = kOffP + 2 * kBlock;               // two buffers: second terms of B~ in turn, or a second and a third
+  static constexpr int kOffTab = kOffBt + 2 * kN1 * kBlock;
   // tables: powers [65], weights of the scores by distance [127], of the state's rows [64]; row scales of P [2][64], lane scales of
   // X [4][128], exchange of maxima [2][2][128], terms of B~'s weights in pairs [65][4]
   static constexpr int kTabPower = 0, kTabScore = 68, kTabRow = 196, kTabP = 260, kTabX = 388, kTabMax = 900, kTabW = 1412, kTabFloats = 1672;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
-  static constexpr int kBars = 2 * kStages + 16;
+  static constexpr int kBars = 2 * kStages + 20;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = kOffMisc + 16 + 1024;
   // tensor memory columns
@@ -146,12 +146,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   float* table = reinterpret_cast<float*>(gen + C::kOffTab);
   const uint32_t bars = base + C::kOffBar;
   const uint32_t b_full = bars, b_empty = bars + 8 * C::kStages;
-  const uint32_t b_s_full = bars + 16 * C::kStages, b_s_empty = b_s_full + 8;
-  const uint32_t b_p_full = b_s_full + 16;                    // [2]
-  const uint32_t b_o_full = b_s_full + 32, b_o_empty = b_s_full + 48;   // [2] each
-  const uint32_t b_bt_full = b_s_full + 64, b_t_full = b_s_full + 72, b_t_empty = b_s_full + 80;
-  const uint32_t b_x_full = b_s_full + 88;
-  const uint32_t b_max = b_s_full + 96;                      // [4]: of the two warps that share lanes
+  // (in pairs: for chunks in turn, where more than one role waits, or one that may be a chunk behind)
+  uint32_t next_bar = bars + 16 * C::kStages;
+  auto bar = [&](int n) { const uint32_t at = next_bar; next_bar += 8 * n; return at; };
+  const uint32_t b_s_full = bar(2), b_s_empty = bar(1), b_p_full = bar(2), b_o_full = bar(2), b_o_empty = bar(2), b_bt_full = bar(2);
+  const uint32_t b_t_full = bar(1), b_t_empty = bar(1), b_x_full = bar(1), b_x_empty = bar(1);
+  const uint32_t b_max = bar(4);   // of the two warps that share lanes
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(gen + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
 
@@ -182,19 +182,20 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       *abort_flag = 0;
       for (int i = 0; i < C::kStages; ++i) {
         mbar_init(b_full + 8 * i, 1);
-        mbar_init(b_empty + 8 * i, states_only ? 1 : 5);
+        mbar_init(b_empty + 8 * i, 1);
       }
-      mbar_init(b_s_full, 1);
       mbar_init(b_s_empty, 2);
       for (int i = 0; i < 2; ++i) {
+        mbar_init(b_s_full + 8 * i, 1);
         mbar_init(b_p_full + 8 * i, 2);
+        mbar_init(b_bt_full + 8 * i, 8);
         mbar_init(b_o_full + 8 * i, 1);
         mbar_init(b_o_empty + 8 * i, 4);
       }
-      mbar_init(b_bt_full, 8);
       mbar_init(b_t_full, 1);
       mbar_init(b_t_empty, 8);
       mbar_init(b_x_full, 8);
+      mbar_init(b_x_empty, 1);
       for (int i = 0; i < 4; ++i) mbar_init(b_max + 8 * i, 2);
       fence_mbar_init();
     }
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           const uint64_t ad = rows_desc + stage(c), bd = ad + (C::kOffB >> 4);
 #pragma unroll
           for (int k = 0; k < D1 / 16; ++k) mma_ss(tmem + C::kColS, ad + row_step(k), bd + row_step(k), idesc_s, k > 0);
-          tc_commit(b_s_full);
+          tc_commit(b_s_full + 8 * (c & 1));
         }
         __syncwarp();
         return true;
@@ -287,35 +288,41 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       for (int c = 0; c < chunks && ok; ++c) {
         const uint64_t ct = cols_desc + stage(c) + (C::kOffC >> 4);
         const uint32_t o = tmem + C::kColO + (c & 1) * 128;
-        if (states_only) {
-          if (!(ok = wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1)))) break;
-        } else {
-          // in front of T, which the state waits for: the state's columns are free as soon as T is there
-          if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
-          if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
-          tc_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int k = 0; k < D1 / 16; ++k) mma_ts(o, tmem + C::kColX + k * 8, rows_desc + stage(c) + row_step(k), idesc_x, k > 0);
-          }
-          __syncwarp();
+        // the next scores first if their tiles are there, as B~ of the next chunk waits for them; what is added to the state; and only then what waits
+        // for the state and for P
+        bool ahead = !states_only && c + 1 < chunks;
+        if (ahead && __all_sync(0xffffffffu, mbar_test(b_full + 8 * ((c + 1) % C::kStages), (uint32_t)(((c + 1) / C::kStages) & 1)))) {
+          if (!(ok = scores(c + 1))) break;
+          ahead = false;
         }
-        if (!(ok = wait(b_bt_full, (uint32_t)(c & 1)))) break;
+        if (!(ok = wait(b_bt_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
         if (!(ok = wait(b_t_empty, (uint32_t)(c & 1) ^ 1u))) break;
         tc_fence_after();
         if (leader) {
-          for (int term = args.terms - 1; term >= 0; --term)   // the smallest first (fp16 holds its second 2^11 times as large)
+          for (int term = args.terms - 1; term >= 0; --term) {   // the smallest first (fp16 holds its second 2^11 times as large)
+            const uint32_t slot = args.terms == 3 ? (uint32_t)(term - 1) : (uint32_t)(c & 1);
+            const uint64_t bt = term == 0 ? cols_desc + stage(c) + (C::kOffB >> 4) : cols_desc + ((C::kOffBt + slot * (C::kN1 * kBlock)) >> 4);
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k) {
-              const uint64_t cd = ct + k * (2048 >> 4), bd = cols_desc + (uint64_t)((C::kOffBt + term * C::kN1 * kBlock + k * 2048) >> 4);
+              const uint64_t cd = ct + k * (2048 >> 4), bd = bt + k * (2048 >> 4);
               if (!BF16 && term == 0 && k == 0) mma_ss_down11(tmem + C::kColT, cd, bd, idesc_t);
               else mma_ss(tmem + C::kColT, cd, bd, idesc_t, term < args.terms - 1 || k > 0);
             }
+          }
           tc_commit(b_t_full);
           if (states_only) tc_commit(b_empty + 8 * (c % C::kStages));
         }
         __syncwarp();
         if (states_only) continue;
+        if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
+        if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D1 / 16; ++k) mma_ts(o, tmem + C::kColX + k * 8, rows_desc + stage(c) + row_step(k), idesc_x, k > 0);
+          tc_commit(b_x_empty);
+        }
+        __syncwarp();
         if (!(ok = wait(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
         tc_fence_after();
         if (leader) {
@@ -326,59 +333,51 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           tc_commit(b_empty + 8 * (c % C::kStages));
         }
         __syncwarp();
-        if (c + 1 < chunks && !(ok = scores(c + 1))) break;
+        if (ahead && !(ok = scores(c + 1))) break;
       }
     } else if (warp < kWarpLoad) {
       // ---- P ----
       if (!states_only && chunks > 0) {
         const int i = warp * 32 + lane;
         const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16) + C::kColS;
-        const float* weight = table + C::kTabScore + 63 + i;   // of column j at -j; exactly zero behind the row
-        auto weighted = [&](uint32_t v, int j) {
-          const float w = weight[-j];
-          return w == 0.f ? 0.f : __uint_as_float(v) * w;   // (whatever stands there)
-        };
+        const float* weight = table + C::kTabScore + 63 + i;
         for (int c = 0; c < chunks; ++c) {
-          if (!wait(b_s_full, (uint32_t)(c & 1))) break;
-          if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
+          if (!wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
           tc_fence_after();
+          uint32_t r[kChunk];
+#pragma unroll
+          for (int j0 = 0; j0 < kChunk; j0 += 32) tmem_ld32(t_s + j0, r + j0);
+          tc_wait_ld();
+          tc_fence_before();
+          arrive(b_s_empty);   // (the next scores need not wait for what follows)
+          float most = 0.f;
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            const float w = weight[-j];   // of column j; exactly zero behind the row
+            const float x = w == 0.f ? 0.f : __uint_as_float(r[j]) * w;   // (whatever stands there)
+            if constexpr (!BF16) most = fmaxf(most, fabsf(x));
+            r[j] = __float_as_uint(x);
+          }
+          if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
           float to = 1.f;
           if constexpr (!BF16) {
-            float most = 0.f, back;
-#pragma unroll 1
-            for (int j0 = 0; j0 < kChunk; j0 += 16) {
-              uint32_t r[16];
-              tmem_ld16(t_s + j0, r);
-              tc_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(weighted(r[j], j0 + j)));
-            }
+            float back;
             scale_of(most, to, back);
             table[C::kTabP + (c & 1) * 64 + i] = back;
           }
           const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
-#pragma unroll 1   // (code that is small enough to stay in the instruction cache: unrolled over the row it took 7400 cycles a chunk)
-          for (int j0 = 0; j0 < kChunk; j0 += 16) {
-            uint32_t r[16], v[8];
-            tmem_ld16(t_s + j0, r);
-            tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              float x = weighted(r[j], j0 + j), y = weighted(r[j + 1], j0 + j + 1);
-              if constexpr (!BF16) x *= to, y *= to;
-              v[j / 2] = pack2<BF16>(x, y);
+          for (int u = 0; u < 8; ++u) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = __uint_as_float(r[8 * u + 2 * k]), y = __uint_as_float(r[8 * u + 2 * k + 1]);
+              v[k] = BF16 ? pack2<BF16>(x, y) : pack2<BF16>(x * to, y * to);
             }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              st_shared_v4(row + (((uint32_t)(j0 / 8 + u) ^ (uint32_t)(i & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+            st_shared_v4(row + (((uint32_t)u ^ (uint32_t)(i & 7)) << 4), v[0], v[1], v[2], v[3]);
           }
           fence_proxy_async_smem();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(b_s_empty);
-            mbar_arrive(b_p_full + 8 * (c & 1));
-          }
+          arrive(b_p_full + 8 * (c & 1));
         }
       }
     } else if (warp < kWarpOut) {
@@ -434,42 +433,55 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         arrive(b_x_full);
         return true;
       };
-      bool ok = states_only || put_state(0);
-      for (int c = 0; c < chunks && ok; ++c) {
+      // B~ of chunk c.  Its first term takes B's place, which the scores have read; the others lie apart: a second one in two buffers in turn, so
+      // that it is formed while the chunk before is multiplied, or (three terms) one buffer each.
+      const int r0 = tid >> 3;                   // this thread's rows are r0 and r0 + 32, of each block of 64 columns
+      const int j_lo = reverse ? kChunk - 1 - r0 : r0, j_hi = reverse ? j_lo - 32 : j_lo + 32;
+      const bool third = args.terms == 3;
+      auto weigh = [&](int c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
-        const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes);
-        if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) break;
+        const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + tid * 16;
+        const uint32_t rest = base + C::kOffBt + (third ? 0 : (c & 1) * (C::kN1 * kBlock)) + tid * 16;
+        if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
+        if (!states_only && !wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) return false;
         if constexpr (BF16) {
           // b w as terms of 16 bits by packed multiply-adds, with w = w0 + w1 + w2 of 8 bits each: b w0 has 16 bits, so that what its rounding leaves is
           // exact, and so on.  (In fp32, with conversions there and back, it took three times the instructions.)
-#pragma unroll 2
-          for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
-            const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
-            const uint4 v = lds128(st + C::kOffB + u * 16);
-            const uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabW + (j < n ? n - lag - j : 0) * 4);
-            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-            uint32_t a[4], e[4], f[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t b2 = j < n ? in[k] : 0u;   // (whatever stands in rows that are not there)
-              a[k] = bf16x2_mul(b2, w.x);
-              const uint32_t rest = bf16x2_fma(b2, w.x, a[k] ^ 0x80008000u);
-              e[k] = bf16x2_fma(b2, w.y, rest);
-              if (args.terms == 3) f[k] = bf16x2_fma(b2, w.z, bf16x2_fma(b2, w.y, bf16x2_sub(rest, e[k])));
+          for (int half_rows = 0; half_rows < 2; ++half_rows) {
+            const int j = half_rows ? j_hi : j_lo;
+            const uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabW + (j < n ? n - lag - j : 0) * 4);
+#pragma unroll
+            for (int block = 0; block < C::kN1; ++block) {
+              const uint32_t at = (uint32_t)(block * kBlock + half_rows * (kBlock / 2));
+              uint4 v = lds128(st + C::kOffB + at);
+              if (j >= n) v = make_uint4(0, 0, 0, 0);   // (whatever stands in rows that are not there)
+              const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+              uint32_t a[4], e[4], f[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                a[k] = bf16x2_mul(in[k], w.x);
+                f[k] = bf16x2_fma(in[k], w.x, a[k] ^ 0x80008000u);
+                e[k] = bf16x2_fma(in[k], w.y, f[k]);
+              }
+              st_shared_v4(st + C::kOffB + at, a[0], a[1], a[2], a[3]);
+              st_shared_v4(rest + at, e[0], e[1], e[2], e[3]);
+              if (third) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = bf16x2_fma(in[k], w.z, bf16x2_fma(in[k], w.y, bf16x2_sub(f[k], e[k])));
+                st_shared_v4(rest + C::kN1 * kBlock + at, f[0], f[1], f[2], f[3]);
+              }
             }
-            const uint32_t to = base + C::kOffBt + u * 16;
-            st_shared_v4(to, a[0], a[1], a[2], a[3]);
-            st_shared_v4(to + C::kN1 * kBlock, e[0], e[1], e[2], e[3]);
-            if (args.terms == 3) st_shared_v4(to + 2 * C::kN1 * kBlock, f[0], f[1], f[2], f[3]);
           }
         } else {
 #pragma unroll 2
-          for (int u = tid; u < C::kN1 * kBlock / 16; u += 256) {
-            const int r = (u % (kBlock / 16)) / 8, j = reverse ? kChunk - 1 - r : r;
+          for (int u = 0; u < 2 * C::kN1; ++u) {
+            const int j = u & 1 ? j_hi : j_lo;
+            const uint32_t at = (uint32_t)(u * (kBlock / 2));
             uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
             if (j < n) {
               const float w = power[n - lag - j];
-              const uint4 v = lds128(st + C::kOffB + u * 16);
+              const uint4 v = lds128(st + C::kOffB + at);
               const uint32_t in[4] = {v.x, v.y, v.z, v.w};
               uint32_t a[4], e[4];
 #pragma unroll
@@ -484,17 +496,23 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
               hi = make_uint4(a[0], a[1], a[2], a[3]);
               lo = make_uint4(e[0], e[1], e[2], e[3]);
             }
-            st_shared_v4(base + C::kOffBt + u * 16, hi.x, hi.y, hi.z, hi.w);
-            st_shared_v4(base + C::kOffBt + C::kN1 * kBlock + u * 16, lo.x, lo.y, lo.z, lo.w);
+            st_shared_v4(st + C::kOffB + at, hi.x, hi.y, hi.z, hi.w);
+            st_shared_v4(rest + at, lo.x, lo.y, lo.z, lo.w);
           }
         }
         if (n < kChunk)
-          for (int u = tid; u < C::kN2 * kBlock / 16; u += 256) {
-            const int r = (u % (kBlock / 16)) / 8;
-            if ((reverse ? kChunk - 1 - r : r) >= n) st_shared_v4(st + C::kOffC + u * 16, 0, 0, 0, 0);
-          }
+#pragma unroll
+          for (int u = 0; u < 2 * C::kN2; ++u)
+            if ((u & 1 ? j_hi : j_lo) >= n) st_shared_v4(st + C::kOffC + u * (kBlock / 2), 0, 0, 0, 0);
         fence_proxy_async_smem();
-        arrive(b_bt_full);
+        arrive(b_bt_full + 8 * (c & 1));
+        return true;
+      };
+      bool ok = (states_only || put_state(0)) && (chunks == 0 || weigh(0));
+      for (int c = 0; c < chunks && ok; ++c) {
+        const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
+        // (in front of T, which is then being formed; with three terms behind it)
+        if (!third && c + 1 < chunks && !weigh(c + 1)) break;
         if (!wait(b_t_full, (uint32_t)(c & 1))) break;
         tc_fence_after();
         if (owner) {
@@ -511,8 +529,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         tc_fence_before();
         arrive(b_t_empty);
         if (!states_only && c + 1 < chunks) {
+          if (!wait(b_x_empty, (uint32_t)(c & 1))) break;
+          tc_fence_after();
           ok = put_state(c + 1);
         }
+        if (third && ok && c + 1 < chunks) ok = weigh(c + 1);
       }
       if (owner && !*abort_flag) {
         float* to = states_only ? work : args.segments == 1 && s.x_last && q.state >= 0 ? s.x_last + (q.state * p.heads + h) * matrix : nullptr;
@@ -592,9 +613,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             store(r0, e, std::integral_constant<int, 16>());
           }
           const bool again = probe != probe;
-          // (the tile is there since before the products; this thread has to see that for itself)
-          if (__any_sync(0xffffffffu, again) && wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) {
-            const uint32_t ct = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + C::kOffC + (d2 / 64) * kBlock, pt = base + C::kOffP + (c & 1) * kBlock;
+          if (__any_sync(0xffffffffu, again)) {   // (the tile of C may have been given back: its column comes from memory once more)
+            const uint32_t pt = base + C::kOffP + (c & 1) * kBlock;
+            const uint16_t* ct = static_cast<const uint16_t*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + (q.row0 + token) * s.cs[2] + d2;
 #pragma unroll 1
             for (int r = 0; r < kChunk; r += 2) {
               uint32_t u[2], v[2];
@@ -610,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
                   part = 0.f;
                   for (int j = reverse ? at : low; j < (reverse ? high : at + 1); ++j)
                     part = fmaf(lds16<BF16>(pt + at * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(at & 7)) << 4) + (j & 7) * 2),
-                                lds16<BF16>(ct + j * 128 + (((uint32_t)((d2 & 63) >> 3) ^ (uint32_t)(j & 7)) << 4) + (d2 & 7) * 2), part);
+                                unpack2<BF16>(ct[j * s.cs[2]]).x, part);
                 }
                 e[k] = value(__uint_as_float(u[k]), part, row_w[at], BF16 ? 1.f : row_p[at]);
               }
@@ -620,10 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(b_o_empty + 8 * (c & 1));
-          mbar_arrive(b_empty + 8 * (c % C::kStages));
-        }
+        if (lane == 0) mbar_arrive(b_o_empty + 8 * (c & 1));
       }
     }
 
