@@ -26,8 +26,6 @@
 // Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
 #include <cuda.h>
 
-#include <type_traits>
-
 #include "linear.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_map.hpp"
@@ -49,21 +47,20 @@ template <int D1, int D2>
 struct Cfg {
   static constexpr int kN1 = D1 / 64, kN2 = D2 / 64;
   static constexpr int kStageBytes = (2 * kN1 + kN2) * kBlock;
-  static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
+  static constexpr int kStages = 196608 / kStageBytes < 8 ? 196608 / kStageBytes : 8;   // up to 192 KB of tiles
   static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
   static constexpr int kOffP = kStages * kStageBytes;             // two buffers
-  static constexpr int kOffBt = kOffP + 2 * kBlock;               // two buffers: second terms of B~ in turn, or a second and a third
-  static constexpr int kOffTab = kOffBt + 2 * kN1 * kBlock;
+  static constexpr int kOffTab = kOffP + 2 * kBlock;
   // tables: powers [65], weights of the scores by distance [127], of the state's rows [64]; row scales of P [2][64], lane scales of
-  // X [4][128], exchange of maxima [2][2][128], terms of B~'s weights in pairs [65][4]
-  static constexpr int kTabPower = 0, kTabScore = 68, kTabRow = 196, kTabP = 260, kTabX = 388, kTabMax = 900, kTabW = 1412, kTabFloats = 1672;
+  // X [4][128], exchange of maxima [2][2][128], weights of C~ by exponent, [3] 16-bit terms of [66]
+  static constexpr int kTabPower = 0, kTabScore = 68, kTabRow = 196, kTabP = 260, kTabX = 388, kTabMax = 900, kTabW = 1412, kTabFloats = 1512;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
   static constexpr int kBars = 2 * kStages + 20;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = kOffMisc + 16 + 1024;
-  // tensor memory columns
-  static constexpr int kColX = 0, kColT = D1 / 2, kColS = kColT + D1, kColO = kColS + 64;   // O: [2][state part, row part]
-  static_assert(kColO + 256 <= 512, "tensor memory");
+  // tensor memory columns: X^T in 16 bits, T^T, S, O^T (state part, row part), C~^T in 16 bits (two terms in two buffers, or three)
+  static constexpr int kColX = 0, kColT = D1 / 2, kColS = kColT + D1, kColO = kColS + 64, kColC = kColO + 128;
+  static_assert(kColC + 128 <= 512, "tensor memory");
 };
 
 struct Maps {
@@ -76,7 +73,7 @@ struct Args {
   int32_t first, count;          // scans of this launch
   int32_t segments, seg_len;     // seg_len: a multiple of kChunk
   int32_t states_only;
-  int32_t terms;                 // of B~: 2, or 3 for bf16 where states go out
+  int32_t terms;                 // of C~: 2, or 3 for bf16 where states go out
   float* work;                   // [scan][sequence, head][segment][D1][D2]
   uint64_t wait_ns;
   int32_t withhold;              // test hook: no loads, so that the waits run out
@@ -127,14 +124,27 @@ __device__ __forceinline__ void scale_of(float largest, float& to, float& back) 
   back = __int_as_float((e - 14) << 23);
 }
 
-// D[tmem] = A[smem] * B[smem] + D * 2^-11
-__device__ __forceinline__ void mma_ss_down11(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+// D[tmem] = A[tmem] * B[smem] + D * 2^-11
+__device__ __forceinline__ void mma_ts_down11(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.eq.b32 p, 0, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 11;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc)
       : "memory");
+}
+// Four 8 x 8 tiles of 16-bit elements, transposed: thread t holds row t / 4 and columns 2 (t % 4), + 1 of each.
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 lanes x 16 columns: r[2 i] holds lane t / 4 and column 4 i + t % 4, r[2 i + 1] the lane 8 above.
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 template <int D1, int D2, bool BF16>
@@ -204,12 +214,13 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const float w = exp2f(g * threadIdx.x);
       table[C::kTabPower + threadIdx.x] = w;
       if constexpr (BF16) {
+        uint16_t* terms = reinterpret_cast<uint16_t*>(table + C::kTabW);
         float left = w * s.key_scale;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          const uint32_t t = pack2<true>(left, left);
-          table[C::kTabW + threadIdx.x * 4 + i] = __uint_as_float(t);
-          left -= __uint_as_float(t & 0xffff0000u);
+          const uint32_t t = pack2<true>(left, 0.f) & 0xffffu;
+          terms[i * 66 + threadIdx.x] = (uint16_t)t;
+          left -= __uint_as_float(t << 16);
         }
       }
     }
@@ -266,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       constexpr uint32_t idesc_s = make_idesc(128, 64, BF16, false);                  // A and B along their rows
       constexpr uint32_t idesc_x = make_idesc(128, 64, BF16, false);                  // X^T from tensor memory, A along its rows
       constexpr uint32_t idesc_p = make_idesc(128, 64, BF16, false) | kTransposeA;    // C^T, P along its rows
-      constexpr uint32_t idesc_t = make_idesc(128, D1, BF16, true) | kTransposeA;     // C^T, B~ across its rows
+      constexpr uint32_t idesc_t = make_idesc(128, D1, BF16, true);                   // C~^T from tensor memory, B across its rows
       // (a descriptor's start address is counted in 16 bytes; what is added to it stays within its field)
       const uint64_t rows_desc = make_smem_desc(base, 16, 1024), cols_desc = make_smem_desc(base, kBlock, 1024);
       auto stage = [&](int c) { return (uint64_t)((c % C::kStages) * (C::kStageBytes >> 4)); };
@@ -287,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       bool ok = states_only || chunks == 0 || scores(0);
       for (int c = 0; c < chunks && ok; ++c) {
         const uint64_t ct = cols_desc + stage(c) + (C::kOffC >> 4);
-        const uint32_t o = tmem + C::kColO + (c & 1) * 128;
+        const uint32_t o = tmem + C::kColO;
         // the next scores first if their tiles are there, as B~ of the next chunk waits for them; what is added to the state; and only then what waits
         // for the state and for P
         bool ahead = !states_only && c + 1 < chunks;
@@ -299,14 +310,13 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         if (!(ok = wait(b_t_empty, (uint32_t)(c & 1) ^ 1u))) break;
         tc_fence_after();
         if (leader) {
+          const uint64_t bt = cols_desc + stage(c) + (C::kOffB >> 4);
           for (int term = args.terms - 1; term >= 0; --term) {   // the smallest first (fp16 holds its second 2^11 times as large)
-            const uint32_t slot = args.terms == 3 ? (uint32_t)(term - 1) : (uint32_t)(c & 1);
-            const uint64_t bt = term == 0 ? cols_desc + stage(c) + (C::kOffB >> 4) : cols_desc + ((C::kOffBt + slot * (C::kN1 * kBlock)) >> 4);
+            const uint32_t at = tmem + C::kColC + (args.terms == 3 ? 0 : (c & 1) * 64) + term * 32;
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k) {
-              const uint64_t cd = ct + k * (2048 >> 4), bd = bt + k * (2048 >> 4);
-              if (!BF16 && term == 0 && k == 0) mma_ss_down11(tmem + C::kColT, cd, bd, idesc_t);
-              else mma_ss(tmem + C::kColT, cd, bd, idesc_t, term < args.terms - 1 || k > 0);
+              if (!BF16 && term == 0 && k == 0) mma_ts_down11(tmem + C::kColT, at, bt, idesc_t);
+              else mma_ts(tmem + C::kColT, at + k * 8, bt + k * (2048 >> 4), idesc_t, term < args.terms - 1 || k > 0);
             }
           }
           tc_commit(b_t_full);
@@ -315,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         __syncwarp();
         if (states_only) continue;
         if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
-        if (!(ok = wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u))) break;
+        if (c > 0 && !(ok = wait(b_o_empty + 8 * ((c - 1) & 1), (uint32_t)(((c - 1) >> 1) & 1)))) break;
         tc_fence_after();
         if (leader) {
 #pragma unroll
@@ -433,78 +443,82 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         arrive(b_x_full);
         return true;
       };
-      // B~ of chunk c.  Its first term takes B's place, which the scores have read; the others lie apart: a second one in two buffers in turn, so
-      // that it is formed while the chunk before is multiplied, or (three terms) one buffer each.
-      const int r0 = tid >> 3;                   // this thread's rows are r0 and r0 + 32, of each block of 64 columns
-      const int j_lo = reverse ? kChunk - 1 - r0 : r0, j_hi = reverse ? j_lo - 32 : j_lo + 32;
+      // C~^T of chunk c to tensor memory: these lanes, rows 32 half .. + 31 of the chunk.  Two terms in two buffers in turn, so that they are formed while
+      // the chunk before is multiplied, or three in one.
       const bool third = args.terms == 3;
+      uint32_t weights[3][4];   // of this thread's pairs of rows in a whole chunk, for BF16
+      auto exponent = [&](int j, int n) { return reverse ? n - lag - (kChunk - 1 - j) : n - lag - j; };   // of tile row j, where it is one of n
+      auto there = [&](int j, int n) { return reverse ? kChunk - 1 - j < n : j < n; };
+      const int j_own = half * 32 + (lane & 3) * 2;   // + 8 i
+      auto load_weights = [&](int n) {
+        const uint16_t* terms = reinterpret_cast<const uint16_t*>(table + C::kTabW);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j_own + 8 * i, e0 = there(j, n) ? exponent(j, n) : 0, e1 = there(j + 1, n) ? exponent(j + 1, n) : 0;
+#pragma unroll
+          for (int t = 0; t < 3; ++t) weights[t][i] = (uint32_t)terms[t * 66 + e0] | (uint32_t)terms[t * 66 + e1] << 16;
+        }
+      };
+      if constexpr (BF16) load_weights(kChunk);
       auto weigh = [&](int c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
-        const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + tid * 16;
-        const uint32_t rest = base + C::kOffBt + (third ? 0 : (c & 1) * (C::kN1 * kBlock)) + tid * 16;
+        const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + C::kOffC;
         if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
-        if (!states_only && !wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) return false;
-        if constexpr (BF16) {
-          // b w as terms of 16 bits by packed multiply-adds, with w = w0 + w1 + w2 of 8 bits each: b w0 has 16 bits, so that what its rounding leaves is
-          // exact, and so on.  (In fp32, with conversions there and back, it took three times the instructions.)
+        if (owner) {
+          if (BF16 && n < kChunk) load_weights(n);
+          const uint32_t to = tmem + lanes + C::kColC + (third ? 0 : (c & 1) * 64) + half * 16;
+          // (matrices of a load: rows j .. j + 7 with columns d, d + 8; rows j + 8 .. j + 15 with the same)
+          const int row = half * 32 + (lane & 7) + ((lane >> 4) << 3), col = quarter * 32 + (lane & 8);
+          const uint32_t from = st + (col / 64) * kBlock + row * 128;
 #pragma unroll
-          for (int half_rows = 0; half_rows < 2; ++half_rows) {
-            const int j = half_rows ? j_hi : j_lo;
-            const uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabW + (j < n ? n - lag - j : 0) * 4);
+          for (int d = 0; d < 32; d += 16) {
+            uint32_t v[8], a[8], e[8];
 #pragma unroll
-            for (int block = 0; block < C::kN1; ++block) {
-              const uint32_t at = (uint32_t)(block * kBlock + half_rows * (kBlock / 2));
-              uint4 v = lds128(st + C::kOffB + at);
-              if (j >= n) v = make_uint4(0, 0, 0, 0);   // (whatever stands in rows that are not there)
-              const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-              uint32_t a[4], e[4], f[4];
+            for (int i = 0; i < 2; ++i) ldmatrix_x4_trans(from + i * (16 * 128) + (((uint32_t)(((col & 63) + d) >> 3) ^ (uint32_t)(row & 7)) << 4), v + 4 * i);
+            if (n < kChunk) {   // (whatever stands in rows that are not there)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                a[k] = bf16x2_mul(in[k], w.x);
-                f[k] = bf16x2_fma(in[k], w.x, a[k] ^ 0x80008000u);
-                e[k] = bf16x2_fma(in[k], w.y, f[k]);
-              }
-              st_shared_v4(st + C::kOffB + at, a[0], a[1], a[2], a[3]);
-              st_shared_v4(rest + at, e[0], e[1], e[2], e[3]);
-              if (third) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = bf16x2_fma(in[k], w.z, bf16x2_fma(in[k], w.y, bf16x2_sub(f[k], e[k])));
-                st_shared_v4(rest + C::kN1 * kBlock + at, f[0], f[1], f[2], f[3]);
+              for (int i = 0; i < 8; ++i) {
+                const int j = j_own + 8 * (i / 2);
+                v[i] &= (there(j, n) ? 0xffffu : 0u) | (there(j + 1, n) ? 0xffff0000u : 0u);
               }
             }
-          }
-        } else {
-#pragma unroll 2
-          for (int u = 0; u < 2 * C::kN1; ++u) {
-            const int j = u & 1 ? j_hi : j_lo;
-            const uint32_t at = (uint32_t)(u * (kBlock / 2));
-            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-            if (j < n) {
-              const float w = power[n - lag - j];
-              const uint4 v = lds128(st + C::kOffB + at);
-              const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-              uint32_t a[4], e[4];
+            if constexpr (BF16) {
+              // c w as terms of 16 bits by packed multiply-adds, with w = w0 + w1 + w2 of 8 bits each: c w0 has 16 bits, so that what its rounding
+              // leaves is exact, and so on.
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float2 f = unpack2<BF16>(in[k]);
-                f.x *= w;
-                f.y *= w;
-                a[k] = pack2<BF16>(f.x, f.y);
-                const float2 t = unpack2<BF16>(a[k]);
-                e[k] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+              for (int i = 0; i < 8; ++i) {
+                a[i] = bf16x2_mul(v[i], weights[0][i / 2]);
+                const uint32_t rest = bf16x2_fma(v[i], weights[0][i / 2], a[i] ^ 0x80008000u);
+                e[i] = bf16x2_fma(v[i], weights[1][i / 2], rest);
+                if (third) v[i] = bf16x2_fma(v[i], weights[2][i / 2], bf16x2_fma(v[i], weights[1][i / 2], bf16x2_sub(rest, e[i])));
               }
-              hi = make_uint4(a[0], a[1], a[2], a[3]);
-              lo = make_uint4(e[0], e[1], e[2], e[3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int j = j_own + 8 * (i / 2);
+                float2 f = unpack2<BF16>(v[i]);
+                f.x *= power[there(j, n) ? exponent(j, n) : 0];
+                f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0];
+                a[i] = pack2<BF16>(f.x, f.y);
+                const float2 t = unpack2<BF16>(a[i]);
+                e[i] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+              }
             }
-            st_shared_v4(st + C::kOffB + at, hi.x, hi.y, hi.z, hi.w);
-            st_shared_v4(rest + at, lo.x, lo.y, lo.z, lo.w);
+            tmem_st_16x128b_x4(to + ((uint32_t)d << 16), a);
+            tmem_st_16x128b_x4(to + ((uint32_t)d << 16) + 32, e);
+            if (third) tmem_st_16x128b_x4(to + ((uint32_t)d << 16) + 64, v);
           }
+          tc_wait_st();
         }
-        if (n < kChunk)
+        if (n < kChunk) {   // what multiplies a zero has to be finite: B's rows in the product with C~, C's in the one with P
+          const int r0 = tid >> 3;   // this thread's rows are r0 and r0 + 32, of each block of 64 columns
+          __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 2 * C::kN2; ++u)
-            if ((u & 1 ? j_hi : j_lo) >= n) st_shared_v4(st + C::kOffC + u * (kBlock / 2), 0, 0, 0, 0);
-        fence_proxy_async_smem();
+          for (int u = 0; u < 2 * (C::kN1 + C::kN2); ++u)   // (C lies behind B)
+            if (!there(r0 + 32 * (u & 1), n)) st_shared_v4(st + C::kOffB - C::kOffC + u * (kBlock / 2) + tid * 16, 0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
         arrive(b_bt_full + 8 * (c & 1));
         return true;
       };
@@ -562,86 +576,82 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         if (!wait(b_o_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
         tc_fence_after();
         if (owner) {
-          const uint32_t t_o = tmem + lanes + C::kColO + (c & 1) * 128;
+          const uint32_t t_o = tmem + lanes + C::kColO;
           const float xs = BF16 ? 1.f : table[C::kTabX + (c & 3) * 128 + d2];
           const float* row_w = table + C::kTabRow;
           const float* row_p = table + C::kTabP + (c & 1) * 64;
           float probe = 0.f;   // NaN as soon as a value of the row part is not finite
           auto value = [&](float state, float part, float w, float ps) { return BF16 ? fmaf(w, state, part) : fmaf(ps, part, w * xs * state); };
-          // rows r .. r + N - 1: 16-bit values in pairs of columns, even lanes of the even rows and odd lanes of the odd ones.  (All exchanges, then
-          // all stores, none behind a branch: one row pair after the other took 100 cycles each.)
-          auto store = [&](int r, const float* e, auto count) {
-            constexpr int N = decltype(count)::value;
-            if (y_f32) {
+          // all of the lane's values first, so that the columns are free for the next chunk while these are stored
+          float e[kChunk];
 #pragma unroll
-              for (int i = 0; i < N; ++i)
-                if (r + i >= low && r + i < high) y32[(int64_t)(token + r + i) * pitch + d2] = e[i];
-            } else {
-              uint32_t v[N / 2];
-#pragma unroll
-              for (int i = 0; i < N; i += 2) {
-                const float got = __shfl_xor_sync(0xffffffffu, odd ? e[i] : e[i + 1], 1);
-                v[i / 2] = pack2<BF16>(odd ? got : e[i], odd ? e[i + 1] : got);
-              }
-              uint16_t* at = y16 + (int64_t)(token + r + odd) * pitch + (d2 & ~1);
-#pragma unroll
-              for (int i = 0; i < N; i += 2) {
-                if (r + i + odd >= low && r + i + odd < high) *reinterpret_cast<uint32_t*>(at) = v[i / 2];
-                at += 2 * pitch;
-              }
-            }
-          };
-#pragma unroll 1
           for (int r0 = 0; r0 < kChunk; r0 += 16) {
             uint32_t u[16], v[16];
             tmem_ld16(t_o + r0, u);
             tmem_ld16(t_o + 64 + r0, v);
-            float w[16], ps[16];
+            tc_wait_ld();
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-              *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(row_w + r0 + r);
-              if constexpr (!BF16) *reinterpret_cast<float4*>(ps + r) = *reinterpret_cast<const float4*>(row_p + r0 + r);
-            }
-            tc_wait_ld();
-            float e[16];
+              const float4 w = *reinterpret_cast<const float4*>(row_w + r0 + r);
+              float4 ps = make_float4(1.f, 1.f, 1.f, 1.f);
+              if constexpr (!BF16) ps = *reinterpret_cast<const float4*>(row_p + r0 + r);
+              const float ww[4] = {w.x, w.y, w.z, w.w}, pp[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float part = __uint_as_float(v[r]);
-              probe = fmaf(part, 0.f, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
-              e[r] = value(__uint_as_float(u[r]), part, w[r], BF16 ? 1.f : ps[r]);
+              for (int k = 0; k < 4; ++k) {
+                const float part = __uint_as_float(v[r + k]);
+                probe = fmaf(part, 0.f, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
+                e[r0 + r + k] = value(__uint_as_float(u[r + k]), part, ww[k], pp[k]);
+              }
             }
-            store(r0, e, std::integral_constant<int, 16>());
           }
           const bool again = probe != probe;
           if (__any_sync(0xffffffffu, again)) {   // (the tile of C may have been given back: its column comes from memory once more)
             const uint32_t pt = base + C::kOffP + (c & 1) * kBlock;
             const uint16_t* ct = static_cast<const uint16_t*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + (q.row0 + token) * s.cs[2] + d2;
-#pragma unroll 1
-            for (int r = 0; r < kChunk; r += 2) {
-              uint32_t u[2], v[2];
-              asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(u[0]), "=r"(u[1]) : "r"(t_o + r) : "memory");
-              asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(t_o + 64 + r) : "memory");
-              tc_wait_ld();
-              float e[2];
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int at = r + k;
-                float part = __uint_as_float(v[k]);
-                if (again) {
-                  part = 0.f;
-                  for (int j = reverse ? at : low; j < (reverse ? high : at + 1); ++j)
-                    part = fmaf(lds16<BF16>(pt + at * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(at & 7)) << 4) + (j & 7) * 2),
-                                unpack2<BF16>(ct[j * s.cs[2]]).x, part);
-                }
-                e[k] = value(__uint_as_float(u[k]), part, row_w[at], BF16 ? 1.f : row_p[at]);
+            for (int r = 0; r < kChunk; ++r) {
+              uint32_t u;
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(u) : "r"(t_o + r) : "memory");
+              tc_wait_ld();
+              if (again && r >= low && r < high) {
+                float part = 0.f;
+#pragma unroll 1
+                for (int j = reverse ? r : low; j < (reverse ? high : r + 1); ++j)
+                  part = fmaf(lds16<BF16>(pt + r * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(r & 7)) << 4) + (j & 7) * 2), unpack2<BF16>(ct[j * s.cs[2]]).x, part);
+                e[r] = value(__uint_as_float(u), part, row_w[r], BF16 ? 1.f : row_p[r]);
               }
-              store(r, e, std::integral_constant<int, 2>());
             }
           }
+          tc_fence_before();
+          arrive(b_o_empty + 8 * (c & 1));
+          if (y_f32) {
+            float* at = y32 + (int64_t)token * pitch + d2;
+#pragma unroll
+            for (int r = 0; r < kChunk; ++r) {
+              if (r >= low && r < high) *at = e[r];
+              at += pitch;
+            }
+          } else {
+            // 16-bit values in pairs of columns: even lanes of the even rows, odd lanes of the odd ones
+            uint16_t* at = y16 + (int64_t)(token + odd) * pitch + (d2 & ~1);
+#pragma unroll
+            for (int r0 = 0; r0 < kChunk; r0 += 16) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, odd ? e[r0 + i] : e[r0 + i + 1], 1);
+                v[i / 2] = pack2<BF16>(odd ? got : e[r0 + i], odd ? e[r0 + i + 1] : got);
+              }
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                if (r0 + i + odd >= low && r0 + i + odd < high) *reinterpret_cast<uint32_t*>(at) = v[i / 2];
+                at += 2 * pitch;
+              }
+            }
+          }
+        } else {
+          arrive(b_o_empty + 8 * (c & 1));
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(b_o_empty + 8 * (c & 1));
       }
     }
 
