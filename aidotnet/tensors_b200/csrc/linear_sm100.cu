@@ -26,6 +26,7 @@
 // Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
 #include <cuda.h>
 
+#include "ffma2.cuh"
 #include "linear.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_map.hpp"
@@ -40,6 +41,7 @@ __device__ int32_t g_linear_status;   // set when a bounded wait gave up (the en
 
 constexpr int kChunk = 64;
 constexpr int kBlock = kChunk * 128;   // 64 rows of 64 16-bit elements
+constexpr int kYBytes = kChunk * 64;   // 64 rows of 32
 constexpr int kThreads = 512;
 constexpr int kWarpLoad = 2, kWarpMma = 3, kWarpState = 4, kWarpOut = 12;   // (warps 0 and 1: P)
 
@@ -47,13 +49,16 @@ template <int D1, int D2>
 struct Cfg {
   static constexpr int kN1 = D1 / 64, kN2 = D2 / 64;
   static constexpr int kStageBytes = (2 * kN1 + kN2) * kBlock;
-  static constexpr int kStages = 196608 / kStageBytes < 8 ? 196608 / kStageBytes : 8;   // up to 192 KB of tiles
+  static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
   static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
   static constexpr int kOffP = kStages * kStageBytes;             // two buffers
-  static constexpr int kOffTab = kOffP + 2 * kBlock;
-  // tables: powers [65], weights of the scores by distance [127], of the state's rows [64]; row scales of P [2][64], lane scales of
-  // X [4][128], exchange of maxima [2][2][128], weights of C~ by exponent, [3] 16-bit terms of [66]
-  static constexpr int kTabPower = 0, kTabScore = 68, kTabRow = 196, kTabP = 260, kTabX = 388, kTabMax = 900, kTabW = 1412, kTabFloats = 1512;
+  static constexpr int kOffY = kOffP + 2 * kBlock;                // output, 64 rows of 32 columns to a warp
+  static constexpr int kOffTab = kOffY + 4 * kYBytes;
+  // tables (floats): powers [65], weights of the scores by distance in four copies, each one element on from the one before (a row's begin anywhere
+  // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of maxima [2][2][128], weights of
+  // C~ by exponent, [3] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [3][2][4][4]
+  static constexpr int kTabPower = 0, kTabScore = 68, kScorePitch = 136, kTabRow = kTabScore + 4 * kScorePitch, kTabP = kTabRow + 64, kTabX = kTabP + 128,
+                       kTabMax = kTabX + 512, kTabW = kTabMax + 512, kTabPairs = kTabW + 100, kTabFloats = kTabPairs + 96;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
   static constexpr int kBars = 2 * kStages + 20;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
@@ -65,6 +70,7 @@ struct Cfg {
 
 struct Maps {
   CUtensorMap t[4];
+  CUtensorMap y[3];
 };
 
 struct Args {
@@ -100,7 +106,7 @@ __device__ __forceinline__ uint32_t bf16x2_sub(uint32_t a, uint32_t b) {
   return d;
 }
 template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
+__device__ __forceinline__ float2 unpack16(uint32_t v) {
   if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
@@ -110,6 +116,25 @@ __device__ __forceinline__ float lds16(uint32_t a) {
   asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
   if constexpr (BF16) return __uint_as_float((uint32_t)v << 16);
   else return __half2float(*reinterpret_cast<__half*>(&v));
+}
+// The rest of a wait that did not end at once, apart from the code of every place that waits: all of it has to stay in the instruction cache.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t wait_ns) {
+  return mbar_wait(bar, parity, abort_flag, wait_ns);
+}
+// One term of the weights of rows j + 8 i, + 1 in a last chunk of n rows, zeros where there are none.
+__device__ __noinline__ uint4 end_weights(const uint16_t* term, int j, int n, int lag, bool reverse) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int at = reverse ? kChunk - 1 - (j + 8 * i + k) : j + 8 * i + k;
+      if (at < n) v |= (uint32_t)term[n - lag - at] << (16 * k);
+    }
+    w[i] = v;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // Powers of two that bring a largest value into [2^14, 2^15) and back.  (What is not finite, or so small that the power has no
 // reciprocal, is left near where it is.)
@@ -139,6 +164,20 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t* r) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+// The other way: four 8 x 8 tiles to shared memory, transposed.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, const uint32_t* r) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) { asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory"); }
+// 16 lanes x 32 columns: r[4 i], r[4 i + 1] hold lane t / 4 and columns 8 i + 2 (t % 4), + 1; r[4 i + 2], r[4 i + 3] the lane 8 above.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 // 16 lanes x 16 columns: r[2 i] holds lane t / 4 and column 4 i + t % 4, r[2 i + 1] the lane 8 above.
 __device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t* r) {
@@ -220,6 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         for (int i = 0; i < 3; ++i) {
           const uint32_t t = pack2<true>(left, 0.f) & 0xffffu;
           terms[i * 66 + threadIdx.x] = (uint16_t)t;
+          const int j = reverse ? (int)threadIdx.x + s.lag - 1 : kChunk - s.lag - (int)threadIdx.x;   // the row of a whole chunk with this exponent
+          if (j >= 0 && j < kChunk)
+            reinterpret_cast<uint16_t*>(table + C::kTabPairs + i * 32)[((j / 32) * 16 + ((j % 8) / 2) * 4 + (j % 32) / 8) * 2 + (j & 1)] = (uint16_t)t;
           left -= __uint_as_float(t << 16);
         }
       }
@@ -227,9 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
     else if (threadIdx.x >= 96 && threadIdx.x < 160) {
       const int r = threadIdx.x - 96;
       table[C::kTabRow + r] = s.row_scale * exp2f(g * ((reverse ? kChunk - 1 - r : r) + s.lag));
-    } else if (threadIdx.x >= 256 && threadIdx.x < 383) {   // at 63 + (i - j); zeros where j follows i
-      const int d = reverse ? 63 - (int)(threadIdx.x - 256) : (int)(threadIdx.x - 256) - 63;
-      table[C::kTabScore + threadIdx.x - 256] = d >= 0 ? p.scale * exp2f(g * d) : 0.f;
+    } else if (threadIdx.x >= 256 && threadIdx.x < 384) {   // of row i and column j at 63 - i + j; zeros where j follows i
+      const int x = (int)threadIdx.x - 256, d = reverse ? x - 63 : 63 - x;
+      const float w = d >= 0 ? p.scale * exp2f(g * d) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (x >= i) table[C::kTabScore + i * C::kScorePitch + x - i] = w;
     }
     if (warp == kWarpMma) {
       tmem_alloc(smem_u32(tmem_ptr), 512);
@@ -240,7 +285,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
     const float* power = table + C::kTabPower;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, wait_ns)); };
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      bool done = mbar_try_wait(bar, parity);
+      if (!done) done = wait_on(bar, parity, abort_flag, wait_ns);
+      return __all_sync(0xffffffffu, done) != 0;
+    };
     auto arrive = [&](uint32_t bar) {
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
@@ -350,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       if (!states_only && chunks > 0) {
         const int i = warp * 32 + lane;
         const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16) + C::kColS;
-        const float* weight = table + C::kTabScore + 63 + i;
+        const int skip = 63 - i;
+        const float* weight = table + C::kTabScore + (skip & 3) * C::kScorePitch + (skip & ~3);   // of column j at j
         for (int c = 0; c < chunks; ++c) {
           if (!wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
           tc_fence_after();
@@ -360,19 +410,33 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           tc_wait_ld();
           tc_fence_before();
           arrive(b_s_empty);   // (the next scores need not wait for what follows)
-          float most = 0.f;
+          uint64_t x[kChunk / 2], probe = 0;
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            const float w = weight[-j];   // of column j; exactly zero behind the row
-            const float x = w == 0.f ? 0.f : __uint_as_float(r[j]) * w;   // (whatever stands there)
-            if constexpr (!BF16) most = fmaxf(most, fabsf(x));
-            r[j] = __float_as_uint(x);
+          for (int j = 0; j < kChunk; j += 4) {
+            const Pair2 w = lds_pairs(weight + j);
+            x[j / 2] = mul2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), w.a);
+            x[j / 2 + 1] = mul2(pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), w.b);
+            probe = fma2(x[j / 2], 0ull, fma2(x[j / 2 + 1], 0ull, probe));
+          }
+          const float2 odd_ones = unpack2(probe);
+          if (__any_sync(0xffffffffu, odd_ones.x + odd_ones.y != 0.f)) {   // NaN: a score is not finite.  Behind the row it counts for nothing.
+#pragma unroll
+            for (int j = 0; j < kChunk; j += 2) {
+              const float2 f = unpack2(x[j / 2]);
+              x[j / 2] = pack2(reverse ? (j < i ? 0.f : f.x) : (j > i ? 0.f : f.x), reverse ? (j + 1 < i ? 0.f : f.y) : (j + 1 > i ? 0.f : f.y));
+            }
           }
           if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
-          float to = 1.f;
+          uint64_t to = 0;
           if constexpr (!BF16) {
-            float back;
-            scale_of(most, to, back);
+            float most = 0.f, up, back;
+#pragma unroll
+            for (int j = 0; j < kChunk / 2; ++j) {
+              const float2 f = unpack2(x[j]);
+              most = fmax3(most, fabsf(f.x), fabsf(f.y));
+            }
+            scale_of(most, up, back);
+            to = pack2(up, up);
             table[C::kTabP + (c & 1) * 64 + i] = back;
           }
           const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
@@ -381,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             uint32_t v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const float x = __uint_as_float(r[8 * u + 2 * k]), y = __uint_as_float(r[8 * u + 2 * k + 1]);
-              v[k] = BF16 ? pack2<BF16>(x, y) : pack2<BF16>(x * to, y * to);
+              const float2 f = unpack2(BF16 ? x[4 * u + k] : mul2(x[4 * u + k], to));
+              v[k] = pack2<BF16>(f.x, f.y);
             }
             st_shared_v4(row + (((uint32_t)u ^ (uint32_t)(i & 7)) << 4), v[0], v[1], v[2], v[3]);
           }
@@ -446,26 +510,25 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       // C~^T of chunk c to tensor memory: these lanes, rows 32 half .. + 31 of the chunk.  Two terms in two buffers in turn, so that they are formed while
       // the chunk before is multiplied, or three in one.
       const bool third = args.terms == 3;
-      uint32_t weights[3][4];   // of this thread's pairs of rows in a whole chunk, for BF16
       auto exponent = [&](int j, int n) { return reverse ? n - lag - (kChunk - 1 - j) : n - lag - j; };   // of tile row j, where it is one of n
       auto there = [&](int j, int n) { return reverse ? kChunk - 1 - j < n : j < n; };
       const int j_own = half * 32 + (lane & 3) * 2;   // + 8 i
-      auto load_weights = [&](int n) {
-        const uint16_t* terms = reinterpret_cast<const uint16_t*>(table + C::kTabW);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = j_own + 8 * i, e0 = there(j, n) ? exponent(j, n) : 0, e1 = there(j + 1, n) ? exponent(j + 1, n) : 0;
-#pragma unroll
-          for (int t = 0; t < 3; ++t) weights[t][i] = (uint32_t)terms[t * 66 + e0] | (uint32_t)terms[t * 66 + e1] << 16;
-        }
-      };
-      if constexpr (BF16) load_weights(kChunk);
       auto weigh = [&](int c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
         const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + C::kOffC;
         if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
         if (owner) {
-          if (BF16 && n < kChunk) load_weights(n);
+          uint32_t weights[3][4];   // of this thread's pairs of rows
+          if constexpr (BF16) {
+            const uint16_t* terms = reinterpret_cast<const uint16_t*>(table + C::kTabW);
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+              if (t == 2 && !third) break;
+              uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabPairs + t * 32 + half * 16 + (lane & 3) * 4);
+              if (n < kChunk) w = end_weights(terms + t * 66, j_own, n, lag, reverse);
+              weights[t][0] = w.x; weights[t][1] = w.y; weights[t][2] = w.z; weights[t][3] = w.w;
+            }
+          }
           const uint32_t to = tmem + lanes + C::kColC + (third ? 0 : (c & 1) * 64) + half * 16;
           // (matrices of a load: rows j .. j + 7 with columns d, d + 8; rows j + 8 .. j + 15 with the same)
           const int row = half * 32 + (lane & 7) + ((lane >> 4) << 3), col = quarter * 32 + (lane & 8);
@@ -496,11 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int j = j_own + 8 * (i / 2);
-                float2 f = unpack2<BF16>(v[i]);
+                float2 f = unpack16<BF16>(v[i]);
                 f.x *= power[there(j, n) ? exponent(j, n) : 0];
                 f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0];
                 a[i] = pack2<BF16>(f.x, f.y);
-                const float2 t = unpack2<BF16>(a[i]);
+                const float2 t = unpack16<BF16>(a[i]);
                 e[i] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
               }
             }
@@ -522,32 +585,48 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         arrive(b_bt_full + 8 * (c & 1));
         return true;
       };
-      bool ok = (states_only || put_state(0)) && (chunks == 0 || weigh(0));
-      for (int c = 0; c < chunks && ok; ++c) {
-        const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
-        // (in front of T, which is then being formed; with three terms behind it)
-        if (!third && c + 1 < chunks && !weigh(c + 1)) break;
-        if (!wait(b_t_full, (uint32_t)(c & 1))) break;
-        tc_fence_after();
-        if (owner) {
-          const float keep = power[n];
+      // One place each for the next C~ and the state's step (their code is long): C~ in front of T, which is then being formed, with three terms behind
+      // it.  c = -1: the first C~ and the first state.
+      bool ok = chunks > 0;
+      for (int c = -1; c < chunks && ok; ++c) {
+#pragma unroll 1
+        for (int turn = 0; turn < 2 && ok; ++turn) {
+          if ((turn == 0) != third) {
+            if (c + 1 < chunks) ok = weigh(c + 1);
+            continue;
+          }
+          if (c >= 0) {
+            const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
+            if (!(ok = wait(b_t_full, (uint32_t)(c & 1)))) break;
+            tc_fence_after();
+            if (owner) {
+              const uint64_t keep = pack2(power[n], power[n]);
 #pragma unroll
-          for (int i0 = 0; i0 < kCols; i0 += 32) {
-            uint32_t r[32];
-            tmem_ld32(tmem + lanes + C::kColT + d1 + i0, r);
-            tc_wait_ld();
+              for (int i0 = 0; i0 < kCols; i0 += 32) {
+                uint32_t r[32];
+                tmem_ld32(tmem + lanes + C::kColT + d1 + i0, r);
+                tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i0 + i] = fmaf(keep, x[i0 + i], BF16 ? __uint_as_float(r[i]) : key_scale * __uint_as_float(r[i]));
+                for (int i = 0; i < 32; i += 2) {
+                  uint64_t t = pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                  if constexpr (!BF16) t = mul2(pack2(key_scale, key_scale), t);
+                  const float2 f = unpack2(fma2(keep, pack2(x[i0 + i], x[i0 + i + 1]), t));
+                  x[i0 + i] = f.x;
+                  x[i0 + i + 1] = f.y;
+                }
+              }
+            }
+            tc_fence_before();
+            arrive(b_t_empty);
+          }
+          if (!states_only && c + 1 < chunks) {
+            if (c >= 0) {
+              if (!(ok = wait(b_x_empty, (uint32_t)(c & 1)))) break;
+              tc_fence_after();
+            }
+            ok = put_state(c + 1);
           }
         }
-        tc_fence_before();
-        arrive(b_t_empty);
-        if (!states_only && c + 1 < chunks) {
-          if (!wait(b_x_empty, (uint32_t)(c & 1))) break;
-          tc_fence_after();
-          ok = put_state(c + 1);
-        }
-        if (third && ok && c + 1 < chunks) ok = weigh(c + 1);
       }
       if (owner && !*abort_flag) {
         float* to = states_only ? work : args.segments == 1 && s.x_last && q.state >= 0 ? s.x_last + (q.state * p.heads + h) * matrix : nullptr;
@@ -564,95 +643,131 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const int quarter = warp & 3, d2 = quarter * 32 + lane;
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const bool owner = quarter * 32 < D2;
-      uint16_t* y16 = static_cast<uint16_t*>(s.y) + y0;
-      float* y32 = static_cast<float*>(s.y) + y0;
       const int64_t pitch = s.ys[2];
       const bool y_f32 = s.y_f32 != 0;
-      const int odd = lane & 1;
+      const int group = lane >> 2, pair = (lane & 3) * 2;
+      const uint32_t mine = base + C::kOffY + quarter * kYBytes;
+      // 16 bytes of a row of this warp's 64 rows of 32 columns, swizzled as the stores out of it expect
+      auto piece = [&](int row, int at) { return mine + (uint32_t)(row * 64) + (((uint32_t)at ^ ((uint32_t)(row >> 1) & 3u)) << 4); };
+      uint64_t row_w[8];   // of rows 8 g + pair and the next
+#pragma unroll
+      for (int g = 0; g < 8; ++g) row_w[g] = *reinterpret_cast<const uint64_t*>(table + C::kTabRow + 8 * g + pair);
+      const bool leader = elect_one();
       for (int c = 0; c < chunks; ++c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
         const int low = reverse ? kChunk - n : 0, high = reverse ? kChunk : n;   // the tile's rows
         const int token = token_of(c);
         if (!wait(b_o_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
         tc_fence_after();
+        auto value = [&](int r, float state, float part) {   // of a lane's own column
+          const float w = table[C::kTabRow + r];
+          return BF16 ? fmaf(w, state, part) : fmaf(table[C::kTabP + (c & 1) * 64 + r], part, w * table[C::kTabX + (c & 3) * 128 + d2] * state);
+        };
         if (owner) {
-          const uint32_t t_o = tmem + lanes + C::kColO;
-          const float xs = BF16 ? 1.f : table[C::kTabX + (c & 3) * 128 + d2];
-          const float* row_w = table + C::kTabRow;
-          const float* row_p = table + C::kTabP + (c & 1) * 64;
-          float probe = 0.f;   // NaN as soon as a value of the row part is not finite
-          auto value = [&](float state, float part, float w, float ps) { return BF16 ? fmaf(w, state, part) : fmaf(ps, part, w * xs * state); };
-          // all of the lane's values first, so that the columns are free for the next chunk while these are stored
-          float e[kChunk];
-#pragma unroll
-          for (int r0 = 0; r0 < kChunk; r0 += 16) {
-            uint32_t u[16], v[16];
-            tmem_ld16(t_o + r0, u);
-            tmem_ld16(t_o + 64 + r0, v);
-            tc_wait_ld();
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-              const float4 w = *reinterpret_cast<const float4*>(row_w + r0 + r);
-              float4 ps = make_float4(1.f, 1.f, 1.f, 1.f);
-              if constexpr (!BF16) ps = *reinterpret_cast<const float4*>(row_p + r0 + r);
-              const float ww[4] = {w.x, w.y, w.z, w.w}, pp[4] = {ps.x, ps.y, ps.z, ps.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float part = __uint_as_float(v[r + k]);
-                probe = fmaf(part, 0.f, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
-                e[r0 + r + k] = value(__uint_as_float(u[r + k]), part, ww[k], pp[k]);
-              }
-            }
-          }
-          const bool again = probe != probe;
-          if (__any_sync(0xffffffffu, again)) {   // (the tile of C may have been given back: its column comes from memory once more)
-            const uint32_t pt = base + C::kOffP + (c & 1) * kBlock;
-            const uint16_t* ct = static_cast<const uint16_t*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + (q.row0 + token) * s.cs[2] + d2;
-#pragma unroll
-            for (int r = 0; r < kChunk; ++r) {
-              uint32_t u;
-              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(u) : "r"(t_o + r) : "memory");
-              tc_wait_ld();
-              if (again && r >= low && r < high) {
-                float part = 0.f;
+          if (leader) bulk_wait_read0();   // (the last chunk's stores have read its rows)
+          __syncwarp();
+          uint64_t probe = 0;   // NaN as soon as a value of the row part is not finite
+          if (y_f32) {          // partial sums: a column to a lane
+            float* at = static_cast<float*>(s.y) + y0 + (int64_t)token * pitch + d2;
 #pragma unroll 1
-                for (int j = reverse ? r : low; j < (reverse ? high : r + 1); ++j)
-                  part = fmaf(lds16<BF16>(pt + r * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(r & 7)) << 4) + (j & 7) * 2), unpack2<BF16>(ct[j * s.cs[2]]).x, part);
-                e[r] = value(__uint_as_float(u), part, row_w[r], BF16 ? 1.f : row_p[r]);
-              }
-            }
-          }
-          tc_fence_before();
-          arrive(b_o_empty + 8 * (c & 1));
-          if (y_f32) {
-            float* at = y32 + (int64_t)token * pitch + d2;
+            for (int r0 = 0; r0 < kChunk; r0 += 8) {
+              uint32_t u[8], v[8];
+              tmem_ld8(tmem + lanes + C::kColO + r0, u);
+              tmem_ld8(tmem + lanes + C::kColO + 64 + r0, v);
+              tc_wait_ld();
 #pragma unroll
-            for (int r = 0; r < kChunk; ++r) {
-              if (r >= low && r < high) *at = e[r];
-              at += pitch;
+              for (int r = 0; r < 8; ++r) {
+                const float f = value(r0 + r, __uint_as_float(u[r]), __uint_as_float(v[r]));
+                probe = fma2(pack2(__uint_as_float(v[r]), 0.f), 0ull, probe);
+                if (r0 + r >= low && r0 + r < high) *at = f;
+                at += pitch;
+              }
             }
           } else {
-            // 16-bit values in pairs of columns: even lanes of the even rows, odd lanes of the odd ones
-            uint16_t* at = y16 + (int64_t)(token + odd) * pitch + (d2 & ~1);
+            // 16 lanes at a time, a thread with two rows of the chunk in eight groups and two lanes: pairs along the rows, transposed on the way to shared
+            // memory
 #pragma unroll
-            for (int r0 = 0; r0 < kChunk; r0 += 16) {
-              uint32_t v[8];
-#pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const float got = __shfl_xor_sync(0xffffffffu, odd ? e[r0 + i] : e[r0 + i + 1], 1);
-                v[i / 2] = pack2<BF16>(odd ? got : e[r0 + i], odd ? e[r0 + i + 1] : got);
+            for (int up = 0; up < 32; up += 16) {
+              const uint32_t t_o = tmem + lanes + ((uint32_t)up << 16) + C::kColO;
+              uint64_t xs[2] = {0, 0};
+              if constexpr (!BF16) {
+                const float* of = table + C::kTabX + (c & 3) * 128 + quarter * 32 + up + group;
+                xs[0] = pack2(of[0], of[0]);
+                xs[1] = pack2(of[8], of[8]);
               }
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                if (r0 + i + odd >= low && r0 + i + odd < high) *reinterpret_cast<uint32_t*>(at) = v[i / 2];
-                at += 2 * pitch;
+              for (int half = 0; half < 2; ++half) {
+                uint32_t u[16], v[16], m[8];
+                tmem_ld_16x256b_x4(t_o + half * 32, u);
+                tmem_ld_16x256b_x4(t_o + 64 + half * 32, v);
+                tc_wait_ld();
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  const uint64_t w = row_w[half * 4 + g];
+                  uint64_t ps = 0;
+                  if constexpr (!BF16) ps = *reinterpret_cast<const uint64_t*>(table + C::kTabP + (c & 1) * 64 + (half * 4 + g) * 8 + pair);
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {   // lanes group and group + 8
+                    const uint64_t state = pack2(__uint_as_float(u[4 * g + 2 * k]), __uint_as_float(u[4 * g + 2 * k + 1]));
+                    const uint64_t part = pack2(__uint_as_float(v[4 * g + 2 * k]), __uint_as_float(v[4 * g + 2 * k + 1]));
+                    probe = fma2(part, 0ull, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
+                    const float2 f = unpack2(BF16 ? fma2(w, state, part) : fma2(ps, part, mul2(mul2(w, xs[k]), state)));
+                    m[2 * g + k] = pack2<BF16>(f.x, f.y);
+                  }
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g += 2)   // matrices: rows 8 g .. of columns up .. and up + 8 .., rows 8 (g + 1) .. of the same
+                  stmatrix_x4_trans(piece((half * 4 + g + (lane >> 4)) * 8 + (lane & 7), up / 8 + ((lane >> 3) & 1)), m + 2 * g);
               }
             }
           }
-        } else {
-          arrive(b_o_empty + 8 * (c & 1));
+          const float2 two = unpack2(probe);
+          if (__any_sync(0xffffffffu, two.x + two.y != 0.f)) {
+            // columns that came out not finite are summed again, a lane to each, over what a row may see (the tile of C may have been given
+            // back: its column comes from memory once more)
+            __syncwarp();
+            const uint32_t pt = base + C::kOffP + (c & 1) * kBlock;
+            const uint16_t* ct = static_cast<const uint16_t*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + (q.row0 + token) * s.cs[2] + d2;
+#pragma unroll 1
+            for (int r = low; r < high; ++r) {
+              uint32_t u, v;
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(u) : "r"(tmem + lanes + C::kColO + r) : "memory");
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(tmem + lanes + C::kColO + 64 + r) : "memory");
+              tc_wait_ld();
+              float part = __uint_as_float(v);
+              if (!(fabsf(part) < INFINITY)) {
+                part = 0.f;
+                for (int j = reverse ? r : low; j < (reverse ? high : r + 1); ++j)
+                  part = fmaf(lds16<BF16>(pt + r * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(r & 7)) << 4) + (j & 7) * 2), unpack16<BF16>(ct[j * s.cs[2]]).x, part);
+              }
+              const float f = value(r, __uint_as_float(u), part);
+              if (y_f32) static_cast<float*>(s.y)[y0 + (int64_t)(token + r) * pitch + d2] = f;
+              else sts16(piece(r, lane >> 3) + (lane & 7) * 2, pack2<BF16>(f, 0.f));
+            }
+          }
+        }
+        tc_fence_before();
+        arrive(b_o_empty + 8 * (c & 1));
+        if (owner && !y_f32) {
+          if (n == kChunk) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (leader) {
+              tma_store_4d(&maps.y[which], mine, quarter * 32, (int)q.row0 + token, h, p.starts ? 0 : b);
+              bulk_commit();
+            }
+          } else {   // not the rows beside the sequence
+            __syncwarp();
+            for (int e = lane; e < n * 4; e += 32) {
+              const int r = low + e / 4;
+              const uint4 f = lds128(piece(r, e & 3));
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(s.y) + y0 + (int64_t)(token + r) * pitch + quarter * 32 + (e & 3) * 8) = f;
+            }
+          }
         }
       }
+      if (leader) bulk_wait_all();   // shared memory outlives the stores that read it
+      __syncwarp();
     }
 
     // ---- teardown ----
@@ -799,7 +914,12 @@ bool scan_sm100_supported(const Params& p) {
       for (int d = 0; d < 3; ++d)
         if (extent[d] > 1 && (stride[t][d] <= 0 || stride[t][d] % 8 != 0 || stride[t][d] >= (1ll << 38))) return false;
     }
-    if (!s.y_f32 && ((uintptr_t)s.y % 4 != 0 || s.ys[0] % 2 != 0 || s.ys[1] % 2 != 0 || s.ys[2] % 2 != 0)) return false;
+    if (!s.y_f32) {
+      if ((uintptr_t)s.y % 16 != 0) return false;
+      const int64_t extent[3] = {p.starts ? 1 : p.batch, p.heads, rows};
+      for (int d = 0; d < 3; ++d)
+        if (extent[d] > 1 && (s.ys[d] <= 0 || s.ys[d] % 8 != 0 || s.ys[d] >= (1ll << 38))) return false;
+    }
   }
   return true;
 }
@@ -842,6 +962,8 @@ cudaError_t launch_scan_sm100(const Params& p, int num_sms, float* work, int64_t
     args.ib[i] = map_of(s.b, s.bs, s.d1, s.b_group);
     args.ic[i] = map_of(s.c, s.cs, s.d2, s.c_group);
     if (args.ia[i] < 0 || args.ib[i] < 0 || args.ic[i] < 0) return cudaErrorInvalidValue;
+    const int64_t st[3] = {s.ys[0], s.ys[1], rows > 1 ? s.ys[2] : s.d2};
+    if (!s.y_f32 && !tmap::encode_bhsd(&maps.y[i], dt, 2, CU_TENSOR_MAP_SWIZZLE_64B, s.y, s.d2, rows, p.heads, batch, st, 32, kChunk)) return cudaErrorInvalidValue;
   }
   args.segments = work && work_bytes >= scan_sm100_bytes(p, num_sms) ? segments_of(p, num_sms) : 1;
   const int64_t per = (p.seq_len + args.segments - 1) / args.segments;
