@@ -212,14 +212,15 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   const int b = item / p.heads, h = item - b * p.heads;
   const Scan& s = p.scan[which];
   const bool states_only = args.states_only != 0;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (shuffled from lane 0: what depends on it is known to be the same in a warp, and stays in uniform registers)
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool reverse = s.reverse != 0;
   const uint64_t wait_ns = args.wait_ns;
 
   const Sequence q = sequence_of(p, b);
   const int64_t t0 = (int64_t)seg * args.seg_len;
   const int rows = q.bad || q.n <= t0 ? 0 : (int)(q.n - t0 < args.seg_len ? q.n - t0 : args.seg_len);
-  const int chunks = (rows + kChunk - 1) / kChunk;
+  const int chunks = __shfl_sync(0xffffffffu, (rows + kChunk - 1) / kChunk, 0);
   const int64_t y0 = (p.starts ? 0 : b * s.ys[0]) + h * s.ys[1] + q.row0 * s.ys[2];
   // rows from tile row r of chunk c: token_of(c) + r, of the sequence
   auto token_of = [&](int c) { return reverse ? (int)(q.n - t0) - (c + 1) * kChunk : (int)t0 + c * kChunk; };
@@ -283,13 +284,15 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_ptr;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
     const float* power = table + C::kTabPower;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       bool done = mbar_try_wait(bar, parity);
       if (!done) done = wait_on(bar, parity, abort_flag, wait_ns);
       return __all_sync(0xffffffffu, done) != 0;
     };
+    // a single thread's
+    auto wait1 = [&](uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || wait_on(bar, parity, abort_flag, wait_ns); };
     auto arrive = [&](uint32_t bar) {
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
@@ -297,102 +300,97 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
 
     if (warp == kWarpLoad) {
       // ---- tiles in ----
-      const bool leader = elect_one();
-      const CUtensorMap* ma = &maps.t[args.ia[which]];
-      const CUtensorMap* mb = &maps.t[args.ib[which]];
-      const CUtensorMap* mc = &maps.t[args.ic[which]];
-      const int ha = h / s.a_group, hb = h / s.b_group, hc = h / s.c_group, bb = p.starts ? 0 : b;
-      for (int c = 0; c < chunks; ++c) {
-        const int st = c % C::kStages;
-        if (!wait(b_empty + 8 * st, (uint32_t)((c / C::kStages) & 1) ^ 1u)) break;
-        if (leader && !args.withhold) {
-          const uint32_t bar = b_full + 8 * st, dst = base + (uint32_t)(st * C::kStageBytes);
-          const int row = (int)q.row0 + token_of(c);
-          mbar_expect_tx(bar, (uint32_t)(states_only ? C::kStageBytes - C::kOffB : C::kStageBytes));
+      if (elect_one()) {
+        const CUtensorMap* ma = &maps.t[args.ia[which]];
+        const CUtensorMap* mb = &maps.t[args.ib[which]];
+        const CUtensorMap* mc = &maps.t[args.ic[which]];
+        const int ha = h / s.a_group, hb = h / s.b_group, hc = h / s.c_group, bb = p.starts ? 0 : b;
+        int at = 0;
+        uint32_t phase = 1;
+        for (int c = 0; c < chunks; ++c) {
+          if (!wait1(b_empty + 8 * at, phase)) break;
+          if (!args.withhold) {
+            const uint32_t bar = b_full + 8 * at, dst = base + (uint32_t)(at * C::kStageBytes);
+            const int row = (int)q.row0 + token_of(c);
+            mbar_expect_tx(bar, (uint32_t)(states_only ? C::kStageBytes - C::kOffB : C::kStageBytes));
 #pragma unroll
-          for (int i = 0; i < C::kN1; ++i) {
-            if (!states_only) tma_load_4d(dst + i * kBlock, ma, bar, i * 64, row, ha, bb);
-            tma_load_4d(dst + C::kOffB + i * kBlock, mb, bar, i * 64, row, hb, bb);
+            for (int i = 0; i < C::kN1; ++i) {
+              if (!states_only) tma_load_4d(dst + i * kBlock, ma, bar, i * 64, row, ha, bb);
+              tma_load_4d(dst + C::kOffB + i * kBlock, mb, bar, i * 64, row, hb, bb);
+            }
+#pragma unroll
+            for (int i = 0; i < C::kN2; ++i) tma_load_4d(dst + C::kOffC + i * kBlock, mc, bar, i * 64, row, hc, bb);
           }
-#pragma unroll
-          for (int i = 0; i < C::kN2; ++i) tma_load_4d(dst + C::kOffC + i * kBlock, mc, bar, i * 64, row, hc, bb);
+          if (++at == C::kStages) at = 0, phase ^= 1u;
         }
-        __syncwarp();
       }
     } else if (warp == kWarpMma) {
       // ---- products ----
-      const bool leader = elect_one();
       constexpr uint32_t kTransposeA = 1u << 15;
-      constexpr uint32_t idesc_s = make_idesc(128, 64, BF16, false);                  // A and B along their rows
-      constexpr uint32_t idesc_x = make_idesc(128, 64, BF16, false);                  // X^T from tensor memory, A along its rows
+      constexpr uint32_t idesc_rows = make_idesc(128, 64, BF16, false);               // S: A and B along their rows; state part: X^T from tensor memory
       constexpr uint32_t idesc_p = make_idesc(128, 64, BF16, false) | kTransposeA;    // C^T, P along its rows
       constexpr uint32_t idesc_t = make_idesc(128, D1, BF16, true);                   // C~^T from tensor memory, B across its rows
       // (a descriptor's start address is counted in 16 bytes; what is added to it stays within its field)
       const uint64_t rows_desc = make_smem_desc(base, 16, 1024), cols_desc = make_smem_desc(base, kBlock, 1024);
-      auto stage = [&](int c) { return (uint64_t)((c % C::kStages) * (C::kStageBytes >> 4)); };
       auto row_step = [](int k) { return (uint64_t)(((k / 4) * kBlock + (k % 4) * 32) >> 4); };   // 16 elements along a row
-      auto scores = [&](int c) {
-        if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
-        if (!wait(b_s_empty, (uint32_t)(c & 1) ^ 1u)) return false;
-        tc_fence_after();
-        if (leader) {
-          const uint64_t ad = rows_desc + stage(c), bd = ad + (C::kOffB >> 4);
+      // One thread for the waits too: a wait of the whole warp takes 100 cycles where there is nothing to wait for.
+      if (elect_one()) {
+        const bool third = args.terms == 3;
+        int at = 0, ahead = 0;   // the chunk's stage; the next chunk whose scores are to be issued
+        uint32_t phase = 0;
+        for (int c = 0; c < chunks; ++c) {
+          const uint64_t stage = (uint64_t)(at * (C::kStageBytes >> 4));
+          const int next = at + 1 == C::kStages ? 0 : at + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          // This chunk's scores, if they are not ahead; the next one's if its tiles are there; what is added to the state; and only then what waits for the
+          // state and for P.
+          bool ok = true;
+          while (!states_only && ahead <= c + 1 && ahead < chunks) {
+            const int slot = ahead == c ? at : next;
+            const uint32_t slot_phase = ahead == c ? phase : next_phase;
+            if (ahead > c && !mbar_test(b_full + 8 * slot, slot_phase)) break;
+            if (!(ok = wait1(b_full + 8 * slot, slot_phase) && wait1(b_s_empty, (uint32_t)(ahead & 1) ^ 1u))) break;
+            tc_fence_after();
+            const uint64_t ad = rows_desc + (uint64_t)(slot * (C::kStageBytes >> 4)), bd = ad + (C::kOffB >> 4);
 #pragma unroll
-          for (int k = 0; k < D1 / 16; ++k) mma_ss(tmem + C::kColS, ad + row_step(k), bd + row_step(k), idesc_s, k > 0);
-          tc_commit(b_s_full + 8 * (c & 1));
-        }
-        __syncwarp();
-        return true;
-      };
-      bool ok = states_only || chunks == 0 || scores(0);
-      for (int c = 0; c < chunks && ok; ++c) {
-        const uint64_t ct = cols_desc + stage(c) + (C::kOffC >> 4);
-        const uint32_t o = tmem + C::kColO;
-        // the next scores first if their tiles are there, as B~ of the next chunk waits for them; what is added to the state; and only then what waits
-        // for the state and for P
-        bool ahead = !states_only && c + 1 < chunks;
-        if (ahead && __all_sync(0xffffffffu, mbar_test(b_full + 8 * ((c + 1) % C::kStages), (uint32_t)(((c + 1) / C::kStages) & 1)))) {
-          if (!(ok = scores(c + 1))) break;
-          ahead = false;
-        }
-        if (!(ok = wait(b_bt_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
-        if (!(ok = wait(b_t_empty, (uint32_t)(c & 1) ^ 1u))) break;
-        tc_fence_after();
-        if (leader) {
-          const uint64_t bt = cols_desc + stage(c) + (C::kOffB >> 4);
-          for (int term = args.terms - 1; term >= 0; --term) {   // the smallest first (fp16 holds its second 2^11 times as large)
-            const uint32_t at = tmem + C::kColC + (args.terms == 3 ? 0 : (c & 1) * 64) + term * 32;
+            for (int k = 0; k < D1 / 16; ++k) mma_ss(tmem + C::kColS, ad + row_step(k), bd + row_step(k), idesc_rows, k > 0);
+            tc_commit(b_s_full + 8 * (ahead & 1));
+            ++ahead;
+          }
+          if (!ok || !wait1(b_full + 8 * at, phase) || !wait1(b_bt_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)) || !wait1(b_t_empty, (uint32_t)(c & 1) ^ 1u)) break;
+          tc_fence_after();
+          const uint64_t ct = cols_desc + stage + (C::kOffC >> 4), bt = cols_desc + stage + (C::kOffB >> 4);
+          const uint32_t first = tmem + C::kColC + (third ? 0 : (c & 1) * 64);
+          // the smallest term first (fp16 holds its second 2^11 times as large)
+          if (third) {
 #pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k) {
-              if (!BF16 && term == 0 && k == 0) mma_ts_down11(tmem + C::kColT, at, bt, idesc_t);
-              else mma_ts(tmem + C::kColT, at + k * 8, bt + k * (2048 >> 4), idesc_t, term < args.terms - 1 || k > 0);
-            }
+            for (int k = 0; k < kChunk / 16; ++k) mma_ts(tmem + C::kColT, first + 64 + k * 8, bt + k * (2048 >> 4), idesc_t, k > 0);
+          }
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k) mma_ts(tmem + C::kColT, first + 32 + k * 8, bt + k * (2048 >> 4), idesc_t, k > 0 || third);
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k) {
+            if (!BF16 && k == 0) mma_ts_down11(tmem + C::kColT, first, bt, idesc_t);
+            else mma_ts(tmem + C::kColT, first + k * 8, bt + k * (2048 >> 4), idesc_t, 1u);
           }
           tc_commit(b_t_full);
-          if (states_only) tc_commit(b_empty + 8 * (c % C::kStages));
-        }
-        __syncwarp();
-        if (states_only) continue;
-        if (!(ok = wait(b_x_full, (uint32_t)(c & 1)))) break;
-        if (c > 0 && !(ok = wait(b_o_empty + 8 * ((c - 1) & 1), (uint32_t)(((c - 1) >> 1) & 1)))) break;
-        tc_fence_after();
-        if (leader) {
+          if (!states_only) {
+            if (!wait1(b_x_full, (uint32_t)(c & 1)) || (c > 0 && !wait1(b_o_empty + 8 * ((c - 1) & 1), (uint32_t)(((c - 1) >> 1) & 1)))) break;
+            tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < D1 / 16; ++k) mma_ts(o, tmem + C::kColX + k * 8, rows_desc + stage(c) + row_step(k), idesc_x, k > 0);
-          tc_commit(b_x_empty);
-        }
-        __syncwarp();
-        if (!(ok = wait(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)))) break;
-        tc_fence_after();
-        if (leader) {
+            for (int k = 0; k < D1 / 16; ++k) mma_ts(tmem + C::kColO, tmem + C::kColX + k * 8, rows_desc + stage + row_step(k), idesc_rows, k > 0);
+            tc_commit(b_x_empty);
+            if (!wait1(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
+            tc_fence_after();
+            const uint64_t pd = rows_desc + (uint64_t)((C::kOffP + (c & 1) * kBlock) >> 4);
 #pragma unroll
-          for (int k = 0; k < kChunk / 16; ++k)
-            mma_ss(o + 64, ct + k * (2048 >> 4), rows_desc + (uint64_t)((C::kOffP + (c & 1) * kBlock + k * 32) >> 4), idesc_p, k > 0);
-          tc_commit(b_o_full + 8 * (c & 1));
-          tc_commit(b_empty + 8 * (c % C::kStages));
+            for (int k = 0; k < kChunk / 16; ++k) mma_ss(tmem + C::kColO + 64, ct + k * (2048 >> 4), pd + k * (32 >> 4), idesc_p, k > 0);
+            tc_commit(b_o_full + 8 * (c & 1));
+          }
+          tc_commit(b_empty + 8 * at);
+          at = next;
+          phase = next_phase;
         }
-        __syncwarp();
-        if (ahead && !(ok = scores(c + 1))) break;
       }
     } else if (warp < kWarpLoad) {
       // ---- P ----
