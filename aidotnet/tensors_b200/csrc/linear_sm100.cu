@@ -402,52 +402,59 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         for (int c = 0; c < chunks; ++c) {
           if (!wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
           tc_fence_after();
-          uint32_t r[kChunk];
-#pragma unroll
-          for (int j0 = 0; j0 < kChunk; j0 += 32) tmem_ld32(t_s + j0, r + j0);
-          tc_wait_ld();
-          tc_fence_before();
-          arrive(b_s_empty);   // (the next scores need not wait for what follows)
-          uint64_t x[kChunk / 2], probe = 0;
-#pragma unroll
-          for (int j = 0; j < kChunk; j += 4) {
-            const Pair2 w = lds_pairs(weight + j);
-            x[j / 2] = mul2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), w.a);
-            x[j / 2 + 1] = mul2(pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), w.b);
-            probe = fma2(x[j / 2], 0ull, fma2(x[j / 2 + 1], 0ull, probe));
-          }
-          const float2 odd_ones = unpack2(probe);
-          if (__any_sync(0xffffffffu, odd_ones.x + odd_ones.y != 0.f)) {   // NaN: a score is not finite.  Behind the row it counts for nothing.
-#pragma unroll
-            for (int j = 0; j < kChunk; j += 2) {
-              const float2 f = unpack2(x[j / 2]);
-              x[j / 2] = pack2(reverse ? (j < i ? 0.f : f.x) : (j > i ? 0.f : f.x), reverse ? (j + 1 < i ? 0.f : f.y) : (j + 1 > i ? 0.f : f.y));
-            }
-          }
           if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
+          const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
           uint64_t to = 0;
           if constexpr (!BF16) {
             float most = 0.f, up, back;
+#pragma unroll 1
+            for (int j0 = 0; j0 < kChunk; j0 += 16) {
+              uint32_t r[16];
+              tmem_ld16(t_s + j0, r);
+              tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < kChunk / 2; ++j) {
-              const float2 f = unpack2(x[j]);
-              most = fmax3(most, fabsf(f.x), fabsf(f.y));
+              for (int j = 0; j < 16; j += 2) {
+                const uint64_t w = *reinterpret_cast<const uint64_t*>(weight + j0 + j);
+                const float2 f = unpack2(mul2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), w));
+                most = fmax3(most, fabsf(f.x), fabsf(f.y));   // (NaN behind the row counts for nothing, an infinity there would be NaN)
+              }
             }
             scale_of(most, up, back);
             to = pack2(up, up);
             table[C::kTabP + (c & 1) * 64 + i] = back;
           }
-          const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
+#pragma unroll 1
+          for (int j0 = 0; j0 < kChunk; j0 += 16) {
+            uint32_t r[16], v[8];
+            tmem_ld16(t_s + j0, r);
+            tc_wait_ld();
+            uint64_t x[8], probe = 0;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            uint32_t v[4];
+            for (int j = 0; j < 16; j += 4) {
+              const Pair2 w = lds_pairs(weight + j0 + j);
+              x[j / 2] = mul2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), w.a);
+              x[j / 2 + 1] = mul2(pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), w.b);
+              probe = fma2(x[j / 2], 0ull, fma2(x[j / 2 + 1], 0ull, probe));
+            }
+            const float2 odd_ones = unpack2(probe);
+            if (__any_sync(0xffffffffu, odd_ones.x + odd_ones.y != 0.f)) {   // NaN: a score is not finite.  Behind the row it counts for nothing.
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = unpack2(BF16 ? x[4 * u + k] : mul2(x[4 * u + k], to));
+              for (int j = 0; j < 16; j += 2) {
+                const float2 f = unpack2(x[j / 2]);
+                const int at = j0 + j;
+                x[j / 2] = pack2((reverse ? at < i : at > i) ? 0.f : f.x, (reverse ? at + 1 < i : at + 1 > i) ? 0.f : f.y);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float2 f = unpack2(BF16 ? x[k] : mul2(x[k], to));
               v[k] = pack2<BF16>(f.x, f.y);
             }
-            st_shared_v4(row + (((uint32_t)u ^ (uint32_t)(i & 7)) << 4), v[0], v[1], v[2], v[3]);
+            st_shared_v4(row + (((uint32_t)(j0 / 8) ^ (uint32_t)(i & 7)) << 4), v[0], v[1], v[2], v[3]);
+            st_shared_v4(row + (((uint32_t)(j0 / 8 + 1) ^ (uint32_t)(i & 7)) << 4), v[4], v[5], v[6], v[7]);
           }
+          tc_fence_before();
+          arrive(b_s_empty);
           fence_proxy_async_smem();
           arrive(b_p_full + 8 * (c & 1));
         }
@@ -531,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           // (matrices of a load: rows j .. j + 7 with columns d, d + 8; rows j + 8 .. j + 15 with the same)
           const int row = half * 32 + (lane & 7) + ((lane >> 4) << 3), col = quarter * 32 + (lane & 8);
           const uint32_t from = st + (col / 64) * kBlock + row * 128;
-#pragma unroll
+#pragma unroll 1
           for (int d = 0; d < 32; d += 16) {
             uint32_t v[8], a[8], e[8];
 #pragma unroll
@@ -647,9 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const uint32_t mine = base + C::kOffY + quarter * kYBytes;
       // 16 bytes of a row of this warp's 64 rows of 32 columns, swizzled as the stores out of it expect
       auto piece = [&](int row, int at) { return mine + (uint32_t)(row * 64) + (((uint32_t)at ^ ((uint32_t)(row >> 1) & 3u)) << 4); };
-      uint64_t row_w[8];   // of rows 8 g + pair and the next
-#pragma unroll
-      for (int g = 0; g < 8; ++g) row_w[g] = *reinterpret_cast<const uint64_t*>(table + C::kTabRow + 8 * g + pair);
       const bool leader = elect_one();
       for (int c = 0; c < chunks; ++c) {
         const int n = rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk;
@@ -684,39 +688,39 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           } else {
             // 16 lanes at a time, a thread with two rows of the chunk in eight groups and two lanes: pairs along the rows, transposed on the way to shared
             // memory
-#pragma unroll
-            for (int up = 0; up < 32; up += 16) {
-              const uint32_t t_o = tmem + lanes + ((uint32_t)up << 16) + C::kColO;
+#pragma unroll 1
+            for (int part_of = 0; part_of < 4; ++part_of) {
+              const int up = (part_of & 1) * 16, half = part_of >> 1;
+              const uint32_t t_o = tmem + lanes + ((uint32_t)up << 16) + C::kColO + half * 32;
+              uint32_t u[16], v[16], m[8];
+              tmem_ld_16x256b_x4(t_o, u);
+              tmem_ld_16x256b_x4(t_o + 64, v);
               uint64_t xs[2] = {0, 0};
               if constexpr (!BF16) {
                 const float* of = table + C::kTabX + (c & 3) * 128 + quarter * 32 + up + group;
                 xs[0] = pack2(of[0], of[0]);
                 xs[1] = pack2(of[8], of[8]);
               }
+              const uint64_t* row_w = reinterpret_cast<const uint64_t*>(table + C::kTabRow + half * 32 + pair);   // of rows 8 g + pair and the next, at 4 g
+              const uint64_t* row_p = reinterpret_cast<const uint64_t*>(table + C::kTabP + (c & 1) * 64 + half * 32 + pair);
+              tc_wait_ld();
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                uint32_t u[16], v[16], m[8];
-                tmem_ld_16x256b_x4(t_o + half * 32, u);
-                tmem_ld_16x256b_x4(t_o + 64 + half * 32, v);
-                tc_wait_ld();
+              for (int g = 0; g < 4; ++g) {
+                const uint64_t w = row_w[4 * g];
+                uint64_t ps = 0;
+                if constexpr (!BF16) ps = row_p[4 * g];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  const uint64_t w = row_w[half * 4 + g];
-                  uint64_t ps = 0;
-                  if constexpr (!BF16) ps = *reinterpret_cast<const uint64_t*>(table + C::kTabP + (c & 1) * 64 + (half * 4 + g) * 8 + pair);
-#pragma unroll
-                  for (int k = 0; k < 2; ++k) {   // lanes group and group + 8
-                    const uint64_t state = pack2(__uint_as_float(u[4 * g + 2 * k]), __uint_as_float(u[4 * g + 2 * k + 1]));
-                    const uint64_t part = pack2(__uint_as_float(v[4 * g + 2 * k]), __uint_as_float(v[4 * g + 2 * k + 1]));
-                    probe = fma2(part, 0ull, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
-                    const float2 f = unpack2(BF16 ? fma2(w, state, part) : fma2(ps, part, mul2(mul2(w, xs[k]), state)));
-                    m[2 * g + k] = pack2<BF16>(f.x, f.y);
-                  }
+                for (int k = 0; k < 2; ++k) {   // lanes group and group + 8
+                  const uint64_t state = pack2(__uint_as_float(u[4 * g + 2 * k]), __uint_as_float(u[4 * g + 2 * k + 1]));
+                  const uint64_t part = pack2(__uint_as_float(v[4 * g + 2 * k]), __uint_as_float(v[4 * g + 2 * k + 1]));
+                  probe = fma2(part, 0ull, probe);   // (of rows that are not there too: at worst the sums below are formed again for nothing)
+                  const float2 f = unpack2(BF16 ? fma2(w, state, part) : fma2(ps, part, mul2(mul2(w, xs[k]), state)));
+                  m[2 * g + k] = pack2<BF16>(f.x, f.y);
                 }
-#pragma unroll
-                for (int g = 0; g < 4; g += 2)   // matrices: rows 8 g .. of columns up .. and up + 8 .., rows 8 (g + 1) .. of the same
-                  stmatrix_x4_trans(piece((half * 4 + g + (lane >> 4)) * 8 + (lane & 7), up / 8 + ((lane >> 3) & 1)), m + 2 * g);
               }
+#pragma unroll
+              for (int g = 0; g < 4; g += 2)   // matrices: rows 8 g .. of columns up .. and up + 8 .., rows 8 (g + 1) .. of the same
+                stmatrix_x4_trans(piece((half * 4 + g + (lane >> 4)) * 8 + (lane & 7), up / 8 + ((lane >> 3) & 1)), m + 2 * g);
             }
           }
           const float2 two = unpack2(probe);
