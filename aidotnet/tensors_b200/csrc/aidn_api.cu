@@ -1144,12 +1144,25 @@ int aidn_rotary(const aidn_rotary_args* a, void* cu_stream) {
   return post_launch_check((cudaStream_t)cu_stream, "aidn_rotary", nullptr);
 }
 
+// Bytes for the states of segments.  (Without a device, where no call runs either, none.)
+static int64_t linear_segment_bytes(const aidn_linear_args& a, const aidn::lin::Params& p) {
+  int sms = 0;
+  if (a.path == AIDN_PATH_GENERIC || device_facts("", &sms) != AIDN_OK) {
+    g_err[0] = 0;
+    return 0;
+  }
+  return aidn::lin::scan_sm100_bytes(p, sms);
+}
+
 int64_t aidn_linear_attention_workspace_bytes(const aidn_linear_args* a) {
   g_err[0] = 0;
   aidn::lin::Params p;
   if (!a) return fail(AIDN_EINVAL, "linear_attention_workspace_bytes: null argument"), -1;
   if (linear_common("linear_attention_workspace_bytes", *a, p) != AIDN_OK) return -1;
-  return 0;
+  p.scans = 1;
+  p.scan[0].d1 = a->key_dim;
+  p.scan[0].d2 = a->value_dim;
+  return linear_segment_bytes(*a, p);
 }
 
 int aidn_linear_attention(const aidn_linear_args* a, void* cu_stream) {
@@ -1195,7 +1208,12 @@ int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linear_bwd_arg
   aidn::lin::Params p;
   if (!a) return fail(AIDN_EINVAL, "linear_attention_backward_workspace_bytes: null argument"), -1;
   if (linear_common("linear_attention_backward_workspace_bytes", a->fwd, p) != AIDN_OK) return -1;
-  return linear_partial_bytes(a->fwd, a->fwd.key_dim) + linear_partial_bytes(a->fwd, a->fwd.value_dim);
+  p.scans = 3;
+  for (int i = 0; i < 3; ++i) {
+    p.scan[i].d1 = i == 2 ? a->fwd.key_dim : a->fwd.value_dim;
+    p.scan[i].d2 = i == 2 ? a->fwd.value_dim : a->fwd.key_dim;
+  }
+  return linear_partial_bytes(a->fwd, a->fwd.key_dim) + linear_partial_bytes(a->fwd, a->fwd.value_dim) + linear_segment_bytes(a->fwd, p);
 }
 
 int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_stream) {
