@@ -1085,7 +1085,7 @@ cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int
   int launches = 0;
   *waits = a.path != AIDN_PATH_GENERIC && aidn::lin::scan_sm100_supported(p);
   return *waits ? aidn::lin::launch_scan_sm100(p, sms, reinterpret_cast<float*>(work), work_bytes, expire, stream, &launches)
-                : aidn::lin::launch_scan_generic(p, stream, &launches);
+                : aidn::lin::launch_scan_generic(p, sms, reinterpret_cast<float*>(work), work_bytes, stream, &launches);
 }
 int linear_check(const char* what, cudaStream_t stream, bool waits) {
   return post_launch_check(stream, what, waits && launch_check_enabled() ? aidn::lin::sm100_status() : nullptr, true);
@@ -1147,11 +1147,13 @@ int aidn_rotary(const aidn_rotary_args* a, void* cu_stream) {
 // Bytes for the states of segments.  (Without a device, where no call runs either, none.)
 static int64_t linear_segment_bytes(const aidn_linear_args& a, const aidn::lin::Params& p) {
   int sms = 0;
-  if (a.path == AIDN_PATH_GENERIC || device_facts("", &sms) != AIDN_OK) {
+  if (device_facts("", &sms) != AIDN_OK) {
     g_err[0] = 0;
     return 0;
   }
-  return aidn::lin::scan_sm100_bytes(p, sms);
+  // (which kernels serve a call depends on its pointers and strides too: enough for either)
+  const int64_t one = a.path != AIDN_PATH_GENERIC ? aidn::lin::scan_sm100_bytes(p, sms) : 0, other = aidn::lin::scan_generic_bytes(p, sms);
+  return one > other ? one : other;
 }
 
 int64_t aidn_linear_attention_workspace_bytes(const aidn_linear_args* a) {

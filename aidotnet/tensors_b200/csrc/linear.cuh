@@ -89,8 +89,20 @@ __device__ __forceinline__ float log2_decay(const float* decay, int h) {
   return fmaxf(g * kLog2e, -1e30f);
 }
 
-// a scan on FFMA, any sizes and types
-cudaError_t launch_scan_generic(const Params& p, cudaStream_t stream, int* launches);
+// Sequences cut into segments: a first launch leaves what each adds to the state in `work` ([scan][sequence, head][segment][d1][d2]),
+// launch_join turns those into the states before them and writes the last ones, and the scan then starts every segment from its own.
+struct Segments {
+  int32_t count;         // 1: uncut
+  int32_t rows;          // of a segment
+  int32_t states_only;   // the first launch
+  float* work;
+};
+// The scans first .. first + scans - 1, of matrix elements a state.
+cudaError_t launch_join(const Params& p, const Segments& g, int first, int scans, int matrix, cudaStream_t stream);
+
+// a scan on FFMA, any sizes and types.  Without its workspace long sequences are not cut.
+int64_t scan_generic_bytes(const Params& p, int num_sms);
+cudaError_t launch_scan_generic(const Params& p, int num_sms, float* work, int64_t work_bytes, cudaStream_t stream, int* launches);
 
 // 16-bit types with sizes of 64 and 128 on tcgen05 (csrc/linear_sm100.cu).  Without its workspace long sequences are not cut.
 bool scan_sm100_supported(const Params& p);

@@ -1,6 +1,7 @@
-// The scan of linear.cuh on FFMA: any type, any head sizes.  A CTA takes some columns of c (and of the state) for one sequence and head and walks
-// its rows in chunks, the state in shared memory in fp32; the chunk's products a . b are formed again for every slice of columns.  What
-// bounds it is arithmetic and the reads of shared memory that feed it.
+// The scan of linear.cuh on FFMA: any type, any head sizes.  A CTA takes some columns of c (and of the state) for one sequence and head, or one segment
+// of them, and walks its rows in chunks, the state in shared memory in fp32; the chunk's products a . b are formed again for every slice of
+// columns.  What bounds it is the reads of shared memory that feed the multiply-adds: all products are tiles of 2 x 2 (a . b, outputs) or
+// 4 x 2 (state) to a thread, read by fours along the sizes.  Few sequences and heads are cut into segments as on the tensor cores.
 #include "linear.cuh"
 
 namespace aidn {
@@ -11,9 +12,11 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 32;
 constexpr int kWidth = 32;   // columns of a slice
 
-__host__ __device__ constexpr int pitch_of(int d) { return d + 1; }   // (odd: rows of a column lie in different banks)
+__host__ __device__ constexpr int pitch_of(int d) { return d + 4; }   // (rows begin in different banks, fours stay aligned)
+constexpr int kPitchW = kWidth + 4, kPitchP = kChunk + 4;
+// shared memory in floats: A, B [chunk][d1], C and weighted C [chunk][width], X [d1][width], P [chunk][chunk], powers
 inline size_t smem_bytes(int d1) {
-  return sizeof(float) * (2 * kChunk * pitch_of(d1) + kChunk * kWidth + (size_t)d1 * kWidth + kChunk * (kChunk + 1) + kChunk + 1);
+  return sizeof(float) * (2 * kChunk * pitch_of(d1) + 2 * kChunk * kPitchW + (size_t)d1 * kPitchW + kChunk * kPitchP + kChunk + 4);
 }
 
 template <typename T>
@@ -22,107 +25,206 @@ __device__ __forceinline__ void put(const Scan& s, int64_t at, float x) {
   else static_cast<T*>(s.y)[at] = from_float<T>(x);
 }
 
+__device__ __forceinline__ float dot4(float4 a, float4 b, float c) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c)))); }
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const Params p) {
-  extern __shared__ float smem[];
+__global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ Params p, const Segments g) {
+  extern __shared__ float4 smem4[];
+  float* smem = reinterpret_cast<float*>(smem4);
   const Scan& s = p.scan[blockIdx.y];
   const int slices = (s.d2 + kWidth - 1) / kWidth;
-  if (blockIdx.x >= (int64_t)p.batch * p.heads * slices) return;   // (the scans of one launch may have different widths)
-  const int item = blockIdx.x / slices, w0 = (blockIdx.x - item * slices) * kWidth;
+  if (blockIdx.x >= (int64_t)p.batch * p.heads * g.count * slices) return;   // (the scans of one launch may have different widths)
+  const int slice = (int)(blockIdx.x % (unsigned)slices), w0 = slice * kWidth;
+  const int unit = (int)(blockIdx.x / (unsigned)slices), seg = unit % g.count, item = unit / g.count;
   const int b = item / p.heads, h = item - b * p.heads;
   const int width = s.d2 - w0 < kWidth ? s.d2 - w0 : kWidth;
   const int d1 = s.d1, pitch = pitch_of(d1), tid = threadIdx.x;
   float* A = smem;
   float* B = A + kChunk * pitch;
   float* C = B + kChunk * pitch;
-  float* X = C + kChunk * kWidth;
-  float* P = X + d1 * kWidth;
-  float* power = P + kChunk * (kChunk + 1);   // lam^0 .. lam^kChunk
+  float* Cw = C + kChunk * kPitchW;
+  float* X = Cw + kChunk * kPitchW;
+  float* P = X + d1 * kPitchW;
+  float* power = P + kChunk * kPitchP;   // lam^0 .. lam^kChunk
 
   const Sequence q = sequence_of(p, b);
+  const int64_t from = (int64_t)seg * g.rows;   // this segment's rows, counted as they are taken
+  const int64_t rows = q.bad || q.n <= from ? 0 : (q.n - from < g.rows ? q.n - from : g.rows);
   const T* a = static_cast<const T*>(s.a) + (p.starts ? 0 : b * s.as[0]) + (h / s.a_group) * s.as[1] + q.row0 * s.as[2];
   const T* bb = static_cast<const T*>(s.b) + (p.starts ? 0 : b * s.bs[0]) + (h / s.b_group) * s.bs[1] + q.row0 * s.bs[2];
   const T* c = static_cast<const T*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + q.row0 * s.cs[2] + w0;
   const int64_t y0 = (p.starts ? 0 : b * s.ys[0]) + h * s.ys[1] + q.row0 * s.ys[2] + w0;
-  if (q.bad) {
-    for (int64_t e = tid; e < q.n * width; e += kThreads) put<T>(s, y0 + (e / width) * s.ys[2] + e % width, __int_as_float(0x7fffffff));
-  } else {
-    const float g = log2_decay(p.decay, h);
-    if (tid <= kChunk) power[tid] = exp2f(g * tid);
-    const int64_t state = (q.state * p.heads + h) * (int64_t)s.d1 * s.d2;
+  const bool hand_on = g.count == 1 && s.x_last && q.state >= 0 && !q.bad;   // (a sequence without rows leaves its state too)
+  if (rows > 0 || hand_on) {
+    const float e2 = log2_decay(p.decay, h);
+    if (tid <= kChunk) power[tid] = exp2f(e2 * tid);
+    const int64_t matrix = (int64_t)d1 * s.d2;
+    const int64_t state = (q.state * p.heads + h) * matrix;
+    float* work = g.count > 1 ? g.work + (((int64_t)blockIdx.y * p.batch * p.heads + item) * g.count + seg) * matrix : nullptr;
     for (int e = tid; e < d1 * kWidth; e += kThreads) {
       const int r = e / kWidth, w = e - r * kWidth;
-      X[e] = s.x_first && q.state >= 0 && w < width ? s.x_first[state + (s.x_transposed ? (int64_t)(w0 + w) * d1 + r : (int64_t)r * s.d2 + w0 + w)] : 0.f;
+      float x = 0.f;
+      if (w < width && !g.states_only) {
+        if (work) x = work[(int64_t)r * s.d2 + w0 + w];
+        else if (s.x_first && q.state >= 0) x = s.x_first[state + (s.x_transposed ? (int64_t)(w0 + w) * d1 + r : (int64_t)r * s.d2 + w0 + w)];
+      }
+      X[r * kPitchW + w] = x;
     }
-    for (int64_t t0 = 0; t0 < q.n; t0 += kChunk) {
-      const int n = (int)(q.n - t0 < kChunk ? q.n - t0 : kChunk);
-      auto row = [&](int i) { return s.reverse ? q.n - 1 - (t0 + i) : t0 + i; };
+    for (int64_t t0 = 0; t0 < rows; t0 += kChunk) {
+      const int n = (int)(rows - t0 < kChunk ? rows - t0 : kChunk);
+      auto row = [&](int i) { return s.reverse ? q.n - 1 - (from + t0 + i) : from + t0 + i; };
       __syncthreads();
       for (int e = tid; e < kChunk * d1; e += kThreads) {
         const int i = e / d1, d = e - i * d1;
-        A[i * pitch + d] = i < n ? to_float(a[row(i) * s.as[2] + d]) : 0.f;
+        if (!g.states_only) A[i * pitch + d] = i < n ? to_float(a[row(i) * s.as[2] + d]) : 0.f;
         B[i * pitch + d] = i < n ? to_float(bb[row(i) * s.bs[2] + d]) : 0.f;
       }
       for (int e = tid; e < kChunk * kWidth; e += kThreads) {
         const int i = e / kWidth, w = e - i * kWidth;
-        C[e] = i < n && w < width ? to_float(c[row(i) * s.cs[2] + w]) : 0.f;
+        const float x = i < n && w < width ? to_float(c[row(i) * s.cs[2] + w]) : 0.f;
+        C[i * kPitchW + w] = x;
+        Cw[i * kPitchW + w] = i < n ? x * (power[n - s.lag - i] * s.key_scale) : 0.f;
       }
       __syncthreads();
-      {
-        // 2 x 2 products to a thread
-        const int i = tid / 16, j = tid % 16;
+      // this thread's rows and columns of the 32 x 32 products: i, i + 16 and j, j + 16
+      const int i = tid / 16, j = tid % 16;
+      if (!g.states_only) {
         float acc[2][2] = {};
-        for (int d = 0; d < d1; ++d) {
-          const float a0 = A[i * pitch + d], a1 = A[(i + 16) * pitch + d], b0 = B[j * pitch + d], b1 = B[(j + 16) * pitch + d];
-          acc[0][0] = fmaf(a0, b0, acc[0][0]);
-          acc[0][1] = fmaf(a0, b1, acc[0][1]);
-          acc[1][0] = fmaf(a1, b0, acc[1][0]);
-          acc[1][1] = fmaf(a1, b1, acc[1][1]);
+        for (int d = 0; d < d1; d += 4) {
+          const float4 a0 = *reinterpret_cast<const float4*>(A + i * pitch + d), a1 = *reinterpret_cast<const float4*>(A + (i + 16) * pitch + d);
+          const float4 b0 = *reinterpret_cast<const float4*>(B + j * pitch + d), b1 = *reinterpret_cast<const float4*>(B + (j + 16) * pitch + d);
+          acc[0][0] = dot4(a0, b0, acc[0][0]);
+          acc[0][1] = dot4(a0, b1, acc[0][1]);
+          acc[1][0] = dot4(a1, b0, acc[1][0]);
+          acc[1][1] = dot4(a1, b1, acc[1][1]);
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const int ii = i + 16 * x, jj = j + 16 * y;
-            if (jj <= ii) P[ii * (kChunk + 1) + jj] = acc[x][y] * (p.scale * power[ii - jj]);
+            if (jj <= ii) P[ii * kPitchP + jj] = acc[x][y] * (p.scale * power[ii - jj]);
           }
-      }
-      __syncthreads();
-      {
-        // a column of four rows to a thread
-        const int w = tid % kWidth, i0 = tid / kWidth;
-        float acc[4] = {};
-        for (int d = 0; d < d1; ++d) {
-          const float x = X[d * kWidth + w];
+        __syncthreads();
+        // outputs: rows i, i + 16, columns 2 j, 2 j + 1
+        float2 o[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        for (int d = 0; d < d1; d += 4) {
+          const float4 a0 = *reinterpret_cast<const float4*>(A + i * pitch + d), a1 = *reinterpret_cast<const float4*>(A + (i + 16) * pitch + d);
+          const float va[4] = {a0.x, a0.y, a0.z, a0.w}, vb[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[r] = fmaf(A[(i0 + 8 * r) * pitch + d], x, acc[r]);
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = *reinterpret_cast<const float2*>(X + (d + k) * kPitchW + 2 * j);
+            o[0].x = fmaf(va[k], x.x, o[0].x);
+            o[0].y = fmaf(va[k], x.y, o[0].y);
+            o[1].x = fmaf(vb[k], x.x, o[1].x);
+            o[1].y = fmaf(vb[k], x.y, o[1].y);
+          }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = i0 + 8 * r;
-          float y = acc[r] * (s.row_scale * exp2f(g * (i + s.lag)));
-          for (int j = 0; j <= i; ++j) y = fmaf(P[i * (kChunk + 1) + j], C[j * kWidth + w], y);
-          if (i < n && w < width) put<T>(s, y0 + row(i) * s.ys[2] + w, y);
+        for (int x = 0; x < 2; ++x) {
+          const int ii = i + 16 * x;
+          const float w = s.row_scale * exp2f(e2 * (ii + s.lag));
+          float2 y = make_float2(o[x].x * w, o[x].y * w);
+          for (int k = 0; k <= ii; ++k) {   // (not a row behind: what stands there may not be finite)
+            const float pk = P[ii * kPitchP + k];
+            const float2 ck = *reinterpret_cast<const float2*>(C + k * kPitchW + 2 * j);
+            y.x = fmaf(pk, ck.x, y.x);
+            y.y = fmaf(pk, ck.y, y.y);
+          }
+          if (ii < n) {
+            if (2 * j < width) put<T>(s, y0 + row(ii) * s.ys[2] + 2 * j, y.x);
+            if (2 * j + 1 < width) put<T>(s, y0 + row(ii) * s.ys[2] + 2 * j + 1, y.y);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
+      // the state: rows 4 i .. + 3 of every 64, columns 2 j, 2 j + 1
       const float keep = power[n];
-      for (int e = tid; e < d1 * kWidth; e += kThreads) {
-        const int r = e / kWidth, w = e - r * kWidth;
-        float acc = 0.f;
-        for (int j = 0; j < n; ++j) acc = fmaf(B[j * pitch + r] * power[n - s.lag - j], C[j * kWidth + w], acc);
-        X[e] = fmaf(keep, X[e], s.key_scale * acc);
+      for (int r = 4 * i; r < d1; r += 64) {
+        float2 x[4] = {};
+        for (int k = 0; k < n; ++k) {
+          const float4 bk = *reinterpret_cast<const float4*>(B + k * pitch + r);
+          const float2 ck = *reinterpret_cast<const float2*>(Cw + k * kPitchW + 2 * j);
+          const float v[4] = {bk.x, bk.y, bk.z, bk.w};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            x[m].x = fmaf(v[m], ck.x, x[m].x);
+            x[m].y = fmaf(v[m], ck.y, x[m].y);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          float2* at = reinterpret_cast<float2*>(X + (r + m) * kPitchW + 2 * j);
+          *at = make_float2(fmaf(keep, at->x, x[m].x), fmaf(keep, at->y, x[m].y));
+        }
       }
     }
-    if (s.x_last && q.state >= 0) {
-      for (int e = tid; e < d1 * kWidth; e += kThreads) {   // (each thread's own elements)
+    __syncthreads();
+    if (g.states_only || hand_on) {
+      for (int e = tid; e < d1 * kWidth; e += kThreads) {
         const int r = e / kWidth, w = e - r * kWidth;
-        if (w < width) s.x_last[state + (s.x_transposed ? (int64_t)(w0 + w) * d1 + r : (int64_t)r * s.d2 + w0 + w)] = X[e];
+        if (w >= width) continue;
+        if (g.states_only) work[(int64_t)r * s.d2 + w0 + w] = X[r * kPitchW + w];
+        else s.x_last[state + (s.x_transposed ? (int64_t)(w0 + w) * d1 + r : (int64_t)r * s.d2 + w0 + w)] = X[r * kPitchW + w];
       }
     }
   }
-  if (!p.starts)   // the rows of padding
-    for (int64_t e = tid + q.n * width; e < p.seq_len * width; e += kThreads) put<T>(s, y0 + (e / width) * s.ys[2] + e % width, 0.f);
+  if (g.states_only) return;
+  // rows without a state, and rows of padding
+  if (!q.bad && p.starts) return;
+  const int64_t end = p.starts ? q.n : p.seq_len, upto = end < from + g.rows ? end : from + g.rows;
+  const int64_t first = q.bad || q.n < from ? from : q.n;
+  for (int64_t e = first * width + tid; e < upto * width; e += kThreads)
+    put<T>(s, y0 + (e / width) * s.ys[2] + e % width, e / width < q.n ? __int_as_float(0x7fffffff) : 0.f);
+}
+
+// The states before the segments, from what each adds, in place; and the state behind the last.  A thread has the same four elements of all
+// segments of a scan, sequence and head.
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, const Segments g, const int first, const int scans, const int matrix) {
+  const int parts = (matrix + 1023) / 1024;
+  const unsigned unit = blockIdx.x / (unsigned)parts;
+  const int which = first + (int)(unit % (unsigned)scans), item = (int)(unit / (unsigned)scans);
+  const int e = ((int)(blockIdx.x % (unsigned)parts) * 256 + threadIdx.x) * 4;
+  const Scan& s = p.scan[which];
+  const int b = item / p.heads, h = item - b * p.heads;
+  const Sequence q = sequence_of(p, b);
+  if (q.bad || e >= matrix) return;
+  const float e2 = log2_decay(p.decay, h);
+  float* work = g.work + ((int64_t)which * p.batch * p.heads + item) * g.count * matrix + e;
+  const int64_t state = (q.state * p.heads + h) * (int64_t)matrix;
+  const int d2 = s.d2, r = e / d2, c = e - r * d2;   // (sizes are multiples of 8: the four are of one row)
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s.x_first && q.state >= 0) {
+    if (s.x_transposed) {
+      const float* f = s.x_first + state + (int64_t)c * s.d1 + r;
+      x = make_float4(f[0], f[s.d1], f[2 * s.d1], f[3 * s.d1]);
+    } else {
+      x = *reinterpret_cast<const float4*>(s.x_first + state + e);
+    }
+  }
+  for (int i = 0; i < g.count; ++i) {
+    const int64_t left = q.n - (int64_t)i * g.rows;
+    if (left <= 0) break;
+    const float keep = exp2f(e2 * (float)(left < g.rows ? left : g.rows));
+    float4* at = reinterpret_cast<float4*>(work + (int64_t)i * matrix);
+    const float4 t = *at;
+    *at = x;
+    x.x = fmaf(keep, x.x, t.x);
+    x.y = fmaf(keep, x.y, t.y);
+    x.z = fmaf(keep, x.z, t.z);
+    x.w = fmaf(keep, x.w, t.w);
+  }
+  if (s.x_last && q.state >= 0) {
+    if (s.x_transposed) {
+      float* f = s.x_last + state + (int64_t)c * s.d1 + r;
+      f[0] = x.x;
+      f[s.d1] = x.y;
+      f[2 * s.d1] = x.z;
+      f[3 * s.d1] = x.w;
+    } else {
+      *reinterpret_cast<float4*>(s.x_last + state + e) = x;
+    }
+  }
 }
 
 template <typename T>
@@ -155,20 +257,61 @@ __global__ void __launch_bounds__(256) group_sum_kernel(const GroupSum p, const 
 
 }  // namespace
 
-cudaError_t launch_scan_generic(const Params& p, cudaStream_t stream, int* launches) {
+cudaError_t launch_join(const Params& p, const Segments& g, int first, int scans, int matrix, cudaStream_t stream) {
+  const int64_t grid = (int64_t)p.batch * p.heads * scans * ((matrix + 1023) / 1024);
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  join_kernel<<<(unsigned)grid, 256, 0, stream>>>(p, g, first, scans, matrix);
+  return cudaGetLastError();
+}
+
+namespace {
+// Segments of two chunks at least, where the slices of all sequences and heads are fewer than two CTAs an SM.  (B2 S1024 H8 D64 in fp32: 32 CTAs
+// uncut; both launches and the join cost about as much again as the uncut scan's work, so that two segments gain nothing.)
+int segments_of(const Params& p, int num_sms) {
+  int64_t ctas = 0;
+  for (int i = 0; i < p.scans; ++i) ctas += (int64_t)p.batch * p.heads * ((p.scan[i].d2 + kWidth - 1) / kWidth);
+  const int64_t most = (p.seq_len + 2 * kChunk - 1) / (2 * kChunk);
+  int64_t n = 2 * num_sms / ctas;
+  n = n < most ? n : most;
+  n = n < 64 ? n : 64;
+  return n >= 3 ? (int)n : 1;
+}
+}  // namespace
+
+int64_t scan_generic_bytes(const Params& p, int num_sms) {
+  const int n = segments_of(p, num_sms);
+  return n == 1 ? 0 : (int64_t)p.scans * p.batch * p.heads * n * p.scan[0].d1 * p.scan[0].d2 * 4;
+}
+
+cudaError_t launch_scan_generic(const Params& p, int num_sms, float* work, int64_t work_bytes, cudaStream_t stream, int* launches) {
   int64_t grid = 0;
   size_t smem = 0;
+  Segments g;
+  g.count = work && work_bytes >= scan_generic_bytes(p, num_sms) ? segments_of(p, num_sms) : 1;
+  const int64_t per = (p.seq_len + g.count - 1) / g.count, rows = (per + kChunk - 1) / kChunk * kChunk;
+  g.rows = (int)(rows < 0x7fffffe0ll ? rows : 0x7fffffe0ll);
+  g.states_only = 0;
+  g.work = work;
   for (int i = 0; i < p.scans; ++i) {
-    const int64_t n = (int64_t)p.batch * p.heads * ((p.scan[i].d2 + kWidth - 1) / kWidth);
+    const int64_t n = (int64_t)p.batch * p.heads * g.count * ((p.scan[i].d2 + kWidth - 1) / kWidth);
     grid = n > grid ? n : grid;
     const size_t need = smem_bytes(p.scan[i].d1);
     smem = need > smem ? need : smem;
   }
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   auto kern = p.dtype == AIDN_F32 ? scan_kernel<float> : p.dtype == AIDN_F16 ? scan_kernel<__half> : scan_kernel<__nv_bfloat16>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(256));
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(256));
   if (e != cudaSuccess) return e;
-  kern<<<dim3((unsigned)grid, (unsigned)p.scans), kThreads, smem, stream>>>(p);
+  if (g.count > 1) {
+    g.states_only = 1;
+    kern<<<dim3((unsigned)grid, (unsigned)p.scans), kThreads, smem, stream>>>(p, g);
+    g.states_only = 0;
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_join(p, g, 0, p.scans, p.scan[0].d1 * p.scan[0].d2, stream);
+    if (e != cudaSuccess) return e;
+    *launches += 2;
+  }
+  kern<<<dim3((unsigned)grid, (unsigned)p.scans), kThreads, smem, stream>>>(p, g);
   ++*launches;
   return cudaGetLastError();
 }

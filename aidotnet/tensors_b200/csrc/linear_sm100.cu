@@ -825,56 +825,6 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   }
 }
 
-// The states before the segments, from what each adds, in place; and the state behind the last.  A thread has the same four elements of all
-// segments of a scan, sequence and head.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args args, const int matrix) {
-  const Params& p = args.p;
-  const int parts = matrix / 1024;
-  const unsigned unit = blockIdx.x / (unsigned)parts;
-  const int which = args.first + (int)(unit % (unsigned)args.count), item = (int)(unit / (unsigned)args.count);
-  const int e = ((int)(blockIdx.x % (unsigned)parts) * 256 + threadIdx.x) * 4;
-  const Scan& s = p.scan[which];
-  const int b = item / p.heads, h = item - b * p.heads;
-  const Sequence q = sequence_of(p, b);
-  if (q.bad) return;
-  const float g = log2_decay(p.decay, h);
-  float* work = args.work + ((int64_t)which * p.batch * p.heads + item) * args.segments * matrix + e;
-  const int64_t state = (q.state * p.heads + h) * (int64_t)matrix;
-  const int d2 = s.d2, r = e / d2, c = e - r * d2;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (s.x_first && q.state >= 0) {
-    if (s.x_transposed) {
-      const float* f = s.x_first + state + (int64_t)c * s.d1 + r;
-      x = make_float4(f[0], f[s.d1], f[2 * s.d1], f[3 * s.d1]);
-    } else {
-      x = *reinterpret_cast<const float4*>(s.x_first + state + e);
-    }
-  }
-  for (int i = 0; i < args.segments; ++i) {
-    const int64_t left = q.n - (int64_t)i * args.seg_len;
-    if (left <= 0) break;
-    const float keep = exp2f(g * (float)(left < args.seg_len ? left : args.seg_len));
-    float4* at = reinterpret_cast<float4*>(work + (int64_t)i * matrix);
-    const float4 t = *at;
-    *at = x;
-    x.x = fmaf(keep, x.x, t.x);
-    x.y = fmaf(keep, x.y, t.y);
-    x.z = fmaf(keep, x.z, t.z);
-    x.w = fmaf(keep, x.w, t.w);
-  }
-  if (s.x_last && q.state >= 0) {
-    if (s.x_transposed) {
-      float* f = s.x_last + state + (int64_t)c * s.d1 + r;
-      f[0] = x.x;
-      f[s.d1] = x.y;
-      f[2 * s.d1] = x.z;
-      f[3 * s.d1] = x.w;
-    } else {
-      *reinterpret_cast<float4*>(s.x_last + state + e) = x;
-    }
-  }
-}
-
 template <int D1, int D2, bool BF16>
 cudaError_t launch_t(const Maps& maps, Args& args, cudaStream_t stream, int* launches) {
   using C = Cfg<D1, D2>;
@@ -888,8 +838,7 @@ cudaError_t launch_t(const Maps& maps, Args& args, cudaStream_t stream, int* lau
     args.states_only = 0;
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    join_kernel<<<items * (unsigned)args.count * (D1 * D2 / 1024), 256, 0, stream>>>(args, D1 * D2);
-    e = cudaGetLastError();
+    e = launch_join(args.p, Segments{args.segments, args.seg_len, 0, args.work}, args.first, args.count, D1 * D2, stream);
     if (e != cudaSuccess) return e;
     *launches += 2;
   }
