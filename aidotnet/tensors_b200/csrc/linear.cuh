@@ -81,13 +81,16 @@ __device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
   return s;
 }
 
-// log2 of a head's decay factor.  0 * -inf is no exponent, so that a decay to nothing is a large finite one; above 0 is refused by NaN.
-__device__ __forceinline__ float log2_decay(const float* decay, int h) {
-  if (!decay) return 0.f;
+// A head's log decay.  0 * -inf is no exponent, so that a decay to nothing is a large finite one; above 0 is refused by NaN.
+__device__ __forceinline__ double log_decay(const float* decay, int h) {
+  if (!decay) return 0.0;
   const float g = decay[h];
-  if (!(g <= 0.f)) return __int_as_float(0x7fffffff);
-  return fmaxf(g * kLog2e, -1e30f);
+  if (!(g <= 0.f)) return __longlong_as_double(0x7ff8000000000000ll);
+  return fmax((double)g, -1e30);
 }
+// Its factor over n rows, rounded once.  (A state is multiplied by the same one chunk after chunk: what exp2f is off by, up to two units in the last
+// place, would add up over all the chunks that the state remembers.)
+__device__ __forceinline__ float decay_power(double g, double n) { return (float)exp(g * n); }
 
 // Sequences cut into segments: a first launch leaves what each adds to the state in `work` ([scan][sequence, head][segment][d1][d2]),
 // launch_join turns those into the states before them and writes the last ones, and the scan then starts every segment from its own.

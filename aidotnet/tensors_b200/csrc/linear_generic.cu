@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ 
   const int64_t y0 = (p.starts ? 0 : b * s.ys[0]) + h * s.ys[1] + q.row0 * s.ys[2] + w0;
   const bool hand_on = g.count == 1 && s.x_last && q.state >= 0 && !q.bad;   // (a sequence without rows leaves its state too)
   if (rows > 0 || hand_on) {
-    const float e2 = log2_decay(p.decay, h);
-    if (tid <= kChunk) power[tid] = exp2f(e2 * tid);
+    const double decay = log_decay(p.decay, h);
+    if (tid <= kChunk) power[tid] = decay_power(decay, tid);
     const int64_t matrix = (int64_t)d1 * s.d2;
     const int64_t state = (q.state * p.heads + h) * matrix;
     float* work = g.count > 1 ? g.work + (((int64_t)blockIdx.y * p.batch * p.heads + item) * g.count + seg) * matrix : nullptr;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ 
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int ii = i + 16 * x;
-          const float w = s.row_scale * exp2f(e2 * (ii + s.lag));
+          const float w = s.row_scale * power[ii + s.lag];
           float2 y = make_float2(o[x].x * w, o[x].y * w);
           for (int k = 0; k <= ii; ++k) {   // (not a row behind: what stands there may not be finite)
             const float pk = P[ii * kPitchP + k];
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   const int b = item / p.heads, h = item - b * p.heads;
   const Sequence q = sequence_of(p, b);
   if (q.bad || e >= matrix) return;
-  const float e2 = log2_decay(p.decay, h);
+  const double decay = log_decay(p.decay, h);
   float* work = g.work + ((int64_t)which * p.batch * p.heads + item) * g.count * matrix + e;
   const int64_t state = (q.state * p.heads + h) * (int64_t)matrix;
   const int d2 = s.d2, r = e / d2, c = e - r * d2;   // (sizes are multiples of 8: the four are of one row)
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   for (int i = 0; i < g.count; ++i) {
     const int64_t left = q.n - (int64_t)i * g.rows;
     if (left <= 0) break;
-    const float keep = exp2f(e2 * (float)(left < g.rows ? left : g.rows));
+    const float keep = decay_power(decay, (double)(left < g.rows ? left : g.rows));
     float4* at = reinterpret_cast<float4*>(work + (int64_t)i * matrix);
     const float4 t = *at;
     *at = x;

@@ -272,9 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       for (int i = 0; i < 4; ++i) mbar_init(b_max + 8 * i, 2);
       fence_mbar_init();
     }
-    const float g = log2_decay(p.decay, h);
+    const double g = log_decay(p.decay, h);
     if (threadIdx.x < 65) {
-      const float w = exp2f(g * threadIdx.x);
+      const float w = decay_power(g, threadIdx.x);
       table[C::kTabPower + threadIdx.x] = w;
       if constexpr (BF16) {
         uint16_t* terms = reinterpret_cast<uint16_t*>(table + C::kTabW);
@@ -292,10 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
     }
     else if (threadIdx.x >= 96 && threadIdx.x < 160) {
       const int r = threadIdx.x - 96;
-      table[C::kTabRow + r] = s.row_scale * exp2f(g * ((reverse ? kChunk - 1 - r : r) + s.lag));
+      table[C::kTabRow + r] = s.row_scale * decay_power(g, (reverse ? kChunk - 1 - r : r) + s.lag);
     } else if (threadIdx.x >= 256 && threadIdx.x < 384) {   // of row i and column j at 63 - i + j; zeros where j follows i
       const int x = (int)threadIdx.x - 256, d = reverse ? x - 63 : 63 - x;
-      const float w = d >= 0 ? p.scale * exp2f(g * d) : 0.f;
+      const float w = d >= 0 ? p.scale * decay_power(g, d) : 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (x >= i) table[C::kTabScore + i * C::kScorePitch + x - i] = w;

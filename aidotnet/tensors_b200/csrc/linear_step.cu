@@ -54,8 +54,7 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const Step p, const int 
   }
   float4 vv = make_float4(0.f, 0.f, 0.f, 0.f);
   if (group < groups) vv = make_float4(to_float(v[0]), to_float(v[1]), to_float(v[2]), to_float(v[3]));
-  const float g = p.decay ? p.decay[h] : 0.f;
-  const float lam = g <= 0.f ? expf(g) : __int_as_float(0x7fffffff);
+  const float lam = decay_power(log_decay(p.decay, h), 1.0);
   __syncthreads();
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int r0 = group; r0 < p.key_dim; r0 += kRows * groups) {
