@@ -229,10 +229,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   const int which = args.first + (int)(blockIdx.x % (unsigned)args.count);
   const unsigned unit = blockIdx.x / (unsigned)args.count;
   const int seg = (int)(unit % (unsigned)args.segments);
-  const int item = (int)(unit / (unsigned)args.segments);
-  int b = item / p.heads;
-  const int h = item - b * p.heads;
+  int b = (int)(unit / (unsigned)args.segments) / p.heads;
+  const int h = (int)(unit / (unsigned)args.segments) - b * p.heads;
   if (by_length(p)) b = sequence_of_rank(p, b);
+  const int item = b * p.heads + h;   // (its states in the workspace are found by it)
   const Scan& s = p.scan[which];
   const bool states_only = args.states_only != 0;
   // (shuffled from lane 0: what depends on it is known to be the same in a warp, and stays in uniform registers)
@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           while (!states_only && ahead <= c + 1 && ahead < chunks) {
             const int slot = ahead == c ? at : next;
             const uint32_t slot_phase = ahead == c ? phase : next_phase;
-            if (ahead > c && !mbar_test(b_full + 8 * slot, slot_phase)) break;
-            if (!(ok = wait1(b_full + 8 * slot, slot_phase) && wait1(b_s_empty, (uint32_t)(ahead & 1) ^ 1u))) break;
+            if (ahead > c ? !mbar_test(b_full + 8 * slot, slot_phase) : !(ok = wait1(b_full + 8 * slot, slot_phase))) break;
+            if (!(ok = wait1(b_s_empty, (uint32_t)(ahead & 1) ^ 1u))) break;
             tc_fence_after();
             const uint64_t ad = rows_desc + (uint64_t)(slot * (C::kStageBytes >> 4)), bd = ad + (C::kOffB >> 4);
 #pragma unroll
@@ -380,7 +380,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             tc_commit(b_s_full + 8 * (ahead & 1));
             ++ahead;
           }
-          if (!ok || !wait1(b_full + 8 * at, phase) || !wait1(b_bt_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1)) || !wait1(b_t_empty, (uint32_t)(c & 1) ^ 1u)) break;
+          // (the tiles have been waited for with the scores; a state that has been put down has left T's columns)
+          if (!ok || !wait1(b_bt_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
+          if (states_only ? !wait1(b_full + 8 * at, phase) || !wait1(b_t_empty, (uint32_t)(c & 1) ^ 1u) : !wait1(b_x_full, (uint32_t)(c & 1))) break;
           tc_fence_after();
           const uint64_t ct = cols_desc + stage + (C::kOffC >> 4), bt = cols_desc + stage + (C::kOffB >> 4);
           const uint32_t first = tmem + C::kColC + (third ? 0 : (c & 1) * 64);
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           }
           tc_commit(b_t_full);
           if (!states_only) {
-            if (!wait1(b_x_full, (uint32_t)(c & 1)) || (c > 0 && !wait1(b_o_empty + 8 * ((c - 1) & 1), (uint32_t)(((c - 1) >> 1) & 1)))) break;
+            if (c > 0 && !wait1(b_o_empty + 8 * ((c - 1) & 1), (uint32_t)(((c - 1) >> 1) & 1))) break;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < D1 / 16; ++k) mma_ts(tmem + C::kColO, tmem + C::kColX + k * 8, rows_desc + stage + row_step(k), idesc_rows, k > 0);
