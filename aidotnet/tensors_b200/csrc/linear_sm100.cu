@@ -3,25 +3,31 @@
 //
 //     S   = A B^T                      scores, 64 x 64 (rows of A in lanes 0-63; the lanes above hold what is not looked at)
 //     P   = S weighted by lam^(i-j), zeros where j follows i, in 16 bits to shared memory
-//     T^T = C^T B~                     B~ = rows of B weighted by lam^(n-lag-j), as two 16-bit terms: what is added to a state is not rounded
+//     T^T = C~^T B                     C~ = rows of C weighted by lam^(n-lag-j), as two or three 16-bit terms: what is added to a state is not rounded
 //     O^T = X^T A^T  and  C^T P^T      apart, since their columns have different factors; X^T in 16 bits in tensor memory
 //     X   = lam^n X + T                in fp32 registers, then X^T rounded for the next chunk
 //
-//   warps 0-1    P            warp 2   TMA producer            warp 3   MMA issuer, owner of tensor memory
-//   warps 4-11   B~ and the state, a lane (column of c) and half of b's columns to a thread
-//   warps 12-15  output: O^T from tensor memory, weighted, pairs of lanes exchanged, 4-byte stores along c's columns
+//   warps 0-1    P            warp 2   TMA producer (one thread)            warp 3   issues the products (one thread), owns tensor memory
+//   warps 4-11   C~ and the state, a lane (column of c) and half of b's columns to a thread; C~^T goes to tensor memory by transposing loads
+//   warps 12-15  output: O^T from tensor memory, weighted, by transposing stores to rows in shared memory, and out by TMA
 //
 // Rows are taken from a sequence's last to its first for the gradients of keys and values: a tile is loaded as it lies, and only masks and
-// exponents turn around.  The last chunk's missing rows are zeros in C and B~.
+// exponents turn around.  The last chunk's missing rows are zeros in C~, and in B and C, which multiply zeros.
 //
 // fp16: a row of P and a lane's row of X^T are scaled by a power of two to their own largest value, as neither is bound by fp16's range; the
-// second term of B~ is held 2^11 times as large, where fp16's smallest numbers do not cut it, and its product divided on the way into the first's.
+// second term of C~ is held 2^11 times as large, where fp16's smallest numbers do not cut it, and its product divided on the way into the first's.
 //
-// What is not finite in C would reach earlier rows of its chunk as 0 * NaN in C^T P^T: a thread whose column came out not finite sums it again, row by
-// row, over what the row may see.
+// What is not finite in C would reach earlier rows of its chunk as 0 * NaN in C^T P^T: columns that come out not finite are summed again, row by row, over
+// what a row may see.
 //
 // Few sequences and heads: their rows are cut into segments.  A first launch forms what each segment adds to the state, a second one turns
 // those into the states before the segments, and the scan then runs on all segments at once, at the price of b and c read twice.
+//
+// What bounds it: a chunk takes 1.3 us (sizes of 64) to 1.7 us (128), with 16 CTAs as with 128, where the bytes of 128 CTAs would take 1.28 us at 128:
+// the chain of waits between the roles and their code, which is longer than the instruction cache holds (8 in 100 fetches of a line miss), not a unit.
+// B4 S2048 H32 D128 in bf16: 68 us, 3.9 TB/s.  Measured on the way (us for that call): roles unrolled over their rows 174, in loops 84, packed
+// arithmetic and stores by TMA 70; C~ by shared memory in place of tensor memory 80; four more warps for C~ at 96 registers a thread 76; products issued by
+// two warps, and those of T and O in turn, made no difference.
 //
 // Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
 #include <cuda.h>
@@ -43,7 +49,6 @@ constexpr int kChunk = 64;
 constexpr int kBlock = kChunk * 128;   // 64 rows of 64 16-bit elements
 constexpr int kYBytes = kChunk * 64;   // 64 rows of 32
 constexpr int kMaxSegments = 64;
-constexpr int kMostRanked = 256;       // sequences of a batch that are taken by their lengths
 constexpr int kThreads = 512;
 constexpr int kWarpLoad = 2, kWarpMma = 3, kWarpState = 4, kWarpOut = 12;   // (warps 0 and 1: P)
 
@@ -188,25 +193,6 @@ __device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_
                : "memory");
 }
 
-// Sequences of unequal lengths are taken from the longest to the shortest, so that none is left over for the end: the sequence that `rank` others precede.
-// (Seven prompts of up to 8192 rows, 32 heads: 300 us in the order of the batch, 225 us so.)
-__device__ __forceinline__ bool by_length(const Params& p) { return (p.starts || p.lengths) && p.batch > 1 && p.batch <= kMostRanked; }
-__device__ __forceinline__ int sequence_of_rank(const Params& p, int rank) {
-  __shared__ int found;
-  auto rows = [&](int i) { return p.starts ? p.starts[i + 1] - p.starts[i] : p.lengths[i]; };
-  if ((int)threadIdx.x < p.batch) {
-    const int mine = rows(threadIdx.x);
-    int before = 0;
-    for (int i = 0; i < p.batch; ++i) {
-      const int n = rows(i);
-      before += n > mine || (n == mine && i < (int)threadIdx.x) ? 1 : 0;
-    }
-    if (before == rank) found = threadIdx.x;
-  }
-  __syncthreads();
-  return found;
-}
-
 template <int D1, int D2, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args args) {
   using C = Cfg<D1, D2>;
@@ -229,10 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   const int which = args.first + (int)(blockIdx.x % (unsigned)args.count);
   const unsigned unit = blockIdx.x / (unsigned)args.count;
   const int seg = (int)(unit % (unsigned)args.segments);
-  int b = (int)(unit / (unsigned)args.segments) / p.heads;
-  const int h = (int)(unit / (unsigned)args.segments) - b * p.heads;
-  if (by_length(p)) b = sequence_of_rank(p, b);
-  const int item = b * p.heads + h;   // (its states in the workspace are found by it)
+  const int item = (int)(unit / (unsigned)args.segments), b = item / p.heads, h = item - b * p.heads;
   const Scan& s = p.scan[which];
   const bool states_only = args.states_only != 0;
   // (shuffled from lane 0: what depends on it is known to be the same in a warp, and stays in uniform registers)
@@ -485,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         }
       }
     } else if (warp < kWarpOut) {
-      // ---- B~ and the state ----
+      // ---- C~ and the state ----
       const int tid = threadIdx.x - kWarpState * 32, quarter = warp & 3, half = (warp - kWarpState) >> 2;
       constexpr int kCols = D1 / 2;              // of a thread
       const int d2 = quarter * 32 + lane, d1 = half * kCols;
@@ -493,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const int64_t matrix = (int64_t)D1 * D2;
       const int lag = s.lag;
-      const float key_scale = s.key_scale;   // in B~'s weights, or behind the product where they might leave fp16's range
+      const float key_scale = s.key_scale;   // in C~'s weights, or behind the product where they might leave fp16's range
       float x[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) x[i] = 0.f;
@@ -857,8 +840,8 @@ cudaError_t launch_sizes(const Maps& maps, Args& args, cudaStream_t stream, int*
 }
 
 // How many segments the sequences are cut into: as many as bring work to all SMs, where that pays.  A row goes through both launches then, the first at 0.7
-// of the second's cost, and the launches with the join between them take some 6 us more, the time of four chunks: a prompt of 517 rows and 16
-// heads of 64 takes 20 us uncut, 14 us in 9 segments.
+// of the second's cost, and the two launches more take the time of ten chunks.  One sequence and 16 heads of 64 in fp16: 2048 rows 62 us uncut, 29 us
+// in 9 segments; 512 rows 18.9 us uncut, 19.5 us cut.  8192 rows of 16 heads of 128 in bf16: 202 and 73 us.
 int segments_of(const Params& p, int num_sms) {
   const int64_t items = (int64_t)p.batch * p.heads * p.scans, chunks = (p.seq_len + kChunk - 1) / kChunk;
   int64_t n = num_sms / items;

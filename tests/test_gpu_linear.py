@@ -301,6 +301,68 @@ def test_state_slots(backend, dtype, dim):
         assert torch.equal(pool[s], was[s])
 
 
+@pytest.mark.parametrize("dtype,key,value", [("bf16", 128, 128), ("f16", 64, 128), ("bf16", 64, 64), ("f32", 64, 64), ("f32", 40, 72), ("bf16", 96, 40)])
+def test_segments(backend, dtype, key, value):
+    """Long sequences of few heads are cut into segments that run at once: ragged ones too, with states in and out, in place and through slots; and the
+    same call without a workspace, which is not cut."""
+    c = Case(dtype, [3000, 1, 0, 2400], 1, 1, key, value, "starts", first=True, seed=20)
+    block = dict(batch=4, heads=1, kv_heads=1, seq_len=3000, key_dim=key, value_dim=value, dtype={"bf16": N.BF16, "f16": N.F16, "f32": N.F32}[dtype])
+    assert N.linear_workspace_bytes(N.linear_block(**block)) > 0
+    check_forward(backend, c)
+    pool = torch.randn(6, 1, key, value, device="cuda")
+    slots = torch.tensor([4, 0, 5, 1], dtype=torch.int32, device="cuda")
+    outs, pools = [], []
+    for cut in (True, False):
+        now, out = pool.clone(), torch.empty(c.shape(1, value), dtype=TORCH_DT[dtype], device="cuda")
+        if cut:
+            backend.LinearAttention(c.buf(c.q), c.buf(c.k), c.buf(c.v), GpuBuffer(out), c.buf(c.decay), *c.sizes(), initialStates=GpuBuffer(now),
+                                    finalStates=GpuBuffer(now), stateSlots=GpuBuffer(slots), **c.kw())
+        else:
+            starts = torch.tensor(c.starts, dtype=torch.int32, device="cuda")
+            N.linear_attention(N.linear_block(q=c.q.data_ptr(), k=c.k.data_ptr(), v=c.v.data_ptr(), out=out.data_ptr(), decay=c.decay.data_ptr(),
+                                              token_starts=starts.data_ptr(), tokens=c.rows, initial_state=now.data_ptr(), final_state=now.data_ptr(),
+                                              state_slots=slots.data_ptr(), num_slots=6, **block), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        outs.append(out[:c.starts[-1]].double())
+        pools.append(now.double())
+    # both are within the bounds of the recurrence, so within twice those of one another
+    for b, n in enumerate(c.lens):
+        q, k, v = c.wide(c.q, b), c.wide(c.k, b), c.wide(c.v, b)
+        size, size_s = recurrence(q.abs(), k.abs(), v.abs(), c.log_decay(), key ** -0.5, pool[slots[b]].double().abs())
+        e, u = e32(max(key, value), n), unit(dtype)
+        rows = slice(c.starts[b], c.starts[b] + n)
+        near(outs[0][rows].transpose(0, 1), outs[1][rows].transpose(0, 1), 2 * (u + e) * size, 2 * torch.finfo(TORCH_DT[dtype]).eps / 2, f"sequence {b}")
+        near(pools[0][slots[b]], pools[1][slots[b]], 2 * (4 * u * u + e) * size_s, 2.0 ** -23, f"state of sequence {b}")
+    assert torch.equal(pools[0][[2, 3]], pool.double()[[2, 3]])
+
+
+@pytest.mark.parametrize("key,value", [(128, 128), (64, 128), (72, 40)])
+def test_segments_backward(backend, key, value):
+    check_backward(backend, Case("bf16", [2300, 5, 1900], 1, 1, key, value, "lengths_token", first=True, seed=21), last=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_tensors_that_no_tile_load_fits(backend, dtype):
+    """Strides of odd numbers of elements, a shared row (stride 0) and unaligned addresses, through the C ABI: other kernels, the same results."""
+    n, heads, dim = 70, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(22)
+    make = lambda: (torch.randn(20000, generator=g, device="cuda") * 0.5).to(TORCH_DT[dtype])  # noqa: E731
+    q = torch.as_strided(make(), (heads, n, dim), (67, 135, 1), 1)
+    k = torch.as_strided(make(), (heads, n, dim), (0, 64, 1), 8)          # one head's keys for both
+    v = torch.as_strided(make(), (heads, n, dim), (4800, 66, 1), 0)
+    to = torch.zeros(20000, dtype=q.dtype, device="cuda")
+    out = torch.as_strided(to, (heads, n, dim), (65, 133, 1), 3)
+    decay = decays(heads, "spread")
+    N.linear_attention(N.linear_block(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), decay=decay.data_ptr(), batch=1, heads=heads,
+                                      kv_heads=heads, seq_len=n, key_dim=dim, value_dim=dim, dtype=N.BF16 if dtype == "bf16" else N.F16,
+                                      q_stride=(0, 67, 135), k_stride=(0, 0, 64), v_stride=(0, 4800, 66), o_stride=(0, 65, 133)),
+                       torch.cuda.current_stream().cuda_stream)
+    ins = [x.double() for x in (q, k, v)]
+    ref, _ = recurrence(*ins, decay.double(), dim ** -0.5)
+    size, _ = recurrence(*(x.abs() for x in ins), decay.double(), dim ** -0.5)
+    near(out, ref, (unit(dtype) + e32(dim, n)) * size, torch.finfo(TORCH_DT[dtype]).eps / 2, "out")
+
+
 # ---- gradients -------------------------------------------------------------------------------------------------------
 
 def run_backward(backend, c, d_last=None, want_first=False):
