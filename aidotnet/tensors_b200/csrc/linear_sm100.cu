@@ -63,9 +63,9 @@ struct Cfg {
   static constexpr int kOffTab = kOffY + 4 * kYBytes;
   // tables (floats): powers [65], weights of the scores by distance in four copies, each one element on from the one before (a row's begin anywhere
   // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of maxima [2][2][128], weights of
-  // C~ by exponent, [3] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [3][2][4][4]
+  // C~ by exponent, [2] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [2][2][4][4]
   static constexpr int kTabPower = 0, kTabScore = 68, kScorePitch = 136, kTabRow = kTabScore + 4 * kScorePitch, kTabP = kTabRow + 64, kTabX = kTabP + 128,
-                       kTabMax = kTabX + 512, kTabW = kTabMax + 512, kTabPairs = kTabW + 100, kTabFloats = kTabPairs + 96;
+                       kTabMax = kTabX + 512, kTabW = kTabMax + 512, kTabPairs = kTabW + 68, kTabFloats = kTabPairs + 64;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
   static constexpr int kBars = 2 * kStages + 20;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
@@ -105,11 +105,6 @@ __device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t bf16x2_sub(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 template <bool BF16>
@@ -263,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         uint16_t* terms = reinterpret_cast<uint16_t*>(table + C::kTabW);
         float left = w * s.key_scale;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const uint32_t t = pack2<true>(left, 0.f) & 0xffffu;
           terms[i * 66 + threadIdx.x] = (uint16_t)t;
           const int j = reverse ? (int)threadIdx.x + s.lag - 1 : kChunk - s.lag - (int)threadIdx.x;   // the row of a whole chunk with this exponent
@@ -531,12 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
         const uint32_t st = base + (uint32_t)((c % C::kStages) * C::kStageBytes) + C::kOffC;
         if (!wait(b_full + 8 * (c % C::kStages), (uint32_t)((c / C::kStages) & 1))) return false;
         if (owner) {
-          uint32_t weights[3][4];   // of this thread's pairs of rows
-          if constexpr (BF16) {
+          uint32_t weights[2][4];   // of this thread's pairs of rows, as two terms
+          if (BF16 && !third) {
             const uint16_t* terms = reinterpret_cast<const uint16_t*>(table + C::kTabW);
 #pragma unroll
-            for (int t = 0; t < 3; ++t) {
-              if (t == 2 && !third) break;
+            for (int t = 0; t < 2; ++t) {
               uint4 w = *reinterpret_cast<const uint4*>(table + C::kTabPairs + t * 32 + half * 16 + (lane & 3) * 4);
               if (n < kChunk) w = end_weights(terms + t * 66, j_own, n, lag, reverse);
               weights[t][0] = w.x; weights[t][1] = w.y; weights[t][2] = w.z; weights[t][3] = w.w;
@@ -558,26 +552,31 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
                 v[i] &= (there(j, n) ? 0xffffu : 0u) | (there(j + 1, n) ? 0xffff0000u : 0u);
               }
             }
-            if constexpr (BF16) {
-              // c w as terms of 16 bits by packed multiply-adds, with w = w0 + w1 + w2 of 8 bits each: c w0 has 16 bits, so that what its rounding
-              // leaves is exact, and so on.
+            if (BF16 && !third) {
+              // c w as two terms by packed multiply-adds, with w = w0 + w1 of 8 bits each: c w0 has 16 bits, so that what its rounding leaves is exact.
+              // (In fp32, with conversions there and back, it takes three times the instructions.)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 a[i] = bf16x2_mul(v[i], weights[0][i / 2]);
-                const uint32_t rest = bf16x2_fma(v[i], weights[0][i / 2], a[i] ^ 0x80008000u);
-                e[i] = bf16x2_fma(v[i], weights[1][i / 2], rest);
-                if (third) v[i] = bf16x2_fma(v[i], weights[2][i / 2], bf16x2_fma(v[i], weights[1][i / 2], bf16x2_sub(rest, e[i])));
+                e[i] = bf16x2_fma(v[i], weights[1][i / 2], bf16x2_fma(v[i], weights[0][i / 2], a[i] ^ 0x80008000u));
               }
             } else {
+              const float factor = BF16 ? key_scale : 1.f;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int j = j_own + 8 * (i / 2);
                 float2 f = unpack16<BF16>(v[i]);
-                f.x *= power[there(j, n) ? exponent(j, n) : 0];
-                f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0];
+                f.x *= power[there(j, n) ? exponent(j, n) : 0] * factor;
+                f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0] * factor;
                 a[i] = pack2<BF16>(f.x, f.y);
-                const float2 t = unpack16<BF16>(a[i]);
-                e[i] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+                float2 t = unpack16<BF16>(a[i]);
+                f.x -= t.x;
+                f.y -= t.y;
+                e[i] = BF16 ? pack2<BF16>(f.x, f.y) : pack2<BF16>(f.x * 2048.f, f.y * 2048.f);
+                if constexpr (BF16) {
+                  t = unpack16<BF16>(e[i]);
+                  v[i] = pack2<BF16>(f.x - t.x, f.y - t.y);
+                }
               }
             }
             tmem_st_16x128b_x4(to + ((uint32_t)d << 16), a);
