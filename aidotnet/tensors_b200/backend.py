@@ -759,7 +759,8 @@ class CudaBackend:
         grads = dict(dout=gradOutput.tensor.data_ptr(), dq=gradQuery.tensor.data_ptr(), dk=gradKey.tensor.data_ptr(),
                      dv=gradValue.tensor.data_ptr(), d_final_state=_address(gradFinalStates), d_initial_state=_address(gradInitialStates),
                      do_stride=os, dq_stride=qs, dk_stride=ks, dv_stride=vs)
-        stream, ws, ws_bytes = self._linear_workspace(N.linear_bwd_block(N.linear_block(**args), **grads), optional=False)
+        # (without shared heads it only holds the states of segments, and sequences are not cut without it)
+        stream, ws, ws_bytes = self._linear_workspace(N.linear_bwd_block(N.linear_block(**args), **grads), optional=heads == kvHeads)
         N.linear_attention_backward(N.linear_bwd_block(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), **grads), stream)
         self.launch_count += 1
 

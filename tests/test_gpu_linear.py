@@ -336,6 +336,23 @@ def test_segments(backend, dtype, key, value):
     assert torch.equal(pools[0][[2, 3]], pool.double()[[2, 3]])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_no_rows_at_all(backend, dtype):
+    """A packed batch of empty sequences: the states go through as they are, forwards and backwards (times one step's decay to the power of no rows)."""
+    empty = lambda h: GpuBuffer(torch.empty(0, h, 64, dtype=TORCH_DT[dtype], device="cuda"))  # noqa: E731
+    first, last, grad, back = torch.randn(2, 4, 64, 64, device="cuda"), *(torch.zeros(2, 4, 64, 64, device="cuda") for _ in range(3))
+    grad.copy_(first.flip(0))
+    starts = GpuBuffer(torch.zeros(3, dtype=torch.int32, device="cuda"))
+    decay = decays(4, "spread")
+    sizes = (2, 4, 2, 8, 64, 64)
+    backend.LinearAttention(empty(4), empty(2), empty(2), empty(4), GpuBuffer(decay), *sizes, tokenStarts=starts, initialStates=GpuBuffer(first),
+                            finalStates=GpuBuffer(last))
+    backend.LinearAttentionBackward(empty(4), empty(4), empty(2), empty(2), empty(4), empty(2), empty(2), GpuBuffer(decay), *sizes, tokenStarts=starts,
+                                    initialStates=GpuBuffer(first), gradFinalStates=GpuBuffer(grad), gradInitialStates=GpuBuffer(back))
+    torch.cuda.synchronize()
+    assert torch.equal(last, first) and torch.equal(back, grad)
+
+
 @pytest.mark.parametrize("key,value", [(128, 128), (64, 128), (72, 40)])
 def test_segments_backward(backend, key, value):
     check_backward(backend, Case("bf16", [2300, 5, 1900], 1, 1, key, value, "lengths_token", first=True, seed=21), last=True)
