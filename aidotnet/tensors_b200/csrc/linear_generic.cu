@@ -1,7 +1,7 @@
 // The scan of linear.cuh on FFMA: any type, any head sizes.  A CTA takes some columns of c (and of the state) for one sequence and head, or one segment
 // of them, and walks its rows in chunks, the state in shared memory in fp32; the chunk's products a . b are formed again for every slice of
-// columns.  What bounds it is the reads of shared memory that feed the multiply-adds: all products are tiles of 2 x 2 (a . b, outputs) or
-// 4 x 2 (state) to a thread, read by fours along the sizes.  Few sequences and heads are cut into segments as on the tensor cores.
+// columns.  What bounds it is the reads of shared memory that feed the multiply-adds: all products are tiles of 2 x 2 (a . b), 2 x N (outputs) or
+// 4 x N (state; N = 2 or 4 for 32 or 64 columns) to a thread, read by fours along the sizes.  Few sequences and heads are cut into segments as on the tensor cores.
 #include "linear.cuh"
 
 namespace aidn {
@@ -10,14 +10,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 32;
-constexpr int kWidth = 32;   // columns of a slice
-
 __host__ __device__ constexpr int pitch_of(int d) { return d + 4; }   // (rows begin in different banks, fours stay aligned)
-constexpr int kPitchW = kWidth + 4, kPitchP = kChunk + 4;
+constexpr int kPitchP = kChunk + 4;
 // shared memory in floats: A, B [chunk][d1], C and weighted C [chunk][width], X [d1][width], P [chunk][chunk], powers
-inline size_t smem_bytes(int d1) {
-  return sizeof(float) * (2 * kChunk * pitch_of(d1) + 2 * kChunk * kPitchW + (size_t)d1 * kPitchW + kChunk * kPitchP + kChunk + 4);
+inline size_t smem_bytes(int d1, int width) {
+  return sizeof(float) * (2 * kChunk * pitch_of(d1) + (2 * kChunk + (size_t)d1) * (width + 4) + kChunk * kPitchP + kChunk + 4);
 }
+
+__host__ __device__ constexpr int ctas_of(int width) { return width == 64 ? 2 : 3; }   // CTAs that an SM's registers hold
 
 template <typename T>
 __device__ __forceinline__ void put(const Scan& s, int64_t at, float x) {
@@ -27,8 +27,21 @@ __device__ __forceinline__ void put(const Scan& s, int64_t at, float x) {
 
 __device__ __forceinline__ float dot4(float4 a, float4 b, float c) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c)))); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ Params p, const Segments g) {
+// N floats side by side.
+template <int N>
+__device__ __forceinline__ void load_n(const float* from, float (&to)[N]) {
+  if constexpr (N == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(from);
+    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(from);
+    to[0] = v.x; to[1] = v.y;
+  }
+}
+
+template <typename T, int kWidth>
+__global__ void __launch_bounds__(kThreads, ctas_of(kWidth)) scan_kernel(const __grid_constant__ Params p, const Segments g) {
+  constexpr int kPitchW = kWidth + 4, N = kWidth / 16;   // N: columns of a thread
   extern __shared__ float4 smem4[];
   float* smem = reinterpret_cast<float*>(smem4);
   const Scan& s = p.scan[blockIdx.y];
@@ -106,57 +119,63 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ 
             if (jj <= ii) P[ii * kPitchP + jj] = acc[x][y] * (p.scale * power[ii - jj]);
           }
         __syncthreads();
-        // outputs: rows i, i + 16, columns 2 j, 2 j + 1
-        float2 o[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // outputs: rows i, i + 16, columns N j .. + N - 1
+        float o[2][N] = {};
         for (int d = 0; d < d1; d += 4) {
           const float4 a0 = *reinterpret_cast<const float4*>(A + i * pitch + d), a1 = *reinterpret_cast<const float4*>(A + (i + 16) * pitch + d);
           const float va[4] = {a0.x, a0.y, a0.z, a0.w}, vb[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float2 x = *reinterpret_cast<const float2*>(X + (d + k) * kPitchW + 2 * j);
-            o[0].x = fmaf(va[k], x.x, o[0].x);
-            o[0].y = fmaf(va[k], x.y, o[0].y);
-            o[1].x = fmaf(vb[k], x.x, o[1].x);
-            o[1].y = fmaf(vb[k], x.y, o[1].y);
+            float x[N];
+            load_n<N>(X + (d + k) * kPitchW + N * j, x);
+#pragma unroll
+            for (int m = 0; m < N; ++m) {
+              o[0][m] = fmaf(va[k], x[m], o[0][m]);
+              o[1][m] = fmaf(vb[k], x[m], o[1][m]);
+            }
           }
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int ii = i + 16 * x;
           const float w = s.row_scale * power[ii + s.lag];
-          float2 y = make_float2(o[x].x * w, o[x].y * w);
+#pragma unroll
+          for (int m = 0; m < N; ++m) o[x][m] *= w;
           for (int k = 0; k <= ii; ++k) {   // (not a row behind: what stands there may not be finite)
             const float pk = P[ii * kPitchP + k];
-            const float2 ck = *reinterpret_cast<const float2*>(C + k * kPitchW + 2 * j);
-            y.x = fmaf(pk, ck.x, y.x);
-            y.y = fmaf(pk, ck.y, y.y);
+            float ck[N];
+            load_n<N>(C + k * kPitchW + N * j, ck);
+#pragma unroll
+            for (int m = 0; m < N; ++m) o[x][m] = fmaf(pk, ck[m], o[x][m]);
           }
           if (ii < n) {
-            if (2 * j < width) put<T>(s, y0 + row(ii) * s.ys[2] + 2 * j, y.x);
-            if (2 * j + 1 < width) put<T>(s, y0 + row(ii) * s.ys[2] + 2 * j + 1, y.y);
+#pragma unroll
+            for (int m = 0; m < N; ++m)
+              if (N * j + m < width) put<T>(s, y0 + row(ii) * s.ys[2] + N * j + m, o[x][m]);
           }
         }
         __syncthreads();
       }
-      // the state: rows 4 i .. + 3 of every 64, columns 2 j, 2 j + 1
+      // the state: rows 4 i .. + 3 of every 64, columns N j .. + N - 1
       const float keep = power[n];
       for (int r = 4 * i; r < d1; r += 64) {
-        float2 x[4] = {};
+        float x[4][N] = {};
         for (int k = 0; k < n; ++k) {
-          const float4 bk = *reinterpret_cast<const float4*>(B + k * pitch + r);
-          const float2 ck = *reinterpret_cast<const float2*>(Cw + k * kPitchW + 2 * j);
-          const float v[4] = {bk.x, bk.y, bk.z, bk.w};
+          float v[4], ck[N];
+          load_n<4>(B + k * pitch + r, v);
+          load_n<N>(Cw + k * kPitchW + N * j, ck);
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            x[m].x = fmaf(v[m], ck.x, x[m].x);
-            x[m].y = fmaf(v[m], ck.y, x[m].y);
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int m = 0; m < N; ++m) x[e][m] = fmaf(v[e], ck[m], x[e][m]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int m = 0; m < N; ++m) {
+            float* at = X + (r + e) * kPitchW + N * j + m;
+            *at = fmaf(keep, *at, x[e][m]);
           }
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          float2* at = reinterpret_cast<float2*>(X + (r + m) * kPitchW + 2 * j);
-          *at = make_float2(fmaf(keep, at->x, x[m].x), fmaf(keep, at->y, x[m].y));
-        }
       }
     }
     __syncthreads();
@@ -265,42 +284,69 @@ cudaError_t launch_join(const Params& p, const Segments& g, int first, int scans
 }
 
 namespace {
-// Segments of two chunks at least, where the slices of all sequences and heads are fewer than two CTAs an SM.  (B2 S1024 H8 D64 in fp32: 32 CTAs
-// uncut; both launches and the join cost about as much again as the uncut scan's work, so that two segments gain nothing.)
-int segments_of(const Params& p, int num_sms) {
-  int64_t ctas = 0;
-  for (int i = 0; i < p.scans; ++i) ctas += (int64_t)p.batch * p.heads * ((p.scan[i].d2 + kWidth - 1) / kWidth);
-  const int64_t most = (p.seq_len + 2 * kChunk - 1) / (2 * kChunk);
-  int64_t n = 2 * num_sms / ctas;
-  n = n < most ? n : most;
-  n = n < 64 ? n : 64;
-  return n >= 3 ? (int)n : 1;
+struct Plan { int width, segments; };
+// Segments: two chunks each at least, where the slices of all sequences and heads are fewer than two CTAs an SM; fewer than three gain nothing, as both
+// passes and the join cost about the uncut scan's work again.  Width: slices of 64 columns feed more multiply-adds from each read and form a . b half
+// as often, but there are half as many, they take 7/6 of the time of 32 columns and fewer of them fit an SM.  So each is reckoned as passes x waves x
+// chunks of a CTA (bf16, 16 heads, 32 against 64 columns, us): heads of 256, B4 S1024, 6057 / 3531 (four waves / two); 192: 2162 / 2386 (two / two);
+// 160: 1517 / 1036 (two / one); 136, B1: 392 / 285 (3 / 6 segments); 256, B1 S128: 137 / 158 (one / one).
+Plan plan_of(const Params& p, int num_sms) {
+  Plan best{};
+  int64_t least = 0;
+  const int64_t chunks = ((int64_t)p.seq_len + kChunk - 1) / kChunk;
+  for (int width = 32; width <= 64; width += 32) {
+    int64_t ctas = 0;
+    size_t smem = 0;
+    for (int i = 0; i < p.scans; ++i) {
+      ctas += (int64_t)p.batch * p.heads * ((p.scan[i].d2 + width - 1) / width);
+      const size_t need = smem_bytes(p.scan[i].d1, width);
+      smem = need > smem ? need : smem;
+    }
+    if (ctas == 0) return Plan{32, 1};
+    const int64_t most = (chunks + 1) / 2;
+    int64_t n = 2 * num_sms / ctas;
+    n = n < most ? n : most;
+    n = n < 64 ? n : 64;
+    if (n < 3) n = 1;
+    int64_t fit = (int64_t)(228 * 1024 / (smem + 1024));
+    fit = fit < ctas_of(width) ? fit : ctas_of(width);
+    const int64_t at_once = (fit > 1 ? fit : 1) * num_sms;
+    const int64_t cost = (n > 1 ? 2 : 1) * ((ctas * n + at_once - 1) / at_once) * ((chunks + n - 1) / n) * (width == 64 ? 7 : 6);
+    if (best.width == 0 || cost < least) {
+      best = Plan{width, (int)n};
+      least = cost;
+    }
+  }
+  return best;
 }
 }  // namespace
 
 int64_t scan_generic_bytes(const Params& p, int num_sms) {
-  const int n = segments_of(p, num_sms);
+  const int n = plan_of(p, num_sms).segments;
   return n == 1 ? 0 : (int64_t)p.scans * p.batch * p.heads * n * p.scan[0].d1 * p.scan[0].d2 * 4;
 }
 
 cudaError_t launch_scan_generic(const Params& p, int num_sms, float* work, int64_t work_bytes, cudaStream_t stream, int* launches) {
   int64_t grid = 0;
   size_t smem = 0;
+  const Plan plan = plan_of(p, num_sms);
+  const int width = plan.width;
   Segments g;
-  g.count = work && work_bytes >= scan_generic_bytes(p, num_sms) ? segments_of(p, num_sms) : 1;
+  g.count = work && work_bytes >= scan_generic_bytes(p, num_sms) ? plan.segments : 1;
   const int64_t per = (p.seq_len + g.count - 1) / g.count, rows = (per + kChunk - 1) / kChunk * kChunk;
   g.rows = (int)(rows < 0x7fffffe0ll ? rows : 0x7fffffe0ll);
   g.states_only = 0;
   g.work = work;
   for (int i = 0; i < p.scans; ++i) {
-    const int64_t n = (int64_t)p.batch * p.heads * g.count * ((p.scan[i].d2 + kWidth - 1) / kWidth);
+    const int64_t n = (int64_t)p.batch * p.heads * g.count * ((p.scan[i].d2 + width - 1) / width);
     grid = n > grid ? n : grid;
-    const size_t need = smem_bytes(p.scan[i].d1);
+    const size_t need = smem_bytes(p.scan[i].d1, width);
     smem = need > smem ? need : smem;
   }
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  auto kern = p.dtype == AIDN_F32 ? scan_kernel<float> : p.dtype == AIDN_F16 ? scan_kernel<__half> : scan_kernel<__nv_bfloat16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(256));
+  auto kern = width == 64 ? (p.dtype == AIDN_F32 ? scan_kernel<float, 64> : p.dtype == AIDN_F16 ? scan_kernel<__half, 64> : scan_kernel<__nv_bfloat16, 64>)
+                          : (p.dtype == AIDN_F32 ? scan_kernel<float, 32> : p.dtype == AIDN_F16 ? scan_kernel<__half, 32> : scan_kernel<__nv_bfloat16, 32>);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(256, width));
   if (e != cudaSuccess) return e;
   if (g.count > 1) {
     g.states_only = 1;
