@@ -3,7 +3,8 @@
 //
 //     S   = A B^T                      scores, 64 x 64 (rows of A in lanes 0-63; the lanes above hold what is not looked at)
 //     P   = S weighted by lam^(i-j), zeros where j follows i, in 16 bits to shared memory
-//     T^T = C~^T B                     C~ = rows of C weighted by lam^(n-lag-j), as two or three 16-bit terms: what is added to a state is not rounded
+//     T^T = C~^T B                     C~ = rows of C weighted by lam^(n-lag-j), as two 16-bit terms (off by 2^-17 of a value in bf16, 2^-22
+//                                      in fp16), or three for bf16 states that go out (2^-24, as fp32 rounds)
 //     O^T = X^T A^T  and  C^T P^T      apart, since their columns have different factors; X^T in 16 bits in tensor memory
 //     X   = lam^n X + T                in fp32 registers, then X^T rounded for the next chunk
 //
@@ -14,8 +15,11 @@
 // Rows are taken from a sequence's last to its first for the gradients of keys and values: a tile is loaded as it lies, and only masks and
 // exponents turn around.  The last chunk's missing rows are zeros in C~, and in B and C, which multiply zeros.
 //
-// fp16: a row of P and a lane's row of X^T are scaled by a power of two to their own largest value, as neither is bound by fp16's range; the
-// second term of C~ is held 2^11 times as large, where fp16's smallest numbers do not cut it, and its product divided on the way into the first's.
+// fp16: a row of P, a lane's row of X^T and a chunk's column of C~ are scaled by a power of two to their own largest value, as none is bound by fp16's
+// range; the second term of C~ is held 2^11 times as large besides, and its product divided on the way into the first's.  A weighted value is then off by
+// 2^-22 of itself, or by 2^-50 of the largest in its column and chunk, where fp16's smallest numbers cut the second term.  (Without C~'s scale that was
+// 2^-36 whatever the values' size: a state of 7e-20 was zero, one of 1e-6 off by 6e-6.  It takes 22.5 -> 26.6 us of a prompt of 517 rows and 16 heads of 64,
+// 76.7 -> 82.0 us of the gradients of 3 sequences to 1531 rows and 12 heads; formed by the output's warps in place of these: 26.6 and 86.0.)
 //
 // What is not finite in C would reach earlier rows of its chunk as 0 * NaN in C^T P^T: columns that come out not finite are summed again, row by row, over
 // what a row may see.
@@ -62,12 +66,12 @@ struct Cfg {
   static constexpr int kOffY = kOffP + 2 * kBlock;                // output, 64 rows of 32 columns to a warp
   static constexpr int kOffTab = kOffY + 4 * kYBytes;
   // tables (floats): powers [65], weights of the scores by distance in four copies, each one element on from the one before (a row's begin anywhere
-  // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of maxima [2][2][128], weights of
-  // C~ by exponent, [2] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [2][2][4][4]
+  // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of the maxima of X and of C~, [2][2][128]
+  // each, weights of C~ by exponent, [2] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [2][2][4][4]
   static constexpr int kTabPower = 0, kTabScore = 68, kScorePitch = 136, kTabRow = kTabScore + 4 * kScorePitch, kTabP = kTabRow + 64, kTabX = kTabP + 128,
-                       kTabMax = kTabX + 512, kTabW = kTabMax + 512, kTabPairs = kTabW + 68, kTabFloats = kTabPairs + 64;
+                       kTabMax = kTabX + 512, kTabC = kTabMax + 512, kTabW = kTabC + 512, kTabPairs = kTabW + 68, kTabFloats = kTabPairs + 64;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
-  static constexpr int kBars = 2 * kStages + 20;
+  static constexpr int kBars = 2 * kStages + 24;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = kOffMisc + 16 + 1024;
   // tensor memory columns: X^T in 16 bits, T^T, S, O^T (state part, row part), C~^T in 16 bits (two terms in two buffers, or three)
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
   auto bar = [&](int n) { const uint32_t at = next_bar; next_bar += 8 * n; return at; };
   const uint32_t b_s_full = bar(2), b_s_empty = bar(1), b_p_full = bar(2), b_o_full = bar(2), b_o_empty = bar(2), b_bt_full = bar(2);
   const uint32_t b_t_full = bar(1), b_t_empty = bar(1), b_x_full = bar(1), b_x_empty = bar(1);
-  const uint32_t b_max = bar(4);   // of the two warps that share lanes
+  const uint32_t b_max = bar(4), b_most = bar(4);   // of the two warps that share lanes: X, C~
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(gen + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
 
@@ -247,7 +251,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       mbar_init(b_t_empty, 8);
       mbar_init(b_x_full, 8);
       mbar_init(b_x_empty, 1);
-      for (int i = 0; i < 4; ++i) mbar_init(b_max + 8 * i, 2);
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(b_max + 8 * i, 2);
+        mbar_init(b_most + 8 * i, 2);
+      }
       fence_mbar_init();
     }
     const double g = log_decay(p.decay, h);
@@ -471,7 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const int64_t matrix = (int64_t)D1 * D2;
       const int lag = s.lag;
-      const float key_scale = s.key_scale;   // in C~'s weights, or behind the product where they might leave fp16's range
+      const float key_scale = s.key_scale;   // in C~'s weights, for fp16 behind the product
+      float t_scale = key_scale, t_scale_next = key_scale;   // fp16: of T's lane, for this chunk and the next
       float x[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) x[i] = 0.f;
@@ -540,6 +548,39 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           // (matrices of a load: rows j .. j + 7 with columns d, d + 8; rows j + 8 .. j + 15 with the same)
           const int row = half * 32 + (lane & 7) + ((lane >> 4) << 3), col = quarter * 32 + (lane & 8);
           const uint32_t from = st + (col / 64) * kBlock + row * 128;
+          float w[8], up_all = 1.f;   // fp16: weights of this thread's rows, zeros where there are none; the power of two of column (lane & 3) * 8 + lane / 4
+          if constexpr (!BF16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int j = j_own + 8 * (i / 2) + (i & 1);
+              w[i] = there(j, n) ? power[exponent(j, n)] : 0.f;
+            }
+            float most[4] = {0.f, 0.f, 0.f, 0.f};   // of columns lane / 4, 8, 16 and 24 further
+#pragma unroll
+            for (int d = 0; d < 32; d += 16) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) ldmatrix_x4_trans(from + i * (16 * 128) + (((uint32_t)(((col & 63) + d) >> 3) ^ (uint32_t)(row & 7)) << 4), v + 4 * i);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 f = unpack16<BF16>(v[i]);
+                float& m = most[d / 8 + (i & 1)];
+                m = fmax3(m, fabsf(f.x * w[(i / 2) * 2]), fabsf(f.y * w[(i / 2) * 2 + 1]));   // (NaN counts for nothing)
+              }
+            }
+            // of four lanes and four columns, a column to each
+            const bool odd = lane & 1, upper = lane & 2;
+            const float m0 = fmaxf(odd ? most[1] : most[0], __shfl_xor_sync(0xffffffffu, odd ? most[0] : most[1], 1));
+            const float m1 = fmaxf(odd ? most[3] : most[2], __shfl_xor_sync(0xffffffffu, odd ? most[2] : most[3], 1));
+            float m = fmaxf(upper ? m1 : m0, __shfl_xor_sync(0xffffffffu, upper ? m0 : m1, 2));
+            float* most_of = table + C::kTabC + (c & 1) * 256 + quarter * 32 + lane;   // of 32 rows; the other warp's 128 further (two in turn, as above)
+            most_of[half * 128] = m;
+            arrive(b_most + 8 * quarter);
+            if (!wait(b_most + 8 * quarter, (uint32_t)(c & 1))) return false;
+            float back;
+            scale_of(fmaxf(m, most_of[(half ^ 1) * 128]), up_all, back);
+            t_scale_next = key_scale * __shfl_sync(0xffffffffu, back, (lane & 7) * 4 + lane / 8);
+          }
 #pragma unroll 1
           for (int d = 0; d < 32; d += 16) {
             uint32_t v[8], a[8], e[8];
@@ -560,23 +601,34 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
                 a[i] = bf16x2_mul(v[i], weights[0][i / 2]);
                 e[i] = bf16x2_fma(v[i], weights[1][i / 2], bf16x2_fma(v[i], weights[0][i / 2], a[i] ^ 0x80008000u));
               }
-            } else {
-              const float factor = BF16 ? key_scale : 1.f;
+            } else if constexpr (BF16) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int j = j_own + 8 * (i / 2);
                 float2 f = unpack16<BF16>(v[i]);
-                f.x *= power[there(j, n) ? exponent(j, n) : 0] * factor;
-                f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0] * factor;
+                f.x *= power[there(j, n) ? exponent(j, n) : 0] * key_scale;
+                f.y *= power[there(j + 1, n) ? exponent(j + 1, n) : 0] * key_scale;
                 a[i] = pack2<BF16>(f.x, f.y);
                 float2 t = unpack16<BF16>(a[i]);
                 f.x -= t.x;
                 f.y -= t.y;
-                e[i] = BF16 ? pack2<BF16>(f.x, f.y) : pack2<BF16>(f.x * 2048.f, f.y * 2048.f);
-                if constexpr (BF16) {
-                  t = unpack16<BF16>(e[i]);
-                  v[i] = pack2<BF16>(f.x - t.x, f.y - t.y);
-                }
+                e[i] = pack2<BF16>(f.x, f.y);
+                t = unpack16<BF16>(e[i]);
+                v[i] = pack2<BF16>(f.x - t.x, f.y - t.y);
+              }
+            } else {
+              float up[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) up[i] = __shfl_sync(0xffffffffu, up_all, (lane & ~3) + d / 8 + i);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int at = (i / 2) * 2;
+                float2 f = unpack16<BF16>(v[i]);
+                f.x *= w[at] * up[i & 1];
+                f.y *= w[at + 1] * up[i & 1];
+                a[i] = pack2<BF16>(f.x, f.y);
+                const float2 t = unpack16<BF16>(a[i]);
+                e[i] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
               }
             }
             tmem_st_16x128b_x4(to + ((uint32_t)d << 16), a);
@@ -621,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                   uint64_t t = pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                  if constexpr (!BF16) t = mul2(pack2(key_scale, key_scale), t);
+                  if constexpr (!BF16) t = mul2(pack2(t_scale, t_scale), t);
                   const float2 f = unpack2(fma2(keep, pack2(x[i0 + i], x[i0 + i + 1]), t));
                   x[i0 + i] = f.x;
                   x[i0 + i + 1] = f.y;
@@ -631,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             tc_fence_before();
             arrive(b_t_empty);
           }
+          t_scale = t_scale_next;
           if (!states_only && c + 1 < chunks) {
             if (c >= 0) {
               if (!(ok = wait(b_x_empty, (uint32_t)(c & 1)))) break;

@@ -1,0 +1,82 @@
+"""Linear attention at the edges of its types, sizes and calls.  Bounds not named here are those of test_gpu_linear."""
+import math
+
+import pytest
+import torch
+
+from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
+from tests._harness import TORCH_DT
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def backend():
+    return CudaBackend()
+
+
+# ---- fp16 values that are small, or weighted to little ---------------------------------------------------------------
+
+def one_row(dim, n, row, size, others, seed):
+    """fp16 [1, 1, n, dim]: N(0, size) in one row; the others hold as much, or zeros."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn((1, 1, n, dim), generator=g, device="cuda") * size).half()
+    keep = x.clone()
+    if not others:
+        x.zero_()
+    x[:, :, row] = keep[:, :, row]
+    return x
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [64, 50])
+@pytest.mark.parametrize("decay,size", [(math.log(0.7), 1.3e-6), (-0.7, 1.0), (-0.7, 1e-6), (-0.1, 60.0)])
+@pytest.mark.parametrize("back", [False, True])
+def test_small_fp16_values_in_states(backend, dim, n, decay, size, back):
+    """What one row adds to a state of a chunk: S = w k v^T (w = exp(decay * rows behind it)), and for the gradient of a first state scale * w q do^T.
+    The weight is off by 2^-24, its product with a value by 2^-24, two fp16 terms leave 2^-22, two exact products are added (2^-22 where bits are
+    cut off), and scale and its product are off by 2^-24 each: 0.82 * 2^-20 of S.  Where other rows of a column have larger weighted values,
+    fp16's smallest numbers leave 2^-50 of the largest of them besides."""
+    for row in (0, n - 2, n - 1):
+        for others in (False, True):
+            thick = one_row(dim, n, row, size, others, row)                  # values, or gradients of outputs
+            thin = one_row(dim, n, row, 0.5, not others, row + 1)            # keys, or queries
+            g = torch.tensor([decay], device="cuda")
+            behind = torch.arange(1, n + 1, device="cuda") if back else torch.arange(n - 1, -1, -1, device="cuda")
+            w = torch.exp(g.double() * behind)[:, None]
+            rest = torch.zeros(1, 1, n, dim, dtype=torch.float16, device="cuda")
+            got = torch.full((1, 1, dim, dim), math.nan, device="cuda")
+            if back:
+                outs = [torch.empty_like(rest) for _ in range(3)]
+                backend.LinearAttentionBackward(GpuBuffer(thick), GpuBuffer(thin), GpuBuffer(rest), GpuBuffer(rest.clone()), *(GpuBuffer(x) for x in outs),
+                                                GpuBuffer(g), 1, 1, 1, n, dim, dim, gradInitialStates=GpuBuffer(got))
+                w = w * dim ** -0.5
+            else:
+                backend.LinearAttention(GpuBuffer(rest), GpuBuffer(thin), GpuBuffer(thick), GpuBuffer(torch.empty_like(rest)), GpuBuffer(g), 1, 1, 1, n, dim,
+                                        dim, finalStates=GpuBuffer(got))
+            a, b = thin[0, 0].double(), thick[0, 0].double() * w
+            ref = a[row][:, None] * b[row][None, :]
+            floor = a[row].abs()[:, None] * b.abs().amax(0)[None, :] * 2.0 ** -50 if others else 0.0
+            off = (got[0, 0].double() - ref).abs()
+            assert bool((off <= 2.0 ** -20 * ref.abs() + floor).all()), (row, others, float((off / ref.abs()).nan_to_num().max()))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_fp16_values_stay_in_their_columns(backend, dim):
+    """A column's own scale: an infinity or NaN in one column of the values leaves the states' other columns as they were."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = ((torch.randn((1, 2, 150, dim), generator=g, device="cuda") * 0.5).half() for _ in range(3))
+    decay, out = torch.tensor([-0.01, -0.3], device="cuda"), torch.empty_like(q)
+
+    def states():
+        last = torch.empty(1, 2, dim, dim, device="cuda")
+        backend.LinearAttention(*(GpuBuffer(x) for x in (q, k, v, out, decay)), 1, 2, 2, 150, dim, dim, finalStates=GpuBuffer(last))
+        return last
+
+    clean = states()
+    for bad in (math.inf, math.nan):
+        v[0, 1, 70, 5] = bad
+        last = states()
+        hit = torch.zeros_like(last, dtype=torch.bool)
+        hit[0, 1, :, 5] = True
+        assert torch.equal(last[~hit], clean[~hit]) and not bool(torch.isfinite(last[hit]).any())
