@@ -799,6 +799,11 @@ class CudaBackend:
         if batch > 0:
             self.launch_count += 1
 
+    def LinearAttentionPoll(self) -> None:
+        """Waits for this backend's stream and raises if a ``LinearAttention`` or ``LinearAttentionBackward`` of its device gave up a bounded wait since this
+        stream was last told (none does in normal operation): what they wrote since then is not to be used."""
+        N.linear_attention_poll(self._raw_stream)
+
     def FlashAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer,
                                output: GpuBuffer, softmaxStats: GpuBuffer, gradQuery: GpuBuffer, gradKey: GpuBuffer,
                                gradValue: GpuBuffer, batch: int, numHeads: int, seqQ: int, seqK: int, headDim: int,

@@ -8,8 +8,10 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <new>
+#include <utility>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -1087,8 +1089,41 @@ cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int
   return *waits ? aidn::lin::launch_scan_sm100(p, sms, reinterpret_cast<float*>(work), work_bytes, expire, stream, &launches)
                 : aidn::lin::launch_scan_generic(p, sms, reinterpret_cast<float*>(work), work_bytes, stream, &launches);
 }
+// Waits for `stream` and reports a wait given up in its context that was not yet reported for this stream.  What each stream was told is kept here, and
+// only where there was something to tell; a stream's id is never another one's, its handle may be.
+int linear_report(const char* op, cudaStream_t stream, const char* prefix = "") {
+  cudaError_t e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess) return fail_cuda(e, op);
+  const uint32_t* word = aidn::lin::sm100_gave_up();
+  if (!word) return fail(AIDN_ECUDA, "%s: no count of waits in the current context", op);
+  uint32_t count = 0;
+  unsigned long long id = 0;
+  e = cudaMemcpyAsync(&count, word, sizeof(count), cudaMemcpyDeviceToHost, stream);   // (on this stream: no other is waited for)
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess) return fail_cuda(e, op);
+  if (count == 0) return AIDN_OK;
+  e = cudaStreamGetId(stream, &id);
+  if (e != cudaSuccess) return fail_cuda(e, op);
+  static std::mutex lock;
+  try {
+    const std::lock_guard<std::mutex> guard(lock);
+    static auto& told = *new std::map<std::pair<const uint32_t*, unsigned long long>, uint32_t>;   // (never destroyed: threads may outlive main)
+    uint32_t& last = told[{word, id}];
+    if (last == count) return AIDN_OK;
+    last = count;
+  } catch (...) {   // no memory to remember it in: it will be told again
+  }
+  return fail(AIDN_ETIMEOUT, "%s%s: a kernel gave up a bounded wait", prefix, op);
+}
 int linear_check(const char* what, cudaStream_t stream, bool waits) {
-  return post_launch_check(stream, what, waits && launch_check_enabled() ? aidn::lin::sm100_status() : nullptr, true);
+  const int rc = post_launch_check(stream, what, nullptr);
+  if (rc != AIDN_OK || !waits || !launch_check_enabled()) return rc;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return AIDN_OK;
+  }
+  return linear_report(what, stream, "[LAUNCH-FAULT] ");
 }
 }  // namespace
 
@@ -1305,16 +1340,7 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
 
 int aidn_linear_attention_poll(void* cu_stream) {
   g_err[0] = 0;
-  cudaError_t e = cudaStreamSynchronize((cudaStream_t)cu_stream);
-  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_poll: stream");
-  int32_t* status = aidn::lin::sm100_status();
-  if (!status) return fail(AIDN_ECUDA, "linear_attention_poll: no status word in the current context");
-  int32_t st = 0;
-  e = cudaMemcpy(&st, status, sizeof(st), cudaMemcpyDeviceToHost);
-  if (e != cudaSuccess) return fail_cuda(e, "linear_attention_poll: status read");
-  if (st == 0) return AIDN_OK;
-  cudaMemset(status, 0, sizeof(st));
-  return fail(AIDN_ETIMEOUT, "linear_attention_poll: a kernel gave up a bounded wait (status word 0x%x)", st);
+  return linear_report("linear_attention_poll", (cudaStream_t)cu_stream);
 }
 
 int aidn_linear_attention_step(const aidn_linear_step_args* a, void* cu_stream) {

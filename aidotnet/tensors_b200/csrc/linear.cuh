@@ -112,7 +112,7 @@ bool scan_sm100_supported(const Params& p);
 int64_t scan_sm100_bytes(const Params& p, int num_sms);
 // expire: test hook - the loads are withheld and bounded waits give up after 20 ms.
 cudaError_t launch_scan_sm100(const Params& p, int num_sms, float* work, int64_t work_bytes, bool expire, cudaStream_t stream, int* launches);
-int32_t* sm100_status();   // address of its status word in the current context, or null
+uint32_t* sm100_gave_up();   // address of its count of CTAs that gave up in the current context, or null
 
 // dk / dv of shared heads: fp32 partial sums [.., heads, .., d] summed over each group in order
 struct GroupSum {

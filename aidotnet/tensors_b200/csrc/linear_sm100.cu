@@ -33,7 +33,7 @@
 // arithmetic and stores by TMA 70; C~ by shared memory in place of tensor memory 80; four more warps for C~ at 96 registers a thread 76; products issued by
 // two warps, and those of T and O in turn, made no difference.
 //
-// Every wait is bounded; a CTA that gives up sets the status word and leaves through the common teardown.
+// Every wait is bounded; a CTA that gives up counts itself and leaves through the common teardown.
 #include <cuda.h>
 
 #include "ffma2.cuh"
@@ -47,7 +47,9 @@ namespace {
 
 using namespace ptx;
 
-__device__ int32_t g_linear_status;   // set when a bounded wait gave up (the entry points have no handle whose status word could say so)
+// How many CTAs gave up a bounded wait in this context.  (The entry points have no handle whose status word could say so; never cleared, so that whoever asks
+// can tell what is new to them.)
+__device__ uint32_t g_linear_gave_up;
 
 constexpr int kChunk = 64;
 constexpr int kBlock = kChunk * 128;   // 64 rows of 64 16-bit elements
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
     if (*abort_flag) {
       if (threadIdx.x == 0) {
         abort_grace();
-        atomicOr(&g_linear_status, kStatusTimeout);
+        atomicAdd(&g_linear_gave_up, 1u);
       }
       __syncthreads();
     }
@@ -904,13 +906,13 @@ int segments_of(const Params& p, int num_sms) {
 
 }  // namespace
 
-int32_t* sm100_status() {
+uint32_t* sm100_gave_up() {
   void* addr = nullptr;
-  if (cudaGetSymbolAddress(&addr, g_linear_status) != cudaSuccess) {
+  if (cudaGetSymbolAddress(&addr, g_linear_gave_up) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
-  return static_cast<int32_t*>(addr);
+  return static_cast<uint32_t*>(addr);
 }
 
 bool scan_sm100_supported(const Params& p) {

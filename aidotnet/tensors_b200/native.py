@@ -690,5 +690,5 @@ def linear_attention_step(*, q: int, k: int, v: int, out: int, states: int, batc
 
 
 def linear_attention_poll(stream: int) -> None:
-    """Synchronises ``stream`` and raises if a linear attention call gave up a bounded wait since the last report."""
+    """Synchronises ``stream`` and raises if a linear attention call of its context gave up a bounded wait since the last report for this stream."""
     check(load().aidn_linear_attention_poll(ctypes.c_void_p(stream)))

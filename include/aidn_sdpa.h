@@ -65,7 +65,7 @@ typedef enum {
   AIDN_ECUDA = 3,        /* a CUDA call failed; aidn_sdpa_last_error() carries its message   */
   AIDN_EWORKSPACE = 4,   /* workspace missing or too small                                   */
   AIDN_ETIMEOUT = 5,     /* a bounded device-side wait expired (reported by aidn_sdpa_poll,
-                            aidn_qkv_rope_poll)                                             */
+                            aidn_qkv_rope_poll, aidn_linear_attention_poll)                 */
   AIDN_ENCCL = 6         /* NCCL missing or an NCCL call failed                              */
 } aidn_status;
 
@@ -458,8 +458,10 @@ typedef struct {
 AIDN_API int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linear_bwd_args* args);
 AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, void* cu_stream);
 
-/* Synchronises `cu_stream` and returns AIDN_ETIMEOUT if one of these calls gave up a bounded wait since the last report (its outputs are then
- * not to be used), AIDN_ECUDA on a CUDA error, else AIDN_OK.  They have no handle: the word is one per CUDA context, and reporting it clears it. */
+/* Synchronises `cu_stream` and returns AIDN_ETIMEOUT if one of these calls gave up a bounded wait since the last report for this stream, or if there was none
+ * since the context was made; AIDN_ECUDA on a CUDA error, else AIDN_OK.  The calls have no handle, and a graph may be replayed on another stream than its
+ * calls were made on: waits are counted by CUDA context, so that one that ran out is told to every stream that asks, once to each.  Outputs and states of
+ * the calls since a stream's report before are then not to be used, as any of them may be the one. */
 AIDN_API int aidn_linear_attention_poll(void* cu_stream);
 
 /* One token of each of `batch` sequences against states that stay where they are: state state_slots[b] (NULL: b) is updated in place.  A

@@ -1,9 +1,13 @@
 """Linear attention at the edges of its types, sizes and calls.  Bounds not named here are those of test_gpu_linear."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
+from aidotnet.tensors_b200 import native as N
 from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
 from tests._harness import TORCH_DT
 
@@ -80,3 +84,76 @@ def test_infinite_fp16_values_stay_in_their_columns(backend, dim):
         hit = torch.zeros_like(last, dtype=torch.bool)
         hit[0, 1, :, 5] = True
         assert torch.equal(last[~hit], clean[~hit]) and not bool(torch.isfinite(last[hit]).any())
+
+
+# ---- waits that ran out, and several streams -------------------------------------------------------------------------
+
+def test_every_stream_is_told_of_a_wait_that_ran_out():
+    """A call on one stream gives up: a poll of another stream tells that stream, and takes the report from neither the first one nor a third."""
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    backends = [CudaBackend(stream=s) for s in streams]
+    x = [[(torch.randn(1, 2, 100, 64, device="cuda") * 0.5).bfloat16() for _ in range(4)] for _ in streams]
+    torch.cuda.synchronize()
+
+    def call(i):
+        backends[i].LinearAttention(*(GpuBuffer(t) for t in x[i]), None, 1, 2, 2, 100, 64, 64)
+
+    def told(i):
+        try:
+            backends[i].LinearAttentionPoll()
+        except N.AidnError as e:
+            assert e.status == N.ETIMEOUT
+            return True
+        return False
+
+    for i in range(3):
+        call(i)
+        told(i)   # (of what tests before this one may have left to tell)
+    assert not any(told(i) for i in range(3))
+    assert N.load().aidn_sdpa_debug_set(None, None, 5) == N.OK
+    call(0)
+    call(1)
+    streams[0].synchronize()
+    assert told(1) and told(0) and told(2)
+    assert not any(told(i) for i in range(3))
+    right = x[1][3].clone()
+    call(0)
+    call(1)
+    assert not told(0) and not told(1)
+    assert torch.equal(x[1][3], right)
+    try:
+        N.linear_attention_poll(torch.cuda.current_stream().cuda_stream)   # (the stream of other tests is told here, not there)
+    except N.AidnError:
+        pass
+
+
+_CHECKED = """
+import torch
+from aidotnet.tensors_b200 import native as N
+from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
+b, other = CudaBackend(), CudaBackend(stream=torch.cuda.Stream())
+x = [(torch.randn(1, 2, 100, 64, device="cuda") * 0.5).bfloat16() for _ in range(4)]
+torch.cuda.synchronize()
+go = lambda b: b.LinearAttention(*(GpuBuffer(t) for t in x), None, 1, 2, 2, 100, 64, 64)
+go(b); go(other)
+assert N.load().aidn_sdpa_debug_set(None, None, 5) == N.OK
+try:
+    go(b)
+    raise SystemExit("the call did not report the wait that ran out")
+except N.AidnError as e:
+    assert e.status == N.ETIMEOUT and "LAUNCH-FAULT" in e.message, (e.status, e.message)
+go(b); b.LinearAttentionPoll()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=other.stream):
+    go(other)
+graph.replay(); torch.cuda.synchronize()
+print("launch check ok")
+"""
+
+
+def test_launch_check_reports_a_wait_that_ran_out():
+    """With AIDOTNET_KERNEL_LAUNCH_CHECK the call itself reports it, once; calls that are captured are not checked.  (The variable is read once.)"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, AIDOTNET_KERNEL_LAUNCH_CHECK="1", PYTHONPATH=root)
+    r = subprocess.run([sys.executable, "-c", _CHECKED], capture_output=True, text=True, timeout=300, env=env, cwd=root)
+    assert r.returncode == 0 and "launch check ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
