@@ -2,12 +2,13 @@
 //     (a, b) -> amplitude * (a cos - b sin, a sin + b cos);  the gradient is the same with the angle negated.
 //
 // Bound by memory: every element once in and once out.  The angles of a token serve all of its heads, so a CTA takes a few tokens
-// with all heads, forms their cosines and sines once in shared memory and then streams.  An angle is formed in 64 bits, in turns: the
-// nearest whole turn is taken off there, and what is left (at most half a turn) has an error of 2^-25 turns in 32 bits wherever the
-// position is; a product in 32 bits would be off by the position times 2^-24.
+// with all heads, forms their cosines and sines once in shared memory and then streams.  An angle is formed in turns as
+// two numbers of 64 bits each, the second what the first one's rounding leaves: the nearest whole turn is taken off the first, and what is left (at most
+// half a turn) has an error of 2^-25 turns in 32 bits for every position that 64 bits hold as they are, up to 2^53.  (One number of 64 bits would be off by
+// position * frequency * 2^-55 turns, a product in 32 bits by the position times 2^-24.)
 //
-// Two units of 32 bytes in flight to a thread and six CTAs an SM: 8192 tokens of 40 heads of 128 (bf16, out of a packed projection) 34.9 us, 4.8 TB/s;
-// four units and three CTAs 38.1 us, two units and twice the tokens to a CTA 36.2 us.
+// Two units of 32 bytes in flight to a thread and six CTAs an SM: 8192 tokens of 40 heads of 128 (bf16, out of a packed projection) 35.4 us, 4.7 TB/s
+// (34.9 with angles of one number); four units and three CTAs 38.1 us, two units and twice the tokens to a CTA 36.2 us.
 #include "linear.cuh"
 
 namespace aidn {
@@ -17,6 +18,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBatch = 2;          // units of a thread whose loads are in flight together
 constexpr int kMaxTokens = 16;     // of a CTA
+constexpr double kPerRadian = 0.15915494309189535, kPerRadianLeft = -9.839338337591243e-18;   // 1 / 2 pi, and what its rounding leaves
 
 template <int BYTES>
 struct Raw;
@@ -70,9 +72,12 @@ __global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const Rotary p, con
     if (!p.positions) pos = p.start + (t0 + t) % p.seq_len;
     else if (p.wide_positions) pos = static_cast<const int64_t*>(p.positions)[t0 + t];
     else pos = static_cast<const int32_t*>(p.positions)[t0 + t];
-    const double turns = (double)pos * (p.frequencies[i] * 0.15915494309189533577);
+    // turns a position, f / 2 pi, with 1 / 2 pi in two numbers; then turns, and what is left of them
+    const double f = p.frequencies[i], x = (double)pos;
+    const double per = f * kPerRadian, per_left = fma(f, kPerRadian, -per) + f * kPerRadianLeft;
+    const double turns = x * per, turns_left = fma(x, per, -turns) + x * per_left;
     float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    sincospif(2.f * (float)((turns - rint(turns)) + turns_left), &s, &c);
     table[e] = make_float2(c * p.amplitude, s * p.amplitude * p.sign);
   }
   __syncthreads();

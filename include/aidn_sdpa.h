@@ -360,8 +360,8 @@ AIDN_API int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* args, con
 
 /* ---- rotary positions -------------------------------------------------------------------------------------------------
  * The pairs of the first rotary_dim elements of every head, turned by position * frequency:
- * (a, b) -> amplitude * (a cos - b sin, a sin + b cos); the elements behind them are copied.  Angles are formed in 64 bits from the
- * frequencies, so that a position far into a long context is as exact as the first, and any scaling for long contexts is a choice of
+ * (a, b) -> amplitude * (a cos - b sin, a sin + b cos); the elements behind them are copied.  Angles are formed from the frequencies in
+ * twice 64 bits, so that a position far into a long context (up to 2^53) is as exact as the first, and any scaling for long contexts is a choice of
  * frequencies and amplitude.  Products and sums in fp32, one rounding.  With `inverse` the angles are negated: the gradient.
  * Queries, and keys if there are any, in one launch.  An output may be its input itself, with the same strides; otherwise nothing overlaps. */
 typedef struct {

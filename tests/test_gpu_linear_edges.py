@@ -1,8 +1,9 @@
-"""Linear attention at the edges of its types, sizes and calls.  Bounds not named here are those of test_gpu_linear."""
+"""Rotary positions and linear attention at the edges of its types, sizes and calls.  Bounds not named here are those of test_gpu_linear."""
 import math
 import os
 import subprocess
 import sys
+from fractions import Fraction
 
 import pytest
 import torch
@@ -157,3 +158,23 @@ def test_launch_check_reports_a_wait_that_ran_out():
     env = dict(os.environ, AIDOTNET_KERNEL_LAUNCH_CHECK="1", PYTHONPATH=root)
     r = subprocess.run([sys.executable, "-c", _CHECKED], capture_output=True, text=True, timeout=300, env=env, cwd=root)
     assert r.returncode == 0 and "launch check ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
+
+
+# ---- rotary positions far out ----------------------------------------------------------------------------------------
+
+TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798")
+
+
+@pytest.mark.parametrize("base", [10000.0, 2.0])
+def test_far_positions_are_as_exact_as_near_ones(backend, base):
+    """Angles reduced in whole numbers: test_gpu_rotary's bound, 2^-21 of the pair's magnitudes, at every position that 64 bits hold."""
+    pos = [0, 1, 12345, (1 << 31) - 1, 1 << 31, (1 << 40) + 12345, -(1 << 40) - 7, (1 << 47) + 1, (1 << 52) + 3, (1 << 53) - 1, -(1 << 53) + 1]
+    f = backend.RotaryFrequencies(64, base)
+    left = [[Fraction(w) * p % TWO_PI for w in f.tensor.tolist()] for p in pos]
+    c, s = (torch.tensor([[fn(float(a)) for a in row] for row in left], dtype=torch.float64, device="cuda")[:, None] for fn in (math.cos, math.sin))
+    x = torch.randn(len(pos), 3, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    y = torch.empty_like(x)
+    backend.RotaryEmbedding(GpuBuffer(x), GpuBuffer(y), None, None, f, len(pos), 3, 0, 64, positions=GpuBuffer(torch.tensor(pos, device="cuda")))
+    a, b = x.double()[..., ::2], x.double()[..., 1::2]
+    for got, ref in ((y[..., ::2], a * c - b * s), (y[..., 1::2], a * s + b * c)):
+        assert bool(((got.double() - ref).abs() <= 2.0 ** -24 * ref.abs() + 2.0 ** -21 * (a.abs() + b.abs())).all())
