@@ -601,7 +601,7 @@ class CudaBackend:
         """Turns the first 2 * frequencies.Size elements of every head of ``query`` [tokens, heads, headDim] and, if given, ``key``
         [tokens, kvHeads, headDim] by their token's position: in pairs (2i, 2i+1) or, not ``interleaved``, (i, i + half).  Token t is
         at ``positions``[t] (int32 or int64), without them at startPosition + t % seqLen (0: tokens).  The turned elements are multiplied by
-        ``amplitude``, the others copied.  The outputs are dense, or the inputs themselves.  ``queryStride`` / ``keyStride``: elements
+        ``amplitude``, the others copied.  The outputs are dense, or the inputs themselves (then no two rows may overlap).  ``queryStride`` / ``keyStride``: elements
         from a token to the next and from a head to the next, for rows that hold more than these heads (a packed projection,
         whose queries and keys are heads + kvHeads heads side by side)."""
         self._rotary("RotaryEmbedding", False, query, queryOut, key, keyOut, frequencies, tokens, heads, kvHeads, headDim, seqLen, startPosition,
@@ -716,6 +716,7 @@ class CudaBackend:
         """Linear attention of whole sequences: S_t = exp(decay) S_(t-1) + k_t v_t^T, o_t = scale * q_t S_t (scale 0: 1/sqrt(keyDim)) with
         the head's log ``decay`` [heads] fp32, at most 0 (None: no decay).  ``query`` [batch, heads, seqLen, keyDim], ``key`` and
         ``value`` [batch, kvHeads, seqLen, ..], ``output`` [batch, heads, seqLen, valueDim]; ``tokenMajor``: [batch, seqLen, heads, ..].
+        ``output`` is none of the inputs.
         ``lengths`` int32 [batch]: the rows behind them are padding, and zeros in ``output``.  ``tokenStarts`` int32 [batch + 1]: packed
         rows [tokens, heads, ..] instead, sequence b's from tokenStarts[b] on, at most seqLen of them; rows of no sequence are left.
         Sequence b begins with state stateSlots[b] (or b) of ``initialStates`` [.., heads, keyDim, valueDim] fp32 (None or a negative
@@ -768,7 +769,7 @@ class CudaBackend:
                             decay: Optional[GpuBuffer], batch: int, heads: int, kvHeads: int, keyDim: int, valueDim: int, scale: float = 0.0,
                             stateSlots: Optional[GpuBuffer] = None) -> None:
         """One token of each of ``batch`` sequences: ``query`` [batch, heads, keyDim], ``key`` and ``value`` [batch, kvHeads, ..], ``output``
-        [batch, heads, valueDim].  State stateSlots[b] (or b) of ``states`` [.., heads, keyDim, valueDim] fp32 is updated in place.  A
+        [batch, heads, valueDim], none of the inputs.  State stateSlots[b] (or b) of ``states`` [.., heads, keyDim, valueDim] fp32 is updated in place.  A
         negative slot is a row of padding: zeros, and no state is touched.  A slot that is not there, or an earlier row's, gives NaN and
         touches no state."""
         op = "LinearAttentionStep"

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <new>
@@ -1041,6 +1042,27 @@ bool take_strides(int n, const int64_t* given, const int64_t* dense, int64_t* to
   return true;
 }
 
+// Whether rows of an output may share elements, which two threads would then write in any order: each stride has to hold what the smaller ones span.
+bool rows_meet(int n, const int64_t* extent, const int64_t* stride, int64_t size) {
+  bool done[3] = {false, false, false};
+  for (int i = 0; i < n; ++i) {
+    int least = -1;
+    for (int j = 0; j < n; ++j)
+      if (!done[j] && extent[j] > 1 && (least < 0 || stride[j] < stride[least])) least = j;
+    if (least < 0) return false;
+    if (stride[least] < size) return true;
+    size += (extent[least] - 1) * stride[least];
+    done[least] = true;
+  }
+  return false;
+}
+// Whether an output is one of the tensors that a call reads or writes besides.
+bool is_one_of(const void* out, std::initializer_list<const void*> others) {
+  for (const void* x : others)
+    if (out && out == x) return true;
+  return false;
+}
+
 // The sizes and pointers that a forward and a backward call share.
 int linear_common(const char* op, const aidn_linear_args& a, aidn::lin::Params& p) {
   if (a.batch <= 0 || a.heads <= 0 || a.kv_heads <= 0) return fail(AIDN_EINVAL, "%s: batch, heads and kv_heads must be positive", op);
@@ -1079,6 +1101,11 @@ bool linear_tensor(const aidn_linear_args& a, const void* ptr, const int64_t* gi
 }
 
 bool no_rows(const aidn_linear_args& a) { return a.token_starts && a.tokens == 0; }
+
+bool linear_rows_meet(const aidn_linear_args& a, int64_t heads, int64_t size, const int64_t* stride) {
+  const int64_t extent[3] = {a.token_starts ? 1 : a.batch, heads, a.token_starts ? a.tokens : a.seq_len};
+  return rows_meet(3, extent, stride, size);
+}
 
 // The scans of a call, and the check behind them.
 cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int sms, char* work, int64_t work_bytes, cudaStream_t stream, bool* waits) {
@@ -1158,7 +1185,10 @@ int aidn_rotary(const aidn_rotary_args* a, void* cu_stream) {
     if (!take_strides(2, in[i], dense, p.xs[i]) || !take_strides(2, out[i], dense, p.ys[i])) return fail(AIDN_EINVAL, "rotary: negative stride");
     if (p.heads[i] > 0 && p.x[i] == p.y[i] && (p.xs[i][0] != p.ys[i][0] || p.xs[i][1] != p.ys[i][1]))
       return fail(AIDN_EINVAL, "rotary: in place needs the same strides in and out");
+    const int64_t extent[2] = {a->tokens, p.heads[i]};
+    if (p.heads[i] > 0 && rows_meet(2, extent, p.ys[i], a->head_dim)) return fail(AIDN_EINVAL, "rotary: rows of an output overlap");
   }
+  if (is_one_of(a->query_out, {a->key, a->key_out}) || is_one_of(a->key_out, {a->query})) return fail(AIDN_EINVAL, "rotary: queries and keys overlap");
   p.frequencies = a->frequencies;
   p.positions = a->positions;
   p.tokens = a->tokens;
@@ -1215,6 +1245,8 @@ int aidn_linear_attention(const aidn_linear_args* a, void* cu_stream) {
   if (!linear_tensor(*a, a->q, a->q_stride, a->heads, a->key_dim, s.as) || !linear_tensor(*a, a->k, a->k_stride, a->kv_heads, a->key_dim, s.bs) ||
       !linear_tensor(*a, a->v, a->v_stride, a->kv_heads, a->value_dim, s.cs) || !linear_tensor(*a, a->out, a->o_stride, a->heads, a->value_dim, s.ys))
     return fail(AIDN_EINVAL, "linear_attention: a tensor is not aligned to its elements, or a stride is negative");
+  if (linear_rows_meet(*a, a->heads, a->value_dim, s.ys) || is_one_of(a->out, {a->q, a->k, a->v}))
+    return fail(AIDN_EINVAL, "linear_attention: rows of out overlap one another or an input");
   p.scans = 1;
   s.a = a->q; s.b = a->k; s.c = a->v; s.y = a->out;
   s.a_group = 1;
@@ -1276,6 +1308,10 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
   if (group > 1 && part[0] + part[1] > 0 && (!f.workspace || f.workspace_bytes < part[0] + part[1]))
     return fail(AIDN_EWORKSPACE, "linear_attention_backward: workspace of %lld bytes, need %lld", (long long)(f.workspace ? f.workspace_bytes : 0),
                 (long long)(part[0] + part[1]));
+  if (linear_rows_meet(f, f.heads, dk, dqs) || linear_rows_meet(f, f.kv_heads, dk, dks) || linear_rows_meet(f, f.kv_heads, dv, dvs) ||
+      is_one_of(a->dq, {f.q, f.k, f.v, a->dout, a->dk, a->dv}) || is_one_of(a->dk, {f.q, f.k, f.v, a->dout, a->dv}) ||
+      is_one_of(a->dv, {f.q, f.k, f.v, a->dout}))
+    return fail(AIDN_EINVAL, "linear_attention_backward: rows of gradients overlap one another or an input");
   auto copy3 = [](int64_t* to, const int64_t* from) { std::memcpy(to, from, 3 * sizeof(int64_t)); };
   const int64_t rows = f.token_starts ? f.tokens : f.seq_len;   // of a head of the partial sums
   p.scans = 3;
@@ -1366,6 +1402,8 @@ int aidn_linear_attention_step(const aidn_linear_step_args* a, void* cu_stream) 
   const int64_t dq[2] = {a->heads * kd, kd}, dk[2] = {a->kv_heads * kd, kd}, dv[2] = {a->kv_heads * vd, vd}, dout[2] = {a->heads * vd, vd};
   if (!take_strides(2, a->q_stride, dq, p.qs) || !take_strides(2, a->k_stride, dk, p.ks) || !take_strides(2, a->v_stride, dv, p.vs) || !take_strides(2, a->o_stride, dout, p.os))
     return fail(AIDN_EINVAL, "linear_attention_step: negative stride");
+  const int64_t extent[2] = {a->batch, a->heads};
+  if (rows_meet(2, extent, p.os, vd) || is_one_of(a->out, {a->q, a->k, a->v})) return fail(AIDN_EINVAL, "linear_attention_step: rows of out overlap one another or an input");
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
   p.states = a->states;
   p.decay = a->decay;

@@ -363,7 +363,8 @@ AIDN_API int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* args, con
  * (a, b) -> amplitude * (a cos - b sin, a sin + b cos); the elements behind them are copied.  Angles are formed from the frequencies in
  * twice 64 bits, so that a position far into a long context (up to 2^53) is as exact as the first, and any scaling for long contexts is a choice of
  * frequencies and amplitude.  Products and sums in fp32, one rounding.  With `inverse` the angles are negated: the gradient.
- * Queries, and keys if there are any, in one launch.  An output may be its input itself, with the same strides; otherwise nothing overlaps. */
+ * Queries, and keys if there are any, in one launch.  An output may be its input itself, with the same strides; otherwise nothing overlaps, the rows
+ * of an output among themselves included. */
 typedef struct {
   const void* query;          /* [tokens, heads, head_dim]                                                          */
   void* query_out;
@@ -406,7 +407,7 @@ AIDN_API int aidn_rotary(const aidn_rotary_args* args, void* cu_stream);
  * token_starts[b + 1] - 1, at most seq_len; rows of no sequence are left as they are.
  * States: sequence b begins with initial_state[s] (NULL, or s < 0: zeros) and leaves final_state[s], s = state_slots[b] or b.  final_state may be
  * initial_state itself.  A slot at or above num_slots, or one that an earlier sequence of the call has, gives rows of NaN and touches no state.
- * out overlaps nothing else. */
+ * out overlaps nothing else, and its rows do not overlap one another. */
 typedef struct {
   const void* q;                /* element (b,h,t,d) at b*stride[0] + h*stride[1] + t*stride[2] + d; packed rows: stride[0] unused */
   const void* k;
@@ -440,8 +441,8 @@ AIDN_API int aidn_linear_attention(const aidn_linear_args* args, void* cu_stream
 /* Its gradients, from the same argument block (out, final_state and o_stride are not looked at; state_slots must be NULL): dq, dk, dv in the type of
  * q, from those of out (dout, in that type) and of final_state (d_final_state, or NULL); d_initial_state (or NULL) receives those of
  * initial_state.  States are [batch, heads, key_dim, value_dim].  Gradients of shared heads are summed in fp32 in the heads' order and
- * rounded once; decay has none.  Rows behind a sequence's length are zeros, rows of no sequence are left.  Gradients overlap neither one another nor what the call
- * reads.  The workspace is needed where aidn_linear_attention_backward_workspace_bytes() says so and kv_heads < heads. */
+ * rounded once; decay has none.  Rows behind a sequence's length are zeros, rows of no sequence are left.  Gradients, and rows of one, overlap neither one another nor what the
+ * call reads.  The workspace is needed where aidn_linear_attention_backward_workspace_bytes() says so and kv_heads < heads. */
 typedef struct {
   aidn_linear_args fwd;
   const void* dout;
@@ -465,7 +466,8 @@ AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, vo
 AIDN_API int aidn_linear_attention_poll(void* cu_stream);
 
 /* One token of each of `batch` sequences against states that stay where they are: state state_slots[b] (NULL: b) is updated in place.  A
- * negative slot is a row of padding: its output is zeros and no state is touched.  Other slots as above.  One launch. */
+ * negative slot is a row of padding: its output is zeros and no state is touched.  Other slots as above.  out overlaps nothing else, and its rows do not
+ * overlap one another.  One launch. */
 typedef struct {
   const void* q;                /* [batch, heads, key_dim]                                                          */
   const void* k;                /* [batch, kv_heads, key_dim]                                                       */

@@ -229,3 +229,57 @@ def test_parts_keep_fast_pairs_and_divide_slow_ones():
 def test_frequencies_refuse(args):
     with pytest.raises(ValueError):
         rotary_frequencies(**args)
+
+
+# ---- outputs that overlap --------------------------------------------------------------------------------------------
+
+SPREAD = dict(q=4096, k=8192, v=12288, out=16384, batch=2, heads=4, kv_heads=4, seq_len=8, key_dim=64, value_dim=64, dtype=N.BF16)
+
+
+@pytest.mark.parametrize("change", [dict(query_out_stride=(128, 0)), dict(query_out_stride=(0, 64)), dict(query_out_stride=(127, 64)),
+                                    dict(query_out_stride=(64, 64)), dict(query_out=4096, query_stride=(64, 32), query_out_stride=(64, 32)),
+                                    dict(key=16384, kv_heads=2, key_out=8192), dict(key=8192, kv_heads=2, key_out=16384),
+                                    dict(key=16384, kv_heads=2, key_out=4096),
+                                    dict(key=16384, kv_heads=3, key_out=32768, key_out_stride=(160, 64))])
+def test_rotary_refuses_outputs_that_overlap(lib, change):
+    """(A token stride that leaves no room for its heads, a head stride below the head's size, one buffer for two outputs.)"""
+    with pytest.raises(N.AidnError) as e:
+        N.rotary(**{**ROTARY, **change})
+    assert "overlap" in str(e.value) and e.value.status == N.EINVAL
+
+
+@pytest.mark.parametrize("change", [dict(out=4096), dict(out=8192), dict(out=12288), dict(o_stride=(2048, 0, 64)), dict(o_stride=(2048, 512, 63)),
+                                    dict(o_stride=(511, 64, 256)), dict(o_stride=(64, 2048, 100)), dict(token_starts=256, tokens=9, o_stride=(0, 64, 192))])
+def test_linear_attention_refuses_an_output_that_overlaps(lib, change):
+    with pytest.raises(N.AidnError) as e:
+        N.linear_attention(N.linear_block(**{**SPREAD, **change}), 0)
+    assert "overlap" in str(e.value) and e.value.status == N.EINVAL
+
+
+@pytest.mark.parametrize("grads", [dict(dq=4096), dict(dk=8192), dict(dv=12288), dict(dv=20480), dict(dk=24576), dict(dv=28672), dict(dq=28672),
+                                   dict(dq_stride=(2048, 512, 0)), dict(dk_stride=(2048, 63, 256)), dict(dv_stride=(100, 64, 256))])
+def test_linear_attention_backward_refuses_gradients_that_overlap(lib, grads):
+    made = {**dict(dout=20480, dq=24576, dk=28672, dv=32768), **grads}
+    with pytest.raises(N.AidnError) as e:
+        N.linear_attention_backward(N.linear_bwd_block(N.linear_block(**SPREAD), **made), 0)
+    assert "overlap" in str(e.value) and e.value.status == N.EINVAL
+
+
+@pytest.mark.parametrize("change", [dict(out=4096), dict(o_stride=(255, 64)), dict(o_stride=(256, 60)), dict(o_stride=(64, 64))])
+def test_step_refuses_an_output_that_overlaps(lib, change):
+    with pytest.raises(N.AidnError) as e:
+        N.linear_attention_step(**{**STEP, **change})
+    assert "overlap" in str(e.value) and e.value.status == N.EINVAL
+
+
+def test_outputs_of_every_order_are_taken(lib):
+    """Strides in any order, and any distance where there is one row: what is left to refuse is that there is no device here (or nothing at all)."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are none")
+    for stride in ((2048, 512, 64), (2048, 64, 256), (64, 1024, 128), (0, 0, 0)):
+        with pytest.raises(N.AidnError) as e:
+            N.linear_attention(N.linear_block(**{**SPREAD, "o_stride": stride}), 0)
+        assert "overlap" not in str(e.value)
+    with pytest.raises(N.AidnError) as e:
+        N.linear_attention(N.linear_block(**{**SPREAD, "batch": 1, "seq_len": 1, "o_stride": (1, 64, 1)}), 0)
+    assert "overlap" not in str(e.value)
