@@ -1063,6 +1063,9 @@ bool is_one_of(const void* out, std::initializer_list<const void*> others) {
   return false;
 }
 
+constexpr int64_t kMostRows = 0x7fffff80;   // of a sequence: a whole number of chunks below 2^31
+constexpr int64_t kMostBytes = 1ll << 60;
+
 // The sizes and pointers that a forward and a backward call share.
 int linear_common(const char* op, const aidn_linear_args& a, aidn::lin::Params& p) {
   if (a.batch <= 0 || a.heads <= 0 || a.kv_heads <= 0) return fail(AIDN_EINVAL, "%s: batch, heads and kv_heads must be positive", op);
@@ -1079,13 +1082,19 @@ int linear_common(const char* op, const aidn_linear_args& a, aidn::lin::Params& 
   if ((uintptr_t)a.decay % 4 != 0 || (uintptr_t)a.lengths % 4 != 0 || (uintptr_t)a.token_starts % 4 != 0 || (uintptr_t)a.state_slots % 4 != 0)
     return fail(AIDN_EINVAL, "%s: decay, lengths, token_starts or state_slots is not aligned to its elements", op);
   if (a.state_slots && a.num_slots <= 0) return fail(AIDN_EINVAL, "%s: state_slots needs num_slots > 0", op);
+  // The most rows that a sequence can have: of packed rows, no more than there are, however large a bound seq_len is.  A segment's rows are counted in 32 bits.
+  int64_t longest = a.seq_len;
+  if (a.token_starts && longest > a.tokens) longest = a.tokens > 0 ? a.tokens : 1;
+  if (longest > kMostRows) return fail(AIDN_EINVAL, "%s: a sequence of %lld rows; seq_len and tokens may not both be above %lld", op, (long long)longest, (long long)kMostRows);
+  const int64_t rows = a.token_starts ? a.tokens : a.batch * a.seq_len, row_bytes = (int64_t)a.heads * (a.key_dim > a.value_dim ? a.key_dim : a.value_dim) * 4;
+  if (rows > kMostBytes / row_bytes) return fail(AIDN_EINVAL, "%s: sizes of more than 2^60 bytes", op);
   std::memset(&p, 0, sizeof(p));
   p.decay = a.decay;
   p.lengths = a.lengths;
   p.starts = a.token_starts;
   p.slots = a.state_slots;
   p.tokens = a.tokens;
-  p.seq_len = a.seq_len;
+  p.seq_len = longest;
   p.batch = a.batch;
   p.heads = a.heads;
   p.num_slots = a.state_slots ? a.num_slots : a.batch;
@@ -1366,7 +1375,7 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
     g.d[0] = (int)dk; g.d[1] = (int)dv;
     g.rows = rows;
     g.lengths = f.lengths; g.starts = f.token_starts;
-    g.tokens = f.tokens; g.seq_len = f.seq_len;
+    g.tokens = f.tokens; g.seq_len = p.seq_len;
     g.batch = f.batch; g.kv_heads = f.kv_heads; g.group = group; g.dtype = f.dtype;
     e = aidn::lin::launch_group_sum(g, stream);
   }

@@ -178,3 +178,27 @@ def test_far_positions_are_as_exact_as_near_ones(backend, base):
     a, b = x.double()[..., ::2], x.double()[..., 1::2]
     for got, ref in ((y[..., ::2], a * c - b * s), (y[..., 1::2], a * s + b * c)):
         assert bool(((got.double() - ref).abs() <= 2.0 ** -24 * ref.abs() + 2.0 ** -21 * (a.abs() + b.abs())).all())
+
+
+# ---- packed rows whose seq_len is a bound ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,key,value,heads", [("bf16", 64, 64, 4), ("f16", 128, 64, 2), ("f32", 40, 72, 4)])
+def test_a_bound_on_packed_sequences_changes_nothing(backend, dtype, key, value, heads):
+    """seq_len as large as it may be, against seq_len as long as there are rows: the same plan, and so the same bits; and no workspace for rows that are not there."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n, lens = 260, [0, 3, 200, 57]
+    q, k, v, do = ((torch.randn((n, h, d), generator=g, device="cuda") * 0.5).to(TORCH_DT[dtype]) for h, d in ((heads, key), (1, key), (1, value), (heads, value)))
+    starts = torch.tensor([sum(lens[:i]) for i in range(5)], dtype=torch.int32, device="cuda")
+    decay, got = torch.linspace(-0.2, -0.01, heads, device="cuda"), []
+    for seq in (n, 0x7fffffff):
+        block = N.linear_block(batch=4, heads=heads, kv_heads=1, seq_len=seq, key_dim=key, value_dim=value, dtype=N.BF16 if dtype == "bf16" else N.F16
+                               if dtype == "f16" else N.F32, token_starts=starts.data_ptr(), tokens=n)
+        outs = [torch.zeros_like(x) for x in (do, q, k, v)]
+        last = torch.zeros(4, heads, key, value, device="cuda")
+        ins, at = [GpuBuffer(x) for x in (q, k, v)], [GpuBuffer(x) for x in outs]
+        backend.LinearAttention(*ins, at[0], GpuBuffer(decay), 4, heads, 1, seq, key, value, tokenStarts=GpuBuffer(starts), finalStates=GpuBuffer(last))
+        backend.LinearAttentionBackward(GpuBuffer(do), *ins, *at[1:], GpuBuffer(decay), 4, heads, 1, seq, key, value, tokenStarts=GpuBuffer(starts))
+        got.append((N.linear_workspace_bytes(block), N.linear_workspace_bytes(N.linear_bwd_block(block)), *outs, last))
+    assert got[0][:2] == got[1][:2]
+    for a, b in zip(got[0][2:], got[1][2:]):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())

@@ -283,3 +283,25 @@ def test_outputs_of_every_order_are_taken(lib):
     with pytest.raises(N.AidnError) as e:
         N.linear_attention(N.linear_block(**{**SPREAD, "batch": 1, "seq_len": 1, "o_stride": (1, 64, 1)}), 0)
     assert "overlap" not in str(e.value)
+
+
+# ---- sizes at the ends -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("change", [dict(seq_len=0x7fffffff), dict(seq_len=0x7fffff81), dict(token_starts=4096, seq_len=0x7fffffff, tokens=0x7fffffff)])
+def test_sequences_that_are_too_long_for_a_count_of_rows(lib, change):
+    """What counts a segment's rows has 31 bits, whole chunks of them: a longer sequence would lose its last rows."""
+    small = dict(key_dim=8, value_dim=8, heads=1, kv_heads=1, batch=1)
+    for call in (lambda b: N.linear_attention(b, 0), N.linear_workspace_bytes):
+        with pytest.raises(N.AidnError) as e:
+            call(N.linear_block(**{**LINEAR, **small, **change}))
+        assert "rows" in str(e.value) and e.value.status == N.EINVAL
+
+
+def test_workspace_of_sizes_beyond_64_bits(lib):
+    """Bytes that 64 bits do not hold are refused, not wrapped around."""
+    huge = dict(batch=65535, heads=65535, kv_heads=1, seq_len=0x7fffff80, key_dim=256, value_dim=256)
+    with pytest.raises(N.AidnError) as e:
+        N.linear_workspace_bytes(N.linear_bwd_block(N.linear_block(**{**LINEAR, **huge})))
+    assert "2^60" in str(e.value)
+    block = N.linear_bwd_block(N.linear_block(**{**LINEAR, **dict(batch=1, heads=64, kv_heads=1, seq_len=1 << 20, key_dim=256, value_dim=128)}))
+    assert N.linear_workspace_bytes(block) >= (64 << 20) * (256 + 128) * 4
