@@ -735,7 +735,7 @@ class CudaBackend:
                     o_stride=stride(heads, valueDim), scale=float(scale), path=self._path)
         stream, ws, ws_bytes = self._linear_workspace(N.linear_block(**args), optional=True)
         N.linear_attention(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), stream)
-        self.launch_count += 1
+        self.launch_count += N.linear_last_launch_count()
 
     def LinearAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, gradQuery: GpuBuffer,
                                 gradKey: GpuBuffer, gradValue: GpuBuffer, decay: Optional[GpuBuffer], batch: int, heads: int, kvHeads: int,
@@ -763,7 +763,7 @@ class CudaBackend:
         # (without shared heads it only holds the states of segments, and sequences are not cut without it)
         stream, ws, ws_bytes = self._linear_workspace(N.linear_bwd_block(N.linear_block(**args), **grads), optional=heads == kvHeads)
         N.linear_attention_backward(N.linear_bwd_block(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), **grads), stream)
-        self.launch_count += 1
+        self.launch_count += N.linear_last_launch_count()
 
     def LinearAttentionStep(self, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, output: GpuBuffer, states: GpuBuffer,
                             decay: Optional[GpuBuffer], batch: int, heads: int, kvHeads: int, keyDim: int, valueDim: int, scale: float = 0.0,

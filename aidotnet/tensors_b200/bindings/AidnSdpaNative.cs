@@ -206,6 +206,7 @@ namespace AiDotNet.Tensors.Engines.DirectGpu.CUDA
         [DllImport(Lib)] public static extern long aidn_linear_attention_backward_workspace_bytes(ref AidnLinearBwdArgs args);
         [DllImport(Lib)] public static extern int aidn_linear_attention_backward(ref AidnLinearBwdArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern int aidn_linear_attention_poll(IntPtr cuStream);
+        [DllImport(Lib)] public static extern int aidn_linear_attention_last_launch_count();
         [DllImport(Lib)] public static extern int aidn_linear_attention_step(ref AidnLinearStepArgs args, IntPtr cuStream);
         [DllImport(Lib)] public static extern long aidn_sdpa_backward_workspace_bytes(IntPtr handle, long batch, long seqQ);
         [DllImport(Lib)] public static extern int aidn_sdpa_backward(IntPtr handle, ref AidnSdpaBwdArgs args, IntPtr cuStream);

@@ -23,6 +23,7 @@ namespace {
 
 thread_local char g_err[512] = "";
 thread_local bool g_expire_linear = false;   // the same for aidn_linear_attention and its backward
+thread_local int g_linear_launches = 0;      // of this thread's last aidn_linear_attention or its backward
 thread_local bool g_expire_qkv = false;   // test hook: this thread's next aidn_qkv_rope_cache lets its bounded waits run out
 
 int fail(int code, const char* fmt, ...) {
@@ -1120,10 +1121,10 @@ bool linear_rows_meet(const aidn_linear_args& a, int64_t heads, int64_t size, co
 cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int sms, char* work, int64_t work_bytes, cudaStream_t stream, bool* waits) {
   const bool expire = g_expire_linear;
   g_expire_linear = false;
-  int launches = 0;
+  g_linear_launches = 0;
   *waits = a.path != AIDN_PATH_GENERIC && aidn::lin::scan_sm100_supported(p);
-  return *waits ? aidn::lin::launch_scan_sm100(p, sms, reinterpret_cast<float*>(work), work_bytes, expire, stream, &launches)
-                : aidn::lin::launch_scan_generic(p, sms, reinterpret_cast<float*>(work), work_bytes, stream, &launches);
+  return *waits ? aidn::lin::launch_scan_sm100(p, sms, reinterpret_cast<float*>(work), work_bytes, expire, stream, &g_linear_launches)
+                : aidn::lin::launch_scan_generic(p, sms, reinterpret_cast<float*>(work), work_bytes, stream, &g_linear_launches);
 }
 // Waits for `stream` and reports a wait given up in its context that was not yet reported for this stream.  What each stream was told is kept here, and
 // only where there was something to tell; a stream's id is never another one's, its handle may be.
@@ -1378,10 +1379,13 @@ int aidn_linear_attention_backward(const aidn_linear_bwd_args* a, void* cu_strea
     g.tokens = f.tokens; g.seq_len = p.seq_len;
     g.batch = f.batch; g.kv_heads = f.kv_heads; g.group = group; g.dtype = f.dtype;
     e = aidn::lin::launch_group_sum(g, stream);
+    if (e == cudaSuccess) ++g_linear_launches;
   }
   if (e != cudaSuccess) return fail_cuda(e, "linear_attention_backward");
   return linear_check("aidn_linear_attention_backward", stream, waits);
 }
+
+int aidn_linear_attention_last_launch_count(void) { return g_linear_launches; }
 
 int aidn_linear_attention_poll(void* cu_stream) {
   g_err[0] = 0;

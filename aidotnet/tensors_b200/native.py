@@ -38,6 +38,7 @@ EXPORTS = (
     "aidn_kv8_append", "aidn_sdpa_kv8_workspace_bytes", "aidn_sdpa_launch_kv8",
     "aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_workspace_bytes", "aidn_linear_attention_backward",
     "aidn_linear_attention_backward_workspace_bytes", "aidn_linear_attention_poll", "aidn_linear_attention_step",
+    "aidn_linear_attention_last_launch_count",
     "aidn_sdpa_debug_set",   # include/aidn_sdpa_debug.h
 )
 
@@ -270,6 +271,8 @@ def load() -> ctypes.CDLL:
     lib.aidn_linear_attention_backward.argtypes = [ctypes.POINTER(LinearBwdArgs), ctypes.c_void_p]
     lib.aidn_linear_attention_step.argtypes = [ctypes.POINTER(LinearStepArgs), ctypes.c_void_p]
     lib.aidn_linear_attention_poll.argtypes = [ctypes.c_void_p]
+    lib.aidn_linear_attention_last_launch_count.argtypes = []
+    lib.aidn_linear_attention_last_launch_count.restype = ctypes.c_int
     for name in ("aidn_rotary", "aidn_linear_attention", "aidn_linear_attention_backward", "aidn_linear_attention_step",
                  "aidn_linear_attention_poll"):
         getattr(lib, name).restype = ctypes.c_int
@@ -687,6 +690,11 @@ def linear_attention_step(*, q: int, k: int, v: int, out: int, states: int, batc
         kv_heads, key_dim, value_dim, dtype, num_slots, scale), stream)
     if status != OK:
         raise AidnError(status, last_error())
+
+
+def linear_last_launch_count() -> int:
+    """Kernels that this thread's last ``linear_attention`` or ``linear_attention_backward`` enqueued."""
+    return int((_lib or load()).aidn_linear_attention_last_launch_count())
 
 
 def linear_attention_poll(stream: int) -> None:

@@ -465,6 +465,9 @@ AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, vo
  * the calls since a stream's report before are then not to be used, as any of them may be the one. */
 AIDN_API int aidn_linear_attention_poll(void* cu_stream);
 
+/* Kernels that the calling thread's last aidn_linear_attention or aidn_linear_attention_backward enqueued. */
+AIDN_API int aidn_linear_attention_last_launch_count(void);
+
 /* One token of each of `batch` sequences against states that stay where they are: state state_slots[b] (NULL: b) is updated in place.  A
  * negative slot is a row of padding: its output is zeros and no state is touched.  Other slots as above.  out overlaps nothing else, and its rows do not
  * overlap one another.  One launch. */

@@ -202,3 +202,29 @@ def test_a_bound_on_packed_sequences_changes_nothing(backend, dtype, key, value,
     assert got[0][:2] == got[1][:2]
     for a, b in zip(got[0][2:], got[1][2:]):
         assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+# ---- what a backend counts and passes on -----------------------------------------------------------------------------
+
+def prompt(backend, dtype, n, heads, kv, key, value, backward=False):
+    """A prompt of one sequence, or its gradients; kernels by the backend's count."""
+    make = lambda h, d: GpuBuffer((torch.randn(1, h, n, d, device="cuda") * 0.5).to(TORCH_DT[dtype]))  # noqa: E731
+    q, k, v, o = make(heads, key), make(kv, key), make(kv, value), make(heads, value)
+    before = backend.launch_count
+    if backward:
+        backend.LinearAttentionBackward(o, q, k, v, make(heads, key), make(kv, key), make(kv, value), None, 1, heads, kv, n, key, value)
+    else:
+        backend.LinearAttention(q, k, v, o, None, 1, heads, kv, n, key, value)
+    return backend.launch_count - before
+
+
+@pytest.mark.parametrize("args,forward,backward", [
+    (("bf16", 100, 4, 4, 64, 64), 1, 1),      # the scans
+    (("bf16", 100, 4, 2, 64, 64), 1, 2),      # and the sums of shared heads
+    (("bf16", 100, 4, 2, 64, 128), 1, 3),     # scans of two sizes are two launches
+    (("bf16", 4096, 1, 1, 128, 128), 3, 3),   # in segments: what each adds, the states before them, the scans
+    (("f32", 4096, 2, 1, 40, 72), 3, 4),
+    (("f32", 20, 2, 2, 40, 72), 1, 1)])
+def test_launch_count_is_what_ran(backend, args, forward, backward):
+    assert prompt(backend, *args) == forward
+    assert prompt(backend, *args, backward=True) == backward
