@@ -136,6 +136,7 @@ class CudaBackend:
         torch.cuda.set_device(device)
         self._stream = stream
         self._path = path
+        self._linear_path = path if path == N.PATH_GENERIC else N.PATH_AUTO   # (the other paths are kernels of softmax attention)
         self._decode_chunk = decode_chunk
         self._handles: Dict[Tuple, N.Handle] = {}
         self._scratch: Dict[int, torch.Tensor] = {}   # by stream: calls on different streams may overlap
@@ -732,7 +733,7 @@ class CudaBackend:
                     decay=_address(decay), lengths=_address(lengths), token_starts=_address(tokenStarts), tokens=tokens,
                     initial_state=_address(initialStates), final_state=_address(finalStates), state_slots=_address(stateSlots), num_slots=slots,
                     q_stride=stride(heads, keyDim), k_stride=stride(kvHeads, keyDim), v_stride=stride(kvHeads, valueDim),
-                    o_stride=stride(heads, valueDim), scale=float(scale), path=self._path)
+                    o_stride=stride(heads, valueDim), scale=float(scale), path=self._linear_path)
         stream, ws, ws_bytes = self._linear_workspace(N.linear_block(**args), optional=True)
         N.linear_attention(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), stream)
         self.launch_count += N.linear_last_launch_count()
@@ -756,7 +757,7 @@ class CudaBackend:
         args = dict(q=query.tensor.data_ptr(), k=key.tensor.data_ptr(), v=value.tensor.data_ptr(), batch=batch, heads=heads, kv_heads=kvHeads,
                     seq_len=seqLen, key_dim=keyDim, value_dim=valueDim, dtype=dtype, decay=_address(decay), lengths=_address(lengths),
                     token_starts=_address(tokenStarts), tokens=tokens, initial_state=_address(initialStates), q_stride=qs, k_stride=ks,
-                    v_stride=vs, scale=float(scale), path=self._path)
+                    v_stride=vs, scale=float(scale), path=self._linear_path)
         grads = dict(dout=gradOutput.tensor.data_ptr(), dq=gradQuery.tensor.data_ptr(), dk=gradKey.tensor.data_ptr(),
                      dv=gradValue.tensor.data_ptr(), d_final_state=_address(gradFinalStates), d_initial_state=_address(gradInitialStates),
                      do_stride=os, dq_stride=qs, dk_stride=ks, dv_stride=vs)

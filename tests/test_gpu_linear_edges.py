@@ -228,3 +228,17 @@ def prompt(backend, dtype, n, heads, kv, key, value, backward=False):
 def test_launch_count_is_what_ran(backend, args, forward, backward):
     assert prompt(backend, *args) == forward
     assert prompt(backend, *args, backward=True) == backward
+
+
+@pytest.mark.parametrize("path", [N.PATH_AUTO, N.PATH_GENERIC, N.PATH_DECODE, N.PATH_PREFILL_SM100])
+def test_a_forced_attention_path_is_no_path_of_linear_attention(path):
+    """A backend may be held to one kernel of softmax attention; linear attention has two paths, and heeds GENERIC."""
+    own = CudaBackend(path=path)
+    q, k, v = ((torch.randn(1, 2, 90, 64, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda") * 0.5).bfloat16() for i in range(3))
+    outs = []
+    for b in (own, CudaBackend(path=N.PATH_GENERIC if path == N.PATH_GENERIC else N.PATH_AUTO)):
+        out, grads = torch.empty_like(q), [torch.empty_like(q) for _ in range(3)]
+        b.LinearAttention(*(GpuBuffer(x) for x in (q, k, v, out)), None, 1, 2, 2, 90, 64, 64)
+        b.LinearAttentionBackward(*(GpuBuffer(x) for x in (out, q, k, v, *grads)), None, 1, 2, 2, 90, 64, 64)
+        outs.append((out, *grads))
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(*outs))
