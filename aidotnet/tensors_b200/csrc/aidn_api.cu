@@ -3,6 +3,7 @@
 // of this build can serve is an error.
 #include <dlfcn.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -1010,9 +1011,10 @@ int aidn_sdpa_launch_kv8(aidn_sdpa_t h, const aidn_sdpa_args* a, const aidn_kv8_
 
 // ---- rotary positions, linear attention ------------------------------------------------------------------------------
 namespace {
-// What a device is, looked up once (handle-less entry points have nowhere else to keep it; racing threads write the same values).
+// What a device is, looked up once (handle-less entry points have nowhere else to keep it): its SMs, negative where it is not served.  One value, so that a
+// thread sees all of it or nothing; racing threads write the same.
 int device_facts(const char* op, int* sms) {
-  static int g_sms[64] = {0}, g_ok[64] = {0};
+  static std::atomic<int> facts[64];
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) {
@@ -1020,15 +1022,15 @@ int device_facts(const char* op, int* sms) {
     return fail_cuda(e, op);
   }
   if (dev < 0 || dev >= 64) return fail(AIDN_EUNSUPPORTED, "%s: device ordinal %d", op, dev);
-  if (g_sms[dev] == 0) {
-    int n = 0;
+  int n = facts[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return fail_cuda(e, op);
-    g_ok[dev] = aidn_sdpa_device_supported(dev);
-    g_sms[dev] = n;
+    if (!aidn_sdpa_device_supported(dev)) n = -n;
+    facts[dev].store(n, std::memory_order_relaxed);
   }
-  if (!g_ok[dev]) return fail(AIDN_EUNSUPPORTED, "%s: device %d is not compute capability 10.x", op, dev);
-  *sms = g_sms[dev];
+  if (n < 0) return fail(AIDN_EUNSUPPORTED, "%s: device %d is not compute capability 10.x", op, dev);
+  *sms = n;
   return AIDN_OK;
 }
 

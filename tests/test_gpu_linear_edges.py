@@ -242,3 +242,39 @@ def test_a_forced_attention_path_is_no_path_of_linear_attention(path):
         b.LinearAttentionBackward(*(GpuBuffer(x) for x in (out, q, k, v, *grads)), None, 1, 2, 2, 90, 64, 64)
         outs.append((out, *grads))
     assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(*outs))
+
+
+_THREADS = """
+import threading
+import torch
+from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
+backends = [CudaBackend(stream=torch.cuda.Stream()) for _ in range(16)]
+x = [[(torch.randn(3, 2, 64, device="cuda") * 0.5).bfloat16() for _ in range(4)] for _ in backends]
+states = [torch.zeros(3, 2, 64, 64, device="cuda") for _ in backends]
+torch.cuda.synchronize()
+gate, failed = threading.Barrier(len(backends)), []
+
+def first(i):
+    gate.wait()
+    try:
+        backends[i].LinearAttentionStep(*(GpuBuffer(t) for t in x[i]), GpuBuffer(states[i]), None, 3, 2, 2, 64, 64)
+    except Exception as e:
+        failed.append(e)
+
+threads = [threading.Thread(target=first, args=(i,)) for i in range(len(backends))]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert not failed, failed
+for (q, k, v, out), s in zip(x, states):
+    assert torch.equal(s, k.float()[..., None] * v.float()[..., None, :])
+print("threads ok")
+"""
+
+
+def test_first_calls_of_many_threads():
+    """Calls without a handle learn what the device is when the first of them runs: sixteen first calls at once, in a process of their own."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", _THREADS], capture_output=True, text=True, timeout=300, env=dict(os.environ, PYTHONPATH=root), cwd=root)
+        assert r.returncode == 0 and "threads ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
