@@ -659,7 +659,7 @@ class CudaBackend:
             self.launch_count += 1
 
     def _linear_checks(self, op, tensors, batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts, decay, states,
-                       stateSlots):
+                       stateSlots, tokens):
         """``tensors``: (name, buffer, heads, size).  Returns the number of packed rows, of states, and the strides by (heads, size)."""
         if batch <= 0 or heads <= 0 or kvHeads <= 0 or seqLen <= 0 or keyDim <= 0 or valueDim <= 0:
             raise ValueError(f"{op}: dimensions must be positive")
@@ -675,7 +675,10 @@ class CudaBackend:
         dtype = tensors[0][1].tensor.dtype
         if dtype not in _DTYPE:
             raise ValueError(f"{op}: {dtype} is not served")
-        tokens = 0 if tokenStarts is None else tensors[0][1].tensor.numel() // (tensors[0][2] * tensors[0][3])
+        if tokens < 0 or (tokens > 0 and tokenStarts is None):
+            raise ValueError(f"{op}: tokens must be >= 0, and belongs to tokenStarts")
+        if tokenStarts is not None and tokens == 0:
+            tokens = tensors[0][1].tensor.numel() // (tensors[0][2] * tensors[0][3])
         rows = batch * seqLen if tokenStarts is None else tokens
         for name, buf, h, size in tensors:
             if buf.tensor.dtype != dtype:
@@ -713,13 +716,14 @@ class CudaBackend:
                         heads: int, kvHeads: int, seqLen: int, keyDim: int, valueDim: int, scale: float = 0.0, tokenMajor: bool = False,
                         lengths: Optional[GpuBuffer] = None, tokenStarts: Optional[GpuBuffer] = None,
                         initialStates: Optional[GpuBuffer] = None, finalStates: Optional[GpuBuffer] = None,
-                        stateSlots: Optional[GpuBuffer] = None) -> None:
+                        stateSlots: Optional[GpuBuffer] = None, tokens: int = 0) -> None:
         """Linear attention of whole sequences: S_t = exp(decay) S_(t-1) + k_t v_t^T, o_t = scale * q_t S_t (scale 0: 1/sqrt(keyDim)) with
         the head's log ``decay`` [heads] fp32, at most 0 (None: no decay).  ``query`` [batch, heads, seqLen, keyDim], ``key`` and
         ``value`` [batch, kvHeads, seqLen, ..], ``output`` [batch, heads, seqLen, valueDim]; ``tokenMajor``: [batch, seqLen, heads, ..].
         ``output`` is none of the inputs.
         ``lengths`` int32 [batch]: the rows behind them are padding, and zeros in ``output``.  ``tokenStarts`` int32 [batch + 1]: packed
-        rows [tokens, heads, ..] instead, sequence b's from tokenStarts[b] on, at most seqLen of them; rows of no sequence are left.
+        rows [tokens, heads, ..] instead, sequence b's from tokenStarts[b] on, at most seqLen of them; rows of no sequence are left.  ``tokens``: how
+        many packed rows there are, for buffers with room behind them (0: as many as ``query`` holds).
         Sequence b begins with state stateSlots[b] (or b) of ``initialStates`` [.., heads, keyDim, valueDim] fp32 (None or a negative
         slot: zeros) and leaves its last in ``finalStates``, which may be the same buffer.  A slot that is not there, or an earlier
         sequence's, gives NaN and touches no state."""
@@ -727,7 +731,7 @@ class CudaBackend:
         tokens, slots, dtype, stride = self._linear_checks(
             op, (("query", query, heads, keyDim), ("key", key, kvHeads, keyDim), ("value", value, kvHeads, valueDim),
                  ("output", output, heads, valueDim)), batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts, decay,
-            (("initialStates", initialStates), ("finalStates", finalStates)), stateSlots)
+            (("initialStates", initialStates), ("finalStates", finalStates)), stateSlots, tokens)
         args = dict(q=query.tensor.data_ptr(), k=key.tensor.data_ptr(), v=value.tensor.data_ptr(), out=output.tensor.data_ptr(), batch=batch,
                     heads=heads, kv_heads=kvHeads, seq_len=seqLen, key_dim=keyDim, value_dim=valueDim, dtype=dtype,
                     decay=_address(decay), lengths=_address(lengths), token_starts=_address(tokenStarts), tokens=tokens,
@@ -743,7 +747,7 @@ class CudaBackend:
                                 seqLen: int, keyDim: int, valueDim: int, scale: float = 0.0, tokenMajor: bool = False,
                                 lengths: Optional[GpuBuffer] = None, tokenStarts: Optional[GpuBuffer] = None,
                                 initialStates: Optional[GpuBuffer] = None, gradFinalStates: Optional[GpuBuffer] = None,
-                                gradInitialStates: Optional[GpuBuffer] = None) -> None:
+                                gradInitialStates: Optional[GpuBuffer] = None, tokens: int = 0) -> None:
         """The gradients of ``LinearAttention``'s query, key, value and initial states (all by sequence, [batch, heads, keyDim, valueDim]) from
         those of its output and of its final states.  Gradients have the inputs' dtype and layout; those of shared heads are summed in
         fp32.  decay has none."""
@@ -752,7 +756,7 @@ class CudaBackend:
             op, (("query", query, heads, keyDim), ("key", key, kvHeads, keyDim), ("value", value, kvHeads, valueDim),
                  ("gradOutput", gradOutput, heads, valueDim), ("gradQuery", gradQuery, heads, keyDim), ("gradKey", gradKey, kvHeads, keyDim),
                  ("gradValue", gradValue, kvHeads, valueDim)), batch, heads, kvHeads, seqLen, keyDim, valueDim, tokenMajor, lengths, tokenStarts,
-            decay, (("initialStates", initialStates), ("gradFinalStates", gradFinalStates), ("gradInitialStates", gradInitialStates)), None)
+            decay, (("initialStates", initialStates), ("gradFinalStates", gradFinalStates), ("gradInitialStates", gradInitialStates)), None, tokens)
         qs, ks, os, vs = stride(heads, keyDim), stride(kvHeads, keyDim), stride(heads, valueDim), stride(kvHeads, valueDim)
         args = dict(q=query.tensor.data_ptr(), k=key.tensor.data_ptr(), v=value.tensor.data_ptr(), batch=batch, heads=heads, kv_heads=kvHeads,
                     seq_len=seqLen, key_dim=keyDim, value_dim=valueDim, dtype=dtype, decay=_address(decay), lengths=_address(lengths),

@@ -278,3 +278,30 @@ def test_first_calls_of_many_threads():
     for _ in range(3):
         r = subprocess.run([sys.executable, "-c", _THREADS], capture_output=True, text=True, timeout=300, env=dict(os.environ, PYTHONPATH=root), cwd=root)
         assert r.returncode == 0 and "threads ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
+
+
+# ---- packed rows in buffers with room to spare -----------------------------------------------------------------------
+
+def test_packed_rows_in_larger_buffers(backend):
+    """A query buffer kept for more rows than this batch has, beside keys and values that are just large enough."""
+    n, lens, starts = 90, (40, 50), torch.tensor([0, 40, 90], dtype=torch.int32, device="cuda")
+    make = lambda rows, h: (torch.randn(rows, h, 64, generator=torch.Generator(device="cuda").manual_seed(rows + h), device="cuda") * 0.5).bfloat16()  # noqa: E731
+    q, k, v, do = make(128, 4), make(n, 2), make(n, 2) + 1, make(128, 4) - 1
+    sizes = (2, 4, 2, max(lens), 64, 64)
+    got = []
+    for roomy in (True, False):
+        qq, dd = (q, do) if roomy else (q[:n].contiguous(), do[:n].contiguous())
+        out, grads = torch.full_like(qq, 7.0), [torch.full_like(x, 7.0) for x in (qq, k, v)]
+        kw = dict(tokenStarts=GpuBuffer(starts), **(dict(tokens=n) if roomy else {}))
+        backend.LinearAttention(*(GpuBuffer(x) for x in (qq, k, v, out)), None, *sizes, **kw)
+        backend.LinearAttentionBackward(*(GpuBuffer(x) for x in (dd, qq, k, v, *grads)), None, *sizes, **kw)
+        assert all(bool((x[n:] == 7.0).all()) for x in (out, *grads))
+        got.append([x[:n] for x in (out, *grads)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    bufs = [GpuBuffer(x) for x in (q, k, v, torch.empty_like(q))]
+    for change in (dict(tokens=91, tokenStarts=GpuBuffer(starts)), dict(tokens=-1, tokenStarts=GpuBuffer(starts)), dict(tokens=5), dict(tokenStarts=GpuBuffer(starts))):
+        with pytest.raises(ValueError, match="tokens must be|key is smaller"):
+            backend.LinearAttention(*bufs, None, *sizes, **change)
+    for change in (dict(tokens=91, tokenStarts=GpuBuffer(starts)), dict(tokens=5)):
+        with pytest.raises(ValueError, match="tokens must be|key is smaller"):
+            backend.LinearAttentionBackward(GpuBuffer(do), *bufs[:3], *(GpuBuffer(torch.empty_like(x)) for x in (q, k, v)), None, *sizes, **change)
