@@ -26,6 +26,7 @@ import math
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
+from torch import _C
 
 from . import native as N
 
@@ -153,6 +154,13 @@ class CudaBackend:
     def _raw_stream(self) -> int:
         """``stream.cuda_stream`` without the stream object."""
         return self._stream.cuda_stream if self._stream is not None else torch._C._cuda_getCurrentRawStream(self.device)
+
+    def _here(self, call, *args):
+        """A call without a handle, which runs on the current device: on this backend's."""
+        if _C._cuda_getDevice() == self.device:
+            return call(*args)
+        with torch.cuda.device(self.device):
+            return call(*args)
 
     def AllocateBuffer(self, size: int, dtype: torch.dtype = torch.float32) -> GpuBuffer:
         return GpuBuffer(torch.empty(int(size), dtype=dtype, device=self._torch_device))
@@ -626,7 +634,7 @@ class CudaBackend:
         f = frequencies.tensor
         if f.dtype != torch.float64:
             raise ValueError(f"{op}: frequencies must be a buffer of 64-bit floats")
-        x, dtype, spans, pointers = query.tensor, query.tensor.dtype, [], []
+        dtype, device, spans, pointers = query.tensor.dtype, self.device, [], []
         for name, src, dst, h, stride in (("query", query, queryOut, heads, queryStride), ("key", key, keyOut, kvHeads, keyStride)):
             if src is None:
                 spans.append((0, 0, 0, 0))
@@ -637,22 +645,31 @@ class CudaBackend:
                 raise ValueError(f"{op}: a stride of {name} is negative")
             reach = (tokens - 1) * row + (h - 1) * step + headDim if tokens > 0 else 0
             at, to = src.tensor, dst.tensor
-            same = at.data_ptr() == to.data_ptr()
+            fromAt, toAt = at.data_ptr(), to.data_ptr()
+            same = fromAt == toAt
             if at.dtype != dtype or to.dtype != dtype:
                 raise ValueError(f"{op}: queries and keys, in and out, must share a dtype")
+            if at.get_device() != device or to.get_device() != device:
+                raise ValueError(f"{op}: {name} must be on the backend's device")
             if at.numel() < reach or (not same and to.numel() < tokens * h * headDim):
                 raise ValueError(f"{op}: a buffer of {name} is smaller than [tokens, heads, headDim]")
             spans.append((row, step) + ((row, step) if same else (h * headDim, headDim)))
-            pointers += [at.data_ptr(), to.data_ptr()]
+            pointers += [fromAt, toAt]
         at, width = 0, 4
         if positions is not None:
-            if positions.tensor.dtype not in (torch.int32, torch.int64) or positions.tensor.numel() < tokens:
-                raise ValueError(f"{op}: positions must be int32 or int64 [tokens]")
-            at, width = positions.tensor.data_ptr(), positions.tensor.element_size()
+            to = positions.tensor
+            if to.dtype not in (torch.int32, torch.int64) or to.numel() < tokens or to.get_device() != device:
+                raise ValueError(f"{op}: positions must be int32 or int64 [tokens], on the backend's device")
+            at, width = to.data_ptr(), to.element_size()
+        if f.get_device() != device:
+            raise ValueError(f"{op}: frequencies must be on the backend's device")
         (qr, qh, qor, qoh), (kr, kh, kor, koh) = spans
-        status = N._rotary_packed(N._ROTARY_ARGS.pack(
-            *pointers, qr, qh, qor, qoh, kr, kh, kor, koh, f.data_ptr(), at, tokens, seqLen, startPosition, heads, kvHeads, headDim,
-            2 * f.numel(), _DTYPE[dtype], N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES, width, inverse, amplitude, 0), self._raw_stream)
+        block = N._ROTARY_ARGS.pack(*pointers, qr, qh, qor, qoh, kr, kh, kor, koh, f.data_ptr(), at, tokens, seqLen, startPosition, heads, kvHeads,
+                                    headDim, 2 * f.numel(), _DTYPE[dtype], N.ROPE_INTERLEAVED if interleaved else N.ROPE_HALVES, width, inverse,
+                                    amplitude, 0)
+        # (as in LinearAttentionStep)
+        stream = _C._cuda_getCurrentRawStream(device) if self._stream is None else self._stream.cuda_stream
+        status = N._rotary_packed(block, stream) if _C._cuda_getDevice() == device else self._here(N._rotary_packed, block, stream)
         if status != N.OK:
             raise N.AidnError(status, N.last_error())
         if tokens > 0:
@@ -689,6 +706,9 @@ class CudaBackend:
         given = [s for _, s in states if s is not None]
         if stateSlots is not None and given:
             slots = min(s.tensor.numel() for s in given) // per
+        for buf in (*(t[1] for t in tensors), lengths, tokenStarts, decay, stateSlots, *given):
+            if buf is not None and buf.tensor.get_device() != self.device:
+                raise ValueError(f"{op}: all buffers must be on the backend's device")
         for name, buf in states:
             if buf is not None and (buf.tensor.dtype != torch.float32 or buf.tensor.numel() < max(slots, 1) * per):
                 raise ValueError(f"{op}: {name} must hold fp32 states [.., heads, keyDim, valueDim]")
@@ -702,7 +722,7 @@ class CudaBackend:
 
     def _linear_workspace(self, block, optional):
         """(stream, address, bytes) of a call's workspace."""
-        need = N.linear_workspace_bytes(block)
+        need = self._here(N.linear_workspace_bytes, block)
         stream = self._raw_stream
         if need <= 0:
             return stream, 0, 0
@@ -739,7 +759,7 @@ class CudaBackend:
                     q_stride=stride(heads, keyDim), k_stride=stride(kvHeads, keyDim), v_stride=stride(kvHeads, valueDim),
                     o_stride=stride(heads, valueDim), scale=float(scale), path=self._linear_path)
         stream, ws, ws_bytes = self._linear_workspace(N.linear_block(**args), optional=True)
-        N.linear_attention(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), stream)
+        self._here(N.linear_attention, N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), stream)
         self.launch_count += N.linear_last_launch_count()
 
     def LinearAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, gradQuery: GpuBuffer,
@@ -767,7 +787,7 @@ class CudaBackend:
                      do_stride=os, dq_stride=qs, dk_stride=ks, dv_stride=vs)
         # (without shared heads it only holds the states of segments, and sequences are not cut without it)
         stream, ws, ws_bytes = self._linear_workspace(N.linear_bwd_block(N.linear_block(**args), **grads), optional=heads == kvHeads)
-        N.linear_attention_backward(N.linear_bwd_block(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), **grads), stream)
+        self._here(N.linear_attention_backward, N.linear_bwd_block(N.linear_block(workspace=ws, workspace_bytes=ws_bytes, **args), **grads), stream)
         self.launch_count += N.linear_last_launch_count()
 
     def LinearAttentionStep(self, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer, output: GpuBuffer, states: GpuBuffer,
@@ -792,14 +812,25 @@ class CudaBackend:
         slots = s.numel() // (heads * keyDim * valueDim)
         if s.dtype != torch.float32 or slots < (batch if stateSlots is None else 1):
             raise ValueError(f"{op}: states must hold fp32 states [.., heads, keyDim, valueDim]")
-        if stateSlots is not None and (stateSlots.tensor.dtype != torch.int32 or stateSlots.tensor.numel() < batch):
-            raise ValueError(f"{op}: stateSlots must be int32 [batch]")
-        if decay is not None and (decay.tensor.dtype != torch.float32 or decay.tensor.numel() < heads):
-            raise ValueError(f"{op}: decay must hold an fp32 value for each head")
-        status = N._linear_step_packed(N._LINEAR_STEP_ARGS.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), s.data_ptr(), 0 if decay is None else decay.tensor.data_ptr(),
-            0 if stateSlots is None else stateSlots.tensor.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, batch, heads, kvHeads, keyDim, valueDim,
-            _DTYPE[dtype], slots, float(scale)), self._raw_stream)
+        device = self.device
+        if q.get_device() != device or k.get_device() != device or v.get_device() != device or o.get_device() != device or s.get_device() != device:
+            raise ValueError(f"{op}: all buffers must be on the backend's device")
+        decayAt = slotsAt = 0
+        if decay is not None:
+            g = decay.tensor
+            if g.dtype != torch.float32 or g.numel() < heads or g.get_device() != device:
+                raise ValueError(f"{op}: decay must hold an fp32 value for each head, on the backend's device")
+            decayAt = g.data_ptr()
+        if stateSlots is not None:
+            at = stateSlots.tensor
+            if at.dtype != torch.int32 or at.numel() < batch or at.get_device() != device:
+                raise ValueError(f"{op}: stateSlots must be int32 [batch], on the backend's device")
+            slotsAt = at.data_ptr()
+        block = N._LINEAR_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), s.data_ptr(), decayAt, slotsAt, 0, 0, 0, 0, 0, 0, 0, 0,
+                                         batch, heads, kvHeads, keyDim, valueDim, _DTYPE[dtype], slots, scale)
+        # (_here and _raw_stream, without their calls: this code is as long as a small step's kernel)
+        stream = _C._cuda_getCurrentRawStream(device) if self._stream is None else self._stream.cuda_stream
+        status = N._linear_step_packed(block, stream) if _C._cuda_getDevice() == device else self._here(N._linear_step_packed, block, stream)
         if status != N.OK:
             raise N.AidnError(status, N.last_error())
         if batch > 0:
@@ -808,7 +839,7 @@ class CudaBackend:
     def LinearAttentionPoll(self) -> None:
         """Waits for this backend's stream and raises if a ``LinearAttention`` or ``LinearAttentionBackward`` of its device gave up a bounded wait since this
         stream was last told (none does in normal operation): what they wrote since then is not to be used."""
-        N.linear_attention_poll(self._raw_stream)
+        self._here(N.linear_attention_poll, self._raw_stream)
 
     def FlashAttentionBackward(self, gradOutput: GpuBuffer, query: GpuBuffer, key: GpuBuffer, value: GpuBuffer,
                                output: GpuBuffer, softmaxStats: GpuBuffer, gradQuery: GpuBuffer, gradKey: GpuBuffer,

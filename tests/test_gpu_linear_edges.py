@@ -204,6 +204,25 @@ def test_a_bound_on_packed_sequences_changes_nothing(backend, dtype, key, value,
         assert torch.equal(a, b) and bool(torch.isfinite(a).all())
 
 
+@pytest.mark.parametrize("part", [128, 32])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("seed", [0, 1])
+def test_fp16_results_below_its_normal_numbers(backend, part, interleaved, seed):
+    """Rows of a packed projection.  test_gpu_rotary's bound, and fp16's own: below 2^-14 its numbers are 2^-24 apart, and a rounding is off by 2^-25."""
+    x = torch.randn(19, 12, 128, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    x = (x * 2.0 ** -torch.arange(19, device="cuda")[:, None, None]).half()   # rows of ever smaller values
+    out, f = torch.empty(19, 10, 128, dtype=x.dtype, device="cuda"), backend.RotaryFrequencies(part)
+    backend.RotaryEmbedding(GpuBuffer(x), GpuBuffer(out), None, None, f, 19, 10, 0, 128, interleaved=interleaved, queryStride=(12 * 128, 128))
+    y, angle = x[:, :10].double(), torch.arange(19, device="cuda").double()[:, None] * f.tensor
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    at, bt = (slice(0, part, 2), slice(1, part, 2)) if interleaved else (slice(0, part // 2), slice(part // 2, part))
+    a, b = y[..., at], y[..., bt]
+    for got, ref in ((out[..., at], a * c - b * s), (out[..., bt], a * s + b * c)):
+        most = (2.0 ** -11 * ref.abs()).clamp(min=2.0 ** -25) + 2.0 ** -21 * (a.abs() + b.abs())
+        assert bool(((got.double() - ref).abs() <= most).all())
+    assert torch.equal(out[..., part:], x[:, :10, part:])
+
+
 # ---- what a backend counts and passes on -----------------------------------------------------------------------------
 
 def prompt(backend, dtype, n, heads, kv, key, value, backward=False):
@@ -305,3 +324,84 @@ def test_packed_rows_in_larger_buffers(backend):
     for change in (dict(tokens=91, tokenStarts=GpuBuffer(starts)), dict(tokens=5)):
         with pytest.raises(ValueError, match="tokens must be|key is smaller"):
             backend.LinearAttentionBackward(GpuBuffer(do), *bufs[:3], *(GpuBuffer(torch.empty_like(x)) for x in (q, k, v)), None, *sizes, **change)
+
+
+# ---- devices ---------------------------------------------------------------------------------------------------------
+
+class Elsewhere:
+    """A buffer that says it is on another device (there is one here)."""
+
+    def __init__(self, tensor):
+        self.real = tensor
+
+    @property
+    def tensor(self):
+        return self
+
+    def get_device(self):
+        return 1
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+
+def calls_by_name(backend):
+    """Each method with arguments that are right: (method, its buffers, what else it takes)."""
+    x = lambda *s: GpuBuffer(torch.zeros(s, device="cuda"))  # noqa: E731
+    ints = lambda *v: GpuBuffer(torch.tensor(v, dtype=torch.int32, device="cuda"))  # noqa: E731
+    sizes = dict(batch=1, heads=2, kvHeads=2, keyDim=64, valueDim=64)
+    rotary = dict(tokens=4, heads=2, kvHeads=2, headDim=64)
+    f = backend.RotaryFrequencies(64)
+    return [
+        (backend.RotaryEmbedding, dict(query=x(4, 2, 64), queryOut=x(4, 2, 64), key=x(4, 2, 64), keyOut=x(4, 2, 64), frequencies=f, positions=ints(0, 1, 2, 3)), rotary),
+        (backend.RotaryEmbeddingBackward, dict(gradQueryOut=x(4, 2, 64), gradQuery=x(4, 2, 64), gradKeyOut=x(4, 2, 64), gradKey=x(4, 2, 64), frequencies=f), rotary),
+        (backend.LinearAttention, dict(query=x(1, 2, 8, 64), key=x(1, 2, 8, 64), value=x(1, 2, 8, 64), output=x(1, 2, 8, 64), decay=x(2), lengths=ints(8),
+                                       initialStates=x(1, 2, 64, 64), finalStates=x(1, 2, 64, 64), stateSlots=ints(0)), dict(seqLen=8, **sizes)),
+        (backend.LinearAttention, dict(query=x(8, 2, 64), key=x(8, 2, 64), value=x(8, 2, 64), output=x(8, 2, 64), decay=x(2), tokenStarts=ints(0, 8)),
+         dict(seqLen=8, **sizes)),
+        (backend.LinearAttentionBackward, dict(gradOutput=x(1, 2, 8, 64), query=x(1, 2, 8, 64), key=x(1, 2, 8, 64), value=x(1, 2, 8, 64), gradQuery=x(1, 2, 8, 64),
+                                               gradKey=x(1, 2, 8, 64), gradValue=x(1, 2, 8, 64), decay=x(2), initialStates=x(1, 2, 64, 64),
+                                               gradFinalStates=x(1, 2, 64, 64), gradInitialStates=x(1, 2, 64, 64)), dict(seqLen=8, **sizes)),
+        (backend.LinearAttentionStep, dict(query=x(1, 2, 64), key=x(1, 2, 64), value=x(1, 2, 64), output=x(1, 2, 64), states=x(1, 2, 64, 64), decay=x(2),
+                                           stateSlots=ints(0)), sizes)]
+
+
+def test_buffers_of_another_device_are_refused(backend):
+    for method, buffers, rest in calls_by_name(backend):
+        method(**buffers, **rest)
+        for name, buf in buffers.items():
+            with pytest.raises(ValueError, match="device"):
+                method(**{**buffers, name: Elsewhere(buf.tensor)}, **rest)
+
+
+def test_another_device_may_be_the_current_one(backend, monkeypatch):
+    """Calls without a handle run on the current device: a backend makes its own the current one for them, where it is not."""
+    entered, current = [], [0]
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+            current[0] = self.device
+
+        def __exit__(self, *_):
+            current[0] = 1
+
+    calls = calls_by_name(backend)
+    for method, buffers, rest in calls:
+        method(**buffers, **rest)
+    backend.LinearAttentionPoll()
+    stream = torch.cuda.current_stream()   # (before the current device is another)
+    own = CudaBackend(stream=stream)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    current[0] = 1
+    for method, buffers, rest in calls:
+        entered.clear()
+        getattr(own, method.__name__)(**buffers, **rest)
+        assert entered and set(entered) == {0}, method.__name__
+    entered.clear()
+    own.LinearAttentionPoll()
+    assert entered == [0]
