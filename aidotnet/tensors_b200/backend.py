@@ -635,6 +635,8 @@ class CudaBackend:
         if f.dtype != torch.float64:
             raise ValueError(f"{op}: frequencies must be a buffer of 64-bit floats")
         dtype, device, spans, pointers = query.tensor.dtype, self.device, [], []
+        if dtype not in _DTYPE:
+            raise ValueError(f"{op}: {dtype} is not served")
         for name, src, dst, h, stride in (("query", query, queryOut, heads, queryStride), ("key", key, keyOut, kvHeads, keyStride)):
             if src is None:
                 spans.append((0, 0, 0, 0))
@@ -806,6 +808,8 @@ class CudaBackend:
         dtype = q.dtype
         if k.dtype != dtype or v.dtype != dtype or o.dtype != dtype:
             raise ValueError(f"{op}: query, key, value and output must share a dtype")
+        if dtype not in _DTYPE:
+            raise ValueError(f"{op}: {dtype} is not served")
         if (q.numel() < batch * heads * keyDim or k.numel() < batch * kvHeads * keyDim or v.numel() < batch * kvHeads * valueDim or
                 o.numel() < batch * heads * valueDim):
             raise ValueError(f"{op}: a buffer is smaller than the requested dimensions")

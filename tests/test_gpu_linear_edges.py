@@ -405,3 +405,39 @@ def test_another_device_may_be_the_current_one(backend, monkeypatch):
     entered.clear()
     own.LinearAttentionPoll()
     assert entered == [0]
+
+
+# ---- refusals, one thing changed in each -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int16])
+def test_types_that_are_not_served(backend, dtype):
+    for method, buffers, rest in calls_by_name(backend):
+        small = ("decay", "frequencies", "positions", "lengths", "tokenStarts", "stateSlots")
+        other = {n: b if n in small or "tates" in n else GpuBuffer(b.tensor.to(dtype)) for n, b in buffers.items()}
+        with pytest.raises(ValueError, match="not served"):
+            method(**other, **rest)
+
+
+def test_buffers_that_are_too_small_by_name(backend):
+    """Each buffer one element short, everything else right: the error names it."""
+    names = dict(queryOut="query", keyOut="key", gradQueryOut="query", gradQuery="query", gradKeyOut="key", gradKey="key")   # (a rotation names the pair)
+    for method, buffers, rest in calls_by_name(backend):
+        rotary = "Rotary" in method.__name__
+        for name, buf in buffers.items():
+            if name == "frequencies":
+                continue   # (fewer of them turn a smaller part)
+            if name == "query" and "tokenStarts" in buffers:
+                continue   # (it says how many rows there are)
+            short = GpuBuffer(buf.tensor.reshape(-1)[:-1].clone())
+            step = method.__name__ == "LinearAttentionStep" and name in ("query", "key", "value", "output")
+            match = "smaller" if step else names.get(name, name) if rotary else name
+            with pytest.raises(ValueError, match=match):
+                method(**{**buffers, name: short}, **rest)
+
+
+def test_types_of_decay_and_gradients_by_name(backend):
+    for method, buffers, rest in calls_by_name(backend):
+        for name in ("decay", "gradKey", "gradQuery", "gradValue", "initialStates", "finalStates", "gradFinalStates", "gradInitialStates", "states"):
+            if name in buffers and "Rotary" not in method.__name__:
+                with pytest.raises(ValueError, match=name):
+                    method(**{**buffers, name: GpuBuffer(buffers[name].tensor.half())}, **rest)
