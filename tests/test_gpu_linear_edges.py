@@ -10,7 +10,8 @@ import torch
 
 from aidotnet.tensors_b200 import native as N
 from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
-from tests._harness import TORCH_DT
+from tests._harness import TORCH_DT, check_guards, guarded
+from tests.test_gpu_linear import Case, check_backward, check_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -294,9 +295,8 @@ print("threads ok")
 def test_first_calls_of_many_threads():
     """Calls without a handle learn what the device is when the first of them runs: sixteen first calls at once, in a process of their own."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    for _ in range(3):
-        r = subprocess.run([sys.executable, "-c", _THREADS], capture_output=True, text=True, timeout=300, env=dict(os.environ, PYTHONPATH=root), cwd=root)
-        assert r.returncode == 0 and "threads ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
+    r = subprocess.run([sys.executable, "-c", _THREADS], capture_output=True, text=True, timeout=300, env=dict(os.environ, PYTHONPATH=root), cwd=root)
+    assert r.returncode == 0 and "threads ok" in r.stdout, f"stdout:\n{r.stdout}\nstderr:\n{r.stderr[-2000:]}"
 
 
 # ---- packed rows in buffers with room to spare -----------------------------------------------------------------------
@@ -441,3 +441,92 @@ def test_types_of_decay_and_gradients_by_name(backend):
             if name in buffers and "Rotary" not in method.__name__:
                 with pytest.raises(ValueError, match=name):
                     method(**{**buffers, name: GpuBuffer(buffers[name].tensor.half())}, **rest)
+
+
+# ---- slices of 64 columns that are not full --------------------------------------------------------------------------
+
+# (On 148 SMs slices of 64 columns are taken here, one wave of CTAs against two of slices of 32; the last slice has 8, 32 or 40 columns.  Uncut: there are CTAs
+# enough.  heads is for the forward pass; a gradient's three scans reach the same with a third of them.)
+WIDE = [(136, 136, 96, 32), (256, 96, 64, 32), (256, 40, 100, 34)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("key,value,items,_", WIDE)
+def test_slices_that_are_not_full(backend, dtype, key, value, items, _):
+    check_forward(backend, Case(dtype, [70, 33], items // 2, items // 2, key, value, "starts", first=True, seed=30))
+    check_forward(backend, Case(dtype, [40, 64], items // 2, 1, key, value, "lengths_token", first=True, seed=31))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("key,value,_,items", WIDE)
+def test_slices_that_are_not_full_backward(backend, dtype, key, value, _, items):
+    check_backward(backend, Case(dtype, [70, 33], items // 2, items // 2, key, value, "starts", first=True, seed=32), last=True)
+
+
+# ---- lengths and starts that are none --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f16", 128), ("f32", 40)])
+def test_lengths_beyond_the_ends_are_taken_to_them(backend, dtype, dim):
+    """A length below 0 is 0, one above seq_len is seq_len; starts before the first row or behind the last are those rows.  Nothing outside is written."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = [(torch.randn((3, 2, 70, dim), generator=g, device="cuda") * 0.5).to(TORCH_DT[dtype]) for _ in range(3)]
+    ints = lambda *v: GpuBuffer(torch.tensor(v, dtype=torch.int32, device="cuda"))  # noqa: E731
+    big = (1 << 31) - 1
+    for kw in ((dict(lengths=ints(-3, 1000, 33)), dict(lengths=ints(0, 70, 33))), (dict(lengths=ints(-big, big, 1)), dict(lengths=ints(0, 70, 1))),
+               (dict(tokenStarts=ints(-5, 30, 40, 5000)), dict(tokenStarts=ints(0, 30, 40, 210)))):
+        got = []
+        for k in kw:
+            seq = 70 if "lengths" in k else 210
+            made = [guarded(x[0].shape, x[0].dtype, "cuda", 3.0) for _ in range(4)]
+            bufs = [GpuBuffer(t) for t in x]
+            backend.LinearAttention(*bufs, GpuBuffer(made[0][1]), None, 3, 2, 2, seq, dim, dim, **k)
+            backend.LinearAttentionBackward(bufs[0], *bufs, *(GpuBuffer(m[1]) for m in made[1:]), None, 3, 2, 2, seq, dim, dim, **k)
+            for flat, _ in made:
+                check_guards(flat, "out or gradient")
+            got.append([m[1] for m in made])
+        assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(*got))
+
+
+# ---- graphs that share a stream and a backend ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f32", 40)])
+def test_two_graphs_replayed_at_once(dtype, dim):
+    """Two graphs recorded one after the other on one stream by one backend, with workspaces for segments and for shared heads, replayed on two streams at
+    once, beside eager calls of the same backend: all as alone."""
+    stream = torch.cuda.Stream()
+    own, plain = CudaBackend(stream=stream), CudaBackend()
+    g = torch.Generator(device="cuda").manual_seed(11)
+    sets = []
+    for n in (2500, 1700, 2100):
+        ins = [(torch.randn((1, h, n, dim), generator=g, device="cuda") * 0.3).to(TORCH_DT[dtype]) for h in (2, 1, 1, 2)]
+        sets.append((n, ins, [torch.zeros_like(t) for t in (ins[0], ins[0], ins[1], ins[2])]))
+
+    def calls(backend, which):
+        n, (q, k, v, do), (out, *grads) = sets[which]
+        backend.LinearAttention(*(GpuBuffer(t) for t in (q, k, v, out)), None, 1, 2, 1, n, dim, dim)
+        backend.LinearAttentionBackward(*(GpuBuffer(t) for t in (do, q, k, v, *grads)), None, 1, 2, 1, n, dim, dim)
+
+    right = []
+    for i in range(3):
+        calls(plain, i)
+        right.append([t.clone() for t in sets[i][2]])
+    torch.cuda.synchronize()
+    calls(own, 2)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=stream):
+            calls(own, i)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for _, _, outs in sets:
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        calls(own, 2)
+        torch.cuda.synchronize()
+        for i in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(sets[i][2], right[i])), i
+    del graphs
