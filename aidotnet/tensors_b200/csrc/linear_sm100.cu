@@ -18,8 +18,9 @@
 // fp16: a row of P, a lane's row of X^T and a chunk's column of C~ are scaled by a power of two to their own largest value, as none is bound by fp16's
 // range; the second term of C~ is held 2^11 times as large besides, and its product divided on the way into the first's.  A weighted value is then off by
 // 2^-22 of itself, or by 2^-50 of the largest in its column and chunk, where fp16's smallest numbers cut the second term.  (Without C~'s scale that was
-// 2^-36 whatever the values' size: a state of 7e-20 was zero, one of 1e-6 off by 6e-6.  It takes 22.5 -> 26.6 us of a prompt of 517 rows and 16 heads of 64,
-// 76.7 -> 82.0 us of the gradients of 3 sequences to 1531 rows and 12 heads; formed by the output's warps in place of these: 26.6 and 86.0.)
+// 2^-36 whatever the values' size: a state of 7e-20 was zero, one of 1e-6 off by 6e-6.  It takes 67 -> 77 us of B4 S2048 H32 D64 with
+// states, 83 -> 93 of D128, 233 -> 262 of that one's gradients; with scalar products and weights in registers 80, 101 and 284.  Formed by the output's
+// warps in place of these, no less: what it costs are instructions.)
 //
 // What is not finite in C would reach earlier rows of its chunk as 0 * NaN in C^T P^T: columns that come out not finite are summed again, row by row, over
 // what a row may see.
@@ -69,9 +70,10 @@ struct Cfg {
   static constexpr int kOffTab = kOffY + 4 * kYBytes;
   // tables (floats): powers [65], weights of the scores by distance in four copies, each one element on from the one before (a row's begin anywhere
   // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of the maxima of X and of C~, [2][2][128]
-  // each, weights of C~ by exponent, [2] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [2][2][4][4]
+  // each, weights of C~'s rows with as many zeros [128], weights
+  // of C~ by exponent, [2] 16-bit terms of [66], and of a whole chunk's pairs of rows as the threads take them, [2][2][4][4]
   static constexpr int kTabPower = 0, kTabScore = 68, kScorePitch = 136, kTabRow = kTabScore + 4 * kScorePitch, kTabP = kTabRow + 64, kTabX = kTabP + 128,
-                       kTabMax = kTabX + 512, kTabC = kTabMax + 512, kTabW = kTabC + 512, kTabPairs = kTabW + 68, kTabFloats = kTabPairs + 64;
+                       kTabMax = kTabX + 512, kTabC = kTabMax + 512, kTabRowsC = kTabC + 512, kTabW = kTabRowsC + 128, kTabPairs = kTabW + 68, kTabFloats = kTabPairs + 64;
   static constexpr int kOffBar = kOffTab + kTabFloats * 4;
   static constexpr int kBars = 2 * kStages + 24;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
@@ -274,6 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           if (j >= 0 && j < kChunk)
             reinterpret_cast<uint16_t*>(table + C::kTabPairs + i * 32)[((j / 32) * 16 + ((j % 8) / 2) * 4 + (j % 32) / 8) * 2 + (j & 1)] = (uint16_t)t;
           left -= __uint_as_float(t << 16);
+        }
+      } else {
+        const int j = reverse ? (int)threadIdx.x + s.lag - 1 : kChunk - s.lag - (int)threadIdx.x;   // (as above)
+        if (j >= 0 && j < kChunk) {
+          table[C::kTabRowsC + j + (reverse ? kChunk : 0)] = w;
+          table[C::kTabRowsC + j + (reverse ? 0 : kChunk)] = 0.f;
         }
       }
     }
@@ -550,13 +558,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           // (matrices of a load: rows j .. j + 7 with columns d, d + 8; rows j + 8 .. j + 15 with the same)
           const int row = half * 32 + (lane & 7) + ((lane >> 4) << 3), col = quarter * 32 + (lane & 8);
           const uint32_t from = st + (col / 64) * kBlock + row * 128;
-          float w[8], up_all = 1.f;   // fp16: weights of this thread's rows, zeros where there are none; the power of two of column (lane & 3) * 8 + lane / 4
+          // fp16: weights of row j and the next, zeros where there are none (a chunk of n rows ends with the last weight, and what is not there lies in the
+          // zeros beside them)
+          const float* row_weights = table + C::kTabRowsC + (reverse ? n : kChunk - n) + j_own;
+          auto weights_of = [&](int i) { return pack2(row_weights[8 * i], row_weights[8 * i + 1]); };
+          float up_all = 1.f;  // fp16: the power of two of column (lane & 3) * 8 + lane / 4
           if constexpr (!BF16) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int j = j_own + 8 * (i / 2) + (i & 1);
-              w[i] = there(j, n) ? power[exponent(j, n)] : 0.f;
-            }
             float most[4] = {0.f, 0.f, 0.f, 0.f};   // of columns lane / 4, 8, 16 and 24 further
 #pragma unroll
             for (int d = 0; d < 32; d += 16) {
@@ -565,9 +572,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
               for (int i = 0; i < 2; ++i) ldmatrix_x4_trans(from + i * (16 * 128) + (((uint32_t)(((col & 63) + d) >> 3) ^ (uint32_t)(row & 7)) << 4), v + 4 * i);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float2 f = unpack16<BF16>(v[i]);
+                const float2 c2 = unpack16<BF16>(v[i]), f = unpack2(mul2(pack2(c2.x, c2.y), weights_of(i / 2)));
                 float& m = most[d / 8 + (i & 1)];
-                m = fmax3(m, fabsf(f.x * w[(i / 2) * 2]), fabsf(f.y * w[(i / 2) * 2 + 1]));   // (NaN counts for nothing)
+                m = fmax3(m, fabsf(f.x), fabsf(f.y));   // (NaN counts for nothing)
               }
             }
             // of four lanes and four columns, a column to each
@@ -619,18 +626,21 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
                 v[i] = pack2<BF16>(f.x - t.x, f.y - t.y);
               }
             } else {
-              float up[2];
+              uint64_t up[2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) up[i] = __shfl_sync(0xffffffffu, up_all, (lane & ~3) + d / 8 + i);
+              for (int i = 0; i < 2; ++i) {
+                const float f = __shfl_sync(0xffffffffu, up_all, (lane & ~3) + d / 8 + i);
+                up[i] = pack2(f, f);
+              }
+              const uint64_t minus = pack2(-1.f, -1.f), kilo2 = pack2(2048.f, 2048.f);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const int at = (i / 2) * 2;
-                float2 f = unpack16<BF16>(v[i]);
-                f.x *= w[at] * up[i & 1];
-                f.y *= w[at + 1] * up[i & 1];
-                a[i] = pack2<BF16>(f.x, f.y);
-                const float2 t = unpack16<BF16>(a[i]);
-                e[i] = pack2<BF16>((f.x - t.x) * 2048.f, (f.y - t.y) * 2048.f);
+                const float2 c2 = unpack16<BF16>(v[i]);
+                const uint64_t f = mul2(pack2(c2.x, c2.y), mul2(weights_of(i / 2), up[i & 1]));   // (the weight first: it may be below what a product can hold)
+                const float2 f2 = unpack2(f);
+                a[i] = pack2<BF16>(f2.x, f2.y);
+                const float2 t = unpack16<BF16>(a[i]), r = unpack2(mul2(fma2(pack2(t.x, t.y), minus, f), kilo2));
+                e[i] = pack2<BF16>(r.x, r.y);
               }
             }
             tmem_st_16x128b_x4(to + ((uint32_t)d << 16), a);
