@@ -530,3 +530,29 @@ def test_two_graphs_replayed_at_once(dtype, dim):
         for i in range(3):
             assert all(torch.equal(a, b) for a, b in zip(sets[i][2], right[i])), i
     del graphs
+
+
+# ---- batches that are taken from the longest sequence on -------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,key,value", [("bf16", 64, 64), ("bf16", 128, 128), ("f16", 64, 128)])
+@pytest.mark.parametrize("layout", ["starts", "lengths", "lengths_token"])
+@pytest.mark.parametrize("lens", [[3, 0, 200, 64, 200], [70, 71], [0, 0, 0, 1], list(range(1, 65))])
+def test_ragged_batches_of_more_sequences_and_heads_than_sms(backend, dtype, key, value, layout, lens):
+    """(The order is by lengths here; of equal ones the first is first.)  Every sequence has its rows and its states."""
+    heads = 4 if len(lens) == 64 else 100
+    check_forward(backend, Case(dtype, lens, heads, heads // 2, key, value, layout, first=True, seed=40))
+    check_backward(backend, Case(dtype, lens, heads, heads, key, value, layout, seed=41), last=True)
+
+
+def test_ragged_batch_by_slots(backend):
+    """The same with states by slot: a slot is an earlier sequence's by the batch's order, whatever the order on the device."""
+    lens, heads = [20, 90, 150, 7], 60
+    c = Case("bf16", lens, heads, heads, 64, 64, "starts", seed=42)
+    pool = torch.randn(4, heads, 64, 64, generator=c.g, device="cuda")
+    was, out = pool.clone(), torch.empty(c.shape(heads, 64), dtype=torch.bfloat16, device="cuda")
+    slots = GpuBuffer(torch.tensor([2, 2, -1, 0], dtype=torch.int32, device="cuda"))
+    backend.LinearAttention(c.buf(c.q), c.buf(c.k), c.buf(c.v), GpuBuffer(out), c.buf(c.decay), *c.sizes(), initialStates=GpuBuffer(pool),
+                            finalStates=GpuBuffer(pool), stateSlots=slots, **c.kw())
+    for b, nan in enumerate((False, True, False, False)):
+        assert bool((torch.isnan if nan else torch.isfinite)(c.of(out, b)).all()), b
+    assert torch.equal(pool[[1, 3]], was[[1, 3]]) and not torch.equal(pool[0], was[0]) and not torch.equal(pool[2], was[2])
