@@ -11,7 +11,9 @@ import torch
 from aidotnet.tensors_b200 import native as N
 from aidotnet.tensors_b200.backend import CudaBackend, GpuBuffer
 from tests._harness import TORCH_DT, check_guards, guarded
-from tests.test_gpu_linear import Case, check_backward, check_forward
+from tests.test_gpu_linear import Case, check_backward, check_forward, e32, near, recurrence
+from tests.test_gpu_rotary import check as check_turned
+from tests.test_gpu_rotary import formula
 
 pytestmark = pytest.mark.gpu
 
@@ -556,3 +558,50 @@ def test_ragged_batch_by_slots(backend):
     for b, nan in enumerate((False, True, False, False)):
         assert bool((torch.isnan if nan else torch.isfinite)(c.of(out, b)).all()), b
     assert torch.equal(pool[[1, 3]], was[[1, 3]]) and not torch.equal(pool[0], was[0]) and not torch.equal(pool[2], was[2])
+
+
+# ---- a layer from a packed projection --------------------------------------------------------------------------------
+
+def test_a_layer_from_a_packed_projection(backend):
+    """Prompts of unequal lengths and the tokens that follow them: rotation out of the packed rows, values copied, states by slot, single tokens from there.  The
+    rotated rows are held against the formula, and what is computed of them against the recurrence of whole sequences."""
+    heads, kvHeads, headDim, lens, extra = 4, 2, 64, [70, 3, 130], 3
+    batch, tokens, longest = len(lens), sum(lens), max(lens)
+    g = torch.Generator(device="cuda").manual_seed(50)
+    project = lambda n: (torch.randn((n, heads + 2 * kvHeads, headDim), generator=g, device="cuda") * 0.5).bfloat16()  # noqa: E731
+    dense = lambda n, h: GpuBuffer(torch.empty(n, h, headDim, dtype=torch.bfloat16, device="cuda"))  # noqa: E731
+    ints = lambda x: GpuBuffer(torch.tensor(x, dtype=torch.int32, device="cuda"))  # noqa: E731
+    begin = [sum(lens[:i]) for i in range(batch + 1)]
+    decay, starts, slots = GpuBuffer(torch.tensor([-0.3, -0.1, -0.02, -0.001], device="cuda")), ints(begin), ints([4, 0, 2])
+    pool = GpuBuffer(torch.zeros(6, heads, headDim, headDim, device="cuda"))
+    f = backend.RotaryFrequencies(rotaryDim=64, scaling="parts", factor=8.0, originalLength=4096)
+    row = ((heads + 2 * kvHeads) * headDim, headDim)
+
+    def split(qkv, q, k, tokens, positions):
+        flat = qkv.view(-1)
+        backend.RotaryEmbedding(GpuBuffer(flat), q, GpuBuffer(flat[heads * headDim:]), k, f, tokens, heads, kvHeads, headDim, positions=positions,
+                                queryStride=row, keyStride=row)
+        for got, ins in ((q, qkv[:, :heads]), (k, qkv[:, heads:heads + kvHeads])):
+            check_turned(got.tensor, *formula(ins, f.tensor, positions.tensor, True, 1.0), "bf16")
+        return GpuBuffer(qkv[:, heads + kvHeads:].contiguous())
+
+    q, k, out = dense(tokens, heads), dense(tokens, kvHeads), dense(tokens, heads)
+    v = split(project(tokens), q, k, tokens, ints([t for n in lens for t in range(n)]))
+    backend.LinearAttention(q, k, v, out, decay, batch, heads, kvHeads, longest, headDim, headDim, tokenStarts=starts, initialStates=pool,
+                            finalStates=pool, stateSlots=slots)
+    all_rows = [[x.tensor[begin[b]:begin[b + 1]] for x in (q, k, v, out)] for b in range(batch)]
+    for t in range(extra):
+        q1, k1, out1 = dense(batch, heads), dense(batch, kvHeads), dense(batch, heads)
+        v1 = split(project(batch), q1, k1, batch, ints([n + t for n in lens]))
+        backend.LinearAttentionStep(q1, k1, v1, out1, pool, decay, batch, heads, kvHeads, headDim, headDim, stateSlots=slots)
+        for b in range(batch):
+            all_rows[b] = [torch.cat((x, y.tensor[b:b + 1])) for x, y in zip(all_rows[b], (q1, k1, v1, out1))]
+    for b, n in enumerate(lens):
+        qq, kk, vv = (x.double().transpose(0, 1).repeat_interleave(heads // x.shape[1], 0) for x in all_rows[b][:3])
+        lam = decay.tensor.double()
+        ref, state = recurrence(qq, kk, vv, lam, headDim ** -0.5)
+        size, size_s = recurrence(qq.abs(), kk.abs(), vv.abs(), lam, headDim ** -0.5)
+        u, e = 2.0 ** -8, e32(headDim, n + extra)
+        near(all_rows[b][3].transpose(0, 1), ref, (u + e) * size, u, f"sequence {b}", 3 * u)
+        near(pool.tensor[[4, 0, 2][b]], state, (4 * u * u + e) * size_s, 2.0 ** -24, f"state of sequence {b}", 1e-5)
+    assert bool((pool.tensor[[1, 3, 5]] == 0).all())
