@@ -1066,7 +1066,7 @@ bool is_one_of(const void* out, std::initializer_list<const void*> others) {
   return false;
 }
 
-constexpr int64_t kMostRows = 0x7fffff80;   // of a sequence: a whole number of chunks below 2^31
+constexpr int64_t kMostRows = 0x7fffffc0;   // of a sequence: a whole number of chunks below 2^31
 constexpr int64_t kMostBytes = 1ll << 60;
 
 // The sizes and pointers that a forward and a backward call share.

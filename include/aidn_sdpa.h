@@ -424,7 +424,7 @@ typedef struct {
   int64_t v_stride[3];
   int64_t o_stride[3];
   int64_t tokens;               /* rows of packed tensors                                                           */
-  int64_t seq_len;              /* the most rows of a sequence, up to 2^31-128; of packed rows a bound, up to 2^31-1  */
+  int64_t seq_len;              /* the most rows of a sequence, up to 2^31-64; of packed rows a bound, up to 2^31-1   */
   int32_t batch, heads, kv_heads;
   int32_t key_dim, value_dim;   /* multiples of 8 up to 256                                                         */
   int32_t dtype;                /* aidn_dtype of q, k, v and out                                                    */

@@ -287,7 +287,7 @@ def test_outputs_of_every_order_are_taken(lib):
 
 # ---- sizes at the ends -----------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("change", [dict(seq_len=0x7fffffff), dict(seq_len=0x7fffff81), dict(token_starts=4096, seq_len=0x7fffffff, tokens=0x7fffffff)])
+@pytest.mark.parametrize("change", [dict(seq_len=0x7fffffff), dict(seq_len=0x7fffffc1), dict(token_starts=4096, seq_len=0x7fffffff, tokens=0x7fffffff)])
 def test_sequences_that_are_too_long_for_a_count_of_rows(lib, change):
     """What counts a segment's rows has 31 bits, whole chunks of them: a longer sequence would lose its last rows."""
     small = dict(key_dim=8, value_dim=8, heads=1, kv_heads=1, batch=1)
@@ -299,7 +299,7 @@ def test_sequences_that_are_too_long_for_a_count_of_rows(lib, change):
 
 def test_workspace_of_sizes_beyond_64_bits(lib):
     """Bytes that 64 bits do not hold are refused, not wrapped around."""
-    huge = dict(batch=65535, heads=65535, kv_heads=1, seq_len=0x7fffff80, key_dim=256, value_dim=256)
+    huge = dict(batch=65535, heads=65535, kv_heads=1, seq_len=0x7fffffc0, key_dim=256, value_dim=256)
     with pytest.raises(N.AidnError) as e:
         N.linear_workspace_bytes(N.linear_bwd_block(N.linear_block(**{**LINEAR, **huge})))
     assert "2^60" in str(e.value)
