@@ -2,11 +2,16 @@
 // them) in chunks of 64, with tensor memory lanes along c's columns, so that the state never leaves the registers of the threads that own it:
 //
 //     S   = A B^T                      scores, 64 x 64 (rows of A in lanes 0-63; the lanes above hold what is not looked at)
-//     P   = S weighted by lam^(i-j), zeros where j follows i, in 16 bits to shared memory
+//     P   = S weighted by lam^(i-j), zeros where j follows i, as two 16-bit terms to shared memory
 //     T^T = C~^T B                     C~ = rows of C weighted by lam^(n-lag-j), as two 16-bit terms (off by 2^-17 of a value in bf16, 2^-22
 //                                      in fp16), or three for bf16 states that go out (2^-24, as fp32 rounds)
 //     O^T = X^T A^T  and  C^T P^T      apart, since their columns have different factors; X^T in 16 bits in tensor memory
 //     X   = lam^n X + T                in fp32 registers, then X^T rounded for the next chunk
+//
+// Rounded to 16 bits on the way to an output: X^T, as tensor memory has no columns for a second term of it at 128, and the output itself.  Against one rounding of
+// what is exact, the errors are 1.0 times as large within a sequence's first chunk, 1.06 for a decay of 0.05 a row, and go to 1.41 where a state remembers
+// everything.  (With P in one term they were 1.41 everywhere, up to 1.57 where its part and the state's cancel; its second term takes 2 to 6 % of a
+// call, B4 S2048 H32 D128 in bf16 62.6 -> 66.6 us.)
 //
 //   warps 0-1    P            warp 2   TMA producer (one thread)            warp 3   issues the products (one thread), owns tensor memory
 //   warps 4-11   C~ and the state, a lane (column of c) and half of b's columns to a thread; C~^T goes to tensor memory by transposing loads
@@ -66,8 +71,8 @@ struct Cfg {
   static constexpr int kStageBytes = (2 * kN1 + kN2) * kBlock;
   static constexpr int kStages = 147456 / kStageBytes;            // 144 KB of tiles
   static constexpr int kOffB = kN1 * kBlock, kOffC = 2 * kN1 * kBlock;
-  static constexpr int kOffP = kStages * kStageBytes;             // two buffers
-  static constexpr int kOffY = kOffP + 2 * kBlock;                // output, 64 rows of 32 columns to a warp
+  static constexpr int kOffP = kStages * kStageBytes;             // two buffers of two terms
+  static constexpr int kOffY = kOffP + 4 * kBlock;                // output, 64 rows of 32 columns to a warp
   static constexpr int kOffTab = kOffY + 4 * kYBytes;
   // tables (floats): powers [65], weights of the scores by distance in four copies, each one element on from the one before (a row's begin anywhere
   // and are read by four), of the state's rows [64]; row scales of P [2][64], lane scales of X [4][128], exchange of the maxima of X and of C~, [2][2][128]
@@ -421,9 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             tc_commit(b_x_empty);
             if (!wait1(b_p_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
             tc_fence_after();
-            const uint64_t pd = rows_desc + (uint64_t)((C::kOffP + (c & 1) * kBlock) >> 4);
+            const uint64_t pd = rows_desc + (uint64_t)((C::kOffP + (c & 1) * (2 * kBlock)) >> 4);
 #pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k) mma_ss(tmem + C::kColO + 64, ct + k * (2048 >> 4), pd + k * (32 >> 4), idesc_p, k > 0);
+            for (int k = 0; k < kChunk / 16; ++k) mma_ss(tmem + C::kColO + 64, ct + k * (2048 >> 4), pd + (kBlock >> 4) + k * (32 >> 4), idesc_p, k > 0);
+#pragma unroll
+            for (int k = 0; k < kChunk / 16; ++k) mma_ss(tmem + C::kColO + 64, ct + k * (2048 >> 4), pd + k * (32 >> 4), idesc_p, 1u);
             tc_commit(b_o_full + 8 * (c & 1));
           }
           tc_commit(b_empty + 8 * at);
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           if (!wait(b_s_full + 8 * (c & 1), (uint32_t)((c >> 1) & 1))) break;
           tc_fence_after();
           if (c >= 2 && !wait(b_o_empty + 8 * (c & 1), (uint32_t)((c >> 1) & 1) ^ 1u)) break;
-          const uint32_t row = base + C::kOffP + (c & 1) * kBlock + i * 128;
+          const uint32_t row = base + C::kOffP + (c & 1) * (2 * kBlock) + i * 128;
           uint64_t to = 0;
           if constexpr (!BF16) {
             float most = 0.f, up, back;
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
           }
 #pragma unroll 1
           for (int j0 = 0; j0 < kChunk; j0 += 16) {
-            uint32_t r[16], v[8];
+            uint32_t r[16], v[8], left[8];
             tmem_ld16(t_s + j0, r);
             tc_wait_ld();
             uint64_t x[8], probe = 0;
@@ -476,7 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
               probe = fma2(x[j / 2], 0ull, fma2(x[j / 2 + 1], 0ull, probe));
             }
             const float2 odd_ones = unpack2(probe);
-            if (__any_sync(0xffffffffu, odd_ones.x + odd_ones.y != 0.f)) {   // NaN: a score is not finite.  Behind the row it counts for nothing.
+            const bool odd = __any_sync(0xffffffffu, odd_ones.x + odd_ones.y != 0.f);   // NaN: a score is not finite
+            if (odd) {   // (behind the row it counts for nothing)
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
                 const float2 f = unpack2(x[j / 2]);
@@ -486,11 +494,23 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float2 f = unpack2(BF16 ? x[k] : mul2(x[k], to));
+              if constexpr (!BF16) x[k] = mul2(x[k], to);
+              const float2 f = unpack2(x[k]);
               v[k] = pack2<BF16>(f.x, f.y);
+              const float2 t = unpack16<BF16>(v[k]), e = unpack2(fma2(pack2(t.x, t.y), pack2(-1.f, -1.f), x[k]));
+              left[k] = pack2<BF16>(e.x, e.y);
+            }
+            if (odd) {   // (of what is not finite nothing is left)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float2 e = unpack16<BF16>(left[k]);
+                left[k] = pack2<BF16>(fabsf(e.x) < INFINITY ? e.x : 0.f, fabsf(e.y) < INFINITY ? e.y : 0.f);
+              }
             }
             st_shared_v4(row + (((uint32_t)(j0 / 8) ^ (uint32_t)(i & 7)) << 4), v[0], v[1], v[2], v[3]);
             st_shared_v4(row + (((uint32_t)(j0 / 8 + 1) ^ (uint32_t)(i & 7)) << 4), v[4], v[5], v[6], v[7]);
+            st_shared_v4(row + kBlock + (((uint32_t)(j0 / 8) ^ (uint32_t)(i & 7)) << 4), left[0], left[1], left[2], left[3]);
+            st_shared_v4(row + kBlock + (((uint32_t)(j0 / 8 + 1) ^ (uint32_t)(i & 7)) << 4), left[4], left[5], left[6], left[7]);
           }
           tc_fence_before();
           arrive(b_s_empty);
@@ -819,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
             // columns that came out not finite are summed again, a lane to each, over what a row may see (the tile of C may have been given
             // back: its column comes from memory once more)
             __syncwarp();
-            const uint32_t pt = base + C::kOffP + (c & 1) * kBlock;
+            const uint32_t pt = base + C::kOffP + (c & 1) * (2 * kBlock);
             const uint16_t* ct = static_cast<const uint16_t*>(s.c) + (p.starts ? 0 : b * s.cs[0]) + (h / s.c_group) * s.cs[1] + (q.row0 + token) * s.cs[2] + d2;
 #pragma unroll 1
             for (int r = low; r < high; ++r) {
@@ -830,8 +850,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_sm100_kernel(const __grid_co
               float part = __uint_as_float(v);
               if (!(fabsf(part) < INFINITY)) {
                 part = 0.f;
-                for (int j = reverse ? r : low; j < (reverse ? high : r + 1); ++j)
-                  part = fmaf(lds16<BF16>(pt + r * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(r & 7)) << 4) + (j & 7) * 2), unpack16<BF16>(ct[j * s.cs[2]]).x, part);
+                for (int j = reverse ? r : low; j < (reverse ? high : r + 1); ++j) {
+                  const uint32_t at = pt + r * 128 + (((uint32_t)(j >> 3) ^ (uint32_t)(r & 7)) << 4) + (j & 7) * 2;
+                  part = fmaf(lds16<BF16>(at) + lds16<BF16>(at + kBlock), unpack16<BF16>(ct[j * s.cs[2]]).x, part);
+                }
               }
               const float f = value(r, __uint_as_float(u), part);
               if (y_f32) static_cast<float*>(s.y)[y0 + (int64_t)(token + r) * pitch + d2] = f;

@@ -397,8 +397,8 @@ AIDN_API int aidn_rotary(const aidn_rotary_args* args, void* cu_stream);
  *     S_t = exp(decay) S_(t-1) + k_t v_t^T,   o_t = scale * q_t S_t.
  * decay is the head's log decay, at most 0 (-inf: nothing is kept; above 0 or NaN: the head's outputs are NaN).  Query head h reads key and
  * value head h / (heads / kv_heads); every query head has a state of its own, in fp32.  Sums and states are fp32; 16-bit inputs run on the
- * tensor cores where both sizes are 64 or 128 and all rows begin on 16 bytes (the state, and the weighted products q . k, are rounded to the 16-bit type, relative to their own
- * size, where they meet a 16-bit operand; a weighted value that is added to a state is off by 2^-22 of itself in fp16 (or 2^-50 of the largest of its column
+ * tensor cores where both sizes are 64 or 128 and all rows begin on 16 bytes (the state is rounded to the 16-bit type, relative to its own size, where
+ * queries meet it; a weighted value that is added to a state is off by 2^-22 of itself in fp16 (or 2^-50 of the largest of its column
  * within 64 rows), by 2^-17 in bf16, 2^-24 where the call leaves states), other sizes and fp32 on FFMA.  Results do not depend on launch order.
  * Nothing that follows a row reaches it.  No counterpart in the reference.
  *

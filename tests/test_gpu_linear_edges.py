@@ -605,3 +605,28 @@ def test_a_layer_from_a_packed_projection(backend):
         near(all_rows[b][3].transpose(0, 1), ref, (u + e) * size, u, f"sequence {b}", 3 * u)
         near(pool.tensor[[4, 0, 2][b]], state, (4 * u * u + e) * size_s, 2.0 ** -24, f"state of sequence {b}", 1e-5)
     assert bool((pool.tensor[[1, 3, 5]] == 0).all())
+
+
+# ---- what is rounded on the way to a 16-bit output -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("key,value", [(64, 64), (128, 128), (64, 128), (128, 64)])
+@pytest.mark.parametrize("lens", [[64, 64], [50, 50], [1, 1]])
+def test_weighted_products_are_not_rounded(backend, dtype, key, value, lens):
+    """Behind no state, an output is a sum of weighted products with values: two terms of the type hold a product to u^2 of itself, so that what is left is fp32's
+    errors (test_gpu_linear's e32) and one rounding.  Gradients as well."""
+    u, heads = torch.finfo(TORCH_DT[dtype]).eps / 2, 4
+    c = Case(dtype, lens, heads, heads, key, value, "head", seed=60)
+    out, grads = torch.empty_like(c.do), [torch.empty_like(x) for x in (c.q, c.k, c.v)]
+    backend.LinearAttention(*(GpuBuffer(x) for x in (c.q, c.k, c.v, out, c.decay)), *c.sizes())
+    backend.LinearAttentionBackward(*(GpuBuffer(x) for x in (c.do, c.q, c.k, c.v, *grads, c.decay)), *c.sizes())
+    most = 2 * u * u + e32(max(key, value), lens[0])
+    for b in range(2):
+        def run(ins, do):
+            ins = [x.requires_grad_() for x in ins]
+            ref = recurrence(*ins, c.log_decay(), key ** -0.5)[0]
+            return (ref.detach(), *torch.autograd.grad((ref * do).sum(), ins))
+        wide = [x[b].double() for x in (c.q, c.k, c.v)]
+        refs, sizes = run(wide, c.do[b].double()), run([x.abs().detach() for x in wide], c.do[b].double().abs())
+        for name, got, ref, size in zip(("out", "dq", "dk", "dv"), (out, *grads), refs, sizes):
+            near(got[b], ref, most * size, u, name)
