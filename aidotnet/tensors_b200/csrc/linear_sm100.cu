@@ -8,8 +8,8 @@
 //     O^T = X^T A^T  and  C^T P^T      apart, since their columns have different factors; X^T in 16 bits in tensor memory
 //     X   = lam^n X + T                in fp32 registers, then X^T rounded for the next chunk
 //
-// Rounded to 16 bits on the way to an output: X^T, as tensor memory has no columns for a second term of it at 128, and the output itself.  Against one rounding of
-// what is exact, the errors are 1.0 times as large within a sequence's first chunk, 1.06 for a decay of 0.05 a row, and go to 1.41 where a state remembers
+// Rounded to 16 bits on the way to an output: X^T, as tensor memory has no columns for a second term of it at 128 (through shared memory it takes 67 -> 87 us of
+// B4 S2048 H32 D128 in bf16, in tensor memory 54 -> 58 us of D64), and the output itself.  Against one rounding of what is exact, the errors are 1.0 times as large within a sequence's first chunk, 1.06 for a decay of 0.05 a row, and go to 1.41 where a state remembers
 // everything.  (With P in one term they were 1.41 everywhere, up to 1.57 where its part and the state's cancel; its second term takes 2 to 6 % of a
 // call, B4 S2048 H32 D128 in bf16 62.6 -> 66.6 us.)
 //
