@@ -33,9 +33,9 @@
 // Few sequences and heads: their rows are cut into segments.  A first launch forms what each segment adds to the state, a second one turns
 // those into the states before the segments, and the scan then runs on all segments at once, at the price of b and c read twice.
 //
-// What bounds it: a chunk takes 1.3 us (sizes of 64) to 1.7 us (128), with 16 CTAs as with 128, where the bytes of 128 CTAs would take 1.28 us at 128:
+// What bounds it: a chunk takes 1.4 us (sizes of 64) to 1.8 us (128), with 16 CTAs as with 128, where the bytes of 128 CTAs would take 1.28 us at 128:
 // the chain of waits between the roles and their code, which is longer than the instruction cache holds (8 in 100 fetches of a line miss), not a unit.
-// B4 S2048 H32 D128 in bf16: 68 us, 3.9 TB/s.  Measured on the way (us for that call): roles unrolled over their rows 174, in loops 84, packed
+// B4 S2048 H32 D128 in bf16: 65 to 72 us, 4.1 to 3.7 TB/s.  Measured on the way, with P in one term (us for that call, 63 to 71 then): roles unrolled over their rows 174, in loops 84, packed
 // arithmetic and stores by TMA 70; C~ by shared memory in place of tensor memory 80; four more warps for C~ at 96 registers a thread 76; products issued by
 // two warps, and those of T and O in turn, made no difference.
 //
@@ -945,8 +945,8 @@ cudaError_t launch_sizes(const Maps& maps, Args& args, cudaStream_t stream, int*
 }
 
 // How many segments the sequences are cut into: as many as bring work to all SMs, where that pays.  A row goes through both launches then, the first at 0.7
-// of the second's cost, and the two launches more take the time of ten chunks.  One sequence and 16 heads of 64 in fp16: 2048 rows 62 us uncut, 29 us
-// in 9 segments; 512 rows 18.9 us uncut, 19.5 us cut.  8192 rows of 16 heads of 128 in bf16: 202 and 73 us.
+// of the second's cost, and the two launches more take the time of ten chunks.  One sequence and 16 heads of 64 in fp16, by host and device: 2048 rows 76 us
+// uncut, 37 us in 9 segments; 1024 rows 41 and 30 us; 768 rows 33 us uncut, which is where the rule leaves off.  8192 rows of 16 heads of 128 in bf16: 215 and 84 us.
 int segments_of(const Params& p, int num_sms) {
   const int64_t items = (int64_t)p.batch * p.heads * p.scans, chunks = (p.seq_len + kChunk - 1) / kChunk;
   int64_t n = num_sms / items;
@@ -957,7 +957,7 @@ int segments_of(const Params& p, int num_sms) {
 
 // Whether sequences of unequal lengths are taken from the longest to the shortest: a long one at the end of a batch would run alone.  To find its sequence
 // takes a CTA 0.2 us, so it is done where the longest may take a quarter of the call: seq_len * SMs against rows * heads * scans.  (32 heads of 128 in bf16,
-// as they lie / longest first, us: 7 prompts of 1 to 8192, the shortest first, 221 / 206, with states 362 / 335, gradients 798 / 692; 32 of up to 1023
+// as they lie / longest first, us, with P in one term: 7 prompts of 1 to 8192, the shortest first, 221 / 206, with states 362 / 335, gradients 798 / 692; 32 of up to 1023
 // 155 / 147; 63 of up to 63 and one of 2000 at the end 146 / 123; 16 of 512 each 74.8 / 76.8.)
 bool by_length(const Params& p, int num_sms) {
   if ((!p.starts && !p.lengths) || p.batch < 2 || p.batch > kMaxRanked) return false;
