@@ -1131,7 +1131,14 @@ cudaError_t run_scans(const aidn_linear_args& a, const aidn::lin::Params& p, int
 // Waits for `stream` and reports a wait given up in its context that was not yet reported for this stream.  What each stream was told is kept here, and
 // only where there was something to tell; a stream's id is never another one's, its handle may be.
 int linear_report(const char* op, cudaStream_t stream, const char* prefix = "") {
-  cudaError_t e = cudaStreamSynchronize(stream);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(stream, &cap);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail_cuda(e, op);
+  }
+  if (cap != cudaStreamCaptureStatusNone) return fail(AIDN_EINVAL, "%s: the stream is being captured", op);   // (to wait for it would end the capture)
+  e = cudaStreamSynchronize(stream);
   if (e != cudaSuccess) return fail_cuda(e, op);
   const uint32_t* word = aidn::lin::sm100_gave_up();
   if (!word) return fail(AIDN_ECUDA, "%s: no count of waits in the current context", op);

@@ -460,7 +460,7 @@ AIDN_API int64_t aidn_linear_attention_backward_workspace_bytes(const aidn_linea
 AIDN_API int aidn_linear_attention_backward(const aidn_linear_bwd_args* args, void* cu_stream);
 
 /* Synchronises `cu_stream` and returns AIDN_ETIMEOUT if one of these calls gave up a bounded wait since the last report for this stream, or if there was none
- * since the context was made; AIDN_ECUDA on a CUDA error, else AIDN_OK.  The calls have no handle, and a graph may be replayed on another stream than its
+ * since the context was made; AIDN_EINVAL while the stream is being captured, AIDN_ECUDA on a CUDA error, else AIDN_OK.  The calls have no handle, and a graph may be replayed on another stream than its
  * calls were made on: waits are counted by CUDA context, so that one that ran out is told to every stream that asks, once to each.  Outputs and states of
  * the calls since a stream's report before are then not to be used, as any of them may be the one. */
 AIDN_API int aidn_linear_attention_poll(void* cu_stream);

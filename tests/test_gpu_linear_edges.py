@@ -131,6 +131,29 @@ def test_every_stream_is_told_of_a_wait_that_ran_out():
         pass
 
 
+def test_a_poll_within_a_capture_leaves_it(backend):
+    """A stream that is being captured cannot be waited for: the poll says so, and the capture goes on."""
+    stream = torch.cuda.Stream()
+    own = CudaBackend(stream=stream)
+    x = [(torch.randn(1, 2, 100, 64, device="cuda") * 0.5).bfloat16() for _ in range(4)]
+    torch.cuda.synchronize()
+    call = lambda: own.LinearAttention(*(GpuBuffer(t) for t in x), None, 1, 2, 2, 100, 64, 64)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    right = x[3].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+        with pytest.raises(N.AidnError) as e:
+            own.LinearAttentionPoll()
+    assert e.value.status == N.EINVAL
+    x[3].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x[3], right)
+    del graph
+
+
 _CHECKED = """
 import torch
 from aidotnet.tensors_b200 import native as N
