@@ -631,6 +631,8 @@ class CudaBackend:
             raise ValueError(f"{op}: tokens must be >= 0, heads and headDim positive, kvHeads >= 0")
         if (key is None) != (keyOut is None) or (key is None) != (kvHeads == 0):
             raise ValueError(f"{op}: key, keyOut and kvHeads > 0 come together")
+        if amplitude == 0:   # (the argument block's word for 1)
+            raise ValueError(f"{op}: amplitude must not be 0")
         f = frequencies.tensor
         if f.dtype != torch.float64:
             raise ValueError(f"{op}: frequencies must be a buffer of 64-bit floats")

@@ -653,3 +653,11 @@ def test_weighted_products_are_not_rounded(backend, dtype, key, value, lens):
         refs, sizes = run(wide, c.do[b].double()), run([x.abs().detach() for x in wide], c.do[b].double().abs())
         for name, got, ref, size in zip(("out", "dq", "dk", "dv"), (out, *grads), refs, sizes):
             near(got[b], ref, most * size, u, name)
+
+
+def test_amplitude_of_zero(backend):
+    """It would be a factor of 0; the argument block takes 0 for 1."""
+    for method, buffers, rest in calls_by_name(backend):
+        if "Rotary" in method.__name__:
+            with pytest.raises(ValueError, match="amplitude"):
+                method(**buffers, **rest, amplitude=0.0)
